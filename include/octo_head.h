@@ -86,6 +86,8 @@ extern "C" {
 #define OCTO_WS_STEP        128  /* octo_head_workspace_bytes / octo_head_bwd_plan: for octo_head_step_grpo */
 #define OCTO_WS_NO_GRADH    256  /* octo_head_workspace_bytes / octo_head_bwd_plan: without grad_h        */
 #define OCTO_PAIRS_NONE_AS_COUNT 1 /* octo_label_pairs: positions without a pair get the pair count  */
+#define OCTO_LIST_MAX        256 /* octo_topk, octo_distill_*: the most entries of a row's list           */
+#define OCTO_LIST_RAW          1 /* octo_distill_*: q = exp(t) as given, not the softmax over the row's list */
 
 const char *octo_version(void);
 const char *octo_last_error(void);
@@ -206,6 +208,41 @@ int octo_columns_fwd(const void *logits, int64_t ld, int dtype, const int64_t *l
 int octo_columns_bwd(const void *logits, int64_t ld, int dtype, const int64_t *labels,
                      int64_t n, int V, float inv_T, const float *lse, const float *g,
                      void *dlogits, int64_t ld_d, void *stream);
+
+/* A teacher's list (no counterpart in the reference): of each row of logits [n, ld] (BF16, F16 or F32) the k largest
+ * values, by value descending, equal values by column ascending (NaN counts as the largest): ids[r, :k] their columns,
+ * logp[r, :k] = log_softmax(logits[r] * inv_T) there (fp32). 1 <= k <= min(V, OCTO_LIST_MAX); rows may start at any
+ * element. */
+int octo_topk(const void *logits, int64_t ld, int dtype, int64_t n, int V, float inv_T, int k, int64_t *ids,
+              float *logp, void *stream);
+
+/* Distillation from teachers' lists (no counterpart in the reference). Row r's list holds K slots (ids[r, k],
+ * teacher[r, k]): a token and the teacher's logit or log-probability of it (fp32). A slot with an id outside [0, V) or a
+ * teacher value of -inf is empty; the same token may stand in several slots.
+ *   q = softmax(teacher[r, :]) over the slots that are not empty (OCTO_LIST_RAW: exp of it),  p = softmax(z_r * inv_T)
+ *   kl[r] = sum_k q_k (log q_k - log p_ids[k]),  0 for a row whose slots are all empty.
+ * Over materialised logits [n, ld]: the forward also leaves state [n, 4] (16 bytes a row) and q [n, K] for the backward,
+ *   dlogits[r, v] = g[r] inv_T (Q p_v - sum of q_k over the slots of v),  Q = sum of q,
+ * in the logits' dtype at stride ld_d; a row with Q = 0 gets zeros whatever its logits are. 1 <= K <= OCTO_LIST_MAX. */
+int octo_distill_columns_fwd(const void *logits, int64_t ld, int dtype, const int64_t *ids, const float *teacher,
+                             int64_t n, int V, int K, float inv_T, int flags, float *kl, float *state, float *q,
+                             void *stream);
+int octo_distill_columns_bwd(const void *logits, int64_t ld, int dtype, const int64_t *ids, const float *q, int64_t n,
+                             int V, int K, float inv_T, const float *state, const float *g, void *dlogits,
+                             int64_t ld_d, void *stream);
+
+/* Embedding lookup (no counterpart in the reference): out[t, :d] = scale * w[ids[t], :d] in w's dtype (BF16, F16, F32),
+ * zeros for an id outside [0, V). */
+int octo_embed_fwd(const void *w, int64_t ldw, int dtype, int64_t V, int d, const int64_t *ids, int64_t n, float scale,
+                   void *out, int64_t ldo, void *stream);
+/* Its gradient by sorted tokens: grad_w[v, :d] = scale * sum of grad[t, :d] over the tokens with ids[t] = v, summed in
+ * fp32 in an order that the ids alone decide and rounded once to w_dtype; ids outside [0, V) and padding_idx (-1: none)
+ * are left out. accumulate: added to what grad_w holds, and the rows of other entries are neither read nor written; else
+ * every row is written. ws: octo_embed_bwd_workspace_bytes, 16-byte aligned. */
+int octo_embed_bwd_workspace_bytes(int64_t n, int64_t V, int d, size_t *bytes);
+int octo_embed_bwd(const void *grad, int64_t ldg, int g_dtype, const int64_t *ids, int64_t n, int64_t V, int d,
+                   int64_t padding_idx, float scale, void *grad_w, int64_t ldw, int w_dtype, int accumulate, void *ws,
+                   size_t ws_bytes, void *stream);
 
 /* Pair expansion (prefix_tree.py:419-421): out[t, :C] = pairs[flat_pair[t], :C] when
  * 0 <= flat_pair[t] < P, else 0. */

@@ -22,6 +22,7 @@ ROWS_VIA_IDX, OUT_SCATTER, GRADW_ACCUMULATE, WS_BACKWARD, WS_NO_GRADW, WS_GATHER
 WS_STEP = 128
 WS_NO_GRADH = 256
 PAIRS_NONE_AS_COUNT = 1
+LIST_MAX, LIST_RAW = 256, 1
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -71,6 +72,12 @@ SIGNATURES = {
                              _f32, _i32, _p, _p, _p, _i64, _i64, _p, _i64, _i32, _p, _i32, _p, _sz, _p],
     "octo_columns_fwd": [_p, _i64, _i32, _p, _i64, _i32, _f32, _p, _p, _p],
     "octo_columns_bwd": [_p, _i64, _i32, _p, _i64, _i32, _f32, _p, _p, _p, _i64, _p],
+    "octo_topk": [_p, _i64, _i32, _i64, _i32, _f32, _i32, _p, _p, _p],
+    "octo_distill_columns_fwd": [_p, _i64, _i32, _p, _p, _i64, _i32, _i32, _f32, _i32, _p, _p, _p, _p],
+    "octo_distill_columns_bwd": [_p, _i64, _i32, _p, _p, _i64, _i32, _i32, _f32, _p, _p, _p, _i64, _p],
+    "octo_embed_fwd": [_p, _i64, _i32, _i64, _i32, _p, _i64, _f32, _p, _i64, _p],
+    "octo_embed_bwd_workspace_bytes": [_i64, _i64, _i32, ctypes.POINTER(_sz)],
+    "octo_embed_bwd": [_p, _i64, _i32, _p, _i64, _i64, _i32, _i64, _f32, _p, _i64, _i32, _i32, _p, _sz, _p],
     "octo_pairs_expand": [_p, _i64, _i32, _p, _i64, _p, _p],
     "octo_pairs_grad": [_p, _i64, _i32, _p, _i64, _p, _p],
     "octo_rows_scatter": [_p, _i64, _i32, _p, _p, _i64, _i32, _p, _i64, _i32, _i32, _p],

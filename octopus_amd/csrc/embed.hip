@@ -1,0 +1,491 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens (octo_embed_fwd, octo_embed_bwd).
+//
+//   out[t] = scale W[ids[t]]              (zeros for an id outside [0, V))
+//   grad_W[v] = scale sum of grad[t] over the tokens with ids[t] = v, t ascending; no token of padding_idx
+//
+// Both are bound by memory: the lookup reads and writes a row per token; the gradient reads a row per token and writes
+// one per vocabulary entry (or adds to the entries that occur). A gradient row's sum is taken in fp32 in an order that
+// the tokens alone decide, and rounded once, so equal inputs give equal bits.
+//
+// The gradient takes three launches:
+//   sort   a workgroup per range of kBins vocabulary entries: it reads all ids twice, counts those below its range (the
+//          place of its first token) and those of each entry by wave (a wave takes a contiguous part of the tokens), and
+//          places its tokens, so that sorted tokens of one entry keep their order. No workgroup waits for another.
+//   sum    a wave per kRun sorted tokens x 512 columns: the sum of every entry whose tokens all lie in the piece goes to
+//          grad_W, that of an entry that crosses a piece's border to the piece's two fp32 partial rows (its first and
+//          its last entry). Frequent tokens are so shared out evenly. Behind them, waves that write the zero rows.
+//   join   a workgroup per piece in which a crossing entry starts: its partial rows summed in order.
+#include "octo_common.h"
+#include "row_values.h"
+
+namespace octo {
+
+constexpr int kBins = 512;    // vocabulary entries per sort workgroup
+constexpr int kRun = 32;      // sorted tokens per piece
+constexpr int kCols = 512;    // columns per wave of the sum
+constexpr int kSumLoads = 8;  // rows in flight per wave
+
+// ---- lookup ------------------------------------------------------------------------------------------------------------
+// A wave per token and 2,048 bytes x 2 of its row.
+constexpr int kRowLoadsF = 4;
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void embed_fwd_kernel(const void *w, int64_t ldw, int64_t V, int d,
+                                                        const int64_t *ids, int64_t n, float scale, void *out,
+                                                        int64_t ldo) {
+  constexpr int PER = 16 / Elem<DT>::bytes;
+  typedef typename Elem<DT>::T T;
+  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (t >= n) return;
+  const int64_t id = ids[t];
+  const bool ok = id >= 0 && id < V;
+  const T *src = (const T *)w + (ok ? id : 0) * ldw;
+  T *dst = (T *)out + t * ldo;
+  if constexpr (VEC) {
+    const int chunks = d / PER;
+    const int c0 = blockIdx.y * (64 * kRowLoadsF) + lane;
+    i32x4 v[kRowLoadsF];
+#pragma unroll
+    for (int u = 0; u < kRowLoadsF; ++u) {
+      v[u] = i32x4{0, 0, 0, 0};
+      if (ok && c0 + 64 * u < chunks) v[u] = ((const i32x4 *)src)[c0 + 64 * u];
+    }
+#pragma unroll
+    for (int u = 0; u < kRowLoadsF; ++u) {
+      if (c0 + 64 * u >= chunks) break;
+      float x[PER];
+      unpack_chunk<DT>(v[u], x);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) x[e] = ok ? x[e] * scale : 0.f;
+      ((i32x4 *)dst)[c0 + 64 * u] = pack_chunk<DT>(x);
+    }
+  } else {
+    const int j0 = blockIdx.y * (64 * kRowLoadsF * PER), j1 = min(d, j0 + 64 * kRowLoadsF * PER);
+    for (int j = j0 + lane; j < j1; j += 64) dst[j] = ok ? (T)((float)src[j] * scale) : (T)0.f;
+  }
+}
+
+// ---- sort --------------------------------------------------------------------------------------------------------------
+struct SortOut {
+  int32_t *order;  // [n] token positions by (entry, position)
+  int32_t *entry;  // [n] the entries of them
+  int32_t *start;  // [V + 1] first place of each entry's tokens; start[V]: how many tokens there are
+};
+
+constexpr int kSortWaves = 16, kSortLoads = 4;
+__global__ __launch_bounds__(1024) void embed_sort_kernel(const int64_t *ids, int n, int V, int64_t padding, SortOut o) {
+  __shared__ int hist[kSortWaves][kBins];
+  __shared__ int part[2][kSortWaves];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lo = blockIdx.x * kBins, hi = min(V, lo + kBins);
+  for (int i = threadIdx.x; i < kSortWaves * kBins; i += 1024) ((int *)hist)[i] = 0;
+  __syncthreads();
+  const int seg = (int)round_up(cdiv(n, kSortWaves), 64);
+  const int t0 = min(n, w * seg), t1 = min(n, t0 + seg);
+  int below = 0;
+  for (int s = t0; s < t1; s += 64 * kSortLoads) {
+    int64_t v[kSortLoads];
+#pragma unroll
+    for (int u = 0; u < kSortLoads; ++u) {
+      const int t = s + 64 * u + lane;
+      v[u] = t < t1 ? ids[t] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kSortLoads; ++u) {
+      if (v[u] < 0 || v[u] >= hi || v[u] == padding) continue;
+      if (v[u] < lo) ++below;
+      else atomicAdd(&hist[w][(int)v[u] - lo], 1);
+    }
+  }
+  below = wave_sum(below);
+  if (lane == 0) part[0][w] = below;
+  __syncthreads();
+  int first = 0;
+#pragma unroll
+  for (int k = 0; k < kSortWaves; ++k) first += part[0][k];
+  // places by entry, then by wave
+  int total = 0;
+  if (threadIdx.x < kBins)
+#pragma unroll
+    for (int k = 0; k < kSortWaves; ++k) total += hist[k][threadIdx.x];
+  int x = total;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int y = __shfl_up(x, s, 64);
+    if (lane >= s) x += y;
+  }
+  if (lane == 63) part[1][w] = x;
+  __syncthreads();
+  for (int k = 0; k < w; ++k) x += part[1][k];
+  if (threadIdx.x < kBins) {
+    int at = first + x - total;
+    if (lo + (int)threadIdx.x < hi) o.start[lo + threadIdx.x] = at;
+#pragma unroll
+    for (int k = 0; k < kSortWaves; ++k) {
+      const int h = hist[k][threadIdx.x];
+      hist[k][threadIdx.x] = at;
+      at += h;
+    }
+    if (hi == V && threadIdx.x == kBins - 1) o.start[V] = at;
+  }
+  __syncthreads();
+  // each wave places its tokens in their order; lanes of one entry by lane
+  for (int s = t0; s < t1; s += 64 * kSortLoads) {
+    int64_t v[kSortLoads];
+#pragma unroll
+    for (int u = 0; u < kSortLoads; ++u) {
+      const int t = s + 64 * u + lane;
+      v[u] = t < t1 ? ids[t] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kSortLoads; ++u) {
+      const bool in = v[u] >= lo && v[u] < hi && v[u] != padding;
+      uint64_t same = __ballot(in);
+      if (same == 0) continue;
+      const int bin = in ? (int)v[u] - lo : 0;
+#pragma unroll
+      for (int b = 1; b < kBins; b <<= 1) {
+        const uint64_t on = __ballot(bin & b);
+        same &= bin & b ? on : ~on;
+      }
+      const int rank = __popcll(same & ((1ull << lane) - 1ull));
+      int base = 0;
+      if (in) base = hist[w][bin];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (in) {
+        o.order[base + rank] = s + 64 * u + lane;
+        o.entry[base + rank] = lo + bin;
+        if (rank == 0) hist[w][bin] = base + __popcll(same);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+  }
+}
+
+// ---- sum ---------------------------------------------------------------------------------------------------------------
+struct SumArgs {
+  const void *grad;
+  int64_t ldg;
+  int d, V;
+  int n;  // tokens; as many of them as start[V] says are sorted
+  SortOut s;
+  float scale;
+  void *gw;
+  int64_t ldw;
+  int accumulate;
+  float *part;  // [pieces][2][d]
+  int pieces, colblocks, zero_blocks;
+};
+
+// 8 columns of a row per lane: c0 + 8 lane .. + 8 (VEC), or c0 + lane + 64 e.
+template <int DT, bool VEC> struct Cols {
+  float x[8];
+  __device__ __forceinline__ void load(const void *base, int64_t off, int c0, int lane, int d) {
+    typedef typename Elem<DT>::T T;
+    const T *p = (const T *)base + off;
+    if constexpr (VEC) {
+      const int c = c0 + 8 * lane;
+      constexpr int PER = 16 / Elem<DT>::bytes;
+#pragma unroll
+      for (int h = 0; h < 8 / PER; ++h) {
+        float y[PER];
+        unpack_chunk<DT>(c < d ? *(const i32x4 *)(p + c + h * PER) : i32x4{0, 0, 0, 0}, y);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[h * PER + e] = y[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = c0 + lane + 64 * e;
+        x[e] = c < d ? (float)p[c] : 0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(void *base, int64_t off, int c0, int lane, int d) const {
+    typedef typename Elem<DT>::T T;
+    T *p = (T *)base + off;
+    if constexpr (VEC) {
+      const int c = c0 + 8 * lane;
+      constexpr int PER = 16 / Elem<DT>::bytes;
+      if (c < d)
+#pragma unroll
+        for (int h = 0; h < 8 / PER; ++h) {
+          float y[PER];
+#pragma unroll
+          for (int e = 0; e < PER; ++e) y[e] = x[h * PER + e];
+          *(i32x4 *)(p + c + h * PER) = pack_chunk<DT>(y);
+        }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = c0 + lane + 64 * e;
+        if (c < d) p[c] = (T)x[e];
+      }
+    }
+  }
+};
+
+// grad_W's row v: scale x the sum, rounded once; added to what it holds where asked for.
+template <int WT, bool VEC>
+__device__ __forceinline__ void store_entry(const SumArgs &a, int v, const float (&sum)[8], int c0, int lane) {
+  Cols<WT, VEC> o;
+  const int64_t off = (int64_t)v * a.ldw;
+  if (a.accumulate) {
+    o.load(a.gw, off, c0, lane, a.d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o.x[e] = __builtin_fmaf(a.scale, sum[e], o.x[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o.x[e] = a.scale * sum[e];
+  }
+  o.store(a.gw, off, c0, lane, a.d);
+}
+
+template <int GT, int WT, bool VEC>
+__global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int wave = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int items = a.pieces * a.colblocks;
+  if (wave >= items) {  // the zero rows
+    if (a.accumulate) return;
+    const int z = wave - (int)round_up(items, 4), nz = a.zero_blocks * 4;
+    if (z < 0) return;
+    const float none[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int v0 = z * 64; v0 < a.V; v0 += nz * 64) {  // 64 entries at a time
+      const int v = v0 + lane;
+      uint64_t empty = __ballot(v < a.V && a.s.start[min(v, a.V)] == a.s.start[min(v + 1, a.V)]);
+      while (empty) {
+        const int k = __ffsll((unsigned long long)empty) - 1;
+        empty &= empty - 1;
+        for (int c0 = 0; c0 < a.d; c0 += kCols) {
+          Cols<WT, VEC> o;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o.x[e] = none[e];
+          o.store(a.gw, (int64_t)(v0 + k) * a.ldw, c0, lane, a.d);
+        }
+      }
+    }
+    return;
+  }
+  const int piece = wave / a.colblocks, c0 = (wave - piece * a.colblocks) * kCols;
+  const int m = a.s.start[a.V], i0 = piece * kRun, i1 = min(m, i0 + kRun);
+  if (i0 >= m) return;
+  // this piece's tokens and entries, one per lane; entry -1 beyond
+  int tok = 0, ent = -1;
+  if (lane < kRun && i0 + lane < i1) {
+    tok = a.s.order[i0 + lane];
+    ent = a.s.entry[i0 + lane];
+  }
+  const bool head = i0 > 0 && a.s.entry[i0 - 1] == __shfl(ent, 0, 64);   // the first entry began before the piece
+  const bool tail = i1 < m && a.s.entry[i1] == __shfl(ent, i1 - i0 - 1, 64);  // the last one goes on behind it
+  const int first = __shfl(ent, 0, 64), last = __shfl(ent, i1 - i0 - 1, 64);
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  int cur = first;
+  auto flush = [&](int v) {
+    const bool crosses = (head && v == first) || (tail && v == last);
+    if (!crosses) {
+      store_entry<WT, VEC>(a, v, sum, c0, lane);
+    } else {
+      // the piece's partial rows: 0 of its first entry where that began before it, else 1 of its last
+      float *p = a.part + ((int64_t)piece * 2 + (head && v == first ? 0 : 1)) * a.d;
+      Cols<OCTO_F32, VEC> o;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o.x[e] = sum[e];
+      o.store(p, 0, c0, lane, a.d);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+  };
+  for (int i = i0; i < i1; i += kSumLoads) {
+    Cols<GT, VEC> g[kSumLoads];
+#pragma unroll
+    for (int u = 0; u < kSumLoads; ++u) {
+      const int k = min(i + u, i1 - 1) - i0;  // past the end: the last token again, left out below
+      g[u].load(a.grad, (int64_t)__shfl(tok, k, 64) * a.ldg, c0, lane, a.d);
+    }
+#pragma unroll
+    for (int u = 0; u < kSumLoads; ++u) {
+      if (i + u >= i1) break;
+      const int v = __shfl(ent, i + u - i0, 64);
+      if (v != cur) {
+        flush(cur);
+        cur = v;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += g[u].x[e];
+    }
+  }
+  flush(cur);
+}
+
+// ---- join --------------------------------------------------------------------------------------------------------------
+// The entry that starts in piece p and goes on behind it: its partial rows are row 1 of p and row 0 of the pieces up to
+// the one that holds its last token. 4 waves take them in turn, each in order, and are added in order.
+constexpr int kJoinWaves = 4, kJoinLoads = 4;
+template <int WT, bool VEC>
+__global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(SumArgs a) {
+  __shared__ float sums[kJoinWaves][64][8];
+  const int p = blockIdx.x, c0 = blockIdx.y * kCols;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int m = a.s.start[a.V], i1 = (p + 1) * kRun;
+  if (i1 >= m) return;
+  const int v = a.s.entry[i1 - 1];
+  if (a.s.entry[i1] != v) return;
+  const int s0 = a.s.start[v], s1 = a.s.start[v + 1];
+  if (s0 < p * kRun) return;  // it began before: another workgroup's
+  const int parts = (s1 - 1) / kRun - p + 1;
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int k = w; k < parts; k += kJoinWaves * kJoinLoads) {
+    Cols<OCTO_F32, VEC> x[kJoinLoads];
+#pragma unroll
+    for (int u = 0; u < kJoinLoads; ++u) {
+      const int q = min(k + kJoinWaves * u, parts - 1);
+      x[u].load(a.part, ((int64_t)(p + q) * 2 + (q == 0 ? 1 : 0)) * a.d, c0, lane, a.d);
+    }
+#pragma unroll
+    for (int u = 0; u < kJoinLoads; ++u)
+      if (k + kJoinWaves * u < parts)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += x[u].x[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sums[w][lane][e] = sum[e];
+  __syncthreads();
+  if (w) return;
+#pragma unroll
+  for (int k = 1; k < kJoinWaves; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] += sums[k][lane][e];
+  store_entry<WT, VEC>(a, v, sum, c0, lane);
+}
+
+// ---- workspace ---------------------------------------------------------------------------------------------------------
+static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+static size_t embed_ws(int64_t n, int64_t V, int64_t d, char *ws, SumArgs *a) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    char *p = ws ? ws + off : nullptr;
+    off += align256(bytes);
+    return p;
+  };
+  char *order = take((size_t)n * 4), *entry = take((size_t)n * 4), *start = take((size_t)(V + 1) * 4);
+  const int64_t pieces = cdiv(n, kRun);
+  char *part = take((size_t)pieces * 2 * d * 4);
+  if (a) {
+    a->s.order = (int32_t *)order;
+    a->s.entry = (int32_t *)entry;
+    a->s.start = (int32_t *)start;
+    a->part = (float *)part;
+    a->pieces = (int)pieces;
+  }
+  return off;
+}
+
+template <int GT, int WT, bool VEC> static int go_bwd(const SumArgs &a, hipStream_t st) {
+  const int64_t items = cdiv((int64_t)a.pieces * a.colblocks, 4);
+  hipLaunchKernelGGL((embed_sum_kernel<GT, WT, VEC>), dim3((unsigned)(items + a.zero_blocks)), dim3(256), 0, st, a);
+  OCTO_CHECK_LAUNCH("embed_sum");
+  if (a.pieces > 1) {
+    hipLaunchKernelGGL((embed_join_kernel<WT, VEC>), dim3((unsigned)(a.pieces - 1), (unsigned)a.colblocks),
+                       dim3(64 * kJoinWaves), 0, st, a);
+    OCTO_CHECK_LAUNCH("embed_join");
+  }
+  return OCTO_OK;
+}
+template <int GT, int WT> static int pick_bwd(const SumArgs &a, bool vec, hipStream_t st) {
+  return vec ? go_bwd<GT, WT, true>(a, st) : go_bwd<GT, WT, false>(a, st);
+}
+template <int GT> static int pick_bwd(const SumArgs &a, int wt, bool vec, hipStream_t st) {
+  if (wt == OCTO_BF16) return pick_bwd<GT, OCTO_BF16>(a, vec, st);
+  if (wt == OCTO_F16) return pick_bwd<GT, OCTO_F16>(a, vec, st);
+  return pick_bwd<GT, OCTO_F32>(a, vec, st);
+}
+
+template <int DT>
+static void go_fwd(const void *w, int64_t ldw, int64_t V, int d, const int64_t *ids, int64_t n, float scale, void *out,
+                   int64_t ldo, hipStream_t st) {
+  constexpr int B = Elem<DT>::bytes, PER = 16 / B;
+  const bool vec = d % PER == 0 && ldw % PER == 0 && ldo % PER == 0 && (uintptr_t)w % 16 == 0 && (uintptr_t)out % 16 == 0;
+  const dim3 grid((unsigned)cdiv(n, 4), (unsigned)cdiv(d, 64 * kRowLoadsF * PER));
+  if (vec)
+    hipLaunchKernelGGL((embed_fwd_kernel<DT, true>), grid, dim3(256), 0, st, w, ldw, V, d, ids, n, scale, out, ldo);
+  else
+    hipLaunchKernelGGL((embed_fwd_kernel<DT, false>), grid, dim3(256), 0, st, w, ldw, V, d, ids, n, scale, out, ldo);
+}
+
+}  // namespace octo
+
+using namespace octo;
+
+extern "C" {
+
+int octo_embed_fwd(const void *w, int64_t ldw, int dtype, int64_t V, int d, const int64_t *ids, int64_t n, float scale,
+                   void *out, int64_t ldo, void *stream) {
+  OCTO_CHECK_ARG(V > 0 && V < 0x7fffffff && d > 0 && ldw >= d && ldo >= d && n >= 0 && n < 0x7fffffff,
+                 "embed_fwd: bad shape V=%lld d=%d n=%lld", (long long)V, d, (long long)n);
+  if (!is_float(dtype)) return octo_fail(OCTO_EUNSUPPORTED, "embed_fwd: dtype %d", dtype);
+  if (n == 0) return OCTO_OK;
+  OCTO_CHECK_ARG(w && ids && out, "embed_fwd: null pointer");
+  OCTO_CHECK_ARG((uintptr_t)w % float_bytes(dtype) == 0 && (uintptr_t)out % float_bytes(dtype) == 0,
+                 "embed_fwd: misaligned rows");
+  OCTO_CHECK_ARG(d <= 65535 * 1024, "embed_fwd: d=%d", d);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == OCTO_BF16) go_fwd<OCTO_BF16>(w, ldw, V, d, ids, n, scale, out, ldo, st);
+  else if (dtype == OCTO_F16) go_fwd<OCTO_F16>(w, ldw, V, d, ids, n, scale, out, ldo, st);
+  else go_fwd<OCTO_F32>(w, ldw, V, d, ids, n, scale, out, ldo, st);
+  OCTO_CHECK_LAUNCH("embed_fwd");
+  return OCTO_OK;
+}
+
+int octo_embed_bwd_workspace_bytes(int64_t n, int64_t V, int d, size_t *bytes) {
+  OCTO_CHECK_ARG(bytes != nullptr, "embed_bwd_workspace_bytes: null pointer");
+  OCTO_CHECK_ARG(V > 0 && V < 0x7fffffff - kBins && d > 0 && d <= 65535 * kCols && n >= 0 && n <= (int64_t)1 << 30,
+                 "embed_bwd: bad shape V=%lld d=%d n=%lld", (long long)V, d, (long long)n);
+  *bytes = embed_ws(n, V, d, nullptr, nullptr);
+  return OCTO_OK;
+}
+
+int octo_embed_bwd(const void *grad, int64_t ldg, int g_dtype, const int64_t *ids, int64_t n, int64_t V, int d,
+                   int64_t padding_idx, float scale, void *grad_w, int64_t ldw, int w_dtype, int accumulate, void *ws,
+                   size_t ws_bytes, void *stream) {
+  size_t need = 0;
+  const int rc = octo_embed_bwd_workspace_bytes(n, V, d, &need);
+  if (rc) return rc;
+  OCTO_CHECK_ARG(ldg >= d && ldw >= d, "embed_bwd: row strides below d");
+  if (!is_float(g_dtype) || !is_float(w_dtype))
+    return octo_fail(OCTO_EUNSUPPORTED, "embed_bwd: dtypes %d, %d", g_dtype, w_dtype);
+  OCTO_CHECK_ARG(grad_w && (n == 0 || (grad && ids)), "embed_bwd: null pointer");
+  OCTO_CHECK_ARG((uintptr_t)grad % float_bytes(g_dtype) == 0 && (uintptr_t)grad_w % float_bytes(w_dtype) == 0,
+                 "embed_bwd: misaligned rows");
+  SumArgs a{};
+  if (!ws || ws_bytes < need)
+    return octo_fail(OCTO_EWORKSPACE, "embed_bwd: workspace %zu < %zu bytes", ws ? ws_bytes : (size_t)0, need);
+  OCTO_CHECK_ARG((uintptr_t)ws % 16 == 0, "embed_bwd: misaligned workspace");
+  if (n == 0 && accumulate) return OCTO_OK;
+  embed_ws(n, V, d, (char *)ws, &a);
+  a.grad = grad;
+  a.ldg = ldg;
+  a.d = d;
+  a.V = (int)V;
+  a.n = (int)n;
+  a.scale = scale;
+  a.gw = grad_w;
+  a.ldw = ldw;
+  a.accumulate = accumulate != 0;
+  a.colblocks = (int)cdiv(d, kCols);
+  a.zero_blocks = accumulate ? 0 : (int)(cdiv(V, 256) < 2048 ? cdiv(V, 256) : 2048);
+  OCTO_CHECK_ARG((int64_t)a.pieces * a.colblocks < (int64_t)1 << 30, "embed_bwd: %lld tokens of width %d", (long long)n, d);
+  hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)cdiv(V, kBins)), dim3(1024), 0, st, ids, (int)n, (int)V,
+                     padding_idx, a.s);
+  OCTO_CHECK_LAUNCH("embed_sort");
+  const auto whole = [&](const void *p, int64_t ld, int dt) {
+    return (uintptr_t)p % 16 == 0 && ld * float_bytes(dt) % 16 == 0;
+  };
+  const bool vec = d % 8 == 0 && whole(grad, ldg, g_dtype) && whole(grad_w, ldw, w_dtype);
+  if (g_dtype == OCTO_BF16) return pick_bwd<OCTO_BF16>(a, w_dtype, vec, st);
+  if (g_dtype == OCTO_F16) return pick_bwd<OCTO_F16>(a, w_dtype, vec, st);
+  return pick_bwd<OCTO_F32>(a, w_dtype, vec, st);
+}
+
+}  // extern "C"

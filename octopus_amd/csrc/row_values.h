@@ -156,4 +156,43 @@ struct ColStat {
   }
 };
 
+// One thread's part of a row's logsumexp at c = log2(e) / T: m the running maximum of the logits themselves (-inf before
+// any above it), S the sum of exp2((x - m) c). Against m and not m c: logits masked with the type's lowest value times c
+// overflow, and a row of nothing else still has its logsumexp. -inf adds nothing; a NaN or +inf makes S NaN for good.
+struct RowSum {
+  float m = -INFINITY, S = 0.f;
+  // S against a maximum raised by -d / c; far below the new one it counts for nothing
+  __device__ __forceinline__ void shift(float d) { S = d < -256.f ? (S == S ? 0.f : S) : S * fexp2(d); }
+  __device__ __forceinline__ void raise(float mx, float c) {
+    if (mx > m) {
+      shift((m - mx) * c);
+      m = mx;
+    }
+  }
+  __device__ __forceinline__ void add(float x, float c) {  // after raise() to at least x
+    S += fexp2((x - (m == -INFINITY ? 0.f : m)) * c);
+  }
+};
+
+// A workgroup's logsumexp from its threads' parts: (m, S) in every thread. red: 2 x NW floats of shared memory.
+template <int NW>
+__device__ __forceinline__ void block_row_sum(RowSum st, float c, float (*red)[NW], float &m, float &S) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  m = wave_max(st.m);
+  if (lane == 0) red[0][w] = m;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < NW; ++k) m = fmaxf(m, red[0][k]);
+  if (st.m != -INFINITY) st.shift((st.m - m) * c);  // else S is 0, or NaN
+  const float s = wave_sum(st.S);
+  if (lane == 0) red[1][w] = s;
+  __syncthreads();
+  S = 0.f;
+#pragma unroll
+  for (int k = 0; k < NW; ++k) S += red[1][k];
+}
+
+inline int float_bytes(int dtype) { return dtype == OCTO_F32 ? 4 : 2; }
+inline bool is_float(int dtype) { return dtype == OCTO_BF16 || dtype == OCTO_F16 || dtype == OCTO_F32; }
+
 }  // namespace octo
