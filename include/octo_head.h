@@ -231,6 +231,29 @@ int octo_distill_columns_bwd(const void *logits, int64_t ld, int dtype, const in
                              int V, int K, float inv_T, const float *state, const float *g, void *dlogits,
                              int64_t ld_d, void *stream);
 
+/* The same from hidden rows and the vocabulary weight, without the logits: octo_head_step_grpo's forward and backward in
+ * one call (16-bit or fp8 weights; fp32 operands: OCTO_EUNSUPPORTED), for loss = sum over the compact rows of weight x
+ * kl. Lists and weights are per hidden row (compact row r's at idx[r], or r): ids, teacher [h_rows, K], weight [h_rows]
+ * (NULL: 1). kl [h_rows] is written at the compact rows' hidden rows, loss [1]. dots, q [n_max, K] and g [n_max] are
+ * scratch, as lse [n_max, 2]. grad_h (compact rows) and grad_w as octo_head_step_grpo's; workspace likewise
+ * (OCTO_WS_STEP). kept != NULL: no grad_w, whose operands stay in kept for octo_head_later_grad_w, as
+ * octo_head_step_later (sizes from octo_head_later_bytes). */
+typedef struct octo_distill {
+  const int64_t *ids;
+  const float *teacher;
+  const float *weight;
+  int K;
+  int flags; /* OCTO_LIST_RAW */
+  float *dots, *q, *g;
+  float *kl;
+  float *loss;
+} octo_distill;
+int octo_head_step_distill(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const void *w, int64_t ldw,
+                           int w_dtype, const float *w_scale, const int64_t *idx, const int32_t *count, int64_t n_max,
+                           int d, int V, float inv_T, float pre, float post, int use_tanh, float *lse,
+                           const octo_distill *lists, void *grad_h, int64_t ld_gh, int gh_dtype, void *grad_w,
+                           int gw_dtype, void *kept, size_t kept_bytes, void *ws, size_t ws_bytes, void *stream);
+
 /* Embedding lookup (no counterpart in the reference): out[t, :d] = scale * w[ids[t], :d] in w's dtype (BF16, F16, F32),
  * zeros for an id outside [0, V). */
 int octo_embed_fwd(const void *w, int64_t ldw, int dtype, int64_t V, int d, const int64_t *ids, int64_t n, float scale,

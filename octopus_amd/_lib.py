@@ -38,6 +38,12 @@ class GrpoTail(ctypes.Structure):
                 ("eps_lo", _f32), ("eps_hi", _f32), ("reject_upper", _f32), ("g", _p), ("loss", _p)]
 
 
+class Distill(ctypes.Structure):
+    """octo_distill: the teachers' lists, row weights and outputs of octo_head_step_distill."""
+    _fields_ = [("ids", _p), ("teacher", _p), ("weight", _p), ("K", _i32), ("flags", _i32), ("dots", _p), ("q", _p),
+                ("g", _p), ("kl", _p), ("loss", _p)]
+
+
 # name -> argument types (restype is int unless listed in _RESTYPES)
 SIGNATURES = {
     "octo_version": [],
@@ -75,6 +81,8 @@ SIGNATURES = {
     "octo_topk": [_p, _i64, _i32, _i64, _i32, _f32, _i32, _p, _p, _p],
     "octo_distill_columns_fwd": [_p, _i64, _i32, _p, _p, _i64, _i32, _i32, _f32, _i32, _p, _p, _p, _p],
     "octo_distill_columns_bwd": [_p, _i64, _i32, _p, _p, _i64, _i32, _i32, _f32, _p, _p, _p, _i64, _p],
+    "octo_head_step_distill": [_p, _i64, _i64, _i32, _p, _i64, _i32, _p, _p, _p, _i64, _i32, _i32, _f32, _f32, _f32,
+                               _i32, _p, ctypes.POINTER(Distill), _p, _i64, _i32, _p, _i32, _p, _sz, _p, _sz, _p],
     "octo_embed_fwd": [_p, _i64, _i32, _i64, _i32, _p, _i64, _f32, _p, _i64, _p],
     "octo_embed_bwd_workspace_bytes": [_i64, _i64, _i32, ctypes.POINTER(_sz)],
     "octo_embed_bwd": [_p, _i64, _i32, _p, _i64, _i64, _i32, _i64, _f32, _p, _i64, _i32, _i32, _p, _sz, _p],

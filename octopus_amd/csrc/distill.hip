@@ -8,7 +8,7 @@
 //
 // Both directions are bound by memory: the forward reads each logit once, the backward reads it once more and writes
 // its gradient. The forward leaves q, and the row's (maximum, ln S), for the backward.
-#include "octo_common.h"
+#include "octo_internal.h"
 #include "row_values.h"
 
 namespace octo {
@@ -241,6 +241,181 @@ static void go_bwd(const void *logits, int64_t ld, const int64_t *ids, const flo
       hipLaunchKernelGGL((distill_columns_bwd_kernel<DT, false>), grid, dim3(256), 0, st, z, ld, ids + r0 * K,
                          q + r0 * K, V, K, inv_T, state + 4 * r0, g + r0, d, ld_d);
   }
+}
+
+// ---- the distillation step over hidden rows ---------------------------------------------------------------------------
+// A listed logit in the softmax's base-2 units before the row's maximum is taken off: x c, x the (soft-capped) logit.
+__device__ __forceinline__ float listed_x(const DistillArgs &a, float dot, int64_t y, bool exact_tanh) {
+  const float x = a.w_dtype == OCTO_FP8E4M3 ? dot * a.wscale[y] : dot;
+  return a.use_tanh ? (exact_tanh ? tanhf(a.pre * x) : ftanh(a.pre * x)) : x;
+}
+
+// One workgroup per compact row, a wave per slot in turn.
+constexpr int kDotWaves = 4;
+__global__ __launch_bounds__(64 * kDotWaves) void distill_dots_kernel(DistillArgs a) {
+  __shared__ float best[kDotWaves];
+  if (blockIdx.x == 0)
+    for (int k = threadIdx.x; k < a.nflag; k += 64 * kDotWaves) a.flag_cnt[k] = 0;
+  const int64_t r = blockIdx.x;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t cnt = a.count ? min((int64_t)(*a.count), a.n_max) : a.n_max;
+  if (r >= cnt) return;
+  const int64_t hrow = a.idx ? a.idx[r] : r;
+  float top = -INFINITY;
+  for (int k = w; k < a.K; k += kDotWaves) {
+    const int64_t y = a.ids[hrow * a.K + k];
+    float dot = 0.f;
+    if (y >= 0 && y < a.V && a.teacher[hrow * a.K + k] != -INFINITY) {
+      dot = wave_sum(row_dot(a.h, a.h_dtype, hrow * a.ldh, a.w, a.w_dtype, y * a.ldw, a.d, lane));
+      top = fmaxf(top, listed_x(a, dot, y, false));
+    }
+    if (lane == 0) a.dots[r * a.K + k] = dot;
+  }
+  if (lane == 0) best[w] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int k = 0; k < kDotWaves; ++k) top = fmaxf(top, best[k]);
+    a.xoff[r] = top == -INFINITY ? -INFINITY : __builtin_fmaf(top, a.c, kExAbove);
+  }
+}
+
+// One wave per row: merges the row's partials as merge_kernel does, then lane l takes slots l + 64 i.
+constexpr int kDistMergeRows = 4;
+__global__ __launch_bounds__(64 * kDistMergeRows) void distill_merge_kernel(DistillArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * kDistMergeRows + (threadIdx.x >> 6);
+  const int64_t r = a.r0 + i;
+  const int lane = threadIdx.x & 63;
+  const int64_t cnt = a.count ? min((int64_t)(*a.count), a.n_max) : a.n_max;
+  if (i >= a.rows || r >= cnt) return;
+  const int64_t hrow = a.idx ? a.idx[r] : r;
+  Stat3 st{-INFINITY, 0.f, 0.f};
+  const f32x4 *pr = a.part + i * a.mtiles;
+  for (int64_t k0 = lane; k0 < a.mtiles; k0 += 64 * kRowLoads) {
+    f32x4 p[kRowLoads];
+#pragma unroll
+    for (int u = 0; u < kRowLoads; ++u) p[u] = pr[min(k0 + 64 * u, a.mtiles - 1)];
+#pragma unroll
+    for (int u = 0; u < kRowLoads; ++u) {
+      if (k0 + 64 * u >= a.mtiles) break;
+      st = stat_merge(st, Stat3{fmaxf(p[u][0], p[u][3]), p[u][1], p[u][2]});
+    }
+  }
+  st = wave_stat_merge(st);
+  const float l2S = flog2(st.S);
+  int64_t id[kSlots];
+  float q[kSlots], lq[kSlots], Q, sum = 0.f;
+  teacher_slots(a.ids + hrow * a.K, a.teacher + hrow * a.K, a.K, a.V, a.raw != 0, lane, id, q, lq, Q);
+#pragma unroll
+  for (int s = 0; s < kSlots; ++s) {
+    const int k = lane + 64 * s;
+    if (k >= a.K) break;
+    if (id[s] >= 0 && q[s] != 0.f) {
+      const float x = listed_x(a, a.dots[r * a.K + k], id[s], true);
+      sum += q[s] * (lq[s] - (__builtin_fmaf(x, a.c, -st.m) - l2S) * OCTO_LN2);
+    }
+    a.q[r * a.K + k] = q[s];
+  }
+  sum = wave_sum(sum);
+  if (lane != 0) return;
+  const float wt = a.weight ? a.weight[hrow] : 1.f, g = -wt * Q;
+  a.kl[hrow] = sum;
+  a.g[r] = g;
+  a.lse[2 * r] = st.m;
+  a.lse[2 * r + 1] = l2S;
+  if (a.rowoff) {
+    const float xo = a.xoff[r];
+    if (st.m - xo <= kExClamp) {
+      a.xuse[i] = xo;
+    } else {  // the offset lies too low, or there is none; a row without weight needs no rescale, its scale is 0
+      a.xuse[i] = st.m;
+      if (g != 0.f) a.flag_rows[atomicAdd(a.flag_cnt, 1)] = (int32_t)i;
+    }
+  }
+}
+
+// One wave per row. Slots of one token all write the sum of their weights, taken in the list's order.
+constexpr int kEntryRows = 4;
+__global__ __launch_bounds__(64 * kEntryRows) void distill_entries_kernel(DistillArgs a) {
+  __shared__ int64_t slot_id[kEntryRows][OCTO_LIST_MAX];
+  __shared__ float slot_q[kEntryRows][OCTO_LIST_MAX];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t i = (int64_t)blockIdx.x * kEntryRows + w, r = a.r0 + i;
+  const int64_t cnt = a.count ? min((int64_t)(*a.count), a.n_max) : a.n_max;
+  const bool in = i < a.rows && r < cnt;
+  const int64_t hrow = in ? (a.idx ? a.idx[r] : r) : 0;
+  float Q = 0.f;
+  if (in) {
+    for (int k = lane; k < a.K; k += 64) {
+      const float q = a.q[r * a.K + k];
+      slot_q[w][k] = q;
+      slot_id[w][k] = q != 0.f ? a.ids[hrow * a.K + k] : -1;  // empty slots have q 0
+      Q += q;
+    }
+    Q = wave_sum(Q);
+  }
+  __syncthreads();
+  if (!in) return;
+  const float g = a.g[r];
+  if (g == 0.f) return;
+  const float m2 = a.lse[2 * r], l2S = a.lse[2 * r + 1];
+  for (int k = lane; k < a.K; k += 64) {
+    const int64_t y = slot_id[w][k];
+    if (y < 0) continue;
+    float share = 0.f;
+    for (int j = 0; j < a.K; ++j) share += slot_id[w][j] == y ? slot_q[w][j] : 0.f;
+    const float x = listed_x(a, a.dots[r * a.K + k], y, false);
+    float v = share / Q - fexp2(__builtin_fmaf(x, a.c, -m2) - l2S);
+    if (a.use_tanh) v *= 1.f - x * x;
+    if (a.w_dtype == OCTO_FP8E4M3) v *= a.wscale[y];
+    if (a.rowoff) ((__bf16 *)a.dz)[i * a.ldx + y] = (__bf16)(-v * fexp2(m2 - a.xuse[i] + l2S));
+    else if (a.f16) ((_Float16 *)a.dz)[i * a.ldx + y] = (_Float16)(g * a.gmul * v);
+    else ((__bf16 *)a.dz)[i * a.ldx + y] = (__bf16)(g * a.gmul * v);
+  }
+}
+
+// One workgroup: every thread's rows in order, in 64 bits, then a tree.
+__global__ __launch_bounds__(1024) void distill_loss_kernel(DistillArgs a, float *loss) {
+  __shared__ double part[1024];
+  const int64_t cnt = a.count ? min((int64_t)(*a.count), a.n_max) : a.n_max;
+  double s = 0.0;
+  for (int64_t r = threadIdx.x; r < cnt; r += 1024) {
+    const int64_t hrow = a.idx ? a.idx[r] : r;
+    const float wt = a.weight ? a.weight[hrow] : 1.f;
+    if (wt != 0.f) s += (double)wt * (double)a.kl[hrow];  // a row without weight, whatever its divergence is
+  }
+  part[threadIdx.x] = s;
+  __syncthreads();
+  for (int k = 512; k > 0; k >>= 1) {
+    if (threadIdx.x < k) part[threadIdx.x] += part[threadIdx.x + k];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *loss = (float)part[0];
+}
+
+int launch_distill_dots(const DistillArgs &a, hipStream_t st) {
+  if (a.n_max == 0) return OCTO_OK;
+  hipLaunchKernelGGL(distill_dots_kernel, dim3((unsigned)a.n_max), dim3(64 * kDotWaves), 0, st, a);
+  OCTO_CHECK_LAUNCH("distill_dots");
+  return OCTO_OK;
+}
+int launch_distill_merge(const DistillArgs &a, hipStream_t st) {
+  if (a.rows == 0) return OCTO_OK;
+  hipLaunchKernelGGL(distill_merge_kernel, dim3((unsigned)cdiv(a.rows, kDistMergeRows)), dim3(64 * kDistMergeRows), 0,
+                     st, a);
+  OCTO_CHECK_LAUNCH("distill_merge");
+  return OCTO_OK;
+}
+int launch_distill_entries(const DistillArgs &a, hipStream_t st) {
+  if (a.rows == 0) return OCTO_OK;
+  hipLaunchKernelGGL(distill_entries_kernel, dim3((unsigned)cdiv(a.rows, kEntryRows)), dim3(64 * kEntryRows), 0, st, a);
+  OCTO_CHECK_LAUNCH("distill_entries");
+  return OCTO_OK;
+}
+int launch_distill_loss(const DistillArgs &a, float *loss, hipStream_t st) {
+  hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(1024), 0, st, a, loss);
+  OCTO_CHECK_LAUNCH("distill_loss");
+  return OCTO_OK;
 }
 
 }  // namespace octo

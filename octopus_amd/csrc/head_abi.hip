@@ -406,14 +406,20 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
               int d, int V, int flags, float inv_T, float pre, float post, int use_tanh, float *logp, float *ent,
               float *lse, float *out2, int64_t ld_out2, const octo_grpo_tail *gt, void *grad_h, int64_t ld_gh,
               int gh_dtype, void *grad_w, int gw_dtype, void *ws, size_t ws_bytes, void *stream,
-              const StepPairs *pm = nullptr, void *later = nullptr) {
+              const StepPairs *pm = nullptr, void *later = nullptr, const octo_distill *ds = nullptr) {
   Common cm;
   int rc = check_common(h, h_rows, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, n_max, d, V, flags, inv_T,
                         pre, post, use_tanh, cm);
   if (rc) return rc;
-  OCTO_CHECK_ARG(gt != nullptr, "head_step_grpo: null grpo");
-  OCTO_CHECK_ARG(gt->n_tokens >= 0, "head_step_grpo: n_tokens < 0");
-  OCTO_CHECK_ARG(gt->g && gt->adv && gt->mask, "head_step_grpo: null g, adv or mask");
+  if (ds) {
+    OCTO_CHECK_ARG(ds->K >= 1 && ds->K <= OCTO_LIST_MAX, "head_step_distill: K=%d outside [1, %d]", ds->K, OCTO_LIST_MAX);
+    OCTO_CHECK_ARG((ds->flags & ~OCTO_LIST_RAW) == 0, "head_step_distill: unknown flags %d", ds->flags);
+    OCTO_CHECK_ARG(ds->teacher && ds->dots && ds->q && ds->g && ds->kl && ds->loss, "head_step_distill: null pointer");
+  } else {
+    OCTO_CHECK_ARG(gt != nullptr, "head_step_grpo: null grpo");
+    OCTO_CHECK_ARG(gt->n_tokens >= 0, "head_step_grpo: n_tokens < 0");
+    OCTO_CHECK_ARG(gt->g && gt->adv && gt->mask, "head_step_grpo: null g, adv or mask");
+  }
   OCTO_CHECK_ARG(lse != nullptr, "head_step_grpo: null lse");
   OCTO_CHECK_ARG(!out2 || ld_out2 >= 2, "head_step_grpo: ld_out2 < 2");
   if (grad_h) {
@@ -431,9 +437,10 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
                    "head_step_grpo_pairs: flat_pair, out_flat or ld_out");
     if (cm.dt == OCTO_F32) return octo_fail(OCTO_EUNSUPPORTED, "head_step_grpo_pairs: fp32 operands");
   }
+  if (ds && cm.dt == OCTO_F32) return octo_fail(OCTO_EUNSUPPORTED, "head_step_distill: fp32 operands");
   if (n_max == 0 && !pm) return OCTO_OK;
   // no gradient asked for: the forward with its GRPO tail (its own workspace size)
-  if (!need_gh && !need_gw && !pm && !later)
+  if (!need_gh && !need_gw && !pm && !later && !ds)
     return head_fwd(h, h_rows, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, count, n_max, d, V, flags, inv_T,
                     pre, post, use_tanh, logp, ent, lse, out2, ld_out2, gt, ws, ws_bytes, stream);
   if (cm.dt == OCTO_F32) {  // fp32: the forward, then the backward
@@ -473,7 +480,7 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
   void *ht = keep + L.ht, *dz = keep + L.dz, *wt = wsb + L.wt;
   const int esz = L.esz;
 
-  rc = launch_grpo_count(gt->mask, gt->n_tokens, z, gt->loss, st);  // Z, and the loss zeroed
+  if (gt) rc = launch_grpo_count(gt->mask, gt->n_tokens, z, gt->loss, st);  // Z, and the loss zeroed
   if (rc) return rc;
   const bool grads = need_gh || need_gw || later;
   float *rowout = (float *)(wsb + L.rowout);
@@ -520,7 +527,48 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
   float *xoff = (float *)(wsb + L.xoff), *tdot = (float *)(wsb + L.tdot);
   float *xuse = (float *)(wsb + L.xuse), *rscale = (float *)(wsb + L.scale);
   int32_t *flag_cnt = (int32_t *)(wsb + L.flags), *flag_rows = flag_cnt + L.passes;
-  if (rowoff) {
+  DistillArgs da{};
+  if (ds) {
+    da.h = h;
+    da.ldh = ldh;
+    da.h_dtype = h_dtype;
+    da.w = w;
+    da.ldw = ldw;
+    da.w_dtype = w_dtype;
+    da.wscale = w_scale;
+    da.idx = idx;
+    da.count = count;
+    da.n_max = n_max;
+    da.d = d;
+    da.V = V;
+    da.c = cm.c;
+    da.pre = cm.pre;
+    da.gmul = cm.gmul;
+    da.use_tanh = use_tanh;
+    da.ids = labels;
+    da.teacher = ds->teacher;
+    da.weight = ds->weight;
+    da.K = ds->K;
+    da.raw = (ds->flags & OCTO_LIST_RAW) != 0;
+    da.dots = ds->dots;
+    da.q = ds->q;
+    da.g = ds->g;
+    da.kl = ds->kl;
+    da.lse = lse;
+    da.xoff = xoff;
+    da.xuse = xuse;
+    da.flag_rows = flag_rows;
+    da.part = part;
+    da.mtiles = L.mtiles;
+    da.dz = dz;
+    da.ldx = L.V_pad;
+    da.rowoff = rowoff;
+    da.f16 = cm.dt == OCTO_F16;
+    da.flag_cnt = flag_cnt;
+    da.nflag = (int)L.passes;
+    rc = launch_distill_dots(da, st);
+    if (rc) return rc;
+  } else if (rowoff) {
     RowOffArgs ro{};
     ro.h = h;
     ro.ldh = ldh;
@@ -570,58 +618,66 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
     }
     if (rc) return rc;
 
-    // the pass's outputs, row state, GRPO weight g (the loss summed) and dz at each label per unit of g; pair rows:
-    // the rows' columns to rowout, then each flat token's columns and GRPO weight, summed into its pair's g
-    MergeArgs m = pm ? merge_args(part, L.mtiles, h, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, count,
-                                  n_max, d, V, flags, inv_T, pre, post, use_tanh, logp, ent, lse, rowout, 2, nullptr,
-                                  z)
-                     : merge_args(part, L.mtiles, h, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, count,
-                                  n_max, d, V, flags, inv_T, pre, post, use_tanh, logp, ent, lse, out2, ld_out2, gt, z);
-    m.row_off = r0;
-    m.rows = rows;
-    m.c = cm.c;
-    m.hit = hit;
-    if (rowoff) {
-      m.tdot = tdot;
-      m.exs = dz;
-      m.ldx = L.V_pad;
-      m.xoff = xoff;
-      m.xuse = xuse;
-      m.flag_cnt = flag_cnt + p;
-      m.flag_rows = flag_rows;
-    }
-    if (pm) {
-      m.zero_g = 1;
-      m.g_zero = (double *)(wsb + L.g64);
-    }
-    rc = launch_merge(m, st);
-    if (rc) return rc;
-    if (pm) {
-      PairsGrpoArgs pa{};
-      pa.flat_pair = pm->flat_pair;
-      pa.n_flat = pm->n_flat;
-      pa.r0 = r0;
-      pa.rows = rows;
-      pa.n_max = n_max;
-      pa.count = count;
-      pa.rowout = rowout;
-      pa.prox = gt->prox;
-      pa.old = gt->old;
-      pa.adv = gt->adv;
-      pa.mask = gt->mask;
-      pa.n_tokens = gt->n_tokens;
-      pa.eps_lo = gt->eps_lo;
-      pa.eps_hi = gt->eps_hi;
-      pa.reject_upper = gt->reject_upper;
-      pa.z = z;
-      pa.g64 = (double *)(wsb + L.g64);
-      pa.g = gt->g;
-      pa.loss = gt->loss;
-      pa.out2 = pm->out_flat;
-      pa.ld_out2 = pm->ld_out;
-      pa.first_pass = p == 0;
-      rc = launch_pairs_grpo(pa, st);
+    if (ds) {
+      da.r0 = r0;
+      da.rows = rows;
+      da.flag_cnt = flag_cnt + p;
+      rc = launch_distill_merge(da, st);
       if (rc) return rc;
+    } else {
+      // the pass's outputs, row state, GRPO weight g (the loss summed) and dz at each label per unit of g; pair rows:
+      // the rows' columns to rowout, then each flat token's columns and GRPO weight, summed into its pair's g
+      MergeArgs m = pm ? merge_args(part, L.mtiles, h, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, count,
+                                    n_max, d, V, flags, inv_T, pre, post, use_tanh, logp, ent, lse, rowout, 2, nullptr,
+                                    z)
+                       : merge_args(part, L.mtiles, h, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, count,
+                                    n_max, d, V, flags, inv_T, pre, post, use_tanh, logp, ent, lse, out2, ld_out2, gt, z);
+      m.row_off = r0;
+      m.rows = rows;
+      m.c = cm.c;
+      m.hit = hit;
+      if (rowoff) {
+        m.tdot = tdot;
+        m.exs = dz;
+        m.ldx = L.V_pad;
+        m.xoff = xoff;
+        m.xuse = xuse;
+        m.flag_cnt = flag_cnt + p;
+        m.flag_rows = flag_rows;
+      }
+      if (pm) {
+        m.zero_g = 1;
+        m.g_zero = (double *)(wsb + L.g64);
+      }
+      rc = launch_merge(m, st);
+      if (rc) return rc;
+      if (pm) {
+        PairsGrpoArgs pa{};
+        pa.flat_pair = pm->flat_pair;
+        pa.n_flat = pm->n_flat;
+        pa.r0 = r0;
+        pa.rows = rows;
+        pa.n_max = n_max;
+        pa.count = count;
+        pa.rowout = rowout;
+        pa.prox = gt->prox;
+        pa.old = gt->old;
+        pa.adv = gt->adv;
+        pa.mask = gt->mask;
+        pa.n_tokens = gt->n_tokens;
+        pa.eps_lo = gt->eps_lo;
+        pa.eps_hi = gt->eps_hi;
+        pa.reject_upper = gt->reject_upper;
+        pa.z = z;
+        pa.g64 = (double *)(wsb + L.g64);
+        pa.g = gt->g;
+        pa.loss = gt->loss;
+        pa.out2 = pm->out_flat;
+        pa.ld_out2 = pm->ld_out;
+        pa.first_pass = p == 0;
+        rc = launch_pairs_grpo(pa, st);
+        if (rc) return rc;
+      }
     }
     if (!grads) continue;
 
@@ -636,10 +692,10 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
       fx.xuse = xuse;
       fx.lse = lse;
       fx.lse_pair = (flags & OCTO_LSE_PAIR) != 0;
-      fx.g = gt->g;
+      fx.g = ds ? ds->g : gt->g;
       fx.gmul = cm.gmul;
       fx.hit = hit;
-      fx.labels = labels;
+      fx.labels = ds ? nullptr : labels;
       fx.label_idx = (flags & OCTO_ROWS_VIA_IDX) ? idx : nullptr;
       fx.count = count;
       fx.flag_cnt = flag_cnt + p;
@@ -664,10 +720,10 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
       sa.mtiles = L.mtiles;
       sa.lse = lse;
       sa.lse_pair = (flags & OCTO_LSE_PAIR) != 0;
-      sa.g = gt->g;
+      sa.g = ds ? ds->g : gt->g;
       sa.gmul = cm.gmul;
       sa.wscale = cm.fp8 ? w_scale : nullptr;
-      sa.labels = labels;
+      sa.labels = ds ? nullptr : labels;
       sa.label_idx = (flags & OCTO_ROWS_VIA_IDX) ? idx : nullptr;
       sa.hit = hit;
       sa.count = count;
@@ -679,6 +735,11 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
         TimedLaunch t("dz_scale", st);
         rc = launch_dz_scale(sa, st);
       }
+      if (rc) return rc;
+    }
+
+    if (ds) {
+      rc = launch_distill_entries(da, st);
       if (rc) return rc;
     }
 
@@ -721,7 +782,7 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
     if (!rc && need_gh) rc = launch_split_sum(s2, o2, false, st);
     if (rc) return rc;
   }
-  return OCTO_OK;
+  return ds ? launch_distill_loss(da, ds->loss, st) : OCTO_OK;
 }
 
 // ---- the allocation-free forward (octo_head_fwd_noalloc) ----------------------------------------
@@ -914,6 +975,26 @@ int octo_head_step_grpo_pairs(const void *h, int64_t h_rows, int64_t ldh, int h_
   return head_step(h, h_rows, ldh, h_dtype, w, ldw, w_dtype, w_scale, pair_label, pair_pos, pair_count, n_pairs, d,
                    V, flags, inv_T, pre, post, use_tanh, nullptr, nullptr, lse, nullptr, 2, grpo, grad_h, ld_gh,
                    gh_dtype, grad_w, gw_dtype, ws, ws_bytes, stream, &pm);
+}
+
+int octo_head_step_distill(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const void *w, int64_t ldw,
+                           int w_dtype, const float *w_scale, const int64_t *idx, const int32_t *count, int64_t n_max,
+                           int d, int V, float inv_T, float pre, float post, int use_tanh, float *lse,
+                           const octo_distill *lists, void *grad_h, int64_t ld_gh, int gh_dtype, void *grad_w,
+                           int gw_dtype, void *kept, size_t kept_bytes, void *ws, size_t ws_bytes, void *stream) {
+  OCTO_CHECK_ARG(lists && lists->ids, "head_step_distill: null lists");
+  if (kept) {
+    LaterLayout K;
+    OCTO_CHECK_ARG(n_max > 0 && !grad_w, "head_step_distill: kept operands beside a grad_w, or of no rows");
+    if (d <= 0 || V <= 0 || !later_plan(n_max, d, V, w_dtype, grad_h != nullptr, K))
+      return octo_fail(OCTO_EUNSUPPORTED, "head_step_distill: no kept operands for this call");
+    OCTO_CHECK_ARG((uintptr_t)kept % 16 == 0, "head_step_distill: misaligned buffer");
+    if (kept_bytes < K.kept)
+      return octo_fail(OCTO_EWORKSPACE, "head_step_distill: buffer %zu < %zu bytes", kept_bytes, K.kept);
+  }
+  return head_step(h, h_rows, ldh, h_dtype, w, ldw, w_dtype, w_scale, lists->ids, idx, count, n_max, d, V,
+                   OCTO_LSE_PAIR, inv_T, pre, post, use_tanh, nullptr, nullptr, lse, nullptr, 2, nullptr, grad_h, ld_gh,
+                   gh_dtype, grad_w, gw_dtype, ws, ws_bytes, stream, nullptr, kept, lists);
 }
 
 int octo_head_later_bytes(int64_t n_max, int d, int V, int w_dtype, int need_gh, size_t *kept_bytes, size_t *ws_bytes) {

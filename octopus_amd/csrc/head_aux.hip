@@ -203,7 +203,7 @@ __global__ __launch_bounds__(256) void dz_scale_kernel(DzScaleArgs a) {
   float m2, l2s;
   row_state(a.lse, a.lse_pair, r, m2, l2s);
   const float ngs = -(a.g[r] * a.gmul);
-  const int64_t y = a.labels[a.label_idx ? a.label_idx[r] : r];
+  const int64_t y = a.labels ? a.labels[a.label_idx ? a.label_idx[r] : r] : -1;
   const bool f16 = a.dtype == OCTO_F16;
   const f32x4 *pr = a.part + i * a.mtiles;
   char *row = (char *)a.dz + i * a.ld * 2;
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(256) void ex_fix_kernel(ExFixArgs a) {
     const float xo = a.xoff[r], xn = a.xuse[i];
     float m2, l2s;
     row_state(a.lse, a.lse_pair, r, m2, l2s);
-    const int64_t y = a.labels[a.label_idx ? a.label_idx[r] : r];
+    const int64_t y = a.labels ? a.labels[a.label_idx ? a.label_idx[r] : r] : -1;
     const f32x4 *pr = a.part + i * a.mtiles;
     char *row = (char *)a.ex + i * a.ldx * 2;
     i32x4 v[kExFixLoads];

@@ -279,7 +279,7 @@ struct ExFixArgs {
   const float *g;  // compact rows
   float gmul;
   const float *hit;  // local rows
-  const int64_t *labels;
+  const int64_t *labels;     // NULL: no label entry (launch_distill_entries writes the lists')
   const int64_t *label_idx;  // labels[label_idx[r]] when set
   const int32_t *count;
   const int32_t *flag_cnt, *flag_rows;
@@ -304,7 +304,7 @@ struct DzScaleArgs {
   const float *g;  // global rows
   float gmul;
   const float *wscale;  // [V] fp8 row scales, or NULL
-  const int64_t *labels;
+  const int64_t *labels;     // NULL: no label entry, as ExFixArgs
   const int64_t *label_idx;  // labels[label_idx[r]] when set
   const float *hit;          // local rows
   const int32_t *count;
@@ -360,6 +360,52 @@ struct PairsGrpoArgs {
   int first_pass;
 };
 int launch_pairs_grpo(const PairsGrpoArgs &a, hipStream_t st);
+
+// The distillation step (octo_head_step_distill; distill.hip): row r's list is that of its hidden row, K slots. With
+// q_k the teacher's probabilities, Q their sum and w the row's weight, the row's term is w kl and its dz that of a row
+// with GRPO weight g = -w Q whose one-hot label is spread over the list as q / Q:
+//   dz_v = g gmul (spread_v - p_v) post'(z_v).
+struct DistillArgs {
+  const void *h;
+  int64_t ldh;  // elements
+  int h_dtype;
+  const void *w;
+  int64_t ldw;  // elements
+  int w_dtype;
+  const float *wscale;
+  const int64_t *idx;  // compact row -> hidden row, or NULL
+  const int32_t *count;
+  int64_t n_max;
+  int d;
+  int64_t V;
+  float c, pre, gmul;
+  int use_tanh;
+  const int64_t *ids;  // [h_rows, K]
+  const float *teacher, *weight;
+  int K, raw;
+  float *dots, *q, *g, *kl, *lse;  // dots, q [n_max, K] and g, lse [n_max (, 2)] by compact row, kl by hidden row
+  // row-offset exponentials (bf16): as RowOffArgs and MergeArgs
+  float *xoff, *xuse;
+  int32_t *flag_cnt, *flag_rows;
+  int nflag;
+  // a pass: local row i is compact row r0 + i
+  int64_t r0, rows;
+  const f32x4 *part;  // local rows
+  int64_t mtiles;
+  void *dz;  // local rows: bf16 exponentials relative to xuse (rowoff), else dz in f16
+  int64_t ldx;
+  int rowoff, f16;
+};
+// dots[r][k] = h_r . W_ids[k], fp32 (0 for an empty slot); with xoff, the row's offset: its largest listed logit +
+// kExAbove (-inf for a row without a slot); flag_cnt[0 .. nflag) = 0.
+int launch_distill_dots(const DistillArgs &a, hipStream_t st);
+// The pass's rows: the row state, q, kl, g and, with rowoff, xuse and the flagged rows (launch_merge's).
+int launch_distill_merge(const DistillArgs &a, hipStream_t st);
+// The pass's listed entries of dz over the dense values, after launch_ex_fix or launch_dz_scale.
+int launch_distill_entries(const DistillArgs &a, hipStream_t st);
+// *loss = the sum of weight x kl over the compact rows, in a fixed order.
+int launch_distill_loss(const DistillArgs &a, float *loss, hipStream_t st);
+
 // dst row r (row_bytes, contiguous) = src row idx[r] (ld_src_bytes apart) for r < *count; 16-byte aligned rows
 int launch_rows_gather(const void *src, int64_t ld_src_bytes, const int64_t *idx, const int32_t *count,
                        int64_t n_max, int64_t row_bytes, void *dst, hipStream_t st);

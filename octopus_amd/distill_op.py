@@ -2,6 +2,7 @@
 
     head_topk                          the teacher's list: the k largest logits of a row and their log-probabilities
     octohead::distill_columns_fwd/bwd  the student's divergence from the lists over materialised logits
+    octohead::head_step_distill        the same from hidden rows and the vocabulary weight, loss and gradients in one call
 
 A row's list is K slots (ids[r, k], teacher[r, k]): tokens, and the teacher's logits or log-probabilities of them, as
 head_topk gives them. A slot whose id lies outside [0, V) or whose teacher value is -inf is empty (shorter lists), and the
@@ -16,12 +17,16 @@ HIP tensors only; all work is queued on the current stream of the tensors' devic
 
 from __future__ import annotations
 
+import ctypes
+from typing import Optional
+
 import torch
 from torch import Tensor
 
-from . import _lib
+from . import _lib, head_op
 from .embed_op import _float_rows, _ids, _on_gpu
-from .head_op import _DT, _p, _stream
+from .head_op import (_DT, Post, _dtype_code, _empty, _gather_flag, _index, _later_bytes, _p, _rows2d, _stream,
+                      _workspace, _zeros, later_grad_w, scaled)
 
 
 def _lists(ids: Tensor, teacher: Tensor, rows: int) -> tuple[Tensor, Tensor]:
@@ -144,3 +149,172 @@ def distill_columns(logits: Tensor, temperature: float, ids: Tensor, teacher: Te
     if logits.dim() != 2:
         raise ValueError(f"octohead: logits must be [n, V], got {tuple(logits.shape)}")
     return distill_columns_fwd(logits, ids, teacher.detach(), _inv_T(temperature), not normalise)[0]
+
+
+# ---- the divergence from hidden rows: loss and gradients in one call ------------------------------------------------------
+
+def _step(rows: Tensor, weight: Tensor, w_scale: Optional[Tensor], ids: Tensor, teacher: Tensor,
+          row_weight: Optional[Tensor], idx: Optional[Tensor], count: Optional[Tensor], inv_T: float, pre: float,
+          post: float, use_tanh: bool, raw: bool, need_rows: bool, need_weight: bool, kept: Optional[Tensor]):
+    """(loss, kl, grad_rows, grad_w) of octo_head_step_distill; kept: the buffer that takes grad_w's operands."""
+    dev = _on_gpu(rows, weight, w_scale, ids, teacher, row_weight, idx, count)
+    rows2, weight2, idx = _rows2d(rows), _rows2d(weight), _index(idx)
+    ids, teacher = _lists(ids, teacher, rows2.shape[0])
+    if rows2.shape[1] != weight2.shape[1]:
+        raise ValueError(f"octohead: rows of width {rows2.shape[1]} against a weight of width {weight2.shape[1]}")
+    if row_weight is not None:
+        if row_weight.shape != (rows2.shape[0],):
+            raise ValueError(f"octohead: row weights [{rows2.shape[0]}] expected, got {tuple(row_weight.shape)}")
+        row_weight = row_weight.float().contiguous()
+    n_max = idx.numel() if idx is not None else rows2.shape[0]
+    V, d = weight2.shape
+    K = ids.shape[1]
+    f = lambda *s: torch.empty(*s, dtype=torch.float32, device=dev)  # noqa: E731
+    kl = torch.zeros(rows2.shape[0], dtype=torch.float32, device=dev)
+    loss = torch.zeros((), dtype=torch.float32, device=dev)
+    grad_rows = _zeros(rows) if need_rows else rows.new_empty(0)
+    grad_w = weight.new_empty(0) if not need_weight or kept is not None else \
+        (_zeros(weight) if n_max == 0 else _empty(weight))
+    if n_max == 0:
+        return loss, kl, grad_rows, grad_w
+    code = _dtype_code(weight2)
+    if kept is not None:
+        nbytes = _lib.later_workspace_bytes(n_max, d, V, code, need_rows)
+    else:
+        flags = (_lib.WS_STEP | (0 if need_weight else _lib.WS_NO_GRADW) | (0 if need_rows else _lib.WS_NO_GRADH)
+                 | _gather_flag(rows2, idx))
+        nbytes = _lib.workspace_bytes(n_max, d, V, code, flags)
+        if head_op.STEP_WORKSPACE_BYTES is not None:
+            nbytes = int(head_op.STEP_WORKSPACE_BYTES)
+    ws = _workspace(nbytes, rows2)
+    dots, q, g, lse = f(n_max, K), f(n_max, K), f(n_max), f(n_max, 2)
+    lists = _lib.Distill(_p(ids), _p(teacher), _p(row_weight), K, _lib.LIST_RAW if raw else 0, _p(dots), _p(q), _p(g),
+                         _p(kl), _p(loss))
+    gh = None
+    if need_rows:  # compact-order rows; scattered into grad_rows below
+        gh = grad_rows if idx is None else torch.empty(n_max, d, dtype=rows2.dtype, device=dev)
+    gw = grad_w if need_weight and kept is None else None
+    with torch.cuda.device(dev):
+        _lib.call("octo_head_step_distill", _p(rows2), rows2.shape[0], rows2.stride(0), _dtype_code(rows2),
+                  _p(weight2), weight2.stride(0), code, _p(w_scale), _p(idx), _p(count), n_max, d, V, inv_T, pre, post,
+                  int(use_tanh), _p(lse), ctypes.byref(lists), _p(gh), d,
+                  _dtype_code(rows2) if need_rows else _lib.F32, _p(gw), code if gw is not None else _lib.F32,
+                  _p(kept), 0 if kept is None else kept.numel(), _p(ws), ws.numel(), _stream(rows2))
+        if need_rows and idx is not None:
+            _lib.call("octo_rows_scatter", _p(gh), d, _dtype_code(gh), _p(idx), _p(count), n_max, d, _p(grad_rows),
+                      grad_rows.stride(0), _dtype_code(grad_rows), 0, _stream(rows2))
+    return loss, kl, grad_rows, grad_w
+
+
+@torch.library.custom_op("octohead::head_step_distill", mutates_args=(), device_types="cuda")
+def head_step_distill(rows: Tensor, weight: Tensor, w_scale: Optional[Tensor], ids: Tensor, teacher: Tensor,
+                      row_weight: Optional[Tensor], idx: Optional[Tensor], count: Optional[Tensor], inv_T: float,
+                      pre: float, post: float, use_tanh: bool, raw: bool, need_rows: bool,
+                      need_weight: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(loss, kl [rows], grad_rows [rows, d], grad_weight [V, d]); a gradient not asked for is an empty tensor."""
+    return _step(rows, weight, w_scale, ids, teacher, row_weight, idx, count, inv_T, pre, post, use_tanh, raw,
+                 need_rows, need_weight, None)
+
+
+@head_step_distill.register_fake
+def _(rows, weight, w_scale, ids, teacher, row_weight, idx, count, inv_T, pre, post, use_tanh, raw, need_rows,
+      need_weight):
+    return (rows.new_empty((), dtype=torch.float32), rows.new_empty(rows.shape[0], dtype=torch.float32),
+            _empty(rows) if need_rows else rows.new_empty(0), _empty(weight) if need_weight else weight.new_empty(0))
+
+
+def _step_setup(ctx, inputs, output):
+    # held as detached aliases, not saved: an offload's pack hook never copies the [V, d] gradient to the host
+    ctx.grads = (output[2].detach(), output[3].detach())
+    ctx.need = inputs[-2:]
+    ctx.set_materialize_grads(False)
+
+
+def _step_backward(ctx, gloss, _gkl, _ggr, _ggw):
+    out = []
+    for k in range(2):
+        if not (ctx.need[k] and ctx.needs_input_grad[k]):
+            out.append(None)
+        else:
+            out.append(torch.zeros_like(ctx.grads[k]) if gloss is None else scaled(ctx.grads[k], gloss))
+    return (*out,) + (None,) * 13
+
+
+torch.library.register_autograd("octohead::head_step_distill", _step_backward, setup_context=_step_setup)
+
+
+@torch.library.custom_op("octohead::head_step_distill_later", mutates_args=(), device_types="cuda")
+def head_step_distill_later(rows: Tensor, weight: Tensor, ids: Tensor, teacher: Tensor, row_weight: Optional[Tensor],
+                            idx: Optional[Tensor], count: Optional[Tensor], inv_T: float, pre: float, post: float,
+                            use_tanh: bool, raw: bool, need_rows: bool,
+                            nbytes: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """head_step_distill's (loss, kl, grad_rows), the buffer of nbytes that later_grad_w makes grad_weight of, and the row
+    count as the call found it."""
+    n_max = idx.numel() if idx is not None else rows.shape[0]
+    kept_count = torch.full((1,), n_max, dtype=torch.int32, device=rows.device) if count is None \
+        else count.reshape(-1)[:1].to(torch.int32, copy=True)
+    kept = _workspace(nbytes, rows)
+    loss, kl, grad_rows, _ = _step(rows, weight, None, ids, teacher, row_weight, idx, count, inv_T, pre, post, use_tanh,
+                                   raw, need_rows, True, kept)
+    return loss, kl, grad_rows, kept, kept_count
+
+
+@head_step_distill_later.register_fake
+def _(rows, weight, ids, teacher, row_weight, idx, count, inv_T, pre, post, use_tanh, raw, need_rows, nbytes):
+    return (rows.new_empty((), dtype=torch.float32), rows.new_empty(rows.shape[0], dtype=torch.float32),
+            _empty(rows) if need_rows else rows.new_empty(0), rows.new_empty(nbytes, dtype=torch.uint8),
+            rows.new_empty(1, dtype=torch.int32))
+
+
+def _later_setup(ctx, inputs, output):
+    rows, weight, idx = inputs[0], inputs[1], inputs[5]
+    ctx.held = (output[2].detach(), output[3].detach(), output[4].detach())
+    ctx.sizes = (idx.numel() if idx is not None else rows.shape[0], weight.shape[1], weight.shape[0], weight.dtype)
+    ctx.need_rows = inputs[-2]
+    ctx.set_materialize_grads(False)
+
+
+def _later_backward(ctx, gloss, _gkl, _ggr, _gkept, _gcount):
+    grad_rows, kept, count = ctx.held
+    n_max, d, V, dtype = ctx.sizes
+    gr = gw = None
+    if ctx.need_rows and ctx.needs_input_grad[0]:
+        gr = torch.zeros_like(grad_rows) if gloss is None else scaled(grad_rows, gloss)
+    if ctx.needs_input_grad[1]:
+        gw = torch.zeros(V, d, dtype=dtype, device=kept.device) if gloss is None \
+            else later_grad_w(kept, count, gloss, n_max, d, V, dtype, ctx.need_rows)
+    return (gr, gw) + (None,) * 12
+
+
+torch.library.register_autograd("octohead::head_step_distill_later", _later_backward, setup_context=_later_setup)
+
+
+def fused_distill_head(rows: Tensor, weight: Tensor, ids: Tensor, teacher: Tensor, temperature: float,
+                       row_weight: Optional[Tensor] = None, *, normalise: bool = True, post: Post = Post(),
+                       idx: Optional[Tensor] = None, count: Optional[Tensor] = None,
+                       w_scale: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
+    """(loss, kl): loss = sum over the rows of row_weight x kl (None: 1 each), z = post(rows W^T), and kl [rows] fp32
+    detached, from one call that computes the logits once and also the gradients of the loss in rows and weight (each when
+    it requires grad and grad mode is on). loss.backward() only scales them or, for a short call, makes the weight's from
+    the operands kept, as fused_grpo_head's. ids and teacher are [rows, K], row_weight [rows]. idx, count: the rows that
+    take part (compact_rows; count on the device); the others' kl and gradients are 0. A row of weight 0 adds nothing to
+    the loss, but is computed with: leave rows out by idx. bf16, f16 and fp8 weights (w_scale; no gradient of those).
+    The prefix tree's teacher values depend on the path alone, so a tree's rows are its positions, each once, weighted by
+    the tokens that share it. The gradients or operands are held from this call until the graph goes."""
+    inv_T = _inv_T(temperature)
+    if rows.dim() != 2 or weight.dim() != 2:
+        raise ValueError(f"octohead: rows [n, d] and weight [V, d] expected, got {tuple(rows.shape)} and "
+                         f"{tuple(weight.shape)}")
+    grad_on = torch.is_grad_enabled()
+    need_rows, need_weight = grad_on and rows.requires_grad, grad_on and weight.requires_grad
+    teacher = teacher.detach()
+    row_weight = None if row_weight is None else row_weight.detach()
+    xf = (inv_T, float(post.pre), float(post.post), bool(post.tanh), not normalise)
+    nbytes = _later_bytes(rows, weight, idx, need_rows, need_weight)
+    if nbytes:
+        loss, kl, *_ = head_step_distill_later(rows, weight, ids, teacher, row_weight, idx, count, *xf, need_rows,
+                                               nbytes)
+    else:
+        loss, kl, *_ = head_step_distill(rows, weight, w_scale, ids, teacher, row_weight, idx, count, *xf, need_rows,
+                                         need_weight)
+    return loss, kl.detach()

@@ -1,0 +1,322 @@
+"""fused_distill_head against the 64-bit oracle: the divergence, the loss, both gradients.
+
+Bounds, per element. A logit is a sum of d products in fp32: off by at most (d / 8 + 16) 2^-24 sum |h w| (a matrix
+instruction adds blocks of products; the dot products of the lists add d / 64 per lane and a tree). e_z is that over T, at
+most twice in a divergence: 2 e_z + 4e-5 Q (the bound of distill_columns) + 2^-21 sum q |log q - log p|.
+dz is rounded once to the operands' type, relative to itself (bf16 2^-8 with the fp32 scale's part: 1.05 x 2^-8; f16
+2^-11, twice, and 2^-25 of the half tile's largest where it is subnormal; bf16 exponentials are stored against an offset
+at most 48 bits above the row's maximum, so that what lies below 2^-126 of the offset, p below 2^-78, may be lost; in a row
+that is rescaled a half tile's factor is exp2(m_h - m2 - 64), 0 below 2^-126, so that a half tile whose maximum lies more
+than 62 bits below the row's is lost: 2^-62 g per element), and its p is off by 2 e_z + 2^-14 relative.
+grad_h = dz W takes those through |W|; grad_W = dz^T h through |h|, whose scaled copy is rounded once more (bf16). Both
+are rounded once to their type, and summed in fp32 over up to V or n terms: 2^-14 of the magnitudes' sum."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import distill as odist
+from oracle import fp8 as ofp8
+
+pytestmark = pytest.mark.gpu
+HALF = {torch.bfloat16: 2 ** -8, torch.float16: 2 ** -11}
+
+
+def _batch(n, d, V, K, dtype, seed, spread=2.5, holes=True):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(n, d, generator=g).to(dtype)
+    w = (torch.randn(V, d, generator=g) * (spread / math.sqrt(d))).to(dtype)
+    z = h.double() @ w.double().T + torch.randn(n, V, generator=g)
+    t, ids = z.topk(min(K, V), 1)
+    t = (t - z.logsumexp(1, keepdim=True)).float()
+    if holes:
+        ids[torch.rand(ids.shape, generator=g) < 0.1] = -1
+        ids[torch.rand(ids.shape, generator=g) < 0.02] = V
+        if n > 3:
+            ids[1] = -1
+            t[2] = -math.inf
+            ids[3, :] = ids[3, 0]
+    rw = torch.rand(n, generator=g) + 0.1
+    rw[torch.rand(n, generator=g) < 0.2] = 0.0
+    return h, w, ids, t, rw
+
+
+def _oracle(h, w, ids, t, rw, T, post, normalise=True):
+    pre, pst, tanh = post
+    z = h.double() @ w.double().T
+    th = torch.tanh(pre * z) if tanh else None
+    s = (pst * th if tanh else pre * pst * z) / T
+    slope = pre * pst * ((1 - th ** 2) if tanh else 1.0) / T
+    kl, dkl = odist.divergence(s, ids, t, normalise)
+    dz = dkl * rw.double()[:, None] * slope
+    q = odist.weights(ids, t, w.shape[0], normalise)
+    Q = q.sum(1)
+    lp = torch.log_softmax(s, 1).gather(1, ids.clamp(0, w.shape[0] - 1))
+    terms = torch.where(q > 0, q * (torch.log(q).abs() + lp.abs()), torch.zeros_like(q)).sum(1)
+    ez = (h.shape[1] / 8 + 16) * 2 ** -24 * (h.double().abs() @ w.double().abs().T).amax(1) * abs(pre * pst) / T
+    kl_tol = (2 * ez + 4e-5) * Q.clamp(min=1e-3) + 2 ** -21 * terms
+    spread = torch.zeros_like(z).scatter_add_(1, ids.clamp(0, w.shape[0] - 1), q)
+    size = (Q[:, None] * torch.softmax(s, 1) + spread) * rw.double().abs()[:, None] * abs(slope)
+    lost = 2 ** -62 * (Q * rw.double().abs())[:, None] * torch.as_tensor(slope).abs()
+    return kl, kl_tol, dz, size * (2 * ez + 2 ** -14)[:, None] + lost
+
+
+def _check(h, w, ids, t, rw, T=1.0, post=(1.0, 1.0, False), scored=None, w_scale=None, q8=None, normalise=True, c=1.0,
+           ws=None):
+    from octopus_amd import head_op
+    from octopus_amd.distill_op import fused_distill_head
+    from octopus_amd.head_op import Post, compact_rows
+
+    dtype = h.dtype
+    hd = h.cuda().requires_grad_(True)
+    wd = (w if q8 is None else q8).cuda().requires_grad_(q8 is None)
+    idx = count = None
+    part = torch.ones(len(h), dtype=torch.bool) if scored is None else scored
+    if scored is not None:
+        idx, count = compact_rows(scored.cuda())
+    head_op.STEP_WORKSPACE_BYTES = ws
+    try:
+        loss, kl = fused_distill_head(hd, wd, ids.cuda(), t.cuda(), T, None if rw is None else rw.cuda(),
+                                      normalise=normalise, post=Post(*post), idx=idx, count=count,
+                                      w_scale=None if w_scale is None else w_scale.cuda())
+    finally:
+        head_op.STEP_WORKSPACE_BYTES = None
+    (loss * c).backward()
+    weight = (torch.ones(len(h)) if rw is None else rw) * part
+    # to the oracle the rows that take no part have no list, whatever theirs holds
+    want, kl_tol, dz, dz_err = _oracle(h, w, torch.where(part[:, None], ids, -1), torch.where(part[:, None], t, 0.0),
+                                       weight, T, post, normalise)
+    got = kl.cpu().double()
+    assert (got[~part] == 0).all()
+    assert ((got - want).abs()[part] <= kl_tol[part]).all(), ((got - want).abs() / kl_tol)[part].max()
+    want_loss = (weight.double() * want)[part].sum()
+    assert abs(loss.item() - want_loss.item()) <= ((weight.double().abs() * kl_tol)[part].sum()
+                                                   + 2 ** -23 * want_loss.abs()).item()
+    dz, dz_err = dz * c, dz_err * abs(c)
+    r = HALF[dtype] * 1.05
+    floor = 0.0 if dtype == torch.bfloat16 else 2 ** -24 * max(1.0, abs(c))
+    per = dz_err + (r if dtype == torch.bfloat16 else 2 * r) * dz.abs() + floor
+    wa, ha = w.double().abs(), h.double().abs()
+    gh = dz @ w.double()
+    tol = per @ wa + 2 ** -14 * (dz.abs() @ wa) + 2 * r * gh.abs() + floor  # rounded, scaled by c and rounded again
+    err = (hd.grad.cpu().double() - gh).abs()
+    assert (err <= tol).all(), (err / tol.clamp(min=1e-300)).max()
+    if q8 is None:
+        gw = dz.T @ h.double()
+        tol = (per + r * dz.abs()).T @ ha + 2 ** -14 * (dz.abs().T @ ha) + 2 * r * gw.abs() + floor
+        err = (wd.grad.cpu().double() - gw).abs()
+        assert (err <= tol).all(), (err / tol.clamp(min=1e-300)).max()
+        assert ((wd.grad.cpu().double() - gw).norm() <= 1e-2 * gw.norm() + floor * gw.numel() ** 0.5)
+    assert (hd.grad.cpu().double() - gh).norm() <= 1e-2 * gh.norm() + floor * gh.numel() ** 0.5
+    return loss.detach(), kl, hd.grad, wd.grad
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,d,V,K", [(1, 8, 5, 5), (1, 64, 300, 1), (5, 128, 1000, 7), (70, 256, 2048, 64), (257, 264, 1531, 20),
+                                     (300, 512, 4160, 256)])
+def test_sizes(dtype, n, d, V, K):
+    _check(*_batch(n, d, V, K, dtype, n + V), T=1.0 if V % 2 else 0.7)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("post", [(1 / 30.0, 30.0, True), (0.5, 0.25, False), (2.0, 1.5, False)])
+def test_post_head_transforms(dtype, post):
+    _check(*_batch(90, 256, 1280, 30, dtype, 5, spread=6.0 if post[2] else 2.5), T=0.9, post=post)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_some_rows_take_part(dtype):
+    """Rows left out by a mask (the count stays on the device): none of their lists, weights or hidden values matter."""
+    h, w, ids, t, rw = _batch(150, 128, 900, 12, dtype, 7)
+    scored = torch.rand(150, generator=torch.Generator().manual_seed(8)) < 0.5
+    a = _check(h, w, ids, t, rw, scored=scored)
+    ids2, t2, rw2 = ids.clone(), t.clone(), rw.clone()
+    ids2[~scored], t2[~scored], rw2[~scored] = 3, math.nan, math.nan
+    b = _check(h, w, ids2, torch.where(scored[:, None], t2, torch.nan), torch.where(scored, rw2, 0.0), scored=scored)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    _check(h, w, ids, t, rw, scored=torch.zeros(150, dtype=torch.bool))
+    _check(h, w, ids, t, rw, scored=torch.ones(150, dtype=torch.bool))
+
+
+def test_no_weights_raw_lists_and_a_scaled_loss():
+    h, w, ids, t, rw = _batch(64, 128, 700, 10, torch.bfloat16, 9)
+    _check(h, w, ids, t, None)
+    _check(h, w, ids, t, rw, normalise=False)
+    _check(h, w, ids, t, -rw, c=1 / 3)
+    _check(h, w, torch.full_like(ids, -1), t, rw)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_listed_far_below_the_maximum(dtype):
+    """Lists of unlikely tokens at a low temperature: the largest listed logit lies up to hundreds of bits below the row's
+    maximum, past the stored exponentials' offset."""
+    h, w, ids, t, rw = _batch(130, 64, 600, 6, dtype, 10, holes=False)
+    g = torch.Generator().manual_seed(11)
+    ids = torch.randint(0, 600, ids.shape, generator=g)
+    if dtype == torch.float16:
+        rw = rw * 2 ** -4  # dz up to 1 / T: within the type's range
+    _check(h, w, ids, t, rw, T=0.03)
+
+
+def test_fp8_weights():
+    h, w, ids, t, rw = _batch(140, 256, 1300, 16, torch.bfloat16, 12)
+    scale = (w.float().abs().amax(1) / 448).clamp(min=1e-12)
+    q8 = (w.float() / scale[:, None]).to(torch.float8_e4m3fn)
+    w32 = q8.float() * scale[:, None]
+    z = h.double() @ w32.double().T
+    _check(h, w32, ids, t, rw, w_scale=scale, q8=q8, T=0.8)
+    _check(h, w32, ids, t, rw, w_scale=scale, q8=q8, post=(1 / 20.0, 20.0, True))
+    assert z.isfinite().all()
+
+
+def test_several_passes():
+    """A workspace of several row passes: the same divergences to the bit, gradients within their bounds."""
+    from octopus_amd import _lib
+
+    n, d, V, K = 900, 256, 1536, 24
+    batch = _batch(n, d, V, K, torch.bfloat16, 13)
+    ws = _lib.workspace_bytes(n, d, V, _lib.BF16, _lib.WS_STEP)
+    while _lib.bwd_plan(n, d, V, _lib.BF16, _lib.WS_STEP, ws)[1] < 3:
+        ws = ws * 9 // 10
+    a = _check(*batch)
+    b = _check(*batch, ws=ws)
+    assert torch.equal(a[1], b[1]) and torch.equal(a[0], b[0])
+    scored = torch.arange(n) < 300  # later passes past the device count
+    _check(*batch, ws=ws, scored=scored)
+
+
+def test_weight_gradient_made_in_the_backward():
+    """A short call of a large weight keeps grad_W's operands: the same gradients as the call that makes it at once,
+    through a second backward and a scaled loss."""
+    from octopus_amd import distill_op
+
+    n, d, V, K = 40, 1024, 131072, 16
+    g = torch.Generator(device="cuda").manual_seed(14)
+    h = torch.randn(n, d, device="cuda", generator=g).to(torch.bfloat16).requires_grad_(True)
+    w = (torch.randn(V, d, device="cuda", generator=g) * 0.08).to(torch.bfloat16).requires_grad_(True)
+    ids = torch.randint(0, V, (n, K), device="cuda", generator=g)
+    t = torch.randn(n, K, device="cuda", generator=g)
+    rw = torch.rand(n, device="cuda", generator=g)
+    assert distill_op._later_bytes(h, w, None, True, True)
+    loss, kl = distill_op.fused_distill_head(h, w, ids, t, 1.0, rw)
+    got = torch.autograd.grad(loss * 0.5, (h, w), retain_graph=True)
+    again = torch.autograd.grad(loss * 0.5, (h, w))
+    want = distill_op.head_step_distill(h, w, None, ids, t, rw, None, None, 1.0, 1.0, 1.0, False, False, True, True)
+    assert torch.equal(loss, want[0]) and torch.equal(kl, want[1])
+    for a, b, c in zip(got, again, want[2:]):
+        assert torch.equal(a, b)
+        # the same dz and h^T; grad_h the same sums (split differently), each rounded once or twice
+        assert (a.float() - 0.5 * c.float()).norm() <= 2 ** -8 * 0.5 * c.float().norm()
+
+
+def test_gradient_against_differences():
+    """Central differences of the fused loss's own 64-bit value in a direction of the hidden rows and one of the weight."""
+    h, w, ids, t, rw = _batch(20, 64, 300, 8, torch.bfloat16, 15)
+    _, _, gh, gw = _check(h, w, ids, t, rw)
+    g = torch.Generator().manual_seed(16)
+    dh, dw = torch.randn(h.shape, generator=g).double(), torch.randn(w.shape, generator=g).double()
+    e = 1e-5
+
+    def loss(a, b):
+        s = (h.double() + a * dh) @ (w.double() + b * dw).T
+        return (rw.double() * odist.divergence(s, ids, t)[0]).sum()
+
+    for grad, direction, up, dn in [(gh, dh, loss(e, 0), loss(-e, 0)), (gw, dw, loss(0, e), loss(0, -e))]:
+        want = ((up - dn) / (2 * e)).item()
+        got = (grad.cpu().double() * direction).sum().item()
+        # each gradient element is within 2 x 2^-8 of itself and of its terms: 1e-2 of the norms' product at random signs
+        assert abs(got - want) <= 1e-2 * (grad.cpu().double().norm() * direction.norm()).item()
+
+
+def test_hooks_no_grad_and_frozen_sides():
+    from octopus_amd.distill_op import fused_distill_head
+
+    h, w, ids, t, rw = (x.cuda() for x in _batch(50, 128, 800, 9, torch.bfloat16, 17))
+    with torch.no_grad():
+        loss0, kl0 = fused_distill_head(h, w, ids, t, 1.0, rw)
+    assert not loss0.requires_grad
+    hr, wr = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: packed.append(x.shape) or x, lambda x: x):
+        loss, kl = fused_distill_head(hr, wr, ids, t, 1.0, rw)
+    assert torch.equal(loss0, loss) and torch.equal(kl0, kl) and tuple(w.shape) not in [tuple(s) for s in packed]
+    gh, gw = torch.autograd.grad(loss, (hr, wr))
+    loss, _ = fused_distill_head(hr, w, ids, t, 1.0, rw)
+    (only_h,) = torch.autograd.grad(loss, hr)
+    loss, _ = fused_distill_head(h, wr, ids, t, 1.0, rw)
+    (only_w,) = torch.autograd.grad(loss, wr)
+    assert (only_h - gh).norm() <= 2 ** -8 * gh.norm() and (only_w - gw).norm() <= 2 ** -8 * gw.norm()
+
+
+def test_poisoned_memory_and_repeats():
+    """Every buffer the call allocates filled with 0xFF first: the same bits, twice."""
+    from octopus_amd.distill_op import fused_distill_head
+
+    h, w, ids, t, rw = (x.cuda() for x in _batch(200, 256, 1100, 33, torch.bfloat16, 18))
+    scored = torch.rand(200, generator=torch.Generator().manual_seed(19)).cuda() < 0.6
+    from octopus_amd.head_op import compact_rows
+
+    def once():
+        idx, count = compact_rows(scored)
+        hr, wr = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        loss, kl = fused_distill_head(hr, wr, ids, t, 1.0, rw, idx=idx, count=count)
+        return [x.clone() for x in (loss.detach(), kl, *torch.autograd.grad(loss, (hr, wr)))]
+
+    want = once()
+    real = torch.empty
+
+    def poisoned(*a, **k):
+        x = real(*a, **k)
+        if x.is_cuda and x.numel() and x.is_contiguous():
+            x.view(torch.uint8 if x.dim() else x.dtype).fill_(255) if x.dim() else x.fill_(math.nan)
+        return x
+
+    for _ in range(2):
+        torch.empty = poisoned
+        try:
+            got = once()
+        finally:
+            torch.empty = real
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_graph_replays():
+    from octopus_amd.distill_op import head_step_distill
+
+    h, w, ids, t, rw = (x.cuda() for x in _batch(120, 256, 2000, 20, torch.bfloat16, 20))
+
+    def step():
+        return head_step_distill(h, w, None, ids, t, rw, None, None, 1.0, 1.0, 1.0, False, False, True, True)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = step()
+    for s in range(3):
+        h.copy_(torch.randn(120, 256, generator=torch.Generator().manual_seed(s)).to(torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(kept, step()))
+
+
+def test_refusals():
+    from octopus_amd.distill_op import fused_distill_head
+
+    h, w, ids, t, rw = (x.cuda() for x in _batch(10, 64, 100, 5, torch.bfloat16, 21))
+    wide = torch.zeros(10, 257, device="cuda")
+    for a, k in [((h, w, ids, t, 0.0), {}), ((h, w, ids[:5], t[:5], 1.0), {}), ((h, w, ids, t[:, :3], 1.0), {}),
+                 ((h, w, wide.long(), wide, 1.0), {}), ((h, w, ids, t, 1.0, rw[:5]), {}), ((h[:, :32], w, ids, t, 1.0), {}),
+                 ((h[0], w, ids, t, 1.0), {}), ((h, w, ids.cpu(), t, 1.0), {}), ((h.cpu(), w, ids, t, 1.0), {}),
+                 ((h[:, :12], w[:, :12], ids, t, 1.0), {})]:
+        with pytest.raises((ValueError, NotImplementedError)):
+            fused_distill_head(*a, **k)
+    with pytest.raises(NotImplementedError):
+        fused_distill_head(h.float(), w.float(), ids, t, 1.0)
+    with pytest.raises(NotImplementedError):
+        fused_distill_head(h, w.half(), ids, t, 1.0)
+    hr = h[:0].clone().requires_grad_(True)
+    loss, kl = fused_distill_head(hr, w, ids[:0], t[:0], 1.0)
+    loss.backward()
+    assert loss.item() == 0 and kl.shape == (0,) and hr.grad.shape == (0, 64)
