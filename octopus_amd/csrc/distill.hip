@@ -62,16 +62,35 @@ __device__ __forceinline__ void teacher_slots(const int64_t *ids, const float *t
 }
 
 template <int DT>
-__global__ __launch_bounds__(kDistThreads) void distill_columns_fwd_kernel(const void *logits, int64_t ld,
+__global__ __launch_bounds__(kDistThreads, 8) void distill_columns_fwd_kernel(const void *logits, int64_t ld,
                                                                            const int64_t *ids, const float *teacher,
                                                                            int V, int K, float inv_T, int raw,
                                                                            float *kl, float *state, float *q_out) {
   constexpr int PER = 16 / Elem<DT>::bytes, NW = kDistThreads / 64;
   typedef typename Elem<DT>::T T;
   __shared__ float red[2][NW];
+  __shared__ float slot_q[OCTO_LIST_MAX], slot_lq[OCTO_LIST_MAX], slot_z[OCTO_LIST_MAX];
   const int64_t r = blockIdx.x;
   const T *row = (const T *)logits + r * ld;
   const float c = inv_T * OCTO_LOG2E;
+  // the first wave reads the list, and its logits, ahead of the sweep
+  const int lane = threadIdx.x & 63;
+  float Q = 0.f;
+  if (threadIdx.x < 64) {
+    int64_t id[kSlots];
+    float q[kSlots], lq[kSlots];
+    teacher_slots(ids + r * K, teacher + r * K, K, V, raw != 0, lane, id, q, lq, Q);
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      const int k = lane + 64 * i;
+      if (k < K) {
+        q_out[r * K + k] = q[i];
+        slot_q[k] = q[i];
+        slot_lq[k] = lq[i];
+        slot_z[k] = id[i] >= 0 ? (float)row[id[i]] : 0.f;
+      }
+    }
+  }
   const RowChunks rc = row_chunks<DT>(row, V);
   const i32x4 *vec = (const i32x4 *)(row + rc.head);
   RowSum st;
@@ -104,18 +123,11 @@ __global__ __launch_bounds__(kDistThreads) void distill_columns_fwd_kernel(const
   float m, S;
   block_row_sum<NW>(st, c, red, m, S);
   if (threadIdx.x >= 64) return;
-  const int lane = threadIdx.x;
   const float lnS = flog2(S) * OCTO_LN2;
-  int64_t id[kSlots];
-  float q[kSlots], lq[kSlots], Q, sum = 0.f;
-  teacher_slots(ids + r * K, teacher + r * K, K, V, raw != 0, lane, id, q, lq, Q);
-#pragma unroll
-  for (int i = 0; i < kSlots; ++i) {
-    const int k = lane + 64 * i;
-    // q 0 (an exp that underflows): its term's limit, 0, whatever log p is
-    if (id[i] >= 0 && q[i] != 0.f) sum += q[i] * (lq[i] - (((float)row[id[i]] - m) * inv_T - lnS));
-    if (k < K) q_out[r * K + k] = q[i];
-  }
+  float sum = 0.f;
+  // q 0 (an empty slot, or an exp that underflows): its term's limit, 0, whatever log p is
+  for (int k = lane; k < K; k += 64)
+    if (slot_q[k] != 0.f) sum += slot_q[k] * (slot_lq[k] - ((slot_z[k] - m) * inv_T - lnS));
   sum = wave_sum(sum);
   if (lane == 0) {
     kl[r] = sum;
@@ -126,8 +138,9 @@ __global__ __launch_bounds__(kDistThreads) void distill_columns_fwd_kernel(const
   }
 }
 
-// One workgroup per kDistLoads x 256 chunks of a row. The slots that lie in its columns are marked by chunk in a bit
-// map; a thread with a marked chunk looks through the list.
+// One workgroup per kDistLoads x 256 chunks of a row. Its first wave picks the slots that lie in its columns, in the
+// list's order, and marks their chunks in a bit map; a thread with a marked chunk goes through the picked ones (3 of 64 on
+// average at V 151,936; each thread through the whole list, and per value, made the kernel 680 us at [2048, 151,936]).
 constexpr int kMarkWords = 256 * kDistLoads / 32;
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void distill_columns_bwd_kernel(const void *logits, int64_t ld, const int64_t *ids,
@@ -139,6 +152,7 @@ __global__ __launch_bounds__(256) void distill_columns_bwd_kernel(const void *lo
   __shared__ int slot_col[OCTO_LIST_MAX];
   __shared__ float slot_q[OCTO_LIST_MAX];
   __shared__ uint32_t marks[kMarkWords];
+  __shared__ int picked;
   const int64_t r = blockIdx.y;
   const T *row = (const T *)logits + r * ld;
   T *drow = (T *)dl + r * ld_d;
@@ -161,35 +175,44 @@ __global__ __launch_bounds__(256) void distill_columns_bwd_kernel(const void *lo
     if (edge) drow[je] = (T)0.f;
     return;
   }
-  for (int i = threadIdx.x; i < kMarkWords; i += 256) marks[i] = 0;
-  __syncthreads();
-  for (int k = threadIdx.x; k < K; k += 256) {
-    const float qk = q[r * K + k];
-    const int64_t y = ids[r * K + k];
-    const int col = qk != 0.f && y >= 0 && y < V ? (int)y : -1;
-    slot_col[k] = col;
-    slot_q[k] = qk;
-    if (col >= rc.head && col < tail) {
-      const int at = (col - rc.head) / PER - k0;
-      if (at >= 0 && at < 256 * kDistLoads) atomicOr(&marks[at >> 5], 1u << (at & 31));
-    }
-  }
-  __syncthreads();
-  // the slots of column j, in the order of the list
-  auto listed = [&](int j) {
-    float s = 0.f;
-    for (int k = 0; k < K; ++k) s += slot_col[k] == j ? slot_q[k] : 0.f;
-    return s;
-  };
-  auto dense = [&](float x) { return Q * fexp2((x - m) * c - l2S); };
   i32x4 v[kDistLoads];
   if constexpr (VEC) {
 #pragma unroll
-    for (int u = 0; u < kDistLoads; ++u) {
-      const int k = k0 + u * 256 + threadIdx.x;
-      if (k < rc.chunks) v[u] = *(const i32x4 *)(row + rc.head + k * PER);
-    }
+    for (int u = 0; u < kDistLoads; ++u)  // past the end: the last chunk again, not stored below
+      if (rc.chunks) v[u] = *(const i32x4 *)(row + rc.head + min(k0 + u * 256 + (int)threadIdx.x, rc.chunks - 1) * PER);
   }
+  if (threadIdx.x < 64) {
+    if (threadIdx.x < kMarkWords) marks[threadIdx.x] = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int c0 = rc.head + k0 * PER, c1 = min(tail, c0 + 256 * kDistLoads * PER);
+    int n = 0;
+    for (int s0 = 0; s0 < K; s0 += 64) {
+      const int k = s0 + threadIdx.x;
+      float qk = 0.f;
+      int64_t y = -1;
+      if (k < K) {
+        qk = q[r * K + k];
+        y = ids[r * K + k];
+      }
+      const bool inside = y >= c0 && y < c1;
+      const bool mine = qk != 0.f && y >= 0 && y < V &&
+                        (inside || (blockIdx.x == 0 && (y < rc.head || y >= tail)));
+      const uint64_t all = __ballot(mine);
+      if (mine) {
+        const int at = n + __popcll(all & ((1ull << threadIdx.x) - 1ull));
+        slot_col[at] = (int)y;
+        slot_q[at] = qk;
+        if (inside) {
+          const int chunk = ((int)y - c0) / PER;
+          atomicOr(&marks[chunk >> 5], 1u << (chunk & 31));
+        }
+      }
+      n += __popcll(all);
+    }
+    if (threadIdx.x == 0) picked = n;
+  }
+  __syncthreads();
+  auto dense = [&](float x) { return Q * fexp2((x - m) * c - l2S); };
 #pragma unroll
   for (int u = 0; u < kDistLoads; ++u) {
     const int at = u * 256 + threadIdx.x, k = k0 + at;
@@ -203,8 +226,12 @@ __global__ __launch_bounds__(256) void distill_columns_bwd_kernel(const void *lo
 #pragma unroll
     for (int e = 0; e < PER; ++e) x[e] = dense(x[e]);
     if (marks[at >> 5] >> (at & 31) & 1)
+      for (int s = 0; s < picked; ++s) {
+        const uint32_t o = (uint32_t)(slot_col[s] - j0);
+        if (o < (uint32_t)PER)
 #pragma unroll
-      for (int e = 0; e < PER; ++e) x[e] -= listed(j0 + e);
+          for (int e = 0; e < PER; ++e) x[e] -= (int)o == e ? slot_q[s] : 0.f;
+      }
 #pragma unroll
     for (int e = 0; e < PER; ++e) x[e] *= gs;
     if constexpr (VEC) *(i32x4 *)(drow + j0) = pack_chunk<DT>(x);
@@ -212,7 +239,11 @@ __global__ __launch_bounds__(256) void distill_columns_bwd_kernel(const void *lo
 #pragma unroll
       for (int e = 0; e < PER; ++e) drow[j0 + e] = (T)x[e];
   }
-  if (edge) drow[je] = (T)(gs * (dense((float)row[je]) - listed(je)));
+  if (edge) {
+    float x = dense((float)row[je]);
+    for (int s = 0; s < picked; ++s) x -= slot_col[s] == je ? slot_q[s] : 0.f;
+    drow[je] = (T)(gs * x);
+  }
 }
 
 template <int DT>
@@ -250,8 +281,46 @@ __device__ __forceinline__ float listed_x(const DistillArgs &a, float dot, int64
   return a.use_tanh ? (exact_tanh ? tanhf(a.pre * x) : ftanh(a.pre * x)) : x;
 }
 
-// One workgroup per compact row, a wave per slot in turn.
-constexpr int kDotWaves = 4;
+// One workgroup per compact row. 16-bit operands: a wave takes kDotSlots slots at a time, so that a part of the hidden row
+// is read once for all of them and their loads are in flight together; the lanes' sums are exchanged and halved together.
+// Bound by the gathered weight rows, n K d x 2 bytes out of the caches (2.7 GB at 8,192 rows, K 64, d 2560). fp8 weights:
+// a slot at a time (row_dot).
+constexpr int kDotWaves = 8, kDotSlots = 8;
+template <bool F16>
+__device__ __forceinline__ float dot_slots(const char *h, const char *const (&w)[kDotSlots], int chunks, int lane) {
+  float s[kDotSlots] = {};
+#pragma unroll 2
+  for (int k = lane; k < chunks; k += 64) {
+    i32x4 wv[kDotSlots];
+    const i32x4 hv = *(const i32x4 *)(h + k * 16);
+#pragma unroll
+    for (int j = 0; j < kDotSlots; ++j) wv[j] = *(const i32x4 *)(w[j] + k * 16);
+    float a[8], b[8];
+    unpack8(hv, F16, a);
+#pragma unroll
+    for (int j = 0; j < kDotSlots; ++j) {
+      unpack8(wv[j], F16, b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[j] = __builtin_fmaf(a[e], b[e], s[j]);
+    }
+  }
+  // lane l ends with the sum of slot (l >> 3) & 7
+#pragma unroll
+  for (int half = kDotSlots / 2, o = 32; half >= 1; half >>= 1, o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int j = 0; j < kDotSlots / 2; ++j)
+      if (j < half) {
+        const float keep = up ? s[j + half] : s[j], give = up ? s[j] : s[j + half];
+        s[j] = keep + __shfl_xor(give, o, 64);
+      }
+  }
+  float t = s[0];
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+  return t;
+}
+
 __global__ __launch_bounds__(64 * kDotWaves) void distill_dots_kernel(DistillArgs a) {
   __shared__ float best[kDotWaves];
   if (blockIdx.x == 0)
@@ -261,15 +330,45 @@ __global__ __launch_bounds__(64 * kDotWaves) void distill_dots_kernel(DistillArg
   const int64_t cnt = a.count ? min((int64_t)(*a.count), a.n_max) : a.n_max;
   if (r >= cnt) return;
   const int64_t hrow = a.idx ? a.idx[r] : r;
+  const int64_t *ids = a.ids + hrow * a.K;
+  const float *teacher = a.teacher + hrow * a.K;
+  auto token = [&](int k) {  // -1 for an empty slot
+    if (k >= a.K) return (int64_t)-1;
+    const int64_t y = ids[k];
+    return y >= 0 && y < a.V && teacher[k] != -INFINITY ? y : (int64_t)-1;
+  };
   float top = -INFINITY;
-  for (int k = w; k < a.K; k += kDotWaves) {
-    const int64_t y = a.ids[hrow * a.K + k];
-    float dot = 0.f;
-    if (y >= 0 && y < a.V && a.teacher[hrow * a.K + k] != -INFINITY) {
-      dot = wave_sum(row_dot(a.h, a.h_dtype, hrow * a.ldh, a.w, a.w_dtype, y * a.ldw, a.d, lane));
-      top = fmaxf(top, listed_x(a, dot, y, false));
+  if (a.w_dtype == OCTO_FP8E4M3) {
+    for (int k = w; k < a.K; k += kDotWaves) {
+      const int64_t y = token(k);
+      float dot = 0.f;
+      if (y >= 0) {
+        dot = wave_sum(row_dot(a.h, a.h_dtype, hrow * a.ldh, a.w, a.w_dtype, y * a.ldw, a.d, lane));
+        top = fmaxf(top, listed_x(a, dot, y, false));
+      }
+      if (lane == 0) a.dots[r * a.K + k] = dot;
     }
-    if (lane == 0) a.dots[r * a.K + k] = dot;
+  } else {
+    for (int k0 = w * kDotSlots; k0 < a.K; k0 += kDotWaves * kDotSlots) {
+      const int64_t mine = token(k0 + (lane >> 3));  // the slot whose sum this lane ends with
+      const uint64_t used = __ballot(mine >= 0);
+      float dot = 0.f;
+      if (used) {
+        const int64_t any = __shfl(mine, __ffsll((unsigned long long)used) - 1, 64);
+        const char *rows[kDotSlots];
+#pragma unroll
+        for (int j = 0; j < kDotSlots; ++j) {  // an empty slot reads another's row
+          const int64_t y = __shfl(mine, 8 * j, 64);
+          rows[j] = (const char *)a.w + (y >= 0 ? y : any) * a.ldw * 2;
+        }
+        const char *h = (const char *)a.h + hrow * a.ldh * 2;
+        dot = a.f16 ? dot_slots<true>(h, rows, a.d / 8, lane) : dot_slots<false>(h, rows, a.d / 8, lane);
+        if (mine >= 0) top = fmaxf(top, listed_x(a, dot, mine, false));
+        else dot = 0.f;
+      }
+      if ((lane & 7) == 0 && k0 + (lane >> 3) < a.K) a.dots[r * a.K + k0 + (lane >> 3)] = dot;
+    }
+    top = wave_max(top);
   }
   if (lane == 0) best[w] = top;
   __syncthreads();

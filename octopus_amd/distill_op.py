@@ -24,9 +24,9 @@ import torch
 from torch import Tensor
 
 from . import _lib, head_op
-from .embed_op import _float_rows, _ids, _on_gpu
+from .embed_op import _float_rows, _ids, _on_gpu, _op
 from .head_op import (_DT, Post, _dtype_code, _empty, _gather_flag, _index, _later_bytes, _p, _rows2d, _stream,
-                      _workspace, _zeros, later_grad_w, scaled)
+                      _scale_add, _workspace, _zeros, later_grad_w, scaled)
 
 
 def _lists(ids: Tensor, teacher: Tensor, rows: int) -> tuple[Tensor, Tensor]:
@@ -83,10 +83,8 @@ def head_topk(logits: Tensor, temperature: float, k: int) -> tuple[Tensor, Tenso
 
 # ---- the divergence over materialised logits -----------------------------------------------------------------------------
 
-@torch.library.custom_op("octohead::distill_columns_fwd", mutates_args=(), device_types="cuda")
-def distill_columns_fwd(logits: Tensor, ids: Tensor, teacher: Tensor, inv_T: float,
-                        raw: bool) -> tuple[Tensor, Tensor, Tensor]:
-    """(kl [n], state [n, 4], q [n, K]), the last two for distill_columns_bwd."""
+def _columns_fwd(logits: Tensor, ids: Tensor, teacher: Tensor, inv_T: float,
+                 raw: bool) -> tuple[Tensor, Tensor, Tensor]:
     dev = _on_gpu(logits, ids, teacher)
     z = _float_rows(logits, "logits")
     n, V = z.shape
@@ -101,14 +99,20 @@ def distill_columns_fwd(logits: Tensor, ids: Tensor, teacher: Tensor, inv_T: flo
     return kl, state, q
 
 
+@torch.library.custom_op("octohead::distill_columns_fwd", mutates_args=(), device_types="cuda")
+def distill_columns_fwd(logits: Tensor, ids: Tensor, teacher: Tensor, inv_T: float,
+                        raw: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """(kl [n], state [n, 4], q [n, K]), the last two for distill_columns_bwd."""
+    return _columns_fwd(logits, ids, teacher, inv_T, raw)
+
+
 @distill_columns_fwd.register_fake
 def _(logits, ids, teacher, inv_T, raw):
     f = lambda *s: logits.new_empty(*s, dtype=torch.float32)  # noqa: E731
     return f(logits.shape[0]), f(logits.shape[0], 4), f(*ids.shape)
 
 
-@torch.library.custom_op("octohead::distill_columns_bwd", mutates_args=(), device_types="cuda")
-def distill_columns_bwd(logits: Tensor, ids: Tensor, q: Tensor, inv_T: float, state: Tensor, g: Tensor) -> Tensor:
+def _columns_bwd(logits: Tensor, ids: Tensor, q: Tensor, inv_T: float, state: Tensor, g: Tensor) -> Tensor:
     dev = _on_gpu(logits, ids, q, state, g)
     z = _float_rows(logits, "logits")
     n, V = z.shape
@@ -119,6 +123,11 @@ def distill_columns_bwd(logits: Tensor, ids: Tensor, q: Tensor, inv_T: float, st
         _lib.call("octo_distill_columns_bwd", _p(z), z.stride(0), _DT[z.dtype], _p(ids), _p(q), n, V, ids.shape[1],
                   inv_T, _p(state), _p(g), _p(dz), V, _stream(z))
     return dz
+
+
+@torch.library.custom_op("octohead::distill_columns_bwd", mutates_args=(), device_types="cuda")
+def distill_columns_bwd(logits: Tensor, ids: Tensor, q: Tensor, inv_T: float, state: Tensor, g: Tensor) -> Tensor:
+    return _columns_bwd(logits, ids, q, inv_T, state, g)
 
 
 @distill_columns_bwd.register_fake
@@ -134,11 +143,27 @@ def _columns_setup(ctx, inputs, output):
 
 def _columns_backward(ctx, gkl, _gstate, _gq):
     logits, ids, state, q = ctx.saved_tensors
-    dz = distill_columns_bwd(logits, ids, q, ctx.inv_T, state, gkl) if ctx.needs_input_grad[0] else None
-    return dz, None, None, None, None
+    if not ctx.needs_input_grad[0]:
+        return (None,) * 5
+    return (_op(distill_columns_bwd, _columns_bwd)(logits, ids, q, ctx.inv_T, state, gkl),) + (None,) * 4
 
 
 torch.library.register_autograd("octohead::distill_columns_fwd", _columns_backward, setup_context=_columns_setup)
+
+
+class _Columns(torch.autograd.Function):
+    """distill_columns_fwd and its backward outside a trace, without the registered ops' own bookkeeping on the host (57
+    rows of 128,257: 98 us a forward and backward through the ops)."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        output = _columns_fwd(*args)
+        _columns_setup(ctx, args, output)
+        return output[0]
+
+    @staticmethod
+    def backward(ctx, gkl):
+        return _columns_backward(ctx, gkl, None, None)
 
 
 def distill_columns(logits: Tensor, temperature: float, ids: Tensor, teacher: Tensor, *,
@@ -148,7 +173,10 @@ def distill_columns(logits: Tensor, temperature: float, ids: Tensor, teacher: Te
     log-probabilities whose missing rest is to carry no weight."""
     if logits.dim() != 2:
         raise ValueError(f"octohead: logits must be [n, V], got {tuple(logits.shape)}")
-    return distill_columns_fwd(logits, ids, teacher.detach(), _inv_T(temperature), not normalise)[0]
+    args = (logits, ids, teacher.detach(), _inv_T(temperature), not normalise)
+    if torch.compiler.is_compiling():
+        return distill_columns_fwd(*args)[0]
+    return _Columns.apply(*args) if torch.is_grad_enabled() and logits.requires_grad else _columns_fwd(*args)[0]
 
 
 # ---- the divergence from hidden rows: loss and gradients in one call ------------------------------------------------------
@@ -169,10 +197,10 @@ def _step(rows: Tensor, weight: Tensor, w_scale: Optional[Tensor], ids: Tensor, 
     n_max = idx.numel() if idx is not None else rows2.shape[0]
     V, d = weight2.shape
     K = ids.shape[1]
-    f = lambda *s: torch.empty(*s, dtype=torch.float32, device=dev)  # noqa: E731
-    kl = torch.zeros(rows2.shape[0], dtype=torch.float32, device=dev)
-    loss = torch.zeros((), dtype=torch.float32, device=dev)
-    grad_rows = _zeros(rows) if need_rows else rows.new_empty(0)
+    every = idx is None and count is None  # every row takes part: each output is written whole
+    kl = (torch.empty if every else torch.zeros)(rows2.shape[0], dtype=torch.float32, device=dev)
+    loss = (torch.empty if n_max else torch.zeros)((), dtype=torch.float32, device=dev)
+    grad_rows = (_empty(rows) if every else _zeros(rows)) if need_rows else rows.new_empty(0)
     grad_w = weight.new_empty(0) if not need_weight or kept is not None else \
         (_zeros(weight) if n_max == 0 else _empty(weight))
     if n_max == 0:
@@ -187,7 +215,8 @@ def _step(rows: Tensor, weight: Tensor, w_scale: Optional[Tensor], ids: Tensor, 
         if head_op.STEP_WORKSPACE_BYTES is not None:
             nbytes = int(head_op.STEP_WORKSPACE_BYTES)
     ws = _workspace(nbytes, rows2)
-    dots, q, g, lse = f(n_max, K), f(n_max, K), f(n_max), f(n_max, 2)
+    scratch = torch.empty((2 * K + 3) * n_max, dtype=torch.float32, device=dev)
+    dots, q, lse, g = scratch.split([K * n_max, K * n_max, 2 * n_max, n_max])
     lists = _lib.Distill(_p(ids), _p(teacher), _p(row_weight), K, _lib.LIST_RAW if raw else 0, _p(dots), _p(q), _p(g),
                          _p(kl), _p(loss))
     gh = None
@@ -231,25 +260,20 @@ def _step_setup(ctx, inputs, output):
 
 
 def _step_backward(ctx, gloss, _gkl, _ggr, _ggw):
-    out = []
-    for k in range(2):
-        if not (ctx.need[k] and ctx.needs_input_grad[k]):
-            out.append(None)
-        else:
-            out.append(torch.zeros_like(ctx.grads[k]) if gloss is None else scaled(ctx.grads[k], gloss))
+    # into tensors of their own: the op's outputs are its caller's, and a retained graph's second backward reads them
+    out = [(torch.zeros_like(t) if gloss is None else scaled(t, gloss)) if ctx.need[k] and ctx.needs_input_grad[k] else None
+           for k, t in enumerate(ctx.grads)]
     return (*out,) + (None,) * 13
 
 
 torch.library.register_autograd("octohead::head_step_distill", _step_backward, setup_context=_step_setup)
 
 
-@torch.library.custom_op("octohead::head_step_distill_later", mutates_args=(), device_types="cuda")
-def head_step_distill_later(rows: Tensor, weight: Tensor, ids: Tensor, teacher: Tensor, row_weight: Optional[Tensor],
-                            idx: Optional[Tensor], count: Optional[Tensor], inv_T: float, pre: float, post: float,
-                            use_tanh: bool, raw: bool, need_rows: bool,
-                            nbytes: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    """head_step_distill's (loss, kl, grad_rows), the buffer of nbytes that later_grad_w makes grad_weight of, and the row
-    count as the call found it."""
+def _step_later(rows: Tensor, weight: Tensor, ids: Tensor, teacher: Tensor, row_weight: Optional[Tensor],
+                idx: Optional[Tensor], count: Optional[Tensor], inv_T: float, pre: float, post: float, use_tanh: bool,
+                raw: bool, need_rows: bool, nbytes: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(loss, kl, grad_rows, the buffer of nbytes that later_grad_w makes grad_weight of, the row count as the call found
+    it)."""
     n_max = idx.numel() if idx is not None else rows.shape[0]
     kept_count = torch.full((1,), n_max, dtype=torch.int32, device=rows.device) if count is None \
         else count.reshape(-1)[:1].to(torch.int32, copy=True)
@@ -257,13 +281,6 @@ def head_step_distill_later(rows: Tensor, weight: Tensor, ids: Tensor, teacher: 
     loss, kl, grad_rows, _ = _step(rows, weight, None, ids, teacher, row_weight, idx, count, inv_T, pre, post, use_tanh,
                                    raw, need_rows, True, kept)
     return loss, kl, grad_rows, kept, kept_count
-
-
-@head_step_distill_later.register_fake
-def _(rows, weight, ids, teacher, row_weight, idx, count, inv_T, pre, post, use_tanh, raw, need_rows, nbytes):
-    return (rows.new_empty((), dtype=torch.float32), rows.new_empty(rows.shape[0], dtype=torch.float32),
-            _empty(rows) if need_rows else rows.new_empty(0), rows.new_empty(nbytes, dtype=torch.uint8),
-            rows.new_empty(1, dtype=torch.int32))
 
 
 def _later_setup(ctx, inputs, output):
@@ -274,7 +291,7 @@ def _later_setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
 
 
-def _later_backward(ctx, gloss, _gkl, _ggr, _gkept, _gcount):
+def _later_backward(ctx, gloss):
     grad_rows, kept, count = ctx.held
     n_max, d, V, dtype = ctx.sizes
     gr = gw = None
@@ -283,10 +300,42 @@ def _later_backward(ctx, gloss, _gkl, _ggr, _gkept, _gcount):
     if ctx.needs_input_grad[1]:
         gw = torch.zeros(V, d, dtype=dtype, device=kept.device) if gloss is None \
             else later_grad_w(kept, count, gloss, n_max, d, V, dtype, ctx.need_rows)
-    return (gr, gw) + (None,) * 12
+    return gr, gw
 
 
-torch.library.register_autograd("octohead::head_step_distill_later", _later_backward, setup_context=_later_setup)
+class _Head(torch.autograd.Function):
+    """The step outside a trace. It holds its gradients (or operands) for itself, so that the last backward scales them
+    where they lie, which ends at once for a loss that is not scaled; a copy reads and writes [V, d] ([151,936, 2560] bf16
+    267 us)."""
+
+    @staticmethod
+    def forward(ctx, rows, weight, w_scale, ids, teacher, row_weight, idx, count, xf, need_rows, need_weight, nbytes):
+        ctx.later = bool(nbytes)
+        if nbytes:
+            inputs = (rows, weight, ids, teacher, row_weight, idx, count, *xf, need_rows, nbytes)
+            output = _step_later(*inputs)
+            _later_setup(ctx, inputs, output)
+        else:
+            output = _step(rows, weight, w_scale, ids, teacher, row_weight, idx, count, *xf, need_rows, need_weight, None)
+            ctx.grads, ctx.need = output[2:], (need_rows, need_weight)
+            ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(output[1])
+        return output[0], output[1]
+
+    @staticmethod
+    def backward(ctx, gloss, gkl):
+        if ctx.later:
+            return _later_backward(ctx, gloss) + (None,) * 10
+        if ctx.grads is None:
+            raise RuntimeError("octohead: the gradients held by the distillation step went with its last backward; "
+                               "retain_graph=True keeps them for another")
+        if torch._C._autograd._get_current_graph_task_keep_graph() or gloss is None:
+            return _step_backward(ctx, gloss, None, None, None)[:2] + (None,) * 10
+        held, ctx.grads = ctx.grads, None
+        c = gloss.float().contiguous()
+        with torch.cuda.device(c.device):
+            return tuple(_scale_add(t, None, c, None) if ctx.need[k] and ctx.needs_input_grad[k] else None
+                         for k, t in enumerate(held)) + (None,) * 10
 
 
 def fused_distill_head(rows: Tensor, weight: Tensor, ids: Tensor, teacher: Tensor, temperature: float,
@@ -311,10 +360,11 @@ def fused_distill_head(rows: Tensor, weight: Tensor, ids: Tensor, teacher: Tenso
     row_weight = None if row_weight is None else row_weight.detach()
     xf = (inv_T, float(post.pre), float(post.post), bool(post.tanh), not normalise)
     nbytes = _later_bytes(rows, weight, idx, need_rows, need_weight)
-    if nbytes:
-        loss, kl, *_ = head_step_distill_later(rows, weight, ids, teacher, row_weight, idx, count, *xf, need_rows,
-                                               nbytes)
-    else:
-        loss, kl, *_ = head_step_distill(rows, weight, w_scale, ids, teacher, row_weight, idx, count, *xf, need_rows,
-                                         need_weight)
+    if not torch.compiler.is_compiling():
+        if need_rows or need_weight:
+            return _Head.apply(rows, weight, w_scale, ids, teacher, row_weight, idx, count, xf, need_rows, need_weight,
+                               nbytes)
+        return _step(rows, weight, w_scale, ids, teacher, row_weight, idx, count, *xf, False, False, None)[:2]
+    loss, kl, *_ = head_step_distill(rows, weight, w_scale, ids, teacher, row_weight, idx, count, *xf, need_rows,
+                                     need_weight)
     return loss, kl.detach()

@@ -74,8 +74,9 @@ def test_python_checks_need_no_gpu():
                  lambda: distill_op.head_topk(z, 1.0, 5), lambda: distill_op.distill_columns(z[0], 1.0, ids, t),
                  lambda: distill_op.distill_columns(z, -1.0, ids, t), lambda: embed_op.embed_rows(z[0], ids),
                  lambda: embed_op.embed_rows(z, ids), lambda: embed_op.embed_rows(z, ids, padding_idx=3),
+                 lambda: distill_op.distill_columns(z, 1.0, ids, t),
                  lambda: embed_op.embed_grad_add_(z[0], t, ids)]:
         with pytest.raises(ValueError):
             call()
-    with pytest.raises(NotImplementedError):  # the ops are registered for HIP tensors only
-        distill_op.distill_columns(z, 1.0, ids, t)
+    with pytest.raises(NotImplementedError):  # the registered ops know HIP tensors only
+        distill_op.distill_columns_fwd(z, ids, t, 1.0, False)
