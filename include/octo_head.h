@@ -212,9 +212,10 @@ int octo_columns_bwd(const void *logits, int64_t ld, int dtype, const int64_t *l
 /* A teacher's list (no counterpart in the reference): of each row of logits [n, ld] (BF16, F16 or F32) the k largest
  * values, by value descending, equal values by column ascending (NaN counts as the largest): ids[r, :k] their columns,
  * logp[r, :k] = log_softmax(logits[r] * inv_T) there (fp32). 1 <= k <= min(V, OCTO_LIST_MAX); rows may start at any
- * element. */
+ * element. ws: octo_topk_workspace_bytes (0 unless the rows are few), 8-byte aligned. */
+int octo_topk_workspace_bytes(int64_t n, int V, int dtype, int k, size_t *bytes);
 int octo_topk(const void *logits, int64_t ld, int dtype, int64_t n, int V, float inv_T, int k, int64_t *ids,
-              float *logp, void *stream);
+              float *logp, void *ws, size_t ws_bytes, void *stream);
 
 /* Distillation from teachers' lists (no counterpart in the reference). Row r's list holds K slots (ids[r, k],
  * teacher[r, k]): a token and the teacher's logit or log-probability of it (fp32). A slot with an id outside [0, V) or a

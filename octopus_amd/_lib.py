@@ -78,7 +78,8 @@ SIGNATURES = {
                              _f32, _i32, _p, _p, _p, _i64, _i64, _p, _i64, _i32, _p, _i32, _p, _sz, _p],
     "octo_columns_fwd": [_p, _i64, _i32, _p, _i64, _i32, _f32, _p, _p, _p],
     "octo_columns_bwd": [_p, _i64, _i32, _p, _i64, _i32, _f32, _p, _p, _p, _i64, _p],
-    "octo_topk": [_p, _i64, _i32, _i64, _i32, _f32, _i32, _p, _p, _p],
+    "octo_topk_workspace_bytes": [_i64, _i32, _i32, _i32, ctypes.POINTER(_sz)],
+    "octo_topk": [_p, _i64, _i32, _i64, _i32, _f32, _i32, _p, _p, _p, _sz, _p],
     "octo_distill_columns_fwd": [_p, _i64, _i32, _p, _p, _i64, _i32, _i32, _f32, _i32, _p, _p, _p, _p],
     "octo_distill_columns_bwd": [_p, _i64, _i32, _p, _p, _i64, _i32, _i32, _f32, _p, _p, _p, _i64, _p],
     "octo_head_step_distill": [_p, _i64, _i64, _i32, _p, _i64, _i32, _p, _p, _p, _i64, _i32, _i32, _f32, _f32, _f32,

@@ -10,6 +10,12 @@
 // and the first k ranks are the list. Where more than kCand values reach the bound, a second sweep uses the bound of the
 // whole row; a row with more than kCand even so (runs of equal values), or with a NaN or +inf, is done by a radix select
 // over the values' 32-bit keys.
+//
+// Few rows: a row is cut into slices of a workgroup each (topk_slices), whose lists and sums a second launch joins the same
+// way.
+//
+// Bound by memory, 2 bytes a value at 16 bits: [2048, 151,936] bf16 at k 64 131 us (4.8 TB/s; a 4 GiB copy moves 5.0), fp32
+// 214 (5.8).
 #include "octo_common.h"
 #include "row_values.h"
 
@@ -19,6 +25,7 @@ constexpr int kTopThreads = 512;
 constexpr int kTopLoads = 8;   // 16-byte chunks in flight per thread
 constexpr int kCand = 2048;    // values that may reach the bound
 constexpr int kHits = 1536;    // chunks that may hold them
+constexpr int kJoin = 2048;    // entries a row's join takes from its slices
 constexpr int kTighten = 256;  // chunks from which on the whole row's bound is taken before they are looked through
 
 // The order of the list as unsigned numbers: NaN above +inf, -0 equal to +0.
@@ -33,6 +40,28 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 // larger is earlier in the list
 __device__ __forceinline__ uint64_t list_entry(float x, int col) {
   return ((uint64_t)order_key(x) << 32) | (uint32_t)~col;
+}
+
+// put(u, place) for the lanes whose wanted[u] is set, places counted on in *count: one atomic a wave for all of them, where
+// one per value waited for each in turn.
+template <int N, class F> __device__ __forceinline__ void append(const bool (&wanted)[N], int *count, F put) {
+  uint64_t bal[N];
+  int all = 0;
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    bal[u] = __ballot(wanted[u]);
+    all += __popcll(bal[u]);
+  }
+  if (all == 0) return;
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  if (lane == 0) base = atomicAdd(count, all);
+  base = __builtin_amdgcn_readfirstlane(base);
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    if (wanted[u]) put(u, base + __popcll(bal[u] & ((1ull << lane) - 1ull)));
+    base += __popcll(bal[u]);
+  }
 }
 
 // f(x, column) for every value of the row that this thread takes, each value once over the workgroup; pre(chunk
@@ -65,10 +94,9 @@ __device__ __forceinline__ void sweep_row(const typename Elem<DT>::T *row, int V
   if (j < rc.head || (j >= tail && j < V)) f((float)row[j], j);
 }
 
-// The k-th largest of the threads' values to its upper 16 bits, rounded down, as a value: four bits a step, the threads
-// that reach each of 15 tests counted in cnt (4 x 15, zero at the start).
-__device__ __forceinline__ float kth_bound(float top, int k, int (*cnt)[15]) {
-  const uint32_t key = order_key(top) >> 16;
+// The k-th largest of the threads' keys, its upper 16 bits: four bits a step, the threads that reach each of 15 tests
+// counted in cnt (4 x 15, zero at the start). With N keys a thread, the k-th largest of all of them.
+template <int N> __device__ __forceinline__ uint32_t kth_key(const uint32_t (&top)[N], int k, int (*cnt)[15]) {
   const int lane = threadIdx.x & 63;
   uint32_t bound = 0;
 #pragma unroll
@@ -77,7 +105,9 @@ __device__ __forceinline__ float kth_bound(float top, int k, int (*cnt)[15]) {
     int n = 0;
 #pragma unroll
     for (int q = 0; q < 15; ++q) {
-      const int have = __popcll(__ballot(key >= (bound | ((uint32_t)(q + 1) << sh))));
+      int have = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) have += __popcll(__ballot(top[i] >> 16 >= (bound | ((uint32_t)(q + 1) << sh))));
       n = lane == q ? have : n;
     }
     if (n) atomicAdd(&cnt[s][lane], n);
@@ -86,12 +116,64 @@ __device__ __forceinline__ float kth_bound(float top, int k, int (*cnt)[15]) {
     const uint32_t step = __popcll(__ballot(lane < 15 && cnt[s][min(lane, 14)] >= k));
     bound |= step << sh;
   }
+  return bound;
+}
+// As a value. Up to kOneTop entries a thread's one maximum will do; for longer lists the maxima of its even and odd chunks
+// count each by itself, or k would be half the threads and the bound far below the k-th value (k 256 of 512 maxima: 1,640
+// chunks of a row of 151,936 collected, of 1,024 maxima 1,370).
+constexpr int kOneTop = 64;
+__device__ __forceinline__ float kth_bound(const float (&top)[2], int k, int (*cnt)[15]) {
+  uint32_t bound;
+  if (k <= kOneTop) {
+    const uint32_t one[1] = {order_key(fmaxf(top[0], top[1]))};
+    bound = kth_key(one, k, cnt);
+  } else {
+    const uint32_t two[2] = {order_key(top[0]), order_key(top[1])};
+    bound = kth_key(two, k, cnt);
+  }
   return bound <= 0x007fu ? -INFINITY : key_value(bound << 16);  // 0x007f: the key of -inf, and below
 }
 
-template <int DT>
-__global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits, int64_t ld, int V, float inv_T, int k,
-                                                           int64_t *ids, float *logp) {
+// A ranked value's place in the row's list, if it has one.
+__device__ __forceinline__ void write_value(uint64_t e, int rank, int64_t r, int k, float m, float lnS, float inv_T,
+                                            int64_t *ids, float *logp) {
+  if (rank >= k) return;
+  ids[r * k + rank] = (int)~(uint32_t)e;
+  logp[r * k + rank] = (key_value((uint32_t)(e >> 32)) - m) * inv_T - lnS;
+}
+
+// Ranks of the n collected values in cand (n <= kCand, room up to a multiple of 4): each against a share of the others,
+// four at a time, the list behind them filled up with 0, which is behind every value.
+__device__ __forceinline__ void rank_values(uint64_t *cand, int n, int *ranks) {
+  const int span = (n + 63) & ~63, groups = max(1, min(16, kTopThreads / max(span, 64))), full = (n + 3) & ~3;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kTopThreads) ranks[i] = 0;
+  if (threadIdx.x < full - n) cand[n + threadIdx.x] = 0;
+  __syncthreads();
+  const int g = groups > 1 ? (int)threadIdx.x / span : 0;
+  for (int i = (int)threadIdx.x - g * span; i < n && g < groups; i += kTopThreads) {
+    const uint64_t mine = cand[i];
+    int before = 0;
+#pragma unroll 2
+    for (int j = 4 * g; j < full; j += 4 * groups) {
+      uint64_t o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = cand[j + e];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) before += o[e] > mine ? 1 : 0;
+    }
+    if (groups > 1) atomicAdd(&ranks[i], before);
+    else ranks[i] = before;
+  }
+  __syncthreads();
+}
+
+// SLICED: workgroup (r, s) takes the values s per .. s per + per of row r, and leaves its list as entries [r][s][k] (0
+// where the slice has fewer values) and its (maximum, sum) as sums [r][s].
+template <int DT, bool SLICED>
+__global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits, int64_t ld, int V_, float inv_T, int k_,
+                                                              int64_t *ids, float *logp, int per, uint64_t *entries,
+                                                              float *sums) {
   constexpr int PER = 16 / Elem<DT>::bytes, NW = kTopThreads / 64;
   typedef typename Elem<DT>::T T;
   __shared__ float red[2][NW];
@@ -104,7 +186,8 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
   static_assert(sizeof hit >= kCand * sizeof(int), "room for the ranks");
   int *ranks = (int *)hit, *hist = (int *)hit;  // where the chunks were, once they are looked through
   const int64_t r = blockIdx.x;
-  const T *row = (const T *)logits + r * ld;
+  const int first = SLICED ? (int)blockIdx.y * per : 0, V = SLICED ? min(per, V_ - first) : V_, k = min(k_, V);
+  const T *row = (const T *)logits + r * ld + first;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const float c = inv_T * OCTO_LOG2E;
   for (int i = threadIdx.x; i < 2 * 4 * 15; i += kTopThreads) (&bits[0][0][0])[i] = 0;
@@ -112,7 +195,7 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
 
   // ---- the sweep
   RowSum st;
-  float top = -INFINITY, least = INFINITY;
+  float top[2] = {-INFINITY, -INFINITY}, least = INFINITY;
   const RowChunks rc = row_chunks<DT>(row, V);
   const i32x4 *vec = (const i32x4 *)(row + rc.head);
   const int tail = rc.head + rc.chunks * PER;
@@ -120,7 +203,7 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
   const bool edge = je < rc.head || (je >= tail && je < V);
   const float xe = edge ? (float)row[je] : -INFINITY;
   if (edge) {
-    top = xe;
+    top[0] = xe;
     st.raise(xe, c);
     st.add(xe, c);
   }
@@ -143,7 +226,8 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
         for (int e = 0; e < PER; ++e) mxs[u] = fmaxf(mxs[u], x[e]);
       mx = fmaxf(mx, mxs[u]);
     }
-    top = fmaxf(top, mx);
+#pragma unroll
+    for (int u = 0; u < kTopLoads; ++u) top[u & 1] = fmaxf(top[u & 1], mxs[u]);
     st.raise(mx, c);
 #pragma unroll
     for (int u = 0; u < kTopLoads; ++u)
@@ -158,15 +242,15 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
       __syncthreads();
       least = kth_bound(top, k, bits[0]);
     }
+    bool wanted[kTopLoads];
 #pragma unroll
-    for (int u = 0; u < kTopLoads; ++u)
-      if (k0 + u * kTopThreads < rc.chunks && mxs[u] >= least) {
-        const int at = atomicAdd(&nhit, 1);
-        if (at < kHits) {
-          hit[at] = v[u];
-          hit_at[at] = k0 + u * kTopThreads;
-        }
+    for (int u = 0; u < kTopLoads; ++u) wanted[u] = k0 + u * kTopThreads < rc.chunks && mxs[u] >= least;
+    append(wanted, &nhit, [&](int u, int at) {
+      if (at < kHits) {
+        hit[at] = v[u];
+        hit_at[at] = k0 + u * kTopThreads;
       }
+    });
   }
   float m, S;
   block_row_sum<NW>(st, c, red, m, S);
@@ -183,11 +267,16 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
   if (listed && n > kTighten) least = kth_bound(top, k, bits[1]);  // of the whole row
   if (listed && n <= kHits) {
     if (edge) take(xe, je);
-    for (int i = threadIdx.x; i < n; i += kTopThreads) {
+    for (int i0 = 0; i0 < n; i0 += kTopThreads) {  // whole waves: append counts over them
+      const int i = i0 + threadIdx.x, at0 = i < n ? hit_at[i] : 0;
       float x[PER];
-      unpack_chunk<DT>(hit[i], x);
+      bool wanted[PER];
+      unpack_chunk<DT>(i < n ? hit[i] : i32x4{0, 0, 0, 0}, x);
 #pragma unroll
-      for (int e = 0; e < PER; ++e) take(x[e], rc.head + hit_at[i] * PER + e);
+      for (int e = 0; e < PER; ++e) wanted[e] = i < n && x[e] >= least;
+      append(wanted, &ncand, [&](int e, int at) {
+        if (at < kCand) cand[at] = list_entry(x[e], rc.head + at0 * PER + e);
+      });
     }
   } else if (listed) {
     sweep_row<DT>(row, V, [&](float mx) { return mx >= least; }, take);
@@ -246,37 +335,83 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
     n = k;
   }
 
-  // ---- ranks: each value against a share of the others, four at a time; the list behind them filled up with 0, which is
-  // behind every value
-  const int span = (n + 63) & ~63, groups = max(1, min(16, kTopThreads / span)), full = (n + 3) & ~3;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kTopThreads) ranks[i] = 0;
-  if (threadIdx.x < full - n) cand[n + threadIdx.x] = 0;
-  __syncthreads();
-  const int g = groups > 1 ? (int)threadIdx.x / span : 0;
-  for (int i = (int)threadIdx.x - g * span; i < n && g < groups; i += kTopThreads) {
-    const uint64_t mine = cand[i];
-    int before = 0;
-#pragma unroll 2
-    for (int j = 4 * g; j < full; j += 4 * groups) {
-      uint64_t o[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = cand[j + e];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) before += o[e] > mine ? 1 : 0;
+  rank_values(cand, n, ranks);
+  if constexpr (SLICED) {
+    const int64_t slice = r * gridDim.y + blockIdx.y;
+    for (int i = threadIdx.x; i < n; i += kTopThreads)
+      if (ranks[i] < k) entries[slice * k_ + ranks[i]] = cand[i] - (uint32_t)first;  // ~(column + first)
+    for (int i = k + threadIdx.x; i < k_; i += kTopThreads) entries[slice * k_ + i] = 0;
+    if (threadIdx.x == 0) {
+      sums[2 * slice] = m;
+      sums[2 * slice + 1] = S;
     }
-    if (groups > 1) atomicAdd(&ranks[i], before);
-    else ranks[i] = before;
+  } else {
+    for (int i = threadIdx.x; i < n; i += kTopThreads) write_value(cand[i], ranks[i], r, k, m, lnS, inv_T, ids, logp);
   }
+}
+
+// A row's list from its slices': n = slices x k entries, at least k of them values.
+__global__ __launch_bounds__(kTopThreads) void topk_join_kernel(const uint64_t *entries, const float *sums, int slices,
+                                                                int k, float inv_T, int64_t *ids, float *logp) {
+  __shared__ __attribute__((aligned(16))) uint64_t cand[kCand];
+  __shared__ int ranks[kCand];
+  __shared__ int bits[4][15];
+  __shared__ int ncand;
+  const int64_t r = blockIdx.x;
+  const int n = slices * k;  // at most kJoin
+  const uint64_t *e = entries + r * n;
+  for (int i = threadIdx.x; i < 4 * 15; i += kTopThreads) (&bits[0][0])[i] = 0;
+  if (threadIdx.x == 0) ncand = 0;
+  constexpr int PER = kJoin / kTopThreads;
+  uint64_t mine[PER], top = 0;
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int i = u * kTopThreads + threadIdx.x;
+    mine[u] = i < n ? e[i] : 0;
+    top = max(top, mine[u]);
+  }
+  RowSum st;
+  const float c = inv_T * OCTO_LOG2E;
+  for (int s = 0; s < slices; ++s) st.raise(sums[(r * slices + s) * 2], c);
+  for (int s = 0; s < slices; ++s) {  // a slice of -inf alone adds its sum, 0 or NaN
+    const float m = sums[(r * slices + s) * 2], S = sums[(r * slices + s) * 2 + 1];
+    st.S += m == -INFINITY ? S : S * fexp2((m - st.m) * c);
+  }
+  const float lnS = flog2(st.S) * OCTO_LN2;
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kTopThreads) {
-    const int at = ranks[i];
-    if (at < k) {
-      const uint64_t e = cand[i];
-      ids[r * k + at] = (int)~(uint32_t)e;
-      logp[r * k + at] = (key_value((uint32_t)(e >> 32)) - m) * inv_T - lnS;
-    }
-  }
+  // two of a slice's entries may lie with one thread: the bound is that of the threads' largest, as the sweep's
+  const uint32_t largest[1] = {(uint32_t)(top >> 32)}, bound = kth_key(largest, k, bits);
+#pragma unroll
+  for (int u = 0; u < PER; ++u)
+    if (mine[u] && (uint32_t)(mine[u] >> 48) >= bound) cand[atomicAdd(&ncand, 1)] = mine[u];
+  __syncthreads();
+  const int got = ncand;
+  rank_values(cand, got, ranks);
+  for (int i = threadIdx.x; i < got; i += kTopThreads) write_value(cand[i], ranks[i], r, k, st.m, lnS, inv_T, ids, logp);
+}
+
+// Slices a row of V values is cut into for n rows: rows of 192 KB and more, up to 128 of them, four slices at least. us a
+// call in a captured graph, V 151,936, k 64, whole and sliced: 1 row of bf16 20.6 and 15.2, 64 rows 21.1 and 16.7, 1 row of
+// fp32 24.4 and 14.8. Launched one by one the second launch costs its gain in host time: 1 row of bf16 20.2 and 19.5, 128
+// rows 22.3 and 21.7; below, a loss: 256 rows 25.2 and 28.2, V 32,000 14.2 and 18.6, k 256 28 and 50.
+constexpr int kMaxSlices = 16, kSliceK = 128;
+static int topk_slices(int64_t n, int V, int k, int dtype) {
+  if (n < 1 || n > 128 || k > kSliceK || (int64_t)V * float_bytes(dtype) < 192 * 1024) return 1;
+  const int s = (int)(512 / n);
+  return s < kMaxSlices ? s : kMaxSlices;
+}
+static_assert(kMaxSlices * kSliceK <= kJoin, "the join's entries");
+
+template <bool SLICED>
+static void go_topk(const void *logits, int64_t ld, int dtype, int64_t n, int V, float inv_T, int k, int64_t *ids,
+                    float *logp, int slices, int per, uint64_t *entries, float *sums, hipStream_t st) {
+  const dim3 g((unsigned)n, (unsigned)slices), b(kTopThreads);
+  if (dtype == OCTO_BF16)
+    hipLaunchKernelGGL((topk_kernel<OCTO_BF16, SLICED>), g, b, 0, st, logits, ld, V, inv_T, k, ids, logp, per, entries, sums);
+  else if (dtype == OCTO_F16)
+    hipLaunchKernelGGL((topk_kernel<OCTO_F16, SLICED>), g, b, 0, st, logits, ld, V, inv_T, k, ids, logp, per, entries, sums);
+  else
+    hipLaunchKernelGGL((topk_kernel<OCTO_F32, SLICED>), g, b, 0, st, logits, ld, V, inv_T, k, ids, logp, per, entries, sums);
 }
 
 }  // namespace octo
@@ -285,21 +420,42 @@ using namespace octo;
 
 extern "C" {
 
-int octo_topk(const void *logits, int64_t ld, int dtype, int64_t n, int V, float inv_T, int k, int64_t *ids,
-              float *logp, void *stream) {
-  OCTO_CHECK_ARG(n >= 0 && n <= 0x7fffffff && V > 0 && ld >= V, "topk: bad shape n=%lld V=%d ld=%lld", (long long)n, V,
-                 (long long)ld);
-  OCTO_CHECK_ARG(is_float(dtype), "topk: dtype %d", dtype);
-  OCTO_CHECK_ARG(inv_T > 0.f, "topk: temperature must be positive");
+int octo_topk_workspace_bytes(int64_t n, int V, int dtype, int k, size_t *bytes) {
+  OCTO_CHECK_ARG(bytes != nullptr, "topk_workspace_bytes: null pointer");
+  OCTO_CHECK_ARG(n >= 0 && n <= 0x7fffffff && V > 0, "topk: bad shape n=%lld V=%d", (long long)n, V);
   OCTO_CHECK_ARG(k >= 1 && k <= V && k <= OCTO_LIST_MAX, "topk: k=%d outside [1, min(V, %d)]", k, OCTO_LIST_MAX);
+  OCTO_CHECK_ARG(is_float(dtype), "topk: dtype %d", dtype);
+  const int slices = topk_slices(n, V, k, dtype);
+  *bytes = slices > 1 ? (size_t)n * slices * (k * 8 + 8) : 0;
+  return OCTO_OK;
+}
+
+int octo_topk(const void *logits, int64_t ld, int dtype, int64_t n, int V, float inv_T, int k, int64_t *ids,
+              float *logp, void *ws, size_t ws_bytes, void *stream) {
+  size_t need = 0;
+  const int rc = octo_topk_workspace_bytes(n, V, dtype, k, &need);
+  if (rc) return rc;
+  OCTO_CHECK_ARG(ld >= V, "topk: row stride %lld below V=%d", (long long)ld, V);
+  OCTO_CHECK_ARG(inv_T > 0.f, "topk: temperature must be positive");
   if (n == 0) return OCTO_OK;
   OCTO_CHECK_ARG(logits && ids && logp, "topk: null pointer");
   OCTO_CHECK_ARG((uintptr_t)logits % float_bytes(dtype) == 0, "topk: misaligned logits");
+  if (need && (!ws || ws_bytes < need))
+    return octo_fail(OCTO_EWORKSPACE, "topk: workspace %zu < %zu bytes", ws ? ws_bytes : (size_t)0, need);
+  OCTO_CHECK_ARG((uintptr_t)ws % 8 == 0, "topk: misaligned workspace");
   hipStream_t st = (hipStream_t)stream;
-  const dim3 g((unsigned)n), b(kTopThreads);
-  if (dtype == OCTO_BF16) hipLaunchKernelGGL(topk_kernel<OCTO_BF16>, g, b, 0, st, logits, ld, V, inv_T, k, ids, logp);
-  else if (dtype == OCTO_F16) hipLaunchKernelGGL(topk_kernel<OCTO_F16>, g, b, 0, st, logits, ld, V, inv_T, k, ids, logp);
-  else hipLaunchKernelGGL(topk_kernel<OCTO_F32>, g, b, 0, st, logits, ld, V, inv_T, k, ids, logp);
+  const int slices = topk_slices(n, V, k, dtype);
+  if (slices == 1) {
+    go_topk<false>(logits, ld, dtype, n, V, inv_T, k, ids, logp, 1, 0, nullptr, nullptr, st);
+  } else {
+    const int per = (int)round_up(cdiv(V, slices), 64);  // the last slice has the rest, at least one value
+    uint64_t *entries = (uint64_t *)ws;
+    float *sums = (float *)(entries + n * slices * k);
+    go_topk<true>(logits, ld, dtype, n, V, inv_T, k, ids, logp, slices, per, entries, sums, st);
+    OCTO_CHECK_LAUNCH("topk");
+    hipLaunchKernelGGL(topk_join_kernel, dim3((unsigned)n), dim3(kTopThreads), 0, st, entries, sums, slices, k, inv_T, ids,
+                       logp);
+  }
   OCTO_CHECK_LAUNCH("topk");
   return OCTO_OK;
 }

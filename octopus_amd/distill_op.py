@@ -52,8 +52,12 @@ def _topk(logits: Tensor, inv_T: float, k: int) -> tuple[Tensor, Tensor]:
     n, V = z.shape
     ids = torch.empty(n, k, dtype=torch.int64, device=dev)
     logp = torch.empty(n, k, dtype=torch.float32, device=dev)
+    nbytes = ctypes.c_size_t(0)
+    _lib.call("octo_topk_workspace_bytes", n, V, _DT[z.dtype], k, ctypes.byref(nbytes))
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev) if nbytes.value else None
     with torch.cuda.device(dev):
-        _lib.call("octo_topk", _p(z), z.stride(0), _DT[z.dtype], n, V, inv_T, k, _p(ids), _p(logp), _stream(z))
+        _lib.call("octo_topk", _p(z), z.stride(0), _DT[z.dtype], n, V, inv_T, k, _p(ids), _p(logp), _p(ws), nbytes.value,
+                  _stream(z))
     return ids, logp
 
 

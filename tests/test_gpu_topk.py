@@ -39,11 +39,12 @@ def test_sizes(dtype, n, V, k):
     _check((torch.randn(n, V, generator=g) * 3).to(dtype), 1.0 if V % 2 else 0.7, k)
 
 
+@pytest.mark.parametrize("V", [20000, 100003])
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_ties_and_orders(dtype):
+def test_ties_and_orders(dtype, V):
     """Constant rows, few distinct values, ascending and descending rows, every large value in one thread's chunk, the
     same value at the list's end: rows that pass the candidates' room and rows that do not."""
-    V, k = 20000, 64
+    k = 64
     g = torch.Generator().manual_seed(3)
     rows = [torch.zeros(V), torch.full((V,), -2.5), torch.randint(0, 3, (V,), generator=g).float(),
             torch.linspace(-8, 8, V), torch.linspace(8, -8, V), torch.randn(V, generator=g)]
@@ -56,10 +57,11 @@ def test_ties_and_orders(dtype):
     _check(torch.stack(rows + [tied, signed, few]).to(dtype), 1.0, k)
 
 
+@pytest.mark.parametrize("V", [5000, 100003])
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_masked_values(dtype):
+def test_masked_values(dtype, V):
     """Rows masked with -inf, with the type's lowest value, altogether so; NaN and +inf."""
-    V, k = 5000, 30
+    k = 30
     g = torch.Generator().manual_seed(4)
     z = torch.randn(9, V, generator=g).to(dtype)
     low = torch.finfo(dtype).min
@@ -89,6 +91,24 @@ def test_strided_rows(dtype):
 
     _check(z, 1.0, 40, odd)
     _check(z, 1.0, 40, lambda x: x.T.contiguous().cuda().T)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_and_many_rows(dtype):
+    """Few rows are cut into slices, many are not: the same tokens, log-probabilities within twice the tolerance."""
+    from octopus_amd.distill_op import head_topk
+
+    z = (torch.randn(140, 100001, generator=torch.Generator().manual_seed(6)) * 2).to(dtype).cuda()
+    z[5, 17:] = -math.inf
+    z[6] = 0.25
+    ids, logp = head_topk(z, 0.7, 100)
+    for n in (1, 3, 40, 128):
+        for r in (0, 5, 140 - n):
+            few_ids, few = head_topk(z[r:r + n], 0.7, 100)
+            assert torch.equal(few_ids, ids[r:r + n])
+            fin = few.isfinite()
+            assert torch.equal(fin, logp[r:r + n].isfinite())
+            assert (few - logp[r:r + n])[fin].abs().max() <= 4e-5
 
 
 def test_other_stream_and_graph():

@@ -15,12 +15,24 @@ def _refused(name, *args, exc=ValueError):
 
 
 def test_topk_checks():
-    ok = dict(z=P, ld=100, dt=_lib.BF16, n=4, V=100, inv_T=1.0, k=5, ids=P, logp=P)
+    ok = dict(z=P, ld=100, dt=_lib.BF16, n=4, V=100, inv_T=1.0, k=5, ids=P, logp=P, ws=None, nws=0)
     for change in [dict(ld=99), dict(V=0), dict(n=-1), dict(n=1 << 31), dict(dt=_lib.FP8E4M3), dict(inv_T=0.0),
                    dict(inv_T=float("nan")), dict(k=0), dict(k=101), dict(V=1000, ld=1000, k=257), dict(z=None),
                    dict(ids=None), dict(logp=None), dict(z=ctypes.c_void_p(4097))]:
         _refused("octo_topk", *{**ok, **change}.values(), None)
     _lib.call("octo_topk", *{**ok, "n": 0}.values(), None)
+    out = ctypes.c_size_t(0)
+    _lib.call("octo_topk_workspace_bytes", 2048, 151936, _lib.BF16, 64, ctypes.byref(out))
+    assert out.value == 0
+    _lib.call("octo_topk_workspace_bytes", 3, 151936, _lib.BF16, 64, ctypes.byref(out))
+    assert out.value > 0
+    few = {**ok, "n": 3, "V": 151936, "ld": 151936, "k": 64}
+    for change in [dict(), dict(ws=P, nws=out.value - 1), dict(ws=ctypes.c_void_p(4100), nws=out.value)]:
+        _refused("octo_topk", *{**few, **change}.values(), None)
+    for n, V, k in [(-1, 100, 5), (4, 0, 5), (4, 100, 0), (4, 100, 101), (4, 1000, 257)]:
+        _refused("octo_topk_workspace_bytes", n, V, _lib.F32, k, ctypes.byref(out))
+    _refused("octo_topk_workspace_bytes", 4, 100, _lib.F16, 5, None)
+    _refused("octo_topk_workspace_bytes", 4, 100, _lib.FP8E4M3, 5, ctypes.byref(out))
 
 
 def test_distill_columns_checks():
