@@ -233,8 +233,8 @@ int octo_distill_columns_bwd(const void *logits, int64_t ld, int dtype, const in
                              int64_t ld_d, void *stream);
 
 /* The same from hidden rows and the vocabulary weight, without the logits: octo_head_step_grpo's forward and backward in
- * one call (16-bit or fp8 weights; fp32 operands: OCTO_EUNSUPPORTED), for loss = sum over the compact rows of weight x
- * kl. Lists and weights are per hidden row (compact row r's at idx[r], or r): ids, teacher [h_rows, K], weight [h_rows]
+ * one call (fp32 operands run the forward, then octo_head_bwd's recompute), for loss = sum over the compact rows of weight
+ * x kl. Lists and weights are per hidden row (compact row r's at idx[r], or r): ids, teacher [h_rows, K], weight [h_rows]
  * (NULL: 1). kl [h_rows] is written at the compact rows' hidden rows, loss [1]. dots, q [n_max, K] and g [n_max] are
  * scratch, as lse [n_max, 2]. grad_h (compact rows) and grad_w as octo_head_step_grpo's; workspace likewise
  * (OCTO_WS_STEP). kept != NULL: no grad_w, whose operands stay in kept for octo_head_later_grad_w, as

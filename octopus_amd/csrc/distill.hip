@@ -281,27 +281,28 @@ __device__ __forceinline__ float listed_x(const DistillArgs &a, float dot, int64
   return a.use_tanh ? (exact_tanh ? tanhf(a.pre * x) : ftanh(a.pre * x)) : x;
 }
 
-// One workgroup per compact row. 16-bit operands: a wave takes kDotSlots slots at a time, so that a part of the hidden row
-// is read once for all of them and their loads are in flight together; the lanes' sums are exchanged and halved together.
-// Bound by the gathered weight rows, n K d x 2 bytes out of the caches (2.7 GB at 8,192 rows, K 64, d 2560). fp8 weights:
-// a slot at a time (row_dot).
-constexpr int kDotWaves = 8, kDotSlots = 8;
-template <bool F16>
-__device__ __forceinline__ float dot_slots(const char *h, const char *const (&w)[kDotSlots], int chunks, int lane) {
+// One workgroup per compact row. A wave takes kDotSlots slots at a time, so that a part of the hidden row is read once for
+// all of them and their loads are in flight together; the lanes' sums are exchanged and halved together. fp8 weights are
+// read from their widened copy. Bound by the gathered weight rows, n K d x 2 bytes out of the caches: 8,192 rows, K 64, d
+// 2560 (2.7 GB) 365 us, 7.4 TB/s (8 waves a row 413; a slot at a time 504).
+constexpr int kDotWaves = 4, kDotSlots = 8;
+template <int DT>
+__device__ __forceinline__ float dot_slots(const char *h, const char *const (&w)[kDotSlots], int d, int lane) {
+  constexpr int PER = 16 / Elem<DT>::bytes;
   float s[kDotSlots] = {};
-#pragma unroll 2
-  for (int k = lane; k < chunks; k += 64) {
+#pragma unroll 1
+  for (int k = lane; k < d / PER; k += 64) {
     i32x4 wv[kDotSlots];
     const i32x4 hv = *(const i32x4 *)(h + k * 16);
 #pragma unroll
     for (int j = 0; j < kDotSlots; ++j) wv[j] = *(const i32x4 *)(w[j] + k * 16);
-    float a[8], b[8];
-    unpack8(hv, F16, a);
+    float a[PER], b[PER];
+    unpack_chunk<DT>(hv, a);
 #pragma unroll
     for (int j = 0; j < kDotSlots; ++j) {
-      unpack8(wv[j], F16, b);
+      unpack_chunk<DT>(wv[j], b);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[j] = __builtin_fmaf(a[e], b[e], s[j]);
+      for (int e = 0; e < PER; ++e) s[j] = __builtin_fmaf(a[e], b[e], s[j]);
     }
   }
   // lane l ends with the sum of slot (l >> 3) & 7
@@ -321,12 +322,13 @@ __device__ __forceinline__ float dot_slots(const char *h, const char *const (&w)
   return t;
 }
 
+template <int DT>
 __global__ __launch_bounds__(64 * kDotWaves) void distill_dots_kernel(DistillArgs a) {
   __shared__ float best[kDotWaves];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
   if (blockIdx.x == 0)
-    for (int k = threadIdx.x; k < a.nflag; k += 64 * kDotWaves) a.flag_cnt[k] = 0;
+    for (int k = threadIdx.x; k < a.nflag; k += 64 * waves) a.flag_cnt[k] = 0;
   const int64_t r = blockIdx.x;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t cnt = a.count ? min((int64_t)(*a.count), a.n_max) : a.n_max;
   if (r >= cnt) return;
   const int64_t hrow = a.idx ? a.idx[r] : r;
@@ -338,43 +340,29 @@ __global__ __launch_bounds__(64 * kDotWaves) void distill_dots_kernel(DistillArg
     return y >= 0 && y < a.V && teacher[k] != -INFINITY ? y : (int64_t)-1;
   };
   float top = -INFINITY;
-  if (a.w_dtype == OCTO_FP8E4M3) {
-    for (int k = w; k < a.K; k += kDotWaves) {
-      const int64_t y = token(k);
-      float dot = 0.f;
-      if (y >= 0) {
-        dot = wave_sum(row_dot(a.h, a.h_dtype, hrow * a.ldh, a.w, a.w_dtype, y * a.ldw, a.d, lane));
-        top = fmaxf(top, listed_x(a, dot, y, false));
-      }
-      if (lane == 0) a.dots[r * a.K + k] = dot;
-    }
-  } else {
-    for (int k0 = w * kDotSlots; k0 < a.K; k0 += kDotWaves * kDotSlots) {
-      const int64_t mine = token(k0 + (lane >> 3));  // the slot whose sum this lane ends with
-      const uint64_t used = __ballot(mine >= 0);
-      float dot = 0.f;
-      if (used) {
-        const int64_t any = __shfl(mine, __ffsll((unsigned long long)used) - 1, 64);
-        const char *rows[kDotSlots];
+  for (int k0 = w * kDotSlots; k0 < a.K; k0 += waves * kDotSlots) {
+    const int64_t mine = token(k0 + (lane >> 3));  // the slot whose sum this lane ends with
+    const uint64_t used = __ballot(mine >= 0);
+    float dot = 0.f;
+    if (used) {
+      const int64_t any = __shfl(mine, __ffsll((unsigned long long)used) - 1, 64);
+      const char *rows[kDotSlots];
 #pragma unroll
-        for (int j = 0; j < kDotSlots; ++j) {  // an empty slot reads another's row
-          const int64_t y = __shfl(mine, 8 * j, 64);
-          rows[j] = (const char *)a.w + (y >= 0 ? y : any) * a.ldw * 2;
-        }
-        const char *h = (const char *)a.h + hrow * a.ldh * 2;
-        dot = a.f16 ? dot_slots<true>(h, rows, a.d / 8, lane) : dot_slots<false>(h, rows, a.d / 8, lane);
-        if (mine >= 0) top = fmaxf(top, listed_x(a, dot, mine, false));
-        else dot = 0.f;
+      for (int j = 0; j < kDotSlots; ++j) {  // an empty slot reads another's row
+        const int64_t y = __shfl(mine, 8 * j, 64);
+        rows[j] = (const char *)a.wm + (y >= 0 ? y : any) * a.ldm * Elem<DT>::bytes;
       }
-      if ((lane & 7) == 0 && k0 + (lane >> 3) < a.K) a.dots[r * a.K + k0 + (lane >> 3)] = dot;
+      dot = dot_slots<DT>((const char *)a.h + hrow * a.ldh * Elem<DT>::bytes, rows, a.d, lane);
+      if (mine >= 0) top = fmaxf(top, listed_x(a, dot, mine, false));
+      else dot = 0.f;
     }
-    top = wave_max(top);
+    if ((lane & 7) == 0 && k0 + (lane >> 3) < a.K) a.dots[r * a.K + k0 + (lane >> 3)] = dot;
   }
+  top = wave_max(top);
   if (lane == 0) best[w] = top;
   __syncthreads();
-  if (threadIdx.x == 0) {
-#pragma unroll
-    for (int k = 0; k < kDotWaves; ++k) top = fmaxf(top, best[k]);
+  if (threadIdx.x == 0 && a.xoff) {
+    for (int k = 0; k < waves; ++k) top = fmaxf(top, best[k]);
     a.xoff[r] = top == -INFINITY ? -INFINITY : __builtin_fmaf(top, a.c, kExAbove);
   }
 }
@@ -448,7 +436,8 @@ __global__ __launch_bounds__(64 * kEntryRows) void distill_entries_kernel(Distil
     for (int k = lane; k < a.K; k += 64) {
       const float q = a.q[r * a.K + k];
       slot_q[w][k] = q;
-      slot_id[w][k] = q != 0.f ? a.ids[hrow * a.K + k] : -1;  // empty slots have q 0
+      const int64_t y = a.ids[hrow * a.K + k] - a.v0;
+      slot_id[w][k] = q != 0.f && y >= 0 && y < a.cols ? y : -1;  // an empty slot has q 0
       Q += q;
     }
     Q = wave_sum(Q);
@@ -459,17 +448,16 @@ __global__ __launch_bounds__(64 * kEntryRows) void distill_entries_kernel(Distil
   if (g == 0.f) return;
   const float m2 = a.lse[2 * r], l2S = a.lse[2 * r + 1];
   for (int k = lane; k < a.K; k += 64) {
-    const int64_t y = slot_id[w][k];
-    if (y < 0) continue;
+    const int64_t col = slot_id[w][k], y = col + a.v0;
+    if (col < 0) continue;
     float share = 0.f;
-    for (int j = 0; j < a.K; ++j) share += slot_id[w][j] == y ? slot_q[w][j] : 0.f;
+    for (int j = 0; j < a.K; ++j) share += slot_id[w][j] == col ? slot_q[w][j] : 0.f;
     const float x = listed_x(a, a.dots[r * a.K + k], y, false);
     float v = share / Q - fexp2(__builtin_fmaf(x, a.c, -m2) - l2S);
     if (a.use_tanh) v *= 1.f - x * x;
     if (a.w_dtype == OCTO_FP8E4M3) v *= a.wscale[y];
-    if (a.rowoff) ((__bf16 *)a.dz)[i * a.ldx + y] = (__bf16)(-v * fexp2(m2 - a.xuse[i] + l2S));
-    else if (a.f16) ((_Float16 *)a.dz)[i * a.ldx + y] = (_Float16)(g * a.gmul * v);
-    else ((__bf16 *)a.dz)[i * a.ldx + y] = (__bf16)(g * a.gmul * v);
+    if (a.rowoff) ((__bf16 *)a.dz)[i * a.ldx + col] = (__bf16)(-v * fexp2(m2 - a.xuse[i] + l2S));
+    else store_from_f32(a.dz, a.dt, i * a.ldx + col, g * a.gmul * v);
   }
 }
 
@@ -494,7 +482,11 @@ __global__ __launch_bounds__(1024) void distill_loss_kernel(DistillArgs a, float
 
 int launch_distill_dots(const DistillArgs &a, hipStream_t st) {
   if (a.n_max == 0) return OCTO_OK;
-  hipLaunchKernelGGL(distill_dots_kernel, dim3((unsigned)a.n_max), dim3(64 * kDotWaves), 0, st, a);
+  const int waves = (int)cdiv(a.K, kDotSlots);  // no more than have slots: 4,000 rows of K 20, 149 us with 8 each, 95 with 3
+  const dim3 g((unsigned)a.n_max), b(64 * (waves < kDotWaves ? waves : kDotWaves));
+  if (a.dt == OCTO_BF16) hipLaunchKernelGGL(distill_dots_kernel<OCTO_BF16>, g, b, 0, st, a);
+  else if (a.dt == OCTO_F16) hipLaunchKernelGGL(distill_dots_kernel<OCTO_F16>, g, b, 0, st, a);
+  else hipLaunchKernelGGL(distill_dots_kernel<OCTO_F32>, g, b, 0, st, a);
   OCTO_CHECK_LAUNCH("distill_dots");
   return OCTO_OK;
 }

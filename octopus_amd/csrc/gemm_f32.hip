@@ -415,7 +415,7 @@ XKERNEL gemm_dz_x_kernel(Operand A, Operand B, GemmShape s, DzArgs e) {
     float m2, l2s;
     row_state(e.lse, e.lse_pair, r, m2, l2s);
     const float gs = e.g[r] * e.gmul;
-    const int64_t y = e.labels[e.label_idx ? e.label_idx[r] : r] - ma;
+    const int64_t y = (e.labels ? e.labels[e.label_idx ? e.label_idx[r] : r] : -1) - ma;
     float *dst = (float *)e.dzA + (n0 + t) * e.ldA + m0;
 #pragma unroll
     for (int i = 0; i < AccX::NI; ++i) {

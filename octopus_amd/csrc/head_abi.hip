@@ -325,7 +325,7 @@ int head_fwd(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const void
              const float *w_scale, const int64_t *labels, const int64_t *idx, const int32_t *count, int64_t n_max,
              int d, int V, int flags, float inv_T, float pre, float post, int use_tanh, float *logp, float *ent,
              float *lse, float *out2, int64_t ld_out2, const octo_grpo_tail *gt, void *ws, size_t ws_bytes,
-             void *stream, bool timed = true, const Kept &kept = Kept()) {
+             void *stream, bool timed = true, const Kept &kept = Kept(), const DistillArgs *lists = nullptr) {
   Common cm;
   int rc = check_common(h, h_rows, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, n_max, d, V, flags, inv_T,
                         pre, post, use_tanh, cm);
@@ -378,11 +378,26 @@ int head_fwd(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const void
     if (rc) return rc;
   }
 
+  if (lists) {  // the distillation step's forward (fp32 operands)
+    DistillArgs da = *lists;
+    da.part = e.part;
+    da.mtiles = L.mtiles;
+    da.rows = n_max;
+    rc = launch_distill_dots(da, st);
+    return rc ? rc : launch_distill_merge(da, st);
+  }
   const MergeArgs m = merge_args(e.part, L.mtiles, h, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, count,
                                  n_max, d, V, flags, inv_T, pre, post, use_tanh, logp, ent, lse, out2, ld_out2, gt, z);
   return launch_merge(m, st);
 }
 
+
+// (defined with octo_head_bwd; lists: the distillation step's, of fp32 operands)
+int head_bwd(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const void *w, int64_t ldw, int w_dtype,
+             const float *w_scale, const int64_t *labels, const int64_t *idx, const int32_t *count, int64_t n_max, int d,
+             int V, int flags, float inv_T, float pre, float post, int use_tanh, const float *lse, const float *g,
+             void *grad_h, int64_t ld_gh, int gh_dtype, void *grad_w, int gw_dtype, void *ws, size_t ws_bytes,
+             void *stream, const Kept &kept = Kept(), const DistillArgs *lists = nullptr);
 
 // ---- the fused GRPO step (octo_head_step_grpo) ---------------------------------------------------------
 // Forward, GRPO weight and backward of the compact rows in one call, pass by pass (StepLayout). The logits are
@@ -437,8 +452,36 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
                    "head_step_grpo_pairs: flat_pair, out_flat or ld_out");
     if (cm.dt == OCTO_F32) return octo_fail(OCTO_EUNSUPPORTED, "head_step_grpo_pairs: fp32 operands");
   }
-  if (ds && cm.dt == OCTO_F32) return octo_fail(OCTO_EUNSUPPORTED, "head_step_distill: fp32 operands");
   if (n_max == 0 && !pm) return OCTO_OK;
+  DistillArgs da{};
+  if (ds) {
+    da.h = h;
+    da.ldh = ldh;
+    da.w_dtype = w_dtype;
+    da.wscale = w_scale;
+    da.dt = cm.dt;
+    da.wm = w;
+    da.ldm = ldw;
+    da.idx = idx;
+    da.count = count;
+    da.n_max = n_max;
+    da.d = d;
+    da.V = V;
+    da.c = cm.c;
+    da.pre = cm.pre;
+    da.gmul = cm.gmul;
+    da.use_tanh = use_tanh;
+    da.ids = labels;
+    da.teacher = ds->teacher;
+    da.weight = ds->weight;
+    da.K = ds->K;
+    da.raw = (ds->flags & OCTO_LIST_RAW) != 0;
+    da.dots = ds->dots;
+    da.q = ds->q;
+    da.g = ds->g;
+    da.kl = ds->kl;
+    da.lse = lse;
+  }
   // no gradient asked for: the forward with its GRPO tail (its own workspace size)
   if (!need_gh && !need_gw && !pm && !later && !ds)
     return head_fwd(h, h_rows, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, count, n_max, d, V, flags, inv_T,
@@ -448,8 +491,14 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
       return octo_fail(OCTO_EWORKSPACE, "head_step_grpo: workspace %zu < %zu bytes", ws ? ws_bytes : (size_t)0,
                        step_fallback_bytes(n_max, d, V, w_dtype, need_gw, cm.gather));
     rc = head_fwd(h, h_rows, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, count, n_max, d, V, flags, inv_T,
-                  pre, post, use_tanh, logp, ent, lse, out2, ld_out2, gt, ws, ws_bytes, stream);
+                  pre, post, use_tanh, logp, ent, lse, out2, ld_out2, gt, ws, ws_bytes, stream, true, Kept(),
+                  ds ? &da : nullptr);
+    if (!rc && ds) rc = launch_distill_loss(da, ds->loss, (hipStream_t)stream);
     if (rc || (!need_gh && !need_gw)) return rc;
+    if (ds)
+      return head_bwd(h, h_rows, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, count, n_max, d, V, flags, inv_T,
+                      pre, post, use_tanh, lse, ds->g, grad_h, ld_gh, gh_dtype, grad_w, gw_dtype, ws, ws_bytes, stream,
+                      Kept(), &da);
     return octo_head_bwd(h, h_rows, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, count, n_max, d, V, flags,
                          inv_T, pre, post, use_tanh, lse, gt->g, grad_h, ld_gh, gh_dtype, grad_w, gw_dtype, ws,
                          ws_bytes, stream);
@@ -527,45 +576,20 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
   float *xoff = (float *)(wsb + L.xoff), *tdot = (float *)(wsb + L.tdot);
   float *xuse = (float *)(wsb + L.xuse), *rscale = (float *)(wsb + L.scale);
   int32_t *flag_cnt = (int32_t *)(wsb + L.flags), *flag_rows = flag_cnt + L.passes;
-  DistillArgs da{};
   if (ds) {
-    da.h = h;
-    da.ldh = ldh;
-    da.h_dtype = h_dtype;
-    da.w = w;
-    da.ldw = ldw;
-    da.w_dtype = w_dtype;
-    da.wscale = w_scale;
-    da.idx = idx;
-    da.count = count;
-    da.n_max = n_max;
-    da.d = d;
-    da.V = V;
-    da.c = cm.c;
-    da.pre = cm.pre;
-    da.gmul = cm.gmul;
-    da.use_tanh = use_tanh;
-    da.ids = labels;
-    da.teacher = ds->teacher;
-    da.weight = ds->weight;
-    da.K = ds->K;
-    da.raw = (ds->flags & OCTO_LIST_RAW) != 0;
-    da.dots = ds->dots;
-    da.q = ds->q;
-    da.g = ds->g;
-    da.kl = ds->kl;
-    da.lse = lse;
+    da.wm = Aw.base;
+    da.ldm = Aw.ld / esz;
     da.xoff = xoff;
     da.xuse = xuse;
+    da.flag_cnt = flag_cnt;
+    da.nflag = (int)L.passes;
     da.flag_rows = flag_rows;
     da.part = part;
     da.mtiles = L.mtiles;
     da.dz = dz;
     da.ldx = L.V_pad;
+    da.cols = V;
     da.rowoff = rowoff;
-    da.f16 = cm.dt == OCTO_F16;
-    da.flag_cnt = flag_cnt;
-    da.nflag = (int)L.passes;
     rc = launch_distill_dots(da, st);
     if (rc) return rc;
   } else if (rowoff) {
@@ -1043,11 +1067,15 @@ int octo_head_later_grad_w(const void *kept, const int32_t *count, int64_t n_max
   return launch_gemm_store(w_dtype, A3, B3, shape(V, d, n_max, kGroupM, 3, count, 0), o, (hipStream_t)stream, KM_A);
 }
 
-static int head_bwd(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const void *w, int64_t ldw, int w_dtype,
-                    const float *w_scale, const int64_t *labels, const int64_t *idx, const int32_t *count,
-                    int64_t n_max, int d, int V, int flags, float inv_T, float pre, float post, int use_tanh,
-                    const float *lse, const float *g, void *grad_h, int64_t ld_gh, int gh_dtype, void *grad_w,
-                    int gw_dtype, void *ws, size_t ws_bytes, void *stream, const Kept &kept = Kept()) {
+}  // extern "C"
+
+namespace {
+
+int head_bwd(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const void *w, int64_t ldw, int w_dtype,
+             const float *w_scale, const int64_t *labels, const int64_t *idx, const int32_t *count,
+             int64_t n_max, int d, int V, int flags, float inv_T, float pre, float post, int use_tanh,
+             const float *lse, const float *g, void *grad_h, int64_t ld_gh, int gh_dtype, void *grad_w,
+             int gw_dtype, void *ws, size_t ws_bytes, void *stream, const Kept &kept, const DistillArgs *lists) {
   Common cm;
   int rc = check_common(h, h_rows, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, n_max, d, V, flags, inv_T,
                         pre, post, use_tanh, cm);
@@ -1102,7 +1130,7 @@ static int head_bwd(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, con
     e.lse = lse;
     e.lse_pair = (flags & OCTO_LSE_PAIR) != 0;
     e.g = g;
-    e.labels = labels;
+    e.labels = lists ? nullptr : labels;
     e.label_idx = (flags & OCTO_ROWS_VIA_IDX) ? idx : nullptr;
     e.row_off = r0;
     e.V = V;
@@ -1197,6 +1225,17 @@ static int head_bwd(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, con
                             er, st);
       }
       if (rc) return rc;
+      if (lists) {
+        DistillArgs da = *lists;
+        da.r0 = r0;
+        da.rows = rows;
+        da.dz = dza;
+        da.ldx = L.Vc;
+        da.v0 = v0;
+        da.cols = vc;
+        rc = launch_distill_entries(da, st);
+        if (rc) return rc;
+      }
 
       const Operand A3 = plain_operand(dza, L.Vc * esz, L.Vc, nullptr, 0);  // dz token-major, read K-major
       const Operand B3 = plain_operand(ht, L.P * esz, d, nullptr, 0);
@@ -1253,6 +1292,10 @@ static int head_bwd(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, con
   }
   return OCTO_OK;
 }
+
+}  // namespace
+
+extern "C" {
 
 // The kept logits' arguments: bf16, whole tiles of rows.
 static int check_kept(const float *logits, int64_t ld, int64_t rows, int V, int w_dtype) {

@@ -76,7 +76,7 @@ struct DzArgs {
   int64_t v0;
   const float *lse;
   const float *g;
-  const int64_t *labels;
+  const int64_t *labels;     // fp32 dz: NULL for none (launch_distill_entries writes the lists')
   const int64_t *label_idx;  // labels[label_idx[r]] when set
   int64_t row_off;
   int64_t V;
@@ -368,11 +368,11 @@ int launch_pairs_grpo(const PairsGrpoArgs &a, hipStream_t st);
 struct DistillArgs {
   const void *h;
   int64_t ldh;  // elements
-  int h_dtype;
-  const void *w;
-  int64_t ldw;  // elements
-  int w_dtype;
+  int w_dtype;  // fp8: listed logits take their row's scale
   const float *wscale;
+  const void *wm;  // W as the GEMMs read it: fp8 weights widened
+  int64_t ldm;     // elements
+  int dt;          // its type, and the hidden rows'
   const int64_t *idx;  // compact row -> hidden row, or NULL
   const int32_t *count;
   int64_t n_max;
@@ -392,11 +392,13 @@ struct DistillArgs {
   int64_t r0, rows;
   const f32x4 *part;  // local rows
   int64_t mtiles;
-  void *dz;  // local rows: bf16 exponentials relative to xuse (rowoff), else dz in f16
+  // local rows, columns v0 .. v0 + cols of the vocabulary: bf16 exponentials relative to xuse (rowoff), else dz in dt
+  void *dz;
   int64_t ldx;
-  int rowoff, f16;
+  int64_t v0, cols;
+  int rowoff;
 };
-// dots[r][k] = h_r . W_ids[k], fp32 (0 for an empty slot); with xoff, the row's offset: its largest listed logit +
+// dots[r][k] = h_r . W_ids[k], fp32 (0 for an empty slot); with xoff != NULL, the row's offset: its largest listed logit +
 // kExAbove (-inf for a row without a slot); flag_cnt[0 .. nflag) = 0.
 int launch_distill_dots(const DistillArgs &a, hipStream_t st);
 // The pass's rows: the row state, q, kl, g and, with rowoff, xuse and the flagged rows (launch_merge's).

@@ -351,7 +351,8 @@ def fused_distill_head(rows: Tensor, weight: Tensor, ids: Tensor, teacher: Tenso
     it requires grad and grad mode is on). loss.backward() only scales them or, for a short call, makes the weight's from
     the operands kept, as fused_grpo_head's. ids and teacher are [rows, K], row_weight [rows]. idx, count: the rows that
     take part (compact_rows; count on the device); the others' kl and gradients are 0. A row of weight 0 adds nothing to
-    the loss, but is computed with: leave rows out by idx. bf16, f16 and fp8 weights (w_scale; no gradient of those).
+    the loss, but is computed with: leave rows out by idx. bf16, f16, fp32 and fp8 weights (w_scale; no gradient of
+    those).
     The prefix tree's teacher values depend on the path alone, so a tree's rows are its positions, each once, weighted by
     the tokens that share it. The gradients or operands are held from this call until the graph goes."""
     inv_T = _inv_T(temperature)

@@ -8,6 +8,7 @@ dz is rounded once to the operands' type, relative to itself (bf16 2^-8 with the
 at most 48 bits above the row's maximum, so that what lies below 2^-126 of the offset, p below 2^-78, may be lost; in a row
 that is rescaled a half tile's factor is exp2(m_h - m2 - 64), 0 below 2^-126, so that a half tile whose maximum lies more
 than 62 bits below the row's is lost: 2^-62 g per element), and its p is off by 2 e_z + 2^-14 relative.
+fp32 operands (2^-24, by products of three-part values) take the same bounds.
 grad_h = dz W takes those through |W|; grad_W = dz^T h through |h|, whose scaled copy is rounded once more (bf16). Both
 are rounded once to their type, and summed in fp32 over up to V or n terms: 2^-14 of the magnitudes' sum."""
 
@@ -17,10 +18,10 @@ import pytest
 import torch
 
 from oracle import distill as odist
-from oracle import fp8 as ofp8
 
 pytestmark = pytest.mark.gpu
-HALF = {torch.bfloat16: 2 ** -8, torch.float16: 2 ** -11}
+HALF = {torch.bfloat16: 2 ** -8, torch.float16: 2 ** -11, torch.float32: 2 ** -24}
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 
 
 def _batch(n, d, V, K, dtype, seed, spread=2.5, holes=True):
@@ -95,7 +96,7 @@ def _check(h, w, ids, t, rw, T=1.0, post=(1.0, 1.0, False), scored=None, w_scale
                                                    + 2 ** -23 * want_loss.abs()).item()
     dz, dz_err = dz * c, dz_err * abs(c)
     r = HALF[dtype] * 1.05
-    floor = 0.0 if dtype == torch.bfloat16 else 2 ** -24 * max(1.0, abs(c))
+    floor = 2 ** -24 * max(1.0, abs(c)) if dtype == torch.float16 else 0.0
     per = dz_err + (r if dtype == torch.bfloat16 else 2 * r) * dz.abs() + floor
     wa, ha = w.double().abs(), h.double().abs()
     gh = dz @ w.double()
@@ -112,20 +113,20 @@ def _check(h, w, ids, t, rw, T=1.0, post=(1.0, 1.0, False), scored=None, w_scale
     return loss.detach(), kl, hd.grad, wd.grad
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,d,V,K", [(1, 8, 5, 5), (1, 64, 300, 1), (5, 128, 1000, 7), (70, 256, 2048, 64), (257, 264, 1531, 20),
                                      (300, 512, 4160, 256)])
 def test_sizes(dtype, n, d, V, K):
     _check(*_batch(n, d, V, K, dtype, n + V), T=1.0 if V % 2 else 0.7)
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("post", [(1 / 30.0, 30.0, True), (0.5, 0.25, False), (2.0, 1.5, False)])
 def test_post_head_transforms(dtype, post):
     _check(*_batch(90, 256, 1280, 30, dtype, 5, spread=6.0 if post[2] else 2.5), T=0.9, post=post)
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_some_rows_take_part(dtype):
     """Rows left out by a mask (the count stays on the device): none of their lists, weights or hidden values matter."""
     h, w, ids, t, rw = _batch(150, 128, 900, 12, dtype, 7)
@@ -147,7 +148,7 @@ def test_no_weights_raw_lists_and_a_scaled_loss():
     _check(h, w, torch.full_like(ids, -1), t, rw)
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_listed_far_below_the_maximum(dtype):
     """Lists of unlikely tokens at a low temperature: the largest listed logit lies up to hundreds of bits below the row's
     maximum, past the stored exponentials' offset."""
@@ -157,6 +158,32 @@ def test_listed_far_below_the_maximum(dtype):
     if dtype == torch.float16:
         rw = rw * 2 ** -4  # dz up to 1 / T: within the type's range
     _check(h, w, ids, t, rw, T=0.03)
+
+
+def test_fp32_over_several_chunks():
+    """fp32 operands run the forward, then the recomputing backward over vocabulary chunks (rows x vocabulary past the 2 GiB
+    of staging), each of which gets the list's entries that lie in its columns: against the formula in 64 bits."""
+    from octopus_amd import _lib
+    from octopus_amd.distill_op import fused_distill_head
+
+    n, d, V, K = 4096, 64, 160000, 12
+    assert _lib.bwd_plan(n, d, V, _lib.F32, 0, _lib.workspace_bytes(n, d, V, _lib.F32, _lib.WS_STEP))[3] > 1
+    g = torch.Generator(device="cuda").manual_seed(22)
+    h = torch.randn(n, d, device="cuda", generator=g).requires_grad_(True)
+    w = (torch.randn(V, d, device="cuda", generator=g) * 0.3).requires_grad_(True)
+    ids = torch.randint(0, V, (n, K), device="cuda", generator=g)
+    t = torch.randn(n, K, device="cuda", generator=g)
+    rw = torch.rand(n, device="cuda", generator=g)
+    loss, kl = fused_distill_head(h, w, ids, t, 1.0, rw)
+    gh, gw = torch.autograd.grad(loss, (h, w))
+    with torch.no_grad():
+        lp = torch.log_softmax(h.double() @ w.double().T, 1)
+        q = torch.softmax(t.double(), 1)
+        want = (torch.special.xlogy(q, q) - q * lp.gather(1, ids)).sum(1)
+        dz = lp.exp_().scatter_add_(1, ids, -q).mul_(rw.double()[:, None])
+        want_h, want_w = dz @ w.double(), dz.T @ h.double()
+    assert (kl - want).abs().max() <= 1e-4 and abs(loss - (rw * want).sum()) <= 1e-4 * rw.sum()
+    assert (gh - want_h).norm() <= 1e-4 * want_h.norm() and (gw - want_w).norm() <= 1e-4 * want_w.norm()
 
 
 def test_fp8_weights():
@@ -312,8 +339,6 @@ def test_refusals():
                  ((h[:, :12], w[:, :12], ids, t, 1.0), {})]:
         with pytest.raises((ValueError, NotImplementedError)):
             fused_distill_head(*a, **k)
-    with pytest.raises(NotImplementedError):
-        fused_distill_head(h.float(), w.float(), ids, t, 1.0)
     with pytest.raises(NotImplementedError):
         fused_distill_head(h, w.half(), ids, t, 1.0)
     hr = h[:0].clone().requires_grad_(True)
