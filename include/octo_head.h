@@ -237,7 +237,7 @@ int octo_distill_columns_bwd(const void *logits, int64_t ld, int dtype, const in
  * x kl. Lists and weights are per hidden row (compact row r's at idx[r], or r): ids, teacher [h_rows, K], weight [h_rows]
  * (NULL: 1). kl [h_rows] is written at the compact rows' hidden rows, loss [1]. dots, q [n_max, K] and g [n_max] are
  * scratch, as lse [n_max, 2]. grad_h (compact rows) and grad_w as octo_head_step_grpo's; workspace likewise
- * (OCTO_WS_STEP). kept != NULL: no grad_w, whose operands stay in kept for octo_head_later_grad_w, as
+ * (OCTO_WS_STEP; with neither gradient, unless the weights are fp8, the forward's, without that flag). kept != NULL: no grad_w, whose operands stay in kept for octo_head_later_grad_w, as
  * octo_head_step_later (sizes from octo_head_later_bytes). */
 typedef struct octo_distill {
   const int64_t *ids;

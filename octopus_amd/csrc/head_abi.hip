@@ -378,7 +378,7 @@ int head_fwd(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const void
     if (rc) return rc;
   }
 
-  if (lists) {  // the distillation step's forward (fp32 operands)
+  if (lists) {  // the distillation step's forward
     DistillArgs da = *lists;
     da.part = e.part;
     da.mtiles = L.mtiles;
@@ -486,6 +486,11 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
   if (!need_gh && !need_gw && !pm && !later && !ds)
     return head_fwd(h, h_rows, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, count, n_max, d, V, flags, inv_T,
                     pre, post, use_tanh, logp, ent, lse, out2, ld_out2, gt, ws, ws_bytes, stream);
+  if (ds && !need_gh && !need_gw && !later && !cm.fp8) {  // the divergences alone
+    rc = head_fwd(h, h_rows, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, count, n_max, d, V, flags, inv_T, pre,
+                  post, use_tanh, logp, ent, lse, out2, ld_out2, gt, ws, ws_bytes, stream, true, Kept(), &da);
+    return rc ? rc : launch_distill_loss(da, ds->loss, (hipStream_t)stream);
+  }
   if (cm.dt == OCTO_F32) {  // fp32: the forward, then the backward
     if (!ws || ws_bytes < step_fallback_bytes(n_max, d, V, w_dtype, need_gw, cm.gather))
       return octo_fail(OCTO_EWORKSPACE, "head_step_grpo: workspace %zu < %zu bytes", ws ? ws_bytes : (size_t)0,

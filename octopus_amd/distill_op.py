@@ -22,9 +22,10 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib, head_op
-from .embed_op import _float_rows, _ids, _on_gpu, _op
+from .embed_op import _call_on, _float_rows, _ids, _ld, _on_gpu, _op
 from .head_op import (_DT, Post, _dtype_code, _empty, _gather_flag, _index, _later_bytes, _p, _rows2d, _stream,
                       _scale_add, _workspace, _zeros, later_grad_w, scaled)
 
@@ -41,7 +42,10 @@ def _lists(ids: Tensor, teacher: Tensor, rows: int) -> tuple[Tensor, Tensor]:
 def _inv_T(temperature: float) -> float:
     if not temperature > 0:
         raise ValueError("temperature must be positive")
-    return 1.0 / float(temperature)
+    inv_T = 1.0 / float(temperature)
+    if not 0.0 < inv_T < 1e38:
+        raise ValueError(f"temperature {temperature} lies outside fp32's range")
+    return inv_T
 
 
 # ---- the teacher's list ------------------------------------------------------------------------------------------------
@@ -55,9 +59,8 @@ def _topk(logits: Tensor, inv_T: float, k: int) -> tuple[Tensor, Tensor]:
     nbytes = ctypes.c_size_t(0)
     _lib.call("octo_topk_workspace_bytes", n, V, _DT[z.dtype], k, ctypes.byref(nbytes))
     ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev) if nbytes.value else None
-    with torch.cuda.device(dev):
-        _lib.call("octo_topk", _p(z), z.stride(0), _DT[z.dtype], n, V, inv_T, k, _p(ids), _p(logp), _p(ws), nbytes.value,
-                  _stream(z))
+    _call_on(dev, "octo_topk", _p(z), _ld(z), _DT[z.dtype], n, V, inv_T, k, _p(ids), _p(logp), _p(ws), nbytes.value,
+             _stream(z))
     return ids, logp
 
 
@@ -88,7 +91,7 @@ def head_topk(logits: Tensor, temperature: float, k: int) -> tuple[Tensor, Tenso
 # ---- the divergence over materialised logits -----------------------------------------------------------------------------
 
 def _columns_fwd(logits: Tensor, ids: Tensor, teacher: Tensor, inv_T: float,
-                 raw: bool) -> tuple[Tensor, Tensor, Tensor]:
+                 raw: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     dev = _on_gpu(logits, ids, teacher)
     z = _float_rows(logits, "logits")
     n, V = z.shape
@@ -97,17 +100,16 @@ def _columns_fwd(logits: Tensor, ids: Tensor, teacher: Tensor, inv_T: float,
     kl = torch.empty(n, dtype=torch.float32, device=dev)
     state = torch.empty(n, 4, dtype=torch.float32, device=dev)
     q = torch.empty(n, K, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        _lib.call("octo_distill_columns_fwd", _p(z), z.stride(0), _DT[z.dtype], _p(ids), _p(teacher), n, V, K, inv_T,
-                  _lib.LIST_RAW if raw else 0, _p(kl), _p(state), _p(q), _stream(z))
-    return kl, state, q
+    _call_on(dev, "octo_distill_columns_fwd", _p(z), _ld(z), _DT[z.dtype], _p(ids), _p(teacher), n, V, K, inv_T,
+             _lib.LIST_RAW if raw else 0, _p(kl), _p(state), _p(q), _stream(z))
+    return kl, state, q, ids
 
 
 @torch.library.custom_op("octohead::distill_columns_fwd", mutates_args=(), device_types="cuda")
 def distill_columns_fwd(logits: Tensor, ids: Tensor, teacher: Tensor, inv_T: float,
                         raw: bool) -> tuple[Tensor, Tensor, Tensor]:
     """(kl [n], state [n, 4], q [n, K]), the last two for distill_columns_bwd."""
-    return _columns_fwd(logits, ids, teacher, inv_T, raw)
+    return _columns_fwd(logits, ids, teacher, inv_T, raw)[:3]
 
 
 @distill_columns_fwd.register_fake
@@ -123,9 +125,8 @@ def _columns_bwd(logits: Tensor, ids: Tensor, q: Tensor, inv_T: float, state: Te
     ids, q = _lists(ids, q, n)
     dz = torch.empty(n, V, dtype=z.dtype, device=dev)
     state, g = state.contiguous(), g.float().contiguous()
-    with torch.cuda.device(dev):
-        _lib.call("octo_distill_columns_bwd", _p(z), z.stride(0), _DT[z.dtype], _p(ids), _p(q), n, V, ids.shape[1],
-                  inv_T, _p(state), _p(g), _p(dz), V, _stream(z))
+    _call_on(dev, "octo_distill_columns_bwd", _p(z), _ld(z), _DT[z.dtype], _p(ids), _p(q), n, V, ids.shape[1],
+             inv_T, _p(state), _p(g), _p(dz), V, _stream(z))
     return dz
 
 
@@ -161,11 +162,12 @@ class _Columns(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, *args):
-        output = _columns_fwd(*args)
-        _columns_setup(ctx, args, output)
+        *output, ids = _columns_fwd(*args)
+        _columns_setup(ctx, (args[0], ids, *args[2:]), output)
         return output[0]
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gkl):
         return _columns_backward(ctx, gkl, None, None)
 
@@ -198,6 +200,10 @@ def _step(rows: Tensor, weight: Tensor, w_scale: Optional[Tensor], ids: Tensor, 
         if row_weight.shape != (rows2.shape[0],):
             raise ValueError(f"octohead: row weights [{rows2.shape[0]}] expected, got {tuple(row_weight.shape)}")
         row_weight = row_weight.float().contiguous()
+    if count is not None and (count.dtype != torch.int32 or not count.numel()):
+        raise ValueError(f"octohead: a row count of int32 expected (compact_rows), got {count.dtype}")
+    if w_scale is not None and (w_scale.dtype != torch.float32 or w_scale.shape != weight2.shape[:1]):
+        raise ValueError(f"octohead: one fp32 scale per weight row expected, got {w_scale.dtype} {tuple(w_scale.shape)}")
     n_max = idx.numel() if idx is not None else rows2.shape[0]
     V, d = weight2.shape
     K = ids.shape[1]
@@ -212,6 +218,8 @@ def _step(rows: Tensor, weight: Tensor, w_scale: Optional[Tensor], ids: Tensor, 
     code = _dtype_code(weight2)
     if kept is not None:
         nbytes = _lib.later_workspace_bytes(n_max, d, V, code, need_rows)
+    elif not (need_rows or need_weight) and code != _lib.FP8E4M3:  # the forward alone, in its own workspace
+        nbytes = _lib.workspace_bytes(n_max, d, V, code, _gather_flag(rows2, idx))
     else:
         flags = (_lib.WS_STEP | (0 if need_weight else _lib.WS_NO_GRADW) | (0 if need_rows else _lib.WS_NO_GRADH)
                  | _gather_flag(rows2, idx))
@@ -227,15 +235,14 @@ def _step(rows: Tensor, weight: Tensor, w_scale: Optional[Tensor], ids: Tensor, 
     if need_rows:  # compact-order rows; scattered into grad_rows below
         gh = grad_rows if idx is None else torch.empty(n_max, d, dtype=rows2.dtype, device=dev)
     gw = grad_w if need_weight and kept is None else None
-    with torch.cuda.device(dev):
-        _lib.call("octo_head_step_distill", _p(rows2), rows2.shape[0], rows2.stride(0), _dtype_code(rows2),
-                  _p(weight2), weight2.stride(0), code, _p(w_scale), _p(idx), _p(count), n_max, d, V, inv_T, pre, post,
-                  int(use_tanh), _p(lse), ctypes.byref(lists), _p(gh), d,
-                  _dtype_code(rows2) if need_rows else _lib.F32, _p(gw), code if gw is not None else _lib.F32,
-                  _p(kept), 0 if kept is None else kept.numel(), _p(ws), ws.numel(), _stream(rows2))
-        if need_rows and idx is not None:
-            _lib.call("octo_rows_scatter", _p(gh), d, _dtype_code(gh), _p(idx), _p(count), n_max, d, _p(grad_rows),
-                      grad_rows.stride(0), _dtype_code(grad_rows), 0, _stream(rows2))
+    _call_on(dev, "octo_head_step_distill", _p(rows2), rows2.shape[0], _ld(rows2), _dtype_code(rows2),
+             _p(weight2), _ld(weight2), code, _p(w_scale), _p(idx), _p(count), n_max, d, V, inv_T, pre, post,
+             int(use_tanh), _p(lse), ctypes.byref(lists), _p(gh), d, _dtype_code(rows2) if need_rows else _lib.F32,
+             _p(gw), code if gw is not None else _lib.F32, _p(kept), 0 if kept is None else kept.numel(), _p(ws),
+             ws.numel(), _stream(rows2))
+    if need_rows and idx is not None:
+        _call_on(dev, "octo_rows_scatter", _p(gh), d, _dtype_code(gh), _p(idx), _p(count), n_max, d, _p(grad_rows),
+                 grad_rows.stride(0), _dtype_code(grad_rows), 0, _stream(rows2))
     return loss, kl, grad_rows, grad_w
 
 
@@ -327,6 +334,7 @@ class _Head(torch.autograd.Function):
         return output[0], output[1]
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gloss, gkl):
         if ctx.later:
             return _later_backward(ctx, gloss) + (None,) * 10
@@ -350,7 +358,7 @@ def fused_distill_head(rows: Tensor, weight: Tensor, ids: Tensor, teacher: Tenso
     detached, from one call that computes the logits once and also the gradients of the loss in rows and weight (each when
     it requires grad and grad mode is on). loss.backward() only scales them or, for a short call, makes the weight's from
     the operands kept, as fused_grpo_head's. ids and teacher are [rows, K], row_weight [rows]. idx, count: the rows that
-    take part (compact_rows; count on the device); the others' kl and gradients are 0. A row of weight 0 adds nothing to
+    take part (ascending, as compact_rows gives them; count on the device); the others' kl and gradients are 0. A row of weight 0 adds nothing to
     the loss, but is computed with: leave rows out by idx. bf16, f16, fp32 and fp8 weights (w_scale; no gradient of
     those).
     The prefix tree's teacher values depend on the path alone, so a tree's rows are its positions, each once, weighted by

@@ -15,6 +15,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .head_op import _DT, _p, _stream, _workspace
@@ -28,7 +29,12 @@ def _float_rows(x: Tensor, what: str) -> Tensor:
         raise ValueError(f"octohead: {what} must be [rows, d], got {tuple(x.shape)}")
     if x.dtype not in _FLOATS:
         raise NotImplementedError(f"octohead: {what} of dtype {x.dtype} has no HIP kernel")
-    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+    return x if x.stride(1) == 1 and (x.shape[0] < 2 or x.stride(0) >= x.shape[1]) else x.contiguous()
+
+
+def _ld(x: Tensor) -> int:
+    """Elements between x's rows; one row's stride may be any number."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
 def _on_gpu(*tensors: Optional[Tensor]) -> torch.device:
@@ -37,6 +43,15 @@ def _on_gpu(*tensors: Optional[Tensor]) -> torch.device:
         if t is not None and (not t.is_cuda or t.device != dev):
             raise ValueError(f"octohead: tensors on one HIP device expected, got {dev} and {t.device}")
     return dev
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """_lib.call with dev current; entering a device that is current already would cost a tenth of a short call."""
+    if torch.cuda.current_device() == dev.index:
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args)
 
 
 def _ids(ids: Tensor) -> Tensor:
@@ -53,9 +68,8 @@ def _fwd(weight: Tensor, ids: Tensor, scale: float) -> Tensor:
     if V == 0:
         raise ValueError("octohead: an empty vocabulary")
     out = torch.empty(*ids.shape, d, dtype=w.dtype, device=dev)
-    with torch.cuda.device(dev):
-        _lib.call("octo_embed_fwd", _p(w), w.stride(0), _DT[w.dtype], V, d, _p(flat), flat.numel(), float(scale),
-                  _p(out), d, _stream(w))
+    _call_on(dev, "octo_embed_fwd", _p(w), _ld(w), _DT[w.dtype], V, d, _p(flat), flat.numel(), float(scale),
+             _p(out), d, _stream(w))
     return out
 
 
@@ -70,9 +84,8 @@ def _bwd(into: Tensor, grad: Tensor, ids: Tensor, scale: float, padding_idx: int
     nbytes = ctypes.c_size_t(0)
     _lib.call("octo_embed_bwd_workspace_bytes", n, V, d, ctypes.byref(nbytes))
     ws = _workspace(nbytes.value, into)
-    with torch.cuda.device(dev):
-        _lib.call("octo_embed_bwd", _p(g), g.stride(0), _DT[g.dtype], _p(flat), n, V, d, padding_idx, float(scale),
-                  _p(into), into.stride(0), _DT[into.dtype], int(accumulate), _p(ws), ws.numel(), _stream(into))
+    _call_on(dev, "octo_embed_bwd", _p(g), _ld(g), _DT[g.dtype], _p(flat), n, V, d, padding_idx, float(scale),
+             _p(into), _ld(into), _DT[into.dtype], int(accumulate), _p(ws), ws.numel(), _stream(into))
 
 
 @torch.library.custom_op("octohead::embed_fwd", mutates_args=(), device_types="cuda")
@@ -148,6 +161,7 @@ class _Embed(torch.autograd.Function):
         return _fwd(weight, ids, scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gout):
         return _backward(ctx, gout)
 

@@ -1,0 +1,167 @@
+"""Calls of the lists, the divergence and the embedding that their documentation allows beside the plain ones: rows of any
+stride, second derivatives (refused), traces, another current stream, counts and scales of other types (refused)."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _r(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def test_one_row_of_any_stride():
+    """[V, 1] transposed: a row whose stride is 1."""
+    from octopus_amd import distill_op, embed_op
+
+    col = _r(700, 1)
+    row = col.T
+    assert row.stride(0) == 1
+    a, b = distill_op.head_topk(row, 1.0, 9), distill_op.head_topk(row.clone(memory_format=torch.contiguous_format), 1.0, 9)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    ids, t = a
+    z = row.detach().requires_grad_(True)
+    kl = distill_op.distill_columns(z, 1.0, ids, t + 0.5)
+    (grad,) = torch.autograd.grad(kl.sum(), z)
+    assert grad.shape == (1, 700) and kl.isfinite().all()
+    w = _r(16, 1, seed=1).T  # a vocabulary of one entry
+    out = embed_op.embed_rows(w, torch.zeros(3, dtype=torch.int64, device="cuda"), 2.0)
+    assert torch.equal(out, 2.0 * w.expand(3, 16))
+    h = _r(64, 1, seed=2).to(torch.bfloat16).T
+    weight = _r(300, 64, seed=3).to(torch.bfloat16)
+    top = torch.arange(4, device="cuda")[None]
+    a = distill_op.fused_distill_head(h, weight, top, torch.zeros(1, 4, device="cuda"), 1.0)
+    b = distill_op.fused_distill_head(h.clone(memory_format=torch.contiguous_format), weight, top,
+                                      torch.zeros(1, 4, device="cuda"), 1.0)
+    assert torch.equal(a[0], b[0])
+
+
+def test_second_derivatives_are_refused():
+    """The backward passes are kernels without one of their own: asking for it raises, and is never a silent constant."""
+    from octopus_amd import distill_op, embed_op
+
+    z = _r(4, 200).requires_grad_(True)
+    ids = torch.randint(0, 200, (4, 5), device="cuda")
+    (g,) = torch.autograd.grad(distill_op.distill_columns(z, 1.0, ids, _r(4, 5)).sum(), z, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), z)
+    w = _r(50, 16).requires_grad_(True)
+    out = embed_op.embed_rows(w, ids)
+    gout = _r(4, 5, 16, seed=4).requires_grad_(True)
+    (g,) = torch.autograd.grad(out, w, gout, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), gout)
+    h, weight = _r(4, 64).to(torch.bfloat16).requires_grad_(True), _r(200, 64).to(torch.bfloat16).requires_grad_(True)
+    loss, _ = distill_op.fused_distill_head(h, weight, ids, _r(4, 5), 1.0)
+    (g,) = torch.autograd.grad(loss, h, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.float().sum(), h)
+
+
+def test_backward_after_the_last_one_raises():
+    from octopus_amd import distill_op
+
+    h, weight = _r(4, 64).to(torch.bfloat16).requires_grad_(True), _r(200, 64).to(torch.bfloat16).requires_grad_(True)
+    ids = torch.randint(0, 200, (4, 5), device="cuda")
+    loss, _ = distill_op.fused_distill_head(h, weight, ids, _r(4, 5), 1.0)
+    kept = torch.autograd.grad(loss, (h, weight), retain_graph=True)
+    once = torch.autograd.grad(2 * loss, (h, weight))
+    assert all(torch.equal(2 * a, b) for a, b in zip(kept, once))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, (h, weight))
+
+
+def test_without_gradients_the_forwards_workspace_is_enough():
+    """The divergences alone, bit for bit those of the step, without the step's staging."""
+    from octopus_amd import distill_op
+
+    n, d, V = 600, 128, 40000
+    h, weight = _r(n, d).to(torch.bfloat16), (_r(V, d, seed=1) * 0.2).to(torch.bfloat16)
+    ids, t, rw = torch.randint(0, V, (n, 12), device="cuda"), _r(n, 12, seed=2), torch.rand(n, device="cuda")
+    want = distill_op.fused_distill_head(h.clone().requires_grad_(True), weight, ids, t, 0.9, rw)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = distill_op.fused_distill_head(h, weight, ids, t, 0.9, rw)
+    assert torch.cuda.max_memory_allocated() - before < n * V * 2  # no exponentials
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_traced_ops():
+    """The registered ops: schemas, shapes under tracing and, where they have one, their gradients."""
+    from octopus_amd import distill_op, embed_op
+
+    tests = ("test_schema", "test_faketensor", "test_autograd_registration")
+    z = _r(5, 300).requires_grad_(True)
+    ids = torch.randint(0, 300, (5, 7), device="cuda")
+    t = _r(5, 7, seed=5)
+    torch.library.opcheck(distill_op.topk, (z.detach(), 1.0, 9), test_utils=tests)
+    torch.library.opcheck(distill_op.distill_columns_fwd, (z, ids, t, 1.0, False), test_utils=tests)
+    _, state, q = distill_op.distill_columns_fwd(z.detach(), ids, t, 1.0, False)
+    torch.library.opcheck(distill_op.distill_columns_bwd, (z.detach(), ids, q, 1.0, state, t[:, 0]), test_utils=tests)
+    w = _r(300, 64, seed=6).to(torch.bfloat16).requires_grad_(True)
+    torch.library.opcheck(embed_op.embed_fwd, (w, ids, 2.0, -1), test_utils=tests)
+    torch.library.opcheck(embed_op._embed_bwd, (_r(5, 7, 64), ids, 300, 2.0, -1, torch.float32), test_utils=tests)
+    h = _r(5, 64, seed=7).to(torch.bfloat16).requires_grad_(True)
+    torch.library.opcheck(distill_op.head_step_distill, (h, w, None, ids, t, None, None, None, 1.0, 1.0, 1.0, False, False,
+                                                         True, True), test_utils=tests)
+    loss, kl, gh, gw = distill_op.head_step_distill(h, w, None, ids, t, None, None, None, 1.0, 1.0, 1.0, False, False, True,
+                                                    True)
+    loss2, kl2 = distill_op.fused_distill_head(h, w, ids, t, 1.0)
+    assert torch.equal(loss, loss2) and torch.equal(kl, kl2)
+    for a, b in zip(torch.autograd.grad(3 * loss, (h, w), retain_graph=True), torch.autograd.grad(3 * loss2, (h, w))):
+        assert torch.equal(a, b)
+    assert torch.equal(gh, torch.autograd.grad(loss, h)[0])  # the op's own outputs stay as they were
+
+
+def test_refused_companions():
+    from octopus_amd import distill_op
+
+    h, weight = _r(6, 64).to(torch.bfloat16), _r(200, 64).to(torch.bfloat16)
+    ids, t = torch.randint(0, 200, (6, 5), device="cuda"), _r(6, 5)
+    idx = torch.arange(6, device="cuda")
+    count = torch.tensor([6], device="cuda")
+    with pytest.raises(ValueError):
+        distill_op.fused_distill_head(h, weight, ids, t, 1.0, idx=idx, count=count)
+    q8 = weight.to(torch.float8_e4m3fn)
+    for scale in (torch.ones(199, device="cuda"), torch.ones(200, dtype=torch.float64, device="cuda"), None):
+        with pytest.raises(ValueError):
+            distill_op.fused_distill_head(h, q8, ids, t, 1.0, w_scale=scale)
+    for T in (float("nan"), float("inf"), 1e-39, 0.0):
+        with pytest.raises(ValueError):
+            distill_op.head_topk(h, T, 3)
+    with pytest.raises(NotImplementedError):
+        distill_op.fused_distill_head(h, q8.requires_grad_(True), ids, t, 1.0, w_scale=torch.ones(200, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_behind_the_last_stay_as_they_were(dtype):
+    """Outputs and in-place gradients lie inside larger buffers: nothing around them is written."""
+    from octopus_amd import _lib
+    from octopus_amd.embed_op import embed_grad_add_
+    from octopus_amd.head_op import _DT, _p, _stream
+
+    V, d, n = 37, 40, 90
+    base = torch.full((V + 20, d + 24), 7.0, dtype=dtype, device="cuda")
+    ids = torch.randint(0, V, (n,), device="cuda")
+    embed_grad_add_(base[10:10 + V, 8:8 + d], _r(n, d).to(dtype), ids)
+    edge = base.clone()
+    edge[10:10 + V, 8:8 + d] = 7.0
+    assert (edge == 7.0).all()
+    # the dense gradient through the C ABI into rows a step apart: the gaps keep their values
+    import ctypes
+
+    out = torch.full((V + 2, d + 24), 7.0, dtype=dtype, device="cuda")
+    nbytes = ctypes.c_size_t(0)
+    _lib.call("octo_embed_bwd_workspace_bytes", n, V, d, ctypes.byref(nbytes))
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device="cuda")
+    g = _r(n, d, seed=1).to(dtype)
+    inner = out[1:1 + V, 8:8 + d]
+    _lib.call("octo_embed_bwd", _p(g), d, _DT[dtype], _p(ids), n, V, d, -1, 1.0, _p(inner), d + 24, _DT[dtype], 0, _p(ws),
+              ws.numel(), _stream(g))
+    edge = out.clone()
+    edge[1:1 + V, 8:8 + d] = 7.0
+    assert (edge == 7.0).all()
+    want = torch.zeros(V, d, device="cuda").index_add_(0, ids, g.float())
+    assert (inner.float() - want).abs().max() <= 2 ** -7 * want.abs().max()
