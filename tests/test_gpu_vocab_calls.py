@@ -165,3 +165,112 @@ def test_rows_behind_the_last_stay_as_they_were(dtype):
     assert (edge == 7.0).all()
     want = torch.zeros(V, d, device="cuda").index_add_(0, ids, g.float())
     assert (inner.float() - want).abs().max() <= 2 ** -7 * want.abs().max()
+
+
+def _head_inputs(seed, n=120, d=256, V=3003):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    h = torch.randn(n, d, generator=g, device="cuda").bfloat16().requires_grad_(True)
+    w = (torch.randn(V, d, generator=g, device="cuda") * 0.1).bfloat16().requires_grad_(True)
+    ids = torch.randint(0, V, (n, 20), generator=g, device="cuda")
+    return h, w, ids, torch.randn(n, 20, generator=g, device="cuda"), torch.rand((), generator=g, device="cuda")
+
+
+def _head_step(h, w, ids, t, c):
+    from octopus_amd.distill_op import fused_distill_head
+
+    loss, kl = fused_distill_head(h, w, ids, t, 0.9)
+    return (kl, *torch.autograd.grad(loss, (h, w), c))
+
+
+def _columns_step(h, w, ids, t, c):
+    from octopus_amd.distill_op import distill_columns
+    from octopus_amd.embed_op import embed_rows
+
+    z = w.T[:100, :3001]  # any logits: 100 rows whose columns lie apart
+    kl = distill_columns(z, 0.8, ids[:100], t[:100])
+    out = embed_rows(w, ids, 2.0)
+    return (kl.detach(), *torch.autograd.grad(kl, z, c.expand(100)), *torch.autograd.grad(out, w, torch.ones_like(out)))
+
+
+@pytest.mark.parametrize("step", [_head_step, _columns_step])
+@pytest.mark.parametrize("later", [False, True])
+def test_captured_with_autograd(monkeypatch, step, later):
+    """Forward and backward in one graph, replayed on new values between the program's own calls; later: the head's weight
+    gradient made in the backward from kept operands."""
+    from octopus_amd import head_op
+
+    if later:
+        monkeypatch.setattr(head_op, "_LATER_WEIGHTS", 0)
+        monkeypatch.setattr(head_op, "_LATER_SHARE", 1 << 20)
+    static = _head_inputs(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*static)
+    for seed in (1, 2, 3):
+        new = _head_inputs(seed)
+        with torch.no_grad():
+            for a, b in zip(static, new):
+                a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step(*new)))
+
+
+def test_threads_with_streams_of_their_own():
+    import threading
+
+    inputs = [_head_inputs(k) for k in range(3)]
+    want = [_head_step(*x) + _columns_step(*x) for x in inputs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got = _head_step(*inputs[k]) + _columns_step(*inputs[k])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[k])):
+                    wrong.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_far_offsets():
+    """A weight of more than 2^31 elements, logits of more than 2^32 bytes: the last rows."""
+    from octopus_amd import distill_op, embed_op
+
+    V, d = 1_100_000, 2048  # 2.25e9 elements
+    w = torch.zeros(V, d, dtype=torch.bfloat16, device="cuda")
+    w[-1] = 3.0
+    w[-2] = torch.arange(d, device="cuda") % 128
+    ids = torch.tensor([V - 1, V - 2, V, 0], device="cuda")
+    got = embed_op.embed_rows(w, ids, 0.5)
+    assert (got[0] == 1.5).all() and torch.equal(got[1], w[-2] * 0.5) and (got[2:] == 0).all()
+    embed_op.embed_grad_add_(w, torch.ones(4, d, dtype=torch.bfloat16, device="cuda"), ids)
+    assert (w[-1] == 4.0).all() and (w[0] == 1.0).all() and (w[1:-2].view(torch.int16) == 0).all()
+    del w, got
+    gw = embed_op.embed_bwd(torch.ones(4, d, dtype=torch.bfloat16, device="cuda"), ids, V)
+    assert (gw[-2:] == 1).all() and (gw[0] == 1).all() and (gw[1:-2].view(torch.int16) == 0).all()
+    del gw
+    n, V = 18000, 128257  # 2.3e9 values of 16 bits
+    z = torch.zeros(n, V, dtype=torch.bfloat16, device="cuda")
+    z[-1, 5], z[-1, 128256], z[-2, 77] = 9.0, 9.0, 4.0
+    top, logp = distill_op.head_topk(z, 1.0, 3)
+    assert top[-1].tolist() == [5, 128256, 0] and top[-2].tolist() == [77, 0, 1]
+    z.requires_grad_(True)
+    kl = distill_op.distill_columns(z, 1.0, top, logp)
+    (grad,) = torch.autograd.grad(kl.sum(), z)
+    p = torch.softmax(z.detach()[-2:].double(), 1)
+    q = torch.softmax(logp[-2:].double(), 1)
+    want = p.scatter_add(1, top[-2:], -q)
+    assert ((grad[-2:].double() - want).abs() <= 2 ** -8 * want.abs() + 1e-5 * (p + want.abs())).all()
