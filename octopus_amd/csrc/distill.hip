@@ -7,7 +7,8 @@
 //   dL/dz_v = g (Q p_v - sum of q_k over the slots with id_k = v) / T,   g = dL/dkl
 //
 // Both directions are bound by memory: the forward reads each logit once, the backward reads it once more and writes
-// its gradient. The forward leaves q, and the row's (maximum, ln S), for the backward.
+// its gradient. The forward leaves q, and the row's (maximum, log2 S, Q), for the backward. [2048, 151,936] bf16, K 64:
+// forward 125 us (5.0 TB/s), backward 217 (5.7).
 #include "octo_internal.h"
 #include "row_values.h"
 

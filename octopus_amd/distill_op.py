@@ -26,8 +26,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib, head_op
 from .embed_op import _call_on, _float_rows, _ids, _ld, _on_gpu, _op
-from .head_op import (_DT, Post, _dtype_code, _empty, _gather_flag, _index, _later_bytes, _p, _rows2d, _stream,
-                      _scale_add, _workspace, _zeros, later_grad_w, scaled)
+from .head_op import (_DT, Post, _dtype_code, _empty, _gather_flag, _index, _later_bytes, _p, _rows2d,
+                      _workspace, _zeros, later_grad_w, scaled)
 
 
 def _lists(ids: Tensor, teacher: Tensor, rows: int) -> tuple[Tensor, Tensor]:
@@ -59,8 +59,7 @@ def _topk(logits: Tensor, inv_T: float, k: int) -> tuple[Tensor, Tensor]:
     nbytes = ctypes.c_size_t(0)
     _lib.call("octo_topk_workspace_bytes", n, V, _DT[z.dtype], k, ctypes.byref(nbytes))
     ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev) if nbytes.value else None
-    _call_on(dev, "octo_topk", _p(z), _ld(z), _DT[z.dtype], n, V, inv_T, k, _p(ids), _p(logp), _p(ws), nbytes.value,
-             _stream(z))
+    _call_on(dev, "octo_topk", _p(z), _ld(z), _DT[z.dtype], n, V, inv_T, k, _p(ids), _p(logp), _p(ws), nbytes.value)
     return ids, logp
 
 
@@ -90,8 +89,8 @@ def head_topk(logits: Tensor, temperature: float, k: int) -> tuple[Tensor, Tenso
 
 # ---- the divergence over materialised logits -----------------------------------------------------------------------------
 
-def _columns_fwd(logits: Tensor, ids: Tensor, teacher: Tensor, inv_T: float,
-                 raw: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+def _columns_fwd(logits: Tensor, ids: Tensor, teacher: Tensor, inv_T: float, raw: bool) -> tuple[Tensor, ...]:
+    """(kl, state, q, and the logits and ids as the kernels read them)."""
     dev = _on_gpu(logits, ids, teacher)
     z = _float_rows(logits, "logits")
     n, V = z.shape
@@ -101,8 +100,8 @@ def _columns_fwd(logits: Tensor, ids: Tensor, teacher: Tensor, inv_T: float,
     state = torch.empty(n, 4, dtype=torch.float32, device=dev)
     q = torch.empty(n, K, dtype=torch.float32, device=dev)
     _call_on(dev, "octo_distill_columns_fwd", _p(z), _ld(z), _DT[z.dtype], _p(ids), _p(teacher), n, V, K, inv_T,
-             _lib.LIST_RAW if raw else 0, _p(kl), _p(state), _p(q), _stream(z))
-    return kl, state, q, ids
+             _lib.LIST_RAW if raw else 0, _p(kl), _p(state), _p(q))
+    return kl, state, q, z, ids
 
 
 @torch.library.custom_op("octohead::distill_columns_fwd", mutates_args=(), device_types="cuda")
@@ -123,10 +122,16 @@ def _columns_bwd(logits: Tensor, ids: Tensor, q: Tensor, inv_T: float, state: Te
     z = _float_rows(logits, "logits")
     n, V = z.shape
     ids, q = _lists(ids, q, n)
-    dz = torch.empty(n, V, dtype=z.dtype, device=dev)
-    state, g = state.contiguous(), g.float().contiguous()
-    _call_on(dev, "octo_distill_columns_bwd", _p(z), _ld(z), _DT[z.dtype], _p(ids), _p(q), n, V, ids.shape[1],
-             inv_T, _p(state), _p(g), _p(dz), V, _stream(z))
+    return _columns_grad(z, ids, q, inv_T, state.contiguous(), g)
+
+
+def _columns_grad(z: Tensor, ids: Tensor, q: Tensor, inv_T: float, state: Tensor, g: Tensor) -> Tensor:
+    """Of a forward's own tensors, not looked at again."""
+    n, V = z.shape
+    dz = torch.empty(n, V, dtype=z.dtype, device=z.device)
+    g = g.float().contiguous()
+    _call_on(z.device, "octo_distill_columns_bwd", _p(z), _ld(z), _DT[z.dtype], _p(ids), _p(q), n, V, ids.shape[1],
+             inv_T, _p(state), _p(g), _p(dz), V)
     return dz
 
 
@@ -148,9 +153,8 @@ def _columns_setup(ctx, inputs, output):
 
 def _columns_backward(ctx, gkl, _gstate, _gq):
     logits, ids, state, q = ctx.saved_tensors
-    if not ctx.needs_input_grad[0]:
-        return (None,) * 5
-    return (_op(distill_columns_bwd, _columns_bwd)(logits, ids, q, ctx.inv_T, state, gkl),) + (None,) * 4
+    dz = distill_columns_bwd(logits, ids, q, ctx.inv_T, state, gkl) if ctx.needs_input_grad[0] else None
+    return dz, None, None, None, None
 
 
 torch.library.register_autograd("octohead::distill_columns_fwd", _columns_backward, setup_context=_columns_setup)
@@ -162,14 +166,16 @@ class _Columns(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, *args):
-        *output, ids = _columns_fwd(*args)
-        _columns_setup(ctx, (args[0], ids, *args[2:]), output)
-        return output[0]
+        kl, state, q, z, ids = _columns_fwd(*args)
+        ctx.save_for_backward(z, ids, state, q)
+        ctx.inv_T = args[3]
+        return kl
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gkl):
-        return _columns_backward(ctx, gkl, None, None)
+        z, ids, state, q = ctx.saved_tensors
+        return (_columns_grad(z, ids, q, ctx.inv_T, state, gkl),) + (None,) * 4
 
 
 def distill_columns(logits: Tensor, temperature: float, ids: Tensor, teacher: Tensor, *,
@@ -239,10 +245,10 @@ def _step(rows: Tensor, weight: Tensor, w_scale: Optional[Tensor], ids: Tensor, 
              _p(weight2), _ld(weight2), code, _p(w_scale), _p(idx), _p(count), n_max, d, V, inv_T, pre, post,
              int(use_tanh), _p(lse), ctypes.byref(lists), _p(gh), d, _dtype_code(rows2) if need_rows else _lib.F32,
              _p(gw), code if gw is not None else _lib.F32, _p(kept), 0 if kept is None else kept.numel(), _p(ws),
-             ws.numel(), _stream(rows2))
+             ws.numel())
     if need_rows and idx is not None:
         _call_on(dev, "octo_rows_scatter", _p(gh), d, _dtype_code(gh), _p(idx), _p(count), n_max, d, _p(grad_rows),
-                 grad_rows.stride(0), _dtype_code(grad_rows), 0, _stream(rows2))
+                 grad_rows.stride(0), _dtype_code(grad_rows), 0)
     return loss, kl, grad_rows, grad_w
 
 
@@ -272,8 +278,8 @@ def _step_setup(ctx, inputs, output):
 
 def _step_backward(ctx, gloss, _gkl, _ggr, _ggw):
     # into tensors of their own: the op's outputs are its caller's, and a retained graph's second backward reads them
-    out = [(torch.zeros_like(t) if gloss is None else scaled(t, gloss)) if ctx.need[k] and ctx.needs_input_grad[k] else None
-           for k, t in enumerate(ctx.grads)]
+    wanted = [t if ctx.need[k] and ctx.needs_input_grad[k] else None for k, t in enumerate(ctx.grads)]
+    out = [None if t is None else torch.zeros_like(t) if gloss is None else scaled(t, gloss) for t in wanted]
     return (*out,) + (None,) * 13
 
 
@@ -345,9 +351,11 @@ class _Head(torch.autograd.Function):
             return _step_backward(ctx, gloss, None, None, None)[:2] + (None,) * 10
         held, ctx.grads = ctx.grads, None
         c = gloss.float().contiguous()
-        with torch.cuda.device(c.device):
-            return tuple(_scale_add(t, None, c, None) if ctx.need[k] and ctx.needs_input_grad[k] else None
-                         for k, t in enumerate(held)) + (None,) * 10
+        out = [t if ctx.need[k] and ctx.needs_input_grad[k] else None for k, t in enumerate(held)]
+        for t in out:
+            if t is not None and t.numel():
+                _call_on(t.device, "octo_scale_add", _p(t), None, _DT[t.dtype], t.numel(), _p(c), None)
+        return (*out,) + (None,) * 10
 
 
 def fused_distill_head(rows: Tensor, weight: Tensor, ids: Tensor, teacher: Tensor, temperature: float,
@@ -358,9 +366,9 @@ def fused_distill_head(rows: Tensor, weight: Tensor, ids: Tensor, teacher: Tenso
     detached, from one call that computes the logits once and also the gradients of the loss in rows and weight (each when
     it requires grad and grad mode is on). loss.backward() only scales them or, for a short call, makes the weight's from
     the operands kept, as fused_grpo_head's. ids and teacher are [rows, K], row_weight [rows]. idx, count: the rows that
-    take part (ascending, as compact_rows gives them; count on the device); the others' kl and gradients are 0. A row of weight 0 adds nothing to
-    the loss, but is computed with: leave rows out by idx. bf16, f16, fp32 and fp8 weights (w_scale; no gradient of
-    those).
+    take part (ascending, as compact_rows gives them; count on the device); the others' kl and gradients are 0. A row of
+    weight 0 adds nothing to the loss, but is computed with: leave rows out by idx. bf16, f16, fp32 and fp8 weights
+    (w_scale; no gradient of those).
     The prefix tree's teacher values depend on the path alone, so a tree's rows are its positions, each once, weighted by
     the tokens that share it. The gradients or operands are held from this call until the graph goes."""
     inv_T = _inv_T(temperature)

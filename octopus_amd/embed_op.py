@@ -18,7 +18,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .head_op import _DT, _p, _stream, _workspace
+from .head_op import _DT, _p, _workspace
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -46,12 +46,14 @@ def _on_gpu(*tensors: Optional[Tensor]) -> torch.device:
 
 
 def _call_on(dev: torch.device, name: str, *args) -> None:
-    """_lib.call with dev current; entering a device that is current already would cost a tenth of a short call."""
+    """_lib.call on dev's current stream, its last argument, with dev current. The raw handle, and no entering of a device
+    that is current already: the stream's Python object alone takes 10 us in a backward's thread, a tenth of a short call."""
+    stream = ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(dev.index))
     if torch.cuda.current_device() == dev.index:
-        _lib.call(name, *args)
+        _lib.call(name, *args, stream)
     else:
         with torch.cuda.device(dev):
-            _lib.call(name, *args)
+            _lib.call(name, *args, stream)
 
 
 def _ids(ids: Tensor) -> Tensor:
@@ -69,7 +71,7 @@ def _fwd(weight: Tensor, ids: Tensor, scale: float) -> Tensor:
         raise ValueError("octohead: an empty vocabulary")
     out = torch.empty(*ids.shape, d, dtype=w.dtype, device=dev)
     _call_on(dev, "octo_embed_fwd", _p(w), _ld(w), _DT[w.dtype], V, d, _p(flat), flat.numel(), float(scale),
-             _p(out), d, _stream(w))
+             _p(out), d)
     return out
 
 
@@ -85,7 +87,7 @@ def _bwd(into: Tensor, grad: Tensor, ids: Tensor, scale: float, padding_idx: int
     _lib.call("octo_embed_bwd_workspace_bytes", n, V, d, ctypes.byref(nbytes))
     ws = _workspace(nbytes.value, into)
     _call_on(dev, "octo_embed_bwd", _p(g), _ld(g), _DT[g.dtype], _p(flat), n, V, d, padding_idx, float(scale),
-             _p(into), _ld(into), _DT[into.dtype], int(accumulate), _p(ws), ws.numel(), _stream(into))
+             _p(into), _ld(into), _DT[into.dtype], int(accumulate), _p(ws), ws.numel())
 
 
 @torch.library.custom_op("octohead::embed_fwd", mutates_args=(), device_types="cuda")
