@@ -87,6 +87,7 @@ extern "C" {
 #define OCTO_WS_NO_GRADH    256  /* octo_head_workspace_bytes / octo_head_bwd_plan: without grad_h        */
 #define OCTO_PAIRS_NONE_AS_COUNT 1 /* octo_label_pairs: positions without a pair get the pair count  */
 #define OCTO_LIST_MAX        256 /* octo_topk, octo_distill_*: the most entries of a row's list           */
+#define OCTO_ROW_MAX   (1 << 30) /* octo_topk, octo_distill_columns_*, octo_embed_*: the largest vocabulary  */
 #define OCTO_LIST_RAW          1 /* octo_distill_*: q = exp(t) as given, not the softmax over the row's list */
 
 const char *octo_version(void);
@@ -237,8 +238,9 @@ int octo_distill_columns_bwd(const void *logits, int64_t ld, int dtype, const in
  * x kl. Lists and weights are per hidden row (compact row r's at idx[r], or r): ids, teacher [h_rows, K], weight [h_rows]
  * (NULL: 1). kl [h_rows] is written at the compact rows' hidden rows, loss [1]. dots, q [n_max, K] and g [n_max] are
  * scratch, as lse [n_max, 2]. grad_h (compact rows) and grad_w as octo_head_step_grpo's; workspace likewise
- * (OCTO_WS_STEP; with neither gradient, unless the weights are fp8, the forward's, without that flag). kept != NULL: no grad_w, whose operands stay in kept for octo_head_later_grad_w, as
- * octo_head_step_later (sizes from octo_head_later_bytes). */
+ * (OCTO_WS_STEP; with neither gradient, unless the weights are fp8, the forward's, without that flag). kept != NULL: no
+ * grad_w, whose operands stay in kept for octo_head_later_grad_w, as octo_head_step_later (sizes from
+ * octo_head_later_bytes). */
 typedef struct octo_distill {
   const int64_t *ids;
   const float *teacher;
@@ -262,7 +264,7 @@ int octo_embed_fwd(const void *w, int64_t ldw, int dtype, int64_t V, int d, cons
 /* Its gradient by sorted tokens: grad_w[v, :d] = scale * sum of grad[t, :d] over the tokens with ids[t] = v, summed in
  * fp32 in an order that the ids alone decide and rounded once to w_dtype; ids outside [0, V) and padding_idx (-1: none)
  * are left out. accumulate: added to what grad_w holds, and the rows of other entries are neither read nor written; else
- * every row is written. ws: octo_embed_bwd_workspace_bytes, 16-byte aligned. */
+ * every row is written. n <= 2^27. ws: octo_embed_bwd_workspace_bytes, 16-byte aligned. */
 int octo_embed_bwd_workspace_bytes(int64_t n, int64_t V, int d, size_t *bytes);
 int octo_embed_bwd(const void *grad, int64_t ldg, int g_dtype, const int64_t *ids, int64_t n, int64_t V, int d,
                    int64_t padding_idx, float scale, void *grad_w, int64_t ldw, int w_dtype, int accumulate, void *ws,

@@ -250,8 +250,10 @@ __global__ __launch_bounds__(256) void distill_columns_bwd_kernel(const void *lo
 template <int DT>
 static void go_fwd(const void *logits, int64_t ld, const int64_t *ids, const float *teacher, int64_t n, int V, int K,
                    float inv_T, int raw, float *kl, float *state, float *q, hipStream_t st) {
-  hipLaunchKernelGGL(distill_columns_fwd_kernel<DT>, dim3((unsigned)n), dim3(kDistThreads), 0, st, logits, ld, ids,
-                     teacher, V, K, inv_T, raw, kl, state, q);
+  for (int64_t r0 = 0; r0 < n; r0 += kLaunchRows)
+    hipLaunchKernelGGL(distill_columns_fwd_kernel<DT>, dim3((unsigned)(n - r0 < kLaunchRows ? n - r0 : kLaunchRows)),
+                       dim3(kDistThreads), 0, st, (const char *)logits + r0 * ld * Elem<DT>::bytes, ld, ids + r0 * K,
+                       teacher + r0 * K, V, K, inv_T, raw, kl + r0, state + 4 * r0, q + r0 * K);
 }
 
 template <int DT>
@@ -519,8 +521,8 @@ extern "C" {
 int octo_distill_columns_fwd(const void *logits, int64_t ld, int dtype, const int64_t *ids, const float *teacher,
                              int64_t n, int V, int K, float inv_T, int flags, float *kl, float *state, float *q,
                              void *stream) {
-  OCTO_CHECK_ARG(n >= 0 && n <= 0x7fffffff && V > 0 && ld >= V, "distill_columns_fwd: bad shape n=%lld V=%d ld=%lld",
-                 (long long)n, V, (long long)ld);
+  OCTO_CHECK_ARG(n >= 0 && n <= 0x7fffffff && V > 0 && V <= OCTO_ROW_MAX && ld >= V,
+                 "distill_columns_fwd: bad shape n=%lld V=%d ld=%lld", (long long)n, V, (long long)ld);
   OCTO_CHECK_ARG(K >= 1 && K <= OCTO_LIST_MAX, "distill_columns_fwd: K=%d outside [1, %d]", K, OCTO_LIST_MAX);
   OCTO_CHECK_ARG(is_float(dtype), "distill_columns_fwd: dtype %d", dtype);
   OCTO_CHECK_ARG((flags & ~OCTO_LIST_RAW) == 0, "distill_columns_fwd: unknown flags %d", flags);
@@ -540,7 +542,8 @@ int octo_distill_columns_fwd(const void *logits, int64_t ld, int dtype, const in
 int octo_distill_columns_bwd(const void *logits, int64_t ld, int dtype, const int64_t *ids, const float *q, int64_t n,
                              int V, int K, float inv_T, const float *state, const float *g, void *dlogits,
                              int64_t ld_d, void *stream) {
-  OCTO_CHECK_ARG(n >= 0 && n <= 0x7fffffff && V > 0 && ld >= V && ld_d >= V, "distill_columns_bwd: bad shape");
+  OCTO_CHECK_ARG(n >= 0 && n <= 0x7fffffff && V > 0 && V <= OCTO_ROW_MAX && ld >= V && ld_d >= V,
+                 "distill_columns_bwd: bad shape");
   OCTO_CHECK_ARG(K >= 1 && K <= OCTO_LIST_MAX, "distill_columns_bwd: K=%d outside [1, %d]", K, OCTO_LIST_MAX);
   OCTO_CHECK_ARG(is_float(dtype), "distill_columns_bwd: dtype %d", dtype);
   OCTO_CHECK_ARG(inv_T > 0.f, "distill_columns_bwd: temperature must be positive");

@@ -463,11 +463,16 @@ static void go_fwd(const void *w, int64_t ldw, int64_t V, int d, const int64_t *
                    int64_t ldo, hipStream_t st) {
   constexpr int B = Elem<DT>::bytes, PER = 16 / B;
   const bool vec = d % PER == 0 && ldw % PER == 0 && ldo % PER == 0 && (uintptr_t)w % 16 == 0 && (uintptr_t)out % 16 == 0;
-  const dim3 grid((unsigned)cdiv(n, 4), (unsigned)cdiv(d, 64 * kRowLoadsF * PER));
-  if (vec)
-    hipLaunchKernelGGL((embed_fwd_kernel<DT, true>), grid, dim3(256), 0, st, w, ldw, V, d, ids, n, scale, out, ldo);
-  else
-    hipLaunchKernelGGL((embed_fwd_kernel<DT, false>), grid, dim3(256), 0, st, w, ldw, V, d, ids, n, scale, out, ldo);
+  constexpr int64_t kTokens = 4 * kLaunchRows;
+  for (int64_t t0 = 0; t0 < n; t0 += kTokens) {
+    const int64_t m = n - t0 < kTokens ? n - t0 : kTokens;
+    const dim3 grid((unsigned)cdiv(m, 4), (unsigned)cdiv(d, 64 * kRowLoadsF * PER));
+    char *o = (char *)out + t0 * ldo * B;
+    if (vec)
+      hipLaunchKernelGGL((embed_fwd_kernel<DT, true>), grid, dim3(256), 0, st, w, ldw, V, d, ids + t0, m, scale, o, ldo);
+    else
+      hipLaunchKernelGGL((embed_fwd_kernel<DT, false>), grid, dim3(256), 0, st, w, ldw, V, d, ids + t0, m, scale, o, ldo);
+  }
 }
 
 }  // namespace octo
@@ -478,7 +483,7 @@ extern "C" {
 
 int octo_embed_fwd(const void *w, int64_t ldw, int dtype, int64_t V, int d, const int64_t *ids, int64_t n, float scale,
                    void *out, int64_t ldo, void *stream) {
-  OCTO_CHECK_ARG(V > 0 && V < 0x7fffffff && d > 0 && ldw >= d && ldo >= d && n >= 0 && n < 0x7fffffff,
+  OCTO_CHECK_ARG(V > 0 && V <= OCTO_ROW_MAX && d > 0 && ldw >= d && ldo >= d && n >= 0 && n < 0x7fffffff,
                  "embed_fwd: bad shape V=%lld d=%d n=%lld", (long long)V, d, (long long)n);
   if (!is_float(dtype)) return octo_fail(OCTO_EUNSUPPORTED, "embed_fwd: dtype %d", dtype);
   if (n == 0) return OCTO_OK;
@@ -496,7 +501,7 @@ int octo_embed_fwd(const void *w, int64_t ldw, int dtype, int64_t V, int d, cons
 
 int octo_embed_bwd_workspace_bytes(int64_t n, int64_t V, int d, size_t *bytes) {
   OCTO_CHECK_ARG(bytes != nullptr, "embed_bwd_workspace_bytes: null pointer");
-  OCTO_CHECK_ARG(V > 0 && V < 0x7fffffff - kBins && d > 0 && d <= 65535 * kCols && n >= 0 && n <= (int64_t)1 << 30,
+  OCTO_CHECK_ARG(V > 0 && V <= OCTO_ROW_MAX && d > 0 && d <= 65535 * kCols && n >= 0 && n <= (int64_t)1 << 27,
                  "embed_bwd: bad shape V=%lld d=%d n=%lld", (long long)V, d, (long long)n);
   *bytes = embed_ws(n, V, d, nullptr, nullptr);
   return OCTO_OK;
@@ -530,7 +535,7 @@ int octo_embed_bwd(const void *grad, int64_t ldg, int g_dtype, const int64_t *id
   a.ldw = ldw;
   a.accumulate = accumulate != 0;
   a.colblocks = (int)cdiv(d, kCols);
-  OCTO_CHECK_ARG((int64_t)a.pieces * a.colblocks < (int64_t)1 << 30, "embed_bwd: %lld tokens of width %d", (long long)n, d);
+  OCTO_CHECK_ARG((int64_t)a.pieces * a.colblocks < (int64_t)1 << 26, "embed_bwd: %lld tokens of width %d", (long long)n, d);
   ZeroFill z{};
   if (!accumulate) {
     const int esz = float_bytes(w_dtype);

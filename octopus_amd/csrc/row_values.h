@@ -6,6 +6,9 @@
 
 namespace octo {
 
+// Rows per launch of the kernels with a workgroup a row: a launch has fewer than 2^32 threads.
+constexpr int64_t kLaunchRows = 1 << 21;
+
 // 8 consecutive 16-bit values (one 16-byte chunk) as fp32, and back (round to nearest even).
 __device__ __forceinline__ void unpack8(const i32x4 v, bool f16, float (&x)[8]) {
 #pragma unroll

@@ -422,7 +422,8 @@ extern "C" {
 
 int octo_topk_workspace_bytes(int64_t n, int V, int dtype, int k, size_t *bytes) {
   OCTO_CHECK_ARG(bytes != nullptr, "topk_workspace_bytes: null pointer");
-  OCTO_CHECK_ARG(n >= 0 && n <= 0x7fffffff && V > 0, "topk: bad shape n=%lld V=%d", (long long)n, V);
+  OCTO_CHECK_ARG(n >= 0 && n <= 0x7fffffff && V > 0 && V <= OCTO_ROW_MAX, "topk: bad shape n=%lld V=%d", (long long)n,
+                 V);
   OCTO_CHECK_ARG(k >= 1 && k <= V && k <= OCTO_LIST_MAX, "topk: k=%d outside [1, min(V, %d)]", k, OCTO_LIST_MAX);
   OCTO_CHECK_ARG(is_float(dtype), "topk: dtype %d", dtype);
   const int slices = topk_slices(n, V, k, dtype);
@@ -446,7 +447,9 @@ int octo_topk(const void *logits, int64_t ld, int dtype, int64_t n, int V, float
   hipStream_t st = (hipStream_t)stream;
   const int slices = topk_slices(n, V, k, dtype);
   if (slices == 1) {
-    go_topk<false>(logits, ld, dtype, n, V, inv_T, k, ids, logp, 1, 0, nullptr, nullptr, st);
+    for (int64_t r0 = 0; r0 < n; r0 += kLaunchRows)
+      go_topk<false>((const char *)logits + r0 * ld * float_bytes(dtype), ld, dtype, n - r0 < kLaunchRows ? n - r0 : kLaunchRows,
+                     V, inv_T, k, ids + r0 * k, logp + r0 * k, 1, 0, nullptr, nullptr, st);
   } else {
     const int per = (int)round_up(cdiv(V, slices), 64);  // the last slice has the rest, at least one value
     uint64_t *entries = (uint64_t *)ws;

@@ -193,12 +193,17 @@ def distill_columns(logits: Tensor, temperature: float, ids: Tensor, teacher: Te
 
 # ---- the divergence from hidden rows: loss and gradients in one call ------------------------------------------------------
 
+def _apart(x: Tensor) -> Tensor:
+    """x with rows that do not overlap (a broadcast one's are one row)."""
+    return x if _ld(x) >= x.shape[1] else x.contiguous()
+
+
 def _step(rows: Tensor, weight: Tensor, w_scale: Optional[Tensor], ids: Tensor, teacher: Tensor,
           row_weight: Optional[Tensor], idx: Optional[Tensor], count: Optional[Tensor], inv_T: float, pre: float,
           post: float, use_tanh: bool, raw: bool, need_rows: bool, need_weight: bool, kept: Optional[Tensor]):
     """(loss, kl, grad_rows, grad_w) of octo_head_step_distill; kept: the buffer that takes grad_w's operands."""
     dev = _on_gpu(rows, weight, w_scale, ids, teacher, row_weight, idx, count)
-    rows2, weight2, idx = _rows2d(rows), _rows2d(weight), _index(idx)
+    rows2, weight2, idx = _apart(_rows2d(rows)), _apart(_rows2d(weight)), _index(idx)
     ids, teacher = _lists(ids, teacher, rows2.shape[0])
     if rows2.shape[1] != weight2.shape[1]:
         raise ValueError(f"octohead: rows of width {rows2.shape[1]} against a weight of width {weight2.shape[1]}")
@@ -210,6 +215,7 @@ def _step(rows: Tensor, weight: Tensor, w_scale: Optional[Tensor], ids: Tensor, 
         raise ValueError(f"octohead: a row count of int32 expected (compact_rows), got {count.dtype}")
     if w_scale is not None and (w_scale.dtype != torch.float32 or w_scale.shape != weight2.shape[:1]):
         raise ValueError(f"octohead: one fp32 scale per weight row expected, got {w_scale.dtype} {tuple(w_scale.shape)}")
+    w_scale = None if w_scale is None else w_scale.contiguous()
     n_max = idx.numel() if idx is not None else rows2.shape[0]
     V, d = weight2.shape
     K = ids.shape[1]

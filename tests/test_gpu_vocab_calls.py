@@ -274,3 +274,63 @@ def test_far_offsets():
     q = torch.softmax(logp[-2:].double(), 1)
     want = p.scatter_add(1, top[-2:], -q)
     assert ((grad[-2:].double() - want).abs() <= 2 ** -8 * want.abs() + 1e-5 * (p + want.abs())).all()
+
+
+def test_more_rows_than_a_launch_takes():
+    """Rows past 2^21, tokens past 2^23: the last rows of the first launch, and the second's."""
+    from octopus_amd import distill_op, embed_op
+
+    n, V, K = (1 << 21) + 3, 8, 2
+    g = torch.Generator(device="cuda").manual_seed(3)
+    z = torch.randn(n, V, generator=g, device="cuda").bfloat16()
+    ids, logp = distill_op.head_topk(z, 1.0, K)
+    kl = distill_op.distill_columns(z, 0.5, ids, logp)
+    for part in (slice(0, 5), slice((1 << 21) - 4, None)):
+        few, few_logp = distill_op.head_topk(z[part].clone(), 1.0, K)
+        assert torch.equal(ids[part], few) and torch.equal(logp[part], few_logp)
+        assert torch.equal(kl[part], distill_op.distill_columns(z[part].clone(), 0.5, few, few_logp))
+    w = torch.randn(10, 8, generator=g, device="cuda").bfloat16()
+    tokens = torch.randint(0, 10, ((1 << 23) + 5,), generator=g, device="cuda")
+    assert torch.equal(embed_op.embed_rows(w, tokens), w[tokens])
+
+
+def test_a_strided_weight_scale():
+    """fp8 weights whose scales lie apart."""
+    from octopus_amd import distill_op
+
+    n, d, V, K = 5, 64, 200, 4
+    g = torch.Generator(device="cuda").manual_seed(4)
+    h = torch.randn(n, d, generator=g, device="cuda").bfloat16()
+    W = torch.randn(V, d, generator=g, device="cuda").to(torch.float8_e4m3fn)
+    scale = torch.rand(V, 2, generator=g, device="cuda")[:, 0]
+    ids = torch.randint(0, V, (n, K), generator=g, device="cuda")
+    t = torch.randn(n, K, generator=g, device="cuda")
+    got, want = (distill_op.fused_distill_head(h, W, ids, t, 1.0, w_scale=s)[1] for s in (scale, scale.contiguous()))
+    assert torch.equal(got, want)
+
+
+def test_broadcast_inputs():
+    """One hidden row, one row of logits and one weight shared by all: the gradients add up over what shares them."""
+    from octopus_amd import distill_op, embed_op
+
+    n, d, V, K = 6, 64, 200, 4
+    g = torch.Generator(device="cuda").manual_seed(5)
+    ids = torch.randint(0, V, (n, K), generator=g, device="cuda")
+    t = torch.randn(n, K, generator=g, device="cuda")
+    W = torch.randn(V, d, generator=g, device="cuda")
+    h, z = torch.randn(1, d, generator=g, device="cuda"), torch.randn(1, V, generator=g, device="cuda")
+    tokens, up = torch.randint(0, V, (9,), generator=g, device="cuda"), torch.randn(9, d, generator=g, device="cuda")
+
+    def grad(x, f):
+        x = x.clone().requires_grad_(True)
+        f(x).backward()
+        return x.grad
+
+    for x, shape, f in [(h, (n, d), lambda a: distill_op.fused_distill_head(a, W, ids, t, 1.0)[0]),
+                        (z, (n, V), lambda a: distill_op.distill_columns(a, 1.0, ids, t).sum()),
+                        (W[:, :1], (V, d), lambda a: (embed_op.embed_rows(a, tokens) * up).sum())]:
+        shared, each = grad(x, lambda a: f(a.expand(shape))), grad(x.expand(shape).contiguous(), f)
+        each = each.double().sum_to_size(x.shape)
+        # sums of at most 64 fp32 values: 63 roundings of what they add up to at most
+        bound = 64 * 2.0 ** -24 * grad(x.expand(shape).contiguous(), f).abs().double().sum_to_size(x.shape)
+        assert ((shared.double() - each).abs() <= bound).all()

@@ -92,3 +92,15 @@ def test_python_checks_need_no_gpu():
             call()
     with pytest.raises(NotImplementedError):  # the registered ops know HIP tensors only
         distill_op.distill_columns_fwd(z, ids, t, 1.0, False)
+
+
+def test_sizes_past_the_kernels_counts():
+    """Vocabularies and token counts whose places, or launches, would not fit 32 bits."""
+    V, out = (1 << 30) + 1, ctypes.c_size_t(0)
+    _refused("octo_topk", P, V, _lib.BF16, 4, V, 1.0, 5, P, P, None, 0, None)
+    _refused("octo_topk_workspace_bytes", 4, V, _lib.BF16, 5, ctypes.byref(out))
+    _refused("octo_distill_columns_fwd", P, V, _lib.BF16, P, P, 4, V, 5, 1.0, 0, P, P, P, None)
+    _refused("octo_distill_columns_bwd", P, V, _lib.BF16, P, P, 4, V, 5, 1.0, P, P, P, V, None)
+    _refused("octo_embed_fwd", P, 8, _lib.BF16, V, 8, P, 4, 1.0, P, 8, None)
+    for n, v in [((1 << 27) + 1, 10), (4, V)]:
+        _refused("octo_embed_bwd_workspace_bytes", n, v, 8, ctypes.byref(out))
