@@ -424,11 +424,38 @@ __global__ __launch_bounds__(64 * kDistMergeRows) void distill_merge_kernel(Dist
   }
 }
 
-// One wave per row. Slots of one token all write the sum of their weights, taken in the list's order.
+// A workgroup's sum of the loss: every thread's rows in order, in 64 bits, then a tree.
+constexpr int kLossThreads = 256;
+__device__ __forceinline__ void loss_sum(const DistillArgs &a, double *part) {
+  const int64_t cnt = a.count ? min((int64_t)(*a.count), a.n_max) : a.n_max;
+  double s = 0.0;
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < cnt; r += kLossThreads) {
+    const int64_t hrow = a.idx ? a.idx[r] : r;
+    const float wt = a.weight ? a.weight[hrow] : 1.f, kl = a.kl[hrow];
+    s += wt != 0.f ? (double)wt * (double)kl : 0.0;  // a row without weight, whatever its divergence is
+  }
+  part[threadIdx.x] = s;
+  __syncthreads();
+  for (int k = kLossThreads / 2; k > 0; k >>= 1) {
+    if ((int)threadIdx.x < k) part[threadIdx.x] += part[threadIdx.x + k];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *a.loss = (float)part[0];
+}
+
+// One wave per row. Slots of one token all write the sum of their weights, taken in the list's order. The last pass's
+// launch has a workgroup more, the loss's: every row's kl is there by then (a launch of its own: 4 us of a call's 130 at
+// 225 rows, V 32,000).
 constexpr int kEntryRows = 4;
+static_assert(64 * kEntryRows == kLossThreads, "the loss's workgroup");
 __global__ __launch_bounds__(64 * kEntryRows) void distill_entries_kernel(DistillArgs a) {
   __shared__ int64_t slot_id[kEntryRows][OCTO_LIST_MAX];
   __shared__ float slot_q[kEntryRows][OCTO_LIST_MAX];
+  if ((int64_t)blockIdx.x * kEntryRows >= a.rows) {
+    loss_sum(a, (double *)slot_id);
+    return;
+  }
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int64_t i = (int64_t)blockIdx.x * kEntryRows + w, r = a.r0 + i;
   const int64_t cnt = a.count ? min((int64_t)(*a.count), a.n_max) : a.n_max;
@@ -464,23 +491,9 @@ __global__ __launch_bounds__(64 * kEntryRows) void distill_entries_kernel(Distil
   }
 }
 
-// One workgroup: every thread's rows in order, in 64 bits, then a tree.
-__global__ __launch_bounds__(1024) void distill_loss_kernel(DistillArgs a, float *loss) {
-  __shared__ double part[1024];
-  const int64_t cnt = a.count ? min((int64_t)(*a.count), a.n_max) : a.n_max;
-  double s = 0.0;
-  for (int64_t r = threadIdx.x; r < cnt; r += 1024) {
-    const int64_t hrow = a.idx ? a.idx[r] : r;
-    const float wt = a.weight ? a.weight[hrow] : 1.f;
-    if (wt != 0.f) s += (double)wt * (double)a.kl[hrow];  // a row without weight, whatever its divergence is
-  }
-  part[threadIdx.x] = s;
-  __syncthreads();
-  for (int k = 512; k > 0; k >>= 1) {
-    if (threadIdx.x < k) part[threadIdx.x] += part[threadIdx.x + k];
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) *loss = (float)part[0];
+__global__ __launch_bounds__(kLossThreads) void distill_loss_kernel(DistillArgs a) {
+  __shared__ double part[kLossThreads];
+  loss_sum(a, part);
 }
 
 int launch_distill_dots(const DistillArgs &a, hipStream_t st) {
@@ -502,12 +515,15 @@ int launch_distill_merge(const DistillArgs &a, hipStream_t st) {
 }
 int launch_distill_entries(const DistillArgs &a, hipStream_t st) {
   if (a.rows == 0) return OCTO_OK;
-  hipLaunchKernelGGL(distill_entries_kernel, dim3((unsigned)cdiv(a.rows, kEntryRows)), dim3(64 * kEntryRows), 0, st, a);
+  const int64_t blocks = cdiv(a.rows, kEntryRows) + (a.loss ? 1 : 0);
+  hipLaunchKernelGGL(distill_entries_kernel, dim3((unsigned)blocks), dim3(64 * kEntryRows), 0, st, a);
   OCTO_CHECK_LAUNCH("distill_entries");
   return OCTO_OK;
 }
 int launch_distill_loss(const DistillArgs &a, float *loss, hipStream_t st) {
-  hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(1024), 0, st, a, loss);
+  DistillArgs b = a;
+  b.loss = loss;
+  hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(kLossThreads), 0, st, b);
   OCTO_CHECK_LAUNCH("distill_loss");
   return OCTO_OK;
 }

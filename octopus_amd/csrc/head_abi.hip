@@ -768,6 +768,7 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
     }
 
     if (ds) {
+      if (p + 1 == L.passes) da.loss = ds->loss;
       rc = launch_distill_entries(da, st);
       if (rc) return rc;
     }
@@ -811,7 +812,7 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
     if (!rc && need_gh) rc = launch_split_sum(s2, o2, false, st);
     if (rc) return rc;
   }
-  return ds ? launch_distill_loss(da, ds->loss, st) : OCTO_OK;
+  return ds && !grads ? launch_distill_loss(da, ds->loss, st) : OCTO_OK;
 }
 
 // ---- the allocation-free forward (octo_head_fwd_noalloc) ----------------------------------------

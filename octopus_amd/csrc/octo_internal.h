@@ -397,6 +397,7 @@ struct DistillArgs {
   int64_t ldx;
   int64_t v0, cols;
   int rowoff;
+  float *loss;  // the last pass's entries: *loss as launch_distill_loss leaves it; else NULL
 };
 // dots[r][k] = h_r . W_ids[k], fp32 (0 for an empty slot); with xoff != NULL, the row's offset: its largest listed logit +
 // kExAbove (-inf for a row without a slot); flag_cnt[0 .. nflag) = 0.
