@@ -14,8 +14,8 @@
 // Few rows: a row is cut into slices of a workgroup each (topk_slices), whose lists and sums a second launch joins the same
 // way.
 //
-// Bound by memory, 2 bytes a value at 16 bits: [2048, 151,936] bf16 at k 64 131 us (4.8 TB/s; a 4 GiB copy moves 5.0), fp32
-// 214 (5.8).
+// Bound by memory, 2 bytes a value at 16 bits: [2048, 151,936] bf16 at k 64 118 to 131 us (4.8 to 5.3 TB/s; a 4 GiB copy
+// moves 5.0), fp32 214 (5.8).
 #include "octo_common.h"
 #include "row_values.h"
 

@@ -334,3 +334,56 @@ def test_broadcast_inputs():
         # sums of at most 64 fp32 values: 63 roundings of what they add up to at most
         bound = 64 * 2.0 ** -24 * grad(x.expand(shape).contiguous(), f).abs().double().sum_to_size(x.shape)
         assert ((shared.double() - each).abs() <= bound).all()
+
+
+def test_reads_only_what_it_wrote():
+    """Workspaces and outputs full of NaN and -1 beforehand: lists in slices, the divergence, the embedding's sort with
+    tokens left out."""
+    from octopus_amd import distill_op, embed_op
+    from tests.test_gpu_poisoned import poisoned
+
+    z = _r(3, 60001, seed=1)
+    ids = torch.randint(-40, 700, (1501,), generator=torch.Generator().manual_seed(2)).cuda()
+    up = _r(1501, 72, seed=3).bfloat16()
+    into = _r(700, 72, seed=4).bfloat16()
+
+    def run():
+        lists = distill_op.head_topk(z, 0.7, 20)
+        s = z.clone().requires_grad_(True)
+        kl = distill_op.distill_columns(s, 0.7, *lists)
+        dz, = torch.autograd.grad(kl.sum(), s)
+        return (*lists, kl.detach(), dz, embed_op.embed_rows(into, ids), embed_op.embed_bwd(up, ids, 700, 0.5),
+                embed_op.embed_grad_add_(into.clone(), up, ids, padding_idx=7))
+
+    want = run()
+    with poisoned():
+        got = run()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_a_row_taken_twice(dtype):
+    """idx may name a row again (a run, as row lists of a packed stream do): the row counts as often."""
+    from octopus_amd import distill_op
+
+    n, d, V, K = 9, 64, 300, 5
+    h, W = _r(n, d, seed=1).to(dtype), (_r(V, d, seed=2) * 0.3).to(dtype)
+    ids = torch.randint(0, V, (n, K), generator=torch.Generator().manual_seed(3)).cuda()
+    t = _r(n, K, seed=4)
+    idx = torch.tensor([0, 2, 2, 2, 5, 8, 8], device="cuda")
+    times = torch.bincount(idx, minlength=n).float()
+
+    def run(**kw):
+        hd, Wd = h.clone().requires_grad_(True), W.clone().requires_grad_(True)
+        loss, kl = distill_op.fused_distill_head(hd, Wd, ids, t, 1.0, **kw)
+        loss.backward()
+        return loss.detach(), kl, hd.grad, Wd.grad
+
+    got, want = run(idx=idx), run(row_weight=times)
+    assert abs(got[0] - want[0]) <= 2.0 ** -22 * want[0]  # fp32 of a sum in 64 bits of kl's own bits
+    assert torch.equal(got[1], want[1] * (times > 0))
+    # bf16 and f16: both sides round the stored exponential and the result, and h^T with a scale of their own: four
+    # roundings of half a unit that are not shared; fp32: products of 300 and 9 terms in other orders
+    half = 300 * 2.0 ** -24 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    for a, b in zip(got[2:], want[2:]):
+        assert (a.double() - b.double()).norm() <= 4 * half * b.double().norm()
