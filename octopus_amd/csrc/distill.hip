@@ -415,11 +415,59 @@ __global__ __launch_bounds__(64 * kDistMergeRows) void distill_merge_kernel(Dist
   a.lse[2 * r + 1] = l2S;
   if (a.rowoff) {
     const float xo = a.xoff[r];
-    if (st.m - xo <= kExClamp) {
-      a.xuse[i] = xo;
-    } else {  // the offset lies too low, or there is none; a row without weight needs no rescale, its scale is 0
-      a.xuse[i] = st.m;
-      if (g != 0.f) a.flag_rows[atomicAdd(a.flag_cnt, 1)] = (int32_t)i;
+    const bool low = !(st.m - xo <= kExClamp);  // the offset lies too low, or there is none
+    float xn = low ? st.m : xo;
+    if (a.even) {  // the dz scale |g| gmul exp2(xn - m2 - l2S) a power of two (not of a weight of 0 or inf)
+      const float ls = flog2(fabsf(g) * a.gmul) + (xn - st.m - l2S);
+      if (fabsf(ls) < 1024.f) xn += rintf(ls) - ls;
+    } else if (low && g != 0.f) {  // a row without weight needs no rescale, its scale is 0
+      a.flag_rows[atomicAdd(a.flag_cnt, 1)] = (int32_t)i;
+    }
+    a.xuse[i] = xn;
+  }
+}
+
+// Every row's exponentials from the offset they were stored at to xuse, and its dz scale: launch_ex_fix's work for all rows,
+// where grad_W is asked for. h^T times the row's scale is rounded to bf16 there; at a scale of 2^k (1 + 2^-17 or so, from
+// xuse's own rounding) that product is h's own bits, and what is rounded a second time are the dense entries, small beside the
+// listed ones (at V 151,936 and K 64 one part in 50 of the row's norm): grad_W's error falls from 2.9e-3 to 2.35e-3 (one
+// rounding of the result alone is 1.7e-3). Bound by memory, 4 bytes an element: [8,192, 151,936] 752 us (6.6 TB/s), 5% of
+// the call.
+constexpr int kEvenChunks = 2;  // 16-byte chunks per thread
+__global__ __launch_bounds__(256) void distill_even_kernel(DistillArgs a, float *scale) {
+  const int64_t cnt = a.count ? min((int64_t)(*a.count), a.n_max) : a.n_max;
+  const int64_t chunk0 = (int64_t)blockIdx.x * (256 * kEvenChunks) + threadIdx.x;
+  for (int64_t i = blockIdx.y; i < a.rows; i += gridDim.y) {
+    const int64_t r = a.r0 + i;
+    const bool in = r < cnt;
+    const float g = in ? a.g[r] : 0.f;
+    if (g == 0.f) {  // also past the count: the scale of 0 leaves the row out
+      if (blockIdx.x == 0 && threadIdx.x == 0) scale[i] = 0.f;
+      continue;
+    }
+    const float xo = a.xoff[r], xn = a.xuse[i];
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+      scale[i] = -(g * a.gmul) * fexp2(xn - a.lse[2 * r] - a.lse[2 * r + 1]);
+    const f32x4 *pr = a.part + i * a.mtiles;
+    __bf16 *row = (__bf16 *)a.dz + i * a.ldx;
+    i32x4 v[kEvenChunks];
+#pragma unroll
+    for (int u = 0; u < kEvenChunks; ++u) {
+      const int64_t c0 = (chunk0 + 256 * u) * 8;
+      if (c0 < a.ldx) v[u] = __builtin_nontemporal_load((const i32x4 *)(row + c0));
+    }
+#pragma unroll
+    for (int u = 0; u < kEvenChunks; ++u) {
+      const int64_t c0 = (chunk0 + 256 * u) * 8;
+      if (c0 >= a.ldx) continue;
+      const f32x4 q = pr[c0 >> 8];  // 8 columns never straddle a 128-column half tile
+      const float mh = (c0 & 128) ? q[3] : q[0];  // -inf: no column of the half lies below V (stored zeros)
+      const float fac = mh == -INFINITY ? 0.f : fexp2(mh - xn - fminf(mh - xo, kExClamp));
+      float x[8];
+      unpack8(v[u], false, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= fac;
+      __builtin_nontemporal_store(pack8(x, false), (i32x4 *)(row + c0));
     }
   }
 }
@@ -511,6 +559,14 @@ int launch_distill_merge(const DistillArgs &a, hipStream_t st) {
   hipLaunchKernelGGL(distill_merge_kernel, dim3((unsigned)cdiv(a.rows, kDistMergeRows)), dim3(64 * kDistMergeRows), 0,
                      st, a);
   OCTO_CHECK_LAUNCH("distill_merge");
+  return OCTO_OK;
+}
+int launch_distill_even(const DistillArgs &a, float *scale, hipStream_t st) {
+  if (a.rows == 0) return OCTO_OK;
+  OCTO_CHECK_ARG(a.ldx % 256 == 0 && (uintptr_t)a.dz % 16 == 0, "distill_even: rows of whole 256-column tiles");
+  const dim3 g((unsigned)cdiv(a.ldx / 8, 256 * kEvenChunks), (unsigned)(a.rows < 65535 ? a.rows : 65535));
+  hipLaunchKernelGGL(distill_even_kernel, g, dim3(256), 0, st, a, scale);
+  OCTO_CHECK_LAUNCH("distill_even");
   return OCTO_OK;
 }
 int launch_distill_entries(const DistillArgs &a, hipStream_t st) {

@@ -576,7 +576,9 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
   }
   // bf16 operands: the exponentials are stored relative to per-row offsets (StatsArgs::xoff), so dz is one scale per
   // row times the stored value: grad_h takes the scale in its store, grad_W through the scaled h^T, and no pass of its
-  // own turns the exponentials into dz. f16 (5 exponent bits) keeps the half-tile form and launch_dz_scale.
+  // own turns the exponentials into dz. f16 (5 exponent bits) keeps the half-tile form and launch_dz_scale. The
+  // distillation step, whose listed entries are most of a row's gradient and known exactly, takes a pass that makes the
+  // scale a power of two where grad_W is asked for (launch_distill_even).
   const bool rowoff = grads && cm.dt == OCTO_BF16 && cm.c > 0.f;
   float *xoff = (float *)(wsb + L.xoff), *tdot = (float *)(wsb + L.tdot);
   float *xuse = (float *)(wsb + L.xuse), *rscale = (float *)(wsb + L.scale);
@@ -595,6 +597,7 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
     da.ldx = L.V_pad;
     da.cols = V;
     da.rowoff = rowoff;
+    da.even = rowoff && (need_gw || later);
     rc = launch_distill_dots(da, st);
     if (rc) return rc;
   } else if (rowoff) {
@@ -710,7 +713,10 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
     }
     if (!grads) continue;
 
-    if (rowoff) {  // the rows' dz scales, and any flagged row's exponentials rescaled
+    if (rowoff && da.even) {
+      TimedLaunch t("distill_even", st);
+      rc = launch_distill_even(da, rscale, st);
+    } else if (rowoff) {  // the rows' dz scales, and any flagged row's exponentials rescaled
       ExFixArgs fx{};
       fx.ex = dz;
       fx.ldx = L.V_pad;
@@ -738,7 +744,6 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
         TimedLaunch t("ex_fix", st);
         rc = launch_ex_fix(fx, st);
       }
-      if (rc) return rc;
     } else {
       DzScaleArgs sa;
       sa.dz = dz;
@@ -764,8 +769,8 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
         TimedLaunch t("dz_scale", st);
         rc = launch_dz_scale(sa, st);
       }
-      if (rc) return rc;
     }
+    if (rc) return rc;
 
     if (ds) {
       if (p + 1 == L.passes) da.loss = ds->loss;

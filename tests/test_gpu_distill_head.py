@@ -3,14 +3,14 @@
 Bounds, per element. A logit is a sum of d products in fp32: off by at most (d / 8 + 16) 2^-24 sum |h w| (a matrix
 instruction adds blocks of products; the dot products of the lists add d / 64 per lane and a tree). e_z is that over T, at
 most twice in a divergence: 2 e_z + 4e-5 Q (the bound of distill_columns) + 2^-21 sum q |log q - log p|.
-dz is rounded once to the operands' type, relative to itself (bf16 2^-8 with the fp32 scale's part: 1.05 x 2^-8; f16
-2^-11, twice, and 2^-25 of the half tile's largest where it is subnormal; bf16 exponentials are stored against an offset
+dz is rounded once to the operands' type, relative to itself (bf16 2^-8 with the fp32 scale's part: 1.05 x 2^-8, and the
+dense values a second time where grad_W is asked for, moved to a row scale that is a power of two; f16 2^-11, twice, and 2^-25 of the half tile's largest where it is subnormal; bf16 exponentials are stored against an offset
 at most 48 bits above the row's maximum, so that what lies below 2^-126 of the offset, p below 2^-78, may be lost; in a row
 that is rescaled a half tile's factor is exp2(m_h - m2 - 64), 0 below 2^-126, so that a half tile whose maximum lies more
 than 62 bits below the row's is lost: 2^-62 g per element), and its p is off by 2 e_z + 2^-14 relative.
 fp32 operands (2^-24, by products of three-part values) take the same bounds.
-grad_h = dz W takes those through |W|; grad_W = dz^T h through |h|, whose scaled copy is rounded once more (bf16). Both
-are rounded once to their type, and summed in fp32 over up to V or n terms: 2^-14 of the magnitudes' sum."""
+grad_h = dz W takes those through |W|; grad_W = dz^T h through |h|, whose scaled copy is h itself at such a scale (the
+bound's second r |dz| covers one where it is not). Both are rounded once to their type, and summed in fp32 over up to V or n terms: 2^-14 of the magnitudes' sum."""
 
 import math
 
@@ -97,7 +97,7 @@ def _check(h, w, ids, t, rw, T=1.0, post=(1.0, 1.0, False), scored=None, w_scale
     dz, dz_err = dz * c, dz_err * abs(c)
     r = HALF[dtype] * 1.05
     floor = 2 ** -24 * max(1.0, abs(c)) if dtype == torch.float16 else 0.0
-    per = dz_err + (r if dtype == torch.bfloat16 else 2 * r) * dz.abs() + floor
+    per = dz_err + (r if dtype == torch.bfloat16 and q8 is not None else 2 * r) * dz.abs() + floor
     wa, ha = w.double().abs(), h.double().abs()
     gh = dz @ w.double()
     tol = per @ wa + 2 ** -14 * (dz.abs() @ wa) + 2 * r * gh.abs() + floor  # rounded, scaled by c and rounded again
@@ -235,6 +235,30 @@ def test_weight_gradient_made_in_the_backward():
         assert torch.equal(a, b)
         # the same dz and h^T; grad_h the same sums (split differently), each rounded once or twice
         assert (a.float() - 0.5 * c.float()).norm() <= 2 ** -8 * 0.5 * c.float().norm()
+
+
+@pytest.mark.parametrize("later", [False, True])
+def test_the_weight_gradients_roundings(later, monkeypatch):
+    """grad_W of bf16 operands takes two roundings to 16 bits, the listed values' and the result's (their dense neighbours,
+    rounded once more, are a hundredth of the norm here: q about 1/64 against p about 1/8192). Independent roundings of one
+    size add in squares: below sqrt(2.5) times the one that the exact gradient's own rounding costs, between two and three."""
+    from octopus_amd import distill_op, head_op
+
+    n, d, V, K = 300, 256, 8192, 64
+    g = torch.Generator().manual_seed(21)
+    h, w = torch.randn(n, d, generator=g).to(torch.bfloat16), (torch.randn(V, d, generator=g) * 0.02).to(torch.bfloat16)
+    ids, t = torch.randint(0, V, (n, K), generator=g), torch.randn(n, K, generator=g)
+    rw = torch.rand(n, generator=g) + 0.5
+    monkeypatch.setattr(head_op, "_LATER_SHARE", 1 << 20)
+    monkeypatch.setattr(head_op, "_LATER_WEIGHTS", 0 if later else 1 << 62)
+    monkeypatch.setattr(head_op, "_LATER_WORK", 1 << 62)
+    hd, wd = h.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    assert (distill_op._later_bytes(hd, wd, None, True, True) > 0) == later
+    distill_op.fused_distill_head(hd, wd, ids.cuda(), t.cuda(), 1.0, rw.cuda())[0].backward()
+    dz = odist.divergence(h.double() @ w.double().T, ids, t)[1] * rw.double()[:, None]
+    for got, want in [(wd.grad, dz.T @ h.double()), (hd.grad, dz @ w.double())]:
+        once = (want.to(torch.bfloat16).double() - want).norm()
+        assert (got.cpu().double() - want).norm() <= 2.5 ** 0.5 * once
 
 
 def test_gradient_against_differences():
