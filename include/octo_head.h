@@ -96,7 +96,7 @@ const char *octo_last_error(void);
 /* Kernel timing hook (no counterpart in the reference: a measurement aid for benchmarks). While enabled,
  * every GEMM launch of octo_head_fwd / octo_head_bwd / octo_head_step_grpo is bracketed by HIP events on its
  * stream, under the names "gemm_stats", "gemm_dz", "gemm_store_grad_h" and "gemm_store_grad_w" (and the step's
- * "gemm_grads", "ex_fix" and, for f16 operands, "dz_scale"). octo_timing_read waits for
+ * "gemm_grads", "ex_fix" (distillation: "distill_even") and, for f16 operands, "dz_scale"). octo_timing_read waits for
  * the recorded launches of one name and returns their count and summed duration. octo_timing_enable
  * (either value) discards what was recorded. Off by default; enabling it creates events (allocates). */
 int octo_timing_enable(int on);
