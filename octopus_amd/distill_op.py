@@ -25,7 +25,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib, head_op
-from .embed_op import _call_on, _float_rows, _ids, _ld, _on_gpu, _op
+from .embed_op import _call_on, _float_rows, _ids, _ld, _on_gpu
 from .head_op import (_DT, Post, _dtype_code, _empty, _gather_flag, _index, _later_bytes, _p, _rows2d,
                       _workspace, _zeros, later_grad_w, scaled)
 
