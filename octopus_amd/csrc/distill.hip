@@ -417,8 +417,8 @@ __global__ __launch_bounds__(64 * kDistMergeRows) void distill_merge_kernel(Dist
     const float xo = a.xoff[r];
     const bool low = !(st.m - xo <= kExClamp);  // the offset lies too low, or there is none
     float xn = low ? st.m : xo;
-    if (a.even) {  // the dz scale |g| gmul exp2(xn - m2 - l2S) a power of two (not of a weight of 0 or inf)
-      const float ls = flog2(fabsf(g) * a.gmul) + (xn - st.m - l2S);
+    if (a.even) {  // the dz scale |g gmul| exp2(xn - m2 - l2S) a power of two (not of a weight of 0 or inf)
+      const float ls = flog2(fabsf(g * a.gmul)) + (xn - st.m - l2S);  // gmul < 0: a soft-cap with pre < 0
       if (fabsf(ls) < 1024.f) xn += rintf(ls) - ls;
     } else if (low && g != 0.f) {  // a row without weight needs no rescale, its scale is 0
       a.flag_rows[atomicAdd(a.flag_cnt, 1)] = (int32_t)i;
