@@ -149,11 +149,20 @@ def _columns_setup(ctx, inputs, output):
     logits, ids, _teacher, inv_T, _raw = inputs
     ctx.save_for_backward(logits, ids, output[1], output[2])
     ctx.inv_T = inv_T
+    ctx.set_materialize_grads(False)
 
 
-def _columns_backward(ctx, gkl, _gstate, _gq):
+def _only(name: str, *others: Optional[Tensor]) -> None:
+    """Gradients of an op's outputs beside the differentiable one: none may have come in."""
+    if any(g is not None for g in others):
+        raise RuntimeError(f"octohead: of this op's outputs only {name} is differentiable")
+
+
+def _columns_backward(ctx, gkl, gstate, gq):
+    _only("kl", gstate, gq)
     logits, ids, state, q = ctx.saved_tensors
-    dz = distill_columns_bwd(logits, ids, q, ctx.inv_T, state, gkl) if ctx.needs_input_grad[0] else None
+    dz = distill_columns_bwd(logits, ids, q, ctx.inv_T, state, gkl) \
+        if ctx.needs_input_grad[0] and gkl is not None else None
     return dz, None, None, None, None
 
 
@@ -282,7 +291,8 @@ def _step_setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
 
 
-def _step_backward(ctx, gloss, _gkl, _ggr, _ggw):
+def _step_backward(ctx, gloss, gkl, ggr, ggw):
+    _only("loss", gkl, ggr, ggw)
     # into tensors of their own: the op's outputs are its caller's, and a retained graph's second backward reads them
     wanted = [t if ctx.need[k] and ctx.needs_input_grad[k] else None for k, t in enumerate(ctx.grads)]
     out = [None if t is None else torch.zeros_like(t) if gloss is None else scaled(t, gloss) for t in wanted]

@@ -36,3 +36,53 @@ def test_a_soft_cap_of_negative_slope_keeps_the_roundings(later, monkeypatch):
     for got, want in [(wd.grad, dz.T @ h.double()), (hd.grad, dz @ w.double())]:
         once = (want.to(torch.bfloat16).double() - want).norm()
         assert (got.cpu().double() - want).norm() <= 2.5 ** 0.5 * once
+
+
+def _small(n=6, d=64, V=300, K=5, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(n, d, generator=g).to(torch.bfloat16).cuda().requires_grad_(True)
+    w = (torch.randn(V, d, generator=g) * 0.2).to(torch.bfloat16).cuda().requires_grad_(True)
+    return h, w, torch.randint(0, V, (n, K), generator=g).cuda(), torch.randn(n, K, generator=g).cuda()
+
+
+def test_only_one_output_of_the_registered_ops_is_differentiable():
+    """A loss of the step's divergences or gradients, or of the divergence's state, raises: a gradient of zeros, or one
+    without that part, would be silently wrong."""
+    from octopus_amd import distill_op
+
+    h, w, ids, t = _small()
+    step = lambda: distill_op.head_step_distill(h, w, None, ids, t, None, None, None, 1.0, 1.0, 1.0, False, False,  # noqa
+                                                True, True)
+    loss, kl, gh, gw = step()
+    for out in (kl.sum(), gh.float().sum(), gw.float().sum(), loss + kl.sum()):
+        with pytest.raises(RuntimeError, match="only loss"):
+            torch.autograd.grad(out, (h, w), retain_graph=True)
+    a = torch.autograd.grad(loss, (h, w))
+    assert torch.equal(a[0], gh) and torch.equal(a[1], gw)
+    z = torch.randn(6, 300, generator=torch.Generator().manual_seed(1)).cuda().requires_grad_(True)
+    kl, state, q = distill_op.distill_columns_fwd(z, ids, t, 1.0, False)
+    for out in (state.sum(), q.sum(), kl.sum() + q.sum()):
+        with pytest.raises(RuntimeError, match="only kl"):
+            torch.autograd.grad(out, z, retain_graph=True)
+    (a,) = torch.autograd.grad(kl.sum(), z)
+    (b,) = torch.autograd.grad(distill_op.distill_columns(z, 1.0, ids, t).sum(), z)
+    assert torch.equal(a, b)
+
+
+def test_traced_steps():
+    """Through a tracer: the loss's gradients are the eager call's, the divergences come detached."""
+    from octopus_amd import distill_op
+
+    h, w, ids, t = _small(seed=2)
+
+    def step(h, w):
+        loss, kl = distill_op.fused_distill_head(h, w, ids, t, 1.0)
+        return loss, kl, distill_op.distill_columns((h @ w.T).float(), 1.0, ids, t)
+
+    def all_of(f):
+        loss, kl, cols = f(h, w)
+        assert not kl.requires_grad
+        return (loss.detach(), kl, cols.detach(), *torch.autograd.grad(3 * loss + cols.sum(), (h, w)))
+
+    got = all_of(torch.compile(step, backend="aot_eager", fullgraph=True))
+    assert all(torch.equal(a, b) for a, b in zip(got, all_of(step)))
