@@ -143,10 +143,12 @@ def _setup(ctx, inputs, output):
     ctx.params = (weight.shape[0], scale, padding_idx, weight.dtype)
 
 
-def _backward(ctx, gout):
+def _backward(ctx, gout, gradient=_embed_bwd):
+    """The registered op's own backward calls the registered gradient: a tracer runs it on tensors without data, and with
+    create_graph its result depends on gout, whose derivative is refused and not left out."""
     (ids,) = ctx.saved_tensors
     V, scale, padding_idx, dtype = ctx.params
-    gw = _op(_embed_bwd, _gradient)(gout, ids, V, scale, padding_idx, dtype) if ctx.needs_input_grad[0] else None
+    gw = gradient(gout, ids, V, scale, padding_idx, dtype) if ctx.needs_input_grad[0] else None
     return gw, None, None, None
 
 
@@ -165,7 +167,7 @@ class _Embed(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        return _backward(ctx, gout)
+        return _backward(ctx, gout, _gradient)
 
 
 def _padding(padding_idx: Optional[int], V: int) -> int:

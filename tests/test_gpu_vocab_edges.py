@@ -86,3 +86,24 @@ def test_traced_steps():
 
     got = all_of(torch.compile(step, backend="aot_eager", fullgraph=True))
     assert all(torch.equal(a, b) for a, b in zip(got, all_of(step)))
+
+
+def test_a_traced_lookup_and_its_second_derivative():
+    """embed_rows through a tracer has the eager call's gradient; the registered op's gradient, differentiated again, raises
+    also as part of a larger expression."""
+    from octopus_amd import embed_op
+
+    ids = torch.tensor([[3, 0, 3], [7, -1, 9]], device="cuda")
+    w = torch.randn(9, 16, generator=torch.Generator().manual_seed(3)).cuda().requires_grad_(True)
+    up = torch.randn(2, 3, 16, generator=torch.Generator().manual_seed(4)).cuda().requires_grad_(True)
+    step = lambda w: embed_op.embed_rows(w, ids, 1.5, padding_idx=7)  # noqa: E731
+    out = torch.compile(step, backend="aot_eager", fullgraph=True)(w)
+    assert torch.equal(out, step(w))
+    (a,) = torch.autograd.grad(out, w, up.detach())
+    (b,) = torch.autograd.grad(step(w), w, up.detach())
+    assert torch.equal(a, b)
+    for f in (embed_op.embed_fwd, lambda *x: embed_op.embed_rows(*x)):
+        (g,) = torch.autograd.grad(f(w, ids, 1.5, 7), w, up, create_graph=True)
+        assert torch.equal(g, a)
+        with pytest.raises(RuntimeError):
+            (up.pow(2).sum() + g.pow(2).sum()).backward()
