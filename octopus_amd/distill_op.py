@@ -22,7 +22,6 @@ from typing import Optional
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _lib, head_op
 from .embed_op import _call_on, _float_rows, _ids, _ld, _on_gpu
@@ -171,7 +170,8 @@ torch.library.register_autograd("octohead::distill_columns_fwd", _columns_backwa
 
 class _Columns(torch.autograd.Function):
     """distill_columns_fwd and its backward outside a trace, without the registered ops' own bookkeeping on the host (57
-    rows of 128,257: 98 us a forward and backward through the ops)."""
+    rows of 128,257: 98 us a forward and backward through the ops). With create_graph the backward is the registered op,
+    which ties the gradient to the logits it depends on and refuses its derivative."""
 
     @staticmethod
     def forward(ctx, *args):
@@ -181,9 +181,10 @@ class _Columns(torch.autograd.Function):
         return kl
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gkl):
         z, ids, state, q = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            return (distill_columns_bwd(z, ids, q, ctx.inv_T, state, gkl),) + (None,) * 4
         return (_columns_grad(z, ids, q, ctx.inv_T, state, gkl),) + (None,) * 4
 
 
@@ -194,7 +195,8 @@ def distill_columns(logits: Tensor, temperature: float, ids: Tensor, teacher: Te
     log-probabilities whose missing rest is to carry no weight."""
     if logits.dim() != 2:
         raise ValueError(f"octohead: logits must be [n, V], got {tuple(logits.shape)}")
-    args = (logits, ids, teacher.detach(), _inv_T(temperature), not normalise)
+    # rows the kernels can read from here on, so that what the backward saves is the tensor that autograd knows
+    args = (_float_rows(logits, "logits"), ids, teacher.detach(), _inv_T(temperature), not normalise)
     if torch.compiler.is_compiling():
         return distill_columns_fwd(*args)[0]
     return _Columns.apply(*args) if torch.is_grad_enabled() and logits.requires_grad else _columns_fwd(*args)[0]
@@ -284,10 +286,30 @@ def _(rows, weight, w_scale, ids, teacher, row_weight, idx, count, inv_T, pre, p
             _empty(rows) if need_rows else rows.new_empty(0), _empty(weight) if need_weight else weight.new_empty(0))
 
 
+class _Final(torch.autograd.Function):
+    """A gradient, tied to the tensors it depends on: differentiated, it raises, and is never a silent constant."""
+
+    @staticmethod
+    def forward(ctx, grad, *of):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError("octohead: the gradients of the distillation step have no derivative of their own")
+
+
+def _final(grads, *of: Optional[Tensor]) -> tuple:
+    """The step's gradients as a backward returns them; of: what they depend on."""
+    of = [t for t in of if t is not None and t.requires_grad]
+    if not (torch.is_grad_enabled() and of):  # no create_graph
+        return tuple(grads)
+    return tuple(None if t is None else _Final.apply(t.detach(), *of) for t in grads)
+
+
 def _step_setup(ctx, inputs, output):
     # held as detached aliases, not saved: an offload's pack hook never copies the [V, d] gradient to the host
     ctx.grads = (output[2].detach(), output[3].detach())
-    ctx.need = inputs[-2:]
+    ctx.need, ctx.of = inputs[-2:], inputs[:2]
     ctx.set_materialize_grads(False)
 
 
@@ -296,7 +318,7 @@ def _step_backward(ctx, gloss, gkl, ggr, ggw):
     # into tensors of their own: the op's outputs are its caller's, and a retained graph's second backward reads them
     wanted = [t if ctx.need[k] and ctx.needs_input_grad[k] else None for k, t in enumerate(ctx.grads)]
     out = [None if t is None else torch.zeros_like(t) if gloss is None else scaled(t, gloss) for t in wanted]
-    return (*out,) + (None,) * 13
+    return _final(out, *ctx.of, gloss) + (None,) * 13
 
 
 torch.library.register_autograd("octohead::head_step_distill", _step_backward, setup_context=_step_setup)
@@ -320,7 +342,7 @@ def _later_setup(ctx, inputs, output):
     rows, weight, idx = inputs[0], inputs[1], inputs[5]
     ctx.held = (output[2].detach(), output[3].detach(), output[4].detach())
     ctx.sizes = (idx.numel() if idx is not None else rows.shape[0], weight.shape[1], weight.shape[0], weight.dtype)
-    ctx.need_rows = inputs[-2]
+    ctx.need_rows, ctx.of = inputs[-2], inputs[:2]
     ctx.set_materialize_grads(False)
 
 
@@ -333,7 +355,7 @@ def _later_backward(ctx, gloss):
     if ctx.needs_input_grad[1]:
         gw = torch.zeros(V, d, dtype=dtype, device=kept.device) if gloss is None \
             else later_grad_w(kept, count, gloss, n_max, d, V, dtype, ctx.need_rows)
-    return gr, gw
+    return _final((gr, gw), *ctx.of, gloss)
 
 
 class _Head(torch.autograd.Function):
@@ -350,13 +372,12 @@ class _Head(torch.autograd.Function):
             _later_setup(ctx, inputs, output)
         else:
             output = _step(rows, weight, w_scale, ids, teacher, row_weight, idx, count, *xf, need_rows, need_weight, None)
-            ctx.grads, ctx.need = output[2:], (need_rows, need_weight)
+            ctx.grads, ctx.need, ctx.of = output[2:], (need_rows, need_weight), (rows, weight)
             ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(output[1])
         return output[0], output[1]
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gloss, gkl):
         if ctx.later:
             return _later_backward(ctx, gloss) + (None,) * 10
@@ -365,7 +386,7 @@ class _Head(torch.autograd.Function):
                                "retain_graph=True keeps them for another")
         if torch._C._autograd._get_current_graph_task_keep_graph() or gloss is None:
             return _step_backward(ctx, gloss, None, None, None)[:2] + (None,) * 10
-        held, ctx.grads = ctx.grads, None
+        held, ctx.grads, ctx.of = ctx.grads, None, ()
         c = gloss.float().contiguous()
         out = [t if ctx.need[k] and ctx.needs_input_grad[k] else None for k, t in enumerate(held)]
         for t in out:
@@ -386,7 +407,8 @@ def fused_distill_head(rows: Tensor, weight: Tensor, ids: Tensor, teacher: Tenso
     weight 0 adds nothing to the loss, but is computed with: leave rows out by idx. bf16, f16, fp32 and fp8 weights
     (w_scale; no gradient of those).
     The prefix tree's teacher values depend on the path alone, so a tree's rows are its positions, each once, weighted by
-    the tokens that share it. The gradients or operands are held from this call until the graph goes."""
+    the tokens that share it. The gradients or operands, and rows and weight by
+    reference, are held from this call until the graph goes. The gradients have no derivative of their own: one raises."""
     inv_T = _inv_T(temperature)
     if rows.dim() != 2 or weight.dim() != 2:
         raise ValueError(f"octohead: rows [n, d] and weight [V, d] expected, got {tuple(rows.shape)} and "

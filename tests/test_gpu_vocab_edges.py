@@ -107,3 +107,41 @@ def test_a_traced_lookup_and_its_second_derivative():
         assert torch.equal(g, a)
         with pytest.raises(RuntimeError):
             (up.pow(2).sum() + g.pow(2).sum()).backward()
+
+
+@pytest.mark.parametrize("form", ["step", "later", "registered", "columns", "columns_apart", "registered_columns"])
+def test_second_derivatives_inside_a_larger_expression(form, monkeypatch):
+    """A penalty on the gradient beside a term that has a derivative: the penalty's own raises by every way that asks for
+    it, where a constant in its place would leave it out without a word. The first derivatives are the plain ones."""
+    from octopus_amd import distill_op, head_op
+
+    h, w, ids, t = _small(seed=5)
+    rw = torch.rand(6, generator=torch.Generator().manual_seed(6)).cuda()
+    monkeypatch.setattr(head_op, "_LATER_SHARE", 1 << 20)
+    monkeypatch.setattr(head_op, "_LATER_WEIGHTS", 0 if form == "later" else 1 << 62)
+    monkeypatch.setattr(head_op, "_LATER_WORK", 1 << 62)
+    if "columns" in form:
+        base = torch.randn(300, 6, generator=torch.Generator().manual_seed(7)).cuda() if form == "columns_apart" else None
+        x = (torch.randn(6, 300, generator=torch.Generator().manual_seed(7)).cuda() if base is None else base.T)
+        leaves = (x.detach().requires_grad_(True),)
+        call = distill_op.distill_columns_fwd if form == "registered_columns" else None
+        f = lambda: (call(leaves[0], ids, t, 1.0, False)[0] if call  # noqa: E731
+                     else distill_op.distill_columns(leaves[0], 1.0, ids, t)).sum()
+    else:
+        leaves = (h, w)
+        args = (h, w, None, ids, t, rw, None, None, 1.0, 1.0, 1.0, False, False, True, True)
+        f = lambda: (distill_op.head_step_distill(*args) if form == "registered"  # noqa: E731
+                     else distill_op.fused_distill_head(h, w, ids, t, 1.0, rw))[0]
+    want = torch.autograd.grad(f(), leaves)
+
+    def penalised():
+        loss = f()
+        grads = torch.autograd.grad(loss, leaves, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(grads, want))
+        return loss + sum(g.float().pow(2).sum() for g in grads) + sum(x.float().sum() for x in leaves)
+
+    with pytest.raises(RuntimeError):
+        penalised().backward()
+    for x in leaves:
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(penalised(), x)
