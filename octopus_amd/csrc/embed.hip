@@ -17,7 +17,7 @@
 //          grad_W, that of an entry that crosses a piece's border to the piece's two fp32 partial rows (its first and
 //          its last entry). Frequent tokens are so shared out evenly.
 //   join   a workgroup per piece in which a crossing entry starts: its partial rows summed in order.
-// 32,768 tokens of text, d 2560, V 151,936, bf16: 209 us (0.95 GB at 4.5 TB/s: sort and zeros 120, sum 75, of which half is
+// 32,768 tokens of text, d 2560, V 151,936, bf16: 207 us (0.95 GB at 4.6 TB/s: sort and zeros 115, sum 75, of which half is
 // the zeros' way out of the caches, join 13); added in place 80 (sort 18, sum 27 to 50). One entry alone: 112 in place.
 #include "octo_common.h"
 #include "row_values.h"
@@ -78,30 +78,33 @@ struct SortOut {
 
 constexpr int kSortWaves = 16, kSortLoads = 8;
 constexpr int kListed = 1024;  // tokens of its range that a wave notes on its first sweep
+// The zeros: `rows` runs of `bytes` bytes, `stride` apart. A gradient without gaps is one run.
 struct ZeroFill {
-  char *at;        // the gradient's rows
-  int64_t stride;  // bytes between them
-  int64_t bytes;   // of one
-  int64_t rows;
-  int whole;       // rows of whole, aligned 16-byte chunks
-  int flat;        // and no gap between them: `bytes` of them all
+  char *at;
+  int64_t stride, bytes, rows;
   int blocks;
 };
+// A workgroup's first kZeroThreads threads write kZeroTurns chunks each: memory takes stores best from few waves at a time
+// that move through it as one front. us of an fp32 gradient of 8 tokens, [151,936, 2560] and [151,935, 2559], and a bf16 one
+// of 1,501 tokens, [32,000, 1024]: 242, 246, 26; one turn 230, 233, 28; all 1,024 threads, one turn 255, 258, 27, four turns
+// 274, .., 26 (a fill and an index_add_: 262, 261, 91).
+constexpr int kZeroThreads = 512, kZeroTurns = 2;
+// Thread t of T: the 16-byte chunks t, t + T, .. of the run at p, and the 2-byte values before the first and after the last.
+__device__ __forceinline__ void zero_run(char *p, int64_t bytes, int64_t t, int64_t T) {
+  const int64_t head = min(bytes, (int64_t)((16 - ((uintptr_t)p & 15)) & 15)), chunks = (bytes - head) / 16;
+  for (int64_t k = t; k < chunks; k += T) ((i32x4 *)(p + head))[k] = i32x4{0, 0, 0, 0};
+  const int64_t tail = head + 16 * chunks;
+  if (t < head / 2) ((uint16_t *)p)[t] = 0;
+  if (t < (bytes - tail) / 2) ((uint16_t *)(p + tail))[t] = 0;
+}
 __device__ __forceinline__ void zero_rows(const ZeroFill &z, int block) {
-  const i32x4 none = {0, 0, 0, 0};
-  if (z.flat) {
-    const int64_t chunks = z.bytes / 16;
-    for (int64_t k = (int64_t)block * 1024 + threadIdx.x; k < chunks; k += (int64_t)z.blocks * 1024)
-      ((i32x4 *)z.at)[k] = none;
+  if (z.rows == 1) {
+    if ((int)threadIdx.x < kZeroThreads)
+      zero_run(z.at, z.bytes, (int64_t)block * kZeroThreads + threadIdx.x, (int64_t)z.blocks * kZeroThreads);
     return;
   }
-  for (int64_t r = (int64_t)block * kSortWaves + (threadIdx.x >> 6); r < z.rows; r += (int64_t)z.blocks * kSortWaves) {
-    char *p = z.at + r * z.stride;
-    if (z.whole)
-      for (int64_t k = threadIdx.x & 63; k < z.bytes / 16; k += 64) ((i32x4 *)p)[k] = none;
-    else
-      for (int64_t k = threadIdx.x & 63; k < z.bytes / 2; k += 64) ((uint16_t *)p)[k] = 0;
-  }
+  for (int64_t r = (int64_t)block * kSortWaves + (threadIdx.x >> 6); r < z.rows; r += (int64_t)z.blocks * kSortWaves)
+    zero_run(z.at + r * z.stride, z.bytes, threadIdx.x & 63, 64);
 }
 
 __global__ __launch_bounds__(1024) void embed_sort_kernel(const int64_t *ids, int n, int V, int64_t padding, SortOut o,
@@ -538,15 +541,13 @@ int octo_embed_bwd(const void *grad, int64_t ldg, int g_dtype, const int64_t *id
   OCTO_CHECK_ARG((int64_t)a.pieces * a.colblocks < (int64_t)1 << 26, "embed_bwd: %lld tokens of width %d", (long long)n, d);
   ZeroFill z{};
   if (!accumulate) {
-    const int esz = float_bytes(w_dtype);
+    const int64_t row = (int64_t)d * float_bytes(w_dtype);
+    const bool one = ldw == d || V == 1;
     z.at = (char *)grad_w;
-    z.stride = ldw * esz;
-    z.bytes = (int64_t)d * esz;
-    z.rows = V;
-    z.whole = (uintptr_t)grad_w % 16 == 0 && z.stride % 16 == 0 && z.bytes % 16 == 0;
-    z.flat = (uintptr_t)grad_w % 16 == 0 && ldw == d && V * z.bytes % 16 == 0;
-    if (z.flat) z.bytes *= V;
-    const int64_t work = cdiv(V * d * esz, 65536);  // 64 KB a workgroup
+    z.stride = ldw * float_bytes(w_dtype);
+    z.bytes = one ? V * row : row;
+    z.rows = one ? 1 : V;
+    const int64_t work = one ? cdiv(z.bytes, kZeroThreads * 16 * kZeroTurns) : cdiv(V * row, 65536);  // 64 KB of rows apart
     z.blocks = (int)(work < (1 << 20) ? work : 1 << 20);
   }
   const int ranges = (int)cdiv(V, kBins);
