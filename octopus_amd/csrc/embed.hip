@@ -244,7 +244,7 @@ template <int DT, bool VEC> struct Cols {
   typedef typename Elem<DT>::T T;
   static constexpr int PER = 16 / Elem<DT>::bytes;
   i32x4 v[8 / PER];
-  T s[8];
+  uint32_t s[8];  // bits, 16 of them by themselves: two loads into one register would wait for each other
   __device__ __forceinline__ void load(const void *base, int64_t off, int c0, int lane, int d) {
     const T *p = (const T *)base + off;
     if constexpr (VEC) {
@@ -256,10 +256,10 @@ template <int DT, bool VEC> struct Cols {
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = c0 + lane + 64 * e;
-        s[e] = (T)0.f;
-        if (c < d) s[e] = p[c];
+      for (int e = 0; e < 8; ++e) {  // past the end: the last column, not stored
+        const int c = min(c0 + lane + 64 * e, d - 1);
+        if constexpr (DT == OCTO_F32) s[e] = ((const uint32_t *)p)[c];
+        else s[e] = ((const uint16_t *)p)[c];
       }
     }
   }
@@ -274,7 +274,11 @@ template <int DT, bool VEC> struct Cols {
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (float)s[e];
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (DT == OCTO_F32) x[e] = __uint_as_float(s[e]);
+        else if constexpr (DT == OCTO_F16) x[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)s[e]);
+        else x[e] = __uint_as_float(s[e] << 16);
+      }
     }
   }
   static __device__ __forceinline__ void store(const float (&x)[8], void *base, int64_t off, int c0, int lane, int d) {
