@@ -7,15 +7,17 @@
 // largest of its threads' maxima, so that one is a lower bound of the list. It is taken after the first kTopLoads chunks
 // of every thread (32,768 values of 16 bits); from there on the sweep collects what reaches it (300 of 151,936 values at k
 // 64), and sums the row's exponentials as it goes. Every collected value is ranked against the others by (value, column),
-// and the first k ranks are the list. Where more than kCand values reach the bound, a second sweep uses the bound of the
-// whole row; a row with more than kCand even so (runs of equal values), or with a NaN or +inf, is done by a radix select
-// over the values' 32-bit keys.
+// and the first k ranks are the list. Where more than kCand values reach the bound (runs of equal values: rows with fewer
+// than k unmasked logits), a second sweep takes those above the bound of the whole row, and the rest of the list are the
+// first columns that equal it. A row with more than kCand even so, or with a NaN or +inf, is done by a radix select over the
+// values' 32-bit keys.
 //
 // Few rows: a row is cut into slices of a workgroup each (topk_slices), whose lists and sums a second launch joins the same
 // way.
 //
 // Bound by memory, 2 bytes a value at 16 bits: [2048, 151,936] bf16 at k 64 118 to 131 us (4.8 to 5.3 TB/s; a 4 GiB copy
-// moves 5.0), fp32 214 (5.8).
+// moves 5.0), fp32 214 (5.8). Rows with 10 unmasked values 189 and 395 (by the radix select, whose counts of one value
+// wait for each other, 4,560 and 4,640).
 #include "octo_common.h"
 #include "row_values.h"
 
@@ -26,7 +28,8 @@ constexpr int kTopLoads = 8;   // 16-byte chunks in flight per thread
 constexpr int kCand = 2048;    // values that may reach the bound
 constexpr int kHits = 1536;    // chunks that may hold them
 constexpr int kJoin = 2048;    // entries a row's join takes from its slices
-constexpr int kTighten = 256;  // chunks from which on the whole row's bound is taken before they are looked through
+constexpr int kTighten = 254;  // chunks from which on the whole row's bound is taken before they are looked through
+static_assert(kTighten * 8 + 2 * 7 <= kCand, "so many chunks' values, and those before and behind the chunks, have room");
 
 // The order of the list as unsigned numbers: NaN above +inf, -0 equal to +0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -122,16 +125,26 @@ template <int N> __device__ __forceinline__ uint32_t kth_key(const uint32_t (&to
 // count each by itself, or k would be half the threads and the bound far below the k-th value (k 256 of 512 maxima: 1,640
 // chunks of a row of 151,936 collected, of 1,024 maxima 1,370).
 constexpr int kOneTop = 64;
-__device__ __forceinline__ float kth_bound(const float (&top)[2], int k, int (*cnt)[15]) {
-  uint32_t bound;
+__device__ __forceinline__ uint32_t kth_bound(const float (&top)[2], int k, int (*cnt)[15]) {
   if (k <= kOneTop) {
     const uint32_t one[1] = {order_key(fmaxf(top[0], top[1]))};
-    bound = kth_key(one, k, cnt);
-  } else {
-    const uint32_t two[2] = {order_key(top[0]), order_key(top[1])};
-    bound = kth_key(two, k, cnt);
+    return kth_key(one, k, cnt);
   }
+  const uint32_t two[2] = {order_key(top[0]), order_key(top[1])};
+  return kth_key(two, k, cnt);
+}
+__device__ __forceinline__ float bound_value(uint32_t bound) {
   return bound <= 0x007fu ? -INFINITY : key_value(bound << 16);  // 0x007f: the key of -inf, and below
+}
+// The lower 16 bits too: the k-th largest itself.
+__device__ __forceinline__ float kth_value(const float (&top)[2], int k, uint32_t bound, int (*cnt)[15]) {
+  const uint32_t keys[2] = {order_key(k <= kOneTop ? fmaxf(top[0], top[1]) : top[0]),
+                            k <= kOneTop ? 0u : order_key(top[1])};
+  uint32_t rest[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    rest[i] = keys[i] >> 16 == bound ? keys[i] << 16 : keys[i] >> 16 > bound ? 0xffffffffu : 0u;
+  return key_value(bound << 16 | kth_key(rest, k, cnt));
 }
 
 // A ranked value's place in the row's list, if it has one.
@@ -181,7 +194,7 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
   __shared__ __attribute__((aligned(16))) uint64_t cand[kCand];
   __shared__ i32x4 hit[kHits];    // chunks with a value that reaches the bound, as they were loaded
   __shared__ int hit_at[kHits];   // and their place in the row
-  __shared__ int bits[2][4][15];
+  __shared__ int bits[3][4][15];
   __shared__ int nhit, ncand, sel_bin, sel_above;
   static_assert(sizeof hit >= kCand * sizeof(int), "room for the ranks");
   int *ranks = (int *)hit, *hist = (int *)hit;  // where the chunks were, once they are looked through
@@ -190,7 +203,7 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
   const T *row = (const T *)logits + r * ld + first;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const float c = inv_T * OCTO_LOG2E;
-  for (int i = threadIdx.x; i < 2 * 4 * 15; i += kTopThreads) (&bits[0][0][0])[i] = 0;
+  for (int i = threadIdx.x; i < 3 * 4 * 15; i += kTopThreads) (&bits[0][0][0])[i] = 0;
   if (threadIdx.x == 0) nhit = ncand = 0;
 
   // ---- the sweep
@@ -240,7 +253,7 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
       }
     if (b == 0) {
       __syncthreads();
-      least = kth_bound(top, k, bits[0]);
+      least = bound_value(kth_bound(top, k, bits[0]));
     }
     bool wanted[kTopLoads];
 #pragma unroll
@@ -257,16 +270,18 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
   const float lnS = flog2(S) * OCTO_LN2;
   bool listed = S == S;  // no NaN, no +inf
   // ---- the values that reach the bound
-  auto take = [&](float x, int j) {
-    if (x >= least) {
-      const int at = atomicAdd(&ncand, 1);
-      if (at < kCand) cand[at] = list_entry(x, j);
-    }
-  };
   int n = nhit;
-  if (listed && n > kTighten) least = kth_bound(top, k, bits[1]);  // of the whole row
-  if (listed && n <= kHits) {
-    if (edge) take(xe, je);
+  bool more = n > kHits;
+  uint32_t bound = 0;
+  if (listed && n > kTighten) {  // of the whole row
+    bound = kth_bound(top, k, bits[1]);
+    least = bound_value(bound);
+  }
+  if (listed && !more) {
+    if (edge && xe >= least) {
+      const int at = atomicAdd(&ncand, 1);
+      if (at < kCand) cand[at] = list_entry(xe, je);
+    }
     for (int i0 = 0; i0 < n; i0 += kTopThreads) {  // whole waves: append counts over them
       const int i = i0 + threadIdx.x, at0 = i < n ? hit_at[i] : 0;
       float x[PER];
@@ -278,13 +293,50 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
         if (at < kCand) cand[at] = list_entry(x[e], rc.head + at0 * PER + e);
       });
     }
-  } else if (listed) {
-    sweep_row<DT>(row, V, [&](float mx) { return mx >= least; }, take);
+    __syncthreads();
+    n = ncand;
+    more = n > kCand;
   }
-  __syncthreads();
-  n = ncand;
+  // put(place, x, column) for the first `need` columns whose value is wanted
+  auto first_of = [&](int need, auto wanted, auto put) {
+    int seen = 0;
+    for (int s0 = 0, it = 0; s0 < V && seen < need; s0 += kTopThreads, ++it) {
+      const int j = s0 + (int)threadIdx.x;
+      const float x = j < V ? (float)row[j] : 0.f;
+      const bool mine = j < V && wanted(x);
+      const uint64_t bal = __ballot(mine);
+      if (lane == 0) cnts[it & 1][w] = __popcll(bal);
+      __syncthreads();
+      int off = seen;
+#pragma unroll
+      for (int u = 0; u < NW; ++u) {
+        off += u < w ? cnts[it & 1][u] : 0;
+        seen += cnts[it & 1][u];
+      }
+      off += __popcll(bal & ((1ull << lane) - 1ull));
+      if (mine && off < need) put(off, x, j);
+    }
+  };
+  if (__builtin_expect(listed && more, 0)) {
+    // ---- runs of equal values at the bound (fewer than k unmasked logits, say): those above it, then its first columns
+    least = kth_value(top, k, bound, bits[2]);
+    if (threadIdx.x == 0) ncand = 0;  // read by all before the barriers of kth_value
+    __syncthreads();
+    sweep_row<DT>(row, V, [&](float mx) { return mx > least; }, [&](float x, int j) {
+      if (x > least) {
+        const int at = atomicAdd(&ncand, 1);
+        if (at < kCand) cand[at] = list_entry(x, j);
+      }
+    });
+    __syncthreads();
+    n = ncand;
+    if (n < k) {  // k values at least are no smaller than `least`
+      first_of(k - n, [&](float x) { return x == least; }, [&](int at, float x, int j) { cand[n + at] = list_entry(x, j); });
+      n = k;
+    }
+  }
   listed = listed && n <= kCand;
-  if (!listed) {
+  if (__builtin_expect(!listed, 0)) {
     // ---- radix select: the key of the k-th value, 8 bits at a time
     uint32_t prefix = 0;
     int above = 0;  // values whose key is larger than every key that starts with prefix
@@ -312,26 +364,11 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
     // the values above it, and of its equals the first k - above columns
     if (threadIdx.x == 0) ncand = 0;
     __syncthreads();
-    int equals = 0;
-    for (int s0 = 0, it = 0; s0 < V; s0 += kTopThreads, ++it) {
-      const int j = s0 + (int)threadIdx.x;
-      const float x = j < V ? (float)row[j] : 0.f;
-      const uint32_t q = order_key(x);
-      const bool eq = j < V && q == prefix;
-      if (j < V && q > prefix) cand[atomicAdd(&ncand, 1)] = list_entry(x, j);  // fewer than k of them
-      const uint64_t bal = __ballot(eq);
-      if (lane == 0) cnts[it & 1][w] = __popcll(bal);
-      __syncthreads();
-      int off = equals;
-#pragma unroll
-      for (int u = 0; u < NW; ++u) {
-        off += u < w ? cnts[it & 1][u] : 0;
-        equals += cnts[it & 1][u];
-      }
-      off += __popcll(bal & ((1ull << lane) - 1ull));
-      if (eq && off < k - above) cand[k - 1 - off] = list_entry(x, j);  // from the other end: above + equals = k
-    }
-    __syncthreads();
+    sweep_row<DT>(row, V, [](float) { return true; }, [&](float x, int j) {
+      if (order_key(x) > prefix) cand[atomicAdd(&ncand, 1)] = list_entry(x, j);  // `above` of them, fewer than k
+    });
+    first_of(k - above, [&](float x) { return order_key(x) == prefix; },
+             [&](int at, float x, int j) { cand[above + at] = list_entry(x, j); });
     n = k;
   }
 

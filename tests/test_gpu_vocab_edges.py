@@ -220,3 +220,47 @@ def test_odd_widths_cost_about_what_even_ones_do(dtype):
     got = embed_bwd(g, ids, 3)
     want = torch.zeros(3, 65, device="cuda").index_add_(0, ids, g.float())
     assert torch.equal(got.float().nan_to_num(9.0), want.nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [700, 5000, 100003])
+@pytest.mark.parametrize("k", [1, 30, 65, 200])
+def test_lists_of_few_values_above_a_run_of_equal_ones(dtype, V, k):
+    """Allow-lists: fewer than k values above a mask of any value, none, one more than k; values and equal ones behind
+    each other's columns; zeros of both signs; the oracle's lists, whole or in slices."""
+    from octopus_amd.distill_op import head_topk
+
+    g = torch.Generator().manual_seed(V + k)
+    rows = []
+    for mask in (-torch.inf, torch.finfo(dtype).min, -1e4, -0.3, 0.0, -0.0, 2.0):
+        for kept in (0, 1, k - 1, k + 1):
+            x = torch.full((V,), mask)
+            at = torch.randperm(V, generator=g)[:min(kept, V - 1)]
+            x[at] = 3.0 + torch.rand(len(at), generator=g)
+            rows.append(x)
+            below = x.clone()  # and below it, all over the row
+            low = torch.randperm(V, generator=g)[:V // 2]
+            below[low[x[low] < 2.5]] = -torch.inf
+            rows.append(below)
+    z = torch.stack(rows).to(dtype)
+    want_ids, want = odist.topk(z, 1.0, k)
+    for part in (slice(None), slice(0, 3)):  # three rows of 100,003: in slices where the type makes them long enough
+        ids, logp = head_topk(z[part].cuda(), 1.0, k)
+        assert torch.equal(ids.cpu(), want_ids[part])
+        got, fin = logp.cpu().double(), want[part].isfinite()
+        assert torch.equal(got == -torch.inf, want[part] == -torch.inf)
+        # as tests/test_gpu_topk.py derives it
+        assert ((got - want[part]).abs()[fin] <= 2e-5 + 2 ** -22 * want[part].abs()[fin]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("mask", [-torch.inf, -1e30])
+def test_masked_rows_cost_a_second_sweep(dtype, mask):
+    """512 rows of 151,936 with 10 unmasked logits each, k 64: below 6 times the time of unmasked rows (34 times as a radix
+    select over one bin)."""
+    from octopus_amd.distill_op import head_topk
+
+    z = torch.randn(512, 151936, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    plain = _fastest(lambda: head_topk(z, 1.0, 64), calls=3)
+    z[:, torch.arange(151936, device="cuda") % 15000 != 7] = mask
+    assert _fastest(lambda: head_topk(z, 1.0, 64), calls=3) <= 6 * plain
