@@ -329,9 +329,9 @@ template <int DT>
 __global__ __launch_bounds__(64 * kDotWaves) void distill_dots_kernel(DistillArgs a) {
   __shared__ float best[kDotWaves];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  if (blockIdx.x == 0)
+  const int64_t r = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  if (r == 0)
     for (int k = threadIdx.x; k < a.nflag; k += 64 * waves) a.flag_cnt[k] = 0;
-  const int64_t r = blockIdx.x;
   const int64_t cnt = a.count ? min((int64_t)(*a.count), a.n_max) : a.n_max;
   if (r >= cnt) return;
   const int64_t hrow = a.idx ? a.idx[r] : r;
@@ -547,7 +547,8 @@ __global__ __launch_bounds__(kLossThreads) void distill_loss_kernel(DistillArgs 
 int launch_distill_dots(const DistillArgs &a, hipStream_t st) {
   if (a.n_max == 0) return OCTO_OK;
   const int waves = (int)cdiv(a.K, kDotSlots);  // no more than have slots: 4,000 rows of K 20, 149 us with 8 each, 95 with 3
-  const dim3 g((unsigned)a.n_max), b(64 * (waves < kDotWaves ? waves : kDotWaves));
+  const dim3 g((unsigned)(a.n_max < kLaunchRows ? a.n_max : kLaunchRows), (unsigned)cdiv(a.n_max, kLaunchRows));
+  const dim3 b(64 * (waves < kDotWaves ? waves : kDotWaves));
   if (a.dt == OCTO_BF16) hipLaunchKernelGGL(distill_dots_kernel<OCTO_BF16>, g, b, 0, st, a);
   else if (a.dt == OCTO_F16) hipLaunchKernelGGL(distill_dots_kernel<OCTO_F16>, g, b, 0, st, a);
   else hipLaunchKernelGGL(distill_dots_kernel<OCTO_F32>, g, b, 0, st, a);

@@ -264,3 +264,25 @@ def test_masked_rows_cost_a_second_sweep(dtype, mask):
     plain = _fastest(lambda: head_topk(z, 1.0, 64), calls=3)
     z[:, torch.arange(151936, device="cuda") % 15000 != 7] = mask
     assert _fastest(lambda: head_topk(z, 1.0, 64), calls=3) <= 6 * plain
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_more_hidden_rows_than_a_launch_has_threads_for(grad):
+    """2^24 rows and more, each a workgroup of 256 threads: the last rows' divergences and gradients are a small call's."""
+    from octopus_amd.distill_op import fused_distill_head
+
+    n, d, V, K, few = (1 << 24) + 5, 8, 9, 25, 70
+    g = torch.Generator(device="cuda").manual_seed(8)
+    h = torch.randn(n, d, generator=g, device="cuda").bfloat16().requires_grad_(grad)
+    w = torch.randn(V, d, generator=g, device="cuda").bfloat16()
+    ids = torch.randint(0, V, (n, K), generator=g, device="cuda")
+    t = torch.randn(n, K, generator=g, device="cuda")
+    loss, kl = fused_distill_head(h, w, ids, t, 1.0)
+    last = h.detach()[-few:].clone().requires_grad_(True)
+    few_loss, few_kl = fused_distill_head(last, w, ids[-few:], t[-few:], 1.0)
+    assert torch.equal(kl[-few:], few_kl)
+    assert abs(loss.item() - kl.double().sum().item()) <= 2.0 ** -23 * loss.item()
+    if grad:
+        (a,), (b,) = torch.autograd.grad(loss, h), torch.autograd.grad(few_loss, last)
+        assert (a[-few:] - b).norm() <= 2 ** -7 * b.norm()  # stored exponentials and results of 16 bits, on both sides
+        assert (a.float().norm(dim=1) > 0).all()
