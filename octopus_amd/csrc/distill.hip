@@ -427,16 +427,31 @@ __global__ __launch_bounds__(64 * kDistMergeRows) void distill_merge_kernel(Dist
   }
 }
 
+// The maximum of a half tile's 128 exponentials, whose value is known in fp32, before it was rounded to 16 bits. 16
+// neighbouring lanes, all active, hold 8 of them each: v as stored, x as fp32. Where one value of them all has the maximum's
+// bits `top`, its x becomes `exact`; where more do, which of them is the maximum cannot be told.
+__device__ __forceinline__ void unround_max(const i32x4 v, uint32_t top, float exact, float (&x)[8]) {
+  uint32_t hit = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) hit |= (((uint32_t)v[e >> 1] >> (16 * (e & 1))) & 0xffffu) == top ? 1u << e : 0u;
+  const uint64_t lanes = __ballot(hit != 0) >> (threadIdx.x & 48) & 0xffffu;
+  if ((hit & (hit - 1)) || __popcll(lanes) != 1) hit = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = hit >> e & 1 ? exact : x[e];
+}
+
 // Every row's exponentials from the offset they were stored at to xuse, and its dz scale: launch_ex_fix's work for all rows,
 // where grad_W is asked for. h^T times the row's scale is rounded to bf16 there; at a scale of 2^k (1 + 2^-17 or so, from
-// xuse's own rounding) that product is h's own bits, and what is rounded a second time are the dense entries, small beside the
-// listed ones (at V 151,936 and K 64 one part in 50 of the row's norm): grad_W's error falls from 2.9e-3 to 2.35e-3 (one
-// rounding of the result alone is 1.7e-3). Bound by memory, 4 bytes an element: [8,192, 151,936] 752 us (6.6 TB/s), 5% of
-// the call.
+// xuse's own rounding) that product is h's own bits, and what is rounded a second time are the dense entries. The ones that
+// weigh, a student's own likely tokens, are nearly always their half tile's maximum, which the statistics keep in fp32: they
+// are made of that and rounded once. So are the listed ones, and grad_W's error falls from 2.9e-3 to 2.35e-3 (one rounding of
+// the result alone is 1.7e-3); a student certain of tokens off its list (0.3 of the norm's square) 2.54e-3 with the maxima
+// rounded twice, 2.4e-3 now. Bound by memory, 4 bytes an element: [8,192, 151,936] 752 us (6.6 TB/s), 5% of the call.
 constexpr int kEvenChunks = 2;  // 16-byte chunks per thread
 __global__ __launch_bounds__(256) void distill_even_kernel(DistillArgs a, float *scale) {
   const int64_t cnt = a.count ? min((int64_t)(*a.count), a.n_max) : a.n_max;
   const int64_t chunk0 = (int64_t)blockIdx.x * (256 * kEvenChunks) + threadIdx.x;
+  const float inv_c = 1.f / a.c;
   for (int64_t i = blockIdx.y; i < a.rows; i += gridDim.y) {
     const int64_t r = a.r0 + i;
     const bool in = r < cnt;
@@ -462,11 +477,13 @@ __global__ __launch_bounds__(256) void distill_even_kernel(DistillArgs a, float 
       if (c0 >= a.ldx) continue;
       const f32x4 q = pr[c0 >> 8];  // 8 columns never straddle a 128-column half tile
       const float mh = (c0 & 128) ? q[3] : q[0];  // -inf: no column of the half lies below V (stored zeros)
-      const float fac = mh == -INFINITY ? 0.f : fexp2(mh - xn - fminf(mh - xo, kExClamp));
+      const float above = fminf(mh - xo, kExClamp), fac = mh == -INFINITY ? 0.f : fexp2(mh - xn - above);
       float x[8];
       unpack8(v[u], false, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= fac;
+      const float th = a.use_tanh ? mh * inv_c : 0.f, slope = 1.f - th * th;  // as the epilogue stored it
+      unround_max(v[u], __builtin_bit_cast(uint16_t, (__bf16)(slope * fexp2(above))), slope * fexp2(mh - xn), x);
       __builtin_nontemporal_store(pack8(x, false), (i32x4 *)(row + c0));
     }
   }

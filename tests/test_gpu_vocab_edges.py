@@ -286,3 +286,26 @@ def test_more_hidden_rows_than_a_launch_has_threads_for(grad):
         (a,), (b,) = torch.autograd.grad(loss, h), torch.autograd.grad(few_loss, last)
         assert (a[-few:] - b).norm() <= 2 ** -7 * b.norm()  # stored exponentials and results of 16 bits, on both sides
         assert (a.float().norm(dim=1) > 0).all()
+
+
+def test_a_confident_student_beside_its_list(monkeypatch):
+    """bf16, one listed token of probability near 0 and a student that puts more than half of its mass on another: 0.3 of
+    dz's square are dense entries. Every entry that weighs takes one rounding and the gradient's own is the second, so its
+    error is sqrt(2) times that of the exact gradient rounded, below sqrt(2.2). Dense entries rounded twice: sqrt(2.3)."""
+    from octopus_amd import distill_op, head_op
+
+    n, d, V = 400, 256, 16384
+    g = torch.Generator().manual_seed(31)
+    h = torch.randn(n, d, generator=g).to(torch.bfloat16)
+    w = (torch.randn(V, d, generator=g) * 0.45).to(torch.bfloat16)
+    ids, t = torch.randint(0, V, (n, 1), generator=g), torch.zeros(n, 1)
+    rw = torch.rand(n, generator=g) + 0.5
+    monkeypatch.setattr(head_op, "_LATER_WEIGHTS", 1 << 62)
+    monkeypatch.setattr(head_op, "_LATER_WORK", 1 << 62)
+    hd, wd = h.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    distill_op.fused_distill_head(hd, wd, ids.cuda(), t.cuda(), 1.0, rw.cuda())[0].backward()
+    dz = odist.divergence(h.double() @ w.double().T, ids, t)[1] * rw.double()[:, None]
+    assert dz.gather(1, ids).pow(2).sum() <= 0.7 * dz.pow(2).sum()
+    for got, want in [(wd.grad, dz.T @ h.double()), (hd.grad, dz @ w.double())]:
+        once = (want.to(torch.bfloat16).double() - want).norm()
+        assert (got.cpu().double() - want).norm() <= 2.2 ** 0.5 * once
