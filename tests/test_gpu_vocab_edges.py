@@ -309,3 +309,62 @@ def test_a_confident_student_beside_its_list(monkeypatch):
     for got, want in [(wd.grad, dz.T @ h.double()), (hd.grad, dz @ w.double())]:
         once = (want.to(torch.bfloat16).double() - want).norm()
         assert (got.cpu().double() - want).norm() <= 2.2 ** 0.5 * once
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_some_rows_of_more_than_2_gib(dtype):
+    """Rows that take part, gathered from a hidden matrix past the 32-bit offsets of a mapped operand: the call of those
+    rows by themselves, with and without gradients."""
+    from octopus_amd.distill_op import fused_distill_head
+
+    d, V, K = 2048, 1000, 6
+    n = (1 << 31) // (d * dtype.itemsize) + 3000
+    g = torch.Generator(device="cuda").manual_seed(9)
+    h = torch.zeros(n, d, dtype=dtype, device="cuda")
+    idx = torch.cat([torch.arange(0, n - 400, n // 100, device="cuda"), torch.arange(n - 300, n, device="cuda")])
+    h[idx] = torch.randn(len(idx), d, generator=g, device="cuda").to(dtype)
+    w = (torch.randn(V, d, generator=g, device="cuda") * 0.05).to(dtype)
+    ids = torch.randint(0, V, (n, K), generator=g, device="cuda")
+    t, rw = torch.randn(n, K, generator=g, device="cuda"), torch.rand(n, generator=g, device="cuda")
+    count = torch.tensor([len(idx) - 5], dtype=torch.int32, device="cuda")
+    part = idx[:-5]
+
+    def run(h, idx, count, rows, grad):
+        h, v = h.detach().requires_grad_(grad), w.detach().requires_grad_(grad)
+        loss, kl = fused_distill_head(h, v, ids[rows], t[rows], 1.0, rw[rows], idx=idx, count=count)
+        return loss.detach(), kl, *(torch.autograd.grad(loss, (h, v)) if grad else ())
+
+    for grad in (False, True):
+        got, want = run(h, idx, count, slice(None), grad), run(h[part], None, None, part, grad)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1][part], want[1])
+        rest = torch.ones(n, dtype=torch.bool, device="cuda").index_fill_(0, part, False)
+        assert (got[1][rest] == 0).all()
+        if grad:  # the same sums, over other tiles: a step of the type, or fp32's own
+            step = torch.finfo(dtype).eps * (1 if dtype == torch.bfloat16 else 32)
+            assert (got[2][part] - want[2]).norm() <= step * want[2].norm() and (got[2][rest] == 0).all()
+            assert (got[3] - want[3]).norm() <= step * want[3].norm()
+
+
+def test_a_later_weight_gradient_of_some_rows(monkeypatch):
+    """The kept operands of rows that take part by idx and a count that changes after the call."""
+    from octopus_amd import distill_op, head_op
+    from octopus_amd.head_op import compact_rows
+
+    n, d, V, K = 200, 256, 3000, 12
+    h, w, ids, t = _small(n, d, V, K, seed=10)
+    rw = torch.rand(n, generator=torch.Generator().manual_seed(11)).cuda()
+    idx, count = compact_rows(torch.rand(n, generator=torch.Generator().manual_seed(12)).cuda() < 0.4)
+    monkeypatch.setattr(head_op, "_LATER_SHARE", 1 << 20)
+    out = []
+    for later in (True, False):
+        monkeypatch.setattr(head_op, "_LATER_WEIGHTS", 0 if later else 1 << 62)
+        monkeypatch.setattr(head_op, "_LATER_WORK", 1 << 62)
+        assert (distill_op._later_bytes(h, w, idx, True, True) > 0) == later
+        c = count.clone()
+        loss, kl = distill_op.fused_distill_head(h, w, ids, t, 1.0, rw, idx=idx, count=c)
+        c.fill_(3)
+        out.append((loss.detach(), kl, *torch.autograd.grad(loss, (h, w))))
+    a, b = out
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for x, y in zip(a[2:], b[2:]):
+        assert (x - y).norm() <= 2 ** -8 * y.norm()  # the same products, split differently, and the result's rounding
