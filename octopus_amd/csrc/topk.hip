@@ -427,13 +427,15 @@ __global__ __launch_bounds__(kTopThreads) void topk_join_kernel(const uint64_t *
   for (int i = threadIdx.x; i < got; i += kTopThreads) write_value(cand[i], ranks[i], r, k, st.m, lnS, inv_T, ids, logp);
 }
 
-// Slices a row of V values is cut into for n rows: rows of 192 KB and more, up to 128 of them, four slices at least. us a
-// call in a captured graph, V 151,936, k 64, whole and sliced: 1 row of bf16 20.6 and 15.2, 64 rows 21.1 and 16.7, 1 row of
-// fp32 24.4 and 14.8. Launched one by one the second launch costs its gain in host time: 1 row of bf16 20.2 and 19.5, 128
-// rows 22.3 and 21.7; below, a loss: 256 rows 25.2 and 28.2, V 32,000 14.2 and 18.6, k 256 28 and 50.
+// Slices a row of V values is cut into for n rows: rows of 192 KB and of 60,000 values and more, up to 128 of them, four
+// slices at least. us a call in a captured graph at k 64, whole and sliced, for 1, 16 and 128 rows. bf16, V 151,936: 21.0
+// and 15.5, 21.7 and 15.5, 23.0 and 21.8; 100,000 (195 KB): 17.0 and 15.3, 17.6 and 15.4, 19.1 and 17.8; 64,000 (125 KB): 12.9
+// and 15.2, 13.7 and 15.2, 13.6 and 16.3. fp32, V 64,000 (250 KB): 15.0 and 14.7, 15.8 and 14.9, 17.0 and 16.5; 49,152 (192
+// KB): 13.5 and 14.8, 13.6 and 14.8, 14.2 and 15.8. More rows or longer lists lose by it: 256 rows 25.2 and 28.2, k 256 28
+// and 50.
 constexpr int kMaxSlices = 16, kSliceK = 128;
 static int topk_slices(int64_t n, int V, int k, int dtype) {
-  if (n < 1 || n > 128 || k > kSliceK || (int64_t)V * float_bytes(dtype) < 192 * 1024) return 1;
+  if (n < 1 || n > 128 || k > kSliceK || V < 60000 || (int64_t)V * float_bytes(dtype) < 192 * 1024) return 1;
   const int s = (int)(512 / n);
   return s < kMaxSlices ? s : kMaxSlices;
 }

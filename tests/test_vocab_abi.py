@@ -104,3 +104,14 @@ def test_sizes_past_the_kernels_counts():
     _refused("octo_embed_fwd", P, 8, _lib.BF16, V, 8, P, 4, 1.0, P, 8, None)
     for n, v in [((1 << 27) + 1, 10), (4, V)]:
         _refused("octo_embed_bwd_workspace_bytes", n, v, 8, ctypes.byref(out))
+
+
+def test_rows_that_go_whole_need_no_workspace():
+    """Few fp32 rows from 60,000 values on, and of 16 bits from 192 KB, are cut into slices; shorter ones are faster whole."""
+    out = ctypes.c_size_t(0)
+    for n, V, dtype, k, sliced in [(1, 49152, _lib.F32, 64, False), (1, 59999, _lib.F32, 64, False),
+                                   (1, 60000, _lib.F32, 64, True), (128, 98304, _lib.BF16, 128, True),
+                                   (128, 98303, _lib.F16, 128, False), (129, 151936, _lib.BF16, 64, False),
+                                   (1, 151936, _lib.BF16, 129, False)]:
+        _lib.call("octo_topk_workspace_bytes", n, V, dtype, k, ctypes.byref(out))
+        assert (out.value > 0) == sliced
