@@ -219,11 +219,12 @@ int octo_topk(const void *logits, int64_t ld, int dtype, int64_t n, int V, float
               float *logp, void *ws, size_t ws_bytes, void *stream);
 
 /* Distillation from teachers' lists (no counterpart in the reference). Row r's list holds K slots (ids[r, k],
- * teacher[r, k]): a token and the teacher's logit or log-probability of it (fp32). A slot with an id outside [0, V) or a
- * teacher value of -inf is empty; the same token may stand in several slots.
+ * teacher[r, k]): a token and the teacher's logit or log-probability of it (fp32). A slot with an id outside [0, V) or
+ * a teacher value of -inf is empty; the same token may stand in several slots.
  *   q = softmax(teacher[r, :]) over the slots that are not empty (OCTO_LIST_RAW: exp of it),  p = softmax(z_r * inv_T)
  *   kl[r] = sum_k q_k (log q_k - log p_ids[k]),  0 for a row whose slots are all empty.
- * Over materialised logits [n, ld]: the forward also leaves state [n, 4] (16 bytes a row) and q [n, K] for the backward,
+ * Over materialised logits [n, ld]: the forward also leaves state [n, 4] (16 bytes a row) and q [n, K] for the
+ * backward,
  *   dlogits[r, v] = g[r] inv_T (Q p_v - sum of q_k over the slots of v),  Q = sum of q,
  * in the logits' dtype at stride ld_d; a row with Q = 0 gets zeros whatever its logits are. 1 <= K <= OCTO_LIST_MAX. */
 int octo_distill_columns_fwd(const void *logits, int64_t ld, int dtype, const int64_t *ids, const float *teacher,
@@ -233,11 +234,11 @@ int octo_distill_columns_bwd(const void *logits, int64_t ld, int dtype, const in
                              int V, int K, float inv_T, const float *state, const float *g, void *dlogits,
                              int64_t ld_d, void *stream);
 
-/* The same from hidden rows and the vocabulary weight, without the logits: octo_head_step_grpo's forward and backward in
- * one call (fp32 operands run the forward, then octo_head_bwd's recompute), for loss = sum over the compact rows of weight
- * x kl. Lists and weights are per hidden row (compact row r's at idx[r], or r): ids, teacher [h_rows, K], weight [h_rows]
- * (NULL: 1). kl [h_rows] is written at the compact rows' hidden rows, loss [1]. dots, q [n_max, K] and g [n_max] are
- * scratch, as lse [n_max, 2]. grad_h (compact rows) and grad_w as octo_head_step_grpo's; workspace likewise
+/* The same from hidden rows and the vocabulary weight, without the logits: octo_head_step_grpo's forward and backward
+ * in one call (fp32 operands run the forward, then octo_head_bwd's recompute), for loss = sum over the compact rows of
+ * weight x kl. Lists and weights are per hidden row (compact row r's at idx[r], or r): ids, teacher [h_rows, K], weight
+ * [h_rows] (NULL: 1). kl [h_rows] is written at the compact rows' hidden rows, loss [1]. dots, q [n_max, K] and g
+ * [n_max] are scratch, as lse [n_max, 2]. grad_h (compact rows) and grad_w as octo_head_step_grpo's; workspace likewise
  * (OCTO_WS_STEP; with neither gradient, unless the weights are fp8, the forward's, without that flag). kept != NULL: no
  * grad_w, whose operands stay in kept for octo_head_later_grad_w, as octo_head_step_later (sizes from
  * octo_head_later_bytes). */
@@ -263,8 +264,8 @@ int octo_embed_fwd(const void *w, int64_t ldw, int dtype, int64_t V, int d, cons
                    void *out, int64_t ldo, void *stream);
 /* Its gradient by sorted tokens: grad_w[v, :d] = scale * sum of grad[t, :d] over the tokens with ids[t] = v, summed in
  * fp32 in an order that the ids alone decide and rounded once to w_dtype; ids outside [0, V) and padding_idx (-1: none)
- * are left out. accumulate: added to what grad_w holds, and the rows of other entries are neither read nor written; else
- * every row is written. n <= 2^27. ws: octo_embed_bwd_workspace_bytes, 16-byte aligned. */
+ * are left out. accumulate: added to what grad_w holds, and the rows of other entries are neither read nor written;
+ * else every row is written. n <= 2^27. ws: octo_embed_bwd_workspace_bytes, 16-byte aligned. */
 int octo_embed_bwd_workspace_bytes(int64_t n, int64_t V, int d, size_t *bytes);
 int octo_embed_bwd(const void *grad, int64_t ldg, int g_dtype, const int64_t *ids, int64_t n, int64_t V, int d,
                    int64_t padding_idx, float scale, void *grad_w, int64_t ldw, int w_dtype, int accumulate, void *ws,

@@ -140,8 +140,9 @@ __global__ __launch_bounds__(kDistThreads, 8) void distill_columns_fwd_kernel(co
 }
 
 // One workgroup per kDistLoads x 256 chunks of a row. Its first wave picks the slots that lie in its columns, in the
-// list's order, and marks their chunks in a bit map; a thread with a marked chunk goes through the picked ones (3 of 64 on
-// average at V 151,936; each thread through the whole list, and per value, made the kernel 680 us at [2048, 151,936]).
+// list's order, and marks their chunks in a bit map; a thread with a marked chunk goes through the picked ones (3 of 64
+// on average at V 151,936; each thread through the whole list, and per value, made the kernel 680 us at [2048,
+// 151,936]).
 constexpr int kMarkWords = 256 * kDistLoads / 32;
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void distill_columns_bwd_kernel(const void *logits, int64_t ld, const int64_t *ids,
@@ -277,17 +278,17 @@ static void go_bwd(const void *logits, int64_t ld, const int64_t *ids, const flo
   }
 }
 
-// ---- the distillation step over hidden rows ---------------------------------------------------------------------------
+// ---- the distillation step over hidden rows -------------------------------------------------------------------------
 // A listed logit in the softmax's base-2 units before the row's maximum is taken off: x c, x the (soft-capped) logit.
 __device__ __forceinline__ float listed_x(const DistillArgs &a, float dot, int64_t y, bool exact_tanh) {
   const float x = a.w_dtype == OCTO_FP8E4M3 ? dot * a.wscale[y] : dot;
   return a.use_tanh ? (exact_tanh ? tanhf(a.pre * x) : ftanh(a.pre * x)) : x;
 }
 
-// One workgroup per compact row. A wave takes kDotSlots slots at a time, so that a part of the hidden row is read once for
-// all of them and their loads are in flight together; the lanes' sums are exchanged and halved together. fp8 weights are
-// read from their widened copy. Bound by the gathered weight rows, n K d x 2 bytes out of the caches: 8,192 rows, K 64, d
-// 2560 (2.7 GB) 365 us, 7.4 TB/s (8 waves a row 413; a slot at a time 504).
+// One workgroup per compact row. A wave takes kDotSlots slots at a time, so that a part of the hidden row is read once
+// for all of them and their loads are in flight together; the lanes' sums are exchanged and halved together. fp8
+// weights are read from their widened copy. Bound by the gathered weight rows, n K d x 2 bytes out of the caches: 8,192
+// rows, K 64, d 2560 (2.7 GB) 365 us, 7.4 TB/s (8 waves a row 413; a slot at a time 504).
 constexpr int kDotWaves = 4, kDotSlots = 8;
 template <int DT>
 __device__ __forceinline__ float dot_slots(const char *h, const char *const (&w)[kDotSlots], int d, int lane) {
@@ -428,8 +429,8 @@ __global__ __launch_bounds__(64 * kDistMergeRows) void distill_merge_kernel(Dist
 }
 
 // The maximum of a half tile's 128 exponentials, whose value is known in fp32, before it was rounded to 16 bits. 16
-// neighbouring lanes, all active, hold 8 of them each: v as stored, x as fp32. Where one value of them all has the maximum's
-// bits `top`, its x becomes `exact`; where more do, which of them is the maximum cannot be told.
+// neighbouring lanes, all active, hold 8 of them each: v as stored, x as fp32. Where one value of them all has the
+// maximum's bits `top`, its x becomes `exact`; where more do, which of them is the maximum cannot be told.
 __device__ __forceinline__ void unround_max(const i32x4 v, uint32_t top, float exact, float (&x)[8]) {
   uint32_t hit = 0;
 #pragma unroll
@@ -440,13 +441,14 @@ __device__ __forceinline__ void unround_max(const i32x4 v, uint32_t top, float e
   for (int e = 0; e < 8; ++e) x[e] = hit >> e & 1 ? exact : x[e];
 }
 
-// Every row's exponentials from the offset they were stored at to xuse, and its dz scale: launch_ex_fix's work for all rows,
-// where grad_W is asked for. h^T times the row's scale is rounded to bf16 there; at a scale of 2^k (1 + 2^-17 or so, from
-// xuse's own rounding) that product is h's own bits, and what is rounded a second time are the dense entries. The ones that
-// weigh, a student's own likely tokens, are nearly always their half tile's maximum, which the statistics keep in fp32: they
-// are made of that and rounded once. So are the listed ones, and grad_W's error falls from 2.9e-3 to 2.35e-3 (one rounding of
-// the result alone is 1.7e-3); a student certain of tokens off its list (0.3 of the norm's square) 2.54e-3 with the maxima
-// rounded twice, 2.4e-3 now. Bound by memory, 4 bytes an element: [8,192, 151,936] 752 us (6.6 TB/s), 5% of the call.
+// Every row's exponentials from the offset they were stored at to xuse, and its dz scale: launch_ex_fix's work for all
+// rows, where grad_W is asked for. h^T times the row's scale is rounded to bf16 there; at a scale of 2^k (1 + 2^-17 or
+// so, from xuse's own rounding) that product is h's own bits, and what is rounded a second time are the dense entries.
+// The ones that weigh, a student's own likely tokens, are nearly always their half tile's maximum, which the statistics
+// keep in fp32: they are made of that and rounded once. So are the listed ones, and grad_W's error falls from 2.9e-3 to
+// 2.35e-3 (one rounding of the result alone is 1.7e-3); a student certain of tokens off its list (0.3 of the norm's
+// square) 2.54e-3 with the maxima rounded twice, 2.4e-3 now. Bound by memory, 4 bytes an element: [8,192, 151,936] 790
+// us (6.3 TB/s), 5% of the call.
 constexpr int kEvenChunks = 2;  // 16-byte chunks per thread
 __global__ __launch_bounds__(256) void distill_even_kernel(DistillArgs a, float *scale) {
   const int64_t cnt = a.count ? min((int64_t)(*a.count), a.n_max) : a.n_max;
@@ -510,8 +512,8 @@ __device__ __forceinline__ void loss_sum(const DistillArgs &a, double *part) {
 }
 
 // One wave per row. Slots of one token all write the sum of their weights, taken in the list's order. The last pass's
-// launch has a workgroup more, the loss's: every row's kl is there by then (a launch of its own: 4 us of a call's 130 at
-// 225 rows, V 32,000).
+// launch has a workgroup more, the loss's: every row's kl is there by then (a launch of its own: 4 us of a call's 130
+// at 225 rows, V 32,000).
 constexpr int kEntryRows = 4;
 static_assert(64 * kEntryRows == kLossThreads, "the loss's workgroup");
 __global__ __launch_bounds__(64 * kEntryRows) void distill_entries_kernel(DistillArgs a) {
@@ -563,7 +565,8 @@ __global__ __launch_bounds__(kLossThreads) void distill_loss_kernel(DistillArgs 
 
 int launch_distill_dots(const DistillArgs &a, hipStream_t st) {
   if (a.n_max == 0) return OCTO_OK;
-  const int waves = (int)cdiv(a.K, kDotSlots);  // no more than have slots: 4,000 rows of K 20, 149 us with 8 each, 95 with 3
+  // no more waves than have slots: 4,000 rows of K 20, 149 us with 8 each, 95 with 3
+  const int waves = (int)cdiv(a.K, kDotSlots);
   const dim3 g((unsigned)(a.n_max < kLaunchRows ? a.n_max : kLaunchRows), (unsigned)cdiv(a.n_max, kLaunchRows));
   const dim3 b(64 * (waves < kDotWaves ? waves : kDotWaves));
   if (a.dt == OCTO_BF16) hipLaunchKernelGGL(distill_dots_kernel<OCTO_BF16>, g, b, 0, st, a);

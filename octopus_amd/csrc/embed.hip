@@ -8,17 +8,18 @@
 // the tokens alone decide, and rounded once, so equal inputs give equal bits.
 //
 // The gradient takes three launches:
-//   sort   a workgroup per range of kBins vocabulary entries: it reads all ids, counts those below its range (the place of
-//          its first token) and those of each entry by wave (a wave takes a contiguous part of the tokens), and places its
-//          tokens, so that sorted tokens of one entry keep their order. No workgroup waits for another. Behind them, in the
-//          same launch, workgroups that write the zeros of the whole gradient while the sort waits for its loads: the rows
-//          that tokens name are written twice, 9,000 of 151,936 for 32,768 tokens of text.
-//   sum    a wave per kRun sorted tokens x 512 columns: the sum of every entry whose tokens all lie in the piece goes to
-//          grad_W, that of an entry that crosses a piece's border to the piece's two fp32 partial rows (its first and
-//          its last entry). Frequent tokens are so shared out evenly.
+//   sort   a workgroup per range of kBins vocabulary entries: it reads all ids, counts those below its range (the place
+//          of its first token) and those of each entry by wave (a wave takes a contiguous part of the tokens), and
+//          places its tokens, so that sorted tokens of one entry keep their order. No workgroup waits for another.
+//          Behind them, in the same launch, workgroups that write the zeros of the whole gradient while the sort waits
+//          for its loads: the rows that tokens name are written twice, 9,000 of 151,936 for 32,768 tokens of text.
+//   sum    a wave per kRun sorted tokens x 512 columns: the sum of every entry whose tokens all lie in the piece goes
+//          to grad_W, that of an entry that crosses a piece's border to the piece's two fp32 partial rows (its first
+//          and its last entry). Frequent tokens are so shared out evenly.
 //   join   a workgroup per piece in which a crossing entry starts: its partial rows summed in order.
-// 32,768 tokens of text, d 2560, V 151,936, bf16: 207 us (0.95 GB at 4.6 TB/s: sort and zeros 115, sum 75, of which half is
-// the zeros' way out of the caches, join 13); added in place 80 (sort 18, sum 27 to 50). One entry alone: 112 in place.
+// 32,768 tokens of text, d 2560, V 151,936, bf16: 207 us (0.95 GB at 4.6 TB/s: sort and zeros 115, sum 75, of which
+// half is the zeros' way out of the caches, join 13); added in place 80 (sort 18, sum 27 to 50). One entry alone: 112
+// in place.
 #include "octo_common.h"
 #include "row_values.h"
 
@@ -29,7 +30,7 @@ constexpr int kRun = 32;      // sorted tokens per piece
 constexpr int kCols = 512;    // columns per wave of the sum
 constexpr int kSumLoads = 8;  // rows in flight per wave
 
-// ---- lookup ------------------------------------------------------------------------------------------------------------
+// ---- lookup ---------------------------------------------------------------------------------------------------------
 // A wave per token and 4 KB of its row: 32,768 tokens of d 2560, V 151,936 in bf16 38 us (8,200 distinct rows).
 constexpr int kRowLoadsF = 4;
 template <int DT, bool VEC>
@@ -69,7 +70,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void *w, int64_t l
   }
 }
 
-// ---- sort --------------------------------------------------------------------------------------------------------------
+// ---- sort -----------------------------------------------------------------------------------------------------------
 struct SortOut {
   int32_t *order;  // [n] token positions by (entry, position)
   int32_t *entry;  // [n] the entries of them
@@ -84,12 +85,13 @@ struct ZeroFill {
   int64_t stride, bytes, rows;
   int blocks;
 };
-// A workgroup's first kZeroThreads threads write kZeroTurns chunks each: memory takes stores best from few waves at a time
-// that move through it as one front. us of an fp32 gradient of 8 tokens, [151,936, 2560] and [151,935, 2559], and a bf16 one
-// of 1,501 tokens, [32,000, 1024]: 242, 246, 26; one turn 230, 233, 28; all 1,024 threads, one turn 255, 258, 27, four turns
-// 274, .., 26 (a fill and an index_add_: 262, 261, 91).
+// A workgroup's first kZeroThreads threads write kZeroTurns chunks each: memory takes stores best from few waves at a
+// time that move through it as one front. us of an fp32 gradient of 8 tokens, [151,936, 2560] and [151,935, 2559], and
+// a bf16 one of 1,501 tokens, [32,000, 1024]: 242, 246, 26; one turn 230, 233, 28; all 1,024 threads, one turn 255,
+// 258, 27, four turns 274, .., 26 (a fill and an index_add_: 262, 261, 91).
 constexpr int kZeroThreads = 512, kZeroTurns = 2;
-// Thread t of T: the 16-byte chunks t, t + T, .. of the run at p, and the 2-byte values before the first and after the last.
+// Thread t of T: the 16-byte chunks t, t + T, .. of the run at p, and the 2-byte values before the first and after the
+// last.
 __device__ __forceinline__ void zero_run(char *p, int64_t bytes, int64_t t, int64_t T) {
   const int64_t head = min(bytes, (int64_t)((16 - ((uintptr_t)p & 15)) & 15)), chunks = (bytes - head) / 16;
   for (int64_t k = t; k < chunks; k += T) ((i32x4 *)(p + head))[k] = i32x4{0, 0, 0, 0};
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(1024) void embed_sort_kernel(const int64_t *ids, in
   }
 }
 
-// ---- sum ---------------------------------------------------------------------------------------------------------------
+// ---- sum ------------------------------------------------------------------------------------------------------------
 struct SumArgs {
   const void *grad;
   int64_t ldg;
@@ -328,8 +330,8 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
   const int items = a.pieces * a.colblocks;
   if (wave >= items) return;
   const int piece = wave / a.colblocks, c0 = (wave - piece * a.colblocks) * kCols;
-  // this piece's tokens and entries, one per lane; lanes kRun and kRun + 1 hold the entries before and behind it. What lies
-  // at or past start[V] is not there (and was not written).
+  // this piece's tokens and entries, one per lane; lanes kRun and kRun + 1 hold the entries before and behind it. What
+  // lies at or past start[V] is not there (and was not written).
   const int m = a.s.start[a.V], i0 = piece * kRun, i1 = min(m, i0 + kRun);
   const int at = lane < kRun ? i0 + lane : lane == kRun ? i0 - 1 : i0 + kRun;
   const bool there = at >= 0 && at < a.n;
@@ -377,7 +379,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
   flush(cur);
 }
 
-// ---- join --------------------------------------------------------------------------------------------------------------
+// ---- join -----------------------------------------------------------------------------------------------------------
 // The entry that starts in piece p and goes on behind it: its partial rows are row 1 of p and row 0 of the pieces up to
 // the one that holds its last token. The waves take them in turn, each in order, and are added in order.
 constexpr int kJoinWaves = 8, kJoinLoads = 8;
@@ -421,7 +423,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(SumArgs a) 
   store_entry<WT, VEC, ACC>(a, v, sum, c0, lane);
 }
 
-// ---- workspace ---------------------------------------------------------------------------------------------------------
+// ---- workspace ------------------------------------------------------------------------------------------------------
 static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 static size_t embed_ws(int64_t n, int64_t V, int64_t d, char *ws, SumArgs *a) {
   size_t off = 0;
@@ -469,16 +471,19 @@ template <int DT>
 static void go_fwd(const void *w, int64_t ldw, int64_t V, int d, const int64_t *ids, int64_t n, float scale, void *out,
                    int64_t ldo, hipStream_t st) {
   constexpr int B = Elem<DT>::bytes, PER = 16 / B;
-  const bool vec = d % PER == 0 && ldw % PER == 0 && ldo % PER == 0 && (uintptr_t)w % 16 == 0 && (uintptr_t)out % 16 == 0;
+  const bool vec = d % PER == 0 && ldw % PER == 0 && ldo % PER == 0 && (uintptr_t)w % 16 == 0 &&
+                   (uintptr_t)out % 16 == 0;
   constexpr int64_t kTokens = 4 * kLaunchRows;
   for (int64_t t0 = 0; t0 < n; t0 += kTokens) {
     const int64_t m = n - t0 < kTokens ? n - t0 : kTokens;
     const dim3 grid((unsigned)cdiv(m, 4), (unsigned)cdiv(d, 64 * kRowLoadsF * PER));
     char *o = (char *)out + t0 * ldo * B;
     if (vec)
-      hipLaunchKernelGGL((embed_fwd_kernel<DT, true>), grid, dim3(256), 0, st, w, ldw, V, d, ids + t0, m, scale, o, ldo);
+      hipLaunchKernelGGL((embed_fwd_kernel<DT, true>), grid, dim3(256), 0, st, w, ldw, V, d, ids + t0, m, scale, o,
+                         ldo);
     else
-      hipLaunchKernelGGL((embed_fwd_kernel<DT, false>), grid, dim3(256), 0, st, w, ldw, V, d, ids + t0, m, scale, o, ldo);
+      hipLaunchKernelGGL((embed_fwd_kernel<DT, false>), grid, dim3(256), 0, st, w, ldw, V, d, ids + t0, m, scale, o,
+                         ldo);
   }
 }
 
@@ -542,7 +547,8 @@ int octo_embed_bwd(const void *grad, int64_t ldg, int g_dtype, const int64_t *id
   a.ldw = ldw;
   a.accumulate = accumulate != 0;
   a.colblocks = (int)cdiv(d, kCols);
-  OCTO_CHECK_ARG((int64_t)a.pieces * a.colblocks < (int64_t)1 << 26, "embed_bwd: %lld tokens of width %d", (long long)n, d);
+  OCTO_CHECK_ARG((int64_t)a.pieces * a.colblocks < (int64_t)1 << 26, "embed_bwd: %lld tokens of width %d", (long long)n,
+                 d);
   ZeroFill z{};
   if (!accumulate) {
     const int64_t row = (int64_t)d * float_bytes(w_dtype);
@@ -551,7 +557,8 @@ int octo_embed_bwd(const void *grad, int64_t ldg, int g_dtype, const int64_t *id
     z.stride = ldw * float_bytes(w_dtype);
     z.bytes = one ? V * row : row;
     z.rows = one ? 1 : V;
-    const int64_t work = one ? cdiv(z.bytes, kZeroThreads * 16 * kZeroTurns) : cdiv(V * row, 65536);  // 64 KB of rows apart
+    // rows apart: 64 KB of them a workgroup
+    const int64_t work = one ? cdiv(z.bytes, kZeroThreads * 16 * kZeroTurns) : cdiv(V * row, 65536);
     z.blocks = (int)(work < (1 << 20) ? work : 1 << 20);
   }
   const int ranges = (int)cdiv(V, kBins);

@@ -427,7 +427,8 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
                         pre, post, use_tanh, cm);
   if (rc) return rc;
   if (ds) {
-    OCTO_CHECK_ARG(ds->K >= 1 && ds->K <= OCTO_LIST_MAX, "head_step_distill: K=%d outside [1, %d]", ds->K, OCTO_LIST_MAX);
+    OCTO_CHECK_ARG(ds->K >= 1 && ds->K <= OCTO_LIST_MAX, "head_step_distill: K=%d outside [1, %d]", ds->K,
+                   OCTO_LIST_MAX);
     OCTO_CHECK_ARG((ds->flags & ~OCTO_LIST_RAW) == 0, "head_step_distill: unknown flags %d", ds->flags);
     OCTO_CHECK_ARG(ds->teacher && ds->dots && ds->q && ds->g && ds->kl && ds->loss, "head_step_distill: null pointer");
   } else {
@@ -663,7 +664,8 @@ int head_step(const void *h, int64_t h_rows, int64_t ldh, int h_dtype, const voi
                                     n_max, d, V, flags, inv_T, pre, post, use_tanh, logp, ent, lse, rowout, 2, nullptr,
                                     z)
                        : merge_args(part, L.mtiles, h, ldh, h_dtype, w, ldw, w_dtype, w_scale, labels, idx, count,
-                                    n_max, d, V, flags, inv_T, pre, post, use_tanh, logp, ent, lse, out2, ld_out2, gt, z);
+                                    n_max, d, V, flags, inv_T, pre, post, use_tanh, logp, ent, lse, out2, ld_out2, gt,
+                                    z);
       m.row_off = r0;
       m.rows = rows;
       m.c = cm.c;

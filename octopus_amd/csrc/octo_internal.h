@@ -400,10 +400,11 @@ struct DistillArgs {
   int even;  // rowoff: xuse such that the row's dz scale is a power of two (launch_distill_even)
   float *loss;  // the last pass's entries: *loss as launch_distill_loss leaves it; else NULL
 };
-// dots[r][k] = h_r . W_ids[k], fp32 (0 for an empty slot); with xoff != NULL, the row's offset: its largest listed logit +
-// kExAbove (-inf for a row without a slot); flag_cnt[0 .. nflag) = 0.
+// dots[r][k] = h_r . W_ids[k], fp32 (0 for an empty slot); with xoff != NULL, the row's offset: its largest listed
+// logit + kExAbove (-inf for a row without a slot); flag_cnt[0 .. nflag) = 0.
 int launch_distill_dots(const DistillArgs &a, hipStream_t st);
-// The pass's rows: the row state, q, kl, g and, with rowoff, xuse and, without `even`, the flagged rows (launch_merge's).
+// The pass's rows: the row state, q, kl, g and, with rowoff, xuse and, without `even`, the flagged rows
+// (launch_merge's).
 int launch_distill_merge(const DistillArgs &a, hipStream_t st);
 // With `even`, in place of launch_ex_fix: the pass's exponentials moved to xuse, the rows' dz scales [rows].
 int launch_distill_even(const DistillArgs &a, float *scale, hipStream_t st);

@@ -159,9 +159,10 @@ struct ColStat {
   }
 };
 
-// One thread's part of a row's logsumexp at c = log2(e) / T: m the running maximum of the logits themselves (-inf before
-// any above it), S the sum of exp2((x - m) c). Against m and not m c: logits masked with the type's lowest value times c
-// overflow, and a row of nothing else still has its logsumexp. -inf adds nothing; a NaN or +inf makes S NaN for good.
+// One thread's part of a row's logsumexp at c = log2(e) / T: m the running maximum of the logits themselves (-inf
+// before any above it), S the sum of exp2((x - m) c). Against m and not m c: logits masked with the type's lowest value
+// times c overflow, and a row of nothing else still has its logsumexp. -inf adds nothing; a NaN or +inf makes S NaN for
+// good.
 struct RowSum {
   float m = -INFINITY, S = 0.f;
   // S against a maximum raised by -d / c; far below the new one it counts for nothing

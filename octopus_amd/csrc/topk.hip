@@ -4,20 +4,20 @@
 //   logp[r][j] = z_r,ids[j] / T - logsumexp_v(z_rv / T)
 //
 // One workgroup per row, one sweep over it. Of the values a workgroup has seen, at least k are no smaller than the k-th
-// largest of its threads' maxima, so that one is a lower bound of the list. It is taken after the first kTopLoads chunks
-// of every thread (32,768 values of 16 bits); from there on the sweep collects what reaches it (300 of 151,936 values at k
-// 64), and sums the row's exponentials as it goes. Every collected value is ranked against the others by (value, column),
-// and the first k ranks are the list. Where more than kCand values reach the bound (runs of equal values: rows with fewer
-// than k unmasked logits), a second sweep takes those above the bound of the whole row, and the rest of the list are the
-// first columns that equal it. A row with more than kCand even so, or with a NaN or +inf, is done by a radix select over the
-// values' 32-bit keys.
+// largest of its threads' maxima, so that one is a lower bound of the list. It is taken after the first kTopLoads
+// chunks of every thread (32,768 values of 16 bits); from there on the sweep collects what reaches it (300 of 151,936
+// values at k 64), and sums the row's exponentials as it goes. Every collected value is ranked against the others by
+// (value, column), and the first k ranks are the list. Where more than kCand values reach the bound (runs of equal
+// values: rows with fewer than k unmasked logits), a second sweep takes those above the bound of the whole row, and the
+// rest of the list are the first columns that equal it. A row with more than kCand even so, or with a NaN or +inf, is
+// done by a radix select over the values' 32-bit keys.
 //
-// Few rows: a row is cut into slices of a workgroup each (topk_slices), whose lists and sums a second launch joins the same
-// way.
+// Few rows: a row is cut into slices of a workgroup each (topk_slices), whose lists and sums a second launch joins the
+// same way.
 //
-// Bound by memory, 2 bytes a value at 16 bits: [2048, 151,936] bf16 at k 64 118 to 131 us (4.8 to 5.3 TB/s; a 4 GiB copy
-// moves 5.0), fp32 214 (5.8). Rows with 10 unmasked values 189 and 395 (by the radix select, whose counts of one value
-// wait for each other, 4,560 and 4,640).
+// Bound by memory, 2 bytes a value at 16 bits: [2048, 151,936] bf16 at k 64 118 to 131 us (4.8 to 5.3 TB/s; a 4 GiB
+// copy moves 5.0), fp32 214 (5.8). Rows with 10 unmasked values 189 and 395 (by the radix select, whose counts of one
+// value wait for each other, 4,560 and 4,640).
 #include "octo_common.h"
 #include "row_values.h"
 
@@ -29,7 +29,7 @@ constexpr int kCand = 2048;    // values that may reach the bound
 constexpr int kHits = 1536;    // chunks that may hold them
 constexpr int kJoin = 2048;    // entries a row's join takes from its slices
 constexpr int kTighten = 254;  // chunks from which on the whole row's bound is taken before they are looked through
-static_assert(kTighten * 8 + 2 * 7 <= kCand, "so many chunks' values, and those before and behind the chunks, have room");
+static_assert(kTighten * 8 + 2 * 7 <= kCand, "room for so many chunks' values, and those before and behind the chunks");
 
 // The order of the list as unsigned numbers: NaN above +inf, -0 equal to +0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -45,8 +45,8 @@ __device__ __forceinline__ uint64_t list_entry(float x, int col) {
   return ((uint64_t)order_key(x) << 32) | (uint32_t)~col;
 }
 
-// put(u, place) for the lanes whose wanted[u] is set, places counted on in *count: one atomic a wave for all of them, where
-// one per value waited for each in turn.
+// put(u, place) for the lanes whose wanted[u] is set, places counted on in *count: one atomic a wave for all of them,
+// where one per value waited for each in turn.
 template <int N, class F> __device__ __forceinline__ void append(const bool (&wanted)[N], int *count, F put) {
   uint64_t bal[N];
   int all = 0;
@@ -121,9 +121,9 @@ template <int N> __device__ __forceinline__ uint32_t kth_key(const uint32_t (&to
   }
   return bound;
 }
-// As a value. Up to kOneTop entries a thread's one maximum will do; for longer lists the maxima of its even and odd chunks
-// count each by itself, or k would be half the threads and the bound far below the k-th value (k 256 of 512 maxima: 1,640
-// chunks of a row of 151,936 collected, of 1,024 maxima 1,370).
+// As a value. Up to kOneTop entries a thread's one maximum will do; for longer lists the maxima of its even and odd
+// chunks count each by itself, or k would be half the threads and the bound far below the k-th value (k 256 of 512
+// maxima: 1,640 chunks of a row of 151,936 collected, of 1,024 maxima 1,370).
 constexpr int kOneTop = 64;
 __device__ __forceinline__ uint32_t kth_bound(const float (&top)[2], int k, int (*cnt)[15]) {
   if (k <= kOneTop) {
@@ -184,9 +184,9 @@ __device__ __forceinline__ void rank_values(uint64_t *cand, int n, int *ranks) {
 // SLICED: workgroup (r, s) takes the values s per .. s per + per of row r, and leaves its list as entries [r][s][k] (0
 // where the slice has fewer values) and its (maximum, sum) as sums [r][s].
 template <int DT, bool SLICED>
-__global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits, int64_t ld, int V_, float inv_T, int k_,
-                                                              int64_t *ids, float *logp, int per, uint64_t *entries,
-                                                              float *sums) {
+__global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits, int64_t ld, int V_, float inv_T,
+                                                              int k_, int64_t *ids, float *logp, int per,
+                                                              uint64_t *entries, float *sums) {
   constexpr int PER = 16 / Elem<DT>::bytes, NW = kTopThreads / 64;
   typedef typename Elem<DT>::T T;
   __shared__ float red[2][NW];
@@ -318,7 +318,8 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
     }
   };
   if (__builtin_expect(listed && more, 0)) {
-    // ---- runs of equal values at the bound (fewer than k unmasked logits, say): those above it, then its first columns
+    // ---- runs of equal values at the bound (fewer than k unmasked logits, say): those above it, then its first
+    // columns
     least = kth_value(top, k, bound, bits[2]);
     if (threadIdx.x == 0) ncand = 0;  // read by all before the barriers of kth_value
     __syncthreads();
@@ -331,7 +332,8 @@ __global__ __launch_bounds__(kTopThreads, 6) void topk_kernel(const void *logits
     __syncthreads();
     n = ncand;
     if (n < k) {  // k values at least are no smaller than `least`
-      first_of(k - n, [&](float x) { return x == least; }, [&](int at, float x, int j) { cand[n + at] = list_entry(x, j); });
+      first_of(k - n, [&](float x) { return x == least; },
+               [&](int at, float x, int j) { cand[n + at] = list_entry(x, j); });
       n = k;
     }
   }
@@ -424,15 +426,16 @@ __global__ __launch_bounds__(kTopThreads) void topk_join_kernel(const uint64_t *
   __syncthreads();
   const int got = ncand;
   rank_values(cand, got, ranks);
-  for (int i = threadIdx.x; i < got; i += kTopThreads) write_value(cand[i], ranks[i], r, k, st.m, lnS, inv_T, ids, logp);
+  for (int i = threadIdx.x; i < got; i += kTopThreads)
+    write_value(cand[i], ranks[i], r, k, st.m, lnS, inv_T, ids, logp);
 }
 
-// Slices a row of V values is cut into for n rows: rows of 192 KB and of 60,000 values and more, up to 128 of them, four
-// slices at least. us a call in a captured graph at k 64, whole and sliced, for 1, 16 and 128 rows. bf16, V 151,936: 21.0
-// and 15.5, 21.7 and 15.5, 23.0 and 21.8; 100,000 (195 KB): 17.0 and 15.3, 17.6 and 15.4, 19.1 and 17.8; 64,000 (125 KB): 12.9
-// and 15.2, 13.7 and 15.2, 13.6 and 16.3. fp32, V 64,000 (250 KB): 15.0 and 14.7, 15.8 and 14.9, 17.0 and 16.5; 49,152 (192
-// KB): 13.5 and 14.8, 13.6 and 14.8, 14.2 and 15.8. More rows or longer lists lose by it: 256 rows 25.2 and 28.2, k 256 28
-// and 50.
+// Slices a row of V values is cut into for n rows: rows of 192 KB and of 60,000 values and more, up to 128 of them,
+// four slices at least. us a call in a captured graph at k 64, whole and sliced, for 1, 16 and 128 rows. bf16, V
+// 151,936: 21.0 and 15.5, 21.7 and 15.5, 23.0 and 21.8; 100,000 (195 KB): 17.0 and 15.3, 17.6 and 15.4, 19.1 and 17.8;
+// 64,000 (125 KB): 12.9 and 15.2, 13.7 and 15.2, 13.6 and 16.3. fp32, V 64,000 (250 KB): 15.0 and 14.7, 15.8 and 14.9,
+// 17.0 and 16.5; 49,152 (192 KB): 13.5 and 14.8, 13.6 and 14.8, 14.2 and 15.8. More rows or longer lists lose by it:
+// 256 rows 25.2 and 28.2, k 256 28 and 50.
 constexpr int kMaxSlices = 16, kSliceK = 128;
 static int topk_slices(int64_t n, int V, int k, int dtype) {
   if (n < 1 || n > 128 || k > kSliceK || V < 60000 || (int64_t)V * float_bytes(dtype) < 192 * 1024) return 1;
@@ -446,11 +449,14 @@ static void go_topk(const void *logits, int64_t ld, int dtype, int64_t n, int V,
                     float *logp, int slices, int per, uint64_t *entries, float *sums, hipStream_t st) {
   const dim3 g((unsigned)n, (unsigned)slices), b(kTopThreads);
   if (dtype == OCTO_BF16)
-    hipLaunchKernelGGL((topk_kernel<OCTO_BF16, SLICED>), g, b, 0, st, logits, ld, V, inv_T, k, ids, logp, per, entries, sums);
+    hipLaunchKernelGGL((topk_kernel<OCTO_BF16, SLICED>), g, b, 0, st, logits, ld, V, inv_T, k, ids, logp, per, entries,
+                       sums);
   else if (dtype == OCTO_F16)
-    hipLaunchKernelGGL((topk_kernel<OCTO_F16, SLICED>), g, b, 0, st, logits, ld, V, inv_T, k, ids, logp, per, entries, sums);
+    hipLaunchKernelGGL((topk_kernel<OCTO_F16, SLICED>), g, b, 0, st, logits, ld, V, inv_T, k, ids, logp, per, entries,
+                       sums);
   else
-    hipLaunchKernelGGL((topk_kernel<OCTO_F32, SLICED>), g, b, 0, st, logits, ld, V, inv_T, k, ids, logp, per, entries, sums);
+    hipLaunchKernelGGL((topk_kernel<OCTO_F32, SLICED>), g, b, 0, st, logits, ld, V, inv_T, k, ids, logp, per, entries,
+                       sums);
 }
 
 }  // namespace octo
@@ -487,16 +493,17 @@ int octo_topk(const void *logits, int64_t ld, int dtype, int64_t n, int V, float
   const int slices = topk_slices(n, V, k, dtype);
   if (slices == 1) {
     for (int64_t r0 = 0; r0 < n; r0 += kLaunchRows)
-      go_topk<false>((const char *)logits + r0 * ld * float_bytes(dtype), ld, dtype, n - r0 < kLaunchRows ? n - r0 : kLaunchRows,
-                     V, inv_T, k, ids + r0 * k, logp + r0 * k, 1, 0, nullptr, nullptr, st);
+      go_topk<false>((const char *)logits + r0 * ld * float_bytes(dtype), ld, dtype,
+                     n - r0 < kLaunchRows ? n - r0 : kLaunchRows, V, inv_T, k, ids + r0 * k, logp + r0 * k, 1, 0,
+                     nullptr, nullptr, st);
   } else {
     const int per = (int)round_up(cdiv(V, slices), 64);  // the last slice has the rest, at least one value
     uint64_t *entries = (uint64_t *)ws;
     float *sums = (float *)(entries + n * slices * k);
     go_topk<true>(logits, ld, dtype, n, V, inv_T, k, ids, logp, slices, per, entries, sums, st);
     OCTO_CHECK_LAUNCH("topk");
-    hipLaunchKernelGGL(topk_join_kernel, dim3((unsigned)n), dim3(kTopThreads), 0, st, entries, sums, slices, k, inv_T, ids,
-                       logp);
+    hipLaunchKernelGGL(topk_join_kernel, dim3((unsigned)n), dim3(kTopThreads), 0, st, entries, sums, slices, k, inv_T,
+                       ids, logp);
   }
   OCTO_CHECK_LAUNCH("topk");
   return OCTO_OK;

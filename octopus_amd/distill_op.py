@@ -2,12 +2,12 @@
 
     head_topk                          the teacher's list: the k largest logits of a row and their log-probabilities
     octohead::distill_columns_fwd/bwd  the student's divergence from the lists over materialised logits
-    octohead::head_step_distill        the same from hidden rows and the vocabulary weight, loss and gradients in one call
+    octohead::head_step_distill        the same from hidden rows and the vocabulary weight, with both gradients
 
 A row's list is K slots (ids[r, k], teacher[r, k]): tokens, and the teacher's logits or log-probabilities of them, as
-head_topk gives them. A slot whose id lies outside [0, V) or whose teacher value is -inf is empty (shorter lists), and the
-same token may stand in several slots. With q the softmax of the teacher's values over a row's slots and p = softmax(z /
-T) the student's distribution over the whole vocabulary,
+head_topk gives them. A slot whose id lies outside [0, V) or whose teacher value is -inf is empty (shorter lists), and
+the same token may stand in several slots. With q the softmax of the teacher's values over a row's slots and p =
+softmax(z / T) the student's distribution over the whole vocabulary,
 
     kl_r = sum_k q_k (log q_k - log p_ids[k])                             (a row without a slot: 0)
     dL/dz_v = g_r (Q p_v - sum of q_k over the slots of v) / T,  Q = sum q,  g_r = dL/dkl_r.
@@ -47,7 +47,7 @@ def _inv_T(temperature: float) -> float:
     return inv_T
 
 
-# ---- the teacher's list ------------------------------------------------------------------------------------------------
+# ---- the teacher's list ----------------------------------------------------------------------------------------------
 
 def _topk(logits: Tensor, inv_T: float, k: int) -> tuple[Tensor, Tensor]:
     dev = _on_gpu(logits)
@@ -86,7 +86,7 @@ def head_topk(logits: Tensor, temperature: float, k: int) -> tuple[Tensor, Tenso
     return topk(logits, inv_T, k) if torch.compiler.is_compiling() else _topk(logits, inv_T, k)
 
 
-# ---- the divergence over materialised logits -----------------------------------------------------------------------------
+# ---- the divergence over materialised logits -------------------------------------------------------------------------
 
 def _columns_fwd(logits: Tensor, ids: Tensor, teacher: Tensor, inv_T: float, raw: bool) -> tuple[Tensor, ...]:
     """(kl, state, q, and the logits and ids as the kernels read them)."""
@@ -202,7 +202,7 @@ def distill_columns(logits: Tensor, temperature: float, ids: Tensor, teacher: Te
     return _Columns.apply(*args) if torch.is_grad_enabled() and logits.requires_grad else _columns_fwd(*args)[0]
 
 
-# ---- the divergence from hidden rows: loss and gradients in one call ------------------------------------------------------
+# ---- the divergence from hidden rows: loss and gradients in one call -------------------------------------------------
 
 def _apart(x: Tensor) -> Tensor:
     """x with rows that do not overlap (a broadcast one's are one row)."""
@@ -225,7 +225,8 @@ def _step(rows: Tensor, weight: Tensor, w_scale: Optional[Tensor], ids: Tensor, 
     if count is not None and (count.dtype != torch.int32 or not count.numel()):
         raise ValueError(f"octohead: a row count of int32 expected (compact_rows), got {count.dtype}")
     if w_scale is not None and (w_scale.dtype != torch.float32 or w_scale.shape != weight2.shape[:1]):
-        raise ValueError(f"octohead: one fp32 scale per weight row expected, got {w_scale.dtype} {tuple(w_scale.shape)}")
+        raise ValueError(f"octohead: one fp32 scale per weight row expected, got {w_scale.dtype} "
+                         f"{tuple(w_scale.shape)}")
     w_scale = None if w_scale is None else w_scale.contiguous()
     n_max = idx.numel() if idx is not None else rows2.shape[0]
     V, d = weight2.shape
@@ -327,8 +328,8 @@ torch.library.register_autograd("octohead::head_step_distill", _step_backward, s
 def _step_later(rows: Tensor, weight: Tensor, ids: Tensor, teacher: Tensor, row_weight: Optional[Tensor],
                 idx: Optional[Tensor], count: Optional[Tensor], inv_T: float, pre: float, post: float, use_tanh: bool,
                 raw: bool, need_rows: bool, nbytes: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    """(loss, kl, grad_rows, the buffer of nbytes that later_grad_w makes grad_weight of, the row count as the call found
-    it)."""
+    """(loss, kl, grad_rows, the buffer of nbytes that later_grad_w makes grad_weight of, the row count as the call
+    found it)."""
     n_max = idx.numel() if idx is not None else rows.shape[0]
     kept_count = torch.full((1,), n_max, dtype=torch.int32, device=rows.device) if count is None \
         else count.reshape(-1)[:1].to(torch.int32, copy=True)
@@ -360,8 +361,8 @@ def _later_backward(ctx, gloss):
 
 class _Head(torch.autograd.Function):
     """The step outside a trace. It holds its gradients (or operands) for itself, so that the last backward scales them
-    where they lie, which ends at once for a loss that is not scaled; a copy reads and writes [V, d] ([151,936, 2560] bf16
-    267 us)."""
+    where they lie, which ends at once for a loss that is not scaled; a copy reads and writes [V, d] ([151,936, 2560]
+    bf16 267 us)."""
 
     @staticmethod
     def forward(ctx, rows, weight, w_scale, ids, teacher, row_weight, idx, count, xf, need_rows, need_weight, nbytes):
@@ -371,7 +372,8 @@ class _Head(torch.autograd.Function):
             output = _step_later(*inputs)
             _later_setup(ctx, inputs, output)
         else:
-            output = _step(rows, weight, w_scale, ids, teacher, row_weight, idx, count, *xf, need_rows, need_weight, None)
+            output = _step(rows, weight, w_scale, ids, teacher, row_weight, idx, count, *xf, need_rows, need_weight,
+                           None)
             ctx.grads, ctx.need, ctx.of = output[2:], (need_rows, need_weight), (rows, weight)
             ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(output[1])
@@ -400,15 +402,17 @@ def fused_distill_head(rows: Tensor, weight: Tensor, ids: Tensor, teacher: Tenso
                        idx: Optional[Tensor] = None, count: Optional[Tensor] = None,
                        w_scale: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
     """(loss, kl): loss = sum over the rows of row_weight x kl (None: 1 each), z = post(rows W^T), and kl [rows] fp32
-    detached, from one call that computes the logits once and also the gradients of the loss in rows and weight (each when
-    it requires grad and grad mode is on). loss.backward() only scales them or, for a short call, makes the weight's from
-    the operands kept, as fused_grpo_head's. ids and teacher are [rows, K], row_weight [rows]. idx, count: the rows that
-    take part (ascending, as compact_rows gives them; count on the device); the others' kl and gradients are 0. A row of
-    weight 0 adds nothing to the loss, but is computed with: leave rows out by idx. bf16, f16, fp32 and fp8 weights
-    (w_scale; no gradient of those).
-    The prefix tree's teacher values depend on the path alone, so a tree's rows are its positions, each once, weighted by
-    the tokens that share it. The gradients or operands, and rows and weight by
-    reference, are held from this call until the graph goes. The gradients have no derivative of their own: one raises."""
+    detached, from one call that computes the logits once and also the gradients of the loss in rows and weight (each
+    when it requires grad and grad mode is on). loss.backward() only scales them or, for a short call, makes the
+    weight's from the operands kept, as fused_grpo_head's. ids and teacher are [rows, K], row_weight [rows]. idx, count:
+    the rows that take part (ascending, as compact_rows gives them; count on the device); the others' kl and gradients
+    are 0. A row of weight 0, or without a slot, adds nothing to the loss, but is computed with: leave rows out by idx,
+    and those whose hidden values may be no numbers have to be. bf16, f16, fp32 and fp8 weights (w_scale; no gradient of
+    those). The gradients are formed at row_weight's scale and rounded to the operands' type there; in f16 a loss scale
+    belongs into row_weight, since loss.backward() multiplies what is rounded already.
+    The prefix tree's teacher values depend on the path alone, so a tree's rows are its positions, each once, weighted
+    by the tokens that share it. The gradients or operands, and rows and weight by reference, are held from this call
+    until the graph goes. The gradients have no derivative of their own: one raises."""
     inv_T = _inv_T(temperature)
     if rows.dim() != 2 or weight.dim() != 2:
         raise ValueError(f"octohead: rows [n, d] and weight [V, d] expected, got {tuple(rows.shape)} and "

@@ -3,8 +3,8 @@
     octohead::embed_fwd / embed_bwd    scale W[ids], and the gradient in W over the whole vocabulary
     octohead::embed_grad_add           the same gradient added to rows of a gradient that exists already
 
-The other end of the vocabulary matrix that the head multiplies with: a model with tied weights looks its tokens up in W,
-and both gradients belong to the one [V, d] tensor. HIP tensors only; all work is queued on the current stream of the
+The other end of the vocabulary matrix that the head multiplies with: a model with tied weights looks its tokens up in
+W, and both gradients belong to the one [V, d] tensor. HIP tensors only; all work is queued on the current stream of the
 tensors' device, nothing synchronises with the host.
 """
 
@@ -46,8 +46,9 @@ def _on_gpu(*tensors: Optional[Tensor]) -> torch.device:
 
 
 def _call_on(dev: torch.device, name: str, *args) -> None:
-    """_lib.call on dev's current stream, its last argument, with dev current. The raw handle, and no entering of a device
-    that is current already: the stream's Python object alone takes 10 us in a backward's thread, a tenth of a short call."""
+    """_lib.call on dev's current stream, its last argument, with dev current. The raw handle, and no entering of a
+    device that is current already: the stream's Python object alone takes 10 us in a backward's thread, a tenth of a
+    short call."""
     stream = ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(dev.index))
     if torch.cuda.current_device() == dev.index:
         _lib.call(name, *args, stream)
@@ -144,8 +145,8 @@ def _setup(ctx, inputs, output):
 
 
 def _backward(ctx, gout, gradient=_embed_bwd):
-    """The registered op's own backward calls the registered gradient: a tracer runs it on tensors without data, and with
-    create_graph its result depends on gout, whose derivative is refused and not left out."""
+    """The registered op's own backward calls the registered gradient: a tracer runs it on tensors without data, and
+    with create_graph its result depends on gout, whose derivative is refused and not left out."""
     (ids,) = ctx.saved_tensors
     V, scale, padding_idx, dtype = ctx.params
     gw = gradient(gout, ids, V, scale, padding_idx, dtype) if ctx.needs_input_grad[0] else None
@@ -156,8 +157,8 @@ torch.library.register_autograd("octohead::embed_fwd", _backward, setup_context=
 
 
 class _Embed(torch.autograd.Function):
-    """embed_fwd outside a trace: the registered op's own bookkeeping takes longer on the host than the kernel does for a
-    step's tokens (16 tokens: 31 us a call through the op, 13 through the library)."""
+    """embed_fwd outside a trace: the registered op's own bookkeeping takes longer on the host than the kernel does for
+    a step's tokens (16 tokens: 31 us a call through the op, 13 through the library)."""
 
     @staticmethod
     def forward(ctx, weight, ids, scale, padding_idx):
@@ -179,9 +180,9 @@ def _padding(padding_idx: Optional[int], V: int) -> int:
 
 
 def embed_rows(weight: Tensor, ids: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
-    """[*ids.shape, d] in weight's dtype: scale x weight[ids], the product formed in fp32 and rounded once; zeros for an id
-    outside [0, V) (a packed stream's filling). Differentiable in weight: embed_bwd's gradient, dense over the vocabulary.
-    padding_idx: an entry that is looked up and gets no gradient."""
+    """[*ids.shape, d] in weight's dtype: scale x weight[ids], the product formed in fp32 and rounded once; zeros for an
+    id outside [0, V) (a packed stream's filling). Differentiable in weight: embed_bwd's gradient, dense over the
+    vocabulary. padding_idx: an entry that is looked up and gets no gradient."""
     if weight.dim() != 2:
         raise ValueError(f"octohead: weight must be [V, d], got {tuple(weight.shape)}")
     pad = _padding(padding_idx, weight.shape[0])

@@ -12,8 +12,8 @@ pytestmark = pytest.mark.gpu
 def test_a_soft_cap_of_negative_slope_keeps_the_roundings(later, monkeypatch):
     """z = 30 tanh(-x / 30): the weight gradient of bf16 operands takes two roundings of half a step each, the listed
     values' and the result's, as with a positive slope. Roundings of one size add in squares, so its error lies below
-    sqrt(2.5) times the one that the exact gradient's own rounding costs; a third (h^T times a scale that is not a power of
-    two) would bring it to sqrt(3)."""
+    sqrt(2.5) times the one that the exact gradient's own rounding costs; a third (h^T times a scale that is not a power
+    of two) would bring it to sqrt(3)."""
     from octopus_amd import distill_op, head_op
     from octopus_amd.head_op import Post
 
@@ -27,7 +27,8 @@ def test_a_soft_cap_of_negative_slope_keeps_the_roundings(later, monkeypatch):
     monkeypatch.setattr(head_op, "_LATER_WORK", 1 << 62)
     hd, wd = h.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
     assert (distill_op._later_bytes(hd, wd, None, True, True) > 0) == later
-    loss, kl = distill_op.fused_distill_head(hd, wd, ids.cuda(), t.cuda(), 1.0, rw.cuda(), post=Post(-1 / cap, cap, True))
+    loss, kl = distill_op.fused_distill_head(hd, wd, ids.cuda(), t.cuda(), 1.0, rw.cuda(),
+                                             post=Post(-1 / cap, cap, True))
     loss.backward()
     th = torch.tanh(-(h.double() @ w.double().T) / cap)
     want_kl, dkl = odist.divergence(cap * th, ids, t)
@@ -51,9 +52,8 @@ def test_only_one_output_of_the_registered_ops_is_differentiable():
     from octopus_amd import distill_op
 
     h, w, ids, t = _small()
-    step = lambda: distill_op.head_step_distill(h, w, None, ids, t, None, None, None, 1.0, 1.0, 1.0, False, False,  # noqa
-                                                True, True)
-    loss, kl, gh, gw = step()
+    loss, kl, gh, gw = distill_op.head_step_distill(h, w, None, ids, t, None, None, None, 1.0, 1.0, 1.0, False, False,
+                                                    True, True)
     for out in (kl.sum(), gh.float().sum(), gw.float().sum(), loss + kl.sum()):
         with pytest.raises(RuntimeError, match="only loss"):
             torch.autograd.grad(out, (h, w), retain_graph=True)
@@ -89,8 +89,8 @@ def test_traced_steps():
 
 
 def test_a_traced_lookup_and_its_second_derivative():
-    """embed_rows through a tracer has the eager call's gradient; the registered op's gradient, differentiated again, raises
-    also as part of a larger expression."""
+    """embed_rows through a tracer has the eager call's gradient; the registered op's gradient, differentiated again,
+    raises also as part of a larger expression."""
     from octopus_amd import embed_op
 
     ids = torch.tensor([[3, 0, 3], [7, -1, 9]], device="cuda")
@@ -111,8 +111,9 @@ def test_a_traced_lookup_and_its_second_derivative():
 
 @pytest.mark.parametrize("form", ["step", "later", "registered", "columns", "columns_apart", "registered_columns"])
 def test_second_derivatives_inside_a_larger_expression(form, monkeypatch):
-    """A penalty on the gradient beside a term that has a derivative: the penalty's own raises by every way that asks for
-    it, where a constant in its place would leave it out without a word. The first derivatives are the plain ones."""
+    """A penalty on the gradient beside a term that has a derivative: the penalty's own raises by every way that asks
+    for it, where a constant in its place would leave it out without a word. The first derivatives are the plain
+    ones."""
     from octopus_amd import distill_op, head_op
 
     h, w, ids, t = _small(seed=5)
@@ -121,8 +122,9 @@ def test_second_derivatives_inside_a_larger_expression(form, monkeypatch):
     monkeypatch.setattr(head_op, "_LATER_WEIGHTS", 0 if form == "later" else 1 << 62)
     monkeypatch.setattr(head_op, "_LATER_WORK", 1 << 62)
     if "columns" in form:
-        base = torch.randn(300, 6, generator=torch.Generator().manual_seed(7)).cuda() if form == "columns_apart" else None
-        x = (torch.randn(6, 300, generator=torch.Generator().manual_seed(7)).cuda() if base is None else base.T)
+        shape = (300, 6) if form == "columns_apart" else (6, 300)
+        x = torch.randn(shape, generator=torch.Generator().manual_seed(7)).cuda()
+        x = x.T if form == "columns_apart" else x
         leaves = (x.detach().requires_grad_(True),)
         call = distill_op.distill_columns_fwd if form == "registered_columns" else None
         f = lambda: (call(leaves[0], ids, t, 1.0, False)[0] if call  # noqa: E731
@@ -165,11 +167,11 @@ def _fastest(f, calls=10, turns=5):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("V,d,ld,off", [(1, 1, 1, 0), (1, 3, 9, 5), (3, 1, 1, 1), (5, 7, 7, 3), (37, 41, 41, 0),
-                                        (37, 41, 41, 1), (37, 41, 45, 2), (700, 64, 64, 4), (3, 5, 8, 7), (513, 1031, 1031, 6),
-                                        (40, 2047, 2050, 1)])
+                                        (37, 41, 41, 1), (37, 41, 45, 2), (700, 64, 64, 4), (3, 5, 8, 7),
+                                        (513, 1031, 1031, 6), (40, 2047, 2050, 1)])
 def test_gradients_zeros_end_where_it_does(dtype, V, d, ld, off):
-    """The dense gradient at every offset from a 16-byte boundary, of odd lengths, with and without gaps between its rows:
-    zeros where no token is, and nothing written around it."""
+    """The dense gradient at every offset from a 16-byte boundary, of odd lengths, with and without gaps between its
+    rows: zeros where no token is, and nothing written around it."""
     import ctypes
 
     from octopus_amd import _lib
@@ -193,8 +195,8 @@ def test_gradients_zeros_end_where_it_does(dtype, V, d, ld, off):
 
 
 def test_a_gradient_of_few_tokens_is_not_slower_than_a_fill():
-    """fp32, an odd vocabulary of odd width, which no row of ends on a 16-byte boundary: a fill and an index_add_ take 261
-    us, value-wise zeros made it 339, now 246."""
+    """fp32, an odd vocabulary of odd width, which no row of ends on a 16-byte boundary: a fill and an index_add_ take
+    261 us, value-wise zeros made it 339, now 246."""
     from octopus_amd.embed_op import embed_bwd
 
     V, d, n = 151935, 2559, 8
@@ -206,8 +208,8 @@ def test_a_gradient_of_few_tokens_is_not_slower_than_a_fill():
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_odd_widths_cost_about_what_even_ones_do(dtype):
-    """The gradient of 1,501 tokens over [31,999, 1023] beside [32,000, 1024]: 95 and 26 us with loads that waited for each
-    other, now 30 and 26; values that are no numbers stay in their columns, at the last one too."""
+    """The gradient of 1,501 tokens over [31,999, 1023] beside [32,000, 1024]: 95 and 26 us with loads that waited for
+    each other, now 30 and 26; values that are no numbers stay in their columns, at the last one too."""
     from octopus_amd.embed_op import embed_bwd
 
     def one(V, d):
@@ -256,8 +258,8 @@ def test_lists_of_few_values_above_a_run_of_equal_ones(dtype, V, k):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("mask", [-torch.inf, -1e30])
 def test_masked_rows_cost_a_second_sweep(dtype, mask):
-    """512 rows of 151,936 with 10 unmasked logits each, k 64: below 6 times the time of unmasked rows (34 times as a radix
-    select over one bin)."""
+    """512 rows of 151,936 with 10 unmasked logits each, k 64: below 6 times the time of unmasked rows (34 times as a
+    radix select over one bin)."""
     from octopus_amd.distill_op import head_topk
 
     z = torch.randn(512, 151936, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
@@ -268,7 +270,8 @@ def test_masked_rows_cost_a_second_sweep(dtype, mask):
 
 @pytest.mark.parametrize("grad", [False, True])
 def test_more_hidden_rows_than_a_launch_has_threads_for(grad):
-    """2^24 rows and more, each a workgroup of 256 threads: the last rows' divergences and gradients are a small call's."""
+    """2^24 rows and more, each a workgroup of 256 threads: the last rows' divergences and gradients are a small
+    call's."""
     from octopus_amd.distill_op import fused_distill_head
 
     n, d, V, K, few = (1 << 24) + 5, 8, 9, 25, 70
@@ -289,9 +292,10 @@ def test_more_hidden_rows_than_a_launch_has_threads_for(grad):
 
 
 def test_a_confident_student_beside_its_list(monkeypatch):
-    """bf16, one listed token of probability near 0 and a student that puts more than half of its mass on another: 0.3 of
-    dz's square are dense entries. Every entry that weighs takes one rounding and the gradient's own is the second, so its
-    error is sqrt(2) times that of the exact gradient rounded, below sqrt(2.2). Dense entries rounded twice: sqrt(2.3)."""
+    """bf16, one listed token of probability near 0 and a student that puts more than half of its mass on another: 0.3
+    of dz's square are dense entries. Every entry that weighs takes one rounding and the gradient's own is the second,
+    so its error is sqrt(2) times that of the exact gradient rounded, below sqrt(2.2). Dense entries rounded twice:
+    sqrt(2.3)."""
     from octopus_amd import distill_op, head_op
 
     n, d, V = 400, 256, 16384
