@@ -85,11 +85,14 @@ struct ZeroFill {
   int64_t stride, bytes, rows;
   int blocks;
 };
-// A workgroup's first kZeroThreads threads write kZeroTurns chunks each: memory takes stores best from few waves at a
-// time that move through it as one front. us of an fp32 gradient of 8 tokens, [151,936, 2560] and [151,935, 2559], and
-// a bf16 one of 1,501 tokens, [32,000, 1024]: 242, 246, 26; one turn 230, 233, 28; all 1,024 threads, one turn 255,
-// 258, 27, four turns 274, .., 26 (a fill and an index_add_: 262, 261, 91).
-constexpr int kZeroThreads = 512, kZeroTurns = 2;
+// A workgroup's first kZeroThreads threads write one chunk each, or two of a gradient below kZeroTwo bytes: memory
+// takes stores best from few waves at a time that move through it as one front, and a small gradient is bound by the
+// launching of the workgroups. us of embed_bwd, one and two: fp32, 8 tokens, [151,936, 2560] (1.56 GB) 230 and 242,
+// [64,000, 2304] (590 MB) 93 and 99; bf16, 8 tokens, [151,936, 2560] (778 MB) 121 and 126; 1,501 tokens, f16 [64,000,
+// 2304] (295 MB) 63 and 60, bf16 [32,000, 1024] (66 MB) 28 and 26. All 1,024 threads, four each, a quarter of the
+// gradient apart: 274, 111, 141, 61, 26; a fill and an index_add_ in fp32: 261, 119.
+constexpr int kZeroThreads = 512;
+constexpr int64_t kZeroTwo = 512 << 20;
 // Thread t of T: the 16-byte chunks t, t + T, .. of the run at p, and the 2-byte values before the first and after the
 // last.
 __device__ __forceinline__ void zero_run(char *p, int64_t bytes, int64_t t, int64_t T) {
@@ -558,7 +561,7 @@ int octo_embed_bwd(const void *grad, int64_t ldg, int g_dtype, const int64_t *id
     z.bytes = one ? V * row : row;
     z.rows = one ? 1 : V;
     // rows apart: 64 KB of them a workgroup
-    const int64_t work = one ? cdiv(z.bytes, kZeroThreads * 16 * kZeroTurns) : cdiv(V * row, 65536);
+    const int64_t work = one ? cdiv(z.bytes, kZeroThreads * 16 * (z.bytes < kZeroTwo ? 2 : 1)) : cdiv(V * row, 65536);
     z.blocks = (int)(work < (1 << 20) ? work : 1 << 20);
   }
   const int ranges = (int)cdiv(V, kBins);

@@ -195,8 +195,8 @@ def test_gradients_zeros_end_where_it_does(dtype, V, d, ld, off):
 
 
 def test_a_gradient_of_few_tokens_is_not_slower_than_a_fill():
-    """fp32, an odd vocabulary of odd width, which no row of ends on a 16-byte boundary: a fill and an index_add_ take
-    261 us, value-wise zeros made it 339, now 246."""
+    """fp32, an odd vocabulary of odd width, where no row ends on a 16-byte boundary: a fill and an index_add_ take 261
+    us, value-wise zeros made it 339, now 231."""
     from octopus_amd.embed_op import embed_bwd
 
     V, d, n = 151935, 2559, 8
