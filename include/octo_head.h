@@ -87,6 +87,7 @@ extern "C" {
 #define OCTO_WS_NO_GRADH    256  /* octo_head_workspace_bytes / octo_head_bwd_plan: without grad_h        */
 #define OCTO_PAIRS_NONE_AS_COUNT 1 /* octo_label_pairs: positions without a pair get the pair count  */
 #define OCTO_LIST_MAX        256 /* octo_topk, octo_distill_*: the most entries of a row's list           */
+#define OCTO_DRAFTS_MAX       63 /* octo_verify_drafts: the most drafts of a sequence                        */
 #define OCTO_ROW_MAX   (1 << 30) /* octo_topk, octo_distill_columns_*, octo_embed_*: the largest vocabulary  */
 #define OCTO_LIST_RAW          1 /* octo_distill_*: q = exp(t) as given, not the softmax over the row's list */
 
@@ -339,6 +340,55 @@ int octo_gather_f32(const float *src, int64_t ld_src, const int64_t *idx, const 
  * weight format of its fp8-weight configuration (per-row scale = absmax / 448) on the device. */
 int octo_quantise_fp8_rows(const void *w, int64_t ldw, int w_dtype, int64_t V, int d,
                            uint8_t *q, int64_t ldq, float *scale, void *stream);
+
+/* Rows held as 8-bit integers (no counterpart in the reference): x [rows, ldx] (BF16, F16 or F32), group 0 (the row),
+ * 32, 64, 128 or 256 values to a scale, groups = group ? ceil(d / group) : 1. Of each group, with a = max |x|:
+ *   scale[r * groups + j] = a / 127 in fp32;  q[r * ldq + k] = x / scale to the nearest integer, ties to even
+ * from the exact quotient; a < 2^-119: scale 0 and zeros; a not finite: scale NaN and zeros. ldq is a multiple of 16 and
+ * q 16-byte aligned; the bytes from d up to the next multiple of 16 are written 0. Rows of x may start at any element.
+ * octo_widen_i8_rows: out[r, k] = q scale, rounded once to out_dtype. */
+int octo_quantise_i8_rows(const void *x, int64_t ldx, int x_dtype, int64_t rows, int d, int group, int8_t *q,
+                          int64_t ldq, float *scale, void *stream);
+int octo_widen_i8_rows(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int d, int group, void *out,
+                       int64_t ldo, int out_dtype, void *stream);
+
+/* The head's logits from 8-bit integers (no counterpart in the reference):
+ *   logits[r, v] = x_scale[r] w_scale[v] sum_k xq[r, k] wq[v, k], the sum exact, rounded once to z_dtype
+ * for n rows of x (quantised here as octo_quantise_i8_rows does, group 0, into xq and x_scale) or, with rows NULL, of xq
+ * and x_scale as they are. wq [V, ldw], xq [n, ldxq]: strides multiples of 16, 16-byte aligned, readable up to the next
+ * multiple of 16 behind d (xq's bytes there 0; wq's may be any). d <= 131,072; V, n <= 2^21. logits [n, ldz] may start
+ * at any element. */
+int octo_head_logits_i8(const void *rows, int64_t ldx, int x_dtype, const int8_t *wq, int64_t ldw, const float *w_scale,
+                        int64_t n, int d, int V, int8_t *xq, int64_t ldxq, float *x_scale, void *logits, int64_t ldz,
+                        int z_dtype, void *stream);
+/* Its gradients for g = dL/dlogits [n, ldg], straight through the rounding (NULL skips one):
+ *   grad_rows[r, k] = sum_v g[r, v] w_scale[v] wq[v, k];  grad_w[v, k] = sum_r g[r, v] x_scale[r] xq[r, k]
+ * The products run in g's type (F32 as three bf16 parts), the 8-bit operand times its scale rounded once to it, summed
+ * in fp32 and rounded once. ws: octo_head_grads_i8_workspace_bytes, 256-byte aligned. */
+int octo_head_grads_i8_workspace_bytes(int64_t n, int d, int V, int dtype, int need_rows, int need_w, size_t *bytes);
+int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq, int64_t ldxq, const float *x_scale,
+                       const int8_t *wq, int64_t ldw, const float *w_scale, int64_t n, int d, int V, void *grad_rows,
+                       int64_t ld_gr, int gr_dtype, void *grad_w, int64_t ld_gw, int gw_dtype, void *ws,
+                       size_t ws_bytes, void *stream);
+
+/* Drafted tokens checked against the target's probabilities (no counterpart in the reference). Sequence s has K + 1 rows
+ * of target logits (row i at s ld_seq + i ld_row elements; row i answers the position of draft i, the last the one
+ * behind the drafts), K drafts, and their own logits (K rows, or NULL: each draft is certain under its model), lengths[s]
+ * of them (clamped to [0, K]; NULL: K). With p = softmax(logits inv_T), q the draft's, u = uniform[s, :]:
+ *   draft i is accepted when u_i q_i(x_i) < p_i(x_i); accepted[s] = a, the first that is not (or the length)
+ *   tokens[s, :a] = the accepted drafts, tokens[s, a] = the lowest v whose running sum of r exceeds u_K sum r,
+ *   r = max(p_a - q_a, 0) behind a rejected draft (p_a where that leaves nothing), p_a behind the last; -1 further on
+ *   logp[s, i] = log p_i(tokens[s, i]), 0 further on
+ * Probabilities and sums in 64 bits. greedy: a draft is accepted when it is its row's first largest logit, which is also
+ * the next token; u and the draft logits are not read (may be NULL). A draft outside [0, V), or whose logits' row has no
+ * softmax (a NaN, +inf, or nothing above -inf), is rejected and the token drawn from p_a; where p_a has none, the token
+ * is -1 and its logp NaN. A u_K that is no number below 1 takes the last v with r_v > 0. Rows behind a sequence's length are not read. K <= OCTO_DRAFTS_MAX, S <=
+ * 2^20. Rows may start at any element. ws: octo_verify_workspace_bytes, 16-byte aligned. */
+int octo_verify_workspace_bytes(int64_t S, int K, int V, size_t *bytes);
+int octo_verify_drafts(const void *logits, int64_t ld_seq, int64_t ld_row, const void *draft_logits, int64_t ld_seq_d,
+                       int64_t ld_row_d, int dtype, const int64_t *drafts, const int64_t *lengths, const float *uniform,
+                       int64_t S, int K, int V, double inv_T, int greedy, int64_t *tokens, int64_t *accepted,
+                       float *logp, void *ws, size_t ws_bytes, void *stream);
 
 /* octo_head_fwd followed, in its last kernel, by the GRPO weight of each compact row: what octo_grpo_grad computes
  * for the row's flat token t = (idx ? idx[r] : r) from the row's logprob (the same per-token formula), written in

@@ -23,6 +23,7 @@ WS_STEP = 128
 WS_NO_GRADH = 256
 PAIRS_NONE_AS_COUNT = 1
 LIST_MAX, LIST_RAW = 256, 1
+DRAFTS_MAX = 63
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -97,6 +98,15 @@ SIGNATURES = {
     "octo_label_pairs_workspace_bytes": [_i64, _i64, ctypes.POINTER(_sz)],
     "octo_label_pairs": [_p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _i32, _p, _sz, _p],
     "octo_quantise_fp8_rows": [_p, _i64, _i32, _i64, _i32, _p, _i64, _p, _p],
+    "octo_quantise_i8_rows": [_p, _i64, _i32, _i64, _i32, _i32, _p, _i64, _p, _p],
+    "octo_widen_i8_rows": [_p, _i64, _p, _i64, _i32, _i32, _p, _i64, _i32, _p],
+    "octo_head_logits_i8": [_p, _i64, _i32, _p, _i64, _p, _i64, _i32, _i32, _p, _i64, _p, _p, _i64, _i32, _p],
+    "octo_head_grads_i8_workspace_bytes": [_i64, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_sz)],
+    "octo_head_grads_i8": [_p, _i64, _i32, _p, _i64, _p, _p, _i64, _p, _i64, _i32, _i32, _p, _i64, _i32, _p, _i64,
+                           _i32, _p, _sz, _p],
+    "octo_verify_workspace_bytes": [_i64, _i32, _i32, ctypes.POINTER(_sz)],
+    "octo_verify_drafts": [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _p, _p, _i64, _i32, _i32, ctypes.c_double, _i32,
+                           _p, _p, _p, _p, _sz, _p],
     "octo_grpo_workspace_bytes": [ctypes.POINTER(_sz)],
     "octo_grpo_grad": [_p, _p, _p, _p, _p, _i64, _f32, _f32, _f32, _p, _p, _p, _sz, _p],
 }

@@ -272,7 +272,16 @@ __host__ __device__ constexpr bool ring5_ok(int dt) { return dt == OCTO_BF16 || 
 #define OCTO_MFMA_SNAKE 1
 #endif
 
+// 8-bit integer operands (int8_head.hip): 64 of them are a K-step's 64 bytes of a row, so slices, fragments and stages
+// are those of the 16-bit types; the accumulators' bits are the 32-bit integer sums.
+constexpr int DT_I8 = 16;
+
 template <int DT> struct Mfma16;
+template <> struct Mfma16<DT_I8> {
+  static __device__ __forceinline__ void run(const i32x4 a, const i32x4 b, f32x4 &c) {
+    c = __builtin_bit_cast(f32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, __builtin_bit_cast(i32x4, c), 0, 0, 0));
+  }
+};
 template <> struct Mfma16<OCTO_BF16> {
   static __device__ __forceinline__ void run(const i32x4 a, const i32x4 b, f32x4 &c) {
     c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -423,16 +432,16 @@ __device__ __forceinline__ int ring5_run(const OA &opa, const OB &opb, int sa0, 
   return ring_slot(sa + 2);
 }
 
-// smem: SMEM_RING5 bytes. 16-bit types only.
+// smem: SMEM_RING5 bytes. K_eff in elements; 16-bit types, or 8-bit integers in whole 16-byte chunks.
 template <int DT, typename OA, typename OB, bool SPLIT = false, bool TR = false>
 __device__ __forceinline__ void mainloop_ring5(const Operand &A, const Operand &B, int64_t m0, int64_t n0,
                                                int64_t K_eff, lds_char *smem, f32x4 (&acc)[OA::NB][OB::NB]) {
-  static_assert(DT == OCTO_BF16 || DT == OCTO_F16, "16-bit operands");
+  static_assert(DT == OCTO_BF16 || DT == OCTO_F16 || DT == DT_I8, "16-bit or 8-bit integer operands");
   static_assert(OA::NI == OB::NI, "one workgroup shape");
   constexpr int NWN = TN / (16 * OB::NB);  // waves along N
   const int w = threadIdx.x >> 6;
   const int wm = w / NWN, wn = w % NWN;
-  const uint32_t kbytes = (uint32_t)(K_eff * 2);
+  const uint32_t kbytes = (uint32_t)(K_eff * (DT == DT_I8 ? 1 : 2));
   const int nk = (int)((kbytes + EKB - 1) / EKB);
   OA opa;
   OB opb;

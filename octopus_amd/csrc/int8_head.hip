@@ -1,0 +1,281 @@
+// The head's logits from 8-bit integers, and their gradients (octo_head_logits_i8, octo_head_grads_i8).
+//
+//   z[r, v] = sx[r] sw[v] sum_k qx[r, k] qw[v, k]          (the sum exact in 32 bits: d <= 131,072)
+//   dx[r, k] = sum_v g[r, v] sw[v] qw[v, k]                (straight through the rounding of rows and weights)
+//   dW[v, k] = sum_r g[r, v] sx[r] qx[r, k]
+#include <type_traits>
+
+#include "gemm_nt.h"
+#include "octo_internal.h"
+#include "row_values.h"
+
+namespace octo {
+
+constexpr int kMaxD8 = 131072;       // 127^2 d < 2^31
+constexpr int kMaxV8 = 1 << 21;      // a tile's 256 rows of g within 32-bit offsets
+constexpr int64_t kMaxN8 = 1 << 21;  // the same of the transposed rows
+constexpr int kGroup8 = 4;
+
+typedef __attribute__((address_space(3))) f32x4 lds_f4;
+typedef i32x4 i32x4_el __attribute__((aligned(2)));
+
+struct Logits8 {
+  const float *sx, *sw;
+  void *z;
+  int64_t ldz;
+};
+
+// The product over tiles of 256 vocabulary rows x 256 tokens, weights as the MFMA's first operand: a lane's 4 sums of a
+// block are 4 neighbouring logits of one token. Scaled, rounded once, and out through the LDS in rows of 256 logits.
+// A slot holds 4 logits; slot s of token t sits at s ^ 4 (t & 15): a write's 16 tokens x 4 slots cover all banks.
+template <typename OT>
+__device__ __forceinline__ void store_logits8(const f32x4 (&acc)[8][4], const Logits8 &e, int64_t v0, int64_t n0, int V,
+                                              int64_t nvalid, lds_char *smem) {
+  typedef Acc16N<4> L;
+  constexpr int SLOT = 4 * sizeof(OT), ROW = 64 * SLOT, HALVES = sizeof(OT) == 4 ? 2 : 1, TOK = 256 / HALVES;
+  constexpr int LPR = ROW / 16, PER = 16 / sizeof(OT);  // lanes of a row, logits of a lane
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wm = L::wm(w), wn = L::wn(w);
+  const int vvalid = (int)min((int64_t)TM, V - v0);
+  float sx[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int t = L::col(wn, j, lane);
+    sx[j] = t < nvalid ? e.sx[n0 + t] : 0.f;
+  }
+  OT *out = (OT *)e.z + n0 * e.ldz + v0;
+  const bool whole = vvalid == TM && (sizeof(OT) == 2 || ((uintptr_t)e.z % 4 == 0));
+  for (int h = 0; h < HALVES; ++h) {
+    if (h) __syncthreads();
+    if (HALVES == 1 || (wn >> 1) == h) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int m = L::row(wm, i, 0, lane);
+        float sw[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) sw[v] = m + v < vvalid ? e.sw[v0 + m + v] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const i32x4 q = __builtin_bit_cast(i32x4, acc[i][j]);
+          const int t = L::col(wn, j, lane) - h * TOK;
+          OT o[4];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) o[v] = (OT)((float)q[v] * sx[j] * sw[v]);
+          lds_char *at = smem + t * ROW + (((m >> 2) ^ ((t & 15) << 2)) * SLOT);
+          if constexpr (sizeof(OT) == 4) *(lds_i32x4 *)at = __builtin_bit_cast(i32x4, o);
+          else *(__attribute__((address_space(3))) i32x2 *)at = __builtin_bit_cast(i32x2, o);
+        }
+      }
+    }
+    __syncthreads();
+    const int c = threadIdx.x % LPR, c0 = c * PER;
+    for (int t = threadIdx.x / LPR; t < TOK && h * TOK + t < nvalid; t += 512 / LPR) {
+      const i32x4 v = *(const lds_i32x4 *)(smem + t * ROW + (c * 16 ^ (((t & 15) << 2) * SLOT)));
+      OT *o = out + (h * TOK + t) * e.ldz + c0;
+      if (whole) {
+        __builtin_nontemporal_store(v, (i32x4_el *)o);
+      } else {
+        OT x[PER];
+        __builtin_memcpy(x, &v, 16);
+#pragma unroll
+        for (int u = 0; u < PER; ++u)
+          if (c0 + u < vvalid) o[u] = x[u];
+      }
+    }
+  }
+}
+
+template <typename OT>
+__global__ __launch_bounds__(2 * NTHREADS, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_kernel(Operand A, Operand B, GemmShape s, Logits8 e) {
+  __shared__ __attribute__((aligned(16))) char smem_[SMEM_RING5];
+  lds_char *smem = (lds_char *)smem_;
+  int mt, nt;
+  if (!tile_of(s, mt, nt)) return;
+  const int64_t m0 = (int64_t)mt * TM, n0 = (int64_t)nt * TN;
+  f32x4 acc[8][4];
+  mainloop_ring5<DT_I8, OpRowsN<8, 128>, OpRowsN<8, 64>, true>(A, B, m0, n0, s.K, smem, acc);
+  store_logits8<OT>(acc, e, m0, n0, (int)s.M, min(s.N - n0, (int64_t)TN), smem);
+}
+
+static Operand operand8(const void *base, int64_t ld_bytes, int64_t rows) {
+  Operand X;
+  X.base = (const char *)base;
+  X.ld = ld_bytes;
+  X.map = nullptr;
+  X.rows = rows;
+  X.count = nullptr;
+  X.count_off = 0;
+  X.extent = 0;
+  return X;
+}
+
+static GemmShape shape8(int64_t M, int64_t N, int64_t K) {
+  GemmShape s;
+  s.M = M;
+  s.N = N;
+  s.K = K;
+  s.mtiles = (int)cdiv(M, TM);
+  s.ntiles = (int)cdiv(N, TN);
+  s.group_m = kGroup8;
+  s.count_on = 0;
+  s.count = nullptr;
+  s.count_off = 0;
+  return s;
+}
+
+// Workspace of the gradients: the widened weight [V, d] (K-major for dx) and the partial tiles of its split; the
+// transposed rows [d, n]; g where its rows cannot be read as they are. Sizes padded as the K-major loads read.
+struct Grads8Layout {
+  int64_t Vr, dp, np, Vp;  // rows and columns of the copies
+  size_t wide, xt, g, split, total;
+  int64_t split_items;
+};
+
+static Grads8Layout grads8_layout(int64_t n, int d, int V, int dtype, bool need_rows, bool need_w) {
+  const int esz = float_bytes(dtype);
+  Grads8Layout L;
+  L.Vr = round_up(V, 64);
+  L.dp = round_up(d, TN);
+  L.np = round_up(n, 64);
+  L.Vp = round_up(V, TM);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t p = at;
+    at += (size_t)round_up((int64_t)bytes, 256);
+    return p;
+  };
+  L.split_items = 0;
+  if (need_rows) {
+    const int64_t nt = cdiv(d, dtype == OCTO_F32 ? 128 : TN), nk = cdiv(V, 64);
+    const int64_t mt = cdiv(n, TM);
+    if (mt * nt < octo_tiles::kSplitItemsMax) {
+      const int S = octo_tiles::k_splits((int)(mt * nt), (int)nk, !need_w || dtype == OCTO_F32,
+                                         octo_tiles::kSplitItemsMax);
+      if (S > 1) L.split_items = mt * nt * S;
+    }
+  }
+  L.wide = take(need_rows ? (size_t)L.Vr * L.dp * esz : 0);
+  L.xt = take(need_w ? (size_t)d * L.np * esz : 0);
+  L.g = take((size_t)L.np * L.Vp * esz);
+  L.split = take((size_t)L.split_items * TM * (dtype == OCTO_F32 ? 128 : TN) * 4);
+  L.total = at;
+  return L;
+}
+
+static int head8_checks(const char *what, int64_t n, int d, int V, int64_t ldxq, int64_t ldw) {
+  OCTO_CHECK_ARG(n >= 0 && n <= kMaxN8, "%s: n=%lld outside [0, %lld]", what, (long long)n, (long long)kMaxN8);
+  OCTO_CHECK_ARG(d > 0 && d <= kMaxD8, "%s: d=%d outside [1, %d]", what, d, kMaxD8);
+  OCTO_CHECK_ARG(V > 0 && V <= kMaxV8, "%s: V=%d outside [1, %d]", what, V, kMaxV8);
+  for (int64_t ld : {ldxq, ldw})
+    OCTO_CHECK_ARG(ld >= round_up(d, 16) && ld % 16 == 0 && ld <= 2 * kMaxD8,
+                   "%s: 8-bit rows of stride %lld (a multiple of 16, at least d=%d)", what, (long long)ld, d);
+  return OCTO_OK;
+}
+
+}  // namespace octo
+
+using namespace octo;
+
+extern "C" {
+
+int octo_head_logits_i8(const void *rows, int64_t ldx, int x_dtype, const int8_t *wq, int64_t ldw, const float *w_scale,
+                        int64_t n, int d, int V, int8_t *xq, int64_t ldxq, float *x_scale, void *logits, int64_t ldz,
+                        int z_dtype, void *stream) {
+  int rc = head8_checks("head_logits_i8", n, d, V, ldxq, ldw);
+  if (rc) return rc;
+  OCTO_CHECK_ARG(ldz >= V, "head_logits_i8: row stride %lld below V=%d", (long long)ldz, V);
+  if (!is_float(z_dtype)) return octo_fail(OCTO_EUNSUPPORTED, "head_logits_i8: dtype %d", z_dtype);
+  if (n == 0) return OCTO_OK;
+  OCTO_CHECK_ARG(wq && w_scale && xq && x_scale && logits, "head_logits_i8: null pointer");
+  OCTO_CHECK_ARG((uintptr_t)wq % 16 == 0 && (uintptr_t)xq % 16 == 0 && (uintptr_t)w_scale % 4 == 0 &&
+                     (uintptr_t)x_scale % 4 == 0 && (uintptr_t)logits % float_bytes(z_dtype) == 0,
+                 "head_logits_i8: misaligned pointer");
+  hipStream_t st = (hipStream_t)stream;
+  if (rows) {
+    rc = octo_quantise_i8_rows(rows, ldx, x_dtype, n, d, 0, xq, ldxq, x_scale, stream);
+    if (rc) return rc;
+  }
+  const Logits8 e{x_scale, w_scale, logits, ldz};
+  const GemmShape s = shape8(V, n, round_up(d, 16));
+  const Operand A = operand8(wq, ldw, V), B = operand8(xq, ldxq, n);
+  const dim3 grid((unsigned)tile_grid(s.mtiles, s.ntiles));
+  switch (z_dtype) {
+    case OCTO_BF16: hipLaunchKernelGGL(gemm_i8_kernel<__bf16>, grid, dim3(2 * NTHREADS), 0, st, A, B, s, e); break;
+    case OCTO_F16: hipLaunchKernelGGL(gemm_i8_kernel<_Float16>, grid, dim3(2 * NTHREADS), 0, st, A, B, s, e); break;
+    default: hipLaunchKernelGGL(gemm_i8_kernel<float>, grid, dim3(2 * NTHREADS), 0, st, A, B, s, e); break;
+  }
+  OCTO_CHECK_LAUNCH("gemm_i8");
+  return OCTO_OK;
+}
+
+int octo_head_grads_i8_workspace_bytes(int64_t n, int d, int V, int dtype, int need_rows, int need_w, size_t *bytes) {
+  OCTO_CHECK_ARG(bytes != nullptr, "head_grads_i8_workspace_bytes: null pointer");
+  const int rc = head8_checks("head_grads_i8", n, d, V, round_up(d < 1 ? 1 : d, 16), round_up(d < 1 ? 1 : d, 16));
+  if (rc) return rc;
+  if (!is_float(dtype)) return octo_fail(OCTO_EUNSUPPORTED, "head_grads_i8: dtype %d", dtype);
+  *bytes = grads8_layout(n, d, V, dtype, need_rows != 0, need_w != 0).total;
+  return OCTO_OK;
+}
+
+int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq, int64_t ldxq, const float *x_scale,
+                       const int8_t *wq, int64_t ldw, const float *w_scale, int64_t n, int d, int V, void *grad_rows,
+                       int64_t ld_gr, int gr_dtype, void *grad_w, int64_t ld_gw, int gw_dtype, void *ws,
+                       size_t ws_bytes, void *stream) {
+  int rc = head8_checks("head_grads_i8", n, d, V, ldxq, ldw);
+  if (rc) return rc;
+  for (int t : {g_dtype, grad_rows ? gr_dtype : OCTO_F32, grad_w ? gw_dtype : OCTO_F32})
+    if (!is_float(t)) return octo_fail(OCTO_EUNSUPPORTED, "head_grads_i8: dtype %d", t);
+  OCTO_CHECK_ARG(n > 0, "head_grads_i8: no rows");
+  OCTO_CHECK_ARG(ldg >= V && (!grad_rows || ld_gr >= d) && (!grad_w || ld_gw >= d), "head_grads_i8: row strides");
+  if (!grad_rows && !grad_w) return OCTO_OK;
+  OCTO_CHECK_ARG(g && (!grad_rows || (wq && w_scale)) && (!grad_w || (xq && x_scale)), "head_grads_i8: null pointer");
+  OCTO_CHECK_ARG((uintptr_t)wq % 16 == 0 && (uintptr_t)xq % 16 == 0 && (uintptr_t)w_scale % 4 == 0 &&
+                     (uintptr_t)x_scale % 4 == 0 && (uintptr_t)g % float_bytes(g_dtype) == 0 &&
+                     (uintptr_t)grad_rows % float_bytes(gr_dtype) == 0 &&
+                     (uintptr_t)grad_w % float_bytes(gw_dtype) == 0 && (uintptr_t)ws % 256 == 0,
+                 "head_grads_i8: misaligned pointer");
+  const Grads8Layout L = grads8_layout(n, d, V, g_dtype, grad_rows != nullptr, grad_w != nullptr);
+  if (!ws || ws_bytes < L.total)
+    return octo_fail(OCTO_EWORKSPACE, "head_grads_i8: workspace %zu < %zu bytes", ws ? ws_bytes : (size_t)0, L.total);
+  hipStream_t st = (hipStream_t)stream;
+  char *wsb = (char *)ws;
+  const int esz = float_bytes(g_dtype);
+
+  rc = launch_stage_rows(g, ldg, g_dtype, n, V, wsb + L.g, L.Vp, L.np, (int)L.Vp, st);
+  if (rc) return rc;
+  const char *gs = wsb + L.g;
+  const int64_t lds = L.Vp * esz;
+  StoreArgs oh, ow;
+  const Operand Ah = operand8(gs, lds, n), Bh = operand8(wsb + L.wide, L.dp * esz, d);
+  const GemmShape sh = shape8(n, d, V);
+  if (grad_rows) {
+    rc = launch_widen_rows(wq, ldw, w_scale, V, d, 0, wsb + L.wide, L.dp, g_dtype, L.Vr, (int)L.dp, st);
+    if (rc) return rc;
+    oh.C = grad_rows;
+    oh.ldc = ld_gr;
+    oh.dtype = gr_dtype;
+    if (L.split_items) {
+      oh.split = (float *)(wsb + L.split);
+      oh.split_cap = (int)L.split_items;
+      oh.split_alone = !grad_w || g_dtype == OCTO_F32;
+    }
+  }
+  const Operand Aw = operand8(gs, lds, V), Bw = operand8(wsb + L.xt, L.np * esz, d);
+  const GemmShape sw = shape8(V, d, n);
+  if (grad_w) {
+    rc = launch_widen_t(xq, ldxq, x_scale, n, d, wsb + L.xt, L.np, g_dtype, st);
+    if (rc) return rc;
+    ow.C = grad_w;
+    ow.ldc = ld_gw;
+    ow.dtype = gw_dtype;
+  }
+  if (grad_rows && grad_w && g_dtype != OCTO_F32) {
+    rc = launch_gemm_grads(g_dtype, Ah, Bh, sh, oh, true, Aw, Bw, sw, ow, st);
+  } else {
+    if (grad_rows) rc = launch_gemm_store(g_dtype, Ah, Bh, sh, oh, st, KM_B);
+    if (!rc && grad_w) rc = launch_gemm_store(g_dtype, Aw, Bw, sw, ow, st, KM_A);
+  }
+  if (!rc && grad_rows) rc = launch_split_sum(sh, oh, g_dtype == OCTO_F32, st);
+  return rc;
+}
+
+}  // extern "C"

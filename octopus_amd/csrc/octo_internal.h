@@ -428,4 +428,16 @@ int launch_transpose(const void *src, int64_t ld_src, int src_dtype, const float
                      const int64_t *map, const int32_t *count, int64_t count_off, int64_t rows,
                      int64_t rows_pad, int64_t cols, void *dst, int64_t ld_dst, int dst_dtype, hipStream_t st);
 
+// ---- rows of 8-bit integers (rows8.hip) ------------------------------------------------------------
+// out[r, c] = q[r, c] scale (of row r's group of c; group 0: of the row), rounded once to dtype, for r < rows, c < d;
+// zeros for the other r < rows_pad, c < cols_pad.
+int launch_widen_rows(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int d, int group, void *out,
+                      int64_t ldo, int dtype, int64_t rows_pad, int cols_pad, hipStream_t st);
+// The transpose of it: out[c, r] = q[r, c] scale[r] for c < d, zeros for rows <= r < ldo (a multiple of 64).
+int launch_widen_t(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int d, void *out, int64_t ldo,
+                   int dtype, hipStream_t st);
+// A copy of g [n, V] with rows of ldo elements (whole 16 bytes), zeros behind it up to rows_pad and cols_pad.
+int launch_stage_rows(const void *g, int64_t ldg, int dtype, int64_t n, int V, void *out, int64_t ldo, int64_t rows_pad,
+                      int cols_pad, hipStream_t st);
+
 }  // namespace octo

@@ -20,6 +20,7 @@ from torch.utils.checkpoint import checkpoint
 
 TILE = 16384
 _INNER = True  # tiles checkpointed; no_inner() turns this off
+_HELD8 = None  # the group of the 8-bit rows that tiles' checkpoints hold; held8() sets it
 COMPILE = os.environ.get("OCTOPUS_COMPILE", "1") != "0"
 
 
@@ -39,7 +40,12 @@ def _fused(fn=None, *, hip=None):
 
 
 def _checkpoint(fn, *args):
-    return checkpoint(fn, *args, use_reentrant=False) if _INNER else fn(*args)
+    if not _INNER:
+        return fn(*args)
+    if _HELD8 is not None:
+        from ..int8_op import checkpoint8
+        return checkpoint8(fn, *args, group=_HELD8)
+    return checkpoint(fn, *args, use_reentrant=False)
 
 
 _REFERENCE_TILES = "octopus.rl.seq_tiles"  # the trainer's own module, whose flag its patched decoder layers read
@@ -64,6 +70,22 @@ def no_inner():
         _INNER = True
         if ref is not None:
             ref._INNER = ref_before
+
+
+@contextlib.contextmanager
+def held8(group: int = 128):
+    """Tiles begun inside hold their inputs in 8 bits between the forward and their recompute (int8_op.checkpoint8: the
+    HIP tensors that require a gradient), a scale for each `group` values of a row: 1.03 bytes a value in place of 2.
+    Tiles on the CPU, and no_inner()'s, are as without it."""
+    from ..int8_op import GROUPS
+    global _HELD8
+    if group not in GROUPS:
+        raise ValueError(f"octohead: groups of {GROUPS} values, got {group}")
+    before, _HELD8 = _HELD8, group
+    try:
+        yield
+    finally:
+        _HELD8 = before
 
 
 def tiled(fn, *xs):
