@@ -343,7 +343,7 @@ int octo_quantise_fp8_rows(const void *w, int64_t ldw, int w_dtype, int64_t V, i
 
 /* Rows held as 8-bit integers (no counterpart in the reference): x [rows, ldx] (BF16, F16 or F32), group 0 (the row),
  * 32, 64, 128 or 256 values to a scale, groups = group ? ceil(d / group) : 1. Of each group, with a = max |x|:
- *   scale[r * groups + j] = a / 127 in fp32;  q[r * ldq + k] = x / scale to the nearest integer, ties to even
+ *   scale[r * groups + j] = a times 1/127 (both fp32);  q[r * ldq + k] = x / scale to the nearest integer, ties to even
  * from the exact quotient; a < 2^-119: scale 0 and zeros; a not finite: scale NaN and zeros. ldq is a multiple of 16 and
  * q 16-byte aligned; the bytes from d up to the next multiple of 16 are written 0. Rows of x may start at any element.
  * octo_widen_i8_rows: out[r, k] = q scale, rounded once to out_dtype. */

@@ -1,7 +1,7 @@
 // Rows held as 8-bit integers with fp32 scales (octo_quantise_i8_rows, octo_widen_i8_rows), and the copies that the
 // gradients of the 8-bit head multiply with (launch_widen_t, launch_stage_rows).
 //
-//   a = max |x| of a group of a row's values (the whole row, or 32 to 256 of them), scale = a / 127 rounded to fp32,
+//   a = max |x| of a group of a row's values (the whole row, or 32 to 256 of them), scale = a times 1/127, both in fp32,
 //   q = the exact quotient x / scale to the nearest integer, ties to even;   x^ = q scale, rounded once
 //
 // A group below 2^-119 (its scale would not be a normal number) is held as zeros, one with a NaN or an infinity as NaN
@@ -52,7 +52,7 @@ template <int LANES> __device__ __forceinline__ uint32_t lanes_max(uint32_t m) {
 __device__ __forceinline__ float scale_of(uint32_t maxbits) {
   if (maxbits >= 0x7f800000u) return __builtin_nanf("");
   const float a = __uint_as_float(maxbits);
-  return a < kLeastMax ? 0.f : a / 127.f;
+  return a < kLeastMax ? 0.f : a * (1.f / 127.f);
 }
 // 8 quotients as bytes. x inv is within an integer of x / s and the remainder x - q s is exact in one fma (at most 7
 // bits of q times 24 of s, less x: within fp32's 24 bits above the finer of the two last places), so comparing it with

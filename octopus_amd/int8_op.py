@@ -4,8 +4,8 @@
     octohead::head_logits_i8 / head_grads_i8   rows W^T in 8-bit integers with a scale for each row of both; its gradients
     checkpoint8                                a checkpoint that holds its inputs in 8 bits
 
-Of a row, or of each group of 32 to 256 of its values, with a the largest magnitude: scale = a / 127 in fp32, q the exact
-quotient x / scale to the nearest integer (ties to even). A group below 2^-119 is held as zeros, one with a NaN or an
+Of a row, or of each group of 32 to 256 of its values, with a the largest magnitude: scale = a times 1/127, both
+in fp32, q the exact quotient x / scale to the nearest integer (ties to even). A group below 2^-119 is held as zeros, one with a NaN or an
 infinity as NaN. int8 rows start on 16-byte boundaries, zeros between them (quantise_rows gives them so).
 
 The logits are x_scale w_scale sum_k xq wq, the sum exact. Their gradients go straight through the rounding: in the rows

@@ -26,7 +26,7 @@ def quantise(x, group=0, exact=False):
         part = x[:, j * width:(j + 1) * width]
         a = np.abs(part).max(1)
         with np.errstate(invalid="ignore"):
-            s = (a.astype(np.float32) / np.float32(127)).astype(np.float64)
+            s = (a.astype(np.float32) * (np.float32(1) / np.float32(127))).astype(np.float64)
         s[a < LEAST] = 0.0
         s[~np.isfinite(a)] = np.nan
         scale[:, j] = s
