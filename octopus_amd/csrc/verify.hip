@@ -8,10 +8,15 @@
 // rounding of any number, and then another token is answered. So the exponentials and sums are taken in 64 bits (exp64
 // below, 6e-15 relative), and a draw differs from the exact one with a probability of about V times that.
 //
-// Three launches. stats: a workgroup per slice of a row, the slice's maximum and its sum of exponentials against it.
-// residual: a workgroup per slice of a sequence's row a; each joins the rows' slices and finds a by itself, and sums
-// its slice's r. pick: a workgroup per sequence finds the slice in which the running sum passes u_K sum r, and in it the
-// token. All sums are in an order that the sizes alone decide.
+// Rows are summed by waves, a part of a row each, in an order that the sizes alone decide. Few logits take three
+// launches, all in 64 bits:
+//   stats     each part's maximum and its sum of exponentials against it, every row that a sequence may need
+//   residual  each workgroup joins its sequence's rows, finds a by itself, and its waves sum their parts' r
+//   pick      a workgroup per sequence finds the part in which the running sum passes u_K sum r, and in it the token
+// Many take the exponentials of stats in 32 bits (64-bit ones are 20 instructions each, and stats is most of the work),
+// which leave each row's sum within 4e-6 (see fast_part). That decides a draft unless u q and p are closer than 2^-15;
+// then the row and its draft's are summed again in 64 bits there. Two launches more, decide and sums, stand between stats
+// and residual: a is found once a sequence, and row a of both models summed in 64 bits.
 #include "octo_common.h"
 #include "row_values.h"
 
@@ -19,34 +24,36 @@ namespace octo {
 
 constexpr int kVThreads = 256, kVWaves = kVThreads / 64;
 constexpr int kVDrafts = OCTO_DRAFTS_MAX;
-constexpr int kVSlices = 1024;  // slices of a row, at most
+constexpr int kVParts = 1024;   // parts of a row, at most
+constexpr int kVBlock = 2048;   // values that a wave holds at a time: 4 chunks of 8 a lane
+constexpr double kVClose = 1.0 / 32768;
+constexpr double kVLn2 = 0.69314718055994530942;
 
-// 2^(y) for y = x log2(e): the nearest integer's power by the exponent, the rest, within 1/2, by exp's series in
-// f ln 2: the first term left out is (ln 2 / 2)^12 / 12! = 6e-15.
-__device__ __forceinline__ double exp64(double x) {  // x <= 0 or -inf; below -760 it gives 0
-  const double y = fmax(x, -800.0) * 1.4426950408889634074;
-  const double n = __builtin_rint(y);
-  const double f = __builtin_fma(n, -0.69314718055994530942, fmax(x, -800.0));
-  const double g = __builtin_fma(n, -2.3190468138462996e-17, f);  // ln 2's rest below its 53 bits
-  double e = 1.0 / 39916800.0;
-  e = __builtin_fma(e, g, 1.0 / 3628800.0);
-  e = __builtin_fma(e, g, 1.0 / 362880.0);
-  e = __builtin_fma(e, g, 1.0 / 40320.0);
-  e = __builtin_fma(e, g, 1.0 / 5040.0);
-  e = __builtin_fma(e, g, 1.0 / 720.0);
-  e = __builtin_fma(e, g, 1.0 / 120.0);
-  e = __builtin_fma(e, g, 1.0 / 24.0);
-  e = __builtin_fma(e, g, 1.0 / 6.0);
-  e = __builtin_fma(e, g, 0.5);
-  e = __builtin_fma(e, g, 1.0);
-  e = __builtin_fma(e, g, 1.0);
-  return ldexp(e, (int)n);
+// 2^t for t <= 0, -inf included (below -1000: 0), within 4e-16 of its value: t = n + f, |f| <= 1/2, n from the last bits
+// of t + 1.5 x 2^52, and 2^f by the polynomial of degree 10 through it at the 11 Chebyshev nodes of [-1/2, 1/2]. No
+// conversion, rounding or ldexp of 64 bits, which take four times an fma's cycles: [256 x 2, 151,936] sums 109 us with
+// them and exp's series, 64 so.
+__device__ __forceinline__ double exp2_64(double t) {
+  const double shift = 6755399441055744.0, b = t + shift, f = t - (b - shift);
+  double e = 7.072585949269223e-09;
+  e = __builtin_fma(e, f, 1.0208690299958306e-07);
+  e = __builtin_fma(e, f, 1.321544258792169e-06);
+  e = __builtin_fma(e, f, 1.5252657260200837e-05);
+  e = __builtin_fma(e, f, 0.0001540353044173605);
+  e = __builtin_fma(e, f, 0.0013333558230164974);
+  e = __builtin_fma(e, f, 0.009618129107606888);
+  e = __builtin_fma(e, f, 0.05550410866444772);
+  e = __builtin_fma(e, f, 0.24022650695910097);
+  e = __builtin_fma(e, f, 0.69314718055995);
+  e = __builtin_fma(e, f, 1.0);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, e) + ((uint64_t)(uint32_t)__builtin_bit_cast(uint64_t, b) << 52);
+  return t < -1000.0 ? 0.0 : __builtin_bit_cast(double, bits);
 }
 
-struct SliceStat {
-  double S;   // sum of exp((z - m) / T); NaN where the slice has a NaN or +inf
+struct PartStat {
+  double S;   // sum of exp((z - m) / T); NaN where the part has a NaN or +inf
   float m;    // maximum
-  int first;  // its first column
+  int first;  // its first column (greedy)
 };
 struct RowStat {
   double inv;  // 1 / sum over the row; 0 where the row has no distribution
@@ -62,11 +69,13 @@ struct VerifyArgs {
   const float *u;          // [S, K + 1] (NULL: greedy)
   int64_t S;
   int K, V;
-  double inv_T;
+  double c;                   // log2(e) / T
+  float c_hi, c_lo, d_least;  // the same in two parts, and a difference whose exponential is 0 in 32 bits
   int greedy;
-  int slices, per;   // per: values of a slice, a multiple of 64
-  SliceStat *stats;  // [S, 2 K + 1, slices]: target rows, then draft rows
-  double *sums;      // [S, slices]: r's
+  int parts, part;  // parts of a row, values of each (a multiple of kVBlock)
+  int turns;        // parts a wave takes (sums, residual)
+  PartStat *stats;  // [S, 2 K + 1, parts]: target rows, then draft rows
+  double *sum_p, *sum_q, *sum_r;  // [S, parts]: of exp((z - m) / T) of row a, of its draft row's; of r
   struct Decision {
     RowStat p, q;
     int a, residual, x, pad;  // residual: 0 r = p, 1 r = p - q, 2 r = p without x
@@ -78,6 +87,11 @@ struct VerifyArgs {
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
   return v;
 }
 
@@ -92,211 +106,402 @@ __device__ __forceinline__ const typename Elem<DT>::T *row_of(const void *z, int
   return (const typename Elem<DT>::T *)z + s * ls + i * lr;
 }
 
-// f(value, column) for the columns [c0, c1) that this thread takes, 16-byte loads where the row's alignment allows.
-template <int DT, class F>
-__device__ __forceinline__ void sweep_slice(const typename Elem<DT>::T *row, int c0, int c1, F f) {
-  constexpr int PER = 16 / Elem<DT>::bytes;
-  const int head = min(c1 - c0, (int)((16 - ((uintptr_t)(row + c0) & 15)) & 15) / Elem<DT>::bytes);
-  const int chunks = (c1 - c0 - head) / PER;
-  const i32x4 *vec = (const i32x4 *)(row + c0 + head);
-  for (int k0 = threadIdx.x; k0 < chunks; k0 += 4 * kVThreads) {
-    i32x4 v[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = vec[min(k0 + u * kVThreads, chunks - 1)];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int k = k0 + u * kVThreads;
-      if (k >= chunks) break;
-      float x[PER];
-      unpack_chunk<DT>(v[u], x);
-#pragma unroll
-      for (int e = 0; e < PER; ++e) f(x[e], c0 + head + k * PER + e);
-    }
-  }
-  const int tail = c0 + head + chunks * PER, t = threadIdx.x;
-  const int j = t < head ? c0 + t : tail + t - head;
-  if (j < c1) f((float)row[j], j);
-}
-
+// Chunk u of a lane of the kVBlock values from column c on: columns c + 512 u + 8 lane .. + 7, -inf from c1 on. Rows may
+// start at any element (16-byte global loads need no alignment).
+typedef i32x4 i32x4_any2 __attribute__((aligned(2)));
+typedef i32x4 i32x4_any4 __attribute__((aligned(4)));
 template <int DT>
-__global__ __launch_bounds__(kVThreads) void verify_stats_kernel(VerifyArgs a) {
-  const int64_t s = blockIdx.y / (2 * a.K + 1);
-  const int i = (int)(blockIdx.y - s * (2 * a.K + 1)), len = drafts_of(a, s);
-  const bool draft = i > a.K;
-  if (draft ? (!a.zd || i - a.K - 1 >= len) : i > len) return;  // nobody asks for the row
-  const typename Elem<DT>::T *row = draft ? row_of<DT>(a.zd, a.ls_d, a.lr_d, s, i - a.K - 1)
-                                          : row_of<DT>(a.z, a.ls, a.lr, s, i);
-  const int c0 = blockIdx.x * a.per, c1 = min(a.V, c0 + a.per);
-  __shared__ float sm[kVWaves];
-  __shared__ int si[kVWaves];
-  __shared__ double ss[kVWaves];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  float m = -INFINITY;
-  bool bad = false;
-  sweep_slice<DT>(row, c0, c1, [&](float x, int) {
-    m = fmaxf(m, x);
-    bad |= !(x < INFINITY);
-  });
-  m = wave_max(m);
-  if (lane == 0) sm[w] = m;
-  bad = __syncthreads_or(bad);
+__device__ __forceinline__ void load_whole(const typename Elem<DT>::T *p, float (&x)[8]) {
+  if constexpr (DT == OCTO_F32) {
 #pragma unroll
-  for (int k = 0; k < kVWaves; ++k) m = fmaxf(m, sm[k]);
-  double S = 0.0;
-  int first = 0x7fffffff;
-  const double md = m == -INFINITY ? 0.0 : (double)m;
-  sweep_slice<DT>(row, c0, c1, [&](float x, int c) {
-    S += exp64(((double)x - md) * a.inv_T);
-    if (x == m) first = min(first, c);
-  });
-  S = wave_sum64(S);
+    for (int h = 0; h < 2; ++h) {
+      const i32x4 v = ((const i32x4_any4 *)p)[h];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, 64));
-  if (lane == 0) {
-    ss[w] = S;
-    si[w] = first;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    SliceStat out;
-    out.S = 0.0;
-    out.first = 0x7fffffff;
-    for (int k = 0; k < kVWaves; ++k) {
-      out.S += ss[k];
-      out.first = min(out.first, si[k]);
+      for (int e = 0; e < 4; ++e) x[4 * h + e] = __int_as_float(v[e]);
     }
-    out.m = m;
-    if (bad) out.S = __builtin_nan("");
-    a.stats[(s * (2 * a.K + 1) + i) * a.slices + blockIdx.x] = out;
+  } else {
+    unpack8(*(const i32x4_any2 *)p, DT == OCTO_F16, x);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void load_values(const typename Elem<DT>::T *row, int c, int c1, float (&x)[8]) {
+  if (c + 8 <= c1) {
+    load_whole<DT>(row + c, x);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = c + e < c1 ? (float)row[c + e] : -INFINITY;
+  }
+}
+// All of them at once but for a row's last block: a branch a chunk makes each load wait for the one before.
+template <int DT>
+__device__ __forceinline__ void load_block(const typename Elem<DT>::T *row, int c, int c1, float (&x)[4][8]) {
+  const int lane = threadIdx.x & 63;
+  if (c + kVBlock <= c1) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) load_whole<DT>(row + c + 512 * u + 8 * lane, x[u]);
+  } else {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) load_values<DT>(row, c + 512 * u + 8 * lane, c1, x[u]);
   }
 }
 
-// Row i's statistics from its slices, by one wave; the same in every lane.
-__device__ __forceinline__ RowStat join_row(const VerifyArgs &a, int64_t s, int i) {
-  const SliceStat *p = a.stats + (s * (2 * a.K + 1) + i) * a.slices;
-  const int lane = threadIdx.x & 63;
+// A wave's part in 64 bits.
+template <int DT>
+__device__ __forceinline__ PartStat exact_part(const VerifyArgs &a, const typename Elem<DT>::T *row, int c0, int c1) {
   float m = -INFINITY;
-  for (int k = lane; k < a.slices; k += 64) m = fmaxf(m, p[k].m);
-  m = wave_max(m);
   double S = 0.0;
   int first = 0x7fffffff;
-  for (int k = lane; k < a.slices; k += 64) {
-    const SliceStat t = p[k];
-    if (t.m != -INFINITY || !(t.S == 0.0)) S += t.S * exp64(((double)t.m - (double)m) * a.inv_T);
-    if (t.m == m) first = min(first, t.first);
-  }
-  S = wave_sum64(S);
+  bool bad = false;
+  for (int c = c0; c < c1; c += kVBlock) {
+    float x[4][8], mx = m;
+    load_block<DT>(row, c, c1, x);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, 64));
-  RowStat r;
-  r.inv = S > 0.0 && m != -INFINITY ? 1.0 / S : 0.0;  // NaN: no distribution
-  r.m = m;
-  r.first = first;
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        mx = fmaxf(mx, x[u][e]);
+        bad |= !(x[u][e] < INFINITY);
+      }
+    if (mx > m) {
+      S *= exp2_64(((double)m - (double)mx) * a.c);
+      first = 0x7fffffff;
+      m = mx;
+    }
+    const double md = m == -INFINITY ? 0.0 : (double)m;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) S += exp2_64(((double)x[u][e] - md) * a.c);
+    if (a.greedy) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (x[u][e] == m) first = min(first, c + 512 * u + 8 * (int)(threadIdx.x & 63) + e);
+    }
+  }
+  PartStat r;
+  r.m = wave_max(m);
+  r.S = wave_sum64(m == -INFINITY ? 0.0 : S * exp2_64(((double)m - (double)r.m) * a.c));
+  if (__any(bad)) r.S = __builtin_nan("");
+  r.first = wave_min(m == r.m ? first : 0x7fffffff);
   return r;
 }
 
-__device__ __forceinline__ double prob(float x, const RowStat &r, double inv_T) {
-  return exp64(((double)x - (double)r.m) * inv_T) * r.inv;
+// A wave's part with exponentials in 32 bits. exp2 is within 2^-23 of its value, and its argument d c, d = z - m <= 0,
+// off by at most 2^-23 |d c| (d, and the product with c in two parts, rounded once each), which makes ln 2 times that of
+// the value: over a row at most 2^-23 (1 + 0.7 x 20), as the mean of |d c| under the softmax is at most log2 V. Eight
+// values are summed in 32 bits (3 x 2^-24), all else in 64. Together below 4e-6 of the row's sum.
+template <int DT>
+__device__ __forceinline__ PartStat fast_part(const VerifyArgs &a, const typename Elem<DT>::T *row, int c0, int c1) {
+  float m = -INFINITY;
+  double S = 0.0;
+  int first = 0x7fffffff;
+  bool bad = false;
+  for (int c = c0; c < c1; c += kVBlock) {
+    float x[4][8], mx = m;
+    load_block<DT>(row, c, c1, x);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        mx = fmaxf(mx, x[u][e]);
+        bad |= !(x[u][e] < INFINITY);
+      }
+    if (mx > m) {
+      S *= exp2_64(((double)m - (double)mx) * a.c);
+      first = 0x7fffffff;
+      m = mx;
+    }
+    const float mf = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float t[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = fmaxf(x[u][e] - mf, a.d_least);
+        t[e] = fexp2(__builtin_fmaf(d, a.c_hi, d * a.c_lo));
+      }
+      S += (double)(((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7])));
+    }
+    if (a.greedy) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (x[u][e] == m) first = min(first, c + 512 * u + 8 * (int)(threadIdx.x & 63) + e);
+    }
+  }
+  PartStat r;
+  r.m = wave_max(m);
+  r.S = wave_sum64(m == -INFINITY ? 0.0 : S * exp2_64(((double)m - (double)r.m) * a.c));
+  if (__any(bad)) r.S = __builtin_nan("");
+  r.first = wave_min(m == r.m ? first : 0x7fffffff);
+  return r;
+}
+
+template <int DT, bool EXACT>
+__global__ __launch_bounds__(kVThreads) void verify_stats_kernel(VerifyArgs a) {
+  const int rows = 2 * a.K + 1;
+  const int64_t s = blockIdx.y / rows;
+  const int i = (int)(blockIdx.y - s * rows), len = drafts_of(a, s);
+  const int k = __builtin_amdgcn_readfirstlane(blockIdx.x * kVWaves + (threadIdx.x >> 6));
+  const bool draft = i > a.K;
+  if (draft ? (!a.zd || i - a.K - 1 >= len) : i > len) return;  // nobody asks for the row
+  if (k >= a.parts) return;
+  const typename Elem<DT>::T *row = draft ? row_of<DT>(a.zd, a.ls_d, a.lr_d, s, i - a.K - 1)
+                                          : row_of<DT>(a.z, a.ls, a.lr, s, i);
+  const int c0 = k * a.part, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.part);
+  const PartStat r = EXACT ? exact_part<DT>(a, row, c0, c1) : fast_part<DT>(a, row, c0, c1);
+  if ((threadIdx.x & 63) == 0) a.stats[(int64_t)blockIdx.y * a.parts + k] = r;
+}
+
+// Row i's statistics from its parts, by one wave; the same in every lane.
+__device__ __forceinline__ RowStat join_row(const VerifyArgs &a, int64_t s, int i) {
+  const PartStat *p = a.stats + (s * (2 * a.K + 1) + i) * a.parts;
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY;
+  double S = 0.0;
+  int first = 0x7fffffff;
+  for (int k = lane; k < a.parts; k += 64) {
+    const PartStat t = p[k];
+    const float mx = fmaxf(m, t.m);
+    if (mx > m) {
+      S = m == -INFINITY ? S : S * exp2_64(((double)m - (double)mx) * a.c);
+      first = 0x7fffffff;
+      m = mx;
+    }
+    S += t.m == -INFINITY ? t.S : t.S * exp2_64(((double)t.m - (double)m) * a.c);
+    if (t.m == m) first = min(first, t.first);
+  }
+  RowStat r;
+  r.m = wave_max(m);
+  S = wave_sum64(m == -INFINITY ? S : S * exp2_64(((double)m - (double)r.m) * a.c));
+  r.first = wave_min(m == r.m ? first : 0x7fffffff);
+  r.inv = S > 0.0 && r.m != -INFINITY && r.m != INFINITY ? 1.0 / S : 0.0;  // NaN: no distribution
+  return r;
+}
+
+__device__ __forceinline__ double prob(float x, const RowStat &r, double c) {
+  return exp2_64(((double)x - (double)r.m) * c) * r.inv;
+}
+
+// 1 / the sum of a whole row in 64 bits, by the workgroup.
+template <int DT, int NW>
+__device__ double exact_inv(const VerifyArgs &a, const typename Elem<DT>::T *row, float m, double *red) {
+  double S = 0.0;
+  for (int64_t c = (int64_t)(threadIdx.x >> 6) * kVBlock; c < a.V; c += NW * kVBlock) {
+    float x[4][8];
+    load_block<DT>(row, (int)c, a.V, x);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) S += exp2_64(((double)x[u][e] - (double)m) * a.c);
+  }
+  S = wave_sum64(S);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = S;
+  __syncthreads();
+  S = 0.0;
+  for (int k = 0; k < NW; ++k) S += red[k];
+  return 1.0 / S;
 }
 
 // The sequence's rows joined, the first draft that is not accepted found; tokens and log-probabilities of the accepted
 // ones written by the workgroup that is told to.
-template <int DT>
+template <int DT, bool EXACT, int NW>
 __device__ void decide(const VerifyArgs &a, int64_t s, bool write, VerifyArgs::Decision &dec) {
   __shared__ RowStat rows[2 * kVDrafts + 1];
+  __shared__ VerifyArgs::Decision found;
+  __shared__ double red[NW];
+  __shared__ int again;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, len = drafts_of(a, s);
-  for (int i = w; i < 2 * a.K + 1; i += kVWaves) {
+  for (int i = w; i < 2 * a.K + 1; i += NW) {
     const bool draft = i > a.K;
     if (draft ? (!a.zd || i - a.K - 1 >= len) : i > len) continue;
     const RowStat r = join_row(a, s, i);
     if (lane == 0) rows[i] = r;
   }
   __syncthreads();
-  __shared__ VerifyArgs::Decision found;
-  if (w == 0) {
-    int64_t x = -1;
-    bool ok = false, token = false;
-    double lp = 0.0;
-    RowStat p{}, q{};
-    if (lane < len) {
-      x = a.drafts[s * a.K + lane];
-      p = rows[lane];
-      token = x >= 0 && x < a.V;
-      if (a.greedy) {
-        ok = p.inv > 0.0 && x == p.first;
-      } else if (token && p.inv > 0.0) {
-        double qx = 1.0;
-        if (a.zd) {
-          q = rows[a.K + 1 + lane];
-          qx = q.inv > 0.0 ? prob((float)row_of<DT>(a.zd, a.ls_d, a.lr_d, s, lane)[x], q, a.inv_T) : __builtin_nan("");
-        }
-        ok = (double)a.u[s * (a.K + 1) + lane] * qx < prob((float)row_of<DT>(a.z, a.ls, a.lr, s, lane)[x], p, a.inv_T);
-      }
-      if (ok && write)
-        lp = ((double)(float)row_of<DT>(a.z, a.ls, a.lr, s, lane)[x] - (double)p.m) * a.inv_T + log(p.inv);
-    }
-    const uint64_t no = __ballot(!ok);  // lanes from len on are among them; K < 64
-    const int at = __ffsll((long long)no) - 1;
-    if (write && lane <= a.K) {
-      a.tokens[s * (a.K + 1) + lane] = lane < at ? x : -1;
-      a.logp[s * (a.K + 1) + lane] = lane < at ? (float)lp : 0.f;
-      if (lane == 0) a.accepted[s] = at;
-    }
-    if (lane == at) {  // at <= len <= K
-      found.p = rows[at];
-      found.a = at;
-      found.residual = 0;
-      found.x = (int)x;
-      if (at < len && token && !a.greedy) {
-        if (!a.zd) found.residual = 2;
-        else if (q.inv > 0.0) found.residual = 1;
-      }
-      found.q = found.residual == 1 ? q : RowStat{0.0, 0.f, 0};
+  int64_t x = -1;
+  bool ok = false, token = false, close = false;
+  float zp = 0.f, zq = 0.f, u = 0.f;
+  RowStat p{}, q{};
+  if (w == 0 && lane < len) {
+    x = a.drafts[s * a.K + lane];
+    token = x >= 0 && x < a.V;
+    if (!a.greedy) u = a.u[s * (a.K + 1) + lane];
+    if (token) {
+      zp = (float)row_of<DT>(a.z, a.ls, a.lr, s, lane)[x];
+      if (a.zd) zq = (float)row_of<DT>(a.zd, a.ls_d, a.lr_d, s, lane)[x];
     }
   }
-  __syncthreads();
+  for (int32_t known = -1;;) {  // once, and again for every draft whose rows have to be summed in 64 bits
+    if (w == 0) {
+      if (lane < len) {
+        p = rows[lane];
+        if (a.zd) q = rows[a.K + 1 + lane];
+        if (a.greedy) {
+          ok = p.inv > 0.0 && x == p.first;
+        } else if (token && p.inv > 0.0 && !(a.zd && !(q.inv > 0.0))) {
+          const double lhs = (double)u * (a.zd ? prob(zq, q, a.c) : 1.0), rhs = prob(zp, p, a.c);
+          ok = lhs < rhs;
+          close = !EXACT && lane > known && fabs(lhs - rhs) <= kVClose * rhs;
+        }
+      }
+      const uint64_t no = __ballot(!ok), near = __ballot(close);  // lanes from len on are in `no`; K < 64
+      const int at = __ffsll((long long)no) - 1, first_near = near ? __ffsll((long long)near) - 1 : 64;
+      if (first_near <= at && first_near < len) {
+        if (lane == 0) again = first_near;
+      } else {
+        if (lane == 0) again = -1;
+        if (write && lane <= a.K) {
+          a.tokens[s * (a.K + 1) + lane] = lane < at ? x : -1;
+          a.logp[s * (a.K + 1) + lane] =
+              lane < at ? (float)(((double)zp - (double)p.m) * a.c * kVLn2 + log(p.inv)) : 0.f;
+          if (lane == 0) a.accepted[s] = at;
+        }
+        if (lane == at) {  // at <= len <= K
+          found.p = rows[at];
+          found.a = at;
+          found.residual = 0;
+          found.x = (int)x;
+          if (at < len && token && !a.greedy) {
+            if (!a.zd) found.residual = 2;
+            else if (q.inv > 0.0) found.residual = 1;
+          }
+          found.q = found.residual == 1 ? q : RowStat{0.0, 0.f, 0};
+        }
+      }
+    }
+    __syncthreads();
+    const int i = again;
+    if (EXACT || i < 0) break;
+    const double inv_p = exact_inv<DT, NW>(a, row_of<DT>(a.z, a.ls, a.lr, s, i), rows[i].m, red);
+    const double inv_q = a.zd ? exact_inv<DT, NW>(a, row_of<DT>(a.zd, a.ls_d, a.lr_d, s, i), rows[a.K + 1 + i].m, red) : 0.0;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      rows[i].inv = inv_p;
+      if (a.zd) rows[a.K + 1 + i].inv = inv_q;
+    }
+    __syncthreads();
+    known = i;
+    close = false;
+  }
   dec = found;
 }
 
-// r of one column.
+// r of one column. MODE: Decision::residual.
+template <int MODE>
 __device__ __forceinline__ double mass(const VerifyArgs &a, const VerifyArgs::Decision &d, float x, float y, int c) {
-  const double p = prob(x, d.p, a.inv_T);
-  if (d.residual == 1) return fmax(p - prob(y, d.q, a.inv_T), 0.0);
-  return d.residual == 2 && c == d.x ? 0.0 : p;
+  const double p = prob(x, d.p, a.c);
+  if (MODE == 1) return fmax(p - prob(y, d.q, a.c), 0.0);
+  return MODE == 2 && c == d.x ? 0.0 : p;
+}
+
+__device__ __forceinline__ double sum_parts(const double *v, int n) {  // by each wave; the same in every lane
+  double S = 0.0;
+  for (int k = threadIdx.x & 63; k < n; k += 64) S += v[k];
+  return wave_sum64(S);
+}
+// Row a's statistics with the sums of the sums launch.
+__device__ __forceinline__ void exact_rows(const VerifyArgs &a, int64_t s, VerifyArgs::Decision &d) {
+  if (d.p.inv > 0.0) d.p.inv = 1.0 / sum_parts(a.sum_p + s * a.parts, a.parts);
+  if (d.residual == 1) d.q.inv = 1.0 / sum_parts(a.sum_q + s * a.parts, a.parts);
+}
+
+// A row a wave, for up to 8 drafts.
+constexpr int kVDecide = 1024;
+template <int DT>
+__global__ __launch_bounds__(kVDecide) void verify_decide_kernel(VerifyArgs a) {
+  VerifyArgs::Decision d;
+  decide<DT, false, kVDecide / 64>(a, blockIdx.x, true, d);
+  if (threadIdx.x == 0) a.dec[blockIdx.x] = d;
 }
 
 template <int DT>
+__global__ __launch_bounds__(kVThreads) void verify_sums_kernel(VerifyArgs a) {
+  const int64_t s = blockIdx.y;
+  const VerifyArgs::Decision d = a.dec[s];
+  if (!(d.p.inv > 0.0)) return;
+  for (int t = 0; t < a.turns; ++t) {
+    const int k = __builtin_amdgcn_readfirstlane((blockIdx.x * kVWaves + (threadIdx.x >> 6)) * a.turns + t);
+    if (k >= a.parts) return;
+    const int c0 = k * a.part, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.part);
+    for (int which = 0; which < (d.residual == 1 ? 2 : 1); ++which) {
+      const typename Elem<DT>::T *row = which ? row_of<DT>(a.zd, a.ls_d, a.lr_d, s, d.a)
+                                              : row_of<DT>(a.z, a.ls, a.lr, s, d.a);
+      const double md = which ? d.q.m : d.p.m;
+      double S = 0.0;
+      for (int c = c0; c < c1; c += kVBlock) {
+        float x[4][8];
+        load_block<DT>(row, c, c1, x);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) S += exp2_64(((double)x[u][e] - md) * a.c);
+      }
+      S = wave_sum64(S);
+      if ((threadIdx.x & 63) == 0) (which ? a.sum_q : a.sum_p)[s * a.parts + k] = S;
+    }
+  }
+}
+
+template <int DT, int MODE>
+__device__ __forceinline__ double part_mass(const VerifyArgs &a, const VerifyArgs::Decision &d,
+                                            const typename Elem<DT>::T *row, const typename Elem<DT>::T *rowd, int c0,
+                                            int c1) {
+  const int lane = threadIdx.x & 63;
+  double S = 0.0;
+  for (int c = c0; c < c1; c += kVBlock) {
+    float x[4][8], y[4][8];
+    load_block<DT>(row, c, c1, x);
+    if (MODE == 1) load_block<DT>(rowd, c, c1, y);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        S += mass<MODE>(a, d, x[u][e], MODE == 1 ? y[u][e] : 0.f, c + 512 * u + 8 * lane + e);
+  }
+  return wave_sum64(S);
+}
+
+template <int DT, bool EXACT>
 __global__ __launch_bounds__(kVThreads) void verify_residual_kernel(VerifyArgs a) {
   const int64_t s = blockIdx.y;
+  const int lane = threadIdx.x & 63;
   VerifyArgs::Decision d;
-  decide<DT>(a, s, blockIdx.x == 0, d);
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.dec[s] = d;
+  if constexpr (EXACT) {
+    decide<DT, true, kVWaves>(a, s, blockIdx.x == 0, d);
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.dec[s] = d;
+  } else {
+    d = a.dec[s];
+  }
   if (d.residual == 0 || !(d.p.inv > 0.0)) return;
-  const int c0 = blockIdx.x * a.per, c1 = min(a.V, c0 + a.per);
+  if constexpr (!EXACT) exact_rows(a, s, d);
   const typename Elem<DT>::T *row = row_of<DT>(a.z, a.ls, a.lr, s, d.a);
   const typename Elem<DT>::T *rowd = d.residual == 1 ? row_of<DT>(a.zd, a.ls_d, a.lr_d, s, d.a) : row;
-  double sum = 0.0;
-  sweep_slice<DT>(row, c0, c1, [&](float x, int c) { sum += mass(a, d, x, d.residual == 1 ? (float)rowd[c] : 0.f, c); });
-  __shared__ double ss[kVWaves];
-  sum = wave_sum64(sum);
-  if ((threadIdx.x & 63) == 0) ss[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    sum = 0.0;
-    for (int k = 0; k < kVWaves; ++k) sum += ss[k];
-    a.sums[s * a.slices + blockIdx.x] = sum;
+  for (int t = 0; t < a.turns; ++t) {
+    const int k = __builtin_amdgcn_readfirstlane((blockIdx.x * kVWaves + (threadIdx.x >> 6)) * a.turns + t);
+    if (k >= a.parts) return;
+    const int c0 = k * a.part, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.part);
+    const double S = d.residual == 1 ? part_mass<DT, 1>(a, d, row, rowd, c0, c1)
+                                     : part_mass<DT, 2>(a, d, row, rowd, c0, c1);
+    if (lane == 0) a.sum_r[s * a.parts + k] = S;
   }
 }
 
 // Of values that the threads hold in order (v, no less than 0): the first whose running sum, from `base` on, exceeds t,
-// else the last above 0; -1 without one. before: the running sum ahead of it. buf: kVThreads doubles.
-__device__ __forceinline__ int find_passing(double v, int n, double base, double t, double *buf, double &before) {
+// else the last above 0; -1 without one. before: the running sum ahead of it. buf: kVThreads + 2 doubles.
+__device__ __forceinline__ int find_passing(double v, double base, double t, double *buf, double &before) {
+  constexpr int RUN = kVThreads / 64;
   buf[threadIdx.x] = v;
   __syncthreads();
   if (threadIdx.x < 64) {  // each lane a run of the values, the runs' sums scanned
-    const int run = (n + 63) / 64, lo = min(n, (int)threadIdx.x * run), hi = min(n, lo + run);
+    const int lo = (int)threadIdx.x * RUN;
     double mine = 0.0;
-    for (int k = lo; k < hi; ++k) mine += buf[k];
+#pragma unroll
+    for (int k = 0; k < RUN; ++k) mine += buf[lo + k];
     double incl = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -306,13 +511,14 @@ __device__ __forceinline__ int find_passing(double v, int n, double base, double
     double cum = base + (incl - mine);
     int at = -1, last = -1;
     double ahead = 0.0, ahead_last = 0.0;
-    for (int k = lo; k < hi; ++k) {
-      const double x = buf[k];
+#pragma unroll
+    for (int k = 0; k < RUN; ++k) {
+      const double x = buf[lo + k];
       if (x > 0.0) {
-        last = k;
+        last = lo + k;
         ahead_last = cum;
         if (at < 0 && cum + x > t) {
-          at = k;
+          at = lo + k;
           ahead = cum;
         }
       }
@@ -342,21 +548,36 @@ __device__ __forceinline__ int find_passing(double v, int n, double base, double
   return got;
 }
 
-template <int DT>
+// A thread's run of columns.
+template <int DT, int MODE>
+__device__ __forceinline__ double run_mass(const VerifyArgs &a, const VerifyArgs::Decision &d,
+                                           const typename Elem<DT>::T *row, const typename Elem<DT>::T *rowd, int lo,
+                                           int hi) {
+  double S = 0.0;
+  for (int c = lo; c < hi; c += 8) {
+    float x[8], y[8];
+    load_values<DT>(row, c, hi, x);
+    if (MODE == 1) load_values<DT>(rowd, c, hi, y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) S += mass<MODE>(a, d, x[e], MODE == 1 ? y[e] : 0.f, c + e);
+  }
+  return S;
+}
+
+template <int DT, bool EXACT>
 __global__ __launch_bounds__(kVThreads) void verify_pick_kernel(VerifyArgs a) {
-  __shared__ double part[kVSlices];
+  __shared__ double part[kVParts];
   __shared__ double buf[kVThreads + 2];
   __shared__ int token;
   const int64_t s = blockIdx.x;
   VerifyArgs::Decision d;
-  if (a.greedy) decide<DT>(a, s, true, d);
+  if (a.greedy) decide<DT, EXACT, kVWaves>(a, s, true, d);
   else d = a.dec[s];
   const int64_t out = s * (a.K + 1) + d.a;
   if (!(d.p.inv > 0.0)) {  // the target's row has no distribution: no token
     if (threadIdx.x == 0) a.logp[out] = __builtin_nanf("");
     return;
   }
-  const typename Elem<DT>::T *row = row_of<DT>(a.z, a.ls, a.lr, s, d.a);
   if (a.greedy) {
     if (threadIdx.x == 0) {
       a.tokens[out] = d.p.first;
@@ -364,19 +585,23 @@ __global__ __launch_bounds__(kVThreads) void verify_pick_kernel(VerifyArgs a) {
     }
     return;
   }
+  if constexpr (!EXACT) exact_rows(a, s, d);
+  const typename Elem<DT>::T *row = row_of<DT>(a.z, a.ls, a.lr, s, d.a);
   const typename Elem<DT>::T *rowd = d.residual == 1 ? row_of<DT>(a.zd, a.ls_d, a.lr_d, s, d.a) : row;
-  // the slices' sums; where p - q leaves nothing (p = q up to rounding), p itself
+  // the parts' sums; where p - q leaves nothing (p = q up to rounding), p itself
   double all = 0.0;
-  for (int pass = 0; pass < 2; ++pass) {
+  for (;;) {
     const bool res = d.residual != 0;
     double mine = 0.0;
-    for (int k = threadIdx.x; k < a.slices; k += kVThreads) {
+    for (int k = threadIdx.x; k < a.parts; k += kVThreads) {
       double x;
       if (res) {
-        x = a.sums[s * a.slices + k];
+        x = a.sum_r[s * a.parts + k];
+      } else if constexpr (EXACT) {
+        const PartStat t = a.stats[(s * (2 * a.K + 1) + d.a) * a.parts + k];
+        x = t.m == -INFINITY ? 0.0 : t.S * exp2_64(((double)t.m - (double)d.p.m) * a.c) * d.p.inv;
       } else {
-        const SliceStat t = a.stats[(s * (2 * a.K + 1) + d.a) * a.slices + k];
-        x = t.m == -INFINITY ? 0.0 : t.S * exp64(((double)t.m - (double)d.p.m) * a.inv_T) * d.p.inv;
+        x = a.sum_p[s * a.parts + k] * d.p.inv;
       }
       part[k] = x;
       mine += x;
@@ -391,103 +616,120 @@ __global__ __launch_bounds__(kVThreads) void verify_pick_kernel(VerifyArgs a) {
     d.residual = 0;
   }
   const double t = (double)a.u[s * (a.K + 1) + a.K] * all;
-  // the slice: each thread a run of slices
-  const int srun = (a.slices + kVThreads - 1) / kVThreads;
+  // the part: each thread a run of them
+  const int run = (a.parts + kVThreads - 1) / kVThreads;
   double mine = 0.0;
-  for (int k = threadIdx.x * srun; k < min(a.slices, (int)(threadIdx.x + 1) * srun); ++k) mine += part[k];
+  for (int k = threadIdx.x * run; k < min(a.parts, (int)(threadIdx.x + 1) * run); ++k) mine += part[k];
   double base;
-  const int owner = find_passing(mine, kVThreads, 0.0, t, buf, base);
-  if (owner < 0) {  // u is no number, or nothing is left
+  const int owner = find_passing(mine, 0.0, t, buf, base);
+  if (owner < 0) {  // nothing is left
     if (threadIdx.x == 0) a.logp[out] = __builtin_nanf("");
     return;
   }
-  int slice = owner * srun, last = slice;
-  double cum = base, cum_last = base;
-  for (int k = slice, done = 0; k < min(a.slices, (owner + 1) * srun) && !done; ++k) {
+  int got = owner * run;
+  double cum = base;
+  for (int k = got, done = 0; k < min(a.parts, (owner + 1) * run) && !done; ++k) {
     if (part[k] > 0.0) {
-      last = k;
-      cum_last = cum;
+      got = k;
+      base = cum;
       done = cum + part[k] > t;
     }
     cum += part[k];
   }
-  slice = last;
-  base = cum_last;
-  // the token: each thread a run of the slice's columns
-  const int c0 = slice * a.per, c1 = min(a.V, c0 + a.per), run = a.per / kVThreads;
-  const int lo = min(c1, c0 + (int)threadIdx.x * run), hi = min(c1, lo + run);
-  mine = 0.0;
-  for (int c = lo; c < hi; ++c) mine += mass(a, d, (float)row[c], d.residual == 1 ? (float)rowd[c] : 0.f, c);
-  const int who = find_passing(mine, kVThreads, base, t, buf, base);
+  // the token: each thread a run of the part's columns, 8 at a time
+  const int c0 = got * a.part, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.part), width = a.part / kVThreads;
+  const int lo = min(c1, c0 + (int)threadIdx.x * width), hi = min(c1, lo + width);
+  mine = d.residual == 1 ? run_mass<DT, 1>(a, d, row, rowd, lo, hi)
+         : d.residual == 2 ? run_mass<DT, 2>(a, d, row, rowd, lo, hi)
+                           : run_mass<DT, 0>(a, d, row, rowd, lo, hi);
+  const int who = find_passing(mine, base, t, buf, base);
   if (threadIdx.x == 0) token = -1;
   __syncthreads();
   if ((int)threadIdx.x == who) {
-    int got = -1;
-    double run_sum = base;
+    int v = -1;
+    double sum = base;
     for (int c = lo; c < hi; ++c) {
-      const double x = mass(a, d, (float)row[c], d.residual == 1 ? (float)rowd[c] : 0.f, c);
+      const float z = (float)row[c];
+      const double x = d.residual == 1 ? mass<1>(a, d, z, (float)rowd[c], c)
+                       : d.residual == 2 ? mass<2>(a, d, z, z, c) : mass<0>(a, d, z, z, c);
       if (x > 0.0) {
-        got = c;
-        if (run_sum + x > t) break;
+        v = c;
+        if (sum + x > t) break;
       }
-      run_sum += x;
+      sum += x;
     }
-    token = got;
+    token = v;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
     a.tokens[out] = token;
-    a.logp[out] = token < 0 ? __builtin_nanf("") : (float)(((double)(float)row[token] - (double)d.p.m) * a.inv_T + log(d.p.inv));
+    a.logp[out] = token < 0 ? __builtin_nanf("")
+                            : (float)(((double)(float)row[token] - (double)d.p.m) * a.c * kVLn2 + log(d.p.inv));
   }
 }
 
-// Values of a slice: 4,096, and as many times 1,024 more as keep a row within kVSlices slices.
-static int slice_values(int V) {
-  const int64_t least = round_up(cdiv(V, kVSlices), 1024);
-  return (int)(least > 4096 ? least : 4096);
-}
+// Parts of one block, and as many blocks more as keep a row within kVParts parts.
+static int part_values(int V) { return (int)round_up(cdiv(V, kVParts), kVBlock); }
+
+// Rows that are summed with 32-bit exponentials, from this many logits on.
+constexpr int64_t kVMany = (int64_t)1 << 24;
 
 struct VerifyLayout {
-  int slices, per;
+  int parts, part;
   size_t stats, sums, dec, total;
 };
 static VerifyLayout verify_layout(int64_t S, int K, int V) {
   VerifyLayout L;
-  L.per = slice_values(V);
-  L.slices = (int)cdiv(V, L.per);
+  L.part = part_values(V);
+  L.parts = (int)cdiv(V, L.part);
   L.stats = 0;
-  L.sums = (size_t)S * (2 * K + 1) * L.slices * sizeof(SliceStat);
-  L.dec = L.sums + (size_t)round_up(S * L.slices * 8, 16);
+  L.sums = (size_t)S * (2 * K + 1) * L.parts * sizeof(PartStat);
+  L.dec = L.sums + (size_t)round_up(3 * S * L.parts * 8, 16);
   L.total = L.dec + (size_t)S * sizeof(VerifyArgs::Decision);
   return L;
 }
 
-template <int DT> static int go_verify(const VerifyArgs &a, hipStream_t st) {
+template <int DT, bool EXACT> static int go_launches(const VerifyArgs &a, hipStream_t st) {
+  const dim3 parts((unsigned)cdiv(a.parts, kVWaves), (unsigned)(a.S * (2 * a.K + 1)));
+  const dim3 taken((unsigned)cdiv(a.parts, (int64_t)kVWaves * a.turns), (unsigned)a.S);
+  hipLaunchKernelGGL((verify_stats_kernel<DT, EXACT>), parts, dim3(kVThreads), 0, st, a);
+  OCTO_CHECK_LAUNCH("verify_stats");
+  if (!a.greedy && !EXACT) {
+    hipLaunchKernelGGL(verify_decide_kernel<DT>, dim3((unsigned)a.S), dim3(kVDecide), 0, st, a);
+    OCTO_CHECK_LAUNCH("verify_decide");
+    hipLaunchKernelGGL(verify_sums_kernel<DT>, taken, dim3(kVThreads), 0, st, a);
+    OCTO_CHECK_LAUNCH("verify_sums");
+  }
+  if (!a.greedy && (EXACT || a.K > 0)) {
+    hipLaunchKernelGGL((verify_residual_kernel<DT, EXACT>), taken, dim3(kVThreads), 0, st, a);
+    OCTO_CHECK_LAUNCH("verify_residual");
+  }
+  hipLaunchKernelGGL((verify_pick_kernel<DT, EXACT>), dim3((unsigned)a.S), dim3(kVThreads), 0, st, a);
+  OCTO_CHECK_LAUNCH("verify_pick");
+  return OCTO_OK;
+}
+
+template <int DT> static int go_verify(const VerifyArgs &a, bool exact, hipStream_t st) {
   const int rows = 2 * a.K + 1;
-  VerifyArgs b = a;
   const int64_t step = 65535 / rows;  // sequences a launch: a grid's second dimension
   for (int64_t s0 = 0; s0 < a.S; s0 += step) {
-    const int64_t n = a.S - s0 < step ? a.S - s0 : step;
-    b.S = n;
+    VerifyArgs b = a;
+    b.S = a.S - s0 < step ? a.S - s0 : step;
     b.z = (const typename Elem<DT>::T *)a.z + s0 * a.ls;
     b.zd = a.zd ? (const typename Elem<DT>::T *)a.zd + s0 * a.ls_d : nullptr;
     b.drafts = a.drafts + s0 * a.K;
     b.lengths = a.lengths ? a.lengths + s0 : nullptr;
     b.u = a.u ? a.u + s0 * (a.K + 1) : nullptr;
-    b.stats = a.stats + s0 * rows * a.slices;
-    b.sums = a.sums + s0 * a.slices;
+    b.stats = a.stats + s0 * rows * a.parts;
+    b.sum_p = a.sum_p + s0 * a.parts;
+    b.sum_q = a.sum_q + s0 * a.parts;
+    b.sum_r = a.sum_r + s0 * a.parts;
     b.dec = a.dec + s0;
     b.tokens = a.tokens + s0 * (a.K + 1);
     b.accepted = a.accepted + s0;
     b.logp = a.logp + s0 * (a.K + 1);
-    hipLaunchKernelGGL(verify_stats_kernel<DT>, dim3((unsigned)a.slices, (unsigned)(n * rows)), dim3(kVThreads), 0, st, b);
-    OCTO_CHECK_LAUNCH("verify_stats");
-    if (!a.greedy) {
-      hipLaunchKernelGGL(verify_residual_kernel<DT>, dim3((unsigned)a.slices, (unsigned)n), dim3(kVThreads), 0, st, b);
-      OCTO_CHECK_LAUNCH("verify_residual");
-    }
-    hipLaunchKernelGGL(verify_pick_kernel<DT>, dim3((unsigned)n), dim3(kVThreads), 0, st, b);
-    OCTO_CHECK_LAUNCH("verify_pick");
+    const int rc = exact ? go_launches<DT, true>(b, st) : go_launches<DT, false>(b, st);
+    if (rc) return rc;
   }
   return OCTO_OK;
 }
@@ -538,20 +780,30 @@ int octo_verify_drafts(const void *logits, int64_t ld_seq, int64_t ld_row, const
   a.S = S;
   a.K = K;
   a.V = V;
-  a.inv_T = inv_T;
   a.greedy = greedy != 0;
-  a.slices = L.slices;
-  a.per = L.per;
-  a.stats = (SliceStat *)((char *)ws + L.stats);
-  a.sums = (double *)((char *)ws + L.sums);
+  const double c = inv_T * 1.4426950408889634074;
+  a.c = c;
+  a.c_hi = (float)c;
+  a.c_lo = (float)(c - (double)a.c_hi);
+  a.d_least = (float)(-300.0 / c);
+  a.parts = L.parts;
+  a.part = L.part;
+  // a wave takes several parts where there are many: each of its workgroups first joins the sequence's rows
+  const int64_t turns = S * L.parts / (kVWaves * 2048);
+  a.turns = (int)(turns < 1 ? 1 : (turns > 8 ? 8 : turns));
+  a.stats = (PartStat *)((char *)ws + L.stats);
+  a.sum_p = (double *)((char *)ws + L.sums);
+  a.sum_q = a.sum_p + S * L.parts;
+  a.sum_r = a.sum_q + S * L.parts;
   a.dec = (VerifyArgs::Decision *)((char *)ws + L.dec);
   a.tokens = tokens;
   a.accepted = accepted;
   a.logp = logp;
+  const bool exact = S * (a.zd ? 2 * K + 1 : K + 1) * (int64_t)V < kVMany || !(c >= 0x1p-40 && c <= 0x1p40);
   switch (dtype) {
-    case OCTO_BF16: return go_verify<OCTO_BF16>(a, (hipStream_t)stream);
-    case OCTO_F16: return go_verify<OCTO_F16>(a, (hipStream_t)stream);
-    default: return go_verify<OCTO_F32>(a, (hipStream_t)stream);
+    case OCTO_BF16: return go_verify<OCTO_BF16>(a, exact, (hipStream_t)stream);
+    case OCTO_F16: return go_verify<OCTO_F16>(a, exact, (hipStream_t)stream);
+    default: return go_verify<OCTO_F32>(a, exact, (hipStream_t)stream);
   }
 }
 

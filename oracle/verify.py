@@ -70,3 +70,38 @@ def verify(logits, drafts, uniform, T, draft_logits=None, lengths=None, greedy=F
         tokens.append(out + [-1] * (rows - len(out)))
         logp.append(lps + [0.0] * (rows - len(lps)))
     return tokens, accepted, logp
+
+
+def verify_dense(logits, drafts, uniform, T, draft_logits=None, lengths=None):
+    """The same by whole rows of tensors, for large vocabularies; rows with a softmax only."""
+    import torch
+    S, rows, V = logits.shape
+    K = rows - 1
+    tokens = torch.full((S, rows), -1, dtype=torch.int64)
+    logp = torch.zeros(S, rows, dtype=torch.float64)
+    accepted = torch.zeros(S, dtype=torch.int64)
+    for s in range(S):
+        n = K if lengths is None else min(max(int(lengths[s]), 0), K)
+        lp = torch.log_softmax(logits[s].double() / T, 1)
+        lq = None if draft_logits is None else torch.log_softmax(draft_logits[s].double() / T, 1)
+        a = 0
+        while a < n:
+            x = int(drafts[s, a])
+            qx = 1.0 if lq is None else lq[a, x].exp().item()
+            if not float(uniform[s, a]) * qx < lp[a, x].exp().item():
+                break
+            tokens[s, a], logp[s, a] = x, lp[a, x]
+            a += 1
+        r = lp[a].exp()
+        if a < n:
+            less = r.clone()
+            if lq is None:
+                less[int(drafts[s, a])] = 0.0
+            else:
+                less = (r - lq[a].exp()).clamp(min=0.0)
+            r = less if less.any() else r
+        cum = r.cumsum(0)
+        v = int((cum <= float(uniform[s, K]) * cum[-1]).sum())
+        v = min(v, int(r.nonzero()[-1, 0]))
+        tokens[s, a], logp[s, a], accepted[s] = v, lp[a, v], a
+    return tokens, accepted, logp

@@ -154,6 +154,80 @@ def test_strides():
     assert (one[0] == one[0][:1]).all()
 
 
+# ---- many logits: the rows' sums with 32-bit exponentials first -------------------------------------------------------
+
+def _check_many(z, x, u, T=1.0, zd=None, lengths=None):
+    d = lambda t: None if t is None else t.to(DEV)  # noqa: E731
+    assert z.numel() + (0 if zd is None else zd.numel()) >= 1 << 24
+    tokens, accepted, logp = verify_op.verify_drafts(d(z), d(x), d(u), T, draft_logits=d(zd), lengths=d(lengths))
+    want, count, lp = oracle.verify_dense(z, x, u, T, zd, lengths)
+    assert torch.equal(accepted.cpu(), count) and torch.equal(tokens.cpu(), want)
+    # the accepted drafts' by a row sum that 32-bit exponentials make, within 4e-6 of it
+    torch.testing.assert_close(logp.cpu().double(), lp, rtol=2.0 ** -24, atol=4e-6)
+    return tokens.cpu(), accepted.cpu()
+
+
+@pytest.mark.parametrize("dtype,S,K,V,T", [(torch.bfloat16, 40, 3, 61003, 1.0), (torch.float16, 300, 0, 56000, 0.7),
+                                           (torch.float32, 9, 7, 128257, 1.3), (torch.bfloat16, 1030, 1, 5500, 1.0),
+                                           (torch.bfloat16, 3, 1, 3000001, 0.9)])
+def test_many_logits(dtype, S, K, V, T):
+    z, zd, x, u = _inputs(S, K, V, dtype, S)
+    n = torch.randint(0, K + 1, (S,), generator=torch.Generator().manual_seed(1))
+    _check_many(z, x, u, T, zd if K else None)
+    z[S // 2, :, 60:], zd[S // 2, :, 60:], x[S // 2] = NINF, NINF, 7
+    _check_many(z, x, u, T, zd if K else None, n)
+    if K and z.numel() >= 1 << 24:
+        _check_many(z, x, u, T)
+
+
+@pytest.mark.parametrize("sampled", [True, False])
+def test_many_drafts_on_the_border(sampled):
+    """u the number of 32 bits next to p / q: below, accepted, above, rejected, 2^-25 of it or less to decide by."""
+    S, K, V = 150, 2, 40000
+    z, zd, x, u = _inputs(S, K, V, torch.bfloat16, 5)
+    zd = zd if sampled else None
+    p = torch.log_softmax(z[:, :K].double(), 2).gather(2, x[:, :, None])[:, :, 0]
+    q = torch.log_softmax(zd.double(), 2).gather(2, x[:, :, None])[:, :, 0] if sampled else torch.zeros_like(p)
+    ratio = (p - q).exp()
+    near = ratio.float()
+    step = torch.where(near.double() < ratio, near, torch.nextafter(near, torch.zeros_like(near)))  # the largest below
+    above = torch.nextafter(step, torch.full_like(step, 9.0))
+    up = torch.rand(S, K, generator=torch.Generator().manual_seed(2)) < 0.4
+    apart = (above.double() - ratio).abs() > 1e-12 * ratio
+    u[:, :K] = torch.where(up & apart, above, step)
+    _, acc = _check_many(z, x, u, 1.0, zd)
+    assert torch.equal(acc, (~(up & apart)).long().cumprod(1).sum(1))
+
+
+def test_many_without_a_distribution():
+    z, zd, x, u = _inputs(700, 1, 13000, torch.bfloat16, 8)
+    z[0, 0], z[1, 0, 12999], z[2, 0, 0] = NINF, math.nan, math.inf
+    zd[3, 0], zd[4, 0, 1], x[5, 0] = NINF, math.inf, -1
+    z[6] = torch.finfo(torch.bfloat16).min
+    tokens, acc, logp = verify_op.verify_drafts(z.to(DEV), x.to(DEV), u.to(DEV), 1.0, draft_logits=zd.to(DEV))
+    assert acc[:6].tolist() == [0] * 6 and tokens[:3].tolist() == [[-1, -1]] * 3 and torch.isnan(logp[:3, 0]).all()
+    assert (logp[:6, 1] == 0).all() and (tokens[:6, 1] == -1).all()
+    want, count, lp = oracle.verify_dense(z[3:6, 0:1], x[3:6, :0], u[3:6, 1:], 1.0)  # drawn from the target alone
+    assert tokens[3:6, 0].tolist() == want[:, 0].tolist()
+    want, count, _ = oracle.verify_dense(z[6:], x[6:], u[6:], 1.0, zd[6:])
+    assert torch.equal(tokens[6:].cpu(), want) and torch.equal(acc[6:].cpu(), count)
+    got = verify_op.verify_drafts(z.to(DEV), x.to(DEV), None, 1.0, greedy=True)
+    assert got[0][:3].tolist() == [[-1, -1]] * 3
+    best = z[7:].float().argmax(2)
+    assert torch.equal(got[1][7:].cpu(), (x[7:, 0] == best[:, 0]).long())
+
+
+def test_extreme_temperatures():
+    z, zd, x, u = _inputs(3, 2, 200, torch.float32)
+    for T in (1e-13, 1e-3, 1e4, 1e13):
+        _check(z, x, u, T)
+    z, zd, x, u = _inputs(700, 1, 13000, torch.float32)
+    z[::3, :, ::2] = NINF
+    x.clamp_(1, 12999).bitwise_or_(1)
+    for T in (1e-13, 1e-5, 1e13):
+        _check_many(z, x, u, T)
+
+
 def test_refusals():
     z, zd, x, u = (t.to(DEV) for t in _inputs(3, 2, 50, torch.bfloat16))
     ok = dict(draft_logits=zd)

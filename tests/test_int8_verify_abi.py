@@ -133,3 +133,15 @@ def test_oracle_verify_greedy_and_masks():
     z = torch.tensor([[[0.0, 2.0, 2.0], [1.0, 0.0, 0.0]], [[-math.inf] * 3, [0.0] * 3]])
     tokens, acc, logp = verify.verify(z, torch.tensor([[1], [0]]), None, 1.0, greedy=True)
     assert tokens == [[1, 0], [-1, -1]] and acc == [1, 0] and math.isnan(logp[1][0])
+
+
+def test_oracle_verify_dense():
+    g = torch.Generator().manual_seed(0)
+    z, zd = torch.randn(30, 4, 50, generator=g) * 2, torch.randn(30, 3, 50, generator=g) * 2
+    zd[5, :, 9:], z[5, :, 9:] = -math.inf, -math.inf
+    x, u = torch.randint(0, 9, (30, 3), generator=g), torch.rand(30, 4, generator=g)
+    n = torch.randint(0, 4, (30,), generator=g)
+    for d in (zd, None):
+        a, b = verify.verify(z, x, u, 0.8, d, n), verify.verify_dense(z, x, u, 0.8, d, n)
+        assert a[0] == b[0].tolist() and a[1] == b[1].tolist()
+        assert (torch.tensor(a[2], dtype=torch.float64) - b[2]).abs().max() < 1e-12
