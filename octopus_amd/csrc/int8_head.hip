@@ -8,6 +8,7 @@
 #include "gemm_nt.h"
 #include "octo_internal.h"
 #include "row_values.h"
+#include "rows8.h"
 
 namespace octo {
 
@@ -18,6 +19,8 @@ constexpr int kGroup8 = 4;
 
 typedef __attribute__((address_space(3))) f32x4 lds_f4;
 typedef i32x4 i32x4_el __attribute__((aligned(2)));
+typedef i32x4 i32x4_el4 __attribute__((aligned(4)));
+typedef i32x2 i32x2_el __attribute__((aligned(2)));
 
 struct Logits8 {
   const float *sx, *sw;
@@ -94,6 +97,137 @@ __global__ __launch_bounds__(2 * NTHREADS, 1) __attribute__((amdgpu_waves_per_eu
   f32x4 acc[8][4];
   mainloop_ring5<DT_I8, OpRowsN<8, 128>, OpRowsN<8, 64>, true>(A, B, m0, n0, s.K, smem, acc);
   store_logits8<OT>(acc, e, m0, n0, (int)s.M, min(s.N - n0, (int64_t)TN), smem);
+}
+
+// ---- few rows --------------------------------------------------------------------------------------------------------
+//
+// Up to 32 rows the weight's bytes set the time. The rows, quantised by every workgroup for itself (which saves a launch;
+// workgroup 0 leaves them to the caller), stay in the LDS, and each wave runs through a share of the weight rows of its
+// own, 16 at a time: the MFMA's first operand comes from global memory as it lies (lane l: row l & 15, 16 bytes at
+// 16 (l >> 4) of each 64), kFewSteps loads ahead, also into the next 16 rows, and no wave waits for another. The shares
+// are equal to 4 rows, so that all waves end together: in blocks of 16 rows 9,496 blocks on 6,144 waves take as long as
+// 12,288 would. A share's last block repeats its last row (no bytes of its own, and its MFMAs are idle time).
+constexpr int kFewSteps = 8;
+constexpr int kFewLds = 156 * 1024;  // with the scales, what a workgroup can have
+constexpr int64_t kFewRows = 32;
+
+struct Few8 {
+  const void *x;
+  int64_t ldx;
+  const int8_t *wq;
+  int64_t ldw;
+  const float *sw;
+  int n, d, V, share;  // share: weight rows a wave takes
+  int8_t *xq;
+  int64_t ldxq;
+  float *sx;
+  void *z;
+  int64_t ldz;
+};
+
+// LDS bytes between rows: the next multiple of 64 (a step), and 16 so that rows start on different banks.
+__host__ __device__ constexpr int few_ld(int d) { return (d + 63) / 64 * 64 + 16; }
+
+template <int DT, typename OT, int NB, int NW>
+__global__ __launch_bounds__(64 * NW) void few_i8_kernel(Few8 a) {
+  extern __shared__ __attribute__((aligned(16))) char few_smem[];
+  __shared__ float scales[16 * NB];
+  lds_char *smem = (lds_char *)few_smem;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qd = lane >> 4;
+  const int chunks = (a.d + 15) >> 4, steps = (chunks + 3) >> 2, ld = few_ld(a.d);
+  const int first = (blockIdx.x * NW + w) * a.share, last = min(first + a.share, a.V);
+  i32x4 cur[kFewSteps], nxt[kFewSteps];
+  // steps s0 .. of the 16 rows from m0; chunks past a row's end: its last one, times the zeros of x there
+  auto load = [&](i32x4(&v)[kFewSteps], int m0, int s0) {
+    const i32x4 *p = (const i32x4 *)(a.wq + (int64_t)min(m0 + (lane & 15), last - 1) * a.ldw);
+#pragma unroll
+    for (int u = 0; u < kFewSteps; ++u) v[u] = p[min(4 * (s0 + u) + qd, chunks - 1)];
+  };
+  if (first < last) load(cur, first, 0);
+  for (int r = w; r < a.n; r += NW) {
+    lds_char *row = smem + r * ld;
+    int8_t *kept = blockIdx.x == 0 ? a.xq + r * a.ldxq : nullptr;
+    const float s = quantise_row<DT, (DT == OCTO_F32 ? 2 : 4)>((const typename Elem<DT>::T *)a.x + r * a.ldx, a.d, (a.d + 63) / 64 * 8,
+                                     [&](int c, i32x2 v) {
+      *(__attribute__((address_space(3))) i32x2 *)(row + 8 * c) = v;
+      if (kept && c < 2 * chunks) *(i32x2 *)(kept + 8 * c) = v;
+    });
+    if (lane == 0) {
+      scales[r] = s;
+      if (kept) a.sx[r] = s;
+    }
+  }
+  __syncthreads();
+  if (first >= last) return;
+  const lds_char *xl[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) xl[b] = smem + min(16 * b + (lane & 15), a.n - 1) * ld + 16 * qd;
+  for (int m0 = first; m0 < last; m0 += 16) {
+    i32x4 acc[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = i32x4{0, 0, 0, 0};
+    for (int s0 = 0; s0 < steps; s0 += kFewSteps) {
+      const bool more = s0 + kFewSteps < steps;
+      if (more || m0 + 16 < last) load(nxt, more ? m0 : m0 + 16, more ? s0 + kFewSteps : 0);
+#pragma unroll
+      for (int u = 0; u < kFewSteps; ++u) {
+        if (s0 + u >= steps) break;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          acc[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur[u], *(const lds_i32x4 *)(xl[b] + 64 * (s0 + u)), acc[b], 0,
+                                                         0, 0);
+      }
+#pragma unroll
+      for (int u = 0; u < kFewSteps; ++u) cur[u] = nxt[u];
+    }
+    const int v0 = m0 + 4 * qd;
+    if (v0 < last) {
+      float sw[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sw[e] = a.sw[min(v0 + e, a.V - 1)];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int t = 16 * b + (lane & 15);
+        if (t >= a.n) continue;
+        OT o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (OT)((float)acc[b][e] * scales[t] * sw[e]);
+        OT *out = (OT *)a.z + t * a.ldz + v0;
+        if (v0 + 4 <= a.V) {
+          if constexpr (sizeof(OT) == 2) *(i32x2_el *)out = __builtin_bit_cast(i32x2, o);
+          else *(i32x4_el4 *)out = __builtin_bit_cast(i32x4, o);
+        } else {
+          for (int e = 0; v0 + e < a.V; ++e) out[e] = o[e];
+        }
+      }
+    }
+  }
+}
+
+// Whether the rows fit.
+static bool few_fits(int64_t n, int d) { return n <= kFewRows && n * few_ld(d) <= kFewLds; }
+
+template <int DT, typename OT, int NB> static int go_few(Few8 a, hipStream_t st) {
+  const int lds = a.n * few_ld(a.d);
+  // 16 waves a CU: two workgroups of 8 where two fit, else one of 16
+  const int wgs = lds <= 78 * 1024 ? 2 : 1, NW = 16 / wgs;
+  const int64_t waves = (int64_t)octo_tiles::kCus * wgs * NW;
+  a.share = (int)round_up(cdiv(a.V, waves), 4);
+  const dim3 grid((unsigned)cdiv(a.V, (int64_t)a.share * NW));
+  if (wgs > 1) hipLaunchKernelGGL((few_i8_kernel<DT, OT, NB, 8>), grid, dim3(512), lds, st, a);
+  else hipLaunchKernelGGL((few_i8_kernel<DT, OT, NB, 16>), grid, dim3(1024), lds, st, a);
+  OCTO_CHECK_LAUNCH("few_i8");
+  return OCTO_OK;
+}
+template <int DT, typename OT> static int go_few(const Few8 &a, hipStream_t st) {
+  return a.n <= 16 ? go_few<DT, OT, 1>(a, st) : go_few<DT, OT, 2>(a, st);
+}
+template <typename OT> static int go_few(const Few8 &a, int x_dtype, hipStream_t st) {
+  switch (x_dtype) {
+    case OCTO_BF16: return go_few<OCTO_BF16, OT>(a, st);
+    case OCTO_F16: return go_few<OCTO_F16, OT>(a, st);
+    default: return go_few<OCTO_F32, OT>(a, st);
+  }
 }
 
 static Operand operand8(const void *base, int64_t ld_bytes, int64_t rows) {
@@ -182,6 +316,7 @@ int octo_head_logits_i8(const void *rows, int64_t ldx, int x_dtype, const int8_t
                         int z_dtype, void *stream) {
   int rc = head8_checks("head_logits_i8", n, d, V, ldxq, ldw);
   if (rc) return rc;
+  if (rows && !is_float(x_dtype)) return octo_fail(OCTO_EUNSUPPORTED, "head_logits_i8: dtype %d", x_dtype);
   OCTO_CHECK_ARG(ldz >= V, "head_logits_i8: row stride %lld below V=%d", (long long)ldz, V);
   if (!is_float(z_dtype)) return octo_fail(OCTO_EUNSUPPORTED, "head_logits_i8: dtype %d", z_dtype);
   if (n == 0) return OCTO_OK;
@@ -190,6 +325,15 @@ int octo_head_logits_i8(const void *rows, int64_t ldx, int x_dtype, const int8_t
                      (uintptr_t)x_scale % 4 == 0 && (uintptr_t)logits % float_bytes(z_dtype) == 0,
                  "head_logits_i8: misaligned pointer");
   hipStream_t st = (hipStream_t)stream;
+  if (rows && few_fits(n, d)) {
+    OCTO_CHECK_ARG(ldx >= d && (uintptr_t)rows % float_bytes(x_dtype) == 0, "head_logits_i8: row stride or alignment");
+    const Few8 a{rows, ldx, wq, ldw, w_scale, (int)n, d, V, 0, xq, ldxq, x_scale, logits, ldz};
+    switch (z_dtype) {
+      case OCTO_BF16: return go_few<__bf16>(a, x_dtype, st);
+      case OCTO_F16: return go_few<_Float16>(a, x_dtype, st);
+      default: return go_few<float>(a, x_dtype, st);
+    }
+  }
   if (rows) {
     rc = octo_quantise_i8_rows(rows, ldx, x_dtype, n, d, 0, xq, ldxq, x_scale, stream);
     if (rc) return rc;

@@ -11,66 +11,10 @@
 // between its maximum and its quotients.
 #include "octo_internal.h"
 #include "row_values.h"
+#include "rows8.h"
 
 namespace octo {
 
-constexpr int kHeldChunks = 8;  // chunks of 8 values a lane keeps: rows of up to 4,096
-constexpr float kLeastMax = 0x1p-119f;
-
-// 8 consecutive values from an address of any element alignment (global loads of 16 bytes need none).
-typedef i32x4 i32x4_any __attribute__((aligned(2)));
-typedef i32x4 i32x4_any4 __attribute__((aligned(4)));
-template <int DT> __device__ __forceinline__ void load8(const typename Elem<DT>::T *p, int valid, float (&x)[8]) {
-  if (valid >= 8) {
-    if constexpr (DT == OCTO_F32) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const i32x4 v = *((const i32x4_any4 *)p + h);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * h + e] = __int_as_float(v[e]);
-      }
-    } else {
-      unpack8(*(const i32x4_any *)p, DT == OCTO_F16, x);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = e < valid ? (float)p[e] : 0.f;
-  }
-}
-
-// The magnitudes' bits compare as the magnitudes do, NaN above all.
-__device__ __forceinline__ uint32_t max_bits(const float (&x)[8], uint32_t m) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
-  return m;
-}
-template <int LANES> __device__ __forceinline__ uint32_t lanes_max(uint32_t m) {
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-  return m;
-}
-__device__ __forceinline__ float scale_of(uint32_t maxbits) {
-  if (maxbits >= 0x7f800000u) return __builtin_nanf("");
-  const float a = __uint_as_float(maxbits);
-  return a < kLeastMax ? 0.f : a * (1.f / 127.f);
-}
-// 8 quotients as bytes. x inv is within an integer of x / s and the remainder x - q s is exact in one fma (at most 7
-// bits of q times 24 of s, less x: within fp32's 24 bits above the finer of the two last places), so comparing it with
-// s / 2 gives the quotient's rounding exactly.
-__device__ __forceinline__ i32x2 quotients(const float (&x)[8], float s, float inv) {
-  const float half = 0.5f * s;
-  i32x2 out = {0, 0};
-  if (!(s > 0.f)) return out;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float q = __builtin_rintf(x[e] * inv);
-    const float r = __builtin_fmaf(-q, s, x[e]), ar = fabsf(r);
-    const int odd = (int)q & 1;
-    if (ar > half || (ar == half && odd)) q += __builtin_copysignf(1.f, r);
-    out[e >> 2] |= ((int)q & 0xff) << (8 * (e & 3));
-  }
-  return out;
-}
 
 // GL: lanes of a group (8 values each); 0: the group is the row. Zeros behind the row, up to its next 16 bytes.
 template <int DT, int GL>
@@ -82,56 +26,23 @@ __global__ __launch_bounds__(256) void quantise_i8_kernel(const typename Elem<DT
   const typename Elem<DT>::T *row = x + r * ldx;
   int8_t *out = q + r * ldq;
   const int chunks = (d + 7) >> 3, padded = ((d + 15) >> 4) << 1;
-  float v[kHeldChunks][8];
-  float s = 0.f, inv = 0.f;
-  if (GL == 0) {
-    uint32_t m = 0;
-    if (chunks > 64 * kHeldChunks) {  // a long row is read twice
-      for (int c = lane; c < chunks; c += 64) {
-        load8<DT>(row + 8 * c, d - 8 * c, v[0]);
-        m = max_bits(v[0], m);
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < kHeldChunks; ++u) {
-        if (64 * u >= chunks) break;
-        const int c = 64 * u + lane;
-        load8<DT>(row + 8 * c, d - 8 * c, v[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < kHeldChunks; ++u) {
-        if (64 * u >= chunks) break;
-        m = max_bits(v[u], m);
-      }
-    }
-    s = scale_of(lanes_max<64>(m));
-    inv = 1.f / s;
+  if constexpr (GL == 0) {
+    const float s = quantise_row<DT, 8>(row, d, padded, [&](int c, i32x2 v) { *(i32x2 *)(out + 8 * c) = v; });
     if (lane == 0) scale[r] = s;
-    if (chunks <= 64 * kHeldChunks) {
+  } else {
+    const int groups = (chunks + GL - 1) / GL;
+    for (int c0 = 0; c0 < padded; c0 += 64 * 4) {  // 4 chunks in flight
+      Raw8<DT> v[4];
+      load_chunks<DT, 4>(row, d, c0, v);
 #pragma unroll
-      for (int u = 0; u < kHeldChunks; ++u) {
-        const int c = 64 * u + lane;
-        if (c < padded) *(i32x2 *)(out + 8 * c) = quotients(v[u], s, inv);
+      for (int u = 0; u < 4; ++u) {
+        const int c = c0 + 64 * u + lane;
+        float x[8];
+        values8<DT>(v[u], x);
+        const float s = scale_of(lanes_max<GL>(max_bits(x, 0)));
+        if (lane % GL == 0 && c < chunks) scale[r * groups + c / GL] = s;
+        if (c < padded) *(i32x2 *)(out + 8 * c) = quotients(x, s, 1.f / s);
       }
-      return;
-    }
-  }
-  const int groups = GL ? (chunks + GL - 1) / GL : 1;
-  for (int c0 = 0; c0 < padded; c0 += 64 * 4) {  // 4 chunks in flight
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int c = c0 + 64 * u + lane;
-      load8<DT>(row + 8 * c, d - 8 * c, v[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int c = c0 + 64 * u + lane;
-      if (GL) {
-        s = scale_of(lanes_max<(GL ? GL : 64)>(max_bits(v[u], 0)));
-        inv = 1.f / s;
-        if (lane % (GL ? GL : 64) == 0 && c < chunks) scale[r * groups + c / (GL ? GL : 1)] = s;
-      }
-      if (c < padded) *(i32x2 *)(out + 8 * c) = quotients(v[u], s, inv);
     }
   }
 }
