@@ -132,10 +132,13 @@ static_assert(SMEM_RING5 <= 160 * 1024, "LDS budget");
 // per SIMD, so one issues MFMAs while the other waits on a stage or runs its epilogue). An operand's SUB is the
 // wave's rows of it (128; 64 for the B operand of the 8-wave loop). A slice takes 32 DMA instructions, 32 / NW per
 // wave.
-template <int NW, int SUB>
+// ROWS: the tile's rows of the operand (256; less in the narrower tiles of int8_head.hip, whose slices are smaller).
+template <int NW, int SUB, int ROWS_ = 256>
 struct OpRowsN {
-  static constexpr int NI = 32 / NW;   // DMA instructions per wave and stage
-  static constexpr int NB = SUB / 16;  // the wave's 16-row fragment blocks
+  static constexpr int ROWS = ROWS_;
+  static constexpr int SLICE = ROWS * EKB;
+  static constexpr int NI = ROWS / 8 / NW;  // DMA instructions per wave and stage
+  static constexpr int NB = SUB / 16;       // the wave's 16-row fragment blocks
   typedef i32x4 F;  // fragment as held between its read and its MFMAs
   static __device__ __forceinline__ i32x4 op(const F &f) { return f; }
   __amdgpu_buffer_rsrc_t rs;
@@ -172,7 +175,7 @@ struct OpRowsN {
       off[q] = rowoff + coff;
     }
     if (op.map) rs = make_rsrc(uniform_ptr(op.base), op.extent);
-    else rs = make_rsrc(uniform_ptr(op.base + row0 * op.ld), (uint32_t)(256 * op.ld));
+    else rs = make_rsrc(uniform_ptr(op.base + row0 * op.ld), (uint32_t)(ROWS * op.ld));
     // lane l holds row l & 15 of a 16-row block and chunk 4 ks + (l >> 4) of K-step ks; (row >> 1) & 7 depends on
     // l & 15 alone, and 4 ks + g = (4 ks) ^ g for g < 4, so K-step 1's offset is K-step 0's with chunk bit 2 flipped
     const int row = wsub * SUB + (lane & 15);
@@ -215,6 +218,8 @@ __device__ __forceinline__ s16x4 lds_read_tr16(lds_s16x4 *__restrict__ p) {
 // Nothing is bounds-checked: the caller guarantees K-rows up to the next multiple of 64 exist and read zero past K.
 template <int NW, int SUB>
 struct OpColsN {
+  static constexpr int ROWS = 256;
+  static constexpr int SLICE = ESLICE;
   static constexpr int NI = 32 / NW;
   static constexpr int NB = SUB / 16;
   // A fragment is carried as its two 8-byte halves and joined at each MFMA: a joined 16-byte value carried across
@@ -293,6 +298,16 @@ template <> struct Mfma16<OCTO_F16> {
   }
 };
 
+// MFMAs from one DMA issue to the next: ni of them from MFMA d0 on, spread over a K-step of nq.
+constexpr int ring5_every(int ni, int nq, int d0) {
+  const int up = (nq - d0 + ni - 1) / ni;
+  return d0 + (ni - 1) * up < nq ? up : (nq - d0) / ni;
+}
+// Bytes of a ring slot: the larger slice.
+template <typename OA, typename OB> constexpr int ring5_slot() {
+  return OA::SLICE > OB::SLICE ? OA::SLICE : OB::SLICE;
+}
+
 // One stage of the ring loop on the stage in slots (sa, sa + 1): two K-steps of K = 32, each 64 v_mfma_f32_16x16x32
 // over the wave's 8 x 8 blocks (A fragment i reused by 8 consecutive MFMAs). The 16 fragment reads of the next K-step
 // go under the first 16 MFMAs (double-buffered: K-step ks uses fa[ks], fb[ks]); the barrier B_k sits between the two
@@ -308,14 +323,17 @@ template <int DT, typename OA, typename OB, bool DMA, bool NEXT, bool XFRAG, boo
 __device__ __forceinline__ void ring5_stage(const OA &opa, const OB &opb, int kd, int sa, uint32_t kbytes,
                                             lds_char *smem, typename OA::F (&fa)[2][OA::NB],
                                             typename OB::F (&fb)[2][OB::NB], f32x4 (&acc)[OA::NB][OB::NB]) {
-  constexpr int NA = OA::NB, NBB = OB::NB, NQ = NA * NBB, NR = NA + NBB, NI = OA::NI;
-  constexpr int D0 = NR + 1, DS = (NQ - D0 + NI - 1) / NI;  // DMA issues: MFMA D0, D0 + DS, ... (4 waves: 17 + 6 j)
+  constexpr int NA = OA::NB, NBB = OB::NB, NQ = NA * NBB, NR = NA + NBB;
+  // DMA issues: MFMA D0, D0 + DS, ... (4 waves: 17 + 6 j)
+  constexpr int D0 = NR + 1;
+  constexpr int DSA = ring5_every(OA::NI, NQ, D0), DSB = ring5_every(OB::NI, NQ, D0);
   // SPLIT: L_k at MFMA QX; DQX DMA instructions of this K-step are issued before it
-  constexpr int QX = NQ / 2, DQX = QX <= D0 ? 0 : ((QX - 1 - D0) / DS + 1 < NI ? (QX - 1 - D0) / DS + 1 : NI);
-  static_assert(!SPLIT || QX + NR <= NQ, "next-stage fragment reads fit the K-step");
+  constexpr int QX = NQ / 2 + NR <= NQ ? NQ / 2 : NQ - NR;
+  constexpr int DQX = QX <= D0 ? 0 : ((QX - 1 - D0) / DSB + 1 < OB::NI ? (QX - 1 - D0) / DSB + 1 : OB::NI);
+  static_assert(QX > 0 && D0 + (OA::NI - 1) * DSA < NQ && D0 + (OB::NI - 1) * DSB < NQ, "all within the K-step");
   constexpr int XQ = SPLIT ? QX : 0;  // first MFMA under which stage k + 1's fragments are read
   // slots: stage k at (sa, sa + 1), stage k + 1 at (sa + 2, sa + 3), stage k + 2's A at sa + 4, its B at sa
-  auto slot = [&](int d) -> lds_char * { const int x = sa + d; return smem + (x >= ENSLOT ? x - ENSLOT : x) * ESLICE; };
+  auto slot = [&](int d) -> lds_char * { const int x = sa + d; return smem + (x >= ENSLOT ? x - ENSLOT : x) * ring5_slot<OA, OB>(); };
   const lds_char *cA = slot(0), *cB = slot(1);
   const lds_char *nA = slot(2), *nB = slot(3);
   lds_char *dA = slot(4), *dB = slot(0);
@@ -324,7 +342,7 @@ __device__ __forceinline__ void ring5_stage(const OA &opa, const OB &opb, int kd
     if (ks == 1 && NEXT) {
       __builtin_amdgcn_s_waitcnt(WAIT_LGKM0);  // this wave's reads of stage k are done
       if (!SPLIT) {
-        if (DMA) __builtin_amdgcn_s_waitcnt(waitcnt_vm(NI));  // stage k + 1 landed (k + 2's A may be in flight)
+        if (DMA) __builtin_amdgcn_s_waitcnt(waitcnt_vm(OA::NI));  // stage k + 1 landed (k + 2's A may be in flight)
         else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
       }
       __builtin_amdgcn_s_barrier();  // ... in every wave; stage k's slots are free
@@ -336,7 +354,7 @@ __device__ __forceinline__ void ring5_stage(const OA &opa, const OB &opb, int kd
     for (int q = 0; q < NQ; ++q) {
       if (SPLIT && ks == 1 && NEXT && q == QX) {
         // L_k: stage k + 1 landed (stage k + 2's A and this K-step's first B issues may be in flight) ... everywhere
-        if (DMA) __builtin_amdgcn_s_waitcnt(waitcnt_vm(NI + DQX));
+        if (DMA) __builtin_amdgcn_s_waitcnt(waitcnt_vm(OA::NI + DQX));
         else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
         __builtin_amdgcn_s_barrier();
         OCTO_FENCE();
@@ -357,9 +375,12 @@ __device__ __forceinline__ void ring5_stage(const OA &opa, const OB &opb, int kd
         else fb[0][q - XQ - NA] = opb.frag(nB, 0, q - XQ - NA);
         OCTO_FENCE();
       }
-      if (DMA && q >= D0 && (q - D0) % DS == 0 && (q - D0) / DS < NI) {
-        if (ks == 0) opa.dma(kd, (q - D0) / DS, kbytes, dA);
-        else opb.dma(kd, (q - D0) / DS, kbytes, dB);
+      if (DMA && ks == 0 && q >= D0 && (q - D0) % DSA == 0 && (q - D0) / DSA < OA::NI) {
+        opa.dma(kd, (q - D0) / DSA, kbytes, dA);
+        OCTO_FENCE();
+      }
+      if (DMA && ks == 1 && q >= D0 && (q - D0) % DSB == 0 && (q - D0) / DSB < OB::NI) {
+        opb.dma(kd, (q - D0) / DSB, kbytes, dB);
         OCTO_FENCE();
       }
     }
@@ -370,34 +391,34 @@ __device__ __forceinline__ int ring_slot(int s) { return s >= ENSLOT ? s - ENSLO
 
 // The ring loop's prologue: stage 0 into slots (sa0, sa0 + 1), its A slice first and by itself (the B operand may still
 // wait for its row map then), stage 1 (when nk > 1) into (sa0 + 2, sa0 + 3), mod 5.
-template <typename OA>
+template <typename OA, typename OB>
 __device__ __forceinline__ void ring5_prologue_a(const OA &opa, int sa0, uint32_t kbytes, lds_char *smem) {
 #pragma unroll
-  for (int q = 0; q < OA::NI; ++q) opa.dma(0, q, kbytes, smem + ring_slot(sa0) * ESLICE);
+  for (int q = 0; q < OA::NI; ++q) opa.dma(0, q, kbytes, smem + ring_slot(sa0) * ring5_slot<OA, OB>());
   OCTO_FENCE();
 }
 template <typename OA, typename OB>
 __device__ __forceinline__ void ring5_prologue(const OA &opa, const OB &opb, int sa0, uint32_t kbytes, int nk,
                                                lds_char *smem) {
-  constexpr int NI = OA::NI;
+  constexpr int SLOT = ring5_slot<OA, OB>();
 #pragma unroll
-  for (int q = 0; q < NI; ++q) opb.dma(0, q, kbytes, smem + ring_slot(sa0 + 1) * ESLICE);
+  for (int q = 0; q < OB::NI; ++q) opb.dma(0, q, kbytes, smem + ring_slot(sa0 + 1) * SLOT);
   if (nk > 1) {
 #pragma unroll
-    for (int q = 0; q < NI; ++q) opa.dma(1, q, kbytes, smem + ring_slot(sa0 + 2) * ESLICE);
+    for (int q = 0; q < OA::NI; ++q) opa.dma(1, q, kbytes, smem + ring_slot(sa0 + 2) * SLOT);
 #pragma unroll
-    for (int q = 0; q < NI; ++q) opb.dma(1, q, kbytes, smem + ring_slot(sa0 + 3) * ESLICE);
+    for (int q = 0; q < OB::NI; ++q) opb.dma(1, q, kbytes, smem + ring_slot(sa0 + 3) * SLOT);
   }
 }
 
 // The ring loop after its prologue, stage j of the tile in slots (sa0 + 2 j, sa0 + 2 j + 1) mod 5; acc is zeroed
 // here. Ends with every DMA landed and every wave past its last LDS read (the slots are free), and returns the slot
 // that continues the ring, (sa0 + 2 nk) mod 5. VMEM instructions issued after the prologue's (a previous tile's
-// epilogue stores) are fine: loads complete in order among themselves, so at most 2 NI outstanding means stage 0 in.
+// epilogue stores) are fine: loads complete in order among themselves, so at most a stage's instructions outstanding means stage 0 in.
 template <int DT, typename OA, typename OB, bool SPLIT, bool TR>
 __device__ __forceinline__ int ring5_run(const OA &opa, const OB &opb, int sa0, uint32_t kbytes, int nk,
                                          lds_char *smem, f32x4 (&acc)[OA::NB][OB::NB]) {
-  constexpr int NI = OA::NI;
+  constexpr int SLOT = ring5_slot<OA, OB>();
 #pragma unroll
   for (int i = 0; i < OA::NB; ++i)
 #pragma unroll
@@ -405,16 +426,16 @@ __device__ __forceinline__ int ring5_run(const OA &opa, const OB &opb, int sa0, 
 #pragma unroll
       for (int v = 0; v < 4; ++v) acc[i][j][v] = 0.f;
   if (nk == 0) return sa0;
-  if (nk > 1) __builtin_amdgcn_s_waitcnt(waitcnt_vm(2 * NI));  // stage 0 landed
+  if (nk > 1) __builtin_amdgcn_s_waitcnt(waitcnt_vm(OA::NI + OB::NI));  // stage 0 landed
   else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
   __builtin_amdgcn_s_barrier();
 
   typename OA::F fa[2][OA::NB];
   typename OB::F fb[2][OB::NB];
 #pragma unroll
-  for (int b = 0; b < OA::NB; ++b) fa[0][b] = opa.frag(smem + ring_slot(sa0) * ESLICE, 0, b);
+  for (int b = 0; b < OA::NB; ++b) fa[0][b] = opa.frag(smem + ring_slot(sa0) * SLOT, 0, b);
 #pragma unroll
-  for (int b = 0; b < OB::NB; ++b) fb[0][b] = opb.frag(smem + ring_slot(sa0 + 1) * ESLICE, 0, b);
+  for (int b = 0; b < OB::NB; ++b) fb[0][b] = opb.frag(smem + ring_slot(sa0 + 1) * SLOT, 0, b);
   int sa = sa0;  // slot of stage k's A slice: sa0 + 2 k mod 5
   int k = 0;
   for (; k + 2 < nk; ++k) {
@@ -437,8 +458,7 @@ template <int DT, typename OA, typename OB, bool SPLIT = false, bool TR = false>
 __device__ __forceinline__ void mainloop_ring5(const Operand &A, const Operand &B, int64_t m0, int64_t n0,
                                                int64_t K_eff, lds_char *smem, f32x4 (&acc)[OA::NB][OB::NB]) {
   static_assert(DT == OCTO_BF16 || DT == OCTO_F16 || DT == DT_I8, "16-bit or 8-bit integer operands");
-  static_assert(OA::NI == OB::NI, "one workgroup shape");
-  constexpr int NWN = TN / (16 * OB::NB);  // waves along N
+  constexpr int NWN = OB::ROWS / (16 * OB::NB);  // waves along N
   const int w = threadIdx.x >> 6;
   const int wm = w / NWN, wn = w % NWN;
   const uint32_t kbytes = (uint32_t)(K_eff * (DT == DT_I8 ? 1 : 2));
@@ -448,7 +468,7 @@ __device__ __forceinline__ void mainloop_ring5(const Operand &A, const Operand &
   if (nk > 0) {
     opa.init(A, m0, wm, OA::rows(A, m0));
     opb.init(B, n0, wn, OB::rows(B, n0));
-    ring5_prologue_a(opa, 0, kbytes, smem);
+    ring5_prologue_a<OA, OB>(opa, 0, kbytes, smem);
     ring5_prologue(opa, opb, 0, kbytes, nk, smem);
   }
   ring5_run<DT, OA, OB, SPLIT, TR>(opa, opb, 0, kbytes, nk, smem, acc);

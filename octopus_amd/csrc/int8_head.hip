@@ -16,8 +16,8 @@ constexpr int kMaxD8 = 131072;       // 127^2 d < 2^31
 constexpr int kMaxV8 = 1 << 21;      // a tile's 256 rows of g within 32-bit offsets
 constexpr int64_t kMaxN8 = 1 << 21;  // the same of the transposed rows
 constexpr int kGroup8 = 4;
+constexpr int64_t kSmallRows = 128;
 
-typedef __attribute__((address_space(3))) f32x4 lds_f4;
 typedef i32x4 i32x4_el __attribute__((aligned(2)));
 typedef i32x4 i32x4_el4 __attribute__((aligned(4)));
 typedef i32x2 i32x2_el __attribute__((aligned(2)));
@@ -28,42 +28,57 @@ struct Logits8 {
   int64_t ldz;
 };
 
-// The product over tiles of 256 vocabulary rows x 256 tokens, weights as the MFMA's first operand: a lane's 4 sums of a
-// block are 4 neighbouring logits of one token. Scaled, rounded once, and out through the LDS in rows of 256 logits.
-// A slot holds 4 logits; slot s of token t sits at s ^ 4 (t & 15): a write's 16 tokens x 4 slots cover all banks.
-template <typename OT>
-__device__ __forceinline__ void store_logits8(const f32x4 (&acc)[8][4], const Logits8 &e, int64_t v0, int64_t n0, int V,
-                                              int64_t nvalid, lds_char *smem) {
-  typedef Acc16N<4> L;
-  constexpr int SLOT = 4 * sizeof(OT), ROW = 64 * SLOT, HALVES = sizeof(OT) == 4 ? 2 : 1, TOK = 256 / HALVES;
-  constexpr int LPR = ROW / 16, PER = 16 / sizeof(OT);  // lanes of a row, logits of a lane
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wm = L::wm(w), wn = L::wn(w);
-  const int vvalid = (int)min((int64_t)TM, V - v0);
-  float sx[4];
+// The product over tiles of VM vocabulary rows x TN tokens, weights as the MFMA's first operand: a lane's 4 sums of a
+// block are 4 neighbouring logits of one token. NW waves, 2 along the vocabulary.
+template <int VM, int TOK, int NW_> struct Tile8 {
+  static constexpr int NW = NW_, NWN = NW / 2, ROWS = VM, TOKENS = TOK;
+  typedef OpRowsN<NW, VM / 2, VM> A;
+  typedef OpRowsN<NW, TOK / NWN, TOK> B;
+  static constexpr int NA = A::NB, NB = B::NB, LDS = ENSLOT * ring5_slot<A, B>();
+  static __device__ __forceinline__ int row(int w, int i, int lane) { return w / NWN * (VM / 2) + i * 16 + 4 * (lane >> 4); }
+  static __device__ __forceinline__ int col(int w, int j, int lane) { return w % NWN * (TOK / NWN) + j * 16 + (lane & 15); }
+};
+typedef Tile8<256, 256, 8> TileWide;    // one workgroup a CU
+typedef Tile8<256, 192, 8> Tile192;     // the last tokens of a wide grid
+typedef Tile8<256, 128, 8> Tile128;
+typedef Tile8<128, 128, 4> TileSmall;   // half the LDS: two workgroups a CU, one of which loads and multiplies while the
+                                        // other begins or stores
+
+// Scaled, rounded once, and out through the LDS in rows of the tile's logits. A slot holds 4 logits; slot s of token t
+// sits at s ^ 4 (t & 15) (128 logits: t & 7): a write's 16 tokens x 4 slots cover all banks.
+template <class L, typename OT>
+__device__ __forceinline__ void store_logits8(const f32x4 (&acc)[L::NA][L::NB], const Logits8 &e, int64_t v0, int64_t n0,
+                                              int V, int64_t nvalid, lds_char *smem) {
+  constexpr int SLOT = 4 * sizeof(OT), ROW = L::ROWS / 4 * SLOT, HALVES = L::TOKENS * ROW > L::LDS ? 2 : 1;
+  constexpr int TOK = L::TOKENS / HALVES;
+  constexpr int LPR = ROW / 16, PER = 16 / sizeof(OT), SWZ = L::ROWS / 16 - 1;  // lanes of a row, logits of a lane
+  static_assert(TOK * ROW <= L::LDS && L::NWN % HALVES == 0, "staged in the ring");
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int vvalid = (int)min((int64_t)L::ROWS, V - v0);
+  float sx[L::NB];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int t = L::col(wn, j, lane);
+  for (int j = 0; j < L::NB; ++j) {
+    const int t = L::col(w, j, lane);
     sx[j] = t < nvalid ? e.sx[n0 + t] : 0.f;
   }
   OT *out = (OT *)e.z + n0 * e.ldz + v0;
-  const bool whole = vvalid == TM && (sizeof(OT) == 2 || ((uintptr_t)e.z % 4 == 0));
   for (int h = 0; h < HALVES; ++h) {
     if (h) __syncthreads();
-    if (HALVES == 1 || (wn >> 1) == h) {
+    if (w % L::NWN / (L::NWN / HALVES) == h) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int m = L::row(wm, i, 0, lane);
+      for (int i = 0; i < L::NA; ++i) {
+        const int m = L::row(w, i, lane);
         float sw[4];
 #pragma unroll
         for (int v = 0; v < 4; ++v) sw[v] = m + v < vvalid ? e.sw[v0 + m + v] : 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < L::NB; ++j) {
           const i32x4 q = __builtin_bit_cast(i32x4, acc[i][j]);
-          const int t = L::col(wn, j, lane) - h * TOK;
+          const int t = L::col(w, j, lane) - h * TOK;
           OT o[4];
 #pragma unroll
           for (int v = 0; v < 4; ++v) o[v] = (OT)((float)q[v] * sx[j] * sw[v]);
-          lds_char *at = smem + t * ROW + (((m >> 2) ^ ((t & 15) << 2)) * SLOT);
+          lds_char *at = smem + t * ROW + (((m >> 2) ^ ((t & SWZ) << 2)) * SLOT);
           if constexpr (sizeof(OT) == 4) *(lds_i32x4 *)at = __builtin_bit_cast(i32x4, o);
           else *(__attribute__((address_space(3))) i32x2 *)at = __builtin_bit_cast(i32x2, o);
         }
@@ -71,11 +86,12 @@ __device__ __forceinline__ void store_logits8(const f32x4 (&acc)[8][4], const Lo
     }
     __syncthreads();
     const int c = threadIdx.x % LPR, c0 = c * PER;
-    for (int t = threadIdx.x / LPR; t < TOK && h * TOK + t < nvalid; t += 512 / LPR) {
-      const i32x4 v = *(const lds_i32x4 *)(smem + t * ROW + (c * 16 ^ (((t & 15) << 2) * SLOT)));
+    for (int t = threadIdx.x / LPR; t < TOK && h * TOK + t < nvalid; t += 64 * L::NW / LPR) {
+      const i32x4 v = *(const lds_i32x4 *)(smem + t * ROW + (c * 16 ^ (((t & SWZ) << 2) * SLOT)));
       OT *o = out + (h * TOK + t) * e.ldz + c0;
-      if (whole) {
-        __builtin_nontemporal_store(v, (i32x4_el *)o);
+      if (vvalid == L::ROWS) {
+        if constexpr (sizeof(OT) == 4) __builtin_nontemporal_store(v, (i32x4_el4 *)o);
+        else __builtin_nontemporal_store(v, (i32x4_el *)o);
       } else {
         OT x[PER];
         __builtin_memcpy(x, &v, 16);
@@ -87,16 +103,28 @@ __device__ __forceinline__ void store_logits8(const f32x4 (&acc)[8][4], const Lo
   }
 }
 
+template <class L, typename OT>
+__device__ __forceinline__ void gemm_i8_tile(const Operand &A, const Operand &B, const GemmShape &s, const Logits8 &e,
+                                             int64_t m0, int64_t n0, lds_char *smem) {
+  f32x4 acc[L::NA][L::NB];
+  mainloop_ring5<DT_I8, typename L::A, typename L::B, true>(A, B, m0, n0, s.K, smem, acc);
+  store_logits8<L, OT>(acc, e, m0, n0, (int)s.M, min(s.N - n0, (int64_t)L::TOKENS), smem);
+}
 template <typename OT>
-__global__ __launch_bounds__(2 * NTHREADS, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_kernel(Operand A, Operand B, GemmShape s, Logits8 e) {
-  __shared__ __attribute__((aligned(16))) char smem_[SMEM_RING5];
-  lds_char *smem = (lds_char *)smem_;
+__global__ __launch_bounds__(512, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_kernel(Operand A, Operand B, GemmShape s, Logits8 e) {
+  __shared__ __attribute__((aligned(16))) char smem_[TileWide::LDS];
   int mt, nt;
   if (!tile_of(s, mt, nt)) return;
-  const int64_t m0 = (int64_t)mt * TM, n0 = (int64_t)nt * TN;
-  f32x4 acc[8][4];
-  mainloop_ring5<DT_I8, OpRowsN<8, 128>, OpRowsN<8, 64>, true>(A, B, m0, n0, s.K, smem, acc);
-  store_logits8<OT>(acc, e, m0, n0, (int)s.M, min(s.N - n0, (int64_t)TN), smem);
+  const int64_t m0 = (int64_t)mt * 256, n0 = (int64_t)nt * 256, left = s.N - n0;
+  if (left <= 128) gemm_i8_tile<Tile128, OT>(A, B, s, e, m0, n0, (lds_char *)smem_);
+  else if (left <= 192) gemm_i8_tile<Tile192, OT>(A, B, s, e, m0, n0, (lds_char *)smem_);
+  else gemm_i8_tile<TileWide, OT>(A, B, s, e, m0, n0, (lds_char *)smem_);
+}
+template <typename OT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_small_kernel(Operand A, Operand B, GemmShape s, Logits8 e) {
+  __shared__ __attribute__((aligned(16))) char smem_[TileSmall::LDS];
+  int mt, nt;
+  if (tile_of(s, mt, nt)) gemm_i8_tile<TileSmall, OT>(A, B, s, e, (int64_t)mt * 128, (int64_t)nt * 128, (lds_char *)smem_);
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
@@ -242,13 +270,13 @@ static Operand operand8(const void *base, int64_t ld_bytes, int64_t rows) {
   return X;
 }
 
-static GemmShape shape8(int64_t M, int64_t N, int64_t K) {
+static GemmShape shape8(int64_t M, int64_t N, int64_t K, int tile = TM) {
   GemmShape s;
   s.M = M;
   s.N = N;
   s.K = K;
-  s.mtiles = (int)cdiv(M, TM);
-  s.ntiles = (int)cdiv(N, TN);
+  s.mtiles = (int)cdiv(M, tile);
+  s.ntiles = (int)cdiv(N, tile);
   s.group_m = kGroup8;
   s.count_on = 0;
   s.count = nullptr;
@@ -339,14 +367,19 @@ int octo_head_logits_i8(const void *rows, int64_t ldx, int x_dtype, const int8_t
     if (rc) return rc;
   }
   const Logits8 e{x_scale, w_scale, logits, ldz};
-  const GemmShape s = shape8(V, n, round_up(d, 16));
   const Operand A = operand8(wq, ldw, V), B = operand8(xq, ldxq, n);
-  const dim3 grid((unsigned)tile_grid(s.mtiles, s.ntiles));
+  const bool small = n <= kSmallRows;
+  const GemmShape s = shape8(V, n, round_up(d, 16), small ? 128 : 256);
+  const dim3 grid((unsigned)tile_grid(s.mtiles, s.ntiles)), block(small ? 256 : 512);
+#define OCTO_GO(OT)                                                                                \
+  if (small) hipLaunchKernelGGL(gemm_i8_small_kernel<OT>, grid, block, 0, st, A, B, s, e);         \
+  else hipLaunchKernelGGL(gemm_i8_kernel<OT>, grid, block, 0, st, A, B, s, e)
   switch (z_dtype) {
-    case OCTO_BF16: hipLaunchKernelGGL(gemm_i8_kernel<__bf16>, grid, dim3(2 * NTHREADS), 0, st, A, B, s, e); break;
-    case OCTO_F16: hipLaunchKernelGGL(gemm_i8_kernel<_Float16>, grid, dim3(2 * NTHREADS), 0, st, A, B, s, e); break;
-    default: hipLaunchKernelGGL(gemm_i8_kernel<float>, grid, dim3(2 * NTHREADS), 0, st, A, B, s, e); break;
+    case OCTO_BF16: OCTO_GO(__bf16); break;
+    case OCTO_F16: OCTO_GO(_Float16); break;
+    default: OCTO_GO(float); break;
   }
+#undef OCTO_GO
   OCTO_CHECK_LAUNCH("gemm_i8");
   return OCTO_OK;
 }

@@ -36,7 +36,9 @@ def _check_logits(z, x, wq, ws, out):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,d,V", [(1, 64, 1000), (1, 2560, 515), (2, 16, 1), (3, 27, 5), (16, 1027, 300), (16, 4200, 100), (9, 4032, 700), (17, 128, 257),
                                    (33, 200, 255), (48, 4100, 131), (64, 1024, 512), (65, 130, 256), (130, 96, 1023), (256, 144, 300),
-                                   (257, 1, 513), (300, 4097, 264)])
+                                   (257, 1, 513), (300, 4097, 264), (129, 300, 515), (192, 65, 256), (193, 512, 511), (384, 97, 300), (400, 96, 513),
+                                   (449, 2048, 260), (513, 200, 300), (600, 1100, 515), (1025, 64, 256),
+                                   (800, 2048, 100)])
 def test_logits(n, d, V, dtype):
     x, w = _inputs(n, d, V, dtype, n + d)
     wq, ws = int8_op.quantise_rows(w.to(DEV))
