@@ -101,7 +101,7 @@ SIGNATURES = {
     "octo_quantise_i8_rows": [_p, _i64, _i32, _i64, _i32, _i32, _p, _i64, _p, _p],
     "octo_widen_i8_rows": [_p, _i64, _p, _i64, _i32, _i32, _p, _i64, _i32, _p],
     "octo_head_logits_i8": [_p, _i64, _i32, _p, _i64, _p, _i64, _i32, _i32, _p, _i64, _p, _p, _i64, _i32, _p],
-    "octo_head_grads_i8_workspace_bytes": [_i64, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_sz)],
+    "octo_head_grads_i8_workspace_bytes": [_p, _i64, _i32, _i64, _i32, _i32, _i32, _i32, ctypes.POINTER(_sz)],
     "octo_head_grads_i8": [_p, _i64, _i32, _p, _i64, _p, _p, _i64, _p, _i64, _i32, _i32, _p, _i64, _i32, _p, _i64,
                            _i32, _p, _sz, _p],
     "octo_verify_workspace_bytes": [_i64, _i32, _i32, ctypes.POINTER(_sz)],

@@ -264,6 +264,28 @@ struct OpColsN {
   }
 };
 
+// OpColsN of a matrix that ends with its last row: what lies at or past K-row op.rows or M value op.extent reads zero
+// where it would lie behind the matrix (op.extent, and the row stride, whole 16-byte chunks; the M values past extent of
+// the rows before are the next rows', and belong to no C).
+template <int NW, int SUB>
+struct OpColsEdge : OpColsN<NW, SUB> {
+  typedef OpColsN<NW, SUB> Base;
+  int64_t left;  // bytes from base to the matrix's end
+  __device__ __forceinline__ void init(const Operand &op, int64_t col0, int wsub, const typename Base::Rows &m) {
+    Base::init(op, col0, wsub, m);
+    left = (op.rows - 1) * op.ld + ((int64_t)op.extent - col0) * 2;
+  }
+  __device__ __forceinline__ void dma(int k, int q, uint32_t /*kbytes*/, lds_char *slice) const {
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r0 = 2 * (q & 1) + 4 * ((q >> 1) & 1) + 8 * NW * (q >> 2);
+    const int64_t stage = (int64_t)k * 64 * this->ld;
+    const int64_t behind = left - stage, most = (int64_t)64 * this->ld + 512;
+    const uint32_t room = (uint32_t)(behind < 0 ? 0 : (behind < most ? behind : most));
+    const uint32_t off = this->lo[q & 1] + (uint32_t)r0 * this->ld;
+    lds_dma16(make_rsrc(this->base + stage, room), off < room ? off : 0x80000000u, slice + (r0 + 8 * w) * 512);
+  }
+};
+
 // What runs the ring loop: bf16 and f16 operands (fp8 weights are widened to bf16 before the GEMM).
 __host__ __device__ constexpr bool ring5_ok(int dt) { return dt == OCTO_BF16 || dt == OCTO_F16; }
 

@@ -515,11 +515,13 @@ __device__ __forceinline__ void store8_tile(const Operand &A, const Operand &B, 
   f32x4 acc[8][4];
   if constexpr (KM == KM_A)
     mainloop_ring5<DT, OpColsN<8, 128>, OpRowsN<8, 64>, false, true>(A, B, m0, n0, K_eff, smem, acc);
+  else if constexpr (KM == KM_EDGE)
+    mainloop_ring5<DT, OpColsEdge<8, 128>, OpRowsN<8, 64>, false, true>(A, B, m0, n0, K_eff, smem, acc);
   else if constexpr (KM == KM_B)
     mainloop_ring5<DT, OpRowsN<8, 128>, OpColsN<8, 64>, true, true>(A, B, m0, n0, K_eff, smem, acc);
   else
     mainloop_ring5<DT, OpRowsN<8, 128>, OpRowsN<8, 64>, true, true>(A, B, m0, n0, K_eff, smem, acc);
-  if (KM != KM_A && part) {
+  if (KM != KM_A && KM != KM_EDGE && part) {
     store_split<L>(acc, part);
     return;
   }
@@ -575,7 +577,7 @@ __global__ __launch_bounds__(2 * NTHREADS, 1) __attribute__((amdgpu_waves_per_eu
   static_assert(ring5_ok(DT), "16-bit operands");
   __shared__ __attribute__((aligned(16))) char smem_[SMEM_RING5];
   lds_char *smem = (lds_char *)smem_;
-  if constexpr (KM != KM_A) {
+  if constexpr (KM != KM_A && KM != KM_EDGE) {
     gradh8_block<DT, OT, KM>(A, B, s, e, blockIdx.x, smem);
   } else {
     int mt, nt;
@@ -592,7 +594,8 @@ __global__ __launch_bounds__(2 * NTHREADS, 1) __attribute__((amdgpu_waves_per_eu
 // grad_h tiles, K = V long, are dispatched first; grad_W's, K = the pass's rows, fill the CUs its grid leaves idle
 // and the rest of its last round (a pass of 6,656 rows at d 2560 has 260 grad_h tiles: alone, a second round for 4
 // of them). KMH: grad_h reads W K-major as stored (KM_B) or a staged W^T (KM_NONE); grad_W reads dz K-major.
-template <int DT, int KMH>
+// KMW: grad_W's dz may end with its last row (KM_EDGE).
+template <int DT, int KMH, int KMW>
 __global__ __launch_bounds__(2 * NTHREADS, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_grads8_kernel(Operand Ah, Operand Bh, GemmShape sh, StoreArgs eh, Operand Aw, Operand Bw, GemmShape sw, StoreArgs ew, unsigned nh) {
   static_assert(ring5_ok(DT), "16-bit operands");
   __shared__ __attribute__((aligned(16))) char smem_[SMEM_RING5];
@@ -608,7 +611,7 @@ __global__ __launch_bounds__(2 * NTHREADS, 1) __attribute__((amdgpu_waves_per_eu
     if (!tile_at(sw, (int)(c & 7), (int64_t)(c >> 3), mtiles, ntiles, mt, nt)) return;
     const int which = pass_store(ew);
     if (which == 0) return;
-    store8_tile<DT, -1, KM_A>(Aw, Bw, sw, ew, mt, nt, which, smem);
+    store8_tile<DT, -1, KMW>(Aw, Bw, sw, ew, mt, nt, which, smem);
   }
 }
 
@@ -794,15 +797,19 @@ static int go_store(const Operand &A, const Operand &B, const GemmShape &s, cons
 
 template <int DT>
 static int go_grads(const Operand &Ah, const Operand &Bh, const GemmShape &sh, const StoreArgs &eh, bool wh_kmajor,
-                    const Operand &Aw, const Operand &Bw, const GemmShape &sw, const StoreArgs &ew, hipStream_t st) {
+                    const Operand &Aw, const Operand &Bw, const GemmShape &sw, const StoreArgs &ew, hipStream_t st,
+                    int aw_kmajor) {
   const int64_t nh = split_grid(sh, eh), nw = tile_grid(sw.mtiles, sw.ntiles);
   if (nh + nw > 0x7fffffffLL) return octo_fail(OCTO_EINVAL, "gemm_grads: %lld tiles", (long long)(nh + nw));
   const dim3 grid((unsigned)(nh + nw));
-  if (wh_kmajor)
-    hipLaunchKernelGGL((gemm_grads8_kernel<DT, KM_B>), grid, dim3(2 * NTHREADS), 0, st, Ah, Bh, sh, eh, Aw, Bw, sw, ew,
+  if (aw_kmajor == KM_EDGE)
+    hipLaunchKernelGGL((gemm_grads8_kernel<DT, KM_B, KM_EDGE>), grid, dim3(2 * NTHREADS), 0, st, Ah, Bh, sh, eh, Aw, Bw,
+                       sw, ew, (unsigned)nh);
+  else if (wh_kmajor)
+    hipLaunchKernelGGL((gemm_grads8_kernel<DT, KM_B, KM_A>), grid, dim3(2 * NTHREADS), 0, st, Ah, Bh, sh, eh, Aw, Bw, sw, ew,
                        (unsigned)nh);
   else
-    hipLaunchKernelGGL((gemm_grads8_kernel<DT, KM_NONE>), grid, dim3(2 * NTHREADS), 0, st, Ah, Bh, sh, eh, Aw, Bw, sw,
+    hipLaunchKernelGGL((gemm_grads8_kernel<DT, KM_NONE, KM_A>), grid, dim3(2 * NTHREADS), 0, st, Ah, Bh, sh, eh, Aw, Bw, sw,
                        ew, (unsigned)nh);
   OCTO_CHECK_LAUNCH("gemm_grads");
   return OCTO_OK;
@@ -814,19 +821,27 @@ static bool kmajor_layout_ok(const Operand &X) {
   return !X.map && !(X.ld & 15) && X.ld >= 512 && X.ld <= 0xffffffffLL / 64 && (uintptr_t)X.base % 16 == 0;
 }
 
+// KM_EDGE: a stage and a tile's columns within 32-bit offsets, edges at whole chunks.
+static bool edge_layout_ok(const Operand &X) {
+  return kmajor_layout_ok(X) && X.rows > 0 && X.extent > 0 && X.extent % 8 == 0 && X.ld <= 0x7fffffffLL / 64 - 1024 &&
+         (int64_t)X.extent * 2 <= X.ld;
+}
+
 int launch_gemm_grads(int dt, const Operand &Ah, const Operand &Bh, const GemmShape &sh, const StoreArgs &eh,
                       bool wh_kmajor, const Operand &Aw, const Operand &Bw, const GemmShape &sw, const StoreArgs &ew,
-                      hipStream_t st) {
+                      hipStream_t st, int aw_kmajor) {
   if (!eh.C || !ew.C || !Ah.base || !Bh.base || !Aw.base || !Bw.base)
     return octo_fail(OCTO_EINVAL, "gemm_grads: null operand or output");
   if (ew.split) return octo_fail(OCTO_EUNSUPPORTED, "gemm_grads: grad_W is not split");
   if (wh_kmajor && !kmajor_layout_ok(Bh)) return octo_fail(OCTO_EINVAL, "gemm_grads: K-major W layout");
   if (!kmajor_layout_ok(Aw)) return octo_fail(OCTO_EINVAL, "gemm_grads: K-major dz layout");
+  if (aw_kmajor == KM_EDGE && !(wh_kmajor && edge_layout_ok(Aw)))
+    return octo_fail(OCTO_EUNSUPPORTED, "gemm_grads: dz without room behind it");
   for (int t : {eh.dtype, ew.dtype})
     if (t != OCTO_BF16 && t != OCTO_F16 && t != OCTO_F32) return octo_fail(OCTO_EUNSUPPORTED, "gemm_grads: output dtype %d", t);
   switch (dt) {
-    case OCTO_BF16: return go_grads<OCTO_BF16>(Ah, Bh, sh, eh, wh_kmajor, Aw, Bw, sw, ew, st);
-    case OCTO_F16: return go_grads<OCTO_F16>(Ah, Bh, sh, eh, wh_kmajor, Aw, Bw, sw, ew, st);
+    case OCTO_BF16: return go_grads<OCTO_BF16>(Ah, Bh, sh, eh, wh_kmajor, Aw, Bw, sw, ew, st, aw_kmajor);
+    case OCTO_F16: return go_grads<OCTO_F16>(Ah, Bh, sh, eh, wh_kmajor, Aw, Bw, sw, ew, st, aw_kmajor);
   }
   return octo_fail(OCTO_EUNSUPPORTED, "gemm_grads: dtype %d", dt);
 }
@@ -835,8 +850,16 @@ int launch_gemm_store(int dt, const Operand &A, const Operand &B, const GemmShap
                       hipStream_t st, int kmajor) {
   if (!e.C || !A.base || !B.base) return octo_fail(OCTO_EINVAL, "gemm_store: null operand or output");
   if (dt == OCTO_F32) return launch_gemm_store_f32(A, B, s, e, st, kmajor);
-  if (e.split && (kmajor == KM_A || e.pass_count))
+  if (e.split && (kmajor == KM_A || kmajor == KM_EDGE || e.pass_count))
     return octo_fail(OCTO_EUNSUPPORTED, "gemm_store: split K of this product");
+  if (kmajor == KM_EDGE) {
+    if (!edge_layout_ok(A)) return octo_fail(OCTO_EINVAL, "gemm_store: K-major operand layout");
+    switch (dt) {
+      case OCTO_BF16: return go_store<OCTO_BF16, KM_EDGE>(A, B, s, e, st);
+      case OCTO_F16: return go_store<OCTO_F16, KM_EDGE>(A, B, s, e, st);
+    }
+    return octo_fail(OCTO_EUNSUPPORTED, "gemm_store: K-major operand of dtype %d", dt);
+  }
   if (kmajor != KM_NONE) {
     if (!kmajor_layout_ok(kmajor == KM_A ? A : B)) return octo_fail(OCTO_EINVAL, "gemm_store: K-major operand layout");
     switch (dt) {

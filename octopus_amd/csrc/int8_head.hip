@@ -285,14 +285,14 @@ static GemmShape shape8(int64_t M, int64_t N, int64_t K, int tile = TM) {
 }
 
 // Workspace of the gradients: the widened weight [V, d] (K-major for dx) and the partial tiles of its split; the
-// transposed rows [d, n]; g where its rows cannot be read as they are. Sizes padded as the K-major loads read.
+// transposed rows [d, n]; g where its rows cannot be read as they are (g_as_is). Sizes padded as the K-major loads read.
 struct Grads8Layout {
   int64_t Vr, dp, np, Vp;  // rows and columns of the copies
   size_t wide, xt, g, split, total;
   int64_t split_items;
 };
 
-static Grads8Layout grads8_layout(int64_t n, int d, int V, int dtype, bool need_rows, bool need_w) {
+static Grads8Layout grads8_layout(int64_t n, int d, int V, int dtype, bool need_rows, bool need_w, bool as_is) {
   const int esz = float_bytes(dtype);
   Grads8Layout L;
   L.Vr = round_up(V, 64);
@@ -310,17 +310,22 @@ static Grads8Layout grads8_layout(int64_t n, int d, int V, int dtype, bool need_
     const int64_t nt = cdiv(d, dtype == OCTO_F32 ? 128 : TN), nk = cdiv(V, 64);
     const int64_t mt = cdiv(n, TM);
     if (mt * nt < octo_tiles::kSplitItemsMax) {
-      const int S = octo_tiles::k_splits((int)(mt * nt), (int)nk, !need_w || dtype == OCTO_F32,
-                                         octo_tiles::kSplitItemsMax);
+      const int S = octo_tiles::k_splits((int)(mt * nt), (int)nk, true, octo_tiles::kSplitItemsMax);
       if (S > 1) L.split_items = mt * nt * S;
     }
   }
   L.wide = take(need_rows ? (size_t)L.Vr * L.dp * esz : 0);
   L.xt = take(need_w ? (size_t)d * L.np * esz : 0);
-  L.g = take((size_t)L.np * L.Vp * esz);
+  L.g = take(as_is ? 0 : (size_t)L.np * L.Vp * esz);
   L.split = take((size_t)L.split_items * TM * (dtype == OCTO_F32 ? 128 : TN) * 4);
   L.total = at;
   return L;
+}
+
+// Whether the products can read g where it lies: 16-bit values in whole 16-byte chunks, a tile's rows and a stage's within
+// 32-bit offsets.
+static bool g_as_is(const void *g, int64_t ldg, int dtype, int V) {
+  return dtype != OCTO_F32 && V % 8 == 0 && V >= TM && ldg % 8 == 0 && ldg <= kMaxV8 && (uintptr_t)g % 16 == 0;
 }
 
 static int head8_checks(const char *what, int64_t n, int d, int V, int64_t ldxq, int64_t ldw) {
@@ -384,12 +389,13 @@ int octo_head_logits_i8(const void *rows, int64_t ldx, int x_dtype, const int8_t
   return OCTO_OK;
 }
 
-int octo_head_grads_i8_workspace_bytes(int64_t n, int d, int V, int dtype, int need_rows, int need_w, size_t *bytes) {
+int octo_head_grads_i8_workspace_bytes(const void *g, int64_t ldg, int dtype, int64_t n, int d, int V, int need_rows,
+                                       int need_w, size_t *bytes) {
   OCTO_CHECK_ARG(bytes != nullptr, "head_grads_i8_workspace_bytes: null pointer");
   const int rc = head8_checks("head_grads_i8", n, d, V, round_up(d < 1 ? 1 : d, 16), round_up(d < 1 ? 1 : d, 16));
   if (rc) return rc;
   if (!is_float(dtype)) return octo_fail(OCTO_EUNSUPPORTED, "head_grads_i8: dtype %d", dtype);
-  *bytes = grads8_layout(n, d, V, dtype, need_rows != 0, need_w != 0).total;
+  *bytes = grads8_layout(n, d, V, dtype, need_rows != 0, need_w != 0, g_as_is(g, ldg, dtype, V)).total;
   return OCTO_OK;
 }
 
@@ -410,48 +416,68 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
                      (uintptr_t)grad_rows % float_bytes(gr_dtype) == 0 &&
                      (uintptr_t)grad_w % float_bytes(gw_dtype) == 0 && (uintptr_t)ws % 256 == 0,
                  "head_grads_i8: misaligned pointer");
-  const Grads8Layout L = grads8_layout(n, d, V, g_dtype, grad_rows != nullptr, grad_w != nullptr);
+  const bool as_is = g_as_is(g, ldg, g_dtype, V);
+  const Grads8Layout L = grads8_layout(n, d, V, g_dtype, grad_rows != nullptr, grad_w != nullptr, as_is);
   if (!ws || ws_bytes < L.total)
     return octo_fail(OCTO_EWORKSPACE, "head_grads_i8: workspace %zu < %zu bytes", ws ? ws_bytes : (size_t)0, L.total);
   hipStream_t st = (hipStream_t)stream;
   char *wsb = (char *)ws;
   const int esz = float_bytes(g_dtype);
-
-  rc = launch_stage_rows(g, ldg, g_dtype, n, V, wsb + L.g, L.Vp, L.np, (int)L.Vp, st);
+  Prepare8 p{};
+  p.wq = wq;
+  p.ldw = ldw;
+  p.ws = w_scale;
+  p.wide = grad_rows ? wsb + L.wide : nullptr;
+  p.Vr = L.Vr;
+  p.dp = (int)L.dp;
+  p.xq = xq;
+  p.ldxq = ldxq;
+  p.xs = x_scale;
+  p.xt = grad_w ? wsb + L.xt : nullptr;
+  p.ldt = L.np;
+  p.g = g;
+  p.ldg = ldg;
+  p.gs = as_is ? nullptr : wsb + L.g;
+  p.np = L.np;
+  p.Vp = L.Vp;
+  p.n = n;
+  p.d = d;
+  p.V = V;
+  rc = launch_prepare8(p, g_dtype, st);
   if (rc) return rc;
-  const char *gs = wsb + L.g;
-  const int64_t lds = L.Vp * esz;
+
+  const char *gs = as_is ? (const char *)g : wsb + L.g;
+  const int64_t lds = (as_is ? ldg : L.Vp) * esz;
   StoreArgs oh, ow;
   const Operand Ah = operand8(gs, lds, n), Bh = operand8(wsb + L.wide, L.dp * esz, d);
-  const GemmShape sh = shape8(n, d, V);
+  const GemmShape sh = shape8(n, d, V), sw = shape8(V, d, n);
+  Operand Aw = operand8(gs, lds, as_is ? n : V);
+  const Operand Bw = operand8(wsb + L.xt, L.np * esz, d);
+  const int kma = as_is ? KM_EDGE : KM_A;
+  if (as_is) Aw.extent = (uint32_t)V;
   if (grad_rows) {
-    rc = launch_widen_rows(wq, ldw, w_scale, V, d, 0, wsb + L.wide, L.dp, g_dtype, L.Vr, (int)L.dp, st);
-    if (rc) return rc;
     oh.C = grad_rows;
     oh.ldc = ld_gr;
     oh.dtype = gr_dtype;
     if (L.split_items) {
       oh.split = (float *)(wsb + L.split);
       oh.split_cap = (int)L.split_items;
-      oh.split_alone = !grad_w || g_dtype == OCTO_F32;
+      oh.split_alone = 1;
     }
   }
-  const Operand Aw = operand8(gs, lds, V), Bw = operand8(wsb + L.xt, L.np * esz, d);
-  const GemmShape sw = shape8(V, d, n);
   if (grad_w) {
-    rc = launch_widen_t(xq, ldxq, x_scale, n, d, wsb + L.xt, L.np, g_dtype, st);
-    if (rc) return rc;
     ow.C = grad_w;
     ow.ldc = ld_gw;
     ow.dtype = gw_dtype;
   }
-  if (grad_rows && grad_w && g_dtype != OCTO_F32) {
-    rc = launch_gemm_grads(g_dtype, Ah, Bh, sh, oh, true, Aw, Bw, sw, ow, st);
-  } else {
-    if (grad_rows) rc = launch_gemm_store(g_dtype, Ah, Bh, sh, oh, st, KM_B);
-    if (!rc && grad_w) rc = launch_gemm_store(g_dtype, Aw, Bw, sw, ow, st, KM_A);
-  }
+  // Both in one launch, dx's runs as long as if it had the card to itself: dW's short tiles follow them on every CU. Two
+  // launches take 20 us more up to 700 rows of d 2560, V 151,936 and as long from 1,024 on; runs cut for sharing the card
+  // (fewer, longer ones) 949 us for 300 rows against 835.
+  const bool both = grad_rows && grad_w && g_dtype != OCTO_F32;
+  if (both) rc = launch_gemm_grads(g_dtype, Ah, Bh, sh, oh, true, Aw, Bw, sw, ow, st, kma);
+  else if (grad_rows) rc = launch_gemm_store(g_dtype, Ah, Bh, sh, oh, st, KM_B);
   if (!rc && grad_rows) rc = launch_split_sum(sh, oh, g_dtype == OCTO_F32, st);
+  if (!rc && grad_w && !both) rc = launch_gemm_store(g_dtype, Aw, Bw, sw, ow, st, kma);
   return rc;
 }
 

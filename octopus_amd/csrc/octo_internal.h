@@ -163,7 +163,9 @@ int launch_gemm_stats(int dt, bool a_fp8, bool tanh, const Operand &A, const Ope
 int launch_gemm_dz(int dt, bool a_fp8, bool tanh, const Operand &A, const Operand &B, const GemmShape &s,
                    const DzArgs &e, hipStream_t st);
 // kmajor: which operand, if any, is a plain K-major matrix (element (k, m) at base + k ld + 2 m; 16-bit types)
-enum { KM_NONE = 0, KM_A = 1, KM_B = 2 };
+// KM_EDGE: KM_A of a matrix without room behind it: rows from A.rows on and columns from A.extent on read as zeros (whole
+// 16-byte chunks; 16-bit types)
+enum { KM_NONE = 0, KM_A = 1, KM_B = 2, KM_EDGE = 3 };
 int launch_gemm_store(int dt, const Operand &A, const Operand &B, const GemmShape &s, const StoreArgs &e,
                       hipStream_t st, int kmajor = KM_NONE);
 // C of a split-K product from its partial tiles (StoreArgs::split), with the shape and store its GEMM had; f32: of fp32
@@ -181,7 +183,7 @@ int launch_gemm_store_f32(const Operand &A, const Operand &B, const GemmShape &s
 // K-major, Bw = h^T) of one row pass in one launch, each with its own shape and store (16-bit operands).
 int launch_gemm_grads(int dt, const Operand &Ah, const Operand &Bh, const GemmShape &sh, const StoreArgs &eh,
                       bool wh_kmajor, const Operand &Aw, const Operand &Bw, const GemmShape &sw, const StoreArgs &ew,
-                      hipStream_t st);
+                      hipStream_t st, int aw_kmajor = KM_A);
 
 // ---- small kernels (head_aux.hip) ---------------------------------------------------------------
 struct MergeArgs {
@@ -429,15 +431,27 @@ int launch_transpose(const void *src, int64_t ld_src, int src_dtype, const float
                      int64_t rows_pad, int64_t cols, void *dst, int64_t ld_dst, int dst_dtype, hipStream_t st);
 
 // ---- rows of 8-bit integers (rows8.hip) ------------------------------------------------------------
-// out[r, c] = q[r, c] scale (of row r's group of c; group 0: of the row), rounded once to dtype, for r < rows, c < d;
-// zeros for the other r < rows_pad, c < cols_pad.
-int launch_widen_rows(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int d, int group, void *out,
-                      int64_t ldo, int dtype, int64_t rows_pad, int cols_pad, hipStream_t st);
-// The transpose of it: out[c, r] = q[r, c] scale[r] for c < d, zeros for rows <= r < ldo (a multiple of 64).
-int launch_widen_t(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int d, void *out, int64_t ldo,
-                   int dtype, hipStream_t st);
-// A copy of g [n, V] with rows of ldo elements (whole 16 bytes), zeros behind it up to rows_pad and cols_pad.
-int launch_stage_rows(const void *g, int64_t ldg, int dtype, int64_t n, int V, void *out, int64_t ldo, int64_t rows_pad,
-                      int cols_pad, hipStream_t st);
+// What the gradients of the 8-bit head read, in g's type: each copy that is not NULL.
+struct Prepare8 {
+  const int8_t *wq;  // [V, ldw]
+  int64_t ldw;
+  const float *ws;
+  void *wide;        // [Vr, dp] = wq ws, zeros past V
+  int64_t Vr;
+  int dp;
+  const int8_t *xq;  // [n, ldxq]
+  int64_t ldxq;
+  const float *xs;
+  void *xt;          // [d, ldt] = (xq xs)^T, zeros past n; ldt a multiple of 64
+  int64_t ldt;
+  const void *g;     // [n, ldg], V columns
+  int64_t ldg;
+  void *gs;          // [np, Vp] = g, zeros behind it; Vp whole 16-byte chunks
+  int64_t np, Vp;
+  int64_t n;
+  int d, V;
+  unsigned wide_blocks, t_blocks, g_parts;  // set by the launch
+};
+int launch_prepare8(Prepare8 a, int dtype, hipStream_t st);
 
 }  // namespace octo

@@ -1,5 +1,5 @@
 // Rows held as 8-bit integers with fp32 scales (octo_quantise_i8_rows, octo_widen_i8_rows), and the copies that the
-// gradients of the 8-bit head multiply with (launch_widen_t, launch_stage_rows).
+// gradients of the 8-bit head multiply with (launch_prepare8).
 //
 //   a = max |x| of a group of a row's values (the whole row, or 32 to 256 of them), scale = a times 1/127, both in fp32,
 //   q = the exact quotient x / scale to the nearest integer, ties to even;   x^ = q scale, rounded once
@@ -52,62 +52,67 @@ __device__ __forceinline__ void unpack_i8(const i32x2 v, float s, float (&x)[8])
   for (int e = 0; e < 8; ++e) x[e] = (float)(int8_t)((uint32_t)v[e >> 2] >> (8 * (e & 3))) * s;
 }
 
-// out[r, c] = q scale for r < rows, c < d; zeros for the other r < rows_pad and c < cols_pad. 8 columns a thread.
+// Row r of out = q scale for the columns c < d, zeros up to cols_pad (and for all of a row past `rows`), by one wave, 4
+// chunks of 8 columns a lane in flight. gshift: log2 of the group, or -1. The bytes of q behind d are readable up to the
+// next multiple of 16.
 template <int DT>
-__global__ __launch_bounds__(256) void widen_i8_kernel(const int8_t *q, int64_t ldq, const float *scale, int64_t rows,
-                                                       int d, int group, typename Elem<DT>::T *out, int64_t ldo,
-                                                       int64_t rows_pad, int cols_pad) {
-  const int64_t chunks = (cols_pad + 7) >> 3, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t r = i / chunks;
-  const int c = (int)(i - r * chunks) * 8;
-  if (r >= rows_pad) return;
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (r < rows && c < d) {
-    const int groups = group ? (d + group - 1) / group : 1;
-    i32x2 v = {0, 0};
-    if (c + 8 <= d) {
-      v = *(const i32x2 *)(q + r * ldq + c);
-    } else {
-      for (int e = 0; c + e < d; ++e) v[e >> 2] |= (q[r * ldq + c + e] & 0xff) << (8 * (e & 3));
-    }
-    unpack_i8(v, scale[r * groups + (group ? c / group : 0)], x);
-  }
-  typename Elem<DT>::T *o = out + r * ldo + c;
-  if (c + 8 <= cols_pad) {
-    if constexpr (DT == OCTO_F32) {
+__device__ __forceinline__ void widen_row(const int8_t *q, const float *scale, bool there, int d, int gshift,
+                                          typename Elem<DT>::T *out, int cols_pad) {
+  const int lane = threadIdx.x & 63;
+  for (int c0 = 8 * lane; c0 < cols_pad; c0 += 512 * 4) {
+    i32x2 v[4];
+    float s[4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        *((i32x4_any4 *)o + h) = i32x4{__float_as_int(x[4 * h]), __float_as_int(x[4 * h + 1]),
-                                       __float_as_int(x[4 * h + 2]), __float_as_int(x[4 * h + 3])};
-    } else {
-      *(i32x4_any *)o = pack8(x, DT == OCTO_F16);
+    for (int u = 0; u < 4; ++u) {
+      const int c = c0 + 512 * u, at = there && c < d ? c : 0;
+      v[u] = there ? *(const i32x2 *)(q + at) : i32x2{0, 0};
+      s[u] = there && c < d ? scale[gshift < 0 ? 0 : at >> gshift] : 0.f;
     }
-  } else {
-    for (int e = 0; c + e < cols_pad; ++e) o[e] = from_f32<DT>(x[e]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int c = c0 + 512 * u;
+      float x[8];
+      unpack_i8(v[u], s[u], x);
+      if (c + 8 <= cols_pad) {
+        if constexpr (DT == OCTO_F32) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            ((i32x4_any4 *)(out + c))[h] = i32x4{__float_as_int(x[4 * h]), __float_as_int(x[4 * h + 1]),
+                                                 __float_as_int(x[4 * h + 2]), __float_as_int(x[4 * h + 3])};
+        } else {
+          *(i32x4_any *)(out + c) = pack8(x, DT == OCTO_F16);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < cols_pad) out[c + e] = from_f32<DT>(x[e]);
+      }
+    }
   }
 }
 
-// out[c, r] = q[r, c] scale[r] for c < d; zeros for rows <= r < rows_pad (a multiple of 64). One 64 x 64 tile a
-// workgroup, through the LDS.
 template <int DT>
-__global__ __launch_bounds__(256) void widen_t_kernel(const int8_t *q, int64_t ldq, const float *scale, int64_t rows,
-                                                      int d, typename Elem<DT>::T *out, int64_t ldo) {
+__global__ __launch_bounds__(256) void widen_i8_kernel(const int8_t *q, int64_t ldq, const float *scale, int64_t rows,
+                                                       int d, int gshift, int groups, typename Elem<DT>::T *out,
+                                                       int64_t ldo) {
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r < rows) widen_row<DT>(q + r * ldq, scale + r * groups, true, d, gshift, out + r * ldo, d);
+}
+
+// out[c, r] = q[r, c] scale[r] for c < d, r0 <= r < r0 + 64; zeros from `rows` on. A 64 x 64 tile through the LDS.
+template <int DT>
+__device__ __forceinline__ void widen_t_tile(const Prepare8 &a, int64_t r0, int c0, typename Elem<DT>::T (*tile)[64 + 16 / Elem<DT>::bytes]) {
   typedef typename Elem<DT>::T T;
-  constexpr int PAD = 16 / sizeof(T), PER = 16 / sizeof(T);
-  __shared__ __attribute__((aligned(16))) T tile[64][64 + PAD];
-  const int64_t r0 = (int64_t)blockIdx.x * 64;
-  const int c0 = blockIdx.y * 64, t = threadIdx.x;
+  constexpr int PER = 16 / sizeof(T);
+  const int t = threadIdx.x;
   {
     const int row = t & 63, c = (t >> 6) * 16;  // a wave's lanes: one 16-byte chunk of 64 rows
     const int64_t r = r0 + row;
     i32x4 v = {0, 0, 0, 0};
     float s = 0.f;
-    if (r < rows && c0 + c < d) {
-      const int8_t *p = q + r * ldq + c0 + c;
-      s = scale[r];
-      if (c0 + c + 16 <= d) v = *(const i32x4 *)p;
-      else
-        for (int e = 0; c0 + c + e < d; ++e) v[e >> 2] |= (p[e] & 0xff) << (8 * (e & 3));
+    if (r < a.n && c0 + c < a.d) {
+      s = a.xs[r];
+      v = *(const i32x4 *)(a.xq + r * a.ldxq + c0 + c);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -121,89 +126,87 @@ __global__ __launch_bounds__(256) void widen_t_kernel(const int8_t *q, int64_t l
 #pragma unroll
   for (int k = 0; k < 64 * 64 / PER / 256; ++k) {
     const int i = t + 256 * k, c = i / (64 / PER), r = (i % (64 / PER)) * PER;
-    if (c0 + c < d) *(i32x4 *)(out + (int64_t)(c0 + c) * ldo + r0 + r) = *(const i32x4 *)&tile[c][r];
+    if (c0 + c < a.d) *(i32x4 *)((T *)a.xt + (int64_t)(c0 + c) * a.ldt + r0 + r) = *(const i32x4 *)&tile[c][r];
   }
 }
 
-// A copy of g [n, V] whose rows start on 16 bytes, zeros behind it up to rows_pad and cols_pad (a multiple of 8).
+// 8,192 bytes of row r of the copy of g, zeros behind it.
 template <int DT>
-__global__ __launch_bounds__(256) void stage_rows_kernel(const typename Elem<DT>::T *g, int64_t ldg, int64_t n, int V,
-                                                         typename Elem<DT>::T *out, int64_t ldo, int cols_pad) {
-  constexpr int PER = 16 / Elem<DT>::bytes;
-  const int64_t r = blockIdx.y;
-  const int c = (blockIdx.x * 256 + threadIdx.x) * PER;
-  if (c >= cols_pad) return;
-  i32x4 v = {0, 0, 0, 0};
-  if (r < n && c < V) {
-    const typename Elem<DT>::T *p = g + r * ldg + c;
-    if (c + PER <= V) {
-      if constexpr (DT == OCTO_F32) v = *(const i32x4_any4 *)p;
-      else v = *(const i32x4_any *)p;
+__device__ __forceinline__ void stage_part(const Prepare8 &a, int64_t r, int part) {
+  typedef typename Elem<DT>::T T;
+  constexpr int PER = 16 / sizeof(T);
+  const T *g = (const T *)a.g + r * a.ldg;
+  i32x4 v[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int c = ((2 * part + u) * 256 + (int)threadIdx.x) * PER;
+    v[u] = i32x4{0, 0, 0, 0};
+    if (r >= a.n || c >= a.V) continue;
+    if (c + PER <= a.V) {
+      if constexpr (DT == OCTO_F32) v[u] = *(const i32x4_any4 *)(g + c);
+      else v[u] = *(const i32x4_any *)(g + c);
     } else {
-      typename Elem<DT>::T x[PER] = {};
-      for (int e = 0; c + e < V; ++e) x[e] = p[e];
-      v = __builtin_bit_cast(i32x4, x);
+      T x[PER] = {};
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        if (c + e < a.V) x[e] = g[c + e];
+      v[u] = __builtin_bit_cast(i32x4, x);
     }
   }
-  *(i32x4 *)(out + r * ldo + c) = v;
-}
-
-int launch_widen_rows(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int d, int group, void *out,
-                      int64_t ldo, int dtype, int64_t rows_pad, int cols_pad, hipStream_t st) {
-  const int64_t chunks = (cols_pad + 7) / 8;
-  const int64_t step = ((int64_t)1 << 31) / chunks;  // rows a launch: fewer than 2^32 threads
-  for (int64_t r0 = 0; r0 < rows_pad; r0 += step) {
-    const int64_t part = rows_pad - r0 < step ? rows_pad - r0 : step;
-    const int64_t have = rows - r0 < 0 ? 0 : (rows - r0 < part ? rows - r0 : part);
-    const int64_t groups = group ? cdiv(d, group) : 1;
-    const dim3 grid((unsigned)cdiv(part * chunks, 256));
-    const int8_t *qr = q + r0 * ldq;
-    const float *sr = scale + r0 * groups;
-    switch (dtype) {
-      case OCTO_BF16:
-        hipLaunchKernelGGL(widen_i8_kernel<OCTO_BF16>, grid, dim3(256), 0, st, qr, ldq, sr, have, d, group,
-                           (__bf16 *)out + r0 * ldo, ldo, part, cols_pad);
-        break;
-      case OCTO_F16:
-        hipLaunchKernelGGL(widen_i8_kernel<OCTO_F16>, grid, dim3(256), 0, st, qr, ldq, sr, have, d, group,
-                           (_Float16 *)out + r0 * ldo, ldo, part, cols_pad);
-        break;
-      default:
-        hipLaunchKernelGGL(widen_i8_kernel<OCTO_F32>, grid, dim3(256), 0, st, qr, ldq, sr, have, d, group,
-                           (float *)out + r0 * ldo, ldo, part, cols_pad);
-        break;
-    }
-    OCTO_CHECK_LAUNCH("widen_i8");
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int c = ((2 * part + u) * 256 + (int)threadIdx.x) * PER;
+    if (c < a.Vp) *(i32x4 *)((T *)a.gs + r * a.Vp + c) = v[u];
   }
-  return OCTO_OK;
 }
 
-int launch_widen_t(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int d, void *out, int64_t ldo,
-                   int dtype, hipStream_t st) {
-  const dim3 grid((unsigned)(ldo / 64), (unsigned)cdiv(d, 64));
+// The copies that the gradients' products read, in one launch: blocks of 4 weight rows, of 64 x 64 tiles of the
+// transposed rows, of parts of g's rows.
+template <int DT>
+__global__ __launch_bounds__(256) void prepare8_kernel(Prepare8 a) {
+  typedef typename Elem<DT>::T T;
+  __shared__ __attribute__((aligned(16))) T tile[64][64 + 16 / sizeof(T)];
+  unsigned b = blockIdx.x;
+  if (b < a.wide_blocks) {
+    const int64_t r = (int64_t)b * 4 + (threadIdx.x >> 6);  // Vr is a multiple of 64
+    widen_row<DT>(a.wq + r * a.ldw, a.ws + r, r < a.V, a.d, -1, (T *)a.wide + r * a.dp, a.dp);
+    return;
+  }
+  b -= a.wide_blocks;
+  if (b < a.t_blocks) {
+    const unsigned tiles = (unsigned)(a.ldt / 64);
+    widen_t_tile<DT>(a, (int64_t)(b % tiles) * 64, (int)(b / tiles) * 64, tile);
+    return;
+  }
+  b -= a.t_blocks;
+  stage_part<DT>(a, b / a.g_parts, (int)(b % a.g_parts));
+}
+
+int launch_prepare8(Prepare8 a, int dtype, hipStream_t st) {
+  const int64_t per = 512 * (16 / float_bytes(dtype));  // values of a part of g
+  const int64_t wide = a.wide ? a.Vr / 4 : 0, t = a.xt ? a.ldt / 64 * cdiv(a.d, 64) : 0;
+  a.g_parts = (unsigned)cdiv(a.Vp, per);
+  const int64_t staged = a.gs ? a.np * a.g_parts : 0, blocks = wide + t + staged;
+  if (blocks == 0) return OCTO_OK;
+  if (blocks >= (1 << 24)) return octo_fail(OCTO_EINVAL, "head_grads_i8: %lld blocks", (long long)blocks);
+  a.wide_blocks = (unsigned)wide;
+  a.t_blocks = (unsigned)t;
+  const dim3 grid((unsigned)blocks);
   switch (dtype) {
-    case OCTO_BF16: hipLaunchKernelGGL(widen_t_kernel<OCTO_BF16>, grid, dim3(256), 0, st, q, ldq, scale, rows, d, (__bf16 *)out, ldo); break;
-    case OCTO_F16: hipLaunchKernelGGL(widen_t_kernel<OCTO_F16>, grid, dim3(256), 0, st, q, ldq, scale, rows, d, (_Float16 *)out, ldo); break;
-    default: hipLaunchKernelGGL(widen_t_kernel<OCTO_F32>, grid, dim3(256), 0, st, q, ldq, scale, rows, d, (float *)out, ldo); break;
+    case OCTO_BF16: hipLaunchKernelGGL(prepare8_kernel<OCTO_BF16>, grid, dim3(256), 0, st, a); break;
+    case OCTO_F16: hipLaunchKernelGGL(prepare8_kernel<OCTO_F16>, grid, dim3(256), 0, st, a); break;
+    default: hipLaunchKernelGGL(prepare8_kernel<OCTO_F32>, grid, dim3(256), 0, st, a); break;
   }
-  OCTO_CHECK_LAUNCH("widen_t");
+  OCTO_CHECK_LAUNCH("prepare8");
   return OCTO_OK;
 }
 
-int launch_stage_rows(const void *g, int64_t ldg, int dtype, int64_t n, int V, void *out, int64_t ldo, int64_t rows_pad,
-                      int cols_pad, hipStream_t st) {
-  const int per = 16 / float_bytes(dtype);
-  for (int64_t r0 = 0; r0 < rows_pad; r0 += 65535) {  // a grid's second dimension
-    const int64_t part = rows_pad - r0 < 65535 ? rows_pad - r0 : 65535, have = n - r0 < 0 ? 0 : n - r0;
-    const dim3 grid((unsigned)cdiv(cols_pad, 256 * per), (unsigned)part);
-    switch (dtype) {
-      case OCTO_BF16: hipLaunchKernelGGL(stage_rows_kernel<OCTO_BF16>, grid, dim3(256), 0, st, (const __bf16 *)g + r0 * ldg, ldg, have, V, (__bf16 *)out + r0 * ldo, ldo, cols_pad); break;
-      case OCTO_F16: hipLaunchKernelGGL(stage_rows_kernel<OCTO_F16>, grid, dim3(256), 0, st, (const _Float16 *)g + r0 * ldg, ldg, have, V, (_Float16 *)out + r0 * ldo, ldo, cols_pad); break;
-      default: hipLaunchKernelGGL(stage_rows_kernel<OCTO_F32>, grid, dim3(256), 0, st, (const float *)g + r0 * ldg, ldg, have, V, (float *)out + r0 * ldo, ldo, cols_pad); break;
-    }
-    OCTO_CHECK_LAUNCH("stage_rows");
-  }
-  return OCTO_OK;
+template <int DT>
+static void go_widen(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int d, int group, void *out,
+                     int64_t ldo, hipStream_t st) {
+  const int gshift = group ? __builtin_ctz((unsigned)group) : -1, groups = group ? (int)cdiv(d, group) : 1;
+  hipLaunchKernelGGL(widen_i8_kernel<DT>, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, q, ldq, scale, rows, d, gshift,
+                     groups, (typename Elem<DT>::T *)out, ldo);
 }
 
 template <int DT>
@@ -271,7 +274,18 @@ int octo_widen_i8_rows(const int8_t *q, int64_t ldq, const float *scale, int64_t
   OCTO_CHECK_ARG(q && scale && out, "widen_i8: null pointer");
   OCTO_CHECK_ARG((uintptr_t)out % float_bytes(out_dtype) == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)scale % 4 == 0,
                  "widen_i8: misaligned pointer");
-  return launch_widen_rows(q, ldq, scale, rows, d, group, out, ldo, out_dtype, rows, d, (hipStream_t)stream);
+  const int64_t groups = group ? cdiv(d, group) : 1;
+  for (int64_t r0 = 0; r0 < rows; r0 += kLaunchRows) {
+    const int64_t n = rows - r0 < kLaunchRows ? rows - r0 : kLaunchRows;
+    char *o = (char *)out + r0 * ldo * float_bytes(out_dtype);
+    switch (out_dtype) {
+      case OCTO_BF16: go_widen<OCTO_BF16>(q + r0 * ldq, ldq, scale + r0 * groups, n, d, group, o, ldo, (hipStream_t)stream); break;
+      case OCTO_F16: go_widen<OCTO_F16>(q + r0 * ldq, ldq, scale + r0 * groups, n, d, group, o, ldo, (hipStream_t)stream); break;
+      default: go_widen<OCTO_F32>(q + r0 * ldq, ldq, scale + r0 * groups, n, d, group, o, ldo, (hipStream_t)stream); break;
+    }
+    OCTO_CHECK_LAUNCH("widen_i8");
+  }
+  return OCTO_OK;
 }
 
 }  // extern "C"

@@ -46,6 +46,8 @@ def _scale_shape(shape, group: int) -> tuple:
 
 def _rows_of(x: Tensor, what: str) -> Tensor:
     """[*, d] as [rows, d] that the kernels can read."""
+    if x.dim() == 2:
+        return _float_rows(x, what)
     if x.dim() < 1 or not x.shape[-1]:
         raise ValueError(f"octohead: {what} must be [*, d], got {tuple(x.shape)}")
     return _float_rows(x.reshape(-1, x.shape[-1]), what)
@@ -55,14 +57,17 @@ def _rows8(q: Tensor) -> Tensor:
     """q [*, d] int8 as [rows, d] with rows on 16-byte boundaries, readable up to the next; a copy where they are not."""
     if q.dtype != torch.int8 or q.dim() < 1 or not q.shape[-1]:
         raise ValueError(f"octohead: int8 rows [*, d] expected, got {q.dtype} {tuple(q.shape)}")
-    q = q.reshape(-1, q.shape[-1])
+    if q.dim() != 2:
+        q = q.reshape(-1, q.shape[-1])
     n, d = q.shape
-    ld = q.stride(0) if n > 1 else _ld8(d)
-    last = q.storage_offset() + max(n - 1, 0) * ld + _ld8(d)
-    if q.stride(1) == 1 and ld % 16 == 0 and _ld8(d) <= ld <= 262144 and q.data_ptr() % 16 == 0 \
-            and q.untyped_storage().nbytes() >= last:
+    whole = _ld8(d)
+    ld, one = q.stride()
+    if n < 2:
+        ld = whole
+    if one == 1 and ld % 16 == 0 and whole <= ld <= 262144 and q.data_ptr() % 16 == 0 and \
+            (ld == d or q.untyped_storage().nbytes() >= q.storage_offset() + max(n - 1, 0) * ld + whole):
         return q
-    out = torch.zeros(n, _ld8(d), dtype=torch.int8, device=q.device)[:, :d]
+    out = torch.zeros(n, whole, dtype=torch.int8, device=q.device)[:, :d]
     return out.copy_(q)
 
 
@@ -71,7 +76,7 @@ def _ldq(q: Tensor) -> int:
 
 
 def _scales(scale: Tensor, shape, what: str) -> Tensor:
-    if scale.dtype != torch.float32 or tuple(scale.shape) != tuple(shape):
+    if scale.dtype != torch.float32 or scale.shape != shape:
         raise ValueError(f"octohead: {what} of fp32 {tuple(shape)} expected, got {scale.dtype} {tuple(scale.shape)}")
     return scale.contiguous()
 
@@ -215,7 +220,7 @@ def _grads(g: Tensor, xq: Tensor, xs: Tensor, w8: Tensor, ws: Tensor, rows_dtype
     if n == 0 or not (need_rows or need_w):
         return gr, gw
     nbytes = ctypes.c_size_t(0)
-    _lib.call("octo_head_grads_i8_workspace_bytes", n, d, V, _DT[g.dtype], int(need_rows), int(need_w),
+    _lib.call("octo_head_grads_i8_workspace_bytes", _p(g), _ld(g), _DT[g.dtype], n, d, V, int(need_rows), int(need_w),
               ctypes.byref(nbytes))
     work = _workspace(nbytes.value, g)
     _call_on(dev, "octo_head_grads_i8", _p(g), _ld(g), _DT[g.dtype], _p(xq), _ldq(xq), _p(xs), _p(w8), _ldq(w8),

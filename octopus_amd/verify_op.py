@@ -92,18 +92,20 @@ def verify_drafts(logits: Tensor, drafts: Tensor, uniform: Optional[Tensor], tem
         raise ValueError(f"octohead: at most {_lib.DRAFTS_MAX} drafts a sequence, got {K}")
     if not temperature > 0 or not 0.0 < 1.0 / float(temperature) < 1e38:
         raise ValueError(f"octohead: temperature {temperature} must be positive and within fp32's range")
-    if tuple(drafts.shape) != (S, K):
+    if drafts.shape != (S, K):
         raise ValueError(f"octohead: drafts [{S}, {K}] expected, got {tuple(drafts.shape)}")
     if uniform is None and not greedy:
         raise ValueError("octohead: uniform numbers are needed unless greedy")
-    if uniform is not None and (tuple(uniform.shape) != (S, rows) or uniform.dtype != torch.float32):
+    if uniform is not None and (uniform.shape != (S, rows) or uniform.dtype != torch.float32):
         raise ValueError(f"octohead: uniform numbers [{S}, {rows}] in fp32 expected, got {uniform.dtype} "
                          f"{tuple(uniform.shape)}")
-    if draft_logits is not None and (tuple(draft_logits.shape) != (S, K, V) or draft_logits.dtype != logits.dtype):
+    if draft_logits is not None and (draft_logits.shape != (S, K, V) or draft_logits.dtype != logits.dtype):
         raise ValueError(f"octohead: draft logits [{S}, {K}, {V}] in {logits.dtype} expected, got "
                          f"{draft_logits.dtype} {tuple(draft_logits.shape)}")
-    if lengths is not None and tuple(lengths.shape) != (S,):
+    if lengths is not None and lengths.shape != (S,):
         raise ValueError(f"octohead: lengths [{S}] expected, got {tuple(lengths.shape)}")
-    args = (logits.detach(), drafts, None if uniform is None else uniform.detach(),
-            None if draft_logits is None else draft_logits.detach(), lengths, 1.0 / float(temperature), bool(greedy))
-    return _verify_op(*args) if torch.compiler.is_compiling() else _verify(*args)
+    inv_T = 1.0 / float(temperature)
+    if torch.compiler.is_compiling():
+        return _verify_op(logits.detach(), drafts, None if uniform is None else uniform.detach(),
+                          None if draft_logits is None else draft_logits.detach(), lengths, inv_T, bool(greedy))
+    return _verify(logits, drafts, uniform, draft_logits, lengths, inv_T, bool(greedy))

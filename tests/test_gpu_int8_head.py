@@ -136,6 +136,28 @@ def test_gradients_of_strided_and_broadcast_g(dtype):
         assert ((a.cpu().double() - gr).abs() <= bound_r).all() and ((b.cpu().double() - gw).abs() <= bound_w).all()
 
 
+@pytest.mark.parametrize("n", [1, 63, 64, 65, 130])
+def test_gradients_of_g_read_where_it_lies(n):
+    """16-bit g in whole chunks, its last row the end of its memory; the columns between its rows are no numbers."""
+    d, V = 80, 264
+    x, w = _inputs(n, d, V, torch.bfloat16)
+    wq, ws = int8_op.quantise_rows(w.to(DEV))
+    xd, wd = x.to(DEV).requires_grad_(True), w.to(DEV).requires_grad_(True)
+    g = (torch.randn(n, V, generator=torch.Generator().manual_seed(n)) / 8).to(torch.bfloat16)
+    gr, gw, bound_r, bound_w = _bound_grads(g, x, wq, ws, torch.bfloat16, torch.bfloat16)
+    for ld, off in ((V, 0), (V + 8, 0), (V + 40, 24)):
+        store = torch.full(((n - 1) * ld + V + off,), float("nan"), dtype=torch.bfloat16, device=DEV)
+        at = store[off:].as_strided((n, V), (ld, 1))
+        at.copy_(g)
+        for rows, weight in ((True, True), (False, True), (True, False)):
+            z = int8_op.int8_head(xd if rows else xd.detach(), wq, ws, weight=wd if weight else None)
+            got = list(torch.autograd.grad(z, [t for t, on in ((xd, rows), (wd, weight)) if on], at))
+            if rows:
+                assert ((got.pop(0).cpu().double() - gr).abs() <= bound_r).all()
+            if weight:
+                assert ((got[0].cpu().double() - gw).abs() <= bound_w).all()
+
+
 def test_gradients_of_other_types():
     """fp32 logits of bf16 rows and weights: gradients in the rows' and the weight's type."""
     x, w = _inputs(50, 64, 200, torch.bfloat16)

@@ -48,9 +48,16 @@ def test_head8_checks():
     _lib.call("octo_head_logits_i8", *{**ok, "n": 0}.values(), None)
     out = ctypes.c_size_t(0)
     for n, d, V in [(-1, 60, 100), (4, 0, 100), (4, 60, 0), (4, 131073, 100), (4, 60, (1 << 21) + 1)]:
-        _refused("octo_head_grads_i8_workspace_bytes", n, d, V, _lib.BF16, 1, 1, ctypes.byref(out))
-    _refused("octo_head_grads_i8_workspace_bytes", 4, 60, 100, _lib.BF16, 1, 1, None)
-    _lib.call("octo_head_grads_i8_workspace_bytes", 4, 60, 100, _lib.BF16, 1, 1, ctypes.byref(out))
+        _refused("octo_head_grads_i8_workspace_bytes", P, V, _lib.BF16, n, d, V, 1, 1, ctypes.byref(out))
+    _refused("octo_head_grads_i8_workspace_bytes", P, 100, _lib.BF16, 4, 60, 100, 1, 1, None)
+    # a gradient that is read where it lies needs no copy
+    size = lambda p, ld, dt, V: _lib.call("octo_head_grads_i8_workspace_bytes", p, ld, dt, 640, 64, V, 0, 1,  # noqa: E731
+                                          ctypes.byref(out)) or out.value
+    copy = 640 * 1024 * 2
+    assert size(P, 1000, _lib.BF16, 1000) + copy == size(P, 1001, _lib.BF16, 1000)
+    assert size(P, 1001, _lib.BF16, 1000) == size(ctypes.c_void_p(4098), 1000, _lib.BF16, 1000) \
+        == size(P, 1008, _lib.BF16, 999)
+    _lib.call("octo_head_grads_i8_workspace_bytes", P, 100, _lib.BF16, 4, 60, 100, 1, 1, ctypes.byref(out))
     ok = dict(g=P, ldg=100, gdt=_lib.BF16, xq=P, ldxq=64, xs=P, wq=P, ldw=64, ws=P, n=4, d=60, V=100, gr=P, ldr=60,
               rdt=_lib.BF16, gw=P, ldgw=60, wdt=_lib.BF16, work=P, nwork=out.value)
     for change in [dict(ldg=99), dict(ldr=59), dict(ldgw=59), dict(n=0), dict(n=-1), dict(d=0), dict(V=0), dict(g=None),
