@@ -15,7 +15,7 @@ namespace octo {
 constexpr int kMaxD8 = 131072;       // 127^2 d < 2^31
 constexpr int kMaxV8 = 1 << 21;      // a tile's 256 rows of g within 32-bit offsets
 constexpr int64_t kMaxN8 = 1 << 21;  // the same of the transposed rows
-constexpr int kGroup8 = 4;
+constexpr int kGroup8 = 8;  // M-tiles that an XCD walks the tokens with: 2,048 rows at d 2560, V 151,936 795 us in fours, 749 in eights
 constexpr int64_t kSmallRows = 128;
 
 typedef i32x4 i32x4_el __attribute__((aligned(2)));
