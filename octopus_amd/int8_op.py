@@ -260,43 +260,29 @@ def _(g, xq, x_scale, wq, w_scale, rows_dtype, w_dtype, need_rows, need_w):
 
 def _setup(ctx, inputs, output):
     rows, wq, w_scale, weight, _ = inputs
-    ctx.save_for_backward(output[1], output[2])
-    _hold(ctx, rows, weight, wq, w_scale, wq, w_scale)
+    ctx.save_for_backward(output[1], output[2], wq, w_scale)
+    ctx.like = (rows.shape, rows.dtype, None if weight is None else weight.dtype)
     ctx.set_materialize_grads(False)
 
 
-def _version(t: Tensor) -> Optional[int]:
-    return None if t.is_inference() else t._version
-
-
-def _hold(ctx, rows, weight, w8, ws, wq, w_scale) -> None:
-    # the weights by reference, not saved: an offload's pack hook never copies the [V, d] bytes to the host
-    ctx.weights, ctx.watched = (w8, ws), [(t, _version(t)) for t in (wq, w_scale)]
-    ctx.like = (rows.shape, rows.dtype, None if weight is None else weight.dtype)
-
-
-def _unchanged(ctx) -> None:
-    for t, version in ctx.watched:
-        if _version(t) != version:
-            raise RuntimeError("octohead: the 8-bit weights were changed in place between the logits and their "
-                               "backward")
-
-
 def _backward(ctx, g, *others):
+    """The registered op's own backward calls the registered gradients: a tracer runs it on tensors without data, and
+    with create_graph its result depends on g, whose derivative is refused and not left out."""
     if any(o is not None for o in others):
         raise RuntimeError("octohead: of this op's outputs only the logits are differentiable")
     need_rows, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[3]
     if g is None or not (need_rows or need_w):
         return (None,) * 5
-    _unchanged(ctx)
-    xq, xs = ctx.saved_tensors
     shape, dtype, w_dtype = ctx.like
-    call = head_grads_i8 if torch.is_grad_enabled() or torch.compiler.is_compiling() else _grads
-    gr, gw = call(g, xq, xs, *ctx.weights, dtype, w_dtype or dtype, need_rows, need_w)
+    gr, gw = head_grads_i8(g, *ctx.saved_tensors, dtype, w_dtype or dtype, need_rows, need_w)
     return gr.view(shape) if need_rows else None, None, None, gw if need_w else None, None
 
 
 torch.library.register_autograd("octohead::head_logits_i8", _backward, setup_context=_setup)
+
+
+def _version(t: Tensor) -> Optional[int]:
+    return None if t.is_inference() else t._version
 
 
 class _Head8(torch.autograd.Function):
@@ -307,12 +293,22 @@ class _Head8(torch.autograd.Function):
     def forward(ctx, rows, wq, w_scale, weight, out_dtype):
         z, xq, xs, w8, ws = _logits(rows, wq, w_scale, weight, out_dtype)
         ctx.save_for_backward(xq, xs)
-        _hold(ctx, rows, weight, w8, ws, wq, w_scale)
+        # the weights by reference, not saved: an offload's pack hook never copies the [V, d] bytes to the host
+        ctx.weights, ctx.watched = (w8, ws), [(t, _version(t)) for t in (wq, w_scale)]
+        ctx.like = (rows.shape, rows.dtype, None if weight is None else weight.dtype)
         return z
 
     @staticmethod
     def backward(ctx, g):
-        return _backward(ctx, g)
+        need_rows, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[3]
+        for t, version in ctx.watched:
+            if _version(t) != version:
+                raise RuntimeError("octohead: the 8-bit weights were changed in place between the logits and their "
+                                   "backward")
+        shape, dtype, w_dtype = ctx.like
+        call = head_grads_i8 if torch.is_grad_enabled() else _grads
+        gr, gw = call(g, *ctx.saved_tensors, *ctx.weights, dtype, w_dtype or dtype, need_rows, need_w)
+        return gr.view(shape) if need_rows else None, None, None, gw if need_w else None, None
 
 
 def int8_head(rows: Tensor, wq: Tensor, w_scale: Tensor, *, weight: Optional[Tensor] = None,
