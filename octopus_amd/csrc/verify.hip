@@ -15,10 +15,11 @@
 //   pick      a workgroup per sequence finds the part in which the running sum passes u_K sum r, and in it the token
 // Many take the exponentials of stats in 32 bits (64-bit ones are 20 instructions each, and stats is most of the work),
 // which leave each row's sum within 4e-6 (see fast_part). That decides a draft unless u q and p are closer than 2^-15;
-// then the row and its draft's are summed again in 64 bits there. Two launches more, decide and sums, stand between stats
-// and residual: a is found once a sequence, and row a of both models summed in 64 bits.
+// then the row and its draft's are summed again in 64 bits there. decide, sums and rest take residual's place: a is found
+// once a sequence, and one sweep over row a of both models finds in 64 bits their sums and those of r (part_sums).
 #include "octo_common.h"
 #include "row_values.h"
+#include "rows8.h"
 
 namespace octo {
 
@@ -75,7 +76,9 @@ struct VerifyArgs {
   int parts, part;  // parts of a row, values of each (a multiple of kVBlock)
   int turns;        // parts a wave takes (sums, residual)
   PartStat *stats;  // [S, 2 K + 1, parts]: target rows, then draft rows
-  double *sum_p, *sum_q, *sum_r;  // [S, parts]: of exp((z - m) / T) of row a, of its draft row's; of r
+  // [S, parts]: of e = exp((z - m) / T) of row a, of its draft row's; of both over the columns with r > 0 (sum_a NaN:
+  // not known yet). Few logits: sum_a holds the sums of r.
+  double *sum_p, *sum_q, *sum_a, *sum_b;
   struct Decision {
     RowStat p, q;
     int a, residual, x, pad;  // residual: 0 r = p, 1 r = p - q, 2 r = p without x
@@ -142,6 +145,26 @@ __device__ __forceinline__ void load_block(const typename Elem<DT>::T *row, int 
   } else {
 #pragma unroll
     for (int u = 0; u < 4; ++u) load_values<DT>(row, c + 512 * u + 8 * lane, c1, x[u]);
+  }
+}
+
+// The same as they lie, for sweeps over two rows: half the registers until each chunk's turn.
+template <int DT>
+__device__ __forceinline__ void load_raw_block(const typename Elem<DT>::T *row, int c, int c1, Raw8<DT> (&v)[4]) {
+  typedef typename Elem<DT>::T T;
+  const int lane = threadIdx.x & 63;
+  if (c + kVBlock <= c1) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = load_raw8<DT>(row + c + 512 * u + 8 * lane);
+  } else {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int at = c + 512 * u + 8 * lane;
+      T x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = at + e < c1 ? row[at + e] : (T)-INFINITY;
+      v[u] = __builtin_bit_cast(Raw8<DT>, x);
+    }
   }
 }
 
@@ -419,6 +442,59 @@ __global__ __launch_bounds__(kVDecide) void verify_decide_kernel(VerifyArgs a) {
   if (threadIdx.x == 0) a.dec[blockIdx.x] = d;
 }
 
+// With S_p and S_q the rows' sums, r > 0 where e_p > rho e_q, rho = S_p / S_q, and there r = e_p / S_p - e_q / S_q: one
+// sweep finds the sums of e_p and e_q over all columns and over those, for which it is enough to know rho within 2^-15
+// (the statistics give it within 8e-6), unless a column's e_p lies that close to rho e_q. A part with such a column (one
+// in fifty where the models differ) is left to the next launch.
+template <int DT, int MODE>
+__device__ __forceinline__ void part_sums(const VerifyArgs &a, const VerifyArgs::Decision &d, int64_t s, int k, int c0,
+                                          int c1) {
+  const int lane = threadIdx.x & 63;
+  const typename Elem<DT>::T *row = row_of<DT>(a.z, a.ls, a.lr, s, d.a);
+  const typename Elem<DT>::T *rowd = MODE == 1 ? row_of<DT>(a.zd, a.ls_d, a.lr_d, s, d.a) : row;
+  const double mp = d.p.m, mq = d.q.m, rho = MODE == 1 ? d.q.inv / d.p.inv : 0.0;
+  double P = 0.0, Q = 0.0, A = 0.0, B = 0.0;
+  bool near = false;
+  for (int c = c0; c < c1; c += kVBlock) {
+    Raw8<DT> xr[4], yr[4];
+    load_raw_block<DT>(row, c, c1, xr);
+    if (MODE == 1) load_raw_block<DT>(rowd, c, c1, yr);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float x[8], y[8];
+      values8<DT>(xr[u], x);
+      if (MODE == 1) values8<DT>(yr[u], y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double ep = exp2_64(((double)x[e] - mp) * a.c);
+        P += ep;
+        if (MODE == 1) {
+          const double eq = exp2_64(((double)y[e] - mq) * a.c), over = __builtin_fma(-rho, eq, ep);
+          Q += eq;
+          A += over > 0.0 ? ep : 0.0;
+          B += over > 0.0 ? eq : 0.0;
+          near |= fabs(over) < kVClose * ep;
+        } else if (MODE == 2) {
+          A += c + 512 * u + 8 * lane + e == d.x ? 0.0 : ep;
+        }
+      }
+    }
+  }
+  P = wave_sum64(P);
+  if (MODE) A = wave_sum64(A);
+  if (MODE == 1) {
+    Q = wave_sum64(Q);
+    B = wave_sum64(B);
+    if (__any(near)) A = __builtin_nan("");
+  }
+  if (lane == 0) {
+    a.sum_p[s * a.parts + k] = P;
+    if (MODE) a.sum_a[s * a.parts + k] = A;
+    if (MODE) a.sum_b[s * a.parts + k] = B;
+    if (MODE == 1) a.sum_q[s * a.parts + k] = Q;
+  }
+}
+
 template <int DT>
 __global__ __launch_bounds__(kVThreads) void verify_sums_kernel(VerifyArgs a) {
   const int64_t s = blockIdx.y;
@@ -428,22 +504,9 @@ __global__ __launch_bounds__(kVThreads) void verify_sums_kernel(VerifyArgs a) {
     const int k = __builtin_amdgcn_readfirstlane((blockIdx.x * kVWaves + (threadIdx.x >> 6)) * a.turns + t);
     if (k >= a.parts) return;
     const int c0 = k * a.part, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.part);
-    for (int which = 0; which < (d.residual == 1 ? 2 : 1); ++which) {
-      const typename Elem<DT>::T *row = which ? row_of<DT>(a.zd, a.ls_d, a.lr_d, s, d.a)
-                                              : row_of<DT>(a.z, a.ls, a.lr, s, d.a);
-      const double md = which ? d.q.m : d.p.m;
-      double S = 0.0;
-      for (int c = c0; c < c1; c += kVBlock) {
-        float x[4][8];
-        load_block<DT>(row, c, c1, x);
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) S += exp2_64(((double)x[u][e] - md) * a.c);
-      }
-      S = wave_sum64(S);
-      if ((threadIdx.x & 63) == 0) (which ? a.sum_q : a.sum_p)[s * a.parts + k] = S;
-    }
+    if (d.residual == 1) part_sums<DT, 1>(a, d, s, k, c0, c1);
+    else if (d.residual == 2) part_sums<DT, 2>(a, d, s, k, c0, c1);
+    else part_sums<DT, 0>(a, d, s, k, c0, c1);
   }
 }
 
@@ -454,40 +517,58 @@ __device__ __forceinline__ double part_mass(const VerifyArgs &a, const VerifyArg
   const int lane = threadIdx.x & 63;
   double S = 0.0;
   for (int c = c0; c < c1; c += kVBlock) {
-    float x[4][8], y[4][8];
-    load_block<DT>(row, c, c1, x);
-    if (MODE == 1) load_block<DT>(rowd, c, c1, y);
+    Raw8<DT> xr[4], yr[4];
+    load_raw_block<DT>(row, c, c1, xr);
+    if (MODE == 1) load_raw_block<DT>(rowd, c, c1, yr);
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < 4; ++u) {
+      float x[8], y[8];
+      values8<DT>(xr[u], x);
+      if (MODE == 1) values8<DT>(yr[u], y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        S += mass<MODE>(a, d, x[u][e], MODE == 1 ? y[u][e] : 0.f, c + 512 * u + 8 * lane + e);
+      for (int e = 0; e < 8; ++e) S += mass<MODE>(a, d, x[e], MODE == 1 ? y[e] : 0.f, c + 512 * u + 8 * lane + e);
+    }
   }
   return wave_sum64(S);
 }
 
-template <int DT, bool EXACT>
+template <int DT>
 __global__ __launch_bounds__(kVThreads) void verify_residual_kernel(VerifyArgs a) {
   const int64_t s = blockIdx.y;
-  const int lane = threadIdx.x & 63;
   VerifyArgs::Decision d;
-  if constexpr (EXACT) {
-    decide<DT, true, kVWaves>(a, s, blockIdx.x == 0, d);
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.dec[s] = d;
-  } else {
-    d = a.dec[s];
-  }
+  decide<DT, true, kVWaves>(a, s, blockIdx.x == 0, d);
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.dec[s] = d;
   if (d.residual == 0 || !(d.p.inv > 0.0)) return;
-  if constexpr (!EXACT) exact_rows(a, s, d);
   const typename Elem<DT>::T *row = row_of<DT>(a.z, a.ls, a.lr, s, d.a);
   const typename Elem<DT>::T *rowd = d.residual == 1 ? row_of<DT>(a.zd, a.ls_d, a.lr_d, s, d.a) : row;
-  for (int t = 0; t < a.turns; ++t) {
-    const int k = __builtin_amdgcn_readfirstlane((blockIdx.x * kVWaves + (threadIdx.x >> 6)) * a.turns + t);
-    if (k >= a.parts) return;
+  const int k = __builtin_amdgcn_readfirstlane(blockIdx.x * kVWaves + (threadIdx.x >> 6));
+  if (k >= a.parts) return;
+  const int c0 = k * a.part, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.part);
+  const double S = d.residual == 1 ? part_mass<DT, 1>(a, d, row, rowd, c0, c1) : part_mass<DT, 2>(a, d, row, rowd, c0, c1);
+  if ((threadIdx.x & 63) == 0) a.sum_a[s * a.parts + k] = S;
+}
+
+// The parts that verify_sums_kernel left: their sum of r, in the form of the others (sum_a / S_p - sum_b / S_q).
+template <int DT>
+__global__ __launch_bounds__(kVThreads) void verify_rest_kernel(VerifyArgs a) {
+  const int64_t s = blockIdx.y;
+  if (a.dec[s].residual != 1) return;
+  bool any = false;
+  const int k0 = __builtin_amdgcn_readfirstlane((blockIdx.x * kVWaves + (threadIdx.x >> 6)) * a.turns);
+  for (int k = k0; k < min(a.parts, k0 + a.turns); ++k) any |= a.sum_a[s * a.parts + k] != a.sum_a[s * a.parts + k];
+  if (!any) return;
+  VerifyArgs::Decision d = a.dec[s];
+  if (!(d.p.inv > 0.0)) return;
+  exact_rows(a, s, d);
+  for (int k = k0; k < min(a.parts, k0 + a.turns); ++k) {
+    if (a.sum_a[s * a.parts + k] == a.sum_a[s * a.parts + k]) continue;
     const int c0 = k * a.part, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.part);
-    const double S = d.residual == 1 ? part_mass<DT, 1>(a, d, row, rowd, c0, c1)
-                                     : part_mass<DT, 2>(a, d, row, rowd, c0, c1);
-    if (lane == 0) a.sum_r[s * a.parts + k] = S;
+    const double S = part_mass<DT, 1>(a, d, row_of<DT>(a.z, a.ls, a.lr, s, d.a),
+                                      row_of<DT>(a.zd, a.ls_d, a.lr_d, s, d.a), c0, c1);
+    if ((threadIdx.x & 63) == 0) {
+      a.sum_a[s * a.parts + k] = S / d.p.inv;
+      a.sum_b[s * a.parts + k] = 0.0;
+    }
   }
 }
 
@@ -596,7 +677,8 @@ __global__ __launch_bounds__(kVThreads) void verify_pick_kernel(VerifyArgs a) {
     for (int k = threadIdx.x; k < a.parts; k += kVThreads) {
       double x;
       if (res) {
-        x = a.sum_r[s * a.parts + k];
+        x = a.sum_a[s * a.parts + k];
+        if constexpr (!EXACT) x = fmax(x * d.p.inv - a.sum_b[s * a.parts + k] * d.q.inv, 0.0);
       } else if constexpr (EXACT) {
         const PartStat t = a.stats[(s * (2 * a.K + 1) + d.a) * a.parts + k];
         x = t.m == -INFINITY ? 0.0 : t.S * exp2_64(((double)t.m - (double)d.p.m) * a.c) * d.p.inv;
@@ -684,7 +766,7 @@ static VerifyLayout verify_layout(int64_t S, int K, int V) {
   L.parts = (int)cdiv(V, L.part);
   L.stats = 0;
   L.sums = (size_t)S * (2 * K + 1) * L.parts * sizeof(PartStat);
-  L.dec = L.sums + (size_t)round_up(3 * S * L.parts * 8, 16);
+  L.dec = L.sums + (size_t)(4 * S * L.parts * 8);
   L.total = L.dec + (size_t)S * sizeof(VerifyArgs::Decision);
   return L;
 }
@@ -700,8 +782,13 @@ template <int DT, bool EXACT> static int go_launches(const VerifyArgs &a, hipStr
     hipLaunchKernelGGL(verify_sums_kernel<DT>, taken, dim3(kVThreads), 0, st, a);
     OCTO_CHECK_LAUNCH("verify_sums");
   }
-  if (!a.greedy && (EXACT || a.K > 0)) {
-    hipLaunchKernelGGL((verify_residual_kernel<DT, EXACT>), taken, dim3(kVThreads), 0, st, a);
+  if (!a.greedy && !EXACT && a.zd) {
+    hipLaunchKernelGGL(verify_rest_kernel<DT>, taken, dim3(kVThreads), 0, st, a);
+    OCTO_CHECK_LAUNCH("verify_rest");
+  }
+  if (!a.greedy && EXACT) {
+    hipLaunchKernelGGL(verify_residual_kernel<DT>, dim3((unsigned)cdiv(a.parts, kVWaves), (unsigned)a.S),
+                       dim3(kVThreads), 0, st, a);
     OCTO_CHECK_LAUNCH("verify_residual");
   }
   hipLaunchKernelGGL((verify_pick_kernel<DT, EXACT>), dim3((unsigned)a.S), dim3(kVThreads), 0, st, a);
@@ -723,7 +810,8 @@ template <int DT> static int go_verify(const VerifyArgs &a, bool exact, hipStrea
     b.stats = a.stats + s0 * rows * a.parts;
     b.sum_p = a.sum_p + s0 * a.parts;
     b.sum_q = a.sum_q + s0 * a.parts;
-    b.sum_r = a.sum_r + s0 * a.parts;
+    b.sum_a = a.sum_a + s0 * a.parts;
+    b.sum_b = a.sum_b + s0 * a.parts;
     b.dec = a.dec + s0;
     b.tokens = a.tokens + s0 * (a.K + 1);
     b.accepted = a.accepted + s0;
@@ -794,7 +882,8 @@ int octo_verify_drafts(const void *logits, int64_t ld_seq, int64_t ld_row, const
   a.stats = (PartStat *)((char *)ws + L.stats);
   a.sum_p = (double *)((char *)ws + L.sums);
   a.sum_q = a.sum_p + S * L.parts;
-  a.sum_r = a.sum_q + S * L.parts;
+  a.sum_a = a.sum_q + S * L.parts;
+  a.sum_b = a.sum_a + S * L.parts;
   a.dec = (VerifyArgs::Decision *)((char *)ws + L.dec);
   a.tokens = tokens;
   a.accepted = accepted;

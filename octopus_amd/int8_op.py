@@ -153,15 +153,19 @@ class _Held:
         return widen_rows(self.q, self.scale, self.dtype, self.group).requires_grad_(True)
 
 
+def _holds(x) -> bool:
+    return isinstance(x, Tensor) and x.requires_grad and torch.is_grad_enabled() and x.is_cuda and \
+        x.dtype in _FLOATS and x.dim() > 0 and x.shape[-1] > 0 and not isinstance(x, torch.nn.Parameter)
+
+
 def checkpoint8(fn, *xs, group: int = 128):
     """fn(*xs), recomputed in the backward (torch.utils.checkpoint, not reentrant) from inputs that are held in 8 bits
     in between: those of bf16, f16 or fp32 on a HIP device that require a gradient. The forward sees them as they are,
     the recompute what their 8 bits stand for, so what fn saves for its gradients is off by the rounding (half of 1/127
-    of a group's largest value). Other arguments (masks, positions, None) are kept by reference."""
+    of a group's largest value). Other arguments (masks, positions, parameters, None) are kept by reference."""
     _groups(1, group)
     live = list(xs)
-    held = [_Held(x, group) if isinstance(x, Tensor) and x.requires_grad and x.is_cuda and x.dtype in _FLOATS
-            and torch.is_grad_enabled() and x.dim() and x.shape[-1] else None for x in xs]
+    held = [_Held(x, group) if _holds(x) else None for x in xs]
     kept = [None if h is not None else x for x, h in zip(xs, held)]
 
     def run():
@@ -318,7 +322,8 @@ def int8_head(rows: Tensor, wq: Tensor, w_scale: Tensor, *, weight: Optional[Ten
     and rounded once. The rows' gradient is that of the weights' 8-bit values. weight: the [V, d] parameter that wq was
     made of, which gets the gradient straight through the rounding; its values are not read, and wq is made again when
     it has changed. Between the two passes the rows are held in 8 bits, and wq and w_scale by reference (changed in
-    place, the backward raises). The gradients have no derivative of their own: one raises."""
+    place, the backward raises). wq and w_scale get no gradient. The gradients have no derivative of
+    their own: one raises."""
     out_dtype = out_dtype or rows.dtype
     if torch.compiler.is_compiling():
         return head_logits_i8(rows, wq, w_scale, weight, out_dtype)[0]

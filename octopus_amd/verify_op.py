@@ -77,7 +77,8 @@ def verify_drafts(logits: Tensor, drafts: Tensor, uniform: Optional[Tensor], tem
     logits [S, K + 1, V] (bf16, f16, fp32): the target's, row i at the position that draft i answers; drafts [S, K];
     uniform [S, K + 1] fp32 in [0, 1): one number a draft and the last for the draw. draft_logits [S, K, V] in the
     logits' type: the distributions that the drafts were sampled from, at the same temperature; None: drafts that were
-    not sampled (looked up, or the draft's best). lengths [S]: how many of the K drafts there are (None: all). greedy:
+    not sampled (looked up, or the draft's best). lengths [S]: how many of the K drafts there are (None: all;
+    clamped to [0, K]); what lies behind them is not read. greedy:
     a draft is accepted when it is its row's first largest logit, which is also the token behind them; uniform (may be
     None) and draft_logits are not read.
 

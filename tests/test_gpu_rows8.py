@@ -148,6 +148,17 @@ def test_checkpoint8_gradients(group):
         assert torch.equal(a, b)
 
 
+def test_checkpoint8_keeps_parameters():
+    """A parameter among the arguments is there anyway: its gradient is that of its own values."""
+    x = torch.randn(9, 64, device=DEV, requires_grad=True)
+    w = torch.nn.Parameter(torch.randn(64, 32, device=DEV))
+    y = int8_op.checkpoint8(lambda a, b: a @ b, x, w)
+    gx, gw = torch.autograd.grad(y.sum(), (x, w))
+    assert torch.equal(gx, torch.ones_like(y) @ w.detach().t())
+    q, s = int8_op.quantise_rows(x, 128)
+    assert torch.equal(gw, int8_op.widen_rows(q, s, x.dtype, 128).t() @ torch.ones_like(y))
+
+
 def test_checkpoint8_twice_and_under_no_grad():
     x = torch.randn(5, 64, device=DEV, requires_grad=True)
     w = torch.randn(64, 64, device=DEV, requires_grad=True)

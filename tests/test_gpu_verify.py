@@ -199,6 +199,20 @@ def test_many_drafts_on_the_border(sampled):
     assert torch.equal(acc, (~(up & apart)).long().cumprod(1).sum(1))
 
 
+@pytest.mark.parametrize("noise", [3e-2, 1e-3, 1e-5])
+def test_many_with_models_alike(noise):
+    """Draft and target all but equal, rejected by numbers near 1: what is left of p - q is little, and in much of the
+    vocabulary the two lie within 2^-15 of each other."""
+    S, K, V = 90, 2, 40000
+    z, _, x, u = _inputs(S, K, V, torch.float32, 6)
+    g = torch.Generator().manual_seed(7)
+    zd = z[:, :K] + noise * torch.randn(S, K, V, generator=g)
+    zd[:, :, V // 2:] = z[:, :K, V // 2:]     # and exactly equal in half of it
+    u[:, :K] = 1.0 - 2.0 ** -24
+    _, acc = _check_many(z, x, u, 1.0, zd)
+    assert (acc < K).any()
+
+
 def test_many_without_a_distribution():
     z, zd, x, u = _inputs(700, 1, 13000, torch.bfloat16, 8)
     z[0, 0], z[1, 0, 12999], z[2, 0, 0] = NINF, math.nan, math.inf
