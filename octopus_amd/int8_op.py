@@ -90,7 +90,7 @@ def _quantise(x: Tensor, group: int) -> tuple[Tensor, Tensor]:
     q = torch.empty(*x.shape[:-1], _ld8(d), dtype=torch.int8, device=dev)
     scale = torch.empty(_scale_shape(x.shape, group), dtype=torch.float32, device=dev)
     _call_on(dev, "octo_quantise_i8_rows", _p(rows), _ld(rows), _DT[rows.dtype], n, d, group, _p(q), _ld8(d), _p(scale))
-    return q[..., :d], scale
+    return q if d % 16 == 0 else q[..., :d], scale
 
 
 @torch.library.custom_op("octohead::quantise_rows", mutates_args=(), device_types="cuda")
@@ -109,8 +109,7 @@ def quantise_rows(x: Tensor, group: int = 0) -> tuple[Tensor, Tensor]:
     """(q int8 [*, d], scale fp32 [*] or, with a group, [*, ceil(d / group)]) of x [*, d] in bf16, f16 or fp32 (the
     module's format). Not differentiable."""
     _groups(1, group)
-    x = x.detach()
-    return _quantise_op(x, group) if torch.compiler.is_compiling() else _quantise(x, group)
+    return _quantise_op(x.detach(), group) if torch.compiler.is_compiling() else _quantise(x, group)
 
 
 def _widen(q: Tensor, scale: Tensor, dtype: torch.dtype, group: int) -> Tensor:
