@@ -363,9 +363,11 @@ int octo_head_logits_i8(const void *rows, int64_t ldx, int x_dtype, const int8_t
                         int z_dtype, void *stream);
 /* Its gradients for g = dL/dlogits [n, ldg], straight through the rounding (NULL skips one):
  *   grad_rows[r, k] = sum_v g[r, v] w_scale[v] wq[v, k];  grad_w[v, k] = sum_r g[r, v] x_scale[r] xq[r, k]
- * The products run in g's type (F32 as three bf16 parts), the 8-bit operand times its scale rounded once to it, summed
- * in fp32 and rounded once. ws: octo_head_grads_i8_workspace_bytes, 256-byte aligned; with room for a copy of g where
- * that is not of 16-bit values, rows of whole 16-byte chunks (V too) and 256 columns or more (g is not read there). */
+ * 16-bit g: the products run in its type, the 8-bit operand times its scale rounded once to it. F32 g (n, V <= 2^20): g
+ * times the scale in three bf16 parts (24 bits; a value that bf16 rounds to infinity is one), times the integers,
+ * exactly. Summed in fp32 and rounded once. ws: octo_head_grads_i8_workspace_bytes, 256-byte aligned; with room for a
+ * copy of g where that is not of 16-bit values, rows of whole 16-byte chunks (V too) and 256 columns or more (g is not
+ * read there), for its parts, 6 bytes a value and gradient, where it is F32. */
 int octo_head_grads_i8_workspace_bytes(const void *g, int64_t ldg, int g_dtype, int64_t n, int d, int V, int need_rows,
                                        int need_w, size_t *bytes);
 int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq, int64_t ldxq, const float *x_scale,

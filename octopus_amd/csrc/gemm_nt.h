@@ -286,6 +286,24 @@ struct OpColsEdge : OpColsN<NW, SUB> {
   }
 };
 
+// OpColsN of a K that runs through the matrix's op.rows rows (a multiple of 64) up to three times, from row 64
+// op.count_off of it on.
+template <int NW, int SUB>
+struct OpColsWrap : OpColsN<NW, SUB> {
+  typedef OpColsN<NW, SUB> Base;
+  int first, period;  // stages
+  __device__ __forceinline__ void init(const Operand &op, int64_t col0, int wsub, const typename Base::Rows &m) {
+    Base::init(op, col0, wsub, m);
+    first = __builtin_amdgcn_readfirstlane((int)op.count_off);
+    period = __builtin_amdgcn_readfirstlane((int)(op.rows / 64));
+  }
+  __device__ __forceinline__ void dma(int k, int q, uint32_t kbytes, lds_char *slice) const {
+    int at = k + first;
+    at -= at >= 2 * period ? 2 * period : (at >= period ? period : 0);
+    Base::dma(at, q, kbytes, slice);
+  }
+};
+
 // What runs the ring loop: bf16 and f16 operands (fp8 weights are widened to bf16 before the GEMM).
 __host__ __device__ constexpr bool ring5_ok(int dt) { return dt == OCTO_BF16 || dt == OCTO_F16; }
 

@@ -519,6 +519,8 @@ __device__ __forceinline__ void store8_tile(const Operand &A, const Operand &B, 
     mainloop_ring5<DT, OpColsEdge<8, 128>, OpRowsN<8, 64>, false, true>(A, B, m0, n0, K_eff, smem, acc);
   else if constexpr (KM == KM_B)
     mainloop_ring5<DT, OpRowsN<8, 128>, OpColsN<8, 64>, true, true>(A, B, m0, n0, K_eff, smem, acc);
+  else if constexpr (KM == KM_WRAP)
+    mainloop_ring5<DT, OpRowsN<8, 128>, OpColsWrap<8, 64>, true, true>(A, B, m0, n0, K_eff, smem, acc);
   else
     mainloop_ring5<DT, OpRowsN<8, 128>, OpRowsN<8, 64>, true, true>(A, B, m0, n0, K_eff, smem, acc);
   if (KM != KM_A && KM != KM_EDGE && part) {
@@ -564,7 +566,8 @@ __device__ __forceinline__ void gradh8_block(Operand A, Operand B, GemmShape s, 
     const int k0 = 64 * __builtin_amdgcn_readfirstlane(octo_tiles::split_stage(run, S, nk));
     const int k1 = 64 * __builtin_amdgcn_readfirstlane(octo_tiles::split_stage(run + 1, S, nk));
     A.base += (int64_t)k0 * 2;
-    B.base += KM == KM_B ? k0 * B.ld : (int64_t)k0 * 2;
+    if constexpr (KM == KM_WRAP) B.count_off = k0 / 64;
+    else B.base += KM == KM_B ? k0 * B.ld : (int64_t)k0 * 2;
     s.K = __builtin_amdgcn_readfirstlane(min(k1, (int)s.K) - k0);
   } else if (!tile_at(s, (int)(b & 7), (int64_t)(b >> 3), mtiles, ntiles, mt, nt)) {
     return;
@@ -852,6 +855,11 @@ int launch_gemm_store(int dt, const Operand &A, const Operand &B, const GemmShap
   if (dt == OCTO_F32) return launch_gemm_store_f32(A, B, s, e, st, kmajor);
   if (e.split && (kmajor == KM_A || kmajor == KM_EDGE || e.pass_count))
     return octo_fail(OCTO_EUNSUPPORTED, "gemm_store: split K of this product");
+  if (kmajor == KM_WRAP) {
+    if (!kmajor_layout_ok(B) || dt != OCTO_BF16 || B.rows % 64 || B.rows <= 0 || s.K > 3 * B.rows || B.count_off || B.count)
+      return octo_fail(OCTO_EINVAL, "gemm_store: wrapped operand layout");
+    return go_store<OCTO_BF16, KM_WRAP>(A, B, s, e, st);
+  }
   if (kmajor == KM_EDGE) {
     if (!edge_layout_ok(A)) return octo_fail(OCTO_EINVAL, "gemm_store: K-major operand layout");
     switch (dt) {

@@ -286,19 +286,27 @@ static GemmShape shape8(int64_t M, int64_t N, int64_t K, int tile = TM) {
 
 // Workspace of the gradients: the widened weight [V, d] (K-major for dx) and the partial tiles of its split; the
 // transposed rows [d, n]; g where its rows cannot be read as they are (g_as_is). Sizes padded as the K-major loads read.
+//
+// fp32 g is not multiplied in fp32: an 8-bit integer is a bf16 number as it stands, so g times the scale that its product
+// sums over, in three bf16 parts, times the integers is exact but for the sum: three bf16 products, where two fp32
+// operands take six. dx: the parts beside each other, K = 3 Vr through the weight's rows three times. dW: the parts below
+// each other, K = 3 np against the rows' integers three times.
 struct Grads8Layout {
   int64_t Vr, dp, np, Vp;  // rows and columns of the copies
-  size_t wide, xt, g, split, total;
+  int64_t Kh;              // dx's K
+  int parts;               // of g
+  size_t wide, xt, g, gh, split, total;
   int64_t split_items;
 };
 
 static Grads8Layout grads8_layout(int64_t n, int d, int V, int dtype, bool need_rows, bool need_w, bool as_is) {
-  const int esz = float_bytes(dtype);
   Grads8Layout L;
+  L.parts = dtype == OCTO_F32 ? 3 : 1;
   L.Vr = round_up(V, 64);
   L.dp = round_up(d, TN);
   L.np = round_up(n, 64);
   L.Vp = round_up(V, TM);
+  L.Kh = L.parts == 1 ? V : 3 * L.Vr;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t p = at;
@@ -307,17 +315,17 @@ static Grads8Layout grads8_layout(int64_t n, int d, int V, int dtype, bool need_
   };
   L.split_items = 0;
   if (need_rows) {
-    const int64_t nt = cdiv(d, dtype == OCTO_F32 ? 128 : TN), nk = cdiv(V, 64);
-    const int64_t mt = cdiv(n, TM);
-    if (mt * nt < octo_tiles::kSplitItemsMax) {
-      const int S = octo_tiles::k_splits((int)(mt * nt), (int)nk, true, octo_tiles::kSplitItemsMax);
-      if (S > 1) L.split_items = mt * nt * S;
+    const int64_t tiles = cdiv(n, TM) * cdiv(d, TN);
+    if (tiles < octo_tiles::kSplitItemsMax) {
+      const int S = octo_tiles::k_splits((int)tiles, (int)cdiv(L.Kh, 64), true, octo_tiles::kSplitItemsMax);
+      if (S > 1) L.split_items = tiles * S;
     }
   }
-  L.wide = take(need_rows ? (size_t)L.Vr * L.dp * esz : 0);
-  L.xt = take(need_w ? (size_t)d * L.np * esz : 0);
-  L.g = take(as_is ? 0 : (size_t)L.np * L.Vp * esz);
-  L.split = take((size_t)L.split_items * TM * (dtype == OCTO_F32 ? 128 : TN) * 4);
+  L.wide = take(need_rows ? (size_t)L.Vr * L.dp * 2 : 0);
+  L.xt = take(need_w ? (size_t)d * L.parts * L.np * 2 : 0);
+  L.g = take(L.parts == 1 ? (as_is ? 0 : (size_t)L.np * L.Vp * 2) : (need_w ? (size_t)3 * L.np * L.Vp * 2 : 0));
+  L.gh = take(L.parts == 3 && need_rows ? (size_t)n * L.Kh * 2 : 0);
+  L.split = take((size_t)L.split_items * TM * TN * 4);
   L.total = at;
   return L;
 }
@@ -408,6 +416,8 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
   for (int t : {g_dtype, grad_rows ? gr_dtype : OCTO_F32, grad_w ? gw_dtype : OCTO_F32})
     if (!is_float(t)) return octo_fail(OCTO_EUNSUPPORTED, "head_grads_i8: dtype %d", t);
   OCTO_CHECK_ARG(n > 0, "head_grads_i8: no rows");
+  OCTO_CHECK_ARG(g_dtype != OCTO_F32 || (V <= kMaxV8 / 2 && n <= kMaxN8 / 2),  // three parts within 32-bit offsets
+                 "head_grads_i8: n=%lld, V=%d with fp32 gradients", (long long)n, V);
   OCTO_CHECK_ARG(ldg >= V && (!grad_rows || ld_gr >= d) && (!grad_w || ld_gw >= d), "head_grads_i8: row strides");
   if (!grad_rows && !grad_w) return OCTO_OK;
   OCTO_CHECK_ARG(g && (!grad_rows || (wq && w_scale)) && (!grad_w || (xq && x_scale)), "head_grads_i8: null pointer");
@@ -422,7 +432,7 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
     return octo_fail(OCTO_EWORKSPACE, "head_grads_i8: workspace %zu < %zu bytes", ws ? ws_bytes : (size_t)0, L.total);
   hipStream_t st = (hipStream_t)stream;
   char *wsb = (char *)ws;
-  const int esz = float_bytes(g_dtype);
+  const bool f32 = g_dtype == OCTO_F32;
   Prepare8 p{};
   p.wq = wq;
   p.ldw = ldw;
@@ -434,10 +444,11 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
   p.ldxq = ldxq;
   p.xs = x_scale;
   p.xt = grad_w ? wsb + L.xt : nullptr;
-  p.ldt = L.np;
+  p.ldt = L.parts * L.np;
   p.g = g;
   p.ldg = ldg;
-  p.gs = as_is ? nullptr : wsb + L.g;
+  p.gs = as_is || (f32 && !grad_w) ? nullptr : wsb + L.g;
+  p.gh = f32 && grad_rows ? wsb + L.gh : nullptr;
   p.np = L.np;
   p.Vp = L.Vp;
   p.n = n;
@@ -446,13 +457,15 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
   rc = launch_prepare8(p, g_dtype, st);
   if (rc) return rc;
 
+  const int dt = f32 ? OCTO_BF16 : g_dtype;
   const char *gs = as_is ? (const char *)g : wsb + L.g;
-  const int64_t lds = (as_is ? ldg : L.Vp) * esz;
+  const int64_t lds = (as_is ? ldg : L.Vp) * 2;
   StoreArgs oh, ow;
-  const Operand Ah = operand8(gs, lds, n), Bh = operand8(wsb + L.wide, L.dp * esz, d);
-  const GemmShape sh = shape8(n, d, V), sw = shape8(V, d, n);
+  const Operand Ah = f32 ? operand8(wsb + L.gh, L.Kh * 2, n) : operand8(gs, lds, n);
+  const Operand Bh = operand8(wsb + L.wide, L.dp * 2, f32 ? L.Vr : d);
+  const GemmShape sh = shape8(n, d, L.Kh), sw = shape8(V, d, f32 ? 3 * L.np : n);
   Operand Aw = operand8(gs, lds, as_is ? n : V);
-  const Operand Bw = operand8(wsb + L.xt, L.np * esz, d);
+  const Operand Bw = operand8(wsb + L.xt, L.parts * L.np * 2, d);
   const int kma = as_is ? KM_EDGE : KM_A;
   if (as_is) Aw.extent = (uint32_t)V;
   if (grad_rows) {
@@ -473,11 +486,11 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
   // Both in one launch, dx's runs as long as if it had the card to itself: dW's short tiles follow them on every CU. Two
   // launches take 20 us more up to 700 rows of d 2560, V 151,936 and as long from 1,024 on; runs cut for sharing the card
   // (fewer, longer ones) 949 us for 300 rows against 835.
-  const bool both = grad_rows && grad_w && g_dtype != OCTO_F32;
-  if (both) rc = launch_gemm_grads(g_dtype, Ah, Bh, sh, oh, true, Aw, Bw, sw, ow, st, kma);
-  else if (grad_rows) rc = launch_gemm_store(g_dtype, Ah, Bh, sh, oh, st, KM_B);
-  if (!rc && grad_rows) rc = launch_split_sum(sh, oh, g_dtype == OCTO_F32, st);
-  if (!rc && grad_w && !both) rc = launch_gemm_store(g_dtype, Aw, Bw, sw, ow, st, kma);
+  const bool both = grad_rows && grad_w && !f32;
+  if (both) rc = launch_gemm_grads(dt, Ah, Bh, sh, oh, true, Aw, Bw, sw, ow, st, kma);
+  else if (grad_rows) rc = launch_gemm_store(dt, Ah, Bh, sh, oh, st, f32 ? KM_WRAP : KM_B);
+  if (!rc && grad_rows) rc = launch_split_sum(sh, oh, false, st);
+  if (!rc && grad_w && !both) rc = launch_gemm_store(dt, Aw, Bw, sw, ow, st, kma);
   return rc;
 }
 

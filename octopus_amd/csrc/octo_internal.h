@@ -165,7 +165,8 @@ int launch_gemm_dz(int dt, bool a_fp8, bool tanh, const Operand &A, const Operan
 // kmajor: which operand, if any, is a plain K-major matrix (element (k, m) at base + k ld + 2 m; 16-bit types)
 // KM_EDGE: KM_A of a matrix without room behind it: rows from A.rows on and columns from A.extent on read as zeros (whole
 // 16-byte chunks; 16-bit types)
-enum { KM_NONE = 0, KM_A = 1, KM_B = 2, KM_EDGE = 3 };
+// KM_WRAP: KM_B of a K that runs through B's B.rows rows (a multiple of 64) up to three times (bf16)
+enum { KM_NONE = 0, KM_A = 1, KM_B = 2, KM_EDGE = 3, KM_WRAP = 4 };
 int launch_gemm_store(int dt, const Operand &A, const Operand &B, const GemmShape &s, const StoreArgs &e,
                       hipStream_t st, int kmajor = KM_NONE);
 // C of a split-K product from its partial tiles (StoreArgs::split), with the shape and store its GEMM had; f32: of fp32
@@ -431,23 +432,26 @@ int launch_transpose(const void *src, int64_t ld_src, int src_dtype, const float
                      int64_t rows_pad, int64_t cols, void *dst, int64_t ld_dst, int dst_dtype, hipStream_t st);
 
 // ---- rows of 8-bit integers (rows8.hip) ------------------------------------------------------------
-// What the gradients of the 8-bit head read, in g's type: each copy that is not NULL.
+// What the gradients of the 8-bit head read: each copy that is not NULL. 16-bit g: the 8-bit operands times their scales
+// in g's type, and g itself where it cannot be read as it lies. fp32 g: the 8-bit operands as bf16 integers, and g times
+// the weights' scales (gh) and times the rows' (gs), each as three bf16 parts.
 struct Prepare8 {
   const int8_t *wq;  // [V, ldw]
   int64_t ldw;
   const float *ws;
-  void *wide;        // [Vr, dp] = wq ws, zeros past V
+  void *wide;        // [Vr, dp], zeros past V; Vr a multiple of 64
   int64_t Vr;
   int dp;
   const int8_t *xq;  // [n, ldxq]
   int64_t ldxq;
   const float *xs;
-  void *xt;          // [d, ldt] = (xq xs)^T, zeros past n; ldt a multiple of 64
+  void *xt;          // [d, ldt] transposed, zeros past n; fp32 g: three times, np columns apart
   int64_t ldt;
   const void *g;     // [n, ldg], V columns
   int64_t ldg;
-  void *gs;          // [np, Vp] = g, zeros behind it; Vp whole 16-byte chunks
-  int64_t np, Vp;
+  void *gs;          // [np, Vp], zeros behind g; fp32 g: [3 np, Vp], a part after the other
+  void *gh;          // fp32 g: [n, 3 Vr], a part beside the other
+  int64_t np, Vp;    // np a multiple of 64, Vp of 8
   int64_t n;
   int d, V;
   unsigned wide_blocks, t_blocks, g_parts;  // set by the launch

@@ -99,7 +99,8 @@ __device__ __forceinline__ void unpack_i8(const i32x2 v, float s, float (&x)[8])
 // Row r of out = q scale for the columns c < d, zeros up to cols_pad (and for all of a row past `rows`), by one wave, 4
 // chunks of 8 columns a lane in flight. gshift: log2 of the group, or -1. The bytes of q behind d are readable up to the
 // next multiple of 16.
-template <int DT>
+// UNIT: the integers themselves (exact in every type).
+template <int DT, bool UNIT = false>
 __device__ __forceinline__ void widen_row(const int8_t *q, const float *scale, bool there, int d, int gshift,
                                           typename Elem<DT>::T *out, int cols_pad) {
   const int lane = threadIdx.x & 63;
@@ -110,7 +111,7 @@ __device__ __forceinline__ void widen_row(const int8_t *q, const float *scale, b
     for (int u = 0; u < 4; ++u) {
       const int c = c0 + 512 * u, at = there && c < d ? c : 0;
       v[u] = there ? *(const i32x2 *)(q + at) : i32x2{0, 0};
-      s[u] = there && c < d ? scale[gshift < 0 ? 0 : at >> gshift] : 0.f;
+      s[u] = !there || c >= d ? 0.f : (UNIT ? 1.f : scale[gshift < 0 ? 0 : at >> gshift]);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -143,9 +144,11 @@ __global__ __launch_bounds__(256) void widen_i8_kernel(const int8_t *q, int64_t 
   if (r < rows) widen_row<DT>(q + r * ldq, scale + r * groups, true, d, gshift, out + r * ldo, d);
 }
 
-// out[c, r] = q[r, c] scale[r] for c < d, r0 <= r < r0 + 64; zeros from `rows` on. A 64 x 64 tile through the LDS.
-template <int DT>
-__device__ __forceinline__ void widen_t_tile(const Prepare8 &a, int64_t r0, int c0, typename Elem<DT>::T (*tile)[64 + 16 / Elem<DT>::bytes]) {
+// xt[c, r] = q[r, c] scale[r] for c < d, r0 <= r < r0 + 64; zeros from n on; `repeats` of it np columns apart. A 64 x 64
+// tile through the LDS.
+template <int DT, bool UNIT = false>
+__device__ __forceinline__ void widen_t_tile(const Prepare8 &a, int64_t r0, int c0, int repeats,
+                                             typename Elem<DT>::T (*tile)[64 + 16 / Elem<DT>::bytes]) {
   typedef typename Elem<DT>::T T;
   constexpr int PER = 16 / sizeof(T);
   const int t = threadIdx.x;
@@ -155,7 +158,7 @@ __device__ __forceinline__ void widen_t_tile(const Prepare8 &a, int64_t r0, int 
     i32x4 v = {0, 0, 0, 0};
     float s = 0.f;
     if (r < a.n && c0 + c < a.d) {
-      s = a.xs[r];
+      s = UNIT ? 1.f : a.xs[r];
       v = *(const i32x4 *)(a.xq + r * a.ldxq + c0 + c);
     }
 #pragma unroll
@@ -170,7 +173,9 @@ __device__ __forceinline__ void widen_t_tile(const Prepare8 &a, int64_t r0, int 
 #pragma unroll
   for (int k = 0; k < 64 * 64 / PER / 256; ++k) {
     const int i = t + 256 * k, c = i / (64 / PER), r = (i % (64 / PER)) * PER;
-    if (c0 + c < a.d) *(i32x4 *)((T *)a.xt + (int64_t)(c0 + c) * a.ldt + r0 + r) = *(const i32x4 *)&tile[c][r];
+    if (c0 + c >= a.d) continue;
+    const i32x4 v = *(const i32x4 *)&tile[c][r];
+    for (int p = 0; p < repeats; ++p) *(i32x4 *)((T *)a.xt + (int64_t)(c0 + c) * a.ldt + p * a.np + r0 + r) = v;
   }
 }
 
@@ -187,8 +192,7 @@ __device__ __forceinline__ void stage_part(const Prepare8 &a, int64_t r, int par
     v[u] = i32x4{0, 0, 0, 0};
     if (r >= a.n || c >= a.V) continue;
     if (c + PER <= a.V) {
-      if constexpr (DT == OCTO_F32) v[u] = *(const i32x4_any4 *)(g + c);
-      else v[u] = *(const i32x4_any *)(g + c);
+      v[u] = *(const i32x4_any *)(g + c);
     } else {
       T x[PER] = {};
 #pragma unroll
@@ -204,33 +208,76 @@ __device__ __forceinline__ void stage_part(const Prepare8 &a, int64_t r, int par
   }
 }
 
+// fp32 g: 8 values of a row times their weights' scales, and times the row's, each as three bf16 parts whose sum it is
+// (24 bits; what bf16 cannot hold stays in the first part alone).
+__device__ __forceinline__ void split_parts(const float (&x)[8], i32x4 (&part)[3]) {
+  float p0[8], p1[8], p2[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    p0[e] = (float)(__bf16)x[e];
+    const bool fine = fabsf(p0[e]) < INFINITY;
+    p1[e] = fine ? (float)(__bf16)(x[e] - p0[e]) : 0.f;
+    p2[e] = fine ? x[e] - p0[e] - p1[e] : 0.f;
+  }
+  part[0] = pack8(p0, false);
+  part[1] = pack8(p1, false);
+  part[2] = pack8(p2, false);
+}
+__device__ __forceinline__ void stage_f32(const Prepare8 &a, int64_t r, int part) {
+  const int c = (part * 256 + (int)threadIdx.x) * 8;
+  float x[8], y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = 0.f;
+  if (r < a.n && c < a.V) values8<OCTO_F32>(load_raw8<OCTO_F32>((const float *)a.g + r * a.ldg + c, a.V - c), x);
+  i32x4 v[3];
+  if (a.gh && r < a.n && c < a.Vr) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = c + e < a.V ? x[e] * a.ws[c + e] : 0.f;
+    split_parts(y, v);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *(i32x4 *)((__bf16 *)a.gh + r * 3 * a.Vr + p * a.Vr + c) = v[p];
+  }
+  if (a.gs && c < a.Vp) {
+    const float s = r < a.n ? a.xs[r] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = r < a.n ? x[e] * s : 0.f;
+    split_parts(y, v);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *(i32x4 *)((__bf16 *)a.gs + (p * a.np + r) * a.Vp + c) = v[p];
+  }
+}
+
 // The copies that the gradients' products read, in one launch: blocks of 4 weight rows, of 64 x 64 tiles of the
 // transposed rows, of parts of g's rows.
 template <int DT>
 __global__ __launch_bounds__(256) void prepare8_kernel(Prepare8 a) {
-  typedef typename Elem<DT>::T T;
+  constexpr bool F32 = DT == OCTO_F32;
+  constexpr int WT = F32 ? OCTO_BF16 : DT;  // fp32 g multiplies with the integers in bf16, its parts with the scales in g
+  typedef typename Elem<WT>::T T;
   __shared__ __attribute__((aligned(16))) T tile[64][64 + 16 / sizeof(T)];
   unsigned b = blockIdx.x;
   if (b < a.wide_blocks) {
     const int64_t r = (int64_t)b * 4 + (threadIdx.x >> 6);  // Vr is a multiple of 64
-    widen_row<DT>(a.wq + r * a.ldw, a.ws + r, r < a.V, a.d, -1, (T *)a.wide + r * a.dp, a.dp);
+    widen_row<WT, F32>(a.wq + r * a.ldw, a.ws + r, r < a.V, a.d, -1, (T *)a.wide + r * a.dp, a.dp);
     return;
   }
   b -= a.wide_blocks;
   if (b < a.t_blocks) {
-    const unsigned tiles = (unsigned)(a.ldt / 64);
-    widen_t_tile<DT>(a, (int64_t)(b % tiles) * 64, (int)(b / tiles) * 64, tile);
+    const unsigned tiles = (unsigned)(a.np / 64);
+    widen_t_tile<WT, F32>(a, (int64_t)(b % tiles) * 64, (int)(b / tiles) * 64, F32 ? 3 : 1, tile);
     return;
   }
   b -= a.t_blocks;
-  stage_part<DT>(a, b / a.g_parts, (int)(b % a.g_parts));
+  if constexpr (F32) stage_f32(a, b / a.g_parts, (int)(b % a.g_parts));
+  else stage_part<DT>(a, b / a.g_parts, (int)(b % a.g_parts));
 }
 
 int launch_prepare8(Prepare8 a, int dtype, hipStream_t st) {
-  const int64_t per = 512 * (16 / float_bytes(dtype));  // values of a part of g
-  const int64_t wide = a.wide ? a.Vr / 4 : 0, t = a.xt ? a.ldt / 64 * cdiv(a.d, 64) : 0;
+  const bool f32 = dtype == OCTO_F32;
+  const int64_t per = f32 ? 256 * 8 : 512 * 8;  // values of a part of g
+  const int64_t wide = a.wide ? a.Vr / 4 : 0, t = a.xt ? a.np / 64 * cdiv(a.d, 64) : 0;
   a.g_parts = (unsigned)cdiv(a.Vp, per);
-  const int64_t staged = a.gs ? a.np * a.g_parts : 0, blocks = wide + t + staged;
+  const int64_t staged = a.gs || a.gh ? a.np * a.g_parts : 0, blocks = wide + t + staged;
   if (blocks == 0) return OCTO_OK;
   if (blocks >= (1 << 24)) return octo_fail(OCTO_EINVAL, "head_grads_i8: %lld blocks", (long long)blocks);
   a.wide_blocks = (unsigned)wide;

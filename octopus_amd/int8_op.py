@@ -4,9 +4,9 @@
     octohead::head_logits_i8 / head_grads_i8   rows W^T in 8-bit integers with a scale for each row of both; its gradients
     checkpoint8                                a checkpoint that holds its inputs in 8 bits
 
-Of a row, or of each group of 32 to 256 of its values, with a the largest magnitude: scale = a times 1/127, both
-in fp32, q the exact quotient x / scale to the nearest integer (ties to even). A group below 2^-119 is held as zeros, one with a NaN or an
-infinity as NaN. int8 rows start on 16-byte boundaries, zeros between them (quantise_rows gives them so).
+Of a row, or of each group of 32 to 256 of its values, with a the largest magnitude: scale = a times 1/127, both in fp32,
+q the exact quotient x / scale to the nearest integer (ties to even). A group below 2^-119 is held as zeros, one with a
+NaN or an infinity as NaN. int8 rows start on 16-byte boundaries, zeros between them (quantise_rows gives them so).
 
 The logits are x_scale w_scale sum_k xq wq, the sum exact. Their gradients go straight through the rounding: in the rows
 g (w_scale wq), in the weight g^T (x_scale xq), so that what is held for them is the 8-bit rows that the product read and
@@ -321,8 +321,8 @@ def int8_head(rows: Tensor, wq: Tensor, w_scale: Tensor, *, weight: Optional[Ten
     and rounded once. The rows' gradient is that of the weights' 8-bit values. weight: the [V, d] parameter that wq was
     made of, which gets the gradient straight through the rounding; its values are not read, and wq is made again when
     it has changed. Between the two passes the rows are held in 8 bits, and wq and w_scale by reference (changed in
-    place, the backward raises). wq and w_scale get no gradient. The gradients have no derivative of
-    their own: one raises."""
+    place, the backward raises). wq and w_scale get no gradient; the gradients have no derivative of their own (one
+    raises)."""
     out_dtype = out_dtype or rows.dtype
     if torch.compiler.is_compiling():
         return head_logits_i8(rows, wq, w_scale, weight, out_dtype)[0]

@@ -172,6 +172,41 @@ def test_gradients_of_other_types():
     assert ((b.cpu().double() - gw).abs() <= bound_w).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [3, 300])
+def test_gradients_that_are_not_finite_stay_in_their_row_and_column(n, dtype):
+    """As the formula has them: row r of the rows' gradient and row v of the weight's."""
+    x, w = _inputs(n, 72, 520, dtype)
+    w[7] = 0
+    wq, ws = int8_op.quantise_rows(w.to(DEV))
+    g = torch.randn(n, 520, generator=torch.Generator().manual_seed(2)).to(dtype)
+    g[1, 7], g[2, 515] = torch.nan, torch.inf
+    xd = x.to(DEV).requires_grad_(True)
+    wd = w.to(DEV).requires_grad_(True)
+    int8_op.int8_head(xd, wq, ws, weight=wd).backward(g.to(DEV))
+    rows, weights = torch.ones(n, dtype=torch.bool), torch.ones(520, dtype=torch.bool)
+    rows[1] = rows[2] = False
+    weights[7] = weights[515] = False
+    for grad, fine in ((xd.grad.cpu(), rows), (wd.grad.cpu(), weights)):
+        assert grad[fine].isfinite().all() and not grad[~fine].isfinite().any()
+
+
+def test_fp32_gradients_keep_24_bits():
+    """Each value of g alone: one nonzero product to a sum, so the error is that of the parts (2^-24 of the value, and
+    of g times the scale) and of the result's rounding; over the range that three parts of normal numbers hold."""
+    n, d, V = 64, 48, 64
+    x, w = _inputs(n, d, V, torch.float32)
+    wq, ws = int8_op.quantise_rows(w.to(DEV))
+    size = torch.logspace(-28, 28, n, dtype=torch.float64)
+    g = torch.diag((torch.rand(n, generator=torch.Generator().manual_seed(3), dtype=torch.float64) + 1) * size).float()
+    xd = x.to(DEV).requires_grad_(True)
+    wd = w.to(DEV).requires_grad_(True)
+    int8_op.int8_head(xd, wq, ws, weight=wd).backward(g.to(DEV))
+    rows, weights, *_ = oracle.grads(g, x, wq.cpu(), ws.cpu())
+    for grad, want in ((xd.grad, rows), (wd.grad, weights)):
+        assert ((grad.cpu().double() - want).abs() <= 4 * 2.0 ** -24 * want.abs()).all()
+
+
 def test_gradients_against_differences():
     """The rows' gradient against differences of the logits of the same 8-bit weights at rows that are not rounded."""
     x, w = _inputs(4, 32, 50, torch.float32)

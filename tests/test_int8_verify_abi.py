@@ -66,6 +66,9 @@ def test_head8_checks():
                    dict(g=ctypes.c_void_p(4097)), dict(gw=ctypes.c_void_p(4097))]:
         _refused("octo_head_grads_i8", *{**ok, **change}.values(), None)
     _refused("octo_head_grads_i8", *{**ok, "gdt": 9}.values(), None, exc=NotImplementedError)
+    far = dict(gdt=_lib.F32, nwork=1 << 62)  # three parts of fp32 gradients lie within 32-bit offsets up to 2^20
+    _refused("octo_head_grads_i8", *{**ok, **far, "n": (1 << 20) + 1}.values(), None)
+    _refused("octo_head_grads_i8", *{**ok, **far, "V": (1 << 20) + 1, "ldg": 1 << 21}.values(), None)
     _lib.call("octo_head_grads_i8", *{**ok, "gr": None, "gw": None}.values(), None)
 
 
