@@ -14,7 +14,7 @@
 //   residual  each workgroup joins its sequence's rows, finds a by itself, and its waves sum their parts' r
 //   pick      a workgroup per sequence finds the part in which the running sum passes u_K sum r, and in it the token
 // Many take the exponentials of stats in 32 bits (64-bit ones are 20 instructions each, and stats is most of the work),
-// which leave each row's sum within 4e-6 (see fast_part). That decides a draft unless u q and p are closer than 2^-15;
+// which leave each row's sum within 4e-6 (see fast_spread). That decides a draft unless u q and p are closer than 2^-15;
 // then the row and its draft's are summed again in 64 bits there. decide, sums and rest take residual's place: a is found
 // once a sequence, and one sweep over row a of both models finds in 64 bits their sums and those of r (part_sums).
 #include "octo_common.h"
@@ -71,11 +71,11 @@ struct VerifyArgs {
   int64_t S;
   int K, V;
   double c;                   // log2(e) / T
-  float c_hi, c_lo, d_least;  // the same in two parts, and a difference whose exponential is 0 in 32 bits
+  float cf;                   // the same in 32 bits
   int greedy;
-  int parts, part;  // parts of a row, values of each (a multiple of kVBlock)
-  int turns;        // parts a wave takes (sums, residual)
-  PartStat *stats;  // [S, 2 K + 1, parts]: target rows, then draft rows
+  int parts, part;      // parts of a row, values of each (a multiple of kVBlock)
+  int sparts, spart;    // the same of stats (EXACT: as these)
+  PartStat *stats;      // [S, 2 K + 1, sparts]: target rows, then draft rows
   // [S, parts]: of e = exp((z - m) / T) of row a, of its draft row's; of both over the columns with r > 0 (sum_a NaN:
   // not known yet). Few logits: sum_a holds the sums of r.
   double *sum_p, *sum_q, *sum_a, *sum_b;
@@ -211,26 +211,25 @@ __device__ __forceinline__ PartStat exact_part(const VerifyArgs &a, const typena
   return r;
 }
 
-// A wave's part with exponentials in 32 bits. exp2 is within 2^-23 of its value, and its argument d c, d = z - m <= 0,
-// off by at most 2^-23 |d c| (d, and the product with c in two parts, rounded once each), which makes ln 2 times that of
-// the value: over a row at most 2^-23 (1 + 0.7 x 20), as the mean of |d c| under the softmax is at most log2 V. Eight
-// values are summed in 32 bits (3 x 2^-24), all else in 64. Together below 4e-6 of the row's sum.
+// A wave's run of blocks with exponentials in 32 bits, the next block's loads in flight. exp2 is within 2^-23 of its value,
+// and its argument (z - m) c, c rounded to 32 bits, off by at most 1.5 x 2^-23 of itself (d, c and the product), which
+// makes ln 2 times that of the value: over a row at most 2^-23 (1 + 1.04 x 20), as the mean of |d c| under the softmax is
+// at most log2 V. Eight values are summed in 32 bits (3 x 2^-24), all else in 64. Together below 4e-6 of the row's sum.
+// A NaN stays one through difference, product and exponential, and +inf makes one (inf - inf): S shows both.
 template <int DT>
-__device__ __forceinline__ PartStat fast_part(const VerifyArgs &a, const typename Elem<DT>::T *row, int c0, int c1) {
+__device__ __forceinline__ PartStat fast_spread(const VerifyArgs &a, const typename Elem<DT>::T *row, int c0, int c1) {
   float m = -INFINITY;
   double S = 0.0;
   int first = 0x7fffffff;
-  bool bad = false;
-  for (int c = c0; c < c1; c += kVBlock) {
+  Raw8<DT> v[2][4];
+  auto take = [&](const Raw8<DT>(&r)[4], int c) {
     float x[4][8], mx = m;
-    load_block<DT>(row, c, c1, x);
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < 4; ++u) {
+      values8<DT>(r[u], x[u]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        mx = fmaxf(mx, x[u][e]);
-        bad |= !(x[u][e] < INFINITY);
-      }
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, x[u][e]);
+    }
     if (mx > m) {
       S *= exp2_64(((double)m - (double)mx) * a.c);
       first = 0x7fffffff;
@@ -241,10 +240,7 @@ __device__ __forceinline__ PartStat fast_part(const VerifyArgs &a, const typenam
     for (int u = 0; u < 4; ++u) {
       float t[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float d = fmaxf(x[u][e] - mf, a.d_least);
-        t[e] = fexp2(__builtin_fmaf(d, a.c_hi, d * a.c_lo));
-      }
+      for (int e = 0; e < 8; ++e) t[e] = fexp2((x[u][e] - mf) * a.cf);
       S += (double)(((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7])));
     }
     if (a.greedy) {
@@ -254,11 +250,19 @@ __device__ __forceinline__ PartStat fast_part(const VerifyArgs &a, const typenam
         for (int e = 0; e < 8; ++e)
           if (x[u][e] == m) first = min(first, c + 512 * u + 8 * (int)(threadIdx.x & 63) + e);
     }
+  };
+  load_raw_block<DT>(row, c0, c1, v[0]);
+  for (int c = c0;;) {
+    if (c + kVBlock < c1) load_raw_block<DT>(row, c + kVBlock, c1, v[1]);
+    take(v[0], c);
+    if ((c += kVBlock) >= c1) break;
+    if (c + kVBlock < c1) load_raw_block<DT>(row, c + kVBlock, c1, v[0]);
+    take(v[1], c);
+    if ((c += kVBlock) >= c1) break;
   }
   PartStat r;
   r.m = wave_max(m);
-  r.S = wave_sum64(m == -INFINITY ? 0.0 : S * exp2_64(((double)m - (double)r.m) * a.c));
-  if (__any(bad)) r.S = __builtin_nan("");
+  r.S = wave_sum64(m == -INFINITY ? S : S * exp2_64(((double)m - (double)r.m) * a.c));  // m -inf: S is 0 or NaN
   r.first = wave_min(m == r.m ? first : 0x7fffffff);
   return r;
 }
@@ -271,22 +275,22 @@ __global__ __launch_bounds__(kVThreads) void verify_stats_kernel(VerifyArgs a) {
   const int k = __builtin_amdgcn_readfirstlane(blockIdx.x * kVWaves + (threadIdx.x >> 6));
   const bool draft = i > a.K;
   if (draft ? (!a.zd || i - a.K - 1 >= len) : i > len) return;  // nobody asks for the row
-  if (k >= a.parts) return;
+  if (k >= a.sparts) return;
   const typename Elem<DT>::T *row = draft ? row_of<DT>(a.zd, a.ls_d, a.lr_d, s, i - a.K - 1)
                                           : row_of<DT>(a.z, a.ls, a.lr, s, i);
-  const int c0 = k * a.part, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.part);
-  const PartStat r = EXACT ? exact_part<DT>(a, row, c0, c1) : fast_part<DT>(a, row, c0, c1);
-  if ((threadIdx.x & 63) == 0) a.stats[(int64_t)blockIdx.y * a.parts + k] = r;
+  const int c0 = k * a.spart, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.spart);
+  const PartStat r = EXACT ? exact_part<DT>(a, row, c0, c1) : fast_spread<DT>(a, row, c0, c1);
+  if ((threadIdx.x & 63) == 0) a.stats[(int64_t)blockIdx.y * a.sparts + k] = r;
 }
 
 // Row i's statistics from its parts, by one wave; the same in every lane.
 __device__ __forceinline__ RowStat join_row(const VerifyArgs &a, int64_t s, int i) {
-  const PartStat *p = a.stats + (s * (2 * a.K + 1) + i) * a.parts;
+  const PartStat *p = a.stats + (s * (2 * a.K + 1) + i) * a.sparts;
   const int lane = threadIdx.x & 63;
   float m = -INFINITY;
   double S = 0.0;
   int first = 0x7fffffff;
-  for (int k = lane; k < a.parts; k += 64) {
+  for (int k = lane; k < a.sparts; k += 64) {
     const PartStat t = p[k];
     const float mx = fmaxf(m, t.m);
     if (mx > m) {
@@ -500,14 +504,12 @@ __global__ __launch_bounds__(kVThreads) void verify_sums_kernel(VerifyArgs a) {
   const int64_t s = blockIdx.y;
   const VerifyArgs::Decision d = a.dec[s];
   if (!(d.p.inv > 0.0)) return;
-  for (int t = 0; t < a.turns; ++t) {
-    const int k = __builtin_amdgcn_readfirstlane((blockIdx.x * kVWaves + (threadIdx.x >> 6)) * a.turns + t);
-    if (k >= a.parts) return;
-    const int c0 = k * a.part, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.part);
-    if (d.residual == 1) part_sums<DT, 1>(a, d, s, k, c0, c1);
-    else if (d.residual == 2) part_sums<DT, 2>(a, d, s, k, c0, c1);
-    else part_sums<DT, 0>(a, d, s, k, c0, c1);
-  }
+  const int k = __builtin_amdgcn_readfirstlane(blockIdx.x * kVWaves + (threadIdx.x >> 6));
+  if (k >= a.parts) return;
+  const int c0 = k * a.part, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.part);
+  if (d.residual == 1) part_sums<DT, 1>(a, d, s, k, c0, c1);
+  else if (d.residual == 2) part_sums<DT, 2>(a, d, s, k, c0, c1);
+  else part_sums<DT, 0>(a, d, s, k, c0, c1);
 }
 
 template <int DT, int MODE>
@@ -553,22 +555,17 @@ template <int DT>
 __global__ __launch_bounds__(kVThreads) void verify_rest_kernel(VerifyArgs a) {
   const int64_t s = blockIdx.y;
   if (a.dec[s].residual != 1) return;
-  bool any = false;
-  const int k0 = __builtin_amdgcn_readfirstlane((blockIdx.x * kVWaves + (threadIdx.x >> 6)) * a.turns);
-  for (int k = k0; k < min(a.parts, k0 + a.turns); ++k) any |= a.sum_a[s * a.parts + k] != a.sum_a[s * a.parts + k];
-  if (!any) return;
+  const int k = __builtin_amdgcn_readfirstlane(blockIdx.x * kVWaves + (threadIdx.x >> 6));
+  if (k >= a.parts || a.sum_a[s * a.parts + k] == a.sum_a[s * a.parts + k]) return;
   VerifyArgs::Decision d = a.dec[s];
   if (!(d.p.inv > 0.0)) return;
   exact_rows(a, s, d);
-  for (int k = k0; k < min(a.parts, k0 + a.turns); ++k) {
-    if (a.sum_a[s * a.parts + k] == a.sum_a[s * a.parts + k]) continue;
-    const int c0 = k * a.part, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.part);
-    const double S = part_mass<DT, 1>(a, d, row_of<DT>(a.z, a.ls, a.lr, s, d.a),
-                                      row_of<DT>(a.zd, a.ls_d, a.lr_d, s, d.a), c0, c1);
-    if ((threadIdx.x & 63) == 0) {
-      a.sum_a[s * a.parts + k] = S / d.p.inv;
-      a.sum_b[s * a.parts + k] = 0.0;
-    }
+  const int c0 = k * a.part, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.part);
+  const double S = part_mass<DT, 1>(a, d, row_of<DT>(a.z, a.ls, a.lr, s, d.a),
+                                    row_of<DT>(a.zd, a.ls_d, a.lr_d, s, d.a), c0, c1);
+  if ((threadIdx.x & 63) == 0) {
+    a.sum_a[s * a.parts + k] = S / d.p.inv;
+    a.sum_b[s * a.parts + k] = 0.0;
   }
 }
 
@@ -755,6 +752,8 @@ static int part_values(int V) { return (int)round_up(cdiv(V, kVParts), kVBlock);
 
 // Rows that are summed with 32-bit exponentials, from this many logits on.
 constexpr int64_t kVMany = (int64_t)1 << 24;
+// Waves of their statistics that the parts of up to 8 blocks leave at least.
+constexpr int64_t kVSpread = 16384;
 
 struct VerifyLayout {
   int parts, part;
@@ -772,23 +771,22 @@ static VerifyLayout verify_layout(int64_t S, int K, int V) {
 }
 
 template <int DT, bool EXACT> static int go_launches(const VerifyArgs &a, hipStream_t st) {
-  const dim3 parts((unsigned)cdiv(a.parts, kVWaves), (unsigned)(a.S * (2 * a.K + 1)));
-  const dim3 taken((unsigned)cdiv(a.parts, (int64_t)kVWaves * a.turns), (unsigned)a.S);
-  hipLaunchKernelGGL((verify_stats_kernel<DT, EXACT>), parts, dim3(kVThreads), 0, st, a);
+  const dim3 spread((unsigned)cdiv(a.sparts, kVWaves), (unsigned)(a.S * (2 * a.K + 1)));
+  const dim3 parts((unsigned)cdiv(a.parts, kVWaves), (unsigned)a.S);
+  hipLaunchKernelGGL((verify_stats_kernel<DT, EXACT>), spread, dim3(kVThreads), 0, st, a);
   OCTO_CHECK_LAUNCH("verify_stats");
   if (!a.greedy && !EXACT) {
     hipLaunchKernelGGL(verify_decide_kernel<DT>, dim3((unsigned)a.S), dim3(kVDecide), 0, st, a);
     OCTO_CHECK_LAUNCH("verify_decide");
-    hipLaunchKernelGGL(verify_sums_kernel<DT>, taken, dim3(kVThreads), 0, st, a);
+    hipLaunchKernelGGL(verify_sums_kernel<DT>, parts, dim3(kVThreads), 0, st, a);
     OCTO_CHECK_LAUNCH("verify_sums");
   }
   if (!a.greedy && !EXACT && a.zd) {
-    hipLaunchKernelGGL(verify_rest_kernel<DT>, taken, dim3(kVThreads), 0, st, a);
+    hipLaunchKernelGGL(verify_rest_kernel<DT>, parts, dim3(kVThreads), 0, st, a);
     OCTO_CHECK_LAUNCH("verify_rest");
   }
   if (!a.greedy && EXACT) {
-    hipLaunchKernelGGL(verify_residual_kernel<DT>, dim3((unsigned)cdiv(a.parts, kVWaves), (unsigned)a.S),
-                       dim3(kVThreads), 0, st, a);
+    hipLaunchKernelGGL(verify_residual_kernel<DT>, parts, dim3(kVThreads), 0, st, a);
     OCTO_CHECK_LAUNCH("verify_residual");
   }
   hipLaunchKernelGGL((verify_pick_kernel<DT, EXACT>), dim3((unsigned)a.S), dim3(kVThreads), 0, st, a);
@@ -807,7 +805,7 @@ template <int DT> static int go_verify(const VerifyArgs &a, bool exact, hipStrea
     b.drafts = a.drafts + s0 * a.K;
     b.lengths = a.lengths ? a.lengths + s0 : nullptr;
     b.u = a.u ? a.u + s0 * (a.K + 1) : nullptr;
-    b.stats = a.stats + s0 * rows * a.parts;
+    b.stats = a.stats + s0 * rows * a.sparts;
     b.sum_p = a.sum_p + s0 * a.parts;
     b.sum_q = a.sum_q + s0 * a.parts;
     b.sum_a = a.sum_a + s0 * a.parts;
@@ -871,14 +869,9 @@ int octo_verify_drafts(const void *logits, int64_t ld_seq, int64_t ld_row, const
   a.greedy = greedy != 0;
   const double c = inv_T * 1.4426950408889634074;
   a.c = c;
-  a.c_hi = (float)c;
-  a.c_lo = (float)(c - (double)a.c_hi);
-  a.d_least = (float)(-300.0 / c);
+  a.cf = (float)c;
   a.parts = L.parts;
   a.part = L.part;
-  // a wave takes several parts where there are many: each of its workgroups first joins the sequence's rows
-  const int64_t turns = S * L.parts / (kVWaves * 2048);
-  a.turns = (int)(turns < 1 ? 1 : (turns > 8 ? 8 : turns));
   a.stats = (PartStat *)((char *)ws + L.stats);
   a.sum_p = (double *)((char *)ws + L.sums);
   a.sum_q = a.sum_p + S * L.parts;
@@ -888,7 +881,11 @@ int octo_verify_drafts(const void *logits, int64_t ld_seq, int64_t ld_row, const
   a.tokens = tokens;
   a.accepted = accepted;
   a.logp = logp;
-  const bool exact = S * (a.zd ? 2 * K + 1 : K + 1) * (int64_t)V < kVMany || !(c >= 0x1p-40 && c <= 0x1p40);
+  const int64_t rows = S * (a.zd ? 2 * K + 1 : K + 1);
+  const bool exact = rows * V < kVMany || !(c >= 0x1p-40 && c <= 0x1p40);
+  const int64_t run = exact ? 1 : rows * L.parts / kVSpread;
+  a.spart = L.part * (int)(run < 1 ? 1 : (run > 8 ? 8 : run));
+  a.sparts = (int)cdiv(V, a.spart);
   switch (dtype) {
     case OCTO_BF16: return go_verify<OCTO_BF16>(a, exact, (hipStream_t)stream);
     case OCTO_F16: return go_verify<OCTO_F16>(a, exact, (hipStream_t)stream);
