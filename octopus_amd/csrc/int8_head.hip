@@ -3,6 +3,14 @@
 //   z[r, v] = sx[r] sw[v] sum_k qx[r, k] qw[v, k]          (the sum exact in 32 bits: d <= 131,072)
 //   dx[r, k] = sum_v g[r, v] sw[v] qw[v, k]                (straight through the rounding of rows and weights)
 //   dW[v, k] = sum_r g[r, v] sx[r] qx[r, k]
+//
+// Three routes for the logits, by the rows. Up to 32 read the weight's bytes once and are bound by them (few_i8_kernel: 1
+// row of d 2560, V 151,936 74 us, 5.2 TB/s). Up to 128 the same in tiles, two workgroups a CU (64 rows 95 us, 4.3 TB/s with
+// the logits). More are bound by the matrix rate: 8,192 rows 2,740 us, 2.33 POP/s with the logits' 2.5 GB written beside it
+// (without them 2,614; a library product of these integers, which writes 32-bit sums, reaches 1.82).
+//
+// The gradients are 16-bit products of the widened operands (prepare8_kernel: 190 us at that weight, a write of 778 MB), at
+// the rate of the head's other gradients: 2,048 rows 2,480 us for both, 1.29 PFLOP/s.
 #include <type_traits>
 
 #include "gemm_nt.h"
@@ -15,7 +23,11 @@ namespace octo {
 constexpr int kMaxD8 = 131072;       // 127^2 d < 2^31
 constexpr int kMaxV8 = 1 << 21;      // a tile's 256 rows of g within 32-bit offsets
 constexpr int64_t kMaxN8 = 1 << 21;  // the same of the transposed rows
-constexpr int kGroup8 = 8;  // M-tiles that an XCD walks the tokens with: 2,048 rows at d 2560, V 151,936 795 us in fours, 749 in eights
+// M-tiles that an XCD walks the tokens with: 2,048 rows at d 2560, V 151,936 795 us in fours, 749 in eights, the same in
+// sixteens, more in thirty-twos.
+constexpr int kGroup8 = 8;
+// Up to here tiles of 128 x 128. The same weight, us with them and with wide ones: 64 rows 95 and 118, 128 104 and 119,
+// 192 147 and 126, 256 157 and 133. (Eight waves on the small tile: 128 rows 111.)
 constexpr int64_t kSmallRows = 128;
 
 typedef i32x4 i32x4_el __attribute__((aligned(2)));
@@ -39,7 +51,7 @@ template <int VM, int TOK, int NW_> struct Tile8 {
   static __device__ __forceinline__ int col(int w, int j, int lane) { return w % NWN * (TOK / NWN) + j * 16 + (lane & 15); }
 };
 typedef Tile8<256, 256, 8> TileWide;    // one workgroup a CU
-typedef Tile8<256, 192, 8> Tile192;     // the last tokens of a wide grid
+typedef Tile8<256, 192, 8> Tile192;     // the last tokens of a wide grid: 320 rows of d 4096 228 us without, 209 with
 typedef Tile8<256, 128, 8> Tile128;
 typedef Tile8<128, 128, 4> TileSmall;   // half the LDS: two workgroups a CU, one of which loads and multiplies while the
                                         // other begins or stores
@@ -111,7 +123,8 @@ __device__ __forceinline__ void gemm_i8_tile(const Operand &A, const Operand &B,
   store_logits8<L, OT>(acc, e, m0, n0, (int)s.M, min(s.N - n0, (int64_t)L::TOKENS), smem);
 }
 template <typename OT>
-__global__ __launch_bounds__(512, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_kernel(Operand A, Operand B, GemmShape s, Logits8 e) {
+__global__ __launch_bounds__(512, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_kernel(Operand A, Operand B,
+                                                                                                    GemmShape s, Logits8 e) {
   __shared__ __attribute__((aligned(16))) char smem_[TileWide::LDS];
   int mt, nt;
   if (!tile_of(s, mt, nt)) return;
@@ -121,7 +134,9 @@ __global__ __launch_bounds__(512, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   else gemm_i8_tile<TileWide, OT>(A, B, s, e, m0, n0, (lds_char *)smem_);
 }
 template <typename OT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_small_kernel(Operand A, Operand B, GemmShape s, Logits8 e) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_small_kernel(Operand A, Operand B,
+                                                                                                       GemmShape s,
+                                                                                                       Logits8 e) {
   __shared__ __attribute__((aligned(16))) char smem_[TileSmall::LDS];
   int mt, nt;
   if (tile_of(s, mt, nt)) gemm_i8_tile<TileSmall, OT>(A, B, s, e, (int64_t)mt * 128, (int64_t)nt * 128, (lds_char *)smem_);
@@ -135,6 +150,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // 16 (l >> 4) of each 64), kFewSteps loads ahead, also into the next 16 rows, and no wave waits for another. The shares
 // are equal to 4 rows, so that all waves end together: in blocks of 16 rows 9,496 blocks on 6,144 waves take as long as
 // 12,288 would. A share's last block repeats its last row (no bytes of its own, and its MFMAs are idle time).
+//
+// d 2560, V 151,936, us so and in tiles of 256 x 256: 1 row 80 and 108, 16 89 and 108, 32 97 and 109; at 33 the small
+// tiles take 96, this 102. Weight loads past the caches (nontemporal): 100 for 1 row.
 constexpr int kFewSteps = 8;
 constexpr int kFewLds = 156 * 1024;  // with the scales, what a workgroup can have
 constexpr int64_t kFewRows = 32;
@@ -290,7 +308,8 @@ static GemmShape shape8(int64_t M, int64_t N, int64_t K, int tile = TM) {
 // fp32 g is not multiplied in fp32: an 8-bit integer is a bf16 number as it stands, so g times the scale that its product
 // sums over, in three bf16 parts, times the integers is exact but for the sum: three bf16 products, where two fp32
 // operands take six. dx: the parts beside each other, K = 3 Vr through the weight's rows three times. dW: the parts below
-// each other, K = 3 np against the rows' integers three times.
+// each other, K = 3 np against the rows' integers three times. d 2560, V 151,936, both gradients of 512 rows 2,690 us,
+// 4,700 as fp32 products (a library's 6,900).
 struct Grads8Layout {
   int64_t Vr, dp, np, Vp;  // rows and columns of the copies
   int64_t Kh;              // dx's K
@@ -330,7 +349,7 @@ static Grads8Layout grads8_layout(int64_t n, int d, int V, int dtype, bool need_
   return L;
 }
 
-// Whether the products can read g where it lies: 16-bit values in whole 16-byte chunks, a tile's rows and a stage's within
+// Whether the products can read g where it lies (2,048 rows of V 151,936: 2,728 us, 2,850 with a copy): 16-bit values in whole 16-byte chunks, a tile's rows and a stage's within
 // 32-bit offsets.
 static bool g_as_is(const void *g, int64_t ldg, int dtype, int V) {
   return dtype != OCTO_F32 && V % 8 == 0 && V >= TM && ldg % 8 == 0 && ldg <= kMaxV8 && (uintptr_t)g % 16 == 0;

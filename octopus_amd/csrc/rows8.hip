@@ -8,15 +8,15 @@
 // (scale NaN, q 0).
 //
 // Bound by memory: a wave per row, 16-byte loads of 8 values (fp32: two), a row of up to 4,096 values in registers
-// between its maximum and its quotients.
+// between its maximum and its quotients. 32,768 x 2,560 bf16: quantised 48 us (5.3 TB/s; groups of 128 54 to 62), widened
+// 40 us (6.3 TB/s, part of it from the caches); a copy of such rows takes 63.
 #include "octo_internal.h"
 #include "row_values.h"
 #include "rows8.h"
 
 namespace octo {
 
-
-constexpr int64_t kFewHeld = 2048;
+constexpr int64_t kFewHeld = 2048;  // quantise_i8_row_kernel up to here
 
 // GL: lanes of a group (8 values each); 0: the group is the row. Zeros behind the row, up to its next 16 bytes.
 template <int DT, int GL>

@@ -5,8 +5,9 @@
 //   the lowest v whose running sum of r_w = max(p_a(w) - q_a(w), 0) exceeds u_K sum r, and r = p_a after the last draft.
 //
 // Which token that is has to be the definition's, not one beside it: of 150,000 running sums some lie within fp32's
-// rounding of any number, and then another token is answered. So the exponentials and sums are taken in 64 bits (exp64
-// below, 6e-15 relative), and a draw differs from the exact one with a probability of about V times that.
+// rounding of any number, and then another token is answered. So the exponentials and sums are taken in 64 bits
+// (exp2_64 below, 4e-16 relative; some 1e-15 with its argument's rounding), and a draw differs from the exact one with a
+// probability of about V times that.
 //
 // Rows are summed by waves, a part of a row each, in an order that the sizes alone decide. Few logits take three
 // launches, all in 64 bits:
@@ -14,9 +15,13 @@
 //   residual  each workgroup joins its sequence's rows, finds a by itself, and its waves sum their parts' r
 //   pick      a workgroup per sequence finds the part in which the running sum passes u_K sum r, and in it the token
 // Many take the exponentials of stats in 32 bits (64-bit ones are 20 instructions each, and stats is most of the work),
-// which leave each row's sum within 4e-6 (see fast_spread). That decides a draft unless u q and p are closer than 2^-15;
+// which leave each row's sum within 5e-6 (see fast_spread). That decides a draft unless u q and p are closer than 2^-15;
 // then the row and its draft's are summed again in 64 bits there. decide, sums and rest take residual's place: a is found
 // once a sequence, and one sweep over row a of both models finds in 64 bits their sums and those of r (part_sums).
+//
+// Few logits are bound by the launches' latency (one sequence, 4 drafts, V 151,936: 6 + 8 + 6 us), many by memory and by
+// 64-bit arithmetic: 256 sequences of up to 7 drafts, bf16, statistics 181 us for 1.1 GB, sums 80 us for 2 x 39 million
+// exponentials, the other three 33 us.
 #include "octo_common.h"
 #include "row_values.h"
 #include "rows8.h"
@@ -31,9 +36,8 @@ constexpr double kVClose = 1.0 / 32768;
 constexpr double kVLn2 = 0.69314718055994530942;
 
 // 2^t for t <= 0, -inf included (below -1000: 0), within 4e-16 of its value: t = n + f, |f| <= 1/2, n from the last bits
-// of t + 1.5 x 2^52, and 2^f by the polynomial of degree 10 through it at the 11 Chebyshev nodes of [-1/2, 1/2]. No
-// conversion, rounding or ldexp of 64 bits, which take four times an fma's cycles: [256 x 2, 151,936] sums 109 us with
-// them and exp's series, 64 so.
+// of t + 1.5 x 2^52, and 2^f by the polynomial of degree 10 through it at the 11 Chebyshev nodes of [-1/2, 1/2]: 17
+// instructions, no conversion, rounding or ldexp of 64 bits.
 __device__ __forceinline__ double exp2_64(double t) {
   const double shift = 6755399441055744.0, b = t + shift, f = t - (b - shift);
   double e = 7.072585949269223e-09;
@@ -213,8 +217,8 @@ __device__ __forceinline__ PartStat exact_part(const VerifyArgs &a, const typena
 
 // A wave's run of blocks with exponentials in 32 bits, the next block's loads in flight. exp2 is within 2^-23 of its value,
 // and its argument (z - m) c, c rounded to 32 bits, off by at most 1.5 x 2^-23 of itself (d, c and the product), which
-// makes ln 2 times that of the value: over a row at most 2^-23 (1 + 1.04 x 20), as the mean of |d c| under the softmax is
-// at most log2 V. Eight values are summed in 32 bits (3 x 2^-24), all else in 64. Together below 4e-6 of the row's sum.
+// makes ln 2 times that of the value: over a row at most 2^-23 (1 + 1.04 x 30), as the mean of |d c| under the softmax is
+// at most log2 V. Eight values are summed in 32 bits (3 x 2^-24), all else in 64. Together below 5e-6 of the row's sum.
 // A NaN stays one through difference, product and exponential, and +inf makes one (inf - inf): S shows both.
 template <int DT>
 __device__ __forceinline__ PartStat fast_spread(const VerifyArgs &a, const typename Elem<DT>::T *row, int c0, int c1) {
@@ -437,7 +441,8 @@ __device__ __forceinline__ void exact_rows(const VerifyArgs &a, int64_t s, Verif
   if (d.residual == 1) d.q.inv = 1.0 / sum_parts(a.sum_q + s * a.parts, a.parts);
 }
 
-// A row a wave, for up to 8 drafts.
+// A row a wave, for up to 8 drafts: 64 sequences of 4 drafts 6 us. Once a sequence: in sums each of some 20 workgroups
+// would join the same rows.
 constexpr int kVDecide = 1024;
 template <int DT>
 __global__ __launch_bounds__(kVDecide) void verify_decide_kernel(VerifyArgs a) {
@@ -448,8 +453,9 @@ __global__ __launch_bounds__(kVDecide) void verify_decide_kernel(VerifyArgs a) {
 
 // With S_p and S_q the rows' sums, r > 0 where e_p > rho e_q, rho = S_p / S_q, and there r = e_p / S_p - e_q / S_q: one
 // sweep finds the sums of e_p and e_q over all columns and over those, for which it is enough to know rho within 2^-15
-// (the statistics give it within 8e-6), unless a column's e_p lies that close to rho e_q. A part with such a column (one
-// in fifty where the models differ) is left to the next launch.
+// (the statistics give it within 1e-5), unless a column's e_p lies that close to rho e_q. A part with such a column (one
+// in fifty where the models differ) is left to the next launch. 256 sequences of V 151,936: the call 358 us in kernels so,
+// 388 with a sweep for S_p and S_q and another for r.
 template <int DT, int MODE>
 __device__ __forceinline__ void part_sums(const VerifyArgs &a, const VerifyArgs::Decision &d, int64_t s, int k, int c0,
                                           int c1) {
@@ -747,12 +753,16 @@ __global__ __launch_bounds__(kVThreads) void verify_pick_kernel(VerifyArgs a) {
   }
 }
 
-// Parts of one block, and as many blocks more as keep a row within kVParts parts.
+// Parts of one block, and as many blocks more as keep a row within kVParts parts: pick scans a row's parts in the LDS and
+// sweeps one again. A wave that takes several of them in sums measured the same.
 static int part_values(int V) { return (int)round_up(cdiv(V, kVParts), kVBlock); }
 
-// Rows that are summed with 32-bit exponentials, from this many logits on.
+// Rows that are summed with 32-bit exponentials, from this many logits on. V 128,256, 4 drafts with logits, us a call
+// without and with: 9.2M logits 32.3 and 37.0, 18.5M 40.9 and 41.4, 36.9M 56.0 and 50.5, 73.9M 89.5 and 74.5.
 constexpr int64_t kVMany = (int64_t)1 << 24;
-// Waves of their statistics that the parts of up to 8 blocks leave at least.
+// Their statistics by runs of up to 4 parts a wave, whose next loads are in flight during a part's arithmetic and whose
+// reductions across lanes come once, as long as that leaves this many waves. 256 x 9 rows of 151,936 bf16 values, us a
+// call: runs of 2 238, 4 222, 8 225; 512 x 15 rows 545, 519, 529. 256 x 15, statistics alone: runs of 1 240, 8 181.
 constexpr int64_t kVSpread = 16384;
 
 struct VerifyLayout {
@@ -884,7 +894,7 @@ int octo_verify_drafts(const void *logits, int64_t ld_seq, int64_t ld_row, const
   const int64_t rows = S * (a.zd ? 2 * K + 1 : K + 1);
   const bool exact = rows * V < kVMany || !(c >= 0x1p-40 && c <= 0x1p40);
   const int64_t run = exact ? 1 : rows * L.parts / kVSpread;
-  a.spart = L.part * (int)(run < 1 ? 1 : (run > 8 ? 8 : run));
+  a.spart = L.part * (int)(run < 1 ? 1 : (run > 4 ? 4 : run));
   a.sparts = (int)cdiv(V, a.spart);
   switch (dtype) {
     case OCTO_BF16: return go_verify<OCTO_BF16>(a, exact, (hipStream_t)stream);
