@@ -367,7 +367,7 @@ int octo_head_logits_i8(const void *rows, int64_t ldx, int x_dtype, const int8_t
  * times the scale in three bf16 parts (24 bits; a value that bf16 rounds to infinity is one), times the integers,
  * exactly. Summed in fp32 and rounded once. ws: octo_head_grads_i8_workspace_bytes, 256-byte aligned; with room for a
  * copy of g where that is not of 16-bit values, rows of whole 16-byte chunks (V too) and 256 columns or more (g is not
- * read there), for its parts, 6 bytes a value and gradient, where it is F32. */
+ * read there), for its parts, 6 bytes a value and gradient, where it is F32 (up to 128 rows neither for grad_rows). */
 int octo_head_grads_i8_workspace_bytes(const void *g, int64_t ldg, int g_dtype, int64_t n, int d, int V, int need_rows,
                                        int need_w, size_t *bytes);
 int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq, int64_t ldxq, const float *x_scale,

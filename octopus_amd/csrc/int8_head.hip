@@ -10,7 +10,8 @@
 // (without them 2,614; a library product of these integers, which writes 32-bit sums, reaches 1.82).
 //
 // The gradients are 16-bit products of the widened operands (prepare8_kernel: 190 us at that weight, a write of 778 MB), at
-// the rate of the head's other gradients: 2,048 rows 2,480 us for both, 1.29 PFLOP/s.
+// the rate of the head's other gradients: 2,048 rows 2,480 us for both, 1.29 PFLOP/s. The rows' gradient of up to 128 reads
+// the 8-bit weight itself (few_dx_kernel).
 #include <type_traits>
 
 #include "gemm_nt.h"
@@ -276,6 +277,190 @@ template <typename OT> static int go_few(const Few8 &a, int x_dtype, hipStream_t
   }
 }
 
+// ---- few rows' gradient --------------------------------------------------------------------------------------------
+//
+// dx of few rows is the weight's bytes too, which a widened copy multiplies by five. Here a wave takes a share of the
+// vocabulary and 256 columns: lane l holds 16 columns (16 bytes at 16 (l & 15)) of 8 rows (8 (l >> 4) ..) of each 32, so
+// that its 8 bytes of a column are 8 neighbours along K, and product j of 16 takes column j of every lane: widened, rounded
+// to g's type and fed without an exchange between lanes. fp32 g: the integers and g's three parts, as in the large
+// products. A workgroup's waves join their sums in the LDS, a second launch the workgroups', both in order.
+//
+// d 2560, V 151,936, us so and by the widened copy: bf16 8 rows 82 (4.8 TB/s) and 404, 32 88 and 403, 64 144 and 404, 128
+// 269 and 409 (blocks of 32 tokens run side by side and share some of their reads); fp32 8 rows 88 and 687, 128 576 and 767.
+constexpr int kDxCols = 256, kDxWaves = 8;
+constexpr int64_t kFewDx = 128;
+
+struct FewDx {
+  const void *g;
+  int64_t ldg;
+  const int8_t *wq;
+  int64_t ldw;
+  const float *sw;
+  int n, d, V;
+  int strips, groups, share;  // columns / 256; workgroups along the vocabulary; rows of one of their waves (32 k)
+  f32x4 *part;                // [token blocks, strips, groups, 16 NB, 64]
+  void *out;
+  int64_t ldo;
+};
+
+template <int DT, int NB>
+__global__ __launch_bounds__(64 * kDxWaves) void few_dx_kernel(FewDx a) {
+  constexpr bool F32 = DT == OCTO_F32;
+  constexpr int WT = F32 ? OCTO_BF16 : DT, NP = F32 ? 3 : 1, R = 16 * NB;
+  typedef typename Elem<DT>::T T;
+  __shared__ f32x4 smem[kDxWaves / 2][R][64];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qd = lane >> 4;
+  const int strip = blockIdx.x % a.strips, group = blockIdx.x / a.strips;
+  const int c = strip * kDxCols + 16 * (lane & 15);
+  const int first = (group * kDxWaves + w) * a.share, last = min(first + a.share, a.V);
+  const int8_t *col = a.wq + (c < a.d ? c : 0);
+  const T *grow[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+    grow[b] = (const T *)a.g + min((int)blockIdx.y * 16 * NB + 16 * b + (lane & 15), a.n - 1) * a.ldg;
+  f32x4 acc[NB][16];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  struct Step {
+    i32x4 q[8];
+    Raw8<DT> g[NB];
+    float s[8];
+  };
+  // rows past the share's end: its last one, times the zeros of g there
+  auto load = [&](Step &t, int v0) {
+    const int v = v0 + 8 * qd;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t r = min(v + e, last - 1);
+      t.q[e] = *(const i32x4 *)(col + r * a.ldw);
+      t.s[e] = a.sw[r];
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      t.g[b] = v0 + 32 <= last ? load_raw8<DT>(grow[b] + v) : load_raw8<DT>(grow[b] + v, last - v);
+  };
+  auto take = [&](const Step &t) {
+    i32x4 gop[NB][NP];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      if constexpr (F32) {
+        float x[8];
+        values8<DT>(t.g[b], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= t.s[e];
+        split_parts(x, gop[b]);
+      } else {
+        gop[b][0] = t.g[b].v[0];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = (float)(int8_t)((uint32_t)t.q[e][j >> 2] >> (8 * (j & 3)));
+        if constexpr (!F32) x[e] *= t.s[e];
+      }
+      const i32x4 op = pack8(x, WT == OCTO_F16);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) Mfma16<WT>::run(op, gop[b][p], acc[b][j]);
+    }
+  };
+  if (first < last) {
+    Step t[2];
+    load(t[0], first);
+    for (int v = first;;) {
+      if (v + 32 < last) load(t[1], v + 32);
+      take(t[0]);
+      if ((v += 32) >= last) break;
+      if (v + 32 < last) load(t[0], v + 32);
+      take(t[1]);
+      if ((v += 32) >= last) break;
+    }
+  }
+#pragma unroll
+  for (int half = kDxWaves / 2; half > 0; half >>= 1) {
+    if (w >= half && w < 2 * half) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) smem[w - half][r][lane] = acc[r >> 4][r & 15];
+    }
+    __syncthreads();
+    if (w < half) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) acc[r >> 4][r & 15] += smem[w][r][lane];
+    }
+    __syncthreads();
+  }
+  if (w == 0) {
+    f32x4 *out = a.part + (((int64_t)blockIdx.y * a.strips + strip) * a.groups + group) * R * 64;
+#pragma unroll
+    for (int r = 0; r < R; ++r) out[r * 64 + lane] = acc[r >> 4][r & 15];
+  }
+}
+
+// The workgroups' sums joined: register r = 16 b + j of lane l holds token 16 b + (l & 15), columns 64 (l >> 4) + 16 e + j.
+template <typename OT, int NB>
+__global__ __launch_bounds__(256) void few_dx_sum_kernel(FewDx a) {
+  constexpr int R = 16 * NB;
+  const int strip = blockIdx.x / (R / 4), r = blockIdx.x % (R / 4) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const f32x4 *p = a.part + ((int64_t)blockIdx.y * a.strips + strip) * a.groups * R * 64 + r * 64 + lane;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int k = 0; k < a.groups; ++k) sum += p[(int64_t)k * R * 64];
+  const int t = (int)blockIdx.y * 16 * NB + (r & ~15) + (lane & 15);
+  const int c = strip * kDxCols + 64 * (lane >> 4) + (r & 15);
+  if (t >= a.n) return;
+  OT *out = (OT *)a.out + t * a.ldo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + 16 * e < a.d) out[c + 16 * e] = (OT)sum[e];
+}
+
+struct DxSplit {
+  int nb, blocks, strips, groups, share;
+  size_t bytes;
+};
+// A workgroup a CU (its registers fill one).
+static DxSplit dx_split(int64_t n, int d, int V, int dtype) {
+  DxSplit s;
+  s.nb = n <= 16 || dtype == OCTO_F32 ? 1 : 2;  // fp32's parts of 32 rows do not fit the registers
+  s.blocks = (int)cdiv(n, 16 * s.nb);
+  s.strips = (int)cdiv(d, kDxCols);
+  const int64_t most = cdiv(V, 32 * kDxWaves), want = octo_tiles::kCus / ((int64_t)s.strips * s.blocks);
+  const int64_t groups = want < 1 ? 1 : (want < most ? want : most);
+  s.share = (int)round_up(cdiv(V, groups * kDxWaves), 32);
+  s.groups = (int)cdiv(V, (int64_t)s.share * kDxWaves);
+  s.bytes = (size_t)s.blocks * s.strips * s.groups * 16 * s.nb * 64 * sizeof(f32x4);
+  return s;
+}
+
+template <int DT, int NB> static int go_few_dx(const FewDx &a, const DxSplit &s, int out_dtype, hipStream_t st) {
+  hipLaunchKernelGGL((few_dx_kernel<DT, NB>), dim3((unsigned)(s.strips * s.groups), (unsigned)s.blocks),
+                     dim3(64 * kDxWaves), 0, st, a);
+  OCTO_CHECK_LAUNCH("few_dx");
+  const dim3 grid((unsigned)(s.strips * 4 * NB), (unsigned)s.blocks);
+  switch (out_dtype) {
+    case OCTO_BF16: hipLaunchKernelGGL((few_dx_sum_kernel<__bf16, NB>), grid, dim3(256), 0, st, a); break;
+    case OCTO_F16: hipLaunchKernelGGL((few_dx_sum_kernel<_Float16, NB>), grid, dim3(256), 0, st, a); break;
+    default: hipLaunchKernelGGL((few_dx_sum_kernel<float, NB>), grid, dim3(256), 0, st, a); break;
+  }
+  OCTO_CHECK_LAUNCH("few_dx_sum");
+  return OCTO_OK;
+}
+static int go_few_dx(const FewDx &a, const DxSplit &s, int dtype, int out_dtype, hipStream_t st) {
+  switch (dtype) {
+    case OCTO_BF16:
+      return s.nb == 1 ? go_few_dx<OCTO_BF16, 1>(a, s, out_dtype, st) : go_few_dx<OCTO_BF16, 2>(a, s, out_dtype, st);
+    case OCTO_F16:
+      return s.nb == 1 ? go_few_dx<OCTO_F16, 1>(a, s, out_dtype, st) : go_few_dx<OCTO_F16, 2>(a, s, out_dtype, st);
+    default: return go_few_dx<OCTO_F32, 1>(a, s, out_dtype, st);
+  }
+}
+
 static Operand operand8(const void *base, int64_t ld_bytes, int64_t rows) {
   Operand X;
   X.base = (const char *)base;
@@ -316,6 +501,7 @@ struct Grads8Layout {
   int parts;               // of g
   size_t wide, xt, g, gh, split, total;
   int64_t split_items;
+  bool few;  // dx by few_dx_kernel, its partial sums in split
 };
 
 static Grads8Layout grads8_layout(int64_t n, int d, int V, int dtype, bool need_rows, bool need_w, bool as_is) {
@@ -333,6 +519,8 @@ static Grads8Layout grads8_layout(int64_t n, int d, int V, int dtype, bool need_
     return p;
   };
   L.split_items = 0;
+  L.few = need_rows && n <= kFewDx;
+  if (L.few) need_rows = false;  // none of the copies for it
   if (need_rows) {
     const int64_t tiles = cdiv(n, TM) * cdiv(d, TN);
     if (tiles < octo_tiles::kSplitItemsMax) {
@@ -342,9 +530,9 @@ static Grads8Layout grads8_layout(int64_t n, int d, int V, int dtype, bool need_
   }
   L.wide = take(need_rows ? (size_t)L.Vr * L.dp * 2 : 0);
   L.xt = take(need_w ? (size_t)d * L.parts * L.np * 2 : 0);
-  L.g = take(L.parts == 1 ? (as_is ? 0 : (size_t)L.np * L.Vp * 2) : (need_w ? (size_t)3 * L.np * L.Vp * 2 : 0));
+  L.g = take(L.parts == 1 ? (as_is || !(need_rows || need_w) ? 0 : (size_t)L.np * L.Vp * 2) : (need_w ? (size_t)3 * L.np * L.Vp * 2 : 0));
   L.gh = take(L.parts == 3 && need_rows ? (size_t)n * L.Kh * 2 : 0);
-  L.split = take((size_t)L.split_items * TM * TN * 4);
+  L.split = take(L.few ? dx_split(n, d, V, dtype).bytes : (size_t)L.split_items * TM * TN * 4);
   L.total = at;
   return L;
 }
@@ -456,7 +644,8 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
   p.wq = wq;
   p.ldw = ldw;
   p.ws = w_scale;
-  p.wide = grad_rows ? wsb + L.wide : nullptr;
+  const bool wide = grad_rows && !L.few;
+  p.wide = wide ? wsb + L.wide : nullptr;
   p.Vr = L.Vr;
   p.dp = (int)L.dp;
   p.xq = xq;
@@ -466,8 +655,8 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
   p.ldt = L.parts * L.np;
   p.g = g;
   p.ldg = ldg;
-  p.gs = as_is || (f32 && !grad_w) ? nullptr : wsb + L.g;
-  p.gh = f32 && grad_rows ? wsb + L.gh : nullptr;
+  p.gs = as_is || (!grad_w && (f32 || !wide)) ? nullptr : wsb + L.g;
+  p.gh = f32 && wide ? wsb + L.gh : nullptr;
   p.np = L.np;
   p.Vp = L.Vp;
   p.n = n;
@@ -475,6 +664,13 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
   p.V = V;
   rc = launch_prepare8(p, g_dtype, st);
   if (rc) return rc;
+  if (L.few) {
+    const DxSplit s = dx_split(n, d, V, g_dtype);
+    const FewDx a{g, ldg, wq, ldw, w_scale, (int)n, d, V, s.strips, s.groups, s.share, (f32x4 *)(wsb + L.split), grad_rows,
+                  ld_gr};
+    rc = go_few_dx(a, s, g_dtype, gr_dtype, st);
+    if (rc) return rc;
+  }
 
   const int dt = f32 ? OCTO_BF16 : g_dtype;
   const char *gs = as_is ? (const char *)g : wsb + L.g;
@@ -487,7 +683,7 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
   const Operand Bw = operand8(wsb + L.xt, L.parts * L.np * 2, d);
   const int kma = as_is ? KM_EDGE : KM_A;
   if (as_is) Aw.extent = (uint32_t)V;
-  if (grad_rows) {
+  if (wide) {
     oh.C = grad_rows;
     oh.ldc = ld_gr;
     oh.dtype = gr_dtype;
@@ -505,10 +701,10 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
   // Both in one launch, dx's runs as long as if it had the card to itself: dW's short tiles follow them on every CU. Two
   // launches take 20 us more up to 700 rows of d 2560, V 151,936 and as long from 1,024 on; runs cut for sharing the card
   // (fewer, longer ones) 949 us for 300 rows against 835.
-  const bool both = grad_rows && grad_w && !f32;
+  const bool both = wide && grad_w && !f32;
   if (both) rc = launch_gemm_grads(dt, Ah, Bh, sh, oh, true, Aw, Bw, sw, ow, st, kma);
-  else if (grad_rows) rc = launch_gemm_store(dt, Ah, Bh, sh, oh, st, f32 ? KM_WRAP : KM_B);
-  if (!rc && grad_rows) rc = launch_split_sum(sh, oh, false, st);
+  else if (wide) rc = launch_gemm_store(dt, Ah, Bh, sh, oh, st, f32 ? KM_WRAP : KM_B);
+  if (!rc && wide) rc = launch_split_sum(sh, oh, false, st);
   if (!rc && grad_w && !both) rc = launch_gemm_store(dt, Aw, Bw, sw, ow, st, kma);
   return rc;
 }

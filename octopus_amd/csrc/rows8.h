@@ -122,4 +122,20 @@ __device__ __forceinline__ float quantise_row(const typename Elem<DT>::T *row, i
   return s;
 }
 
+// 8 fp32 values as three bf16 parts each, whose sum they are (24 bits; one that bf16 cannot hold stays in the first part
+// alone).
+__device__ __forceinline__ void split_parts(const float (&x)[8], i32x4 (&part)[3]) {
+  float p0[8], p1[8], p2[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    p0[e] = (float)(__bf16)x[e];
+    const bool fine = fabsf(p0[e]) < INFINITY;
+    p1[e] = fine ? (float)(__bf16)(x[e] - p0[e]) : 0.f;
+    p2[e] = fine ? x[e] - p0[e] - p1[e] : 0.f;
+  }
+  part[0] = pack8(p0, false);
+  part[1] = pack8(p1, false);
+  part[2] = pack8(p2, false);
+}
+
 }  // namespace octo

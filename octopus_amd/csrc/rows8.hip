@@ -208,21 +208,7 @@ __device__ __forceinline__ void stage_part(const Prepare8 &a, int64_t r, int par
   }
 }
 
-// fp32 g: 8 values of a row times their weights' scales, and times the row's, each as three bf16 parts whose sum it is
-// (24 bits; what bf16 cannot hold stays in the first part alone).
-__device__ __forceinline__ void split_parts(const float (&x)[8], i32x4 (&part)[3]) {
-  float p0[8], p1[8], p2[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    p0[e] = (float)(__bf16)x[e];
-    const bool fine = fabsf(p0[e]) < INFINITY;
-    p1[e] = fine ? (float)(__bf16)(x[e] - p0[e]) : 0.f;
-    p2[e] = fine ? x[e] - p0[e] - p1[e] : 0.f;
-  }
-  part[0] = pack8(p0, false);
-  part[1] = pack8(p1, false);
-  part[2] = pack8(p2, false);
-}
+// fp32 g: 8 values of a row times their weights' scales, and times the row's, in three parts each.
 __device__ __forceinline__ void stage_f32(const Prepare8 &a, int64_t r, int part) {
   const int c = (part * 256 + (int)threadIdx.x) * 8;
   float x[8], y[8];

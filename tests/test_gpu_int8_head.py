@@ -120,6 +120,27 @@ def test_gradients(n, d, V, dtype):
             assert got[0].dtype == dtype and ((got[0].cpu().double() - gw).abs() <= bound_w).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d,V", [(1, 1, 1), (1, 300, 31), (2, 17, 5000), (15, 513, 33), (16, 256, 256), (17, 255, 20011),
+                                   (31, 1027, 515), (32, 2560, 3001), (33, 40, 700), (128, 72, 300), (129, 300, 1000),
+                                   (150, 96, 4001)])
+def test_gradients_of_few_rows(n, d, V, dtype):
+    """g off every 16-byte boundary, with no numbers around its rows; weights whose padding is not zeros."""
+    x, w = _inputs(n, d, V, dtype, n + V)
+    wq, ws = int8_op.quantise_rows(w.to(DEV))
+    full = torch.full((V, wq.stride(0) if V > 1 else -(-d // 16) * 16), 77, dtype=torch.int8, device=DEV)
+    full[:, :d] = wq
+    store = torch.full((n, V + 7), float("nan"), dtype=dtype, device=DEV)
+    g = (torch.randn(n, V, generator=torch.Generator().manual_seed(7)) / 8).to(dtype)
+    store[:, 3:V + 3] = g.to(DEV)
+    gr, gw, bound_r, bound_w = _bound_grads(g, x, wq, ws, dtype, dtype)
+    xd, wd = x.to(DEV).requires_grad_(True), w.to(DEV).requires_grad_(True)
+    alone, = torch.autograd.grad(int8_op.int8_head(xd, full[:, :d], ws), xd, store[:, 3:V + 3])
+    rows, weight = torch.autograd.grad(int8_op.int8_head(xd, full[:, :d], ws, weight=wd), (xd, wd), store[:, 3:V + 3])
+    assert torch.equal(alone, rows) and ((rows.cpu().double() - gr).abs() <= bound_r).all()
+    assert ((weight.cpu().double() - gw).abs() <= bound_w).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_gradients_of_strided_and_broadcast_g(dtype):
     n, d, V = 37, 48, 130
