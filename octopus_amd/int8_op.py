@@ -28,6 +28,7 @@ from .embed_op import _FLOATS, _call_on, _float_rows, _ld, _on_gpu
 from .head_op import _DT, _p, _workspace
 
 GROUPS = (0, 32, 64, 128, 256)
+_F32_GRADS_MAX = 1 << 20  # rows and columns of fp32 gradients: three parts of each within the products' 32-bit offsets
 
 
 def _ld8(d: int) -> int:
@@ -324,8 +325,14 @@ def int8_head(rows: Tensor, wq: Tensor, w_scale: Tensor, *, weight: Optional[Ten
     place, the backward raises). wq and w_scale get no gradient; the gradients have no derivative of their own (one
     raises)."""
     out_dtype = out_dtype or rows.dtype
+    train = torch.is_grad_enabled() and (rows.requires_grad or weight is not None and weight.requires_grad)
+    if train and out_dtype == torch.float32 and wq.dim() == 2:
+        V, d = wq.shape
+        n = rows.numel() // max(d, 1)
+        if max(n, V) > _F32_GRADS_MAX:
+            raise ValueError(f"octohead: fp32 logits [{n}, {V}] have gradients up to {_F32_GRADS_MAX} rows and columns")
     if torch.compiler.is_compiling():
         return head_logits_i8(rows, wq, w_scale, weight, out_dtype)[0]
-    if torch.is_grad_enabled() and (rows.requires_grad or weight is not None and weight.requires_grad):
+    if train:
         return _Head8.apply(rows, wq, w_scale, weight, out_dtype)
     return _logits(rows, wq, w_scale, weight, out_dtype)[0]

@@ -97,6 +97,14 @@ def test_cpu_tensors_are_refused():
         int8_op.quantise_rows(x, 7)
 
 
+def test_fp32_gradients_too_large_are_refused_before_the_forward():
+    big = (1 << 20) + 1
+    wq, ws = torch.zeros(1, 4, dtype=torch.int8).expand(big, 4), torch.ones(1).expand(big)
+    for x, q, s in ((torch.zeros(1, 4), wq, ws), (torch.zeros(1, 4).expand(big, 4), wq[:3], ws[:3])):
+        with pytest.raises(ValueError, match="fp32 logits"):
+            int8_op.int8_head(x.detach().requires_grad_(True), q, s)
+
+
 def test_checkpoint8_keeps_cpu_tensors():
     """CPU tensors are checkpointed as they are, so the seq tiles' CPU tests read the same inside held8()."""
     from octopus_amd.rl import seq_tiles
