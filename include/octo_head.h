@@ -386,8 +386,9 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
  * Probabilities and sums in 64 bits. greedy: a draft is accepted when it is its row's first largest logit, which is also
  * the next token; u and the draft logits are not read (may be NULL). A draft outside [0, V), or whose logits' row has no
  * softmax (a NaN, +inf, or nothing above -inf), is rejected and the token drawn from p_a; where p_a has none, the token
- * is -1 and its logp NaN. A u_K that is no number below 1 takes the last v with r_v > 0. Rows behind a sequence's length are not read. K <= OCTO_DRAFTS_MAX, S <=
- * 2^20. Rows may start at any element. ws: octo_verify_workspace_bytes, 16-byte aligned. */
+ * is -1 and its logp NaN. A u_K that is no number below 1 takes the last v with r_v > 0. Rows behind a sequence's length
+ * are not read. K <= OCTO_DRAFTS_MAX, S <= 2^20. Rows may start at any element. ws: octo_verify_workspace_bytes, 16-byte
+ * aligned. */
 int octo_verify_workspace_bytes(int64_t S, int K, int V, size_t *bytes);
 int octo_verify_drafts(const void *logits, int64_t ld_seq, int64_t ld_row, const void *draft_logits, int64_t ld_seq_d,
                        int64_t ld_row_d, int dtype, const int64_t *drafts, const int64_t *lengths, const float *uniform,

@@ -373,7 +373,10 @@ __device__ __forceinline__ void ring5_stage(const OA &opa, const OB &opb, int kd
   static_assert(QX > 0 && D0 + (OA::NI - 1) * DSA < NQ && D0 + (OB::NI - 1) * DSB < NQ, "all within the K-step");
   constexpr int XQ = SPLIT ? QX : 0;  // first MFMA under which stage k + 1's fragments are read
   // slots: stage k at (sa, sa + 1), stage k + 1 at (sa + 2, sa + 3), stage k + 2's A at sa + 4, its B at sa
-  auto slot = [&](int d) -> lds_char * { const int x = sa + d; return smem + (x >= ENSLOT ? x - ENSLOT : x) * ring5_slot<OA, OB>(); };
+  auto slot = [&](int d) -> lds_char * {
+    const int x = sa + d;
+    return smem + (x >= ENSLOT ? x - ENSLOT : x) * ring5_slot<OA, OB>();
+  };
   const lds_char *cA = slot(0), *cB = slot(1);
   const lds_char *nA = slot(2), *nB = slot(3);
   lds_char *dA = slot(4), *dB = slot(0);
@@ -454,7 +457,8 @@ __device__ __forceinline__ void ring5_prologue(const OA &opa, const OB &opb, int
 // The ring loop after its prologue, stage j of the tile in slots (sa0 + 2 j, sa0 + 2 j + 1) mod 5; acc is zeroed
 // here. Ends with every DMA landed and every wave past its last LDS read (the slots are free), and returns the slot
 // that continues the ring, (sa0 + 2 nk) mod 5. VMEM instructions issued after the prologue's (a previous tile's
-// epilogue stores) are fine: loads complete in order among themselves, so at most a stage's instructions outstanding means stage 0 in.
+// epilogue stores) are fine: loads complete in order among themselves, so at most a stage's instructions outstanding
+// means stage 0 in.
 template <int DT, typename OA, typename OB, bool SPLIT, bool TR>
 __device__ __forceinline__ int ring5_run(const OA &opa, const OB &opb, int sa0, uint32_t kbytes, int nk,
                                          lds_char *smem, f32x4 (&acc)[OA::NB][OB::NB]) {

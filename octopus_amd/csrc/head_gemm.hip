@@ -856,7 +856,8 @@ int launch_gemm_store(int dt, const Operand &A, const Operand &B, const GemmShap
   if (e.split && (kmajor == KM_A || kmajor == KM_EDGE || e.pass_count))
     return octo_fail(OCTO_EUNSUPPORTED, "gemm_store: split K of this product");
   if (kmajor == KM_WRAP) {
-    if (!kmajor_layout_ok(B) || dt != OCTO_BF16 || B.rows % 64 || B.rows <= 0 || s.K > 3 * B.rows || B.count_off || B.count)
+    if (!kmajor_layout_ok(B) || dt != OCTO_BF16 || B.rows % 64 || B.rows <= 0 || s.K > 3 * B.rows || B.count_off ||
+        B.count)
       return octo_fail(OCTO_EINVAL, "gemm_store: wrapped operand layout");
     return go_store<OCTO_BF16, KM_WRAP>(A, B, s, e, st);
   }

@@ -98,8 +98,7 @@ __device__ __forceinline__ void unpack_i8(const i32x2 v, float s, float (&x)[8])
 
 // Row r of out = q scale for the columns c < d, zeros up to cols_pad (and for all of a row past `rows`), by one wave, 4
 // chunks of 8 columns a lane in flight. gshift: log2 of the group, or -1. The bytes of q behind d are readable up to the
-// next multiple of 16.
-// UNIT: the integers themselves (exact in every type).
+// next multiple of 16. UNIT: the integers themselves (exact in every type).
 template <int DT, bool UNIT = false>
 __device__ __forceinline__ void widen_row(const int8_t *q, const float *scale, bool there, int d, int gshift,
                                           typename Elem<DT>::T *out, int cols_pad) {
@@ -338,10 +337,13 @@ int octo_quantise_i8_rows(const void *x, int64_t ldx, int x_dtype, int64_t rows,
   for (int64_t r0 = 0; r0 < rows; r0 += kLaunchRows) {
     const int64_t n = rows - r0 < kLaunchRows ? rows - r0 : kLaunchRows;
     const char *xr = (const char *)x + r0 * ldx * float_bytes(x_dtype);
+    int8_t *qr = q + r0 * ldq;
+    float *sr = scale + r0 * groups;
+    hipStream_t st = (hipStream_t)stream;
     switch (x_dtype) {
-      case OCTO_BF16: go_quantise<OCTO_BF16>(xr, ldx, n, d, group, q + r0 * ldq, ldq, scale + r0 * groups, (hipStream_t)stream); break;
-      case OCTO_F16: go_quantise<OCTO_F16>(xr, ldx, n, d, group, q + r0 * ldq, ldq, scale + r0 * groups, (hipStream_t)stream); break;
-      default: go_quantise<OCTO_F32>(xr, ldx, n, d, group, q + r0 * ldq, ldq, scale + r0 * groups, (hipStream_t)stream); break;
+      case OCTO_BF16: go_quantise<OCTO_BF16>(xr, ldx, n, d, group, qr, ldq, sr, st); break;
+      case OCTO_F16: go_quantise<OCTO_F16>(xr, ldx, n, d, group, qr, ldq, sr, st); break;
+      default: go_quantise<OCTO_F32>(xr, ldx, n, d, group, qr, ldq, sr, st); break;
     }
     OCTO_CHECK_LAUNCH("quantise_i8");
   }
@@ -360,10 +362,13 @@ int octo_widen_i8_rows(const int8_t *q, int64_t ldq, const float *scale, int64_t
   for (int64_t r0 = 0; r0 < rows; r0 += kLaunchRows) {
     const int64_t n = rows - r0 < kLaunchRows ? rows - r0 : kLaunchRows;
     char *o = (char *)out + r0 * ldo * float_bytes(out_dtype);
+    const int8_t *qr = q + r0 * ldq;
+    const float *sr = scale + r0 * groups;
+    hipStream_t st = (hipStream_t)stream;
     switch (out_dtype) {
-      case OCTO_BF16: go_widen<OCTO_BF16>(q + r0 * ldq, ldq, scale + r0 * groups, n, d, group, o, ldo, (hipStream_t)stream); break;
-      case OCTO_F16: go_widen<OCTO_F16>(q + r0 * ldq, ldq, scale + r0 * groups, n, d, group, o, ldo, (hipStream_t)stream); break;
-      default: go_widen<OCTO_F32>(q + r0 * ldq, ldq, scale + r0 * groups, n, d, group, o, ldo, (hipStream_t)stream); break;
+      case OCTO_BF16: go_widen<OCTO_BF16>(qr, ldq, sr, n, d, group, o, ldo, st); break;
+      case OCTO_F16: go_widen<OCTO_F16>(qr, ldq, sr, n, d, group, o, ldo, st); break;
+      default: go_widen<OCTO_F32>(qr, ldq, sr, n, d, group, o, ldo, st); break;
     }
     OCTO_CHECK_LAUNCH("widen_i8");
   }

@@ -409,7 +409,8 @@ __device__ void decide(const VerifyArgs &a, int64_t s, bool write, VerifyArgs::D
     const int i = again;
     if (EXACT || i < 0) break;
     const double inv_p = exact_inv<DT, NW>(a, row_of<DT>(a.z, a.ls, a.lr, s, i), rows[i].m, red);
-    const double inv_q = a.zd ? exact_inv<DT, NW>(a, row_of<DT>(a.zd, a.ls_d, a.lr_d, s, i), rows[a.K + 1 + i].m, red) : 0.0;
+    double inv_q = 0.0;
+    if (a.zd) inv_q = exact_inv<DT, NW>(a, row_of<DT>(a.zd, a.ls_d, a.lr_d, s, i), rows[a.K + 1 + i].m, red);
     __syncthreads();
     if (threadIdx.x == 0) {
       rows[i].inv = inv_p;

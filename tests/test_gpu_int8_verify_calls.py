@@ -319,6 +319,29 @@ def test_far_offsets():
     assert (q[:-1] == 127).all() and torch.equal(back[-1], x[-1]) and torch.equal(back[-2], x[-2])
 
 
+def test_gradients_over_far_offsets():
+    """Weights of more than 2^31 bytes and gradients of more than 2^31 values: the first and the last rows alone."""
+    V, d = (1 << 21) - 8, 1040
+    wq = torch.zeros(V, d, dtype=torch.int8, device=DEV)
+    wq[-1], wq[-2, 7], wq[0, 3] = 3, 100, -5
+    ws = torch.full((V,), 0.5, device=DEV)
+    for n in (3, 40, 1100):
+        g = torch.zeros(n, V, dtype=torch.bfloat16, device=DEV)
+        g[0, 0], g[-1, -1], g[-1, -2] = 2, 4, 8
+        x = torch.ones(n, d, dtype=torch.bfloat16, device=DEV)
+        xq, xs = int8_op.quantise_rows(x)
+        rows, weight = int8_op._grads(g, xq, xs, wq, ws, torch.float32, torch.bfloat16, True, n == 40)
+        want = torch.zeros(n, d, device=DEV)
+        want[0, 3] = -5.0
+        want[-1] = 6.0
+        want[-1, 7] += 400.0
+        assert torch.equal(rows, want)
+        if weight is not None:
+            assert (weight[0] == 2).all() and (weight[-1] == 4).all() and (weight[-2] == 8).all()
+            assert not weight[1:-2].any()
+        del g, weight
+
+
 def test_verify_far_offsets():
     S, K, V = 700, 7, 400000  # 2.2e9 logits
     g = torch.Generator(device=DEV).manual_seed(2)
