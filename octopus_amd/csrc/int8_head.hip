@@ -5,9 +5,10 @@
 //   dW[v, k] = sum_r g[r, v] sx[r] qx[r, k]
 //
 // Three routes for the logits, by the rows. Up to 32 read the weight's bytes once and are bound by them (few_i8_kernel: 1
-// row of d 2560, V 151,936 74 us, 5.2 TB/s). Up to 128 the same in tiles, two workgroups a CU (64 rows 95 us, 4.3 TB/s with
-// the logits). More are bound by the matrix rate: 8,192 rows 2,740 us, 2.33 POP/s with the logits' 2.5 GB written beside it
-// (without them 2,614; a library product of these integers, which writes 32-bit sums, reaches 1.82).
+// row of d 2560, V 151,936 74 us, 5.2 TB/s). Up to 128, and more of a small vocabulary, the same in tiles, two workgroups a
+// CU (64 rows 95 us, 4.3 TB/s with the logits). More are bound by the matrix rate: 8,192 rows 2,740 us, 2.33 POP/s with the
+// logits' 2.5 GB written beside it (without them 2,614; a library product of these integers, which writes 32-bit sums,
+// reaches 1.82).
 //
 // The gradients are 16-bit products of the widened operands (prepare8_kernel: 190 us at that weight, a write of 778 MB), at
 // the rate of the head's other gradients: 2,048 rows 2,480 us for both, 1.29 PFLOP/s. The rows' gradient of up to 128 reads
@@ -27,9 +28,14 @@ constexpr int64_t kMaxN8 = 1 << 21;  // the same of the transposed rows
 // M-tiles that an XCD walks the tokens with: 2,048 rows at d 2560, V 151,936 795 us in fours, 749 in eights, the same in
 // sixteens, more in thirty-twos.
 constexpr int kGroup8 = 8;
-// Up to here tiles of 128 x 128. The same weight, us with them and with wide ones: 64 rows 95 and 118, 128 104 and 119,
-// 192 147 and 126, 256 157 and 133. (Eight waves on the small tile: 128 rows 111.)
+// Tiles of 128 x 128 up to this many rows. The same weight, us with them and with wide ones: 64 rows 95 and 118, 128 104
+// and 119, 192 147 and 126, 256 157 and 133. (Eight waves on the small tile: 128 rows 111.) And where the card holds all of
+// them at once, two a CU: 256 rows of d 1024 V 32,000 20.0 and 22.8, 512 of V 16,000 19.9 and 27.3, 256 of d 4096 V 32,000
+// 41.6 and 46.1; beyond, 512 of V 32,000 31.2 and 27.7, 256 of d 2304 V 64,000 48.8 and 43.2.
 constexpr int64_t kSmallRows = 128;
+static bool small_tiles(int64_t n, int V) {
+  return n <= kSmallRows || cdiv(n, 128) * cdiv(V, 128) <= 2 * octo_tiles::kCus;
+}
 
 typedef i32x4 i32x4_el __attribute__((aligned(2)));
 typedef i32x4 i32x4_el4 __attribute__((aligned(4)));
@@ -588,7 +594,7 @@ int octo_head_logits_i8(const void *rows, int64_t ldx, int x_dtype, const int8_t
   }
   const Logits8 e{x_scale, w_scale, logits, ldz};
   const Operand A = operand8(wq, ldw, V), B = operand8(xq, ldxq, n);
-  const bool small = n <= kSmallRows;
+  const bool small = small_tiles(n, V);
   const GemmShape s = shape8(V, n, round_up(d, 16), small ? 128 : 256);
   const dim3 grid((unsigned)tile_grid(s.mtiles, s.ntiles)), block(small ? 256 : 512);
 #define OCTO_GO(OT)                                                                                \

@@ -45,6 +45,17 @@ def test_logits(n, d, V, dtype):
     _check_logits(int8_op.int8_head(x.to(DEV), wq, ws), x, wq, ws, dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d,V", [(129, 70, 33001), (192, 144, 33000), (193, 65, 33024), (256, 16, 32897), (257, 130, 22016),
+                                   (300, 97, 22017), (385, 64, 17153), (449, 200, 17000), (600, 100, 14001),
+                                   (1025, 48, 8000)])
+def test_logits_of_wide_tiles(n, d, V, dtype):
+    """More rows than 128 and more tiles of 128 x 128 than the card holds: tiles of 256 x 256 and narrower last ones."""
+    x, w = _inputs(n, d, V, dtype, n + d)
+    wq, ws = int8_op.quantise_rows(w.to(DEV))
+    _check_logits(int8_op.int8_head(x.to(DEV), wq, ws), x, wq, ws, dtype)
+
+
 @pytest.mark.parametrize("out", TYPES)
 def test_other_types_and_shapes(out):
     x, w = _inputs(60, 72, 400, torch.bfloat16)
