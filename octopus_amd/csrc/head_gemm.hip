@@ -429,6 +429,38 @@ __device__ __forceinline__ void store_any(const typename L::V (&acc)[L::NI][L::N
   store_tile<L, OT>(acc, e, m0, n0, mvalid, nvalid, smem);
 }
 
+// A whole-width fp32 tile with nothing to add: store_tile's halves, values and slots, out 16 bytes per lane. grad_W of 8
+// rows of d 2560, V 151,936 (1.56 GB) 352 us, 520 value by value.
+template <class L>
+__device__ __forceinline__ void store_staged4(const typename L::V (&acc)[L::NI][L::NJ], const StoreArgs &e, int64_t m0,
+                                              int64_t n0, int64_t mvalid, lds_char *smem) {
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = L::wm(w), wn = L::wn(w);
+  const float alpha = e.alpha ? *e.alpha : 1.f;
+  for (int half = 0; half < 2; ++half) {
+    if (half) __syncthreads();  // the first half's reads are done
+    if (wm == half) {
+#pragma unroll
+      for (int i = 0; i < L::NI; ++i)
+#pragma unroll
+        for (int j = 0; j < L::NJ; ++j) {
+          const int r = L::row(0, i, lane);
+          *(lds_f32x4 *)(smem + r * (TN * 4) + (((L::col(wn, j, lane) >> 2) ^ (r & 15)) << 4)) = acc[i][j];
+        }
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int r = w; r < 128; r += 8) {
+      const int64_t row = m0 + half * 128 + r;
+      if (half * 128 + r >= mvalid) break;
+      const float sc = e.row_scale ? e.row_scale[row] * alpha : alpha;
+      f32x4 x = *(const lds_f32x4 *)(smem + r * (TN * 4) + ((lane ^ (r & 15)) << 4));
+#pragma unroll
+      for (int v = 0; v < 4; ++v) x[v] *= sc;
+      __builtin_nontemporal_store(x, (f32x4 *)((float *)e.C + row * e.ldc + n0 + 4 * lane));
+    }
+  }
+}
+
 // The tile's fp32 partials in the blocked layout (StoreArgs::part_blocked): this wave's 8192 values, element v of
 // block (i, j) of lane l at ((i NJ + j) NV + v) 64 + l, stored or added (no-return atomics).
 template <class L>
@@ -531,6 +563,12 @@ __device__ __forceinline__ void store8_tile(const Operand &A, const Operand &B, 
   if (e.part_blocked && which == 1 && e.addend) {  // the blocked partials added here, C stored as usual
     add_blocked<L>(acc, e.addend, e.ldc, m0, n0);
     eb.addend = nullptr;
+  }
+  if constexpr (OT == OCTO_F32) {
+    if (which == 1 && (uintptr_t)e.C % 16 == 0 && e.ldc % 4 == 0 && !eb.addend && !e.accumulate && nvalid >= TN) {
+      store_staged4<L>(acc, eb, m0, n0, mvalid, smem);
+      return;
+    }
   }
   if constexpr (OT >= 0) {
     store_pass<L, typename Elem<OT>::T>(acc, eb, which, m0, n0, mvalid, nvalid, smem);

@@ -499,8 +499,8 @@ static GemmShape shape8(int64_t M, int64_t N, int64_t K, int tile = TM) {
 // fp32 g is not multiplied in fp32: an 8-bit integer is a bf16 number as it stands, so g times the scale that its product
 // sums over, in three bf16 parts, times the integers is exact but for the sum: three bf16 products, where two fp32
 // operands take six. dx: the parts beside each other, K = 3 Vr through the weight's rows three times. dW: the parts below
-// each other, K = 3 np against the rows' integers three times. d 2560, V 151,936, both gradients of 512 rows 2,690 us,
-// 4,700 as fp32 products (a library's 6,900).
+// each other, K = 3 np against the rows' integers three times. d 2560, V 151,936, both gradients of 512 rows 2,500 us,
+// 4,700 as fp32 products (a library's 6,700).
 struct Grads8Layout {
   int64_t Vr, dp, np, Vp;  // rows and columns of the copies
   int64_t Kh;              // dx's K
