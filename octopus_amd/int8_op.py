@@ -162,21 +162,23 @@ def checkpoint8(fn, *xs, group: int = 128):
     """fn(*xs), recomputed in the backward (torch.utils.checkpoint, not reentrant) from inputs that are held in 8 bits
     in between: those of bf16, f16 or fp32 on a HIP device that require a gradient. The forward sees them as they are,
     the recompute what their 8 bits stand for, so what fn saves for its gradients is off by the rounding (half of 1/127
-    of a group's largest value). Other arguments (masks, positions, parameters, None) are kept by reference."""
+    of a group's largest value). Other arguments (masks, positions, parameters, None) are kept by reference;
+    changed in place before the backward, it raises, as an ordinary checkpoint does."""
     _groups(1, group)
     live = list(xs)
     held = [_Held(x, group) if _holds(x) else None for x in xs]
-    kept = [None if h is not None else x for x, h in zip(xs, held)]
 
-    def run():
+    def run(*kept):
         if live:  # the forward itself
             args = tuple(live)
             live.clear()
         else:
-            args = (x if h is None else h.again() for x, h in zip(kept, held))
+            rest = iter(kept)
+            args = tuple(next(rest) if h is None else h.again() for h in held)
         return fn(*args)
 
-    return checkpoint(run, use_reentrant=False)
+    # what is kept goes through the checkpoint's own arguments, which it watches for changes in place
+    return checkpoint(run, *(x for x, h in zip(xs, held) if h is None), use_reentrant=False)
 
 
 # ---- the head's logits -----------------------------------------------------------------------------------------------
