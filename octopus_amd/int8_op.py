@@ -142,17 +142,6 @@ def widen_rows(q: Tensor, scale: Tensor, dtype: torch.dtype, group: int = 0) -> 
     return _widen_op(q, scale, dtype, group) if torch.compiler.is_compiling() else _widen(q, scale, dtype, group)
 
 
-class _Held:
-    """An activation held in 8 bits."""
-
-    def __init__(self, x: Tensor, group: int):
-        self.q, self.scale = quantise_rows(x, group)
-        self.dtype, self.group = x.dtype, group
-
-    def again(self) -> Tensor:
-        return widen_rows(self.q, self.scale, self.dtype, self.group).requires_grad_(True)
-
-
 def _holds(x) -> bool:
     return isinstance(x, Tensor) and x.requires_grad and torch.is_grad_enabled() and x.is_cuda and \
         x.dtype in _FLOATS and x.dim() > 0 and x.shape[-1] > 0 and not isinstance(x, torch.nn.Parameter)
@@ -166,19 +155,22 @@ def checkpoint8(fn, *xs, group: int = 128):
     changed in place before the backward, it raises, as an ordinary checkpoint does."""
     _groups(1, group)
     live = list(xs)
-    held = [_Held(x, group) if _holds(x) else None for x in xs]
+    dtypes = [x.dtype if _holds(x) else None for x in xs]
 
     def run(*kept):
         if live:  # the forward itself
-            args = tuple(live)
+            args = live[:]
             live.clear()
         else:
             rest = iter(kept)
-            args = tuple(next(rest) if h is None else h.again() for h in held)
+            args = [next(rest) if t is None else widen_rows(next(rest), next(rest), t, group).requires_grad_(True)
+                    for t in dtypes]
         return fn(*args)
 
-    # what is kept goes through the checkpoint's own arguments, which it watches for changes in place
-    return checkpoint(run, *(x for x, h in zip(xs, held) if h is None), use_reentrant=False)
+    # All that is kept, 8-bit rows and scales too, goes through the checkpoint's own arguments: it watches them for
+    # changes in place, finds in them the devices whose random numbers fn draws, and shows them to saved tensors' hooks.
+    kept = [y for x, t in zip(xs, dtypes) for y in ((x,) if t is None else quantise_rows(x, group))]
+    return checkpoint(run, *kept, use_reentrant=False)
 
 
 # ---- the head's logits -----------------------------------------------------------------------------------------------
