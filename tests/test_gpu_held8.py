@@ -19,7 +19,8 @@ def test_random_numbers_are_those_of_the_forward():
     state = torch.cuda.get_rng_state()
     (grad,) = torch.autograd.grad(y.sum(), x)
     assert torch.equal(torch.cuda.get_rng_state(), state)
-    assert torch.equal(grad == 0, y == 0)
+    # the gradient is 2 x mask^2 of the x that the 8 bits stand for: zero where they are zero, or the forward's mask is
+    assert torch.equal(grad == 0, (y == 0) | (int8_op.quantise_rows(x, 128)[0] == 0))
 
 
 def test_held_rows_through_hooks_of_saved_tensors():
