@@ -20,7 +20,7 @@ from torch.utils.checkpoint import checkpoint
 
 TILE = 16384
 _INNER = True  # tiles checkpointed; no_inner() turns this off
-_HELD8 = None  # the group of the 8-bit rows that tiles' checkpoints hold; held8() sets it
+_HELD8 = None  # held8()'s: the group of the 8-bit rows that tiles' checkpoints hold, and the hooks around it
 COMPILE = os.environ.get("OCTOPUS_COMPILE", "1") != "0"
 
 
@@ -39,12 +39,17 @@ def _fused(fn=None, *, hip=None):
     return run
 
 
+def _hooks():
+    """This thread's innermost hooks of saved tensors; a checkpoint's forward and its recompute have some of their own."""
+    return torch._C._autograd._top_saved_tensors_default_hooks(False)
+
+
 def _checkpoint(fn, *args):
     if not _INNER:
         return fn(*args)
-    if _HELD8 is not None:
+    if _HELD8 is not None and _hooks() == _HELD8[1]:
         from ..int8_op import checkpoint8
-        return checkpoint8(fn, *args, group=_HELD8)
+        return checkpoint8(fn, *args, group=_HELD8[0])
     return checkpoint(fn, *args, use_reentrant=False)
 
 
@@ -76,12 +81,14 @@ def no_inner():
 def held8(group: int = 128):
     """Tiles begun inside hold their inputs in 8 bits between the forward and their recompute (int8_op.checkpoint8: the
     HIP tensors that require a gradient), a scale for each `group` values of a row: 1.03 bytes a value in place of 2.
-    Tiles on the CPU, and no_inner()'s, are as without it."""
+    Tiles on the CPU, and no_inner()'s, are as without it, and so are those under hooks of saved tensors that were set
+    inside it, another checkpoint's above all: what that recomputes has to be what its forward ran, also when this
+    context has ended. To hold 8 bits there, open it in the function that the other checkpoint calls."""
     from ..int8_op import GROUPS
     global _HELD8
     if group not in GROUPS:
         raise ValueError(f"octohead: groups of {GROUPS} values, got {group}")
-    before, _HELD8 = _HELD8, group
+    before, _HELD8 = _HELD8, (group, _hooks())
     try:
         yield
     finally:

@@ -39,3 +39,18 @@ def test_held_rows_through_hooks_of_saved_tensors():
     got = torch.autograd.grad(y.sum(), x)
     assert torch.equal(got[0], want[0])
     assert packed == [(torch.int8, 9 * 203), (torch.float32, 9 * 2)]
+
+
+def test_held8_around_another_checkpoint():
+    """The tiles of a layer that a checkpoint recomputes, with the backward behind held8(): as without it."""
+    from torch.utils.checkpoint import checkpoint
+
+    from octopus_amd.rl import seq_tiles
+
+    x = torch.randn(1, 50, 256, device=DEV).requires_grad_(True)
+    layer = lambda t: checkpoint(lambda u: seq_tiles.tiled(torch.sin, u * 2), t, use_reentrant=False)  # noqa: E731
+    (want,) = torch.autograd.grad(layer(x).sum(), x)
+    with seq_tiles.held8():
+        y = layer(x)
+    (got,) = torch.autograd.grad(y.sum(), x)
+    assert torch.equal(got, want)
