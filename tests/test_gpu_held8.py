@@ -54,3 +54,32 @@ def test_held8_around_another_checkpoint():
         y = layer(x)
     (got,) = torch.autograd.grad(y.sum(), x)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("group", [0, 128])
+def test_rows_that_8_bits_do_not_make_smaller_are_kept(dtype, group, monkeypatch):
+    """Rows are padded to 16 bytes and have a scale: a narrow tensor takes fewer bytes as it is."""
+    calls = []
+    real = int8_op.quantise_rows
+    monkeypatch.setattr(int8_op, "quantise_rows", lambda x, g: calls.append(x.shape[-1]) or real(x, g))
+    size = torch.finfo(dtype).bits // 8
+    for d in (1, 2, 5, 8, 9, 10, 11, 12, 16, 17, 18, 19, 40, 200):
+        x = torch.randn(7, d, device=DEV).to(dtype).requires_grad_(True)
+        calls.clear()
+        (grad,) = torch.autograd.grad(int8_op.checkpoint8(torch.sin, x, group=group).sum(), x)
+        smaller = -(-d // 16) * 16 + 4 * (-(-d // group) if group else 1) < d * size
+        assert calls == ([d] if smaller else [])
+        if not smaller:
+            assert torch.equal(grad, torch.cos(x.detach()))
+
+
+def test_expanded_tensors_are_kept(monkeypatch):
+    calls = []
+    real = int8_op.quantise_rows
+    monkeypatch.setattr(int8_op, "quantise_rows", lambda x, g: calls.append(x.shape) or real(x, g))
+    bias = torch.randn(1, 4, 64, device=DEV).requires_grad_(True)
+    x = torch.randn(8, 4, 64, device=DEV).requires_grad_(True)
+    y = int8_op.checkpoint8(lambda a, b: torch.sin(a + b), x, bias.expand(8, 4, 64))
+    gx, gb = torch.autograd.grad(y.sum(), (x, bias))
+    assert calls == [(8, 4, 64)] and torch.allclose(gx.sum(0, keepdim=True), gb, rtol=0, atol=8 * 2.0 ** -22)
