@@ -76,18 +76,17 @@ __device__ __forceinline__ float scale_of(uint32_t maxbits) {
   return a < kLeastMax ? 0.f : a * (1.f / 127.f);
 }
 // 8 quotients as bytes. x inv is within an integer of x / s and the remainder x - q s is exact in one fma (at most 7
-// bits of q times 24 of s, less x: within fp32's 24 bits above the finer of the two last places), so comparing it with
-// s / 2 gives the quotient's rounding exactly.
+// bits of q times 24 of s, less x: within fp32's 24 bits above the finer of the two last places), so comparing twice it
+// with s gives the quotient's rounding exactly (half of an s below 2^-125 is not always a number of fp32).
 __device__ __forceinline__ i32x2 quotients(const float (&x)[8], float s, float inv) {
-  const float half = 0.5f * s;
   i32x2 out = {0, 0};
   if (!(s > 0.f)) return out;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     float q = __builtin_rintf(x[e] * inv);
-    const float r = __builtin_fmaf(-q, s, x[e]), ar = fabsf(r);
+    const float r = __builtin_fmaf(-q, s, x[e]), twice = 2.f * fabsf(r);
     const int odd = (int)q & 1;
-    if (ar > half || (ar == half && odd)) q += __builtin_copysignf(1.f, r);
+    if (twice > s || (twice == s && odd)) q += __builtin_copysignf(1.f, r);
     out[e >> 2] |= ((int)q & 0xff) << (8 * (e & 3));
   }
   return out;
