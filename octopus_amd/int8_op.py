@@ -312,7 +312,9 @@ class _Head8(torch.autograd.Function):
                                    "backward")
         shape, dtype, w_dtype = ctx.like
         call = head_grads_i8 if torch.is_grad_enabled() else _grads
-        gr, gw = call(g, *ctx.saved_tensors, *ctx.weights, dtype, w_dtype or dtype, need_rows, need_w)
+        xq, xs = ctx.saved_tensors
+        xq = _rows8(xq)  # as saved, or as a hook gave them back: without the bytes between the rows
+        gr, gw = call(g, xq, xs, *ctx.weights, dtype, w_dtype or dtype, need_rows, need_w)
         return gr.view(shape) if need_rows else None, None, None, gw if need_w else None, None
 
 
