@@ -21,6 +21,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.utils.checkpoint import checkpoint
 
 from . import _lib
@@ -325,8 +326,8 @@ def int8_head(rows: Tensor, wq: Tensor, w_scale: Tensor, *, weight: Optional[Ten
     and rounded once. The rows' gradient is that of the weights' 8-bit values. weight: the [V, d] parameter that wq was
     made of, which gets the gradient straight through the rounding; its values are not read, and wq is made again when
     it has changed. Between the two passes the rows are held in 8 bits, and wq and w_scale by reference (changed in
-    place, the backward raises). wq and w_scale get no gradient; the gradients have no derivative of their own (one
-    raises)."""
+    place, the backward raises). wq and w_scale get no gradient; the gradients have no derivative of their own and the
+    logits none in forward mode (one raises)."""
     out_dtype = out_dtype or rows.dtype
     train = torch.is_grad_enabled() and (rows.requires_grad or weight is not None and weight.requires_grad)
     if train and out_dtype == torch.float32 and wq.dim() == 2:
@@ -336,6 +337,9 @@ def int8_head(rows: Tensor, wq: Tensor, w_scale: Tensor, *, weight: Optional[Ten
             raise ValueError(f"octohead: fp32 logits [{n}, {V}] have gradients up to {_F32_GRADS_MAX} rows and columns")
     if torch.compiler.is_compiling():
         return head_logits_i8(rows, wq, w_scale, weight, out_dtype)[0]
+    if forward_ad._current_level >= 0 and \
+            any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (rows, w_scale, weight)):
+        raise NotImplementedError("octohead: the 8-bit head's logits have no derivative in forward mode")
     if train:
         return _Head8.apply(rows, wq, w_scale, weight, out_dtype)
     return _logits(rows, wq, w_scale, weight, out_dtype)[0]

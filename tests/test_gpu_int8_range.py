@@ -1,4 +1,5 @@
-"""int8_head and its gradients where the first tests did not go: saved rows that a hook gives back in another layout."""
+"""int8_head and its gradients where the first tests did not go: saved rows that a hook gives back in another layout,
+tangents of forward mode."""
 
 import pytest
 import torch
@@ -22,3 +23,22 @@ def test_saved_rows_in_another_layout(n):
         z = int8_op.int8_head(h, wq, ws, weight=p)
     got = torch.autograd.grad(z, (h, p), up)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_tangents_are_refused():
+    """Forward mode has no derivative here: an error, not logits without their tangent."""
+    import torch.autograd.forward_ad as fwad
+
+    x, w = _inputs(6, 32, 50, torch.float32)
+    x, w = x.to(DEV), w.to(DEV)
+    wq, ws = int8_op.quantise_rows(w)
+    for grad in (False, True):
+        with fwad.dual_level():
+            dual = fwad.make_dual(x.clone().requires_grad_(grad), torch.ones_like(x))
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                int8_op.int8_head(dual, wq, ws)
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                int8_op.int8_head(x, wq, ws, weight=fwad.make_dual(w.clone(), torch.ones_like(w)))
+    with fwad.dual_level():
+        plain = int8_op.int8_head(x, wq, ws)  # no tangent: as ever
+    assert torch.equal(plain, int8_op.int8_head(x, wq, ws))
