@@ -363,8 +363,10 @@ int octo_head_logits_i8(const void *rows, int64_t ldx, int x_dtype, const int8_t
                         int z_dtype, void *stream);
 /* Its gradients for g = dL/dlogits [n, ldg], straight through the rounding (NULL skips one):
  *   grad_rows[r, k] = sum_v g[r, v] w_scale[v] wq[v, k];  grad_w[v, k] = sum_r g[r, v] x_scale[r] xq[r, k]
- * 16-bit g: the products run in its type, the 8-bit operand times its scale rounded once to it. F32 g (n, V <= 2^20): g
- * times the scale in three bf16 parts (24 bits; a value that bf16 rounds to infinity is one), times the integers,
+ * 16-bit g: the products run in its type, the 8-bit operand times its scale rounded once to it (F16: times a power of two
+ * as well, which the sum is divided by, so that operands outside f16's numbers keep its 11 bits down to 2^-29 of the
+ * largest scale). F32 g (n, V <= 2^20): g times the scale in three bf16 parts (24 bits; a value that bf16 rounds to
+ * infinity is one), times the integers,
  * exactly. Summed in fp32 and rounded once. ws: octo_head_grads_i8_workspace_bytes, 256-byte aligned; with room for a
  * copy of g where that is not of 16-bit values, rows of whole 16-byte chunks (V too) and 256 columns or more (g is not
  * read there), for its parts, 6 bytes a value and gradient, where it is F32 (up to 128 rows neither for grad_rows). */

@@ -12,7 +12,8 @@
 //
 // The gradients are 16-bit products of the widened operands (prepare8_kernel: 190 us at that weight, a write of 778 MB), at
 // the rate of the head's other gradients: 2,048 rows 2,480 us for both, 1.29 PFLOP/s. The rows' gradient of up to 128 reads
-// the 8-bit weight itself (few_dx_kernel).
+// the 8-bit weight itself (few_dx_kernel). f16 operands are widened times a power of two (f16_range), for which a launch
+// finds the largest scale: 225 rows of d 1024, V 32,000 80.7 us, 76.3 without, where rows of 1e5 gave NaN.
 #include <type_traits>
 
 #include "gemm_nt.h"
@@ -288,7 +289,8 @@ template <typename OT> static int go_few(const Few8 &a, int x_dtype, hipStream_t
 // dx of few rows is the weight's bytes too, which a widened copy multiplies by five. Here a wave takes a share of the
 // vocabulary and 256 columns: lane l holds 16 columns (16 bytes at 16 (l & 15)) of 8 rows (8 (l >> 4) ..) of each 32, so
 // that its 8 bytes of a column are 8 neighbours along K, and product j of 16 takes column j of every lane: widened, rounded
-// to g's type and fed without an exchange between lanes. fp32 g: the integers and g's three parts, as in the large
+// to g's type and fed without an exchange between lanes. f16: each wave widens by the power of two of its own share's scales
+// (f16_range) and takes it back before the sums are joined. fp32 g: the integers and g's three parts, as in the large
 // products. A workgroup's waves join their sums in the LDS, a second launch the workgroups', both in order.
 //
 // d 2560, V 151,936, us so and by the widened copy: bf16 8 rows 82 (4.8 TB/s) and 404, 32 88 and 403, 64 144 and 404, 128
@@ -347,7 +349,8 @@ __global__ __launch_bounds__(64 * kDxWaves) void few_dx_kernel(FewDx a) {
     for (int b = 0; b < NB; ++b)
       t.g[b] = v0 + 32 <= last ? load_raw8<DT>(grow[b] + v) : load_raw8<DT>(grow[b] + v, last - v);
   };
-  auto take = [&](const Step &t) {
+  float times = 1.f, back = 1.f;  // f16: f16_range of the share's scales
+  auto take = [&](Step &t) {
     i32x4 gop[NB][NP];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -360,6 +363,10 @@ __global__ __launch_bounds__(64 * kDxWaves) void few_dx_kernel(FewDx a) {
       } else {
         gop[b][0] = t.g[b].v[0];
       }
+    }
+    if constexpr (DT == OCTO_F16) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t.s[e] *= times;
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -378,6 +385,12 @@ __global__ __launch_bounds__(64 * kDxWaves) void few_dx_kernel(FewDx a) {
   };
   if (first < last) {
     Step t[2];
+    if constexpr (DT == OCTO_F16) {
+      uint32_t m = 0;
+#pragma unroll 4
+      for (int v = first + lane; v < last; v += 64) m = max(m, finite_bits(a.sw[v]));
+      f16_range((uint32_t)__builtin_amdgcn_readfirstlane((int)lanes_max<64>(m)), times, back);
+    }
     load(t[0], first);
     for (int v = first;;) {
       if (v + 32 < last) load(t[1], v + 32);
@@ -390,14 +403,15 @@ __global__ __launch_bounds__(64 * kDxWaves) void few_dx_kernel(FewDx a) {
   }
 #pragma unroll
   for (int half = kDxWaves / 2; half > 0; half >>= 1) {
+    const float own = DT == OCTO_F16 && half == kDxWaves / 2 ? back : 1.f;
     if (w >= half && w < 2 * half) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) smem[w - half][r][lane] = acc[r >> 4][r & 15];
+      for (int r = 0; r < R; ++r) smem[w - half][r][lane] = acc[r >> 4][r & 15] * own;
     }
     __syncthreads();
     if (w < half) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) acc[r >> 4][r & 15] += smem[w][r][lane];
+      for (int r = 0; r < R; ++r) acc[r >> 4][r & 15] = acc[r >> 4][r & 15] * own + smem[w][r][lane];
     }
     __syncthreads();
   }
@@ -505,7 +519,7 @@ struct Grads8Layout {
   int64_t Vr, dp, np, Vp;  // rows and columns of the copies
   int64_t Kh;              // dx's K
   int parts;               // of g
-  size_t wide, xt, g, gh, split, total;
+  size_t norm, wide, xt, g, gh, split, total;
   int64_t split_items;
   bool few;  // dx by few_dx_kernel, its partial sums in split
 };
@@ -539,6 +553,7 @@ static Grads8Layout grads8_layout(int64_t n, int d, int V, int dtype, bool need_
   L.g = take(L.parts == 1 ? (as_is || !(need_rows || need_w) ? 0 : (size_t)L.np * L.Vp * 2) : (need_w ? (size_t)3 * L.np * L.Vp * 2 : 0));
   L.gh = take(L.parts == 3 && need_rows ? (size_t)n * L.Kh * 2 : 0);
   L.split = take(L.few ? dx_split(n, d, V, dtype).bytes : (size_t)L.split_items * TM * TN * 4);
+  L.norm = take(dtype == OCTO_F16 && (need_rows || need_w) ? sizeof(Norm8) : 0);
   L.total = at;
   return L;
 }
@@ -663,6 +678,7 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
   p.ldg = ldg;
   p.gs = as_is || (!grad_w && (f32 || !wide)) ? nullptr : wsb + L.g;
   p.gh = f32 && wide ? wsb + L.gh : nullptr;
+  p.norm = g_dtype == OCTO_F16 && (wide || grad_w) ? (Norm8 *)(wsb + L.norm) : nullptr;
   p.np = L.np;
   p.Vp = L.Vp;
   p.n = n;
@@ -693,6 +709,7 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
     oh.C = grad_rows;
     oh.ldc = ld_gr;
     oh.dtype = gr_dtype;
+    oh.alpha = p.norm ? &p.norm->back[0] : nullptr;
     if (L.split_items) {
       oh.split = (float *)(wsb + L.split);
       oh.split_cap = (int)L.split_items;
@@ -703,6 +720,7 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
     ow.C = grad_w;
     ow.ldc = ld_gw;
     ow.dtype = gw_dtype;
+    ow.alpha = p.norm ? &p.norm->back[1] : nullptr;
   }
   // Both in one launch, dx's runs as long as if it had the card to itself: dW's short tiles follow them on every CU. Two
   // launches take 20 us more up to 700 rows of d 2560, V 151,936 and as long from 1,024 on; runs cut for sharing the card

@@ -435,6 +435,10 @@ int launch_transpose(const void *src, int64_t ld_src, int src_dtype, const float
 // What the gradients of the 8-bit head read: each copy that is not NULL. 16-bit g: the 8-bit operands times their scales
 // in g's type, and g itself where it cannot be read as it lies. fp32 g: the 8-bit operands as bf16 integers, and g times
 // the weights' scales (gh) and times the rows' (gs), each as three bf16 parts.
+struct Norm8 {
+  uint32_t top[2][64];  // the weights' and the rows' scales: largest finite ones of 64 shares
+  float back[2];        // what the products' results are multiplied by
+};
 struct Prepare8 {
   const int8_t *wq;  // [V, ldw]
   int64_t ldw;
@@ -452,6 +456,7 @@ struct Prepare8 {
   void *gs;          // [np, Vp], zeros behind g; fp32 g: [3 np, Vp], a part after the other
   void *gh;          // fp32 g: [n, 3 Vr], a part beside the other
   int64_t np, Vp;    // np a multiple of 64, Vp of 8
+  Norm8 *norm;       // f16 g with a widened operand
   int64_t n;
   int d, V;
   unsigned wide_blocks, t_blocks, g_parts;  // set by the launch

@@ -137,4 +137,17 @@ __device__ __forceinline__ void split_parts(const float (&x)[8], i32x4 (&part)[3
   part[2] = pack8(p2, false);
 }
 
+// Integers times scales as f16 numbers: bf16 and fp32 rows, and scales as a caller gives them, may lie outside f16's range.
+// times: the power of two that brings 127 of the largest finite scale to [2^14, 2^15), short of f16's infinity (that of
+// -128 too), with f16's 11 bits down to 2^-29 of it; back: its inverse, for the sum. maxbits: that scale's.
+__device__ __forceinline__ uint32_t finite_bits(float s) {
+  const uint32_t b = __float_as_uint(s) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0;
+}
+__device__ __forceinline__ void f16_range(uint32_t maxbits, float &times, float &back) {
+  const int by = min(7 - ((int)(maxbits >> 23) - 127), 120);  // the scale is below 2^(8 - by)
+  times = __uint_as_float((uint32_t)(127 + by) << 23);
+  back = __uint_as_float((uint32_t)(127 - by) << 23);
+}
+
 }  // namespace octo

@@ -98,12 +98,16 @@ __device__ __forceinline__ void unpack_i8(const i32x2 v, float s, float (&x)[8])
 
 // Row r of out = q scale for the columns c < d, zeros up to cols_pad (and for all of a row past `rows`), by one wave, 4
 // chunks of 8 columns a lane in flight. gshift: log2 of the group, or -1. The bytes of q behind d are readable up to the
-// next multiple of 16. UNIT: the integers themselves (exact in every type).
-template <int DT, bool UNIT = false>
+// next multiple of 16. UNIT: the integers themselves (exact in every type). times(): a power of two for all scales, asked
+// for with the loads in flight.
+struct TimesOne {
+  __device__ __forceinline__ float operator()() const { return 1.f; }
+};
+template <int DT, bool UNIT = false, class F = TimesOne>
 __device__ __forceinline__ void widen_row(const int8_t *q, const float *scale, bool there, int d, int gshift,
-                                          typename Elem<DT>::T *out, int cols_pad) {
-  const int lane = threadIdx.x & 63;
-  for (int c0 = 8 * lane; c0 < cols_pad; c0 += 512 * 4) {
+                                          typename Elem<DT>::T *out, int cols_pad, F times = F{}) {
+  for (int start = 0; start < cols_pad; start += 512 * 4) {  // the whole wave: times() may join its lanes
+    const int c0 = start + 8 * (int)(threadIdx.x & 63);
     i32x2 v[4];
     float s[4];
 #pragma unroll
@@ -112,11 +116,12 @@ __device__ __forceinline__ void widen_row(const int8_t *q, const float *scale, b
       v[u] = there ? *(const i32x2 *)(q + at) : i32x2{0, 0};
       s[u] = !there || c >= d ? 0.f : (UNIT ? 1.f : scale[gshift < 0 ? 0 : at >> gshift]);
     }
+    const float by = UNIT ? 1.f : times();
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int c = c0 + 512 * u;
       float x[8];
-      unpack_i8(v[u], s[u], x);
+      unpack_i8(v[u], s[u] * by, x);
       if (c + 8 <= cols_pad) {
         if constexpr (DT == OCTO_F32) {
 #pragma unroll
@@ -143,11 +148,26 @@ __global__ __launch_bounds__(256) void widen_i8_kernel(const int8_t *q, int64_t 
   if (r < rows) widen_row<DT>(q + r * ldq, scale + r * groups, true, d, gshift, out + r * ldo, d);
 }
 
+// f16_range of the weights' scales (k 0) or the rows', its inverse left to the product by one workgroup.
+template <int DT> struct RangeTimes {
+  Norm8 *norm;
+  int k;
+  bool leave;
+  __device__ __forceinline__ float operator()() const {
+    float times = 1.f, back;
+    if constexpr (DT == OCTO_F16) {
+      f16_range(lanes_max<64>(norm->top[k][threadIdx.x & 63]), times, back);
+      if (leave && threadIdx.x == 0) norm->back[k] = back;
+    }
+    return times;
+  }
+};
+
 // xt[c, r] = q[r, c] scale[r] for c < d, r0 <= r < r0 + 64; zeros from n on; `repeats` of it np columns apart. A 64 x 64
 // tile through the LDS.
-template <int DT, bool UNIT = false>
+template <int DT, bool UNIT = false, class F>
 __device__ __forceinline__ void widen_t_tile(const Prepare8 &a, int64_t r0, int c0, int repeats,
-                                             typename Elem<DT>::T (*tile)[64 + 16 / Elem<DT>::bytes]) {
+                                             typename Elem<DT>::T (*tile)[64 + 16 / Elem<DT>::bytes], F times) {
   typedef typename Elem<DT>::T T;
   constexpr int PER = 16 / sizeof(T);
   const int t = threadIdx.x;
@@ -160,6 +180,7 @@ __device__ __forceinline__ void widen_t_tile(const Prepare8 &a, int64_t r0, int 
       s = UNIT ? 1.f : a.xs[r];
       v = *(const i32x4 *)(a.xq + r * a.ldxq + c0 + c);
     }
+    if (!UNIT) s *= times();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float x[8];
@@ -243,18 +264,35 @@ __global__ __launch_bounds__(256) void prepare8_kernel(Prepare8 a) {
   unsigned b = blockIdx.x;
   if (b < a.wide_blocks) {
     const int64_t r = (int64_t)b * 4 + (threadIdx.x >> 6);  // Vr is a multiple of 64
-    widen_row<WT, F32>(a.wq + r * a.ldw, a.ws + r, r < a.V, a.d, -1, (T *)a.wide + r * a.dp, a.dp);
+    const RangeTimes<DT> times{a.norm, 0, b == 0};
+    widen_row<WT, F32>(a.wq + r * a.ldw, a.ws + r, r < a.V, a.d, -1, (T *)a.wide + r * a.dp, a.dp, times);
     return;
   }
   b -= a.wide_blocks;
   if (b < a.t_blocks) {
     const unsigned tiles = (unsigned)(a.np / 64);
-    widen_t_tile<WT, F32>(a, (int64_t)(b % tiles) * 64, (int)(b / tiles) * 64, F32 ? 3 : 1, tile);
+    const RangeTimes<DT> times{a.norm, 1, b == 0};
+    widen_t_tile<WT, F32>(a, (int64_t)(b % tiles) * 64, (int)(b / tiles) * 64, F32 ? 3 : 1, tile, times);
     return;
   }
   b -= a.t_blocks;
   if constexpr (F32) stage_f32(a, b / a.g_parts, (int)(b % a.g_parts));
   else stage_part<DT>(a, b / a.g_parts, (int)(b % a.g_parts));
+}
+
+// The largest finite scales of 64 shares of the weights (blocks 0 .. 63) and of the rows, for f16_range.
+__global__ __launch_bounds__(256) void norm8_kernel(const float *ws, int64_t V, const float *xs, int64_t n, Norm8 *norm) {
+  __shared__ uint32_t top[4];
+  const int k = blockIdx.x >> 6, part = blockIdx.x & 63, t = threadIdx.x;
+  const float *s = k ? xs : ws;
+  const int64_t count = k ? n : V;
+  uint32_t m = 0;
+#pragma unroll 4
+  for (int64_t i = part * 256 + t; i < count; i += 64 * 256) m = max(m, finite_bits(s[i]));
+  m = lanes_max<64>(m);
+  if ((t & 63) == 0) top[t >> 6] = m;
+  __syncthreads();
+  if (t == 0) norm->top[k][part] = max(max(top[0], top[1]), max(top[2], top[3]));
 }
 
 int launch_prepare8(Prepare8 a, int dtype, hipStream_t st) {
@@ -267,6 +305,10 @@ int launch_prepare8(Prepare8 a, int dtype, hipStream_t st) {
   if (blocks >= (1 << 24)) return octo_fail(OCTO_EINVAL, "head_grads_i8: %lld blocks", (long long)blocks);
   a.wide_blocks = (unsigned)wide;
   a.t_blocks = (unsigned)t;
+  if (a.norm) {
+    hipLaunchKernelGGL(norm8_kernel, dim3(128), dim3(256), 0, st, a.ws, a.wide ? a.V : 0, a.xs, a.xt ? a.n : 0, a.norm);
+    OCTO_CHECK_LAUNCH("norm8");
+  }
   const dim3 grid((unsigned)blocks);
   switch (dtype) {
     case OCTO_BF16: hipLaunchKernelGGL(prepare8_kernel<OCTO_BF16>, grid, dim3(256), 0, st, a); break;

@@ -1,4 +1,4 @@
-// The sum of a split-K product's partial tiles (StoreArgs::split): C = rs[row] x sum over the runs (+ addend) (+ C),
+// The sum of a split-K product's partial tiles (StoreArgs::split): C = rs[row] alpha x sum over the runs (+ addend) (+ C),
 // rounded once to C's type.
 //
 // Bound by memory: S partial tiles of 256 KB read per tile of C. One workgroup per 16 rows of a tile, 256 threads: each
@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) void split_sum_kernel(GemmShape s, StoreArgs e
   const int row = threadIdx.x >> 4;
   if (row0 + row >= mvalid) return;
   const int64_t r = m0 + row0 + row;
-  const float sc = e.row_scale ? e.row_scale[r] : 1.f;
+  const float sc = (e.row_scale ? e.row_scale[r] : 1.f) * (e.alpha ? *e.alpha : 1.f);
   OT *C = (OT *)e.C + r * e.ldc + n0;
   const float *add = e.addend ? e.addend + r * e.ld_add + n0 : nullptr;
   typedef OT OT4 __attribute__((ext_vector_type(4)));
