@@ -459,7 +459,7 @@ struct Prepare8 {
   Norm8 *norm;       // f16 g with a widened operand
   int64_t n;
   int d, V;
-  unsigned wide_blocks, t_blocks, g_parts;  // set by the launch
+  unsigned wide_blocks, t_blocks, g_parts, first;  // set by the launch
 };
 int launch_prepare8(Prepare8 a, int dtype, hipStream_t st);
 

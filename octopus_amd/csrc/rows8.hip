@@ -261,7 +261,7 @@ __global__ __launch_bounds__(256) void prepare8_kernel(Prepare8 a) {
   constexpr int WT = F32 ? OCTO_BF16 : DT;  // fp32 g multiplies with the integers in bf16, its parts with the scales in g
   typedef typename Elem<WT>::T T;
   __shared__ __attribute__((aligned(16))) T tile[64][64 + 16 / sizeof(T)];
-  unsigned b = blockIdx.x;
+  unsigned b = a.first + blockIdx.x;
   if (b < a.wide_blocks) {
     const int64_t r = (int64_t)b * 4 + (threadIdx.x >> 6);  // Vr is a multiple of 64
     const RangeTimes<DT> times{a.norm, 0, b == 0};
@@ -295,6 +295,8 @@ __global__ __launch_bounds__(256) void norm8_kernel(const float *ws, int64_t V, 
   if (t == 0) norm->top[k][part] = max(max(top[0], top[1]), max(top[2], top[3]));
 }
 
+// Blocks a launch: 2^24 of 256 threads are more threads than one can have. At most 2^31 in all (2^21 rows and columns).
+constexpr int64_t kPrepareBlocks = 1 << 22;
 int launch_prepare8(Prepare8 a, int dtype, hipStream_t st) {
   const bool f32 = dtype == OCTO_F32;
   const int64_t per = f32 ? 256 * 8 : 512 * 8;  // values of a part of g
@@ -302,20 +304,22 @@ int launch_prepare8(Prepare8 a, int dtype, hipStream_t st) {
   a.g_parts = (unsigned)cdiv(a.Vp, per);
   const int64_t staged = a.gs || a.gh ? a.np * a.g_parts : 0, blocks = wide + t + staged;
   if (blocks == 0) return OCTO_OK;
-  if (blocks >= (1 << 24)) return octo_fail(OCTO_EINVAL, "head_grads_i8: %lld blocks", (long long)blocks);
   a.wide_blocks = (unsigned)wide;
   a.t_blocks = (unsigned)t;
   if (a.norm) {
     hipLaunchKernelGGL(norm8_kernel, dim3(128), dim3(256), 0, st, a.ws, a.wide ? a.V : 0, a.xs, a.xt ? a.n : 0, a.norm);
     OCTO_CHECK_LAUNCH("norm8");
   }
-  const dim3 grid((unsigned)blocks);
-  switch (dtype) {
-    case OCTO_BF16: hipLaunchKernelGGL(prepare8_kernel<OCTO_BF16>, grid, dim3(256), 0, st, a); break;
-    case OCTO_F16: hipLaunchKernelGGL(prepare8_kernel<OCTO_F16>, grid, dim3(256), 0, st, a); break;
-    default: hipLaunchKernelGGL(prepare8_kernel<OCTO_F32>, grid, dim3(256), 0, st, a); break;
+  for (int64_t first = 0; first < blocks; first += kPrepareBlocks) {
+    const dim3 grid((unsigned)(blocks - first < kPrepareBlocks ? blocks - first : kPrepareBlocks));
+    a.first = (unsigned)first;
+    switch (dtype) {
+      case OCTO_BF16: hipLaunchKernelGGL(prepare8_kernel<OCTO_BF16>, grid, dim3(256), 0, st, a); break;
+      case OCTO_F16: hipLaunchKernelGGL(prepare8_kernel<OCTO_F16>, grid, dim3(256), 0, st, a); break;
+      default: hipLaunchKernelGGL(prepare8_kernel<OCTO_F32>, grid, dim3(256), 0, st, a); break;
+    }
+    OCTO_CHECK_LAUNCH("prepare8");
   }
-  OCTO_CHECK_LAUNCH("prepare8");
   return OCTO_OK;
 }
 

@@ -118,3 +118,28 @@ def test_tangents_are_refused():
     with fwad.dual_level():
         plain = int8_op.int8_head(x, wq, ws)  # no tangent: as ever
     assert torch.equal(plain, int8_op.int8_head(x, wq, ws))
+
+
+# ---- many rows ----------------------------------------------------------------------------------------------------------
+
+def test_weight_gradient_of_two_million_rows():
+    """A copy of g of 2^24 blocks and more, 121 GB beside g's 120: the first and the last rows alone."""
+    n, d, V = 1 << 21, 16, 28673
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 250e9:
+        pytest.skip("needs 250 GB of free memory")
+    g = torch.zeros(n, V, dtype=torch.bfloat16, device=DEV)
+    g[0, 0], g[-1, 0], g[-1, -1], g[n // 2, 7] = 2, 4, 8, 16
+    xq = torch.ones(n, d, dtype=torch.int8, device=DEV)
+    xq[-1], xq[n // 2, 3] = 5, 100
+    xs = torch.full((n,), 0.5, device=DEV)
+    wq, ws = torch.ones(V, d, dtype=torch.int8, device=DEV), torch.ones(V, device=DEV)
+    try:
+        _, gw = int8_op._grads(g, xq, xs, wq, ws, torch.bfloat16, torch.bfloat16, False, True)
+        want = torch.zeros(V, d, device=DEV)
+        want[0], want[-1], want[7] = 2 * 0.5 + 4 * 2.5, 8 * 2.5, 16 * 0.5
+        want[7, 3] = 16 * 50
+        assert torch.equal(gw.float(), want)
+    finally:
+        del g
+        torch.cuda.empty_cache()
