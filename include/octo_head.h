@@ -385,12 +385,15 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
  *   tokens[s, :a] = the accepted drafts, tokens[s, a] = the lowest v whose running sum of r exceeds u_K sum r,
  *   r = max(p_a - q_a, 0) behind a rejected draft (p_a where that leaves nothing), p_a behind the last; -1 further on
  *   logp[s, i] = log p_i(tokens[s, i]), 0 further on
- * Probabilities and sums in 64 bits. greedy: a draft is accepted when it is its row's first largest logit, which is also
- * the next token; u and the draft logits are not read (may be NULL). A draft outside [0, V), or whose logits' row has no
- * softmax (a NaN, +inf, or nothing above -inf), is rejected and the token drawn from p_a; where p_a has none, the token
- * is -1 and its logp NaN. A u_K that is no number below 1 takes the last v with r_v > 0. Rows behind a sequence's length
- * are not read. K <= OCTO_DRAFTS_MAX, S <= 2^20. Rows may start at any element. ws: octo_verify_workspace_bytes, 16-byte
- * aligned. */
+ * Decisions and tokens are those of 64-bit probabilities and sums. logp is rounded once from 64 bits for the drawn token,
+ * and below 2^24 logits read (S (K + 1) V, with draft logits S (2 K + 1) V) for all; from there on the accepted drafts'
+ * and, when greedy, all tokens' come from row sums of 32-bit exponentials, within 5e-6 before that rounding, so that they
+ * may depend on how many sequences the call has. greedy: a draft is accepted when it is its row's first largest logit,
+ * which is also the next token; u and the draft logits are not read (may be NULL). A draft outside [0, V), or whose
+ * logits' row has no softmax (a NaN, +inf, or nothing above -inf), is rejected and the token drawn from p_a; where p_a
+ * has none, the token is -1 and its logp NaN. A u_K that is no number below 1 takes the last v with r_v > 0. Rows behind
+ * a sequence's length are not read. K <= OCTO_DRAFTS_MAX, S <= 2^20. Rows may start at any element. ws:
+ * octo_verify_workspace_bytes, 16-byte aligned. */
 int octo_verify_workspace_bytes(int64_t S, int K, int V, size_t *bytes);
 int octo_verify_drafts(const void *logits, int64_t ld_seq, int64_t ld_row, const void *draft_logits, int64_t ld_seq_d,
                        int64_t ld_row_d, int dtype, const int64_t *drafts, const int64_t *lengths, const float *uniform,

@@ -16,7 +16,8 @@
 //   pick      a workgroup per sequence finds the part in which the running sum passes u_K sum r, and in it the token
 // Many take the exponentials of stats in 32 bits (64-bit ones are 20 instructions each, and stats is most of the work),
 // which leave each row's sum within 5e-6 (see fast_spread). That decides a draft unless u q and p are closer than 2^-15;
-// then the row and its draft's are summed again in 64 bits there. decide, sums and rest take residual's place: a is found
+// then the row and its draft's are summed again in 64 bits there. Accepted drafts' and greedy's log-probabilities keep
+// those sums, and with them the 5e-6. decide, sums and rest take residual's place: a is found
 // once a sequence, and one sweep over row a of both models finds in 64 bits their sums and those of r (part_sums).
 //
 // Few logits are bound by the launches' latency (one sequence, 4 drafts, V 151,936: 6 + 8 + 6 us), many by memory and by

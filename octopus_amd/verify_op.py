@@ -82,9 +82,12 @@ def verify_drafts(logits: Tensor, drafts: Tensor, uniform: Optional[Tensor], tem
     a draft is accepted when it is its row's first largest logit, which is also the token behind them; uniform (may be
     None) and draft_logits are not read.
 
-    Probabilities are taken in 64 bits, so the token is the definition's. A draft outside the vocabulary, or whose
-    draft row has no softmax (a NaN, +inf, or every logit masked), is rejected and the token drawn from the target's;
-    where the target's row has none, the token is -1 and its logp NaN."""
+    Decisions and tokens are those of 64-bit probabilities, so the token is the definition's. logp is rounded once from
+    64 bits for the drawn token and, below 2^24 logits read, for all; from there on the accepted drafts' and greedy's are
+    within 5e-6 before that rounding (their rows' sums are of 32-bit exponentials), and may differ by that between calls
+    of other sizes. Nothing is differentiable. A draft outside the vocabulary, or whose draft row has no softmax (a NaN,
+    +inf, or every logit masked), is rejected and the token drawn from the target's; where the target's row has none, the
+    token is -1 and its logp NaN."""
     if logits.dim() != 3 or not logits.shape[1] or not logits.shape[2]:
         raise ValueError(f"octohead: logits must be [S, K + 1, V], got {tuple(logits.shape)}")
     S, rows, V = logits.shape
