@@ -1,12 +1,12 @@
-"""int8_head and its gradients where the first tests did not go: f16 logits of operands outside f16's range, saved rows
-that a hook gives back in another layout, tangents of forward mode."""
+"""int8_head and its gradients where the first tests did not go: f16 logits of operands outside f16's range, dense shares of
+many blocks of weight rows, saved rows that a hook gives back in another layout, tangents of forward mode, many rows."""
 
 import pytest
 import torch
 
 from octopus_amd import int8_op
 from oracle import rows8 as oracle
-from tests.test_gpu_int8_head import _check_logits, _half, _inputs
+from tests.test_gpu_int8_head import TYPES, _bound_grads, _check_logits, _half, _inputs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -83,6 +83,29 @@ def test_f16_gradients_with_a_row_without_scale():
     gr, gw = int8_op.head_grads_i8(up.to(DEV), xq, xs, wq, ws, torch.float32, torch.float32, True, True)
     assert torch.isnan(gw).all()
     _check_f16(gr, None, up, x, wq, ws, xs)
+
+
+# ---- dense shares of many blocks: a wave's later weight rows, the prefetch into them, the cut-off last block -------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d,V", [(1, 256, 151936), (17, 64, 70001), (32, 2560, 3001), (20, 4096, 70001), (32, 4800, 515)])
+def test_few_rows_many_blocks(n, d, V, dtype):
+    x, w = _inputs(n, d, V, dtype, n + d)
+    wq, ws = int8_op.quantise_rows(w.to(DEV))
+    _check_logits(int8_op.int8_head(x.to(DEV), wq, ws), x, wq, ws, dtype)
+
+
+@pytest.mark.parametrize("n,d,V,dtype", [(8, 2560, 40003, torch.bfloat16), (8, 2560, 40003, torch.float16),
+                                         (33, 1027, 60001, torch.bfloat16), (33, 1027, 60001, torch.float16),
+                                         (16, 2304, 40003, torch.float32), (33, 1027, 60001, torch.float32)])
+def test_few_rows_gradient_many_steps(n, d, V, dtype):
+    x, w = _inputs(n, d, V, dtype, n)
+    g = (torch.randn(n, V, generator=torch.Generator().manual_seed(7)) / 8).to(dtype)
+    wq, ws = int8_op.quantise_rows(w.to(DEV))
+    xq, xs = int8_op.quantise_rows(x.to(DEV))
+    gr, _ = int8_op.head_grads_i8(g.to(DEV), xq, xs, wq, ws, dtype, dtype, True, False)
+    want, _, bound, _ = _bound_grads(g, x, wq, ws, dtype, dtype)
+    assert ((gr.cpu().double() - want).abs() <= bound).all()
 
 
 # ---- what is saved, and what is not differentiated -----------------------------------------------------------------------
