@@ -344,32 +344,33 @@ int octo_quantise_fp8_rows(const void *w, int64_t ldw, int w_dtype, int64_t V, i
 /* Rows held as 8-bit integers (no counterpart in the reference): x [rows, ldx] (BF16, F16 or F32), group 0 (the row),
  * 32, 64, 128 or 256 values to a scale, groups = group ? ceil(d / group) : 1. Of each group, with a = max |x|:
  *   scale[r * groups + j] = a times 1/127 (both fp32);  q[r * ldq + k] = x / scale to the nearest integer, ties to even
- * from the exact quotient; a < 2^-119: scale 0 and zeros; a not finite: scale NaN and zeros. ldq is a multiple of 16 and
- * q 16-byte aligned; the bytes from d up to the next multiple of 16 are written 0. Rows of x may start at any element.
- * octo_widen_i8_rows: out[r, k] = q scale, rounded once to out_dtype. */
+ * from the exact quotient; a < 2^-119: scale 0 and zeros; a not finite: scale NaN and zeros. ldq is a multiple of 16
+ * and q 16-byte aligned; the bytes from d up to the next multiple of 16 are written 0. Rows of x may start at any
+ * element. octo_widen_i8_rows: out[r, k] = q scale in fp32, rounded to out_dtype. */
 int octo_quantise_i8_rows(const void *x, int64_t ldx, int x_dtype, int64_t rows, int d, int group, int8_t *q,
                           int64_t ldq, float *scale, void *stream);
 int octo_widen_i8_rows(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int d, int group, void *out,
                        int64_t ldo, int out_dtype, void *stream);
 
 /* The head's logits from 8-bit integers (no counterpart in the reference):
- *   logits[r, v] = x_scale[r] w_scale[v] sum_k xq[r, k] wq[v, k], the sum exact, rounded once to z_dtype
- * for n rows of x (quantised here as octo_quantise_i8_rows does, group 0, into xq and x_scale) or, with rows NULL, of xq
- * and x_scale as they are. wq [V, ldw], xq [n, ldxq]: strides multiples of 16, 16-byte aligned, readable up to the next
- * multiple of 16 behind d (xq's bytes there 0; wq's may be any). d <= 131,072; V, n <= 2^21. logits [n, ldz] may start
- * at any element. */
+ *   logits[r, v] = sum_k xq[r, k] wq[v, k] x_scale[r] w_scale[v]
+ * (the sum exact, then in fp32, the scales in this order, rounded to z_dtype) for n rows of x (quantised here as
+ * octo_quantise_i8_rows does, group 0, into xq and x_scale) or, with rows NULL, of xq and x_scale as they are.
+ * wq [V, ldw], xq [n, ldxq]: strides multiples of 16, 16-byte aligned, readable up to the next multiple of 16 behind d
+ * (xq's bytes there 0; wq's may be any), xq from -127 on. d <= 131,072; V, n <= 2^21. logits [n, ldz] may start at any
+ * element. */
 int octo_head_logits_i8(const void *rows, int64_t ldx, int x_dtype, const int8_t *wq, int64_t ldw, const float *w_scale,
                         int64_t n, int d, int V, int8_t *xq, int64_t ldxq, float *x_scale, void *logits, int64_t ldz,
                         int z_dtype, void *stream);
 /* Its gradients for g = dL/dlogits [n, ldg], straight through the rounding (NULL skips one):
  *   grad_rows[r, k] = sum_v g[r, v] w_scale[v] wq[v, k];  grad_w[v, k] = sum_r g[r, v] x_scale[r] xq[r, k]
- * 16-bit g: the products run in its type, the 8-bit operand times its scale rounded once to it (F16: times a power of two
- * as well, which the sum is divided by, so that operands outside f16's numbers keep its 11 bits down to 2^-29 of the
- * largest scale). F32 g (n, V <= 2^20): g times the scale in three bf16 parts (24 bits; a value that bf16 rounds to
- * infinity is one), times the integers,
- * exactly. Summed in fp32 and rounded once. ws: octo_head_grads_i8_workspace_bytes, 256-byte aligned; with room for a
- * copy of g where that is not of 16-bit values, rows of whole 16-byte chunks (V too) and 256 columns or more (g is not
- * read there), for its parts, 6 bytes a value and gradient, where it is F32 (up to 128 rows neither for grad_rows). */
+ * 16-bit g: the products run in its type, the 8-bit operand times its scale rounded once to it (F16: times a power of
+ * two as well, which the sum is divided by, so that operands outside f16's numbers keep its 11 bits down to 2^-29 of
+ * the largest scale). F32 g (n, V <= 2^20): g times the scale in three bf16 parts (24 bits; a value that bf16 rounds to
+ * infinity is one), times the integers, exactly. Summed in fp32 and rounded once. ws:
+ * octo_head_grads_i8_workspace_bytes, 256-byte aligned; with room for a copy of g where that is not of 16-bit values,
+ * rows of whole 16-byte chunks (V too) and 256 columns or more (g is not read there), for its parts, 6 bytes a value
+ * and gradient, where it is F32 (up to 128 rows neither for grad_rows). */
 int octo_head_grads_i8_workspace_bytes(const void *g, int64_t ldg, int g_dtype, int64_t n, int d, int V, int need_rows,
                                        int need_w, size_t *bytes);
 int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq, int64_t ldxq, const float *x_scale,
@@ -377,23 +378,23 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
                        int64_t ld_gr, int gr_dtype, void *grad_w, int64_t ld_gw, int gw_dtype, void *ws,
                        size_t ws_bytes, void *stream);
 
-/* Drafted tokens checked against the target's probabilities (no counterpart in the reference). Sequence s has K + 1 rows
- * of target logits (row i at s ld_seq + i ld_row elements; row i answers the position of draft i, the last the one
- * behind the drafts), K drafts, and their own logits (K rows, or NULL: each draft is certain under its model), lengths[s]
- * of them (clamped to [0, K]; NULL: K). With p = softmax(logits inv_T), q the draft's, u = uniform[s, :]:
+/* Drafted tokens checked against the target's probabilities (no counterpart in the reference). Sequence s has K + 1
+ * rows of target logits (row i at s ld_seq + i ld_row elements; row i answers the position of draft i, the last the one
+ * behind the drafts), K drafts, and their own logits (K rows, or NULL: each draft is certain under its model),
+ * lengths[s] of them (clamped to [0, K]; NULL: K). With p = softmax(logits inv_T), q the draft's, u = uniform[s, :]:
  *   draft i is accepted when u_i q_i(x_i) < p_i(x_i); accepted[s] = a, the first that is not (or the length)
  *   tokens[s, :a] = the accepted drafts, tokens[s, a] = the lowest v whose running sum of r exceeds u_K sum r,
  *   r = max(p_a - q_a, 0) behind a rejected draft (p_a where that leaves nothing), p_a behind the last; -1 further on
  *   logp[s, i] = log p_i(tokens[s, i]), 0 further on
- * Decisions and tokens are those of 64-bit probabilities and sums. logp is rounded once from 64 bits for the drawn token,
- * and below 2^24 logits read (S (K + 1) V, with draft logits S (2 K + 1) V) for all; from there on the accepted drafts'
- * and, when greedy, all tokens' come from row sums of 32-bit exponentials, within 5e-6 before that rounding, so that they
- * may depend on how many sequences the call has. greedy: a draft is accepted when it is its row's first largest logit,
- * which is also the next token; u and the draft logits are not read (may be NULL). A draft outside [0, V), or whose
- * logits' row has no softmax (a NaN, +inf, or nothing above -inf), is rejected and the token drawn from p_a; where p_a
- * has none, the token is -1 and its logp NaN. A u_K that is no number below 1 takes the last v with r_v > 0. Rows behind
- * a sequence's length are not read. K <= OCTO_DRAFTS_MAX, S <= 2^20. Rows may start at any element. ws:
- * octo_verify_workspace_bytes, 16-byte aligned. */
+ * Decisions and tokens are those of 64-bit probabilities and sums. logp is rounded once from 64 bits for the drawn
+ * token, and below 2^24 logits read (S (K + 1) V, with draft logits S (2 K + 1) V) for all; from there on the accepted
+ * drafts' and, when greedy, all tokens' come from row sums of 32-bit exponentials, within 5e-6 before that rounding, so
+ * that they may depend on how many sequences the call has. greedy: a draft is accepted when it is its row's first
+ * largest logit, which is also the next token; u and the draft logits are not read (may be NULL). A draft outside
+ * [0, V), or whose logits' row has no softmax (a NaN, +inf, or nothing above -inf), is rejected and the token drawn
+ * from p_a; where p_a has none, the token is -1 and its logp NaN. A u_K that is no number below 1 takes the last v with
+ * r_v > 0. Rows behind a sequence's length are not read. K <= OCTO_DRAFTS_MAX, S <= 2^20. Rows may start at any
+ * element. ws: octo_verify_workspace_bytes, 16-byte aligned. */
 int octo_verify_workspace_bytes(int64_t S, int K, int V, size_t *bytes);
 int octo_verify_drafts(const void *logits, int64_t ld_seq, int64_t ld_row, const void *draft_logits, int64_t ld_seq_d,
                        int64_t ld_row_d, int dtype, const int64_t *drafts, const int64_t *lengths, const float *uniform,

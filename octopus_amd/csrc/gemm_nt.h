@@ -265,8 +265,8 @@ struct OpColsN {
 };
 
 // OpColsN of a matrix that ends with its last row: what lies at or past K-row op.rows or M value op.extent reads zero
-// where it would lie behind the matrix (op.extent, and the row stride, whole 16-byte chunks; the M values past extent of
-// the rows before are the next rows', and belong to no C).
+// where it would lie behind the matrix (op.extent, and the row stride, whole 16-byte chunks; the M values past extent
+// of the rows before are the next rows', and belong to no C).
 template <int NW, int SUB>
 struct OpColsEdge : OpColsN<NW, SUB> {
   typedef OpColsN<NW, SUB> Base;

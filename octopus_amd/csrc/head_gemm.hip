@@ -429,8 +429,8 @@ __device__ __forceinline__ void store_any(const typename L::V (&acc)[L::NI][L::N
   store_tile<L, OT>(acc, e, m0, n0, mvalid, nvalid, smem);
 }
 
-// A whole-width fp32 tile with nothing to add: store_tile's halves, values and slots, out 16 bytes per lane. grad_W of 8
-// rows of d 2560, V 151,936 (1.56 GB) 352 us, 520 value by value.
+// A whole-width fp32 tile with nothing to add: store_tile's halves, values and slots, out 16 bytes per lane. grad_W of
+// 8 rows of d 2560, V 151,936 (1.56 GB) 352 us, 520 value by value.
 template <class L>
 __device__ __forceinline__ void store_staged4(const typename L::V (&acc)[L::NI][L::NJ], const StoreArgs &e, int64_t m0,
                                               int64_t n0, int64_t mvalid, lds_char *smem) {
@@ -847,11 +847,11 @@ static int go_grads(const Operand &Ah, const Operand &Bh, const GemmShape &sh, c
     hipLaunchKernelGGL((gemm_grads8_kernel<DT, KM_B, KM_EDGE>), grid, dim3(2 * NTHREADS), 0, st, Ah, Bh, sh, eh, Aw, Bw,
                        sw, ew, (unsigned)nh);
   else if (wh_kmajor)
-    hipLaunchKernelGGL((gemm_grads8_kernel<DT, KM_B, KM_A>), grid, dim3(2 * NTHREADS), 0, st, Ah, Bh, sh, eh, Aw, Bw, sw, ew,
-                       (unsigned)nh);
+    hipLaunchKernelGGL((gemm_grads8_kernel<DT, KM_B, KM_A>), grid, dim3(2 * NTHREADS), 0, st, Ah, Bh, sh, eh, Aw, Bw,
+                       sw, ew, (unsigned)nh);
   else
-    hipLaunchKernelGGL((gemm_grads8_kernel<DT, KM_NONE, KM_A>), grid, dim3(2 * NTHREADS), 0, st, Ah, Bh, sh, eh, Aw, Bw, sw,
-                       ew, (unsigned)nh);
+    hipLaunchKernelGGL((gemm_grads8_kernel<DT, KM_NONE, KM_A>), grid, dim3(2 * NTHREADS), 0, st, Ah, Bh, sh, eh, Aw, Bw,
+                       sw, ew, (unsigned)nh);
   OCTO_CHECK_LAUNCH("gemm_grads");
   return OCTO_OK;
 }

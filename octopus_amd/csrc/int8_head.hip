@@ -4,16 +4,17 @@
 //   dx[r, k] = sum_v g[r, v] sw[v] qw[v, k]                (straight through the rounding of rows and weights)
 //   dW[v, k] = sum_r g[r, v] sx[r] qx[r, k]
 //
-// Three routes for the logits, by the rows. Up to 32 read the weight's bytes once and are bound by them (few_i8_kernel: 1
-// row of d 2560, V 151,936 74 us, 5.2 TB/s). Up to 128, and more of a small vocabulary, the same in tiles, two workgroups a
-// CU (64 rows 95 us, 4.3 TB/s with the logits). More are bound by the matrix rate: 8,192 rows 2,740 us, 2.33 POP/s with the
-// logits' 2.5 GB written beside it (without them 2,614; a library product of these integers, which writes 32-bit sums,
-// reaches 1.82).
+// Three routes for the logits, by the rows. Up to 32 read the weight's bytes once and are bound by them (few_i8_kernel:
+// 1 row of d 2560, V 151,936 74 us, 5.2 TB/s). Up to 128, and more of a small vocabulary, the same in tiles, two
+// workgroups a CU (64 rows 95 us, 4.3 TB/s with the logits). More are bound by the matrix rate: 8,192 rows 2,740 us,
+// 2.33 POP/s with the logits' 2.5 GB written beside it (without them 2,614; a library product of these integers, which
+// writes 32-bit sums, reaches 1.82).
 //
-// The gradients are 16-bit products of the widened operands (prepare8_kernel: 190 us at that weight, a write of 778 MB), at
-// the rate of the head's other gradients: 2,048 rows 2,480 us for both, 1.29 PFLOP/s. The rows' gradient of up to 128 reads
-// the 8-bit weight itself (few_dx_kernel). f16 operands are widened times a power of two (f16_range), for which a launch
-// finds the largest scale: 225 rows of d 1024, V 32,000 80.7 us, 76.3 without, where rows of 1e5 gave NaN.
+// The gradients are 16-bit products of the widened operands (prepare8_kernel: 190 us at that weight, a write of 778
+// MB), at the rate of the head's other gradients: 2,048 rows 2,480 us for both, 1.29 PFLOP/s. The rows' gradient of up
+// to 128 reads the 8-bit weight itself (few_dx_kernel). f16 operands are widened times a power of two (f16_range), for
+// which a launch finds the largest scale: 225 rows of d 1024, V 32,000 80.7 us, 76.3 without, where rows of 1e5 gave
+// NaN.
 #include <type_traits>
 
 #include "gemm_nt.h"
@@ -26,13 +27,13 @@ namespace octo {
 constexpr int kMaxD8 = 131072;       // 127^2 d < 2^31
 constexpr int kMaxV8 = 1 << 21;      // a tile's 256 rows of g within 32-bit offsets
 constexpr int64_t kMaxN8 = 1 << 21;  // the same of the transposed rows
-// M-tiles that an XCD walks the tokens with: 2,048 rows at d 2560, V 151,936 795 us in fours, 749 in eights, the same in
-// sixteens, more in thirty-twos.
+// M-tiles that an XCD walks the tokens with: 2,048 rows at d 2560, V 151,936 795 us in fours, 749 in eights, the same
+// in sixteens, more in thirty-twos.
 constexpr int kGroup8 = 8;
-// Tiles of 128 x 128 up to this many rows. The same weight, us with them and with wide ones: 64 rows 95 and 118, 128 104
-// and 119, 192 147 and 126, 256 157 and 133. (Eight waves on the small tile: 128 rows 111.) And where the card holds all of
-// them at once, two a CU: 256 rows of d 1024 V 32,000 20.0 and 22.8, 512 of V 16,000 19.9 and 27.3, 256 of d 4096 V 32,000
-// 41.6 and 46.1; beyond, 512 of V 32,000 31.2 and 27.7, 256 of d 2304 V 64,000 48.8 and 43.2.
+// Tiles of 128 x 128 up to this many rows. The same weight, us with them and with wide ones: 64 rows 95 and 118, 128
+// 104 and 119, 192 147 and 126, 256 157 and 133. (Eight waves on the small tile: 128 rows 111.) And where the card
+// holds all of them at once, two a CU: 256 rows of d 1024 V 32,000 20.0 and 22.8, 512 of V 16,000 19.9 and 27.3, 256 of
+// d 4096 V 32,000 41.6 and 46.1; beyond, 512 of V 32,000 31.2 and 27.7, 256 of d 2304 V 64,000 48.8 and 43.2.
 constexpr int64_t kSmallRows = 128;
 static bool small_tiles(int64_t n, int V) {
   return n <= kSmallRows || cdiv(n, 128) * cdiv(V, 128) <= 2 * octo_tiles::kCus;
@@ -55,20 +56,25 @@ template <int VM, int TOK, int NW_> struct Tile8 {
   typedef OpRowsN<NW, VM / 2, VM> A;
   typedef OpRowsN<NW, TOK / NWN, TOK> B;
   static constexpr int NA = A::NB, NB = B::NB, LDS = ENSLOT * ring5_slot<A, B>();
-  static __device__ __forceinline__ int row(int w, int i, int lane) { return w / NWN * (VM / 2) + i * 16 + 4 * (lane >> 4); }
-  static __device__ __forceinline__ int col(int w, int j, int lane) { return w % NWN * (TOK / NWN) + j * 16 + (lane & 15); }
+  static __device__ __forceinline__ int row(int w, int i, int lane) {
+    return w / NWN * (VM / 2) + i * 16 + 4 * (lane >> 4);
+  }
+  static __device__ __forceinline__ int col(int w, int j, int lane) {
+    return w % NWN * (TOK / NWN) + j * 16 + (lane & 15);
+  }
 };
-typedef Tile8<256, 256, 8> TileWide;    // one workgroup a CU
-typedef Tile8<256, 192, 8> Tile192;     // the last tokens of a wide grid: 320 rows of d 4096 228 us without, 209 with
+typedef Tile8<256, 256, 8> TileWide;   // one workgroup a CU
+typedef Tile8<256, 192, 8> Tile192;    // the last tokens of a wide grid: 320 rows of d 4096 228 us without, 209 with
 typedef Tile8<256, 128, 8> Tile128;
-typedef Tile8<128, 128, 4> TileSmall;   // half the LDS: two workgroups a CU, one of which loads and multiplies while the
-                                        // other begins or stores
+typedef Tile8<128, 128, 4> TileSmall;  // half the LDS: two workgroups a CU, one loading and multiplying while the other
+                                       // begins or stores
 
-// Scaled, rounded once, and out through the LDS in rows of the tile's logits. A slot holds 4 logits; slot s of token t
-// sits at s ^ 4 (t & 15) (128 logits: t & 7): a write's 16 tokens x 4 slots cover all banks.
+// Scaled in fp32 (the sum, times the token's scale, times the weight's), rounded to the logits' type, and out through
+// the LDS in rows of the tile's logits. A slot holds 4 logits; slot s of token t sits at s ^ 4 (t & 15) (128 logits: t
+// & 7): a write's 16 tokens x 4 slots cover all banks.
 template <class L, typename OT>
-__device__ __forceinline__ void store_logits8(const f32x4 (&acc)[L::NA][L::NB], const Logits8 &e, int64_t v0, int64_t n0,
-                                              int V, int64_t nvalid, lds_char *smem) {
+__device__ __forceinline__ void store_logits8(const f32x4 (&acc)[L::NA][L::NB], const Logits8 &e, int64_t v0,
+                                              int64_t n0, int V, int64_t nvalid, lds_char *smem) {
   constexpr int SLOT = 4 * sizeof(OT), ROW = L::ROWS / 4 * SLOT, HALVES = L::TOKENS * ROW > L::LDS ? 2 : 1;
   constexpr int TOK = L::TOKENS / HALVES;
   constexpr int LPR = ROW / 16, PER = 16 / sizeof(OT), SWZ = L::ROWS / 16 - 1;  // lanes of a row, logits of a lane
@@ -131,8 +137,8 @@ __device__ __forceinline__ void gemm_i8_tile(const Operand &A, const Operand &B,
   store_logits8<L, OT>(acc, e, m0, n0, (int)s.M, min(s.N - n0, (int64_t)L::TOKENS), smem);
 }
 template <typename OT>
-__global__ __launch_bounds__(512, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_kernel(Operand A, Operand B,
-                                                                                                    GemmShape s, Logits8 e) {
+__global__ __launch_bounds__(512, 1) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void gemm_i8_kernel(Operand A, Operand B, GemmShape s, Logits8 e) {
   __shared__ __attribute__((aligned(16))) char smem_[TileWide::LDS];
   int mt, nt;
   if (!tile_of(s, mt, nt)) return;
@@ -142,25 +148,29 @@ __global__ __launch_bounds__(512, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   else gemm_i8_tile<TileWide, OT>(A, B, s, e, m0, n0, (lds_char *)smem_);
 }
 template <typename OT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_i8_small_kernel(Operand A, Operand B,
-                                                                                                       GemmShape s,
-                                                                                                       Logits8 e) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void gemm_i8_small_kernel(Operand A, Operand B, GemmShape s, Logits8 e) {
   __shared__ __attribute__((aligned(16))) char smem_[TileSmall::LDS];
   int mt, nt;
-  if (tile_of(s, mt, nt)) gemm_i8_tile<TileSmall, OT>(A, B, s, e, (int64_t)mt * 128, (int64_t)nt * 128, (lds_char *)smem_);
+  if (!tile_of(s, mt, nt)) return;
+  gemm_i8_tile<TileSmall, OT>(A, B, s, e, (int64_t)mt * 128, (int64_t)nt * 128, (lds_char *)smem_);
 }
 
-// ---- few rows --------------------------------------------------------------------------------------------------------
+// ---- few rows -------------------------------------------------------------------------------------------------------
 //
-// Up to 32 rows the weight's bytes set the time. The rows, quantised by every workgroup for itself (which saves a launch;
-// workgroup 0 leaves them to the caller), stay in the LDS, and each wave runs through a share of the weight rows of its
-// own, 16 at a time: the MFMA's first operand comes from global memory as it lies (lane l: row l & 15, 16 bytes at
-// 16 (l >> 4) of each 64), kFewSteps loads ahead, also into the next 16 rows, and no wave waits for another. The shares
-// are equal to 4 rows, so that all waves end together: in blocks of 16 rows 9,496 blocks on 6,144 waves take as long as
-// 12,288 would. A share's last block repeats its last row (no bytes of its own, and its MFMAs are idle time).
+// Up to 32 rows the weight's bytes set the time. The rows, quantised by every workgroup for itself (which saves a
+// launch; workgroup 0 leaves them to the caller), stay in the LDS, and each wave runs through a share of the weight
+// rows of its own, 16 at a time: the MFMA's first operand comes from global memory as it lies (lane l: row l & 15, 16
+// bytes at 16 (l >> 4) of each 64), kFewSteps loads ahead, also into the next 16 rows, and no wave waits for another.
+// The shares are equal to 4 rows, so that all waves end together: of 16 rows each, 9,496 blocks would take the 4,096
+// waves of 16 a CU three rounds, as long as 12,288. A share's last block repeats its last row (no bytes of its own, and
+// its MFMAs are idle time).
 //
-// d 2560, V 151,936, us so and in tiles of 256 x 256: 1 row 80 and 108, 16 89 and 108, 32 97 and 109; at 33 the small
-// tiles take 96, this 102. Weight loads past the caches (nontemporal): 100 for 1 row.
+// us so and in the small tiles: d 2560, V 151,936, bf16 1 row 74 and 90, 8 80 and 91, 16 87 and 91, 24 94 and 92, 32 96
+// and 92, fp32 1 row 75 and 91, 16 91 and 91, 32 102 and 92; d 4096, V 128,256, bf16 1 row 109 and 121, 17 125 and 124,
+// 32 125 and 126; d 1024, V 32,000, bf16 1 row 8.6 and 12.2, 8 9.5 and 12.5, 16 13.3 and 12.5, 32 18.7 and 12.5. So the
+// crossing lies at 12 to 24 rows, below the limit. Weight loads past the caches (nontemporal) take a quarter longer for
+// 1 row.
 constexpr int kFewSteps = 8;
 constexpr int kFewLds = 156 * 1024;  // with the scales, what a workgroup can have
 constexpr int64_t kFewRows = 32;
@@ -201,11 +211,12 @@ __global__ __launch_bounds__(64 * NW) void few_i8_kernel(Few8 a) {
   for (int r = w; r < a.n; r += NW) {
     lds_char *row = smem + r * ld;
     int8_t *kept = blockIdx.x == 0 ? a.xq + r * a.ldxq : nullptr;
-    const float s = quantise_row<DT, (DT == OCTO_F32 ? 2 : 4)>((const typename Elem<DT>::T *)a.x + r * a.ldx, a.d, (a.d + 63) / 64 * 8,
-                                     [&](int c, i32x2 v) {
+    const auto *x = (const typename Elem<DT>::T *)a.x + r * a.ldx;
+    auto put = [&](int c, i32x2 v) {
       *(__attribute__((address_space(3))) i32x2 *)(row + 8 * c) = v;
       if (kept && c < 2 * chunks) *(i32x2 *)(kept + 8 * c) = v;
-    });
+    };
+    const float s = quantise_row<DT, (DT == OCTO_F32 ? 2 : 4)>(x, a.d, (a.d + 63) / 64 * 8, put);
     if (lane == 0) {
       scales[r] = s;
       if (kept) a.sx[r] = s;
@@ -287,14 +298,21 @@ template <typename OT> static int go_few(const Few8 &a, int x_dtype, hipStream_t
 // ---- few rows' gradient --------------------------------------------------------------------------------------------
 //
 // dx of few rows is the weight's bytes too, which a widened copy multiplies by five. Here a wave takes a share of the
-// vocabulary and 256 columns: lane l holds 16 columns (16 bytes at 16 (l & 15)) of 8 rows (8 (l >> 4) ..) of each 32, so
-// that its 8 bytes of a column are 8 neighbours along K, and product j of 16 takes column j of every lane: widened, rounded
-// to g's type and fed without an exchange between lanes. f16: each wave widens by the power of two of its own share's scales
-// (f16_range) and takes it back before the sums are joined. fp32 g: the integers and g's three parts, as in the large
-// products. A workgroup's waves join their sums in the LDS, a second launch the workgroups', both in order.
+// vocabulary and 256 columns: lane l holds 16 columns (16 bytes at 16 (l & 15)) of 8 rows (8 (l >> 4) ..) of each 32,
+// so that its 8 bytes of a column are 8 neighbours along K, and product j of 16 takes column j of every lane: widened,
+// rounded to g's type and fed without an exchange between lanes. f16: each wave widens by the power of two of its own
+// share's scales (f16_range) and takes it back before the sums are joined. fp32 g: the integers and g's three parts, as
+// in the large products. A workgroup's waves join their sums in the LDS, a second launch the workgroups', both in
+// order.
 //
-// d 2560, V 151,936, us so and by the widened copy: bf16 8 rows 82 (4.8 TB/s) and 404, 32 88 and 403, 64 144 and 404, 128
-// 269 and 409 (blocks of 32 tokens run side by side and share some of their reads); fp32 8 rows 88 and 687, 128 576 and 767.
+// us so and by the widened copy: d 2560, V 151,936, bf16 8 rows 80 (4.9 TB/s) and 404, 32 89 and 403, 64 145 and 404,
+// 128 270 and 408, 160 326 and 409, 192 391 and 412, 225 510 and 413 (blocks of 32 tokens run side by side and share
+// some of their reads); fp32 8 rows 88 and 687, 128 574 and 761, 160 865 and 793; d 1024, V 32,000, bf16 128 rows 34
+// and 57, 225 50 and 58, 384 72 and 64, fp32 128 53 and 92, 256 98 and 108, 384 183 and 136. So the crossing lies
+// between 129 rows (fp32, large) and some 300 (small), at or above the limit.
+//
+// g times the scale in two bf16 parts against the integers, which rounds no operand to g's type, takes twice the
+// products: 16 rows 82 us, but 32 138 and 128 426.
 constexpr int kDxCols = 256, kDxWaves = 8;
 constexpr int64_t kFewDx = 128;
 
@@ -422,7 +440,8 @@ __global__ __launch_bounds__(64 * kDxWaves) void few_dx_kernel(FewDx a) {
   }
 }
 
-// The workgroups' sums joined: register r = 16 b + j of lane l holds token 16 b + (l & 15), columns 64 (l >> 4) + 16 e + j.
+// The workgroups' sums joined: register r = 16 b + j of lane l holds token 16 b + (l & 15), columns 64 (l >> 4) + 16 e
+// + j.
 template <typename OT, int NB>
 __global__ __launch_bounds__(256) void few_dx_sum_kernel(FewDx a) {
   constexpr int R = 16 * NB;
@@ -508,13 +527,18 @@ static GemmShape shape8(int64_t M, int64_t N, int64_t K, int tile = TM) {
 }
 
 // Workspace of the gradients: the widened weight [V, d] (K-major for dx) and the partial tiles of its split; the
-// transposed rows [d, n]; g where its rows cannot be read as they are (g_as_is). Sizes padded as the K-major loads read.
+// transposed rows [d, n]; g where its rows cannot be read as they are (g_as_is). Sizes padded as the K-major loads
+// read.
 //
-// fp32 g is not multiplied in fp32: an 8-bit integer is a bf16 number as it stands, so g times the scale that its product
-// sums over, in three bf16 parts, times the integers is exact but for the sum: three bf16 products, where two fp32
-// operands take six. dx: the parts beside each other, K = 3 Vr through the weight's rows three times. dW: the parts below
-// each other, K = 3 np against the rows' integers three times. d 2560, V 151,936, both gradients of 512 rows 2,500 us,
-// 4,700 as fp32 products (a library's 6,700).
+// 16-bit g: the widened operand is rounded to its type, as the head's other gradients take their operands: 2.4e-3 from
+// 64 bits in bf16, sqrt(2) times one rounding of an exact result. Two parts of g times the scale against the exact
+// integers would double the products, which are most of the time; fp32 logits have gradients within 1e-6.
+//
+// fp32 g is not multiplied in fp32: an 8-bit integer is a bf16 number as it stands, so g times the scale that its
+// product sums over, in three bf16 parts, times the integers is exact but for the sum: three bf16 products, where two
+// fp32 operands take six. dx: the parts beside each other, K = 3 Vr through the weight's rows three times. dW: the
+// parts below each other, K = 3 np against the rows' integers three times. d 2560, V 151,936, both gradients of 512
+// rows 2,500 us, 4,700 as fp32 products (a library's 6,700).
 struct Grads8Layout {
   int64_t Vr, dp, np, Vp;  // rows and columns of the copies
   int64_t Kh;              // dx's K
@@ -550,7 +574,8 @@ static Grads8Layout grads8_layout(int64_t n, int d, int V, int dtype, bool need_
   }
   L.wide = take(need_rows ? (size_t)L.Vr * L.dp * 2 : 0);
   L.xt = take(need_w ? (size_t)d * L.parts * L.np * 2 : 0);
-  L.g = take(L.parts == 1 ? (as_is || !(need_rows || need_w) ? 0 : (size_t)L.np * L.Vp * 2) : (need_w ? (size_t)3 * L.np * L.Vp * 2 : 0));
+  const bool copied = L.parts == 3 ? need_w : !as_is && (need_rows || need_w);
+  L.g = take(copied ? (size_t)L.parts * L.np * L.Vp * 2 : 0);
   L.gh = take(L.parts == 3 && need_rows ? (size_t)n * L.Kh * 2 : 0);
   L.split = take(L.few ? dx_split(n, d, V, dtype).bytes : (size_t)L.split_items * TM * TN * 4);
   L.norm = take(dtype == OCTO_F16 && (need_rows || need_w) ? sizeof(Norm8) : 0);
@@ -558,8 +583,8 @@ static Grads8Layout grads8_layout(int64_t n, int d, int V, int dtype, bool need_
   return L;
 }
 
-// Whether the products can read g where it lies (2,048 rows of V 151,936: 2,728 us, 2,850 with a copy): 16-bit values in whole 16-byte chunks, a tile's rows and a stage's within
-// 32-bit offsets.
+// Whether the products can read g where it lies (2,048 rows of V 151,936: 2,728 us, 2,850 with a copy): 16-bit values
+// in whole 16-byte chunks, a tile's rows and a stage's within 32-bit offsets.
 static bool g_as_is(const void *g, int64_t ldg, int dtype, int V) {
   return dtype != OCTO_F32 && V % 8 == 0 && V >= TM && ldg % 8 == 0 && ldg <= kMaxV8 && (uintptr_t)g % 16 == 0;
 }
@@ -688,8 +713,8 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
   if (rc) return rc;
   if (L.few) {
     const DxSplit s = dx_split(n, d, V, g_dtype);
-    const FewDx a{g, ldg, wq, ldw, w_scale, (int)n, d, V, s.strips, s.groups, s.share, (f32x4 *)(wsb + L.split), grad_rows,
-                  ld_gr};
+    const FewDx a{g,        ldg,      wq,      ldw,                      w_scale,   (int)n, d, V,
+                  s.strips, s.groups, s.share, (f32x4 *)(wsb + L.split), grad_rows, ld_gr};
     rc = go_few_dx(a, s, g_dtype, gr_dtype, st);
     if (rc) return rc;
   }
@@ -722,9 +747,9 @@ int octo_head_grads_i8(const void *g, int64_t ldg, int g_dtype, const int8_t *xq
     ow.dtype = gw_dtype;
     ow.alpha = p.norm ? &p.norm->back[1] : nullptr;
   }
-  // Both in one launch, dx's runs as long as if it had the card to itself: dW's short tiles follow them on every CU. Two
-  // launches take 20 us more up to 700 rows of d 2560, V 151,936 and as long from 1,024 on; runs cut for sharing the card
-  // (fewer, longer ones) 949 us for 300 rows against 835.
+  // Both in one launch, dx's runs as long as if it had the card to itself: dW's short tiles follow them on every CU.
+  // Two launches take 20 us more up to 700 rows of d 2560, V 151,936 and as long from 1,024 on; runs cut for sharing
+  // the card (fewer, longer ones) 949 us for 300 rows against 835.
   const bool both = wide && grad_w && !f32;
   if (both) rc = launch_gemm_grads(dt, Ah, Bh, sh, oh, true, Aw, Bw, sw, ow, st, kma);
   else if (wide) rc = launch_gemm_store(dt, Ah, Bh, sh, oh, st, f32 ? KM_WRAP : KM_B);

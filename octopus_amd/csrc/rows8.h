@@ -7,8 +7,8 @@ namespace octo {
 
 constexpr float kLeastMax = 0x1p-119f;
 
-// 8 consecutive values as they lie, from an address of any element alignment (global loads of 16 bytes need none); zeros
-// from `valid` on.
+// 8 consecutive values as they lie, from an address of any element alignment (global loads of 16 bytes need none);
+// zeros from `valid` on.
 typedef i32x4 i32x4_any __attribute__((aligned(2)));
 typedef i32x4 i32x4_any4 __attribute__((aligned(4)));
 template <int DT> struct Raw8 {
@@ -93,7 +93,8 @@ __device__ __forceinline__ i32x2 quotients(const float (&x)[8], float s, float i
 }
 
 // A row's scale and quotients by one wave, N chunks a lane at a time: put(chunk, bytes) for every chunk of 8 up to
-// `padded` of them (zeros past the row), each by one lane. A row of up to 512 N values is read once, a longer one twice.
+// `padded` of them (zeros past the row), each by one lane. A row of up to 512 N values is read once, a longer one
+// twice.
 template <int DT, int N, class F>
 __device__ __forceinline__ float quantise_row(const typename Elem<DT>::T *row, int d, int padded, F put) {
   const int lane = threadIdx.x & 63, chunks = (d + 7) >> 3;
@@ -121,8 +122,8 @@ __device__ __forceinline__ float quantise_row(const typename Elem<DT>::T *row, i
   return s;
 }
 
-// 8 fp32 values as three bf16 parts each, whose sum they are (24 bits; one that bf16 cannot hold stays in the first part
-// alone).
+// 8 fp32 values as three bf16 parts each, whose sum they are (24 bits; one that bf16 cannot hold stays in the first
+// part alone).
 __device__ __forceinline__ void split_parts(const float (&x)[8], i32x4 (&part)[3]) {
   float p0[8], p1[8], p2[8];
 #pragma unroll
@@ -137,9 +138,9 @@ __device__ __forceinline__ void split_parts(const float (&x)[8], i32x4 (&part)[3
   part[2] = pack8(p2, false);
 }
 
-// Integers times scales as f16 numbers: bf16 and fp32 rows, and scales as a caller gives them, may lie outside f16's range.
-// times: the power of two that brings 127 of the largest finite scale to [2^14, 2^15), short of f16's infinity (that of
-// -128 too), with f16's 11 bits down to 2^-29 of it; back: its inverse, for the sum. maxbits: that scale's.
+// Integers times scales as f16 numbers: bf16 and fp32 rows, and scales as a caller gives them, may lie outside f16's
+// range. times: the power of two that brings the largest finite scale to [2^7, 2^8), so that 128 of it stays short of
+// f16's infinity and its 11 bits reach down to 2^-29 of it; back: the inverse, for the sum. maxbits: that scale's.
 __device__ __forceinline__ uint32_t finite_bits(float s) {
   const uint32_t b = __float_as_uint(s) & 0x7fffffffu;
   return b < 0x7f800000u ? b : 0;

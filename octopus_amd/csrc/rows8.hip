@@ -1,15 +1,15 @@
 // Rows held as 8-bit integers with fp32 scales (octo_quantise_i8_rows, octo_widen_i8_rows), and the copies that the
 // gradients of the 8-bit head multiply with (launch_prepare8).
 //
-//   a = max |x| of a group of a row's values (the whole row, or 32 to 256 of them), scale = a times 1/127, both in fp32,
-//   q = the exact quotient x / scale to the nearest integer, ties to even;   x^ = q scale, rounded once
+//   a = max |x| of a group of a row's values (the whole row, or 32 to 256 of them), scale = a times 1/127 in fp32,
+//   q = the exact quotient x / scale to the nearest integer, ties to even;   x^ = q scale in fp32, then in x's type
 //
 // A group below 2^-119 (its scale would not be a normal number) is held as zeros, one with a NaN or an infinity as NaN
 // (scale NaN, q 0).
 //
 // Bound by memory: a wave per row, 16-byte loads of 8 values (fp32: two), a row of up to 4,096 values in registers
-// between its maximum and its quotients. 32,768 x 2,560 bf16: quantised 48 us (5.3 TB/s; groups of 128 54 to 62), widened
-// 40 us (6.3 TB/s, part of it from the caches); a copy of such rows takes 63.
+// between its maximum and its quotients. 32,768 x 2,560 bf16: quantised 48 us (5.3 TB/s; groups of 128 54 to 62),
+// widened 40 us (6.3 TB/s, part of it from the caches); a copy of such rows takes 63.
 #include "octo_internal.h"
 #include "row_values.h"
 #include "rows8.h"
@@ -52,8 +52,8 @@ __global__ __launch_bounds__(256) void quantise_i8_kernel(const typename Elem<DT
 // Few rows, a scale each: a workgroup per row, whose chain of instructions is the time. 320 rows of 4,096 bf16 values
 // 4.0 us so, 7.2 by a wave each; 2,048 of 2,560 6.6 and 7.4; 8,192 17.2 and 16.7.
 template <int DT>
-__global__ __launch_bounds__(256) void quantise_i8_row_kernel(const typename Elem<DT>::T *x, int64_t ldx, int d, int8_t *q,
-                                                              int64_t ldq, float *scale) {
+__global__ __launch_bounds__(256) void quantise_i8_row_kernel(const typename Elem<DT>::T *x, int64_t ldx, int d,
+                                                              int8_t *q, int64_t ldq, float *scale) {
   constexpr int N = 2;  // chunks of 8 values a thread keeps
   __shared__ uint32_t top[4];
   const int64_t r = blockIdx.x;
@@ -97,9 +97,9 @@ __device__ __forceinline__ void unpack_i8(const i32x2 v, float s, float (&x)[8])
 }
 
 // Row r of out = q scale for the columns c < d, zeros up to cols_pad (and for all of a row past `rows`), by one wave, 4
-// chunks of 8 columns a lane in flight. gshift: log2 of the group, or -1. The bytes of q behind d are readable up to the
-// next multiple of 16. UNIT: the integers themselves (exact in every type). times(): a power of two for all scales, asked
-// for with the loads in flight.
+// chunks of 8 columns a lane in flight. gshift: log2 of the group, or -1. The bytes of q behind d are readable up to
+// the next multiple of 16. UNIT: the integers themselves (exact in every type). times(): a power of two for all scales,
+// asked for with the loads in flight.
 struct TimesOne {
   __device__ __forceinline__ float operator()() const { return 1.f; }
 };
@@ -163,8 +163,8 @@ template <int DT> struct RangeTimes {
   }
 };
 
-// xt[c, r] = q[r, c] scale[r] for c < d, r0 <= r < r0 + 64; zeros from n on; `repeats` of it np columns apart. A 64 x 64
-// tile through the LDS.
+// xt[c, r] = q[r, c] scale[r] for c < d, r0 <= r < r0 + 64; zeros from n on; `repeats` of it np columns apart. A 64 x
+// 64 tile through the LDS.
 template <int DT, bool UNIT = false, class F>
 __device__ __forceinline__ void widen_t_tile(const Prepare8 &a, int64_t r0, int c0, int repeats,
                                              typename Elem<DT>::T (*tile)[64 + 16 / Elem<DT>::bytes], F times) {
@@ -258,7 +258,7 @@ __device__ __forceinline__ void stage_f32(const Prepare8 &a, int64_t r, int part
 template <int DT>
 __global__ __launch_bounds__(256) void prepare8_kernel(Prepare8 a) {
   constexpr bool F32 = DT == OCTO_F32;
-  constexpr int WT = F32 ? OCTO_BF16 : DT;  // fp32 g multiplies with the integers in bf16, its parts with the scales in g
+  constexpr int WT = F32 ? OCTO_BF16 : DT;  // fp32 g: the integers in bf16, the scales in g's parts
   typedef typename Elem<WT>::T T;
   __shared__ __attribute__((aligned(16))) T tile[64][64 + 16 / sizeof(T)];
   unsigned b = a.first + blockIdx.x;
@@ -281,7 +281,8 @@ __global__ __launch_bounds__(256) void prepare8_kernel(Prepare8 a) {
 }
 
 // The largest finite scales of 64 shares of the weights (blocks 0 .. 63) and of the rows, for f16_range.
-__global__ __launch_bounds__(256) void norm8_kernel(const float *ws, int64_t V, const float *xs, int64_t n, Norm8 *norm) {
+__global__ __launch_bounds__(256) void norm8_kernel(const float *ws, int64_t V, const float *xs, int64_t n,
+                                                    Norm8 *norm) {
   __shared__ uint32_t top[4];
   const int k = blockIdx.x >> 6, part = blockIdx.x & 63, t = threadIdx.x;
   const float *s = k ? xs : ws;
@@ -327,8 +328,8 @@ template <int DT>
 static void go_widen(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int d, int group, void *out,
                      int64_t ldo, hipStream_t st) {
   const int gshift = group ? __builtin_ctz((unsigned)group) : -1, groups = group ? (int)cdiv(d, group) : 1;
-  hipLaunchKernelGGL(widen_i8_kernel<DT>, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, q, ldq, scale, rows, d, gshift,
-                     groups, (typename Elem<DT>::T *)out, ldo);
+  hipLaunchKernelGGL(widen_i8_kernel<DT>, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, q, ldq, scale, rows, d,
+                     gshift, groups, (typename Elem<DT>::T *)out, ldo);
 }
 
 template <int DT>

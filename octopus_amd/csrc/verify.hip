@@ -2,27 +2,27 @@
 //
 //   p_i = softmax(z_i / T), q_i = softmax(z'_i / T), or all of it at the draft where the drafts come without logits.
 //   Draft i is accepted when u_i q_i(x_i) < p_i(x_i); the first that is not ends the sequence at a. The next token is
-//   the lowest v whose running sum of r_w = max(p_a(w) - q_a(w), 0) exceeds u_K sum r, and r = p_a after the last draft.
+//   the lowest v whose running sum of r_w = max(p_a(w) - q_a(w), 0) exceeds u_K sum r; r = p_a after the last draft.
 //
 // Which token that is has to be the definition's, not one beside it: of 150,000 running sums some lie within fp32's
 // rounding of any number, and then another token is answered. So the exponentials and sums are taken in 64 bits
-// (exp2_64 below, 4e-16 relative; some 1e-15 with its argument's rounding), and a draw differs from the exact one with a
-// probability of about V times that.
+// (exp2_64 below, 4e-16 relative; some 1e-15 with its argument's rounding), and a draw differs from the exact one with
+// a probability of about V times that.
 //
 // Rows are summed by waves, a part of a row each, in an order that the sizes alone decide. Few logits take three
 // launches, all in 64 bits:
 //   stats     each part's maximum and its sum of exponentials against it, every row that a sequence may need
 //   residual  each workgroup joins its sequence's rows, finds a by itself, and its waves sum their parts' r
 //   pick      a workgroup per sequence finds the part in which the running sum passes u_K sum r, and in it the token
-// Many take the exponentials of stats in 32 bits (64-bit ones are 20 instructions each, and stats is most of the work),
-// which leave each row's sum within 5e-6 (see fast_spread). That decides a draft unless u q and p are closer than 2^-15;
-// then the row and its draft's are summed again in 64 bits there. Accepted drafts' and greedy's log-probabilities keep
-// those sums, and with them the 5e-6. decide, sums and rest take residual's place: a is found
+// Many take the exponentials of stats in 32 bits (64-bit ones are 20 instructions each with their argument, and stats
+// is most of the work), which leave each row's sum within 5e-6 (see fast_spread). That decides a draft unless u q and p
+// are closer than 2^-15; then the row and its draft's are summed again in 64 bits there. Accepted drafts' and greedy's
+// log-probabilities keep those sums, and with them the 5e-6. decide, sums and rest take residual's place: a is found
 // once a sequence, and one sweep over row a of both models finds in 64 bits their sums and those of r (part_sums).
 //
-// Few logits are bound by the launches' latency (one sequence, 4 drafts, V 151,936: 6 + 8 + 6 us), many by memory and by
-// 64-bit arithmetic: 256 sequences of up to 7 drafts, bf16, statistics 181 us for 1.1 GB, sums 80 us for 2 x 39 million
-// exponentials, the other three 33 us.
+// Few logits are bound by the launches' latency (one sequence, 4 drafts, V 151,936: 6 + 8 + 6 us), many by memory and
+// by 64-bit arithmetic: 256 sequences of up to 7 drafts, bf16, statistics 175 us for 1.1 GB, sums 79 us for 2 x 39
+// million exponentials, the other three 33 us.
 #include "octo_common.h"
 #include "row_values.h"
 #include "rows8.h"
@@ -36,9 +36,9 @@ constexpr int kVBlock = 2048;   // values that a wave holds at a time: 4 chunks 
 constexpr double kVClose = 1.0 / 32768;
 constexpr double kVLn2 = 0.69314718055994530942;
 
-// 2^t for t <= 0, -inf included (below -1000: 0), within 4e-16 of its value: t = n + f, |f| <= 1/2, n from the last bits
-// of t + 1.5 x 2^52, and 2^f by the polynomial of degree 10 through it at the 11 Chebyshev nodes of [-1/2, 1/2]: 17
-// instructions, no conversion, rounding or ldexp of 64 bits.
+// 2^t for t <= 0, -inf included (below -1000: 0), within 4e-16 of its value: t = n + f, |f| <= 1/2, n from the last
+// bits of t + 1.5 x 2^52, and 2^f by the polynomial of degree 10 through it at the 11 Chebyshev nodes of [-1/2, 1/2]:
+// 17 instructions, no conversion, rounding or ldexp of 64 bits.
 __device__ __forceinline__ double exp2_64(double t) {
   const double shift = 6755399441055744.0, b = t + shift, f = t - (b - shift);
   double e = 7.072585949269223e-09;
@@ -114,8 +114,8 @@ __device__ __forceinline__ const typename Elem<DT>::T *row_of(const void *z, int
   return (const typename Elem<DT>::T *)z + s * ls + i * lr;
 }
 
-// Chunk u of a lane of the kVBlock values from column c on: columns c + 512 u + 8 lane .. + 7, -inf from c1 on. Rows may
-// start at any element (16-byte global loads need no alignment).
+// Chunk u of a lane of the kVBlock values from column c on: columns c + 512 u + 8 lane .. + 7, -inf from c1 on. Rows
+// may start at any element (16-byte global loads need no alignment).
 typedef i32x4 i32x4_any2 __attribute__((aligned(2)));
 typedef i32x4 i32x4_any4 __attribute__((aligned(4)));
 template <int DT>
@@ -216,11 +216,11 @@ __device__ __forceinline__ PartStat exact_part(const VerifyArgs &a, const typena
   return r;
 }
 
-// A wave's run of blocks with exponentials in 32 bits, the next block's loads in flight. exp2 is within 2^-23 of its value,
-// and its argument (z - m) c, c rounded to 32 bits, off by at most 1.5 x 2^-23 of itself (d, c and the product), which
-// makes ln 2 times that of the value: over a row at most 2^-23 (1 + 1.04 x 30), as the mean of |d c| under the softmax is
-// at most log2 V. Eight values are summed in 32 bits (3 x 2^-24), all else in 64. Together below 5e-6 of the row's sum.
-// A NaN stays one through difference, product and exponential, and +inf makes one (inf - inf): S shows both.
+// A wave's run of blocks with exponentials in 32 bits, the next block's loads in flight. exp2 is within 2^-23 of its
+// value, and its argument (z - m) c, c rounded to 32 bits, off by at most 1.5 x 2^-23 of itself (d, c and the product),
+// which makes ln 2 times that of the value: over a row at most 2^-23 (1 + 1.04 x 30), as the mean of |d c| under the
+// softmax is at most log2 V. Eight values are summed in 32 bits (3 x 2^-24), all else in 64. Together below 5e-6 of the
+// row's sum. A NaN stays one through difference, product and exponential, and +inf makes one (inf - inf): S shows both.
 template <int DT>
 __device__ __forceinline__ PartStat fast_spread(const VerifyArgs &a, const typename Elem<DT>::T *row, int c0, int c1) {
   float m = -INFINITY;
@@ -455,9 +455,9 @@ __global__ __launch_bounds__(kVDecide) void verify_decide_kernel(VerifyArgs a) {
 
 // With S_p and S_q the rows' sums, r > 0 where e_p > rho e_q, rho = S_p / S_q, and there r = e_p / S_p - e_q / S_q: one
 // sweep finds the sums of e_p and e_q over all columns and over those, for which it is enough to know rho within 2^-15
-// (the statistics give it within 1e-5), unless a column's e_p lies that close to rho e_q. A part with such a column (one
-// in fifty where the models differ) is left to the next launch. 256 sequences of V 151,936: the call 358 us in kernels so,
-// 388 with a sweep for S_p and S_q and another for r.
+// (the statistics give it within 1e-5), unless a column's e_p lies that close to rho e_q. A part with such a column
+// (one in fifty where the models differ) is left to the next launch. 256 sequences of V 151,936: the call 358 us in
+// kernels so, 388 with a sweep for S_p and S_q and another for r.
 template <int DT, int MODE>
 __device__ __forceinline__ void part_sums(const VerifyArgs &a, const VerifyArgs::Decision &d, int64_t s, int k, int c0,
                                           int c1) {
@@ -554,7 +554,8 @@ __global__ __launch_bounds__(kVThreads) void verify_residual_kernel(VerifyArgs a
   const int k = __builtin_amdgcn_readfirstlane(blockIdx.x * kVWaves + (threadIdx.x >> 6));
   if (k >= a.parts) return;
   const int c0 = k * a.part, c1 = (int)min((int64_t)a.V, (int64_t)c0 + a.part);
-  const double S = d.residual == 1 ? part_mass<DT, 1>(a, d, row, rowd, c0, c1) : part_mass<DT, 2>(a, d, row, rowd, c0, c1);
+  const double S =
+      d.residual == 1 ? part_mass<DT, 1>(a, d, row, rowd, c0, c1) : part_mass<DT, 2>(a, d, row, rowd, c0, c1);
   if ((threadIdx.x & 63) == 0) a.sum_a[s * a.parts + k] = S;
 }
 
@@ -755,16 +756,19 @@ __global__ __launch_bounds__(kVThreads) void verify_pick_kernel(VerifyArgs a) {
   }
 }
 
-// Parts of one block, and as many blocks more as keep a row within kVParts parts: pick scans a row's parts in the LDS and
-// sweeps one again. A wave that takes several of them in sums measured the same.
+// Parts of one block, and as many blocks more as keep a row within kVParts parts: pick scans a row's parts in the LDS
+// and sweeps one again. A wave that takes several of them in sums measured the same.
 static int part_values(int V) { return (int)round_up(cdiv(V, kVParts), kVBlock); }
 
 // Rows that are summed with 32-bit exponentials, from this many logits on. V 128,256, 4 drafts with logits, us a call
-// without and with: 9.2M logits 32.3 and 37.0, 18.5M 40.9 and 41.4, 36.9M 56.0 and 50.5, 73.9M 89.5 and 74.5.
+// without and with: 9.2M logits 32.3 and 37.0, 18.5M 40.9 and 41.4, 36.9M 56.0 and 50.5, 73.9M 89.5 and 74.5. V
+// 151,936: 128 sequences of one draft without logits 74.1 and 54.6, with them 82.2 and 74.6; 256 of 4 drafts 377 and
+// 209, of 7 599 and 292; greedy, no draft, 42 and 24. A draw without drafts is summed in 64 bits on either route and
+// gains nothing: 128 sequences 33.2 and 38.8, 256 56.6 and 63.9, 512 91.7 and 97.3.
 constexpr int64_t kVMany = (int64_t)1 << 24;
 // Their statistics by runs of up to 4 parts a wave, whose next loads are in flight during a part's arithmetic and whose
 // reductions across lanes come once, as long as that leaves this many waves. 256 x 9 rows of 151,936 bf16 values, us a
-// call: runs of 2 238, 4 222, 8 225; 512 x 15 rows 545, 519, 529. 256 x 15, statistics alone: runs of 1 240, 8 181.
+// call: runs of 2 238, 4 222, 8 225; 512 x 15 rows 545, 519, 529. 256 x 15, statistics alone: runs of 1 240, 4 175.
 constexpr int64_t kVSpread = 16384;
 
 struct VerifyLayout {

@@ -1,17 +1,18 @@
 """8-bit integers at the vocabulary's end, over libocto_head.so: rows held in 8 bits, and the head's logits from them.
 
     octohead::quantise_rows / widen_rows       rows as int8 with fp32 scales, and back
-    octohead::head_logits_i8 / head_grads_i8   rows W^T in 8-bit integers with a scale for each row of both; its gradients
+    octohead::head_logits_i8 / head_grads_i8   rows W^T in 8-bit integers, a scale for each row of both; its gradients
     checkpoint8                                a checkpoint that holds its inputs in 8 bits
 
-Of a row, or of each group of 32 to 256 of its values, with a the largest magnitude: scale = a times 1/127, both in fp32,
-q the exact quotient x / scale to the nearest integer (ties to even). A group below 2^-119 is held as zeros, one with a
-NaN or an infinity as NaN. int8 rows start on 16-byte boundaries, zeros between them (quantise_rows gives them so).
+Of a row, or of each group of 32 to 256 of its values, with a the largest magnitude: scale = a times 1/127, both in
+fp32, q the exact quotient x / scale to the nearest integer (ties to even). A group below 2^-119 is held as zeros, one
+with a NaN or an infinity as NaN. int8 rows start on 16-byte boundaries, zeros between them (quantise_rows gives them
+so).
 
 The logits are x_scale w_scale sum_k xq wq, the sum exact. Their gradients go straight through the rounding: in the rows
-g (w_scale wq), in the weight g^T (x_scale xq), so that what is held for them is the 8-bit rows that the product read and
-not the rows. HIP tensors only; all work is queued on the current stream of the tensors' device, nothing synchronises
-with the host.
+g (w_scale wq), in the weight g^T (x_scale xq), so that what is held for them is the 8-bit rows that the product read
+and not the rows. HIP tensors only; all work is queued on the current stream of the tensors' device, nothing
+synchronises with the host.
 """
 
 from __future__ import annotations
@@ -56,7 +57,7 @@ def _rows_of(x: Tensor, what: str) -> Tensor:
 
 
 def _rows8(q: Tensor) -> Tensor:
-    """q [*, d] int8 as [rows, d] with rows on 16-byte boundaries, readable up to the next; a copy where they are not."""
+    """q [*, d] int8 as [rows, d], rows on 16-byte boundaries and readable up to the next; a copy where they are not."""
     if q.dtype != torch.int8 or q.dim() < 1 or not q.shape[-1]:
         raise ValueError(f"octohead: int8 rows [*, d] expected, got {q.dtype} {tuple(q.shape)}")
     if q.dim() != 2:
@@ -137,15 +138,15 @@ def _(q, scale, dtype, group):
 
 
 def widen_rows(q: Tensor, scale: Tensor, dtype: torch.dtype, group: int = 0) -> Tensor:
-    """[*, d] in dtype: q times its scales, rounded once. What quantise_rows(x, group) took comes back within half a
-    step of its scale and one rounding."""
+    """[*, d] in dtype: q times its scales in fp32, rounded to dtype. What quantise_rows(x, group) took comes back
+    within half a step of its scale and those roundings. Not differentiable."""
     _groups(1, group)
     return _widen_op(q, scale, dtype, group) if torch.compiler.is_compiling() else _widen(q, scale, dtype, group)
 
 
 def _holds(x, group: int) -> bool:
-    """Whether x is held in 8 bits: where the bytes of a row, padded, with its scales, are fewer than x's own (16-bit rows
-    from d 11 on, but for 17 and 18). A tensor that is expanded takes less as it is."""
+    """Whether x is held in 8 bits: where the bytes of a row, padded, with its scales, are fewer than x's own (16-bit
+    rows from d 11 on, but for 17 and 18). A tensor that is expanded takes less as it is."""
     if not (isinstance(x, Tensor) and x.requires_grad and torch.is_grad_enabled() and x.is_cuda and
             x.dtype in _FLOATS and x.dim() > 0 and x.shape[-1] > 0 and not isinstance(x, torch.nn.Parameter)) or \
             any(step == 0 and size > 1 for size, step in zip(x.shape, x.stride())):
@@ -156,11 +157,12 @@ def _holds(x, group: int) -> bool:
 
 def checkpoint8(fn, *xs, group: int = 128):
     """fn(*xs), recomputed in the backward (torch.utils.checkpoint, not reentrant) from inputs that are held in 8 bits
-    in between: those of bf16, f16 or fp32 on a HIP device that require a gradient, are no parameters and take fewer bytes
-    so (not the narrowest rows, nor a tensor that is expanded). The forward sees them as they are, the recompute what their 8 bits stand for, so what fn
-    saves for its gradients is off by the rounding (half of 1/127 of a group's largest value). They have to be finite: a
-    group with a NaN or an infinity (-inf in a bias that is learnt) is NaN in the recompute. Other arguments (masks, positions, parameters, None) are kept by reference;
-    changed in place before the backward, it raises, as an ordinary checkpoint does."""
+    in between: those of bf16, f16 or fp32 on a HIP device that require a gradient, are no parameters and take fewer
+    bytes so (not the narrowest rows, nor a tensor that is expanded). The forward sees them as they are, the recompute
+    what their 8 bits stand for, so what fn saves for its gradients is off by the rounding (half of 1/127 of a group's
+    largest value). They have to be finite: a group with a NaN or an infinity (-inf in a bias that is learnt) is NaN in
+    the recompute. Other arguments (masks, positions, parameters, None) are kept by reference; changed in place before
+    the backward, it raises, as an ordinary checkpoint does."""
     _groups(1, group)
     live = list(xs)
     dtypes = [x.dtype if _holds(x, group) else None for x in xs]
@@ -323,11 +325,13 @@ def int8_head(rows: Tensor, wq: Tensor, w_scale: Tensor, *, weight: Optional[Ten
               out_dtype: Optional[torch.dtype] = None) -> Tensor:
     """Logits [*, V] in out_dtype (None: rows') of rows [*, d] in bf16, f16 or fp32 against a vocabulary matrix in 8
     bits, (wq, w_scale) = quantise_rows(weight): each row quantised here, the product exact in 32-bit integers, scaled
-    and rounded once. The rows' gradient is that of the weights' 8-bit values. weight: the [V, d] parameter that wq was
-    made of, which gets the gradient straight through the rounding; its values are not read, and wq is made again when
-    it has changed. Between the two passes the rows are held in 8 bits, and wq and w_scale by reference (changed in
-    place, the backward raises). wq and w_scale get no gradient; the gradients have no derivative of their own and the
-    logits none in forward mode (one raises)."""
+    in fp32 and rounded to the logits' type. The rows' gradient is that of the weights' 8-bit values. weight: the [V, d]
+    parameter that wq was made of, which gets the gradient straight through the rounding; its values are not read, and
+    wq is made again when it has changed. For 16-bit logits the 8-bit operands times their scales are rounded to the
+    logits' type before the gradients' products, which leaves them 2.4e-3 (bf16) or 2.9e-4 (f16) from 64 bits; those of
+    fp32 logits are within 1e-6. Between the two passes the rows are held in 8 bits, and wq and w_scale by reference
+    (changed in place, the backward raises). wq and w_scale get no gradient; the gradients have no derivative of their
+    own and the logits none in forward mode (one raises)."""
     out_dtype = out_dtype or rows.dtype
     train = torch.is_grad_enabled() and (rows.requires_grad or weight is not None and weight.requires_grad)
     if train and out_dtype == torch.float32 and wq.dim() == 2:

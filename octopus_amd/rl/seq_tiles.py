@@ -40,7 +40,7 @@ def _fused(fn=None, *, hip=None):
 
 
 def _hooks():
-    """This thread's innermost hooks of saved tensors; a checkpoint's forward and its recompute have some of their own."""
+    """This thread's innermost hooks of saved tensors; a checkpoint's forward and its recompute have their own."""
     return torch._C._autograd._top_saved_tensors_default_hooks(False)
 
 

@@ -5,7 +5,7 @@
 With p_i = softmax(target logits_i / T), q_i = softmax(draft logits_i / T) and u given numbers in [0, 1):
 
     draft i is accepted when u_i q_i(x_i) < p_i(x_i); the first that is not ends the drafts at a
-    the next token is the lowest v with sum_{w <= v} r_w > u_K sum r, r = max(p_a - q_a, 0), or p_a behind the last draft
+    the next token is the lowest v with sum_{w <= v} r_w > u_K sum r, r = max(p_a - q_a, 0), p_a behind the last draft
 
 so the answered tokens are distributed as the target's own samples, whatever drafted them. Their log-probabilities under
 the target at T are what a GRPO trainer reads as the behaviour logprobs. HIP tensors only; all work is queued on the
@@ -83,11 +83,11 @@ def verify_drafts(logits: Tensor, drafts: Tensor, uniform: Optional[Tensor], tem
     None) and draft_logits are not read.
 
     Decisions and tokens are those of 64-bit probabilities, so the token is the definition's. logp is rounded once from
-    64 bits for the drawn token and, below 2^24 logits read, for all; from there on the accepted drafts' and greedy's are
-    within 5e-6 before that rounding (their rows' sums are of 32-bit exponentials), and may differ by that between calls
-    of other sizes. Nothing is differentiable. A draft outside the vocabulary, or whose draft row has no softmax (a NaN,
-    +inf, or every logit masked), is rejected and the token drawn from the target's; where the target's row has none, the
-    token is -1 and its logp NaN."""
+    64 bits for the drawn token and, below 2^24 logits read, for all; from there on the accepted drafts' and greedy's
+    are within 5e-6 before that rounding (their rows' sums are of 32-bit exponentials), and may differ by that between
+    calls of other sizes. Nothing is differentiable. A draft outside the vocabulary, or whose draft row has no softmax
+    (a NaN, +inf, or every logit masked), is rejected and the token drawn from the target's; where the target's row has
+    none, the token is -1 and its logp NaN."""
     if logits.dim() != 3 or not logits.shape[1] or not logits.shape[2]:
         raise ValueError(f"octohead: logits must be [S, K + 1, V], got {tuple(logits.shape)}")
     S, rows, V = logits.shape

@@ -1,4 +1,4 @@
-"""checkpoint8 and held8 where nothing is held in 8 bits: on CPU tensors they are the ordinary checkpoint, with its checks."""
+"""checkpoint8 and held8 without a GPU: on CPU tensors they are the ordinary checkpoint, with its checks."""
 
 import pytest
 import torch
@@ -41,7 +41,7 @@ def test_arguments_pass_as_they_are(run):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
-# ---- held8 and other checkpoints, with stand-ins for the kernels -------------------------------------------------------
+# ---- held8 and other checkpoints, with stand-ins for the kernels -----------------------------------------------------
 
 @pytest.fixture
 def held(monkeypatch):
@@ -106,7 +106,8 @@ def test_held8_and_an_offload(held):
     """Hooks of saved tensors set inside held8() see the tensors as they are, those around it the 8 bits."""
     x = torch.randn(1, 6, 8, requires_grad=True)
     seen = []
-    hooks = lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.dtype) or t, lambda t: t)  # noqa: E731
+    pack = lambda t: seen.append(t.dtype) or t  # noqa: E731
+    hooks = lambda: torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t)  # noqa: E731
     with seq_tiles.held8(), hooks():
         y = seq_tiles.tiled(torch.sin, x)
     assert not held and torch.int8 not in seen

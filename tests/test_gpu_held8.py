@@ -1,5 +1,5 @@
-"""checkpoint8 on the GPU where the recompute could differ from the forward by more than the 8 bits: random numbers, hooks
-of saved tensors, tensors that 8 bits do not make smaller."""
+"""checkpoint8 on the GPU where the recompute could differ from the forward by more than the 8 bits: random numbers,
+hooks of saved tensors, tensors that 8 bits do not make smaller."""
 
 import pytest
 import torch
@@ -11,8 +11,8 @@ DEV = "cuda:0"
 
 
 def test_random_numbers_are_those_of_the_forward():
-    """Dropout in fn, every tensor argument held: the recompute draws the forward's mask, and leaves the generator where it
-    was."""
+    """Dropout in fn, every tensor argument held: the recompute draws the forward's mask, and leaves the generator where
+    it was."""
     x = torch.randn(64, 256, device=DEV).requires_grad_(True)
     y = int8_op.checkpoint8(lambda t: torch.nn.functional.dropout(t, 0.5).square(), x)
     torch.rand(3, device=DEV)

@@ -1,5 +1,6 @@
-"""int8_head and its gradients where the first tests did not go: f16 logits of operands outside f16's range, dense shares of
-many blocks of weight rows, saved rows that a hook gives back in another layout, tangents of forward mode, many rows."""
+"""int8_head and its gradients where the first tests did not go: f16 logits of operands outside f16's range, dense
+shares of many blocks of weight rows, saved rows that a hook gives back in another layout, tangents of forward mode,
+many rows."""
 
 import pytest
 import torch
@@ -13,8 +14,8 @@ DEV = "cuda:0"
 
 
 def _f16_bound(ref, mag, terms, out, g_sums, scales):
-    """The widened operand to f16's 11 bits, the fp32 sum, the result. The operand is widened times a power of two 2^k that
-    keeps 127 times the largest scale above 2^14 (so 2^-k <= 2^-7 of that scale); below 2^-14 its step is 2^-24, half of
+    """The widened operand to f16's 11 bits, the fp32 sum, the result. The operand is widened times a power of two 2^k
+    that brings the largest scale to 2^7 or more (2^-k <= 2^-7 of that scale); below 2^-14 its step is 2^-24, half of
     which is off by at most 2^-25 2^-k <= 2^-32 of the largest scale for each of g's values."""
     off = mag * (2.0 ** -11 + (terms + 8) * 2.0 ** -24) + g_sums * scales.max() * 2.0 ** -32
     return off + _half(out) * (ref.abs() + off) + torch.finfo(out).smallest_normal * torch.finfo(out).eps
@@ -54,8 +55,8 @@ def test_f16_gradients_of_operands_outside_f16(rows_dtype, size, n, d, V):
 @pytest.mark.parametrize("far", [False, True])
 @pytest.mark.parametrize("n,V", [(9, 700), (200, 700), (200, 16700), (20, 16700)])
 def test_f16_gradients_of_rows_of_many_sizes(n, V, far):
-    """Rows and weight rows between 2^-20 and 2^10 of the largest, some of zeros: what is small beside the largest is off
-    by a step that is small beside it. far: one row alone lies outside f16's numbers."""
+    """Rows and weight rows between 2^-20 and 2^10, some of zeros: what is small beside the largest is off by a step
+    that is small beside it. far: one row alone lies outside f16's numbers."""
     d = 80
     g = torch.Generator().manual_seed(3)
     x = torch.randn(n, d, generator=g) * torch.exp2(torch.randint(-20, 10, (n, 1), generator=g).float())
@@ -85,10 +86,11 @@ def test_f16_gradients_with_a_row_without_scale():
     _check_f16(gr, None, up, x, wq, ws, xs)
 
 
-# ---- dense shares of many blocks: a wave's later weight rows, the prefetch into them, the cut-off last block -------------
+# ---- dense shares of many blocks: a wave's later weight rows, the prefetch into them, the cut-off last block ---------
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,d,V", [(1, 256, 151936), (17, 64, 70001), (32, 2560, 3001), (20, 4096, 70001), (32, 4800, 515)])
+@pytest.mark.parametrize("n,d,V", [(1, 256, 151936), (17, 64, 70001), (32, 2560, 3001), (20, 4096, 70001),
+                                   (32, 4800, 515)])
 def test_few_rows_many_blocks(n, d, V, dtype):
     x, w = _inputs(n, d, V, dtype, n + d)
     wq, ws = int8_op.quantise_rows(w.to(DEV))
@@ -108,7 +110,7 @@ def test_few_rows_gradient_many_steps(n, d, V, dtype):
     assert ((gr.cpu().double() - want).abs() <= bound).all()
 
 
-# ---- what is saved, and what is not differentiated -----------------------------------------------------------------------
+# ---- what is saved, and what is not differentiated -------------------------------------------------------------------
 
 @pytest.mark.parametrize("n", [1, 2, 70, 200])
 def test_saved_rows_in_another_layout(n):
@@ -143,7 +145,7 @@ def test_tangents_are_refused():
     assert torch.equal(plain, int8_op.int8_head(x, wq, ws))
 
 
-# ---- many rows ----------------------------------------------------------------------------------------------------------
+# ---- many rows -------------------------------------------------------------------------------------------------------
 
 def test_weight_gradient_of_two_million_rows():
     """A copy of g of 2^24 blocks and more, 121 GB beside g's 120: the first and the last rows alone."""

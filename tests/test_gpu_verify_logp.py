@@ -1,6 +1,6 @@
-"""The log-probabilities of verify_drafts on both routes: within one rounding of their value where the rows' sums are taken
-in 64 bits (few logits, and every drawn token), within 5e-6 and one rounding where they are of 32-bit exponentials (2^24
-logits and more: the accepted drafts, and greedy's tokens)."""
+"""The log-probabilities of verify_drafts on both routes: within one rounding of their value where the rows' sums are
+taken in 64 bits (few logits, and every drawn token), within 5e-6 and one rounding where they are of 32-bit exponentials
+(2^24 logits and more: the accepted drafts, and greedy's tokens)."""
 
 import pytest
 import torch
