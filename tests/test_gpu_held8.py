@@ -83,3 +83,29 @@ def test_expanded_tensors_are_kept(monkeypatch):
     y = int8_op.checkpoint8(lambda a, b: torch.sin(a + b), x, bias.expand(8, 4, 64))
     gx, gb = torch.autograd.grad(y.sum(), (x, bias))
     assert calls == [(8, 4, 64)] and torch.allclose(gx.sum(0, keepdim=True), gb, rtol=0, atol=8 * 2.0 ** -22)
+
+
+def test_captured():
+    """Both passes in one graph, replayed on new values between the program's own passes."""
+    w = torch.randn(256, 200, device=DEV).requires_grad_(True)
+    static = torch.randn(33, 256, device=DEV).requires_grad_(True)
+
+    def step(x):
+        y = int8_op.checkpoint8(lambda t: torch.sin(t @ w), x)
+        return (y.detach(), *torch.autograd.grad(y.sum(), (x, w)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(static)
+    for seed in (1, 2, 3):
+        new = torch.randn(33, 256, device=DEV, generator=torch.Generator(DEV).manual_seed(seed)).requires_grad_(True)
+        with torch.no_grad():
+            static.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step(new)))
