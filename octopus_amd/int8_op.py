@@ -146,9 +146,10 @@ def widen_rows(q: Tensor, scale: Tensor, dtype: torch.dtype, group: int = 0) -> 
 
 def _holds(x, group: int) -> bool:
     """Whether x is held in 8 bits: where the bytes of a row, padded, with its scales, are fewer than x's own (16-bit
-    rows from d 11 on, but for 17 and 18). A tensor that is expanded takes less as it is."""
-    if not (isinstance(x, Tensor) and x.requires_grad and torch.is_grad_enabled() and x.is_cuda and
-            x.dtype in _FLOATS and x.dim() > 0 and x.shape[-1] > 0 and not isinstance(x, torch.nn.Parameter)) or \
+    rows from d 11 on, but for 17 and 18). A tensor that is expanded takes less as it is; a parameter is there anyway,
+    and fn may read more of another class of tensors than its values."""
+    if type(x) is not Tensor or not (x.requires_grad and torch.is_grad_enabled() and x.is_cuda and
+                                     x.dtype in _FLOATS and x.dim() > 0 and x.shape[-1] > 0) or \
             any(step == 0 and size > 1 for size, step in zip(x.shape, x.stride())):
         return False
     d = x.shape[-1]
@@ -157,12 +158,12 @@ def _holds(x, group: int) -> bool:
 
 def checkpoint8(fn, *xs, group: int = 128):
     """fn(*xs), recomputed in the backward (torch.utils.checkpoint, not reentrant) from inputs that are held in 8 bits
-    in between: those of bf16, f16 or fp32 on a HIP device that require a gradient, are no parameters and take fewer
-    bytes so (not the narrowest rows, nor a tensor that is expanded). The forward sees them as they are, the recompute
-    what their 8 bits stand for, so what fn saves for its gradients is off by the rounding (half of 1/127 of a group's
-    largest value). They have to be finite: a group with a NaN or an infinity (-inf in a bias that is learnt) is NaN in
-    the recompute. Other arguments (masks, positions, parameters, None) are kept by reference; changed in place before
-    the backward, it raises, as an ordinary checkpoint does."""
+    in between: those of bf16, f16 or fp32 on a HIP device that require a gradient, are plain tensors (no parameters nor
+    other subclasses) and take fewer bytes so (not the narrowest rows, nor a tensor that is expanded). The forward sees
+    them as they are, the recompute what their 8 bits stand for, so what fn saves for its gradients is off by the
+    rounding (half of 1/127 of a group's largest value). They have to be finite: a group with a NaN or an infinity (-inf
+    in a bias that is learnt) is NaN in the recompute. Other arguments (masks, positions, parameters, None) are kept by
+    reference; changed in place before the backward, it raises, as an ordinary checkpoint does."""
     _groups(1, group)
     live = list(xs)
     dtypes = [x.dtype if _holds(x, group) else None for x in xs]

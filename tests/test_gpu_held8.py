@@ -85,6 +85,17 @@ def test_expanded_tensors_are_kept(monkeypatch):
     assert calls == [(8, 4, 64)] and torch.allclose(gx.sum(0, keepdim=True), gb, rtol=0, atol=8 * 2.0 ** -22)
 
 
+class _Marked(torch.Tensor):
+    """A tensor that fn tells from a plain one."""
+
+
+def test_subclasses_are_kept():
+    x = torch.randn(9, 64, device=DEV).as_subclass(_Marked).requires_grad_(True)
+    fn = lambda t: torch.sin(t * (2.0 if isinstance(t, _Marked) else 3.0))  # noqa: E731
+    (got,) = torch.autograd.grad(int8_op.checkpoint8(fn, x).sum(), x)
+    assert torch.equal(got, 2 * torch.cos(2 * x.detach()))
+
+
 def test_captured():
     """Both passes in one graph, replayed on new values between the program's own passes."""
     w = torch.randn(256, 200, device=DEV).requires_grad_(True)
